@@ -36,8 +36,15 @@ KERNEL_SOURCES = [
     "cc1d_bwd_noalloc.hip",
     "cc1d_update.hip",
     "cc1d_varlen_states.hip",
+    "cc1d_delta_api.cpp",
+    "cc1d_delta_step.hip",
+    "cc1d_norm.hip",
 ]
 KERNEL_HEADERS = ["cc1d_device.hpp", "cc1d_internal.hpp", "cc1d_bwd_channellast_kernel.hpp"]
+DELTA_HEADERS = ["cc1d_delta.hpp", "cc1d_delta_host.hpp"]   # of the sources that begin with cc1d_delta
+PUBLIC_HEADERS = ["cc1d.h", "cc1d_mixer.h"]
+BINDING_SOURCES = ["causal_conv1d.cpp", "mixer.cpp"]
+BINDING_HEADERS = ["cc1d_torch.hpp"]
 
 LIB_NAME = "libcc1d.so"
 EXT_NAME = "causal_conv1d_cuda" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so")
@@ -92,13 +99,16 @@ def build_kernels(force=False, extra_flags=(), lib_path=None):
     os.makedirs(OBJDIR, exist_ok=True)
     lib_path = lib_path or os.path.join(HERE, LIB_NAME)
     headers = [os.path.join(CSRC, h) for h in KERNEL_HEADERS] + [os.path.join(INCLUDE, "cc1d.h")]
+    delta = [os.path.join(CSRC, h) for h in DELTA_HEADERS]
+    mixer = [os.path.join(INCLUDE, "cc1d_mixer.h")]
     tag = "" if not extra_flags else "_" + str(abs(hash(tuple(extra_flags))) % 10**8)
     jobs, objs = [], []
     for src in KERNEL_SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJDIR, os.path.splitext(src)[0] + tag + ".o")
         objs.append(o)
-        if force or not _newer(o, [s] + headers):
+        deps = [s] + headers + (delta + mixer if src.startswith("cc1d_delta") else mixer if src == "cc1d_norm.hip" else [])
+        if force or not _newer(o, deps):
             jobs.append(compile_command(src, o, extra_flags))
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(_run, jobs))
@@ -120,20 +130,26 @@ def build_binding(force=False, out_dir=None):
     from torch.utils import cpp_extension as ce
     import torch
 
-    src = os.path.join(CSRC, "causal_conv1d.cpp")
+    srcs = [os.path.join(CSRC, s) for s in BINDING_SOURCES]
+    deps = srcs + [os.path.join(CSRC, h) for h in BINDING_HEADERS] + [os.path.join(INCLUDE, h) for h in PUBLIC_HEADERS]
     out = os.path.join(out_dir or HERE, EXT_NAME)
-    if not force and _newer(out, [src, os.path.join(INCLUDE, "cc1d.h")]):
+    if not force and _newer(out, deps):
         return out
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_EXTENSION_NAME=causal_conv1d_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           "-Wno-deprecated-declarations"]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-DTORCH_EXTENSION_NAME=causal_conv1d_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+             "-Wno-deprecated-declarations"]
     for inc in ce.include_paths():
-        cmd += ["-isystem", inc]
-    cmd += ["-isystem", os.path.join(ROCM, "include"),
-            "-isystem", sysconfig.get_paths()["include"], "-I" + INCLUDE,
-            src, "-o", out]
+        flags += ["-isystem", inc]
+    flags += ["-isystem", os.path.join(ROCM, "include"),
+              "-isystem", sysconfig.get_paths()["include"], "-I" + INCLUDE]
+    cxx = os.environ.get("CXX", "g++")
+    objdir = OBJDIR if out_dir is None else os.path.join(out_dir, "objects")
+    os.makedirs(objdir, exist_ok=True)
+    objs = [os.path.join(objdir, "binding_" + os.path.splitext(s)[0] + ".o") for s in BINDING_SOURCES]
+    with ThreadPoolExecutor(max_workers=len(srcs)) as ex:
+        list(ex.map(_run, [[cxx] + flags + ["-c", s, "-o", o] for s, o in zip(srcs, objs)]))
+    cmd = [cxx, "-shared", "-o", out] + objs
     for lp in ce.library_paths():
         cmd += ["-L" + lp, "-Wl,-rpath," + lp]
     cmd += ["-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",

@@ -278,6 +278,9 @@ const char *cc1d_strerror(int status) {
         case CC1D_ERR_UNKNOWN_TUNABLE: return "unknown tunable name";
         case CC1D_ERR_WORKSPACE_LIMIT: return "backward needs more workspace than the library's built-in array holds; use cc1d_bwd with a caller-owned workspace";
         case CC1D_ERR_IN_PLACE: return "an output shares elements with an input (out with x, dx with x or dout): the kernels do not work in place";
+        case CC1D_ERR_HEADS: return "the number of value heads must be a multiple of the number of key heads";
+        case CC1D_ERR_HEAD_DIM: return "the gated delta rule needs 1 <= dim_k <= 256 and 1 <= dim_v <= 512";
+        case CC1D_ERR_ROW_LAYOUT: return "a tensor does not start on a multiple of its element size";
         default: return "unknown cc1d status";
     }
 }

@@ -1,0 +1,49 @@
+// What the kernels of the gated delta rule share: reading of gates, where a chunk of tokens lies, and
+// products of fp32 matrices on the 16-bit matrix cores.
+#pragma once
+
+#include "cc1d_device.hpp"
+#include "cc1d_internal.hpp"
+#include "cc1d_mixer.h"
+
+namespace cc1d {
+
+constexpr int kChunk = 64;               // tokens of a chunk
+constexpr float kNormEps = 1e-6f;        // under the root of qk_l2norm
+
+__device__ __forceinline__ float load_as_float(const void *p, int64_t i, int dtype) {
+    if (dtype == CC1D_F32) return static_cast<const float *>(p)[i];
+    if (dtype == CC1D_F16) return (float)static_cast<const _Float16 *>(p)[i];
+    return (float)static_cast<const __bf16 *>(p)[i];
+}
+__device__ __forceinline__ void store_from_float(void *p, int64_t i, int dtype, float v) {
+    if (dtype == CC1D_F32) static_cast<float *>(p)[i] = v;
+    else if (dtype == CC1D_F16) static_cast<_Float16 *>(p)[i] = (_Float16)v;
+    else static_cast<__bf16 *>(p)[i] = (__bf16)v;
+}
+
+// exp(-200) is 0 in fp32, and sums of such gates stay finite, so that differences of them do too: -inf ("forget
+// everything") needs no other treatment.  A NaN stays one.
+__device__ __forceinline__ float bounded_gate(float g) { return g < -200.f ? -200.f : g; }
+
+__device__ __forceinline__ int64_t cu_entry(const void *cu, int is64, int i, int64_t most) {
+    int64_t v = is64 ? static_cast<const int64_t *>(cu)[i] : (int64_t)static_cast<const int32_t *>(cu)[i];
+    return v < 0 ? 0 : v > most ? most : v;
+}
+// Tokens [lo, hi) of sequence n, counted inside batch entry b.
+struct TokenRange { int64_t lo, hi; int b; };
+__device__ __forceinline__ TokenRange sequence_tokens(const cc1d_delta_params &p, int n) {
+    if (p.cu_seqlens == nullptr) return {0, p.seqlen, n};
+    const int64_t lo = cu_entry(p.cu_seqlens, p.cu_seqlens_is_int64, n, p.seqlen);
+    const int64_t hi = cu_entry(p.cu_seqlens, p.cu_seqlens_is_int64, n + 1, p.seqlen);
+    return {lo, hi < lo ? lo : hi, 0};
+}
+
+// Orders a wavefront's own LDS writes before its reads of what other lanes wrote.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+}  // namespace cc1d

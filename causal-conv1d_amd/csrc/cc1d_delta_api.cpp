@@ -1,0 +1,97 @@
+// C-ABI front of the gated delta rule (cc1d_mixer.h): argument validation and dispatch to the kernel
+// launchers.  Nothing here allocates or synchronises; validation never touches the GPU.
+#include "cc1d_delta_host.hpp"
+
+using namespace cc1d;
+
+namespace {
+
+bool dtype_ok(int d) { return d == CC1D_F32 || d == CC1D_F16 || d == CC1D_BF16; }
+bool on_elements(const void *p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & ((uintptr_t)elem_bytes(dtype) - 1)) == 0; }
+
+template <typename P>
+int check_sizes(const P &p) {
+    if (!dtype_ok(p.x_dtype) || !dtype_ok(p.g_dtype) || !dtype_ok(p.beta_dtype)) return CC1D_ERR_DTYPE;
+    if (p.batch < 0 || p.seqlen < 0 || p.heads < 1 || p.v_heads < 0) return CC1D_ERR_SHAPE;
+    if (p.v_heads % p.heads != 0) return CC1D_ERR_HEADS;
+    if (p.dim_k < 1 || p.dim_k > 256 || p.dim_v < 1 || p.dim_v > 512) return CC1D_ERR_HEAD_DIM;
+    return CC1D_OK;
+}
+template <typename P>
+int check_inputs(const P &p) {
+    if (p.q == nullptr || p.k == nullptr || p.v == nullptr || p.g == nullptr || p.beta == nullptr) return CC1D_ERR_NULL_POINTER;
+    if (!on_elements(p.q, p.x_dtype) || !on_elements(p.k, p.x_dtype) || !on_elements(p.v, p.x_dtype) || !on_elements(p.g, p.g_dtype) ||
+        !on_elements(p.beta, p.beta_dtype)) return CC1D_ERR_ROW_LAYOUT;
+    return CC1D_OK;
+}
+int check_delta(const cc1d_delta_params &p) {
+    int st = check_sizes(p);
+    if (st != CC1D_OK) return st;
+    if (p.sequences < 0 || (p.cu_seqlens == nullptr ? p.sequences != p.batch : p.batch != 1)) return CC1D_ERR_SHAPE;
+    if (p.batch > 0 && p.seqlen > 0 && p.v_heads > 0) st = check_inputs(p);
+    if (st != CC1D_OK) return st;
+    if (!on_elements(p.initial_states, CC1D_F32) || !on_elements(p.final_states, CC1D_F32) || !on_elements(p.out, p.x_dtype)) return CC1D_ERR_ROW_LAYOUT;
+    return CC1D_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cc1d_validate_delta(const cc1d_delta_params *p) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const int st = check_delta(*p);
+    if (st != CC1D_OK) return st;
+    if (p->batch > 0 && p->seqlen > 0 && p->v_heads > 0 && p->out == nullptr) return CC1D_ERR_NULL_POINTER;
+    return CC1D_OK;
+}
+
+int cc1d_delta_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
+    if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
+    *bytes = 0;
+    const int st = cc1d_validate_delta(p);
+    return st;
+}
+
+int cc1d_delta_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
+    size_t need = 0;
+    const int st = cc1d_delta_workspace_bytes(p, &need);
+    if (st != CC1D_OK) return st;
+    if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
+    if (p->batch == 0 || p->v_heads == 0 || p->sequences == 0) return CC1D_OK;
+    return launch_delta_tokens(*p, nullptr, p->sequences, static_cast<hipStream_t>(stream));
+}
+
+int cc1d_validate_delta_step(const cc1d_delta_step_params *p) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    int st = check_sizes(*p);
+    if (st != CC1D_OK) return st;
+    if (p->state_slots < 0 || (p->state_indices == nullptr && p->state_slots != p->batch)) return CC1D_ERR_SHAPE;
+    if (p->batch == 0 || p->seqlen == 0 || p->v_heads == 0) return CC1D_OK;
+    st = check_inputs(*p);
+    if (st != CC1D_OK) return st;
+    if (p->out == nullptr || (p->state == nullptr && p->state_slots > 0)) return CC1D_ERR_NULL_POINTER;
+    if (!on_elements(p->state, CC1D_F32) || !on_elements(p->out, p->x_dtype)) return CC1D_ERR_ROW_LAYOUT;
+    return CC1D_OK;
+}
+
+int cc1d_delta_step(const cc1d_delta_step_params *s, cc1d_stream_t stream) {
+    const int st = cc1d_validate_delta_step(s);
+    if (st != CC1D_OK || s->batch == 0 || s->seqlen == 0 || s->v_heads == 0) return st;
+    cc1d_delta_params p = {};
+    p.batch = p.sequences = s->batch; p.seqlen = s->seqlen; p.heads = s->heads; p.v_heads = s->v_heads;
+    p.dim_k = s->dim_k; p.dim_v = s->dim_v;
+    p.x_dtype = s->x_dtype; p.g_dtype = s->g_dtype; p.beta_dtype = s->beta_dtype;
+    p.qk_l2norm = s->qk_l2norm; p.scale = s->scale;
+    p.q = s->q; p.q_stride_b = s->q_stride_b; p.q_stride_l = s->q_stride_l; p.q_stride_h = s->q_stride_h;
+    p.k = s->k; p.k_stride_b = s->k_stride_b; p.k_stride_l = s->k_stride_l; p.k_stride_h = s->k_stride_h;
+    p.v = s->v; p.v_stride_b = s->v_stride_b; p.v_stride_l = s->v_stride_l; p.v_stride_h = s->v_stride_h;
+    p.g = s->g; p.g_stride_b = s->g_stride_b; p.g_stride_l = s->g_stride_l; p.g_stride_h = s->g_stride_h;
+    p.beta = s->beta; p.beta_stride_b = s->beta_stride_b; p.beta_stride_l = s->beta_stride_l; p.beta_stride_h = s->beta_stride_h;
+    p.initial_states = s->state; p.init_stride_n = s->state_stride_n; p.init_stride_h = s->state_stride_h; p.init_stride_k = s->state_stride_k;
+    p.final_states = s->state; p.final_stride_n = s->state_stride_n; p.final_stride_h = s->state_stride_h; p.final_stride_k = s->state_stride_k;
+    p.out = s->out; p.out_stride_b = s->out_stride_b; p.out_stride_l = s->out_stride_l; p.out_stride_h = s->out_stride_h;
+    return launch_delta_tokens(p, s->state_indices, s->state_slots, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,233 @@
+// The gated delta rule token by token: the step of a decode loop, and whole sequences that are too short
+// to be worth cutting into chunks.
+//
+//   D = exp(g) S,  u = beta (v - D^T k),  S = D + k u^T,  out = scale S^T q
+//
+// The columns of S (dim_v) do not meet: a wavefront takes 32 of them, all of dim_k, in registers.  A lane holds
+// 4 adjacent columns of KR rows (8 lanes make a row's 128 bytes, 8 groups of lanes take KR rows each), so every
+// row of the state moves as whole 128-byte lines.  q and k go through LDS once, normalised, in fp32.  Both
+// products of a token are formed before its update, out = D^T q + (k.q) u, so that one reduction over the
+// lane groups serves both.  In a decode step nothing is computed worth mentioning: the state, read and written
+// once, is the floor.
+#include "cc1d_delta.hpp"
+#include "cc1d_delta_host.hpp"
+
+namespace cc1d {
+namespace {
+
+constexpr int kStepCols = 32;
+
+struct StepArgs {
+    cc1d_delta_params p;                 // initial_states / final_states: the state, or the caller's two
+    const int32_t *indices;
+    int32_t slots;
+    uint32_t items, col_tiles;
+    uint32_t vec_state, vec_x;           // 16-byte rows of the state / 4 elements of v and out at once
+};
+
+template <int DT>
+__device__ __forceinline__ void load4(const void *base, int64_t at, int n, bool vec, float (&f)[4]) {
+    using T = typename Elem<DT>::type;
+    const T *x = static_cast<const T *>(base) + at;
+    if (vec) {
+        if (DT == CC1D_F32) {
+            const float4 r = *reinterpret_cast<const float4 *>(x);
+            f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
+        } else {
+            const u32x2 r = *reinterpret_cast<const u32x2 *>(x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = i < 2 ? r.x : r.y;
+                const uint16_t h = (uint16_t)(i & 1 ? w >> 16 : w & 0xffffu);
+                f[i] = Elem<DT>::to_float(bitcast<T>(h));
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i < n ? Elem<DT>::to_float(x[i]) : 0.f;
+}
+template <>
+__device__ __forceinline__ void load4<CC1D_F32>(const void *base, int64_t at, int n, bool vec, float (&f)[4]) {
+    const float *x = static_cast<const float *>(base) + at;
+    if (vec) {
+        const float4 r = *reinterpret_cast<const float4 *>(x);
+        f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i < n ? x[i] : 0.f;
+}
+
+// KR: rows of the state a lane holds, dim_k <= 8 KR.
+template <int DT, int KR>
+__global__ void __launch_bounds__(kBlock)
+delta_step_kernel(const StepArgs a) {
+    using T = typename Elem<DT>::type;
+    __shared__ float lds[4][2][8 * KR + 8];
+    const cc1d_delta_params &p = a.p;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t item = blockIdx.x * 4u + (uint32_t)wave;
+    if (item >= a.items) return;                         // no barrier below: wavefronts work alone
+    const int tile = (int)(item % a.col_tiles);
+    const uint32_t nh = item / a.col_tiles;
+    const int h = (int)(nh % (uint32_t)p.v_heads), n = (int)(nh / (uint32_t)p.v_heads);
+    const int hk = h / (p.v_heads / p.heads);
+    const int cg = lane & 7, rg = lane >> 3;
+    const int c0 = tile * kStepCols + 4 * cg;
+    const int cols = p.dim_v - c0;                       // of this lane's four
+    const TokenRange range = sequence_tokens(p, n);
+
+    if (p.cu_seqlens != nullptr && rg == 0) {            // tokens in front of the first sequence and behind the last
+        auto clear = [&](int64_t lo, int64_t hi) {
+            for (int64_t t = lo; t < hi; ++t)
+                for (int i = 0; i < 4 && i < cols; ++i)
+                    static_cast<T *>(p.out)[t * p.out_stride_l + h * p.out_stride_h + c0 + i] = Elem<DT>::from_float(0.f);
+        };
+        if (n == 0) clear(0, range.lo);
+        if (n == p.sequences - 1) clear(range.hi, p.seqlen);
+    }
+
+    int64_t slot = n;
+    if (a.indices != nullptr) slot = a.indices[n];
+    if (slot < 0 || slot >= a.slots) {                   // padding: zeros, no state touched
+        if (rg == 0)
+            for (int64_t t = range.lo; t < range.hi; ++t)
+                for (int i = 0; i < 4 && i < cols; ++i)
+                    static_cast<T *>(p.out)[range.b * p.out_stride_b + t * p.out_stride_l + h * p.out_stride_h + c0 + i] = Elem<DT>::from_float(0.f);
+        return;
+    }
+
+    float s[KR][4];
+    const float *src = p.initial_states == nullptr ? nullptr : p.initial_states + slot * p.init_stride_n + h * p.init_stride_h;
+#pragma unroll
+    for (int i = 0; i < KR; ++i) {
+        const int row = rg * KR + i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+        if (src != nullptr && row < p.dim_k && cols > 0) load4<CC1D_F32>(src, row * p.init_stride_k + c0, cols, a.vec_state, s[i]);
+    }
+
+    float *kq = &lds[wave][0][0], *qq = &lds[wave][1][0];
+    constexpr int NE = (8 * KR + 63) / 64;               // elements of k and q a lane fetches
+    for (int64_t t = range.lo; t < range.hi; ++t) {
+        const T *qp = static_cast<const T *>(p.q) + range.b * p.q_stride_b + t * p.q_stride_l + hk * p.q_stride_h;
+        const T *kp = static_cast<const T *>(p.k) + range.b * p.k_stride_b + t * p.k_stride_l + hk * p.k_stride_h;
+        float ke[NE], qe[NE], kk = 0.f, qs = 0.f, dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            const int i = lane + 64 * e;
+            ke[e] = i < p.dim_k ? Elem<DT>::to_float(kp[i]) : 0.f;
+            qe[e] = i < p.dim_k ? Elem<DT>::to_float(qp[i]) : 0.f;
+        }
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (cols > 0) load4<DT>(p.v, range.b * p.v_stride_b + t * p.v_stride_l + h * p.v_stride_h + c0, cols, a.vec_x, v);
+        const float decay = expf(load_as_float(p.g, range.b * p.g_stride_b + t * p.g_stride_l + h * p.g_stride_h, p.g_dtype));
+        const float beta = load_as_float(p.beta, range.b * p.beta_stride_b + t * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) { kk += ke[e] * ke[e]; qs += qe[e] * qe[e]; dot += ke[e] * qe[e]; }
+        dot = wave_sum(dot);
+        float rk = 1.f, rq = p.scale;
+        if (p.qk_l2norm) {
+            rk = rsqrtf(wave_sum(kk) + kNormEps);
+            rq = p.scale * rsqrtf(wave_sum(qs) + kNormEps);
+        }
+        wave_lds_fence();                                // the token before has been read
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            const int i = lane + 64 * e;
+            if (i < 8 * KR) { kq[i] = ke[e] * rk; qq[i] = qe[e] * rq; }
+        }
+        wave_lds_fence();
+        float sk[4] = {0.f, 0.f, 0.f, 0.f}, sq[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            const float ki = kq[rg * KR + i], qi = qq[rg * KR + i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] *= decay;
+                sk[j] += s[i][j] * ki;
+                sq[j] += s[i][j] * qi;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int d = 8; d < 64; d <<= 1) { sk[j] += __shfl_xor(sk[j], d); sq[j] += __shfl_xor(sq[j], d); }
+        }
+        float u[4], o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            u[j] = beta * (v[j] - sk[j]);
+            o[j] = sq[j] + dot * rk * rq * u[j];
+        }
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            const float ki = kq[rg * KR + i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] += ki * u[j];
+        }
+        if (rg == 0) {
+            T *op = static_cast<T *>(p.out) + range.b * p.out_stride_b + t * p.out_stride_l + h * p.out_stride_h + c0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < cols) op[j] = Elem<DT>::from_float(o[j]);
+        }
+    }
+
+    if (p.final_states == nullptr) return;
+    float *dst = p.final_states + slot * p.final_stride_n + h * p.final_stride_h;
+#pragma unroll
+    for (int i = 0; i < KR; ++i) {
+        const int row = rg * KR + i;
+        if (row >= p.dim_k || cols <= 0) continue;
+        float *d = dst + row * p.final_stride_k + c0;
+        if (a.vec_state) {
+            float4 r; r.x = s[i][0]; r.y = s[i][1]; r.z = s[i][2]; r.w = s[i][3];
+            *reinterpret_cast<float4 *>(d) = r;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < cols) d[j] = s[i][j];
+        }
+    }
+}
+
+template <int DT, int KR>
+int launch_rows(const StepArgs &a, hipStream_t stream) {
+    CC1D_LAUNCH((delta_step_kernel<DT, KR>), dim3((a.items + 3) / 4), dim3(kBlock), 0, stream, a);
+    return launch_status();
+}
+template <int DT>
+int launch_dtype(const StepArgs &a, hipStream_t stream) {
+    return a.p.dim_k <= 64 ? launch_rows<DT, 8>(a, stream) : a.p.dim_k <= 128 ? launch_rows<DT, 16>(a, stream) : launch_rows<DT, 32>(a, stream);
+}
+
+}  // namespace
+
+
+int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, hipStream_t stream) {
+    StepArgs a = {};
+    a.p = p;
+    a.indices = indices;
+    a.slots = slots;
+    a.col_tiles = (uint32_t)((p.dim_v + kStepCols - 1) / kStepCols);
+    const int64_t items = (int64_t)p.sequences * p.v_heads * a.col_tiles;
+    if (items == 0) return CC1D_OK;
+    if (items * 64 >= thread_limit()) return CC1D_ERR_TOO_LARGE;
+    a.items = (uint32_t)items;
+    auto whole = [&](const void *s, int64_t sn, int64_t sh, int64_t sk) {
+        return s == nullptr || (aligned16(s) && sn % 4 == 0 && sh % 4 == 0 && sk % 4 == 0);
+    };
+    a.vec_state = p.dim_v % 4 == 0 && whole(p.initial_states, p.init_stride_n, p.init_stride_h, p.init_stride_k) &&
+                  whole(p.final_states, p.final_stride_n, p.final_stride_h, p.final_stride_k);
+    a.vec_x = p.dim_v % 4 == 0 && p.v_stride_b % 4 == 0 && p.v_stride_l % 4 == 0 && p.v_stride_h % 4 == 0 &&
+              (reinterpret_cast<uintptr_t>(p.v) & (4u * (uint32_t)elem_bytes(p.x_dtype) - 1u)) == 0;
+    switch (p.x_dtype) {
+        case CC1D_F32: return launch_dtype<CC1D_F32>(a, stream);
+        case CC1D_F16: return launch_dtype<CC1D_F16>(a, stream);
+        default: return launch_dtype<CC1D_BF16>(a, stream);
+    }
+}
+
+}  // namespace cc1d

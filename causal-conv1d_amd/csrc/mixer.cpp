@@ -1,0 +1,329 @@
+// PyTorch binding of cc1d_mixer.h: the gated delta rule and the root-mean-square norm as ops of the DaoAILab
+// library, part of the extension module `causal_conv1d_cuda`.  Host-only C++: tensors are checked, results and
+// workspaces come from the caching allocator, launches go to the current stream of the tensors' device.
+#include <torch/library.h>
+#include <torch/types.h>
+#include <c10/core/DeviceGuard.h>
+
+#include <optional>
+#include <tuple>
+
+#include "cc1d_mixer.h"
+#include "cc1d_torch.hpp"
+
+namespace {
+
+using OptTensor = std::optional<at::Tensor>;
+
+// Unit stride along the last dimension (of more than one element).
+bool unit_last(const at::Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
+at::Tensor rows_of(const at::Tensor &t) { return unit_last(t) ? t : t.contiguous(); }
+
+void check_gpu(const at::Tensor &t, const at::Tensor &like, const char *what) {
+    TORCH_CHECK(t.is_cuda(), what, " must be on the GPU");
+    TORCH_CHECK(t.device() == like.device(), what, " must be on the device of the other tensors");
+}
+
+at::Tensor workspace_of(size_t bytes, const at::Tensor &like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// ---- gated delta rule ----------------------------------------------------------------
+
+struct DeltaInputs {
+    at::Tensor q, k, v, g, beta;
+    int64_t batch, seqlen, heads, v_heads, dim_k, dim_v;
+};
+
+DeltaInputs delta_inputs(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta) {
+    check_gpu(q, q, "q"); check_gpu(k, q, "k"); check_gpu(v, q, "v"); check_gpu(g, q, "g"); check_gpu(beta, q, "beta");
+    TORCH_CHECK(q.dim() == 4, "q must be (batch, seqlen, heads, dim_k)");
+    TORCH_CHECK(v.dim() == 4, "v must be (batch, seqlen, v_heads, dim_v)");
+    DeltaInputs d;
+    d.batch = q.size(0); d.seqlen = q.size(1); d.heads = q.size(2); d.dim_k = q.size(3);
+    d.v_heads = v.size(2); d.dim_v = v.size(3);
+    const int64_t batch = d.batch, seqlen = d.seqlen, heads = d.heads, v_heads = d.v_heads, dim_k = d.dim_k, dim_v = d.dim_v;
+    CHECK_SHAPE(k, batch, seqlen, heads, dim_k);
+    CHECK_SHAPE(v, batch, seqlen, v_heads, dim_v);
+    CHECK_SHAPE(g, batch, seqlen, v_heads);
+    CHECK_SHAPE(beta, batch, seqlen, v_heads);
+    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have the same dtype");
+    d.q = rows_of(q); d.k = rows_of(k); d.v = rows_of(v); d.g = g; d.beta = beta;
+    return d;
+}
+
+#define SET_STRIDES(P, NAME, T) P.NAME##_stride_b = T.stride(0); P.NAME##_stride_l = T.stride(1); P.NAME##_stride_h = T.stride(2)
+#define SET_STATE(P, NAME, T) P.NAME##_stride_n = T.stride(0); P.NAME##_stride_h = T.stride(1); P.NAME##_stride_k = T.stride(2)
+
+template <typename P>
+void set_inputs(P &p, const DeltaInputs &d, double scale, bool qk_l2norm) {
+    p.batch = size32(d.batch, "batch"); p.seqlen = size32(d.seqlen, "seqlen");
+    p.heads = size32(d.heads, "heads"); p.v_heads = size32(d.v_heads, "v_heads");
+    p.dim_k = size32(d.dim_k, "dim_k"); p.dim_v = size32(d.dim_v, "dim_v");
+    p.x_dtype = to_cc1d_dtype(d.q.scalar_type(), "q");
+    p.g_dtype = to_cc1d_dtype(d.g.scalar_type(), "g");
+    p.beta_dtype = to_cc1d_dtype(d.beta.scalar_type(), "beta");
+    p.qk_l2norm = qk_l2norm ? 1 : 0;
+    p.scale = (float)scale;
+    p.q = d.q.data_ptr(); SET_STRIDES(p, q, d.q);
+    p.k = d.k.data_ptr(); SET_STRIDES(p, k, d.k);
+    p.v = d.v.data_ptr(); SET_STRIDES(p, v, d.v);
+    p.g = d.g.data_ptr(); SET_STRIDES(p, g, d.g);
+    p.beta = d.beta.data_ptr(); SET_STRIDES(p, beta, d.beta);
+}
+
+void check_states(const at::Tensor &s, const DeltaInputs &d, int64_t n, const char *what) {
+    check_gpu(s, d.q, what);
+    TORCH_CHECK(s.scalar_type() == at::kFloat, what, " must be float32");
+    TORCH_CHECK(s.sizes() == at::IntArrayRef({n, d.v_heads, d.dim_k, d.dim_v}), what, " must have shape (sequences, v_heads, dim_k, dim_v)");
+}
+
+int64_t sequences_of(const DeltaInputs &d, const OptTensor &cu) {
+    if (!cu.has_value()) return d.batch;
+    check_gpu(*cu, d.q, "cu_seqlens");
+    TORCH_CHECK(d.batch == 1, "cu_seqlens needs a batch of 1: sequences packed back to back");
+    TORCH_CHECK(cu->dim() == 1 && cu->size(0) >= 1, "cu_seqlens must be (sequences + 1,)");
+    TORCH_CHECK(cu->is_contiguous(), "cu_seqlens must be contiguous");
+    TORCH_CHECK(cu->scalar_type() == at::kInt || cu->scalar_type() == at::kLong, "cu_seqlens must be int32 or int64");
+    return cu->size(0) - 1;
+}
+
+cc1d_delta_params delta_params(const DeltaInputs &d, const OptTensor &init, const OptTensor &cu, double scale, bool qk_l2norm) {
+    cc1d_delta_params p = {};
+    set_inputs(p, d, scale, qk_l2norm);
+    p.sequences = size32(sequences_of(d, cu), "sequences");
+    if (cu.has_value()) { p.cu_seqlens = cu->data_ptr(); p.cu_seqlens_is_int64 = cu->scalar_type() == at::kLong ? 1 : 0; }
+    if (init.has_value()) {
+        check_states(*init, d, p.sequences, "initial_states");
+        TORCH_CHECK(unit_last(*init), "initial_states must have unit stride along dim_v");
+        p.initial_states = init->data_ptr<float>(); SET_STATE(p, init, (*init));
+    }
+    return p;
+}
+
+at::Tensor delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm) {
+    const DeltaInputs d = delta_inputs(q, k, v, g, beta);
+    OptTensor init = initial_states;
+    if (init.has_value()) init = rows_of(*init);
+    cc1d_delta_params p = delta_params(d, init, cu_seqlens, scale, qk_l2norm);
+    c10::DeviceGuard guard(q.device());
+    at::Tensor out = at::empty({d.batch, d.seqlen, d.v_heads, d.dim_v}, d.v.options());
+    p.out = out.data_ptr(); SET_STRIDES(p, out, out);
+    if (final_states_out.has_value()) {
+        const at::Tensor &f = *final_states_out;
+        check_states(f, d, p.sequences, "final_states_out");
+        TORCH_CHECK(unit_last(f), "final_states_out must have unit stride along dim_v");
+        p.final_states = f.data_ptr<float>(); SET_STATE(p, final, f);
+    }
+    size_t bytes = 0;
+    check_status(cc1d_delta_workspace_bytes(&p, &bytes), "gated_delta_rule");
+    const at::Tensor ws = workspace_of(bytes, q);
+    check_status(cc1d_delta_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "gated_delta_rule");
+    return out;
+}
+
+at::Tensor delta_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                        at::Tensor &state, const OptTensor &state_indices, double scale, bool qk_l2norm) {
+    const bool flat = q.dim() == 3;                      // (batch, heads, dim): one token, no seqlen axis
+    auto with_tokens = [&](const at::Tensor &t) { return flat ? t.unsqueeze(1) : t; };
+    const DeltaInputs d = delta_inputs(with_tokens(q), with_tokens(k), with_tokens(v), with_tokens(g), with_tokens(beta));
+    cc1d_delta_step_params p = {};
+    set_inputs(p, d, scale, qk_l2norm);
+    check_gpu(state, q, "state");
+    TORCH_CHECK(state.dim() == 4, "state must be (slots, v_heads, dim_k, dim_v)");
+    check_states(state, d, state_indices.has_value() ? state.size(0) : d.batch, "state");
+    TORCH_CHECK(unit_last(state), "state must have unit stride along dim_v");
+    p.state_slots = size32(state.size(0), "state slots");
+    p.state = state.data_ptr<float>(); SET_STATE(p, state, state);
+    if (state_indices.has_value()) {
+        const at::Tensor &i = *state_indices;
+        check_gpu(i, q, "state_indices");
+        TORCH_CHECK(i.scalar_type() == at::kInt, "state_indices must be int32");
+        TORCH_CHECK(i.dim() == 1 && i.size(0) == d.batch && i.is_contiguous(), "state_indices must be (batch,), contiguous");
+        p.state_indices = i.data_ptr<int32_t>();
+    }
+    c10::DeviceGuard guard(q.device());
+    at::Tensor out = at::empty({d.batch, d.seqlen, d.v_heads, d.dim_v}, d.v.options());
+    p.out = out.data_ptr(); SET_STRIDES(p, out, out);
+    check_status(cc1d_delta_step(&p, current_stream()), "gated_delta_rule_update");
+    return flat ? out.squeeze(1) : out;
+}
+
+at::Tensor delta_fwd_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const at::Tensor &,
+                          const OptTensor &, const OptTensor &, const OptTensor &, double, bool) {
+    return at::empty_symint(v.sym_sizes(), v.options());
+}
+at::Tensor delta_update_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const at::Tensor &,
+                             at::Tensor &, const OptTensor &, double, bool) {
+    return at::empty_symint(v.sym_sizes(), v.options());
+}
+
+// ---- root-mean-square norm -----------------------------------------------------------
+
+// (rows, dim) view of t (..., dim) with one stride between rows, a copy where there is none.
+at::Tensor as_rows(const at::Tensor &t) {
+    TORCH_CHECK(t.dim() >= 1, "x must have at least one dimension");
+    const int64_t dim = t.size(-1);
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) rows *= t.size(i);
+    return rows_of(t.dim() == 2 ? t : t.reshape({rows, dim}));
+}
+
+struct NormInputs { at::Tensor x, residual, weight; };
+NormInputs norm_inputs(const at::Tensor &x, const at::Tensor &weight, const OptTensor &residual) {
+    check_gpu(x, x, "x"); check_gpu(weight, x, "weight");
+    NormInputs n;
+    n.x = as_rows(x);
+    const int64_t dim = n.x.size(1);
+    CHECK_SHAPE(weight, dim);
+    n.weight = weight.contiguous();
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, "weight must have the dtype of x or float32");
+    if (residual.has_value()) {
+        check_gpu(*residual, x, "residual");
+        TORCH_CHECK(residual->sizes() == x.sizes(), "residual must have the shape of x");
+        TORCH_CHECK(residual->scalar_type() == x.scalar_type() || residual->scalar_type() == at::kFloat, "residual must have the dtype of x or float32");
+        n.residual = as_rows(*residual);
+    }
+    return n;
+}
+
+// y or (y8, scales), and h where there is a residual (else an empty tensor).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_run(const at::Tensor &x, const at::Tensor &weight, const OptTensor &residual, double eps, bool quantised) {
+    const NormInputs n = norm_inputs(x, weight, residual);
+    c10::DeviceGuard guard(x.device());
+    cc1d_norm_params p = {};
+    p.rows = n.x.size(0); p.dim = size32(n.x.size(1), "dim"); p.eps = (float)eps;
+    p.x_dtype = p.r_dtype = to_cc1d_dtype(x.scalar_type(), "x");
+    p.w_dtype = to_cc1d_dtype(weight.scalar_type(), "weight");
+    p.x = n.x.data_ptr(); p.x_stride = n.x.stride(0);
+    p.weight = n.weight.data_ptr();
+    at::Tensor h, scales;
+    if (residual.has_value()) {
+        p.r_dtype = to_cc1d_dtype(residual->scalar_type(), "residual");
+        p.residual = n.residual.data_ptr(); p.residual_stride = n.residual.stride(0);
+        h = at::empty(x.sizes(), residual->options());
+        p.h = h.data_ptr(); p.h_stride = p.dim;
+    } else {
+        h = at::empty({0}, x.options());
+    }
+    at::Tensor y = at::empty(x.sizes(), quantised ? x.options().dtype(at::kFloat8_e4m3fn) : x.options());
+    if (quantised) {
+        scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+        if (p.dim == 0) scales.zero_();
+        p.y8 = y.data_ptr(); p.y8_stride = p.dim; p.scales = scales.data_ptr<float>();
+    } else {
+        p.y = y.data_ptr(); p.y_stride = p.dim;
+    }
+    check_status(cc1d_norm_fwd(&p, current_stream()), "rms_norm");
+    return {y, scales, h};
+}
+
+std::tuple<at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, const at::Tensor &weight, const OptTensor &residual, double eps) {
+    auto r = norm_run(x, weight, residual, eps, false);
+    return {std::get<0>(r), std::get<2>(r)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_quant(const at::Tensor &x, const at::Tensor &weight, const OptTensor &residual, double eps) {
+    return norm_run(x, weight, residual, eps, true);
+}
+
+// h: what was normalised.  dx in the dtype of dy, dresidual in that of h; where the two are the same type they are
+// one tensor, and dresidual comes back empty.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &h, const at::Tensor &weight, const at::Tensor &dy, const OptTensor &dh, double eps) {
+    check_gpu(h, h, "h"); check_gpu(weight, h, "weight"); check_gpu(dy, h, "dy");
+    TORCH_CHECK(dy.sizes() == h.sizes(), "dy must have the shape of h");
+    const at::Tensor hr = as_rows(h), dyr = as_rows(dy), w = weight.contiguous();
+    const int64_t dim = hr.size(1);
+    CHECK_SHAPE(weight, dim);
+    c10::DeviceGuard guard(h.device());
+    cc1d_norm_bwd_params p = {};
+    p.rows = hr.size(0); p.dim = size32(dim, "dim"); p.eps = (float)eps;
+    p.x_dtype = to_cc1d_dtype(dy.scalar_type(), "dy");
+    p.r_dtype = to_cc1d_dtype(h.scalar_type(), "h");
+    p.w_dtype = to_cc1d_dtype(weight.scalar_type(), "weight");
+    p.h = hr.data_ptr(); p.h_stride = hr.stride(0);
+    p.weight = w.data_ptr();
+    p.dy = dyr.data_ptr(); p.dy_stride = dyr.stride(0);
+    at::Tensor dhr;
+    if (dh.has_value()) {
+        check_gpu(*dh, h, "dh");
+        TORCH_CHECK(dh->sizes() == h.sizes() && dh->scalar_type() == h.scalar_type(), "dh must have the shape and dtype of h");
+        dhr = as_rows(*dh);
+        p.dh = dhr.data_ptr(); p.dh_stride = dhr.stride(0);
+    }
+    at::Tensor dx = at::empty(h.sizes(), dy.options());
+    p.dx = dx.data_ptr(); p.dx_stride = dim;
+    const bool both = dy.scalar_type() != h.scalar_type();
+    at::Tensor dres = both ? at::empty(h.sizes(), h.options()) : at::empty({0}, h.options());
+    if (both) { p.dresidual = dres.data_ptr(); p.dresidual_stride = dim; }
+    at::Tensor dw = at::empty({dim}, weight.options());
+    p.dweight = dw.data_ptr();
+    size_t bytes = 0;
+    check_status(cc1d_norm_bwd_workspace_bytes(&p, &bytes), "rms_norm backward");
+    const at::Tensor ws = workspace_of(bytes, h);
+    check_status(cc1d_norm_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "rms_norm backward");
+    return {dx, dres, dw};
+}
+
+at::Tensor dequantize(const at::Tensor &y8, const at::Tensor &scales, at::ScalarType dtype) {
+    check_gpu(y8, y8, "y8"); check_gpu(scales, y8, "scales");
+    TORCH_CHECK(y8.scalar_type() == at::kFloat8_e4m3fn, "y8 must be float8_e4m3fn");
+    TORCH_CHECK(scales.scalar_type() == at::kFloat, "scales must be float32");
+    TORCH_CHECK(y8.dim() >= 1 && scales.sizes() == y8.sizes().slice(0, y8.dim() - 1), "scales must have the shape of y8 without its last dimension");
+    const at::Tensor r = as_rows(y8), s = scales.contiguous();
+    c10::DeviceGuard guard(y8.device());
+    at::Tensor y = at::empty(y8.sizes(), y8.options().dtype(dtype));
+    cc1d_dequantize_params p = {};
+    p.rows = r.size(0); p.dim = size32(r.size(1), "dim"); p.y_dtype = to_cc1d_dtype(dtype, "dtype");
+    p.y8 = r.data_ptr(); p.y8_stride = r.stride(0);
+    p.scales = s.data_ptr<float>();
+    p.y = y.data_ptr(); p.y_stride = p.dim;
+    check_status(cc1d_dequantize_rows(&p, current_stream()), "dequantize_rows");
+    return y;
+}
+
+std::tuple<at::Tensor, at::Tensor> norm_fwd_meta(const at::Tensor &x, const at::Tensor &, const OptTensor &residual, double) {
+    return {at::empty_symint(x.sym_sizes(), x.options()), residual.has_value() ? at::empty_symint(x.sym_sizes(), residual->options()) : at::empty({0}, x.options())};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_quant_meta(const at::Tensor &x, const at::Tensor &, const OptTensor &residual, double) {
+    return {at::empty_symint(x.sym_sizes(), x.options().dtype(at::kFloat8_e4m3fn)), at::empty_symint(x.sym_sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat)),
+            residual.has_value() ? at::empty_symint(x.sym_sizes(), residual->options()) : at::empty({0}, x.options())};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd_meta(const at::Tensor &h, const at::Tensor &weight, const at::Tensor &dy, const OptTensor &, double) {
+    return {at::empty_symint(h.sym_sizes(), dy.options()), dy.scalar_type() != h.scalar_type() ? at::empty_symint(h.sym_sizes(), h.options()) : at::empty({0}, h.options()),
+            at::empty_symint(weight.sym_sizes(), weight.options())};
+}
+at::Tensor dequantize_meta(const at::Tensor &y8, const at::Tensor &, at::ScalarType dtype) {
+    return at::empty_symint(y8.sym_sizes(), y8.options().dtype(dtype));
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(DaoAILab, m) {
+    m.def("_gated_delta_rule_fwd_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? initial_states, "
+          "Tensor? cu_seqlens, Tensor(a!)? final_states_out, float scale, bool qk_l2norm) -> Tensor", {at::Tag::pt2_compliant_tag});
+    m.def("_gated_delta_rule_update_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor(a!) state, "
+          "Tensor? state_indices, float scale, bool qk_l2norm) -> Tensor", {at::Tag::pt2_compliant_tag});
+    m.def("_rms_norm_fwd_cpp(Tensor x, Tensor weight, Tensor? residual, float eps) -> (Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+    m.def("_rms_norm_bwd_cpp(Tensor h, Tensor weight, Tensor dy, Tensor? dh, float eps) -> (Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+    m.def("_rms_norm_quant_cpp(Tensor x, Tensor weight, Tensor? residual, float eps) -> (Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+    m.def("_dequantize_rows_cpp(Tensor y8, Tensor scales, ScalarType dtype) -> Tensor", {at::Tag::pt2_compliant_tag});
+}
+
+TORCH_LIBRARY_IMPL(DaoAILab, CompositeExplicitAutograd, m) {
+    m.impl("_gated_delta_rule_fwd_cpp", &delta_fwd);
+    m.impl("_gated_delta_rule_update_cpp", &delta_update);
+    m.impl("_rms_norm_fwd_cpp", &norm_fwd);
+    m.impl("_rms_norm_bwd_cpp", &norm_bwd);
+    m.impl("_rms_norm_quant_cpp", &norm_quant);
+    m.impl("_dequantize_rows_cpp", &dequantize);
+}
+
+TORCH_LIBRARY_IMPL(DaoAILab, Meta, m) {
+    m.impl("_gated_delta_rule_fwd_cpp", &delta_fwd_meta);
+    m.impl("_gated_delta_rule_update_cpp", &delta_update_meta);
+    m.impl("_rms_norm_fwd_cpp", &norm_fwd_meta);
+    m.impl("_rms_norm_bwd_cpp", &norm_bwd_meta);
+    m.impl("_rms_norm_quant_cpp", &norm_quant_meta);
+    m.impl("_dequantize_rows_cpp", &dequantize_meta);
+}

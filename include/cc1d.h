@@ -60,7 +60,10 @@ typedef enum cc1d_status {
     CC1D_ERR_LAUNCH = -17,           /* the HIP runtime refused the launch */
     CC1D_ERR_UNKNOWN_TUNABLE = -18,
     CC1D_ERR_WORKSPACE_LIMIT = -19,  /* cc1d_bwd_noalloc: the problem needs more than the built-in workspace */
-    CC1D_ERR_IN_PLACE = -20          /* out shares elements with x, or dx with x or dout: no kernel works in place */
+    CC1D_ERR_IN_PLACE = -20,         /* out shares elements with x, or dx with x or dout: no kernel works in place */
+    CC1D_ERR_HEADS = -21,            /* v_heads is no multiple of heads (cc1d_mixer.h) */
+    CC1D_ERR_HEAD_DIM = -22,         /* dim_k outside [1, 256] or dim_v outside [1, 512] (cc1d_mixer.h) */
+    CC1D_ERR_ROW_LAYOUT = -23        /* a stride or an address that is no whole number of elements (cc1d_mixer.h) */
 } cc1d_status;
 
 /* Opaque stream handle: pass a hipStream_t (NULL = the default stream). */
