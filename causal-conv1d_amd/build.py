@@ -38,10 +38,12 @@ KERNEL_SOURCES = [
     "cc1d_varlen_states.hip",
     "cc1d_delta_api.cpp",
     "cc1d_delta_step.hip",
+    "cc1d_delta_prep.hip",
+    "cc1d_delta_scan.hip",
     "cc1d_norm.hip",
 ]
 KERNEL_HEADERS = ["cc1d_device.hpp", "cc1d_internal.hpp", "cc1d_bwd_channellast_kernel.hpp"]
-DELTA_HEADERS = ["cc1d_delta.hpp", "cc1d_delta_host.hpp"]   # of the sources that begin with cc1d_delta
+DELTA_HEADERS = ["cc1d_delta.hpp", "cc1d_delta_chunk.hpp", "cc1d_delta_host.hpp"]   # of the sources that begin with cc1d_delta
 PUBLIC_HEADERS = ["cc1d.h", "cc1d_mixer.h"]
 BINDING_SOURCES = ["causal_conv1d.cpp", "mixer.cpp"]
 BINDING_HEADERS = ["cc1d_torch.hpp"]

@@ -1,5 +1,6 @@
 // C-ABI front of the gated delta rule (cc1d_mixer.h): argument validation and dispatch to the kernel
 // launchers.  Nothing here allocates or synchronises; validation never touches the GPU.
+#include "cc1d_delta_chunk.hpp"
 #include "cc1d_delta_host.hpp"
 
 using namespace cc1d;
@@ -34,6 +35,45 @@ int check_delta(const cc1d_delta_params &p) {
     return CC1D_OK;
 }
 
+// Sequences of this many tokens on average go by chunks.
+constexpr int kChunkedFrom = 24;
+bool chunked(const cc1d_delta_params &p) {
+    return p.batch > 0 && p.v_heads > 0 && p.sequences > 0 && p.seqlen >= (int64_t)kChunkedFrom * (p.cu_seqlens == nullptr ? 1 : p.sequences);
+}
+
+// Places in the workspace; returns its size.
+size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWork &w) {
+    w = ChunkWork();
+    w.chunks = (p.seqlen + kChunk - 1) / kChunk;
+    w.slots = p.cu_seqlens == nullptr ? p.batch * w.chunks : p.seqlen / kChunk + p.sequences + 1;
+    w.ks = key_steps(p.dim_k);
+    w.terms = p.x_dtype == CC1D_BF16 ? 1 : p.x_dtype == CC1D_F16 ? 2 : 3;
+    w.pterms = p.x_dtype == CC1D_F32 ? 3 : 2;
+    w.backward = backward;
+    const size_t keys = (size_t)w.slots * p.heads, values = (size_t)w.slots * p.v_heads;
+    size_t used = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *at = base + used;
+        used += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    w.kf = take(keys * w.kbytes()); w.qf = take(keys * w.kbytes()); w.ktf = take(keys * w.kbytes());
+    w.tf = take(values * w.tbytes()); w.pf = take(values * w.pbytes());
+    w.scalars = reinterpret_cast<float *>(take(values * kScalars * kChunk * sizeof(float)));
+    if (backward) {
+        const size_t state = values * p.dim_k * p.dim_v * sizeof(float), rows = values * kChunk * p.dim_v * sizeof(float);
+        w.qtf = take(keys * w.kbytes()); w.ttf = take(values * w.tbytes()); w.ptf = take(values * w.pbytes());
+        w.s0 = reinterpret_cast<float *>(take(state)); w.ds1 = reinterpret_cast<float *>(take(state));
+        w.u = reinterpret_cast<float *>(take(rows)); w.dx = reinterpret_cast<float *>(take(rows));
+    }
+    return used;
+}
+// Grids of one workgroup a (slot, value head) and of one a (sequence, value head, 16 columns).
+bool fits(const cc1d_delta_params &p, const ChunkWork &w) {
+    const int64_t limit = thread_limit() / kBlock;
+    return (int64_t)w.slots * p.v_heads < limit && ((int64_t)p.sequences * p.v_heads + 8) * ((p.dim_v + 15) / 16) < limit;
+}
+
 }  // namespace
 
 extern "C" {
@@ -50,7 +90,10 @@ int cc1d_delta_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
     *bytes = 0;
     const int st = cc1d_validate_delta(p);
-    return st;
+    if (st != CC1D_OK || !chunked(*p)) return st;
+    ChunkWork w;
+    *bytes = lay_out(*p, false, nullptr, w);
+    return fits(*p, w) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_delta_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
@@ -59,7 +102,12 @@ int cc1d_delta_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace
     if (st != CC1D_OK) return st;
     if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
     if (p->batch == 0 || p->v_heads == 0 || p->sequences == 0) return CC1D_OK;
-    return launch_delta_tokens(*p, nullptr, p->sequences, static_cast<hipStream_t>(stream));
+    const hipStream_t hs = static_cast<hipStream_t>(stream);
+    if (!chunked(*p)) return launch_delta_tokens(*p, nullptr, p->sequences, hs);
+    ChunkWork w;
+    lay_out(*p, false, static_cast<uint8_t *>(workspace), w);
+    const int done = launch_delta_prep(*p, w, hs);
+    return done != CC1D_OK ? done : launch_delta_scan(*p, w, false, hs);
 }
 
 int cc1d_validate_delta_step(const cc1d_delta_step_params *p) {

@@ -1,0 +1,146 @@
+// The gated delta rule by chunks of 64 tokens: what its kernels share.
+//
+// With G the running sum of g inside a chunk, gam_i = exp(G_i), E_ij = exp(G_i - G_j), keys and queries of a chunk the
+// rows of K and Q, S0 the state in front of it:
+//
+//   A = strict lower (beta_i E_ij k_i.k_j),  T = (I + A)^-1,  P = scale lower (E_ij q_i.k_j)
+//   U = T diag(beta) (V - diag(gam) K S0)
+//   O = scale diag(gam) Q S0 + P U,   S1 = gam_last S0 + K^T diag(gam_last / gam_j) U
+//
+// T and P need no state: the prep kernel makes them for all chunks at once.  What is left between one chunk and the
+// next is three products, and columns of S (dim_v) do not meet, so the scan takes 16 of them to a workgroup.
+//
+// Products.  The matrix cores take 16-bit operands; a number x of 24 bits is the exact sum of three bfloat16
+// (each the rest, rounded), so a product of two such is nine exact products, of which the six largest carry it to
+// 2^-25.  bfloat16 q, k, v, dout are one term each and cost nothing, float16 is two.
+// Six products on the 16-bit cores take 0.38 of the time of the fp32 ones; one and three together a third of that.
+//
+// Operand order.  An MFMA of 16 x 16 x 32 wants of its left operand 8 consecutive columns of one row a lane, of its right one 8
+// consecutive rows of one column, and leaves 4 rows of one column.  Which row of a matrix a tile's row is, is free as long
+// as both sides agree: rows are dealt so that the 4 + 4 rows of two result tiles are 8 consecutive ones (row_of),
+// and a result becomes the next product's right operand without leaving its lane.
+#pragma once
+
+#include "cc1d_delta.hpp"
+
+namespace cc1d {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// The row of a matrix that row m of 16-row tile t is.
+__device__ __host__ __forceinline__ constexpr int row_of(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
+
+// Terms of q, k, v, dout; of P, U and S where they make outputs of 16 bits.
+template <int DT> struct Terms { static constexpr int n = DT == CC1D_BF16 ? 1 : DT == CC1D_F16 ? 2 : 3, p = DT == CC1D_F32 ? 3 : 2; };
+
+// Scalars of a chunk's tokens, one vector of 64 each, per (chunk, value head).
+enum { kSeenBeta, kBeta, kReadGate, kCarry, kKeyNorm, kQueryNorm, kGate, kToEnd, kSumHi, kSumLo, kScalars };
+//     beta gam rk   beta   scale gam rq  dec rk  rk        rq          gam    dec     G = hi + lo
+
+constexpr int kFrag = 1024;              // bytes of one operand of 16 x 32 bfloat16
+constexpr int kTriFrags = 6;             // of a triangular 64 x 64 matrix: 2 tiles x 1 step + 2 tiles x 2 steps
+__device__ __host__ __forceinline__ constexpr int lower_frag(int t, int s) { return t < 2 ? t : 2 + 2 * (t - 2) + s; }
+__device__ __host__ __forceinline__ constexpr int upper_frag(int t, int s) { return t < 2 ? 2 * t + s : 4 + (t - 2); }
+
+// Where everything lies in the workspace.  "slot": one chunk of one sequence; without cu_seqlens n ceil(seqlen / 64) + c, with
+// it floor(first token / 64) + n + c, which no two chunks share.
+struct ChunkWork {
+    uint8_t *kf, *qf, *ktf, *qtf;        // per (slot, head): K, Q rows x dim_k; K^T, Q^T dim_k x rows
+    uint8_t *tf, *pf, *ttf, *ptf;        // per (slot, value head): T, P lower; T^T, P^T upper
+    float *scalars;                      // per (slot, value head): [kScalars][64]
+    float *s0, *ds1;                     // per (slot, value head): (dim_k, dim_v)
+    float *u, *dx;                       // per (slot, value head): (64, dim_v)
+    int32_t slots, chunks;               // chunks: of one sequence without cu_seqlens
+    int32_t ks, terms, pterms;           // 32-column steps of dim_k; terms of K and Q; of P
+    int32_t backward;
+    __device__ __host__ int64_t kbytes() const { return (int64_t)4 * ks * terms * kFrag; }
+    __device__ __host__ int64_t tbytes() const { return (int64_t)kTriFrags * 3 * kFrag; }
+    __device__ __host__ int64_t pbytes() const { return (int64_t)kTriFrags * pterms * kFrag; }
+};
+
+// Which chunk a slot is: tokens [lo, lo + count) of batch entry b, sequence n, or count = 0 if it is none.
+struct ChunkAt { int64_t lo; int count, b, n; };
+__device__ __forceinline__ ChunkAt chunk_at(const cc1d_delta_params &p, const ChunkWork &w, int slot) {
+    if (p.cu_seqlens == nullptr) {
+        const int n = slot / w.chunks, c = slot - n * w.chunks;
+        const int64_t lo = (int64_t)c * kChunk, left = p.seqlen - lo;
+        return {lo, (int)(left < kChunk ? left : kChunk), n, n};
+    }
+    // The last sequence whose first slot is not behind this one.
+    int a = 0, b = p.sequences;                          // a: first slot <= slot; sequence 0 begins at slot floor(cu[0] / 64)
+    while (b - a > 1) {
+        const int mid = (a + b) >> 1;
+        const int64_t first = cu_entry(p.cu_seqlens, p.cu_seqlens_is_int64, mid, p.seqlen) / kChunk + mid;
+        if (first <= slot) a = mid; else b = mid;
+    }
+    const TokenRange r = sequence_tokens(p, a);
+    const int64_t lo = r.lo + ((int64_t)slot - (r.lo / kChunk + a)) * kChunk, left = r.hi - lo;
+    if (lo < r.lo || left <= 0) return {0, 0, 0, a};
+    return {lo, (int)(left < kChunk ? left : kChunk), 0, a};
+}
+__device__ __forceinline__ int first_slot(const cc1d_delta_params &p, const ChunkWork &w, int n, const TokenRange &r) {
+    return p.cu_seqlens == nullptr ? n * w.chunks : (int)(r.lo / kChunk) + n;
+}
+
+// N bfloat16 terms of 4 (8) numbers, term i in two (four) words, each the rest rounded to nearest: two leave 2^-18 of a
+// number, three nothing.
+__device__ __forceinline__ uint32_t rounded_pair(float lo, float hi) {
+    bf16x2 h;
+    h.x = (__bf16)lo;
+    h.y = (__bf16)hi;
+    return bitcast<uint32_t>(h);
+}
+template <int N>
+__device__ __forceinline__ void split4(const float (&x)[4], u32x2 (&t)[N]) {
+    float r[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        t[n].x = rounded_pair(r[0], r[1]);
+        t[n].y = rounded_pair(r[2], r[3]);
+        if (n + 1 < N) {
+            r[0] -= bitcast<float>(t[n].x << 16); r[1] -= bitcast<float>(t[n].x & 0xffff0000u);
+            r[2] -= bitcast<float>(t[n].y << 16); r[3] -= bitcast<float>(t[n].y & 0xffff0000u);
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[N]) {
+    const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
+    u32x2 a[N], b[N];
+    split4<N>(lo, a);
+    split4<N>(hi, b);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        u32x4 w; w.x = a[n].x; w.y = a[n].y; w.z = b[n].x; w.w = b[n].y;
+        t[n] = bitcast<bf16x8>(w);
+    }
+}
+
+// acc += sum of a[i] b[j] with i + j <= MOST, the small ones first.
+template <int MOST, int NA, int NB>
+__device__ __forceinline__ f32x4 product(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 acc) {
+#pragma unroll
+    for (int sum = MOST; sum >= 0; --sum)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = sum - i;
+            if (j >= 0 && j < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc, 0, 0, 0);
+        }
+    return acc;
+}
+
+template <int N>
+__device__ __forceinline__ void load_frag(const uint8_t *base, int lane, bf16x8 (&f)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = bitcast<bf16x8>(*reinterpret_cast<const u32x4 *>(base + n * kFrag + lane * 16));
+}
+
+// A barrier that orders LDS alone: loads and stores of global memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+}  // namespace cc1d

@@ -1,13 +1,40 @@
 // Host-side contracts between the front of the gated delta rule (cc1d_delta_api.cpp) and its launchers.
 #pragma once
 
+#include <type_traits>
+
 #include "cc1d_internal.hpp"
 #include "cc1d_mixer.h"
 
 namespace cc1d {
 
+struct ChunkWork;
+
 // Token by token.  initial_states / final_states of `p` are the states read and written, `slots` of them, picked by
 // `indices` (NULL: sequence n has state n).
 int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, hipStream_t stream);
+// By chunks: what needs no state; then the states and outputs (`states`: only the states in front of the chunks and U).
+int launch_delta_prep(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream);
+int launch_delta_scan(const cc1d_delta_params &p, const ChunkWork &w, bool states, hipStream_t stream);
+
+// 32-column steps of dim_k that have kernels.
+inline int key_steps(int dim_k) { return dim_k <= 32 ? 1 : dim_k <= 64 ? 2 : dim_k <= 128 ? 4 : 8; }
+
+template <typename F>
+int by_type_and_steps(int dtype, int steps, F &&f) {
+    auto with = [&](auto dt) {
+        switch (steps) {
+            case 1: return f(dt, std::integral_constant<int, 1>());
+            case 2: return f(dt, std::integral_constant<int, 2>());
+            case 4: return f(dt, std::integral_constant<int, 4>());
+            default: return f(dt, std::integral_constant<int, 8>());
+        }
+    };
+    switch (dtype) {
+        case CC1D_F32: return with(std::integral_constant<int, CC1D_F32>());
+        case CC1D_F16: return with(std::integral_constant<int, CC1D_F16>());
+        default: return with(std::integral_constant<int, CC1D_BF16>());
+    }
+}
 
 }  // namespace cc1d

@@ -1,0 +1,304 @@
+// The gated delta rule by chunks, first kernel: everything of a chunk that needs no state (cc1d_delta_chunk.hpp).
+// One workgroup a chunk and value head: K K^T and Q K^T on the matrix cores, T = (I + A)^-1, and the operands of the
+// later kernels in the order in which these load them.
+//
+// T: the four 16 x 16 blocks on the diagonal by substitution, one wavefront each with a column a lane; the blocks below
+// from T_ij = -T_ii sum_{j <= k < i} A_ik T_kj by fp32 matrix instructions, the distance to the diagonal growing.
+// Substitution and not the series of powers of A: those of keys that resemble each other grow to 1e8 before they vanish.
+#include "cc1d_delta_chunk.hpp"
+#include "cc1d_delta_host.hpp"
+
+namespace cc1d {
+namespace {
+
+constexpr int kPitch = 68;               // floats of a row of a 64 x 64 matrix in LDS
+
+template <int DT, int KS>
+struct PrepLds {
+    uint8_t frags[4 * KS * Terms<DT>::n * kFrag];        // K, later Q
+    float a[kChunk][kPitch], t[kChunk][kPitch];
+    float scratch[4][16][17];
+    float gate[kScalars][kChunk];
+    double sums[kChunk];
+    float norms[2][kChunk];
+};
+
+// 8 elements of a row from column c on, zeros behind `cols`.
+template <int DT>
+__device__ __forceinline__ void load_row8(const typename Elem<DT>::type *row, int c, int cols, bool vec, float (&f)[8]) {
+    if (vec && c + 8 <= cols) {
+        if constexpr (DT == CC1D_F32) {
+            float lo[4], hi[4];
+            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c), lo);
+            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c + 4), hi);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[i + 4] = hi[i]; }
+        } else {
+            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c), f);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? Elem<DT>::to_float(row[c + i]) : 0.f;
+}
+
+// The 16 x 16 product of two blocks in LDS, added to acc.
+__device__ __forceinline__ f32x4 block_product(const float *x, int px, const float *y, int py, f32x4 acc, int m, int g) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[m * px + 4 * s + g], y[(4 * s + g) * py + m], acc, 0, 0, 0);
+    return acc;
+}
+
+template <int DT, int KS>
+__global__ void __launch_bounds__(kBlock)
+delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w, const int vec) {
+    using T = typename Elem<DT>::type;
+    constexpr int NT = Terms<DT>::n, PT = Terms<DT>::p;
+    extern __shared__ uint4 raw[];
+    PrepLds<DT, KS> &lds = *reinterpret_cast<PrepLds<DT, KS> *>(raw);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const int slot = (int)(blockIdx.x / (uint32_t)p.v_heads), h = (int)(blockIdx.x % (uint32_t)p.v_heads);
+    const int group = p.v_heads / p.heads, hk = h / group;
+    const bool first = h % group == 0;                   // this workgroup writes what the heads of the group share
+    const ChunkAt at = chunk_at(p, w, slot);
+    if (at.count <= 0) return;
+    const int64_t sh = (int64_t)slot * p.heads + hk, sv = (int64_t)slot * p.v_heads + h;
+
+    // Rows of K and Q as left operands; their lengths.
+    const int token = row_of(wave, m);
+    const bool there = token < at.count;
+    const T *kp = static_cast<const T *>(p.k) + at.b * p.k_stride_b + (at.lo + (there ? token : 0)) * p.k_stride_l + hk * p.k_stride_h;
+    const T *qp = static_cast<const T *>(p.q) + at.b * p.q_stride_b + (at.lo + (there ? token : 0)) * p.q_stride_l + hk * p.q_stride_h;
+    bf16x8 kf[KS][NT], qf[KS][NT];
+    float kk = 0.f, qq = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        float x[8];
+        const int cols = there ? p.dim_k : 0;
+        load_row8<DT>(kp, 32 * s + 8 * g, cols, vec, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kk += x[i] * x[i];
+        split8<NT>(x, kf[s]);
+        load_row8<DT>(qp, 32 * s + 8 * g, cols, vec, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qq += x[i] * x[i];
+        split8<NT>(x, qf[s]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
+    }
+    if (first) {
+        uint8_t *kd = w.kf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag, *qd = w.qf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                *reinterpret_cast<u32x4 *>(kd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
+                *reinterpret_cast<u32x4 *>(qd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
+            }
+    }
+    kk += __shfl_xor(kk, 16); kk += __shfl_xor(kk, 32);
+    qq += __shfl_xor(qq, 16); qq += __shfl_xor(qq, 32);
+    if (g == 0) {
+        lds.norms[0][token] = p.qk_l2norm ? rsqrtf(kk + kNormEps) : 1.f;
+        lds.norms[1][token] = p.qk_l2norm ? rsqrtf(qq + kNormEps) : 1.f;
+    }
+    __syncthreads();
+
+    // Gates.  Sums in 64 bits, kept as two floats: differences of large sums lose nothing.
+    if (wave == 0) {
+        const bool real = lane < at.count;
+        const int64_t tok = at.lo + (real ? lane : 0);
+        double sum = real ? (double)bounded_gate(load_as_float(p.g, at.b * p.g_stride_b + tok * p.g_stride_l + h * p.g_stride_h, p.g_dtype)) : 0.0;
+        const float beta = real ? load_as_float(p.beta, at.b * p.beta_stride_b + tok * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype) : 0.f;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double o = __shfl_up(sum, d);
+            if (lane >= d) sum += o;
+        }
+        const double last = __shfl(sum, 63);
+        const float hi = (float)sum, gam = expf((float)sum), dec = expf((float)(last - sum));
+        const float rk = lds.norms[0][lane], rq = lds.norms[1][lane];
+        lds.gate[kSeenBeta][lane] = beta * gam * rk;
+        lds.gate[kBeta][lane] = beta;
+        lds.gate[kReadGate][lane] = p.scale * gam * rq;
+        lds.gate[kCarry][lane] = dec * rk;
+        lds.gate[kKeyNorm][lane] = rk;
+        lds.gate[kQueryNorm][lane] = rq;
+        lds.gate[kGate][lane] = gam;
+        lds.gate[kToEnd][lane] = dec;
+        lds.gate[kSumHi][lane] = hi;
+        lds.gate[kSumLo][lane] = (float)(sum - (double)hi);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kScalars * kChunk; i += kBlock) w.scalars[sv * kScalars * kChunk + i] = (&lds.gate[0][0])[i];
+
+    // K K^T and Q K^T: this wavefront's 16 rows; columns behind the rows' last are nothing.
+    f32x4 read[4];                                       // P waits in registers until A is used up
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, r = {0.f, 0.f, 0.f, 0.f};
+        if ((ct >> 1) <= (wave >> 1)) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                bf16x8 b[NT];
+                load_frag<NT>(lds.frags + (ct * KS + s) * NT * kFrag, lane, b);
+                a = product<2>(kf[s], b, a);
+                r = product<2>(qf[s], b, r);
+            }
+        }
+        const int j = row_of(ct, m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = row_of(wave, 4 * g + e);
+            float decay = 0.f;
+            if (i >= j) decay = expf((lds.gate[kSumHi][i] - lds.gate[kSumHi][j]) + (lds.gate[kSumLo][i] - lds.gate[kSumLo][j])) * lds.gate[kKeyNorm][j];
+            lds.a[i][j] = i > j ? a[e] * decay * (lds.gate[kBeta][i] * lds.gate[kKeyNorm][i]) : 0.f;
+            read[ct][e] = i >= j ? r[e] * decay * (p.scale * lds.gate[kQueryNorm][i]) : 0.f;
+        }
+    }
+    __syncthreads();
+
+    // T.  Diagonal blocks: lane = column.
+    {
+        const int o = 16 * wave;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float v = i == m ? 1.f : 0.f;
+#pragma unroll
+            for (int k = 0; k < i; ++k) v -= lds.a[o + i][o + k] * x[k];
+            x[i] = v;
+        }
+        if (g == 0)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lds.t[o + i][o + m] = x[i];
+        for (int i = threadIdx.x; i < kChunk * kChunk; i += kBlock) {   // above the diagonal
+            const int r = i >> 6, c = i & 63;
+            if ((c >> 4) > (r >> 4)) lds.t[r][c] = 0.f;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+        const int i = wave + d, j = wave;                // block (i, j)
+        if (i < 4) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            for (int k = j; k < i; ++k) acc = block_product(&lds.a[16 * i][16 * k], kPitch, &lds.t[16 * k][16 * j], kPitch, acc, m, g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lds.scratch[wave][4 * g + e][m] = -acc[e];
+            wave_lds_fence();
+            acc = {0.f, 0.f, 0.f, 0.f};
+            acc = block_product(&lds.t[16 * i][16 * i], kPitch, &lds.scratch[wave][0][0], 17, acc, m, g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lds.t[16 * i + 4 * g + e][16 * j + m] = acc[e];
+        }
+        __syncthreads();
+    }
+
+    // T and its transpose as left operands.
+    for (int s = 0; s <= (wave >> 1); ++s) {
+        float x[8];
+        bf16x8 f[3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = lds.t[row_of(wave, m)][32 * s + 8 * g + e];
+        split8<3>(x, f);
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+            *reinterpret_cast<u32x4 *>(w.tf + sv * w.tbytes() + (lower_frag(wave, s) * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
+    }
+    if (w.backward)
+        for (int s = wave >> 1; s < 2; ++s) {
+            float x[8];
+            bf16x8 f[3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = lds.t[32 * s + 8 * g + e][row_of(wave, m)];
+            split8<3>(x, f);
+#pragma unroll
+            for (int n = 0; n < 3; ++n)
+                *reinterpret_cast<u32x4 *>(w.ttf + sv * w.tbytes() + (upper_frag(wave, s) * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
+        }
+    // P goes where A was.
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lds.a[row_of(wave, 4 * g + e)][row_of(ct, m)] = read[ct][e];
+    __syncthreads();
+    for (int s = 0; s <= (wave >> 1); ++s) {
+        float x[8];
+        bf16x8 f[PT];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = lds.a[row_of(wave, m)][32 * s + 8 * g + e];
+        split8<PT>(x, f);
+#pragma unroll
+        for (int n = 0; n < PT; ++n)
+            *reinterpret_cast<u32x4 *>(w.pf + sv * w.pbytes() + (lower_frag(wave, s) * PT + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
+    }
+    if (w.backward)
+        for (int s = wave >> 1; s < 2; ++s) {
+            float x[8];
+            bf16x8 f[PT];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = lds.a[32 * s + 8 * g + e][row_of(wave, m)];
+            split8<PT>(x, f);
+#pragma unroll
+            for (int n = 0; n < PT; ++n)
+                *reinterpret_cast<u32x4 *>(w.ptf + sv * w.pbytes() + (upper_frag(wave, s) * PT + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
+        }
+    if (!first) return;
+    // K^T, then Q^T, gathered from the operands in LDS: token 32 s + 8 g + e is row m' of tile ct, dim_k index k is
+    // element k & 7 of lane group (k >> 3) & 3 of step k >> 5.
+    auto transposed = [&](uint8_t *dst) {
+#pragma unroll
+        for (int i = 0; i < (2 * KS + 3) / 4; ++i) {
+            const int t = wave + 4 * i;
+            if (t >= 2 * KS) break;
+            const int k = row_of(t, m);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint16_t x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int ct = 2 * s + (e >> 2), mm = 4 * g + (e & 3);
+                        x[e] = *reinterpret_cast<const uint16_t *>(lds.frags + ((ct * KS + (k >> 5)) * NT + n) * kFrag + (((k >> 3) & 3) * 16 + mm) * 16 + (k & 7) * 2);
+                    }
+                    u32x4 f;
+                    f.x = x[0] | (uint32_t)x[1] << 16; f.y = x[2] | (uint32_t)x[3] << 16;
+                    f.z = x[4] | (uint32_t)x[5] << 16; f.w = x[6] | (uint32_t)x[7] << 16;
+                    *reinterpret_cast<u32x4 *>(dst + ((t * 2 + s) * NT + n) * kFrag + lane * 16) = f;
+                }
+        }
+    };
+    transposed(w.ktf + sh * w.kbytes());
+    if (!w.backward) return;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
+    __syncthreads();
+    transposed(w.qtf + sh * w.kbytes());
+}
+
+template <int DT, int KS>
+int launch(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream) {
+    auto rows = [&](const void *x, int64_t b, int64_t l, int64_t h) {
+        const int v = vec_elems(p.x_dtype);
+        return aligned16(x) && b % v == 0 && l % v == 0 && h % v == 0;
+    };
+    const int vec = rows(p.q, p.q_stride_b, p.q_stride_l, p.q_stride_h) && rows(p.k, p.k_stride_b, p.k_stride_l, p.k_stride_h);
+    CC1D_LAUNCH((delta_prep_kernel<DT, KS>), dim3((uint32_t)((int64_t)w.slots * p.v_heads)), dim3(kBlock), sizeof(PrepLds<DT, KS>), stream, p, w, vec);
+    return launch_status();
+}
+
+}  // namespace
+
+int launch_delta_prep(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream) {
+    return by_type_and_steps(p.x_dtype, w.ks, [&](auto dt, auto ks) { return launch<decltype(dt)::value, decltype(ks)::value>(p, w, stream); });
+}
+
+}  // namespace cc1d
