@@ -40,6 +40,7 @@ KERNEL_SOURCES = [
     "cc1d_delta_step.hip",
     "cc1d_delta_prep.hip",
     "cc1d_delta_scan.hip",
+    "cc1d_delta_bwd.hip",
     "cc1d_norm.hip",
 ]
 KERNEL_HEADERS = ["cc1d_device.hpp", "cc1d_internal.hpp", "cc1d_bwd_channellast_kernel.hpp"]

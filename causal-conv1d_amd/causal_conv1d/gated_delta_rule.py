@@ -22,7 +22,38 @@ import torch
 import causal_conv1d_cuda as _ext  # noqa: F401  (loading it registers the ops)
 
 _fwd = torch.ops.DaoAILab._gated_delta_rule_fwd_cpp
+_bwd = torch.ops.DaoAILab._gated_delta_rule_bwd_cpp
 _update = torch.ops.DaoAILab._gated_delta_rule_update_cpp
+
+
+def _new_states(q, v, cu_seqlens):
+    n = q.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    return torch.empty(n, v.shape[2], q.shape[-1], v.shape[-1], dtype=torch.float32, device=v.device)
+
+
+class GatedDeltaRuleFn(torch.autograd.Function):
+    """Saves only the inputs: the states in front of the chunks are computed again in backward."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, scale, initial_states, return_final_states, cu_seqlens, qk_l2norm):
+        final = _new_states(q, v, cu_seqlens) if return_final_states else None
+        out = _fwd(q, k, v, g, beta, initial_states, cu_seqlens, final, scale, qk_l2norm)
+        ctx.save_for_backward(q, k, v, g, beta, initial_states, cu_seqlens)
+        ctx.scale, ctx.qk_l2norm = scale, qk_l2norm
+        ctx.set_materialize_grads(False)
+        return (out, final) if return_final_states else out
+
+    @staticmethod
+    def backward(ctx, dout, dfinal=None):
+        q, k, v, g, beta, initial_states, cu_seqlens = ctx.saved_tensors
+        if dout is None and dfinal is None:
+            return (None,) * 10
+        if dout is None:                                 # only the states were used
+            dout = torch.zeros_like(v)
+        wants_states = initial_states is not None and ctx.needs_input_grad[6]
+        dq, dk, dv, dg, dbeta, dinitial = _bwd(q, k, v, g, beta, initial_states, cu_seqlens, dout, dfinal, ctx.scale,
+                                               ctx.qk_l2norm, wants_states)
+        return dq, dk, dv, dg, dbeta, None, dinitial if wants_states else None, None, None, None
 
 
 def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_states=None, return_final_states=False,
@@ -31,18 +62,21 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_states=None, retur
 
     scale: 1 / sqrt(dim_k) if None.  qk_l2norm: q and k are divided by their length, sqrt(sum of squares + 1e-6).
     initial_states (sequences, v_heads, dim_k, dim_v) float32, zeros if None; final_states like it, written to
-    final_states_out if given (which may be initial_states itself).
+    final_states_out if given (which may be initial_states itself; without gradients only).
     cu_seqlens (sequences + 1,) int32 or int64, ascending from 0 to seqlen, with a batch of 1: sequence n is tokens
     cu_seqlens[n] .. cu_seqlens[n+1]-1; a sequence may be empty."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if cu_seqlens is not None:
         cu_seqlens = cu_seqlens.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states)):
+        if final_states_out is not None:
+            raise RuntimeError("final_states_out cannot be given where gradients are recorded")
+        return GatedDeltaRuleFn.apply(q, k, v, g, beta, float(scale), initial_states, return_final_states, cu_seqlens, qk_l2norm)
     if not return_final_states:
         final_states_out = None
     elif final_states_out is None:
-        n = q.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
-        final_states_out = torch.empty(n, v.shape[2], q.shape[-1], v.shape[-1], dtype=torch.float32, device=v.device)
+        final_states_out = _new_states(q, v, cu_seqlens)
     out = _fwd(q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, float(scale), qk_l2norm)
     return (out, final_states_out) if return_final_states else out
 

@@ -57,14 +57,16 @@ size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWo
         used += (bytes + 255) / 256 * 256;
         return at;
     };
-    w.kf = take(keys * w.kbytes()); w.qf = take(keys * w.kbytes()); w.ktf = take(keys * w.kbytes());
-    w.tf = take(values * w.tbytes()); w.pf = take(values * w.pbytes());
+    w.kf = take(keys * w.kbytes()); w.ktf = take(keys * w.kbytes());
+    w.tf = take(values * w.tbytes());
     w.scalars = reinterpret_cast<float *>(take(values * kScalars * kChunk * sizeof(float)));
     if (backward) {
         const size_t state = values * p.dim_k * p.dim_v * sizeof(float), rows = values * kChunk * p.dim_v * sizeof(float);
-        w.qtf = take(keys * w.kbytes()); w.ttf = take(values * w.tbytes()); w.ptf = take(values * w.pbytes());
+        w.qtf = take(keys * w.kbytes()); w.ttf = take(values * w.tbytes()); w.ptf = take(values * w.tbytes());
         w.s0 = reinterpret_cast<float *>(take(state)); w.ds1 = reinterpret_cast<float *>(take(state));
         w.u = reinterpret_cast<float *>(take(rows)); w.dx = reinterpret_cast<float *>(take(rows));
+    } else {
+        w.qf = take(keys * w.kbytes()); w.pf = take(values * w.pbytes());
     }
     return used;
 }
@@ -108,6 +110,46 @@ int cc1d_delta_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace
     lay_out(*p, false, static_cast<uint8_t *>(workspace), w);
     const int done = launch_delta_prep(*p, w, hs);
     return done != CC1D_OK ? done : launch_delta_scan(*p, w, false, hs);
+}
+
+int cc1d_validate_delta_bwd(const cc1d_delta_bwd_params *p) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const int st = check_delta(p->fwd);
+    if (st != CC1D_OK) return st;
+    const cc1d_delta_params &f = p->fwd;
+    if (f.batch > 0 && f.seqlen > 0 && f.v_heads > 0 &&
+        (p->dout == nullptr || p->dq == nullptr || p->dk == nullptr || p->dv == nullptr || p->dg == nullptr || p->dbeta == nullptr)) return CC1D_ERR_NULL_POINTER;
+    if (!on_elements(p->dout, f.x_dtype) || !on_elements(p->dq, f.x_dtype) || !on_elements(p->dk, f.x_dtype) || !on_elements(p->dv, f.x_dtype) ||
+        !on_elements(p->dg, f.g_dtype) || !on_elements(p->dbeta, f.beta_dtype) || !on_elements(p->dfinal_states, CC1D_F32) ||
+        !on_elements(p->dinitial_states, CC1D_F32)) return CC1D_ERR_ROW_LAYOUT;
+    return CC1D_OK;
+}
+
+int cc1d_delta_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *bytes) {
+    if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
+    *bytes = 0;
+    const int st = cc1d_validate_delta_bwd(p);
+    if (st != CC1D_OK || p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return st;
+    ChunkWork w;
+    *bytes = lay_out(p->fwd, true, nullptr, w);
+    return fits(p->fwd, w) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+}
+
+int cc1d_delta_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
+    size_t need = 0;
+    int st = cc1d_delta_bwd_workspace_bytes(p, &need);
+    if (st != CC1D_OK) return st;
+    if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
+    if (p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return CC1D_OK;
+    const hipStream_t hs = static_cast<hipStream_t>(stream);
+    ChunkWork w;
+    lay_out(p->fwd, true, static_cast<uint8_t *>(workspace), w);
+    if (w.slots > 0) {
+        st = launch_delta_prep(p->fwd, w, hs);
+        if (st == CC1D_OK) st = launch_delta_scan(p->fwd, w, true, hs);
+        if (st != CC1D_OK) return st;
+    }
+    return launch_delta_bwd(*p, w, hs);
 }
 
 int cc1d_validate_delta_step(const cc1d_delta_step_params *p) {

@@ -16,6 +16,8 @@ int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int 
 // By chunks: what needs no state; then the states and outputs (`states`: only the states in front of the chunks and U).
 int launch_delta_prep(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream);
 int launch_delta_scan(const cc1d_delta_params &p, const ChunkWork &w, bool states, hipStream_t stream);
+// Backward behind both (of a ChunkWork laid out for it): the gradients.
+int launch_delta_bwd(const cc1d_delta_bwd_params &p, const ChunkWork &w, hipStream_t stream);
 
 // 32-column steps of dim_k that have kernels.
 inline int key_steps(int dim_k) { return dim_k <= 32 ? 1 : dim_k <= 64 ? 2 : dim_k <= 128 ? 4 : 8; }

@@ -95,7 +95,7 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w, const int vec) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 *reinterpret_cast<u32x4 *>(kd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
-                *reinterpret_cast<u32x4 *>(qd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
+                if (!w.backward) *reinterpret_cast<u32x4 *>(qd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
             }
     }
     kk += __shfl_xor(kk, 16); kk += __shfl_xor(kk, 32);
@@ -225,7 +225,8 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w, const int vec) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) lds.a[row_of(wave, 4 * g + e)][row_of(ct, m)] = read[ct][e];
     __syncthreads();
-    for (int s = 0; s <= (wave >> 1); ++s) {
+    if (!w.backward)
+        for (int s = 0; s <= (wave >> 1); ++s) {
         float x[8];
         bf16x8 f[PT];
 #pragma unroll
@@ -238,13 +239,13 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w, const int vec) {
     if (w.backward)
         for (int s = wave >> 1; s < 2; ++s) {
             float x[8];
-            bf16x8 f[PT];
+            bf16x8 f[3];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = lds.a[32 * s + 8 * g + e][row_of(wave, m)];
-            split8<PT>(x, f);
+            split8<3>(x, f);
 #pragma unroll
-            for (int n = 0; n < PT; ++n)
-                *reinterpret_cast<u32x4 *>(w.ptf + sv * w.pbytes() + (upper_frag(wave, s) * PT + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
+            for (int n = 0; n < 3; ++n)
+                *reinterpret_cast<u32x4 *>(w.ptf + sv * w.tbytes() + (upper_frag(wave, s) * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
         }
     if (!first) return;
     // K^T, then Q^T, gathered from the operands in LDS: token 32 s + 8 g + e is row m' of tile ct, dim_k index k is

@@ -123,6 +123,41 @@ at::Tensor delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor 
     return out;
 }
 
+// dq, dk, dv, dg, dbeta in their inputs' types, and dinitial_states (empty if not wanted).
+using Gradients6 = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+Gradients6 delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const at::Tensor &dout_, const OptTensor &dfinal_states,
+                     double scale, bool qk_l2norm, bool want_dinitial) {
+    const DeltaInputs d = delta_inputs(q, k, v, g, beta);
+    OptTensor init = initial_states, dfinal = dfinal_states;
+    if (init.has_value()) init = rows_of(*init);
+    c10::DeviceGuard guard(q.device());
+    cc1d_delta_bwd_params p = {};
+    p.fwd = delta_params(d, init, cu_seqlens, scale, qk_l2norm);
+    check_gpu(dout_, q, "dout");
+    TORCH_CHECK(dout_.sizes() == v.sizes() && dout_.scalar_type() == v.scalar_type(), "dout must have the shape and dtype of v");
+    const at::Tensor dout = rows_of(dout_);
+    p.dout = dout.data_ptr(); SET_STRIDES(p, dout, dout);
+    if (dfinal.has_value()) {
+        dfinal = rows_of(*dfinal);
+        check_states(*dfinal, d, p.fwd.sequences, "dfinal_states");
+        p.dfinal_states = dfinal->data_ptr<float>(); SET_STATE(p, dfinal, (*dfinal));
+    }
+    at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+    at::Tensor dg = at::empty(g.sizes(), g.options()), dbeta = at::empty(beta.sizes(), beta.options());
+    p.dq = dq.data_ptr(); SET_STRIDES(p, dq, dq);
+    p.dk = dk.data_ptr(); SET_STRIDES(p, dk, dk);
+    p.dv = dv.data_ptr(); SET_STRIDES(p, dv, dv);
+    p.dg = dg.data_ptr(); p.dbeta = dbeta.data_ptr();
+    at::Tensor dinit = want_dinitial ? at::empty({p.fwd.sequences, d.v_heads, d.dim_k, d.dim_v}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
+    if (want_dinitial) { p.dinitial_states = dinit.data_ptr<float>(); SET_STATE(p, dinit, dinit); }
+    size_t bytes = 0;
+    check_status(cc1d_delta_bwd_workspace_bytes(&p, &bytes), "gated_delta_rule backward");
+    const at::Tensor ws = workspace_of(bytes, q);
+    check_status(cc1d_delta_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "gated_delta_rule backward");
+    return {dq, dk, dv, dg, dbeta, dinit};
+}
+
 at::Tensor delta_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
                         at::Tensor &state, const OptTensor &state_indices, double scale, bool qk_l2norm) {
     const bool flat = q.dim() == 3;                      // (batch, heads, dim): one token, no seqlen axis
@@ -153,6 +188,14 @@ at::Tensor delta_update(const at::Tensor &q, const at::Tensor &k, const at::Tens
 at::Tensor delta_fwd_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const at::Tensor &,
                           const OptTensor &, const OptTensor &, const OptTensor &, double, bool) {
     return at::empty_symint(v.sym_sizes(), v.options());
+}
+Gradients6 delta_bwd_meta(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                          const OptTensor &, const OptTensor &cu, const at::Tensor &, const OptTensor &, double, bool, bool want_dinitial) {
+    auto like = [](const at::Tensor &t) { return at::empty_symint(t.sym_sizes(), t.options()); };
+    const c10::SymInt n = cu.has_value() ? cu->sym_size(0) - 1 : q.sym_size(0);
+    const auto f32 = q.options().dtype(at::kFloat);
+    return {like(q), like(k), like(v), like(g), like(beta),
+            want_dinitial ? at::empty_symint({n, v.sym_size(2), q.sym_size(3), v.sym_size(3)}, f32) : at::empty({0}, f32)};
 }
 at::Tensor delta_update_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const at::Tensor &,
                              at::Tensor &, const OptTensor &, double, bool) {
@@ -302,6 +345,9 @@ at::Tensor dequantize_meta(const at::Tensor &y8, const at::Tensor &, at::ScalarT
 TORCH_LIBRARY_FRAGMENT(DaoAILab, m) {
     m.def("_gated_delta_rule_fwd_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? initial_states, "
           "Tensor? cu_seqlens, Tensor(a!)? final_states_out, float scale, bool qk_l2norm) -> Tensor", {at::Tag::pt2_compliant_tag});
+    m.def("_gated_delta_rule_bwd_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? initial_states, Tensor? cu_seqlens, "
+          "Tensor dout, Tensor? dfinal_states, float scale, bool qk_l2norm, bool want_dinitial) "
+          "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
     m.def("_gated_delta_rule_update_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor(a!) state, "
           "Tensor? state_indices, float scale, bool qk_l2norm) -> Tensor", {at::Tag::pt2_compliant_tag});
     m.def("_rms_norm_fwd_cpp(Tensor x, Tensor weight, Tensor? residual, float eps) -> (Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
@@ -312,6 +358,7 @@ TORCH_LIBRARY_FRAGMENT(DaoAILab, m) {
 
 TORCH_LIBRARY_IMPL(DaoAILab, CompositeExplicitAutograd, m) {
     m.impl("_gated_delta_rule_fwd_cpp", &delta_fwd);
+    m.impl("_gated_delta_rule_bwd_cpp", &delta_bwd);
     m.impl("_gated_delta_rule_update_cpp", &delta_update);
     m.impl("_rms_norm_fwd_cpp", &norm_fwd);
     m.impl("_rms_norm_bwd_cpp", &norm_bwd);
@@ -321,6 +368,7 @@ TORCH_LIBRARY_IMPL(DaoAILab, CompositeExplicitAutograd, m) {
 
 TORCH_LIBRARY_IMPL(DaoAILab, Meta, m) {
     m.impl("_gated_delta_rule_fwd_cpp", &delta_fwd_meta);
+    m.impl("_gated_delta_rule_bwd_cpp", &delta_bwd_meta);
     m.impl("_gated_delta_rule_update_cpp", &delta_update_meta);
     m.impl("_rms_norm_fwd_cpp", &norm_fwd_meta);
     m.impl("_rms_norm_bwd_cpp", &norm_bwd_meta);
