@@ -130,10 +130,96 @@ __device__ __forceinline__ f32x4 product(const bf16x8 (&a)[NA], const bf16x8 (&b
     return acc;
 }
 
+// 8 elements of a row from column c on, `cols` columns long (none: a row that is not there), asked for without a branch and looked
+// at later: a load behind a condition waits for itself, and with it for everything asked for before it.  VEC: cols is a multiple of 8
+// and the row 16-byte aligned.
+template <int DT, bool VEC>
+struct Row8 {
+    static constexpr int N = DT == CC1D_F32 ? 2 : 1;
+    u32x4 r[N];
+    __device__ __forceinline__ void ask(const typename Elem<DT>::type *row, int c, int cols) {
+        if constexpr (VEC) {
+            const u32x4 *at = reinterpret_cast<const u32x4 *>(row + (c < cols ? c : 0));
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = at[i];
+        } else {
+            uint32_t x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = c + i < cols ? c + i : 0;
+                if constexpr (DT == CC1D_F32) x[i] = reinterpret_cast<const uint32_t *>(row)[j];
+                else x[i] = reinterpret_cast<const uint16_t *>(row)[j];
+            }
+            if constexpr (DT == CC1D_F32) {
+                r[0].x = x[0]; r[0].y = x[1]; r[0].z = x[2]; r[0].w = x[3];
+                r[N - 1].x = x[4]; r[N - 1].y = x[5]; r[N - 1].z = x[6]; r[N - 1].w = x[7];
+            } else {
+                r[0].x = x[0] | x[1] << 16; r[0].y = x[2] | x[3] << 16; r[0].z = x[4] | x[5] << 16; r[0].w = x[6] | x[7] << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void get(int c, int cols, float (&f)[8]) const {
+        if constexpr (DT == CC1D_F32) {
+            float lo[4], hi[4];
+            Elem<DT>::unpack(r[0], lo);
+            Elem<DT>::unpack(r[N - 1], hi);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[i + 4] = hi[i]; }
+        } else {
+            Elem<DT>::unpack(r[0], f);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (VEC ? c : c + i) < cols ? f[i] : 0.f;
+    }
+};
+
 template <int N>
 __device__ __forceinline__ void load_frag(const uint8_t *base, int lane, bf16x8 (&f)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n) f[n] = bitcast<bf16x8>(*reinterpret_cast<const u32x4 *>(base + n * kFrag + lane * 16));
+}
+
+// The same for R left operands against one right one; products of different rows follow each other, so none waits for its own sum.
+template <int MOST, int R, int NA, int NB>
+__device__ __forceinline__ void products(const bf16x8 (&a)[R][NA], const bf16x8 (&b)[NB], f32x4 *acc) {
+#pragma unroll
+    for (int sum = MOST; sum >= 0; --sum)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = sum - i;
+            if (j < 0 || j >= NB) continue;
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[r][i], b[j], acc[r], 0, 0, 0);
+        }
+}
+// The right operand that two result tiles are.
+template <int N>
+__device__ __forceinline__ void as_operand(const f32x4 &a, const f32x4 &b, bf16x8 (&t)[N]) {
+    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    split8<N>(x, t);
+}
+
+// Two accumulators, the largest products in one and the rest in the other: two chains of instructions that do not wait for each other.
+template <int MOST, int NA, int NB>
+__device__ __forceinline__ void product2(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 &large, f32x4 &rest) {
+#pragma unroll
+    for (int sum = MOST; sum >= 0; --sum)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = sum - i;
+            if (j < 0 || j >= NB) continue;
+            if (sum == 0) large = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], large, 0, 0, 0);
+            else rest = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], rest, 0, 0, 0);
+        }
+}
+
+// The number that element i of an operand's lane stands for.
+template <int N>
+__device__ __forceinline__ float term_sum(const bf16x8 (&f)[N], int i) {
+    float v = (float)f[N - 1][i];
+#pragma unroll
+    for (int n = N - 2; n >= 0; --n) v += (float)f[n][i];
+    return v;
 }
 
 // A barrier that orders LDS alone: loads and stores of global memory stay in flight.

@@ -23,25 +23,6 @@ struct PrepLds {
     float norms[2][kChunk];
 };
 
-// 8 elements of a row from column c on, zeros behind `cols`.
-template <int DT>
-__device__ __forceinline__ void load_row8(const typename Elem<DT>::type *row, int c, int cols, bool vec, float (&f)[8]) {
-    if (vec && c + 8 <= cols) {
-        if constexpr (DT == CC1D_F32) {
-            float lo[4], hi[4];
-            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c), lo);
-            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c + 4), hi);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[i + 4] = hi[i]; }
-        } else {
-            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c), f);
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? Elem<DT>::to_float(row[c + i]) : 0.f;
-}
-
 // The 16 x 16 product of two blocks in LDS, added to acc.
 __device__ __forceinline__ f32x4 block_product(const float *x, int px, const float *y, int py, f32x4 acc, int m, int g) {
 #pragma unroll
@@ -50,9 +31,9 @@ __device__ __forceinline__ f32x4 block_product(const float *x, int px, const flo
     return acc;
 }
 
-template <int DT, int KS>
+template <int DT, int KS, bool VEC>
 __global__ void __launch_bounds__(kBlock)
-delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w, const int vec) {
+delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n, PT = Terms<DT>::p;
     extern __shared__ uint4 raw[];
@@ -72,21 +53,29 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w, const int vec) {
     const T *qp = static_cast<const T *>(p.q) + at.b * p.q_stride_b + (at.lo + (there ? token : 0)) * p.q_stride_l + hk * p.q_stride_h;
     bf16x8 kf[KS][NT], qf[KS][NT];
     float kk = 0.f, qq = 0.f;
+    const int cols = there ? p.dim_k : 0;
+    {
+        Row8<DT, VEC> kr[KS], qr[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        float x[8];
-        const int cols = there ? p.dim_k : 0;
-        load_row8<DT>(kp, 32 * s + 8 * g, cols, vec, x);
+        for (int s = 0; s < KS; ++s) {
+            kr[s].ask(kp, 32 * s + 8 * g, cols);
+            qr[s].ask(qp, 32 * s + 8 * g, cols);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) kk += x[i] * x[i];
-        split8<NT>(x, kf[s]);
-        load_row8<DT>(qp, 32 * s + 8 * g, cols, vec, x);
+        for (int s = 0; s < KS; ++s) {
+            float x[8];
+            kr[s].get(32 * s + 8 * g, cols, x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) qq += x[i] * x[i];
-        split8<NT>(x, qf[s]);
+            for (int i = 0; i < 8; ++i) kk += x[i] * x[i];
+            split8<NT>(x, kf[s]);
+            qr[s].get(32 * s + 8 * g, cols, x);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
+            for (int i = 0; i < 8; ++i) qq += x[i] * x[i];
+            split8<NT>(x, qf[s]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
+        }
     }
     if (first) {
         uint8_t *kd = w.kf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag, *qd = w.qf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag;
@@ -285,21 +274,20 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w, const int vec) {
     transposed(w.qtf + sh * w.kbytes());
 }
 
-template <int DT, int KS>
+template <int DT, int KS, bool VEC>
 int launch(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream) {
-    auto rows = [&](const void *x, int64_t b, int64_t l, int64_t h) {
-        const int v = vec_elems(p.x_dtype);
-        return aligned16(x) && b % v == 0 && l % v == 0 && h % v == 0;
-    };
-    const int vec = rows(p.q, p.q_stride_b, p.q_stride_l, p.q_stride_h) && rows(p.k, p.k_stride_b, p.k_stride_l, p.k_stride_h);
-    CC1D_LAUNCH((delta_prep_kernel<DT, KS>), dim3((uint32_t)((int64_t)w.slots * p.v_heads)), dim3(kBlock), sizeof(PrepLds<DT, KS>), stream, p, w, vec);
+    CC1D_LAUNCH((delta_prep_kernel<DT, KS, VEC>), dim3((uint32_t)((int64_t)w.slots * p.v_heads)), dim3(kBlock), sizeof(PrepLds<DT, KS>), stream, p, w);
     return launch_status();
 }
 
 }  // namespace
 
 int launch_delta_prep(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream) {
-    return by_type_and_steps(p.x_dtype, w.ks, [&](auto dt, auto ks) { return launch<decltype(dt)::value, decltype(ks)::value>(p, w, stream); });
+    const bool vec = p.dim_k % 8 == 0 && whole_rows(p.x_dtype, p.q, p.q_stride_b, p.q_stride_l, p.q_stride_h) &&
+                     whole_rows(p.x_dtype, p.k, p.k_stride_b, p.k_stride_l, p.k_stride_h);
+    return by_type_and_steps(p.x_dtype, w.ks, [&](auto dt, auto ks) {
+        return vec ? launch<decltype(dt)::value, decltype(ks)::value, true>(p, w, stream) : launch<decltype(dt)::value, decltype(ks)::value, false>(p, w, stream);
+    });
 }
 
 }  // namespace cc1d
