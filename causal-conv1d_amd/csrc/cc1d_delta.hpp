@@ -11,6 +11,29 @@ namespace cc1d {
 constexpr int kChunk = 64;               // tokens of a chunk
 constexpr float kNormEps = 1e-6f;        // under the root of qk_l2norm
 
+// exp(x) as 2^(x log2 e), the product in two floats: off by 2 units in the last place at most, 6 instructions where
+// expf takes 25.  -inf and everything below -104 give 0.
+__device__ __forceinline__ float exp_of(float x) {
+    const float hi = x * 1.44269502f, lo = fmaf(x, 1.44269502f, -hi) + x * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return x < -104.f ? 0.f : fmaf(e, lo * 0.693147182f, e);
+}
+
+// Sums over the 16 lanes of a row of a result tile, and over all 64, by DPP and half swaps: no LDS, the same order every time.
+__device__ __forceinline__ float over_columns(float v) {
+    v += dpp_moved<0xB1>(v);                             // quad_perm: lane ^ 1
+    v += dpp_moved<0x4E>(v);                             // lane ^ 2
+    v += dpp_moved<0x124>(v);                            // row_ror:4
+    return v + dpp_moved<0x128>(v);                      // row_ror:8
+}
+__device__ __forceinline__ float over_rows(float v) {    // over lanes m, m + 16, m + 32, m + 48
+    const auto a = __builtin_amdgcn_permlane16_swap(bitcast<uint32_t>(v), bitcast<uint32_t>(v), false, false);
+    v = bitcast<float>((uint32_t)a[0]) + bitcast<float>((uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(bitcast<uint32_t>(v), bitcast<uint32_t>(v), false, false);
+    return bitcast<float>((uint32_t)b[0]) + bitcast<float>((uint32_t)b[1]);
+}
+__device__ __forceinline__ float over_wave(float v) { return over_rows(over_columns(v)); }
+
 __device__ __forceinline__ float load_as_float(const void *p, int64_t i, int dtype) {
     if (dtype == CC1D_F32) return static_cast<const float *>(p)[i];
     if (dtype == CC1D_F16) return (float)static_cast<const _Float16 *>(p)[i];

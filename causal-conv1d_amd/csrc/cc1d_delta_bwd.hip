@@ -29,31 +29,35 @@ struct BwdScanLds {
 };
 
 template <int DT, int KS>
-__global__ void __launch_bounds__(kBlock, 1)
+__global__ void __launch_bounds__(kBlock, 2)
 delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const uint32_t heads_total, const uint32_t col_tiles) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n;
-    constexpr int TW = (2 * KS + 3) / 4;
+    constexpr int TW = (2 * KS + 3) / 4;                 // 16-row tiles of dS a wavefront owns
     __shared__ BwdScanLds<DT, KS> lds;
     const cc1d_delta_params &p = bp.fwd;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t xcd = blockIdx.x & 7u, idx = blockIdx.x >> 3;
     const uint32_t nh = idx / col_tiles * 8u + xcd;
     if (nh >= heads_total) return;
-    const int col = (int)(idx % col_tiles) * 16 + m;
     const int h = (int)(nh % (uint32_t)p.v_heads), n = (int)(nh / (uint32_t)p.v_heads);
     const int hk = h / (p.v_heads / p.heads);
-    const bool has_col = col < p.dim_v;
     const TokenRange range = sequence_tokens(p, n);
     const int chunks = (int)((range.hi - range.lo + kChunk - 1) / kChunk);
-    const int slot0 = first_slot(p, w, n, range);
+    const int slot0 = first_slot(p, w, n, range), total = (int)(range.hi - range.lo);
+    const int col0 = (int)(idx % col_tiles) * 16 + m;
+    const bool has_col = col0 < p.dim_v;
+    const int col = has_col ? col0 : 0;                  // a column that is there
+    const uint32_t do_pitch = (uint32_t)(bp.dout_stride_l * (int64_t)sizeof(T)), dv_pitch = (uint32_t)(bp.dv_stride_l * (int64_t)sizeof(T));
+    const uint32_t at_col = (uint32_t)col * (uint32_t)sizeof(T);
 
-    T *dv = static_cast<T *>(bp.dv) + range.b * bp.dv_stride_b + h * bp.dv_stride_h + col;
+    T *dv = static_cast<T *>(bp.dv) + range.b * bp.dv_stride_b + h * bp.dv_stride_h;
     if (p.cu_seqlens != nullptr && has_col) {            // tokens in front of the first sequence and behind the last
         if (n == 0)
-            for (int64_t t = wave * 4 + g; t < range.lo; t += 16) dv[t * bp.dv_stride_l] = Elem<DT>::from_float(0.f);
+            for (int64_t t = wave * 4 + g; t < range.lo; t += 16) dv[t * bp.dv_stride_l + col] = Elem<DT>::from_float(0.f);
         if (n == p.sequences - 1)
-            for (int64_t t = range.hi + wave * 4 + g; t < p.seqlen; t += 16) dv[t * bp.dv_stride_l] = Elem<DT>::from_float(0.f);
+            for (int64_t t = range.hi + wave * 4 + g; t < p.seqlen; t += 16) dv[t * bp.dv_stride_l + col] = Elem<DT>::from_float(0.f);
     }
 
     f32x4 s[TW];
@@ -67,59 +71,61 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
         }
     }
 
+    // As in the scan of the forward: operands asked for again between the products that have used them, without conditions.
     bf16x8 kf[KS][NT], tf[2][3], pf[2][3], ktf[TW][2][NT], qtf[TW][2][NT];
     float4 seen, beta, read, carry;
     float last;
-    float d[4];
+    T d[4];
     const int64_t kb = w.kbytes(), tb = w.tbytes();
     const int from = wave >> 1;                          // first step of a row of T^T and P^T
-    auto ask_k = [&](int c) {
-        const int64_t at = ((int64_t)(slot0 + c) * p.heads + hk) * kb + (int64_t)wave * KS * NT * kFrag;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) load_frag<NT>(w.kf + at + i * NT * kFrag, lane, kf[i]);
-        const uint8_t *f = w.ptf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i >= from) load_frag<3>(f + upper_frag(wave, i) * 3 * kFrag, lane, pf[i]);
-    };
+    const int row = row_of(wave, 4 * g);
+    const T *dop = static_cast<const T *>(bp.dout) + range.b * bp.dout_stride_b + range.lo * bp.dout_stride_l + h * bp.dout_stride_h;
+    auto scalars_of = [&](int c) { return w.scalars + ((int64_t)(slot0 + c) * p.v_heads + h) * kScalars * kChunk; };
+    auto ask_k = [&](int c, int i) { load_frag<NT>(w.kf + ((int64_t)(slot0 + c) * p.heads + hk) * kb + (int64_t)(wave * KS + i) * NT * kFrag, lane, kf[i]); };
+    auto ask_p = [&](int c, int i) { load_frag<3>(w.ptf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + upper_frag(wave, i < from ? from : i) * 3 * kFrag, lane, pf[i]); };
+    auto ask_t = [&](int c, int i) { load_frag<3>(w.ttf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + upper_frag(wave, i < from ? from : i) * 3 * kFrag, lane, tf[i]); };
     auto ask_d = [&](int c) {
-        const float *sc = w.scalars + ((int64_t)(slot0 + c) * p.v_heads + h) * kScalars * kChunk;
-        const int row = row_of(wave, 4 * g);
-        seen = *reinterpret_cast<const float4 *>(sc + kSeenBeta * kChunk + row);
-        beta = *reinterpret_cast<const float4 *>(sc + kBeta * kChunk + row);
-        read = *reinterpret_cast<const float4 *>(sc + kReadGate * kChunk + row);
-        carry = *reinterpret_cast<const float4 *>(sc + kCarry * kChunk + row);
-        last = sc[kGate * kChunk + 63];
-        const int64_t lo = range.lo + (int64_t)c * kChunk;
+        read = *reinterpret_cast<const float4 *>(scalars_of(c) + kReadGate * kChunk + row);
+        const uint8_t *dc = reinterpret_cast<const uint8_t *>(dop + (int64_t)c * kChunk * bp.dout_stride_l);
+        const int end = total - c * kChunk - 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t tok = lo + row + e;
-            d[e] = has_col && tok < range.hi ? Elem<DT>::to_float(static_cast<const T *>(bp.dout)[range.b * bp.dout_stride_b + tok * bp.dout_stride_l + h * bp.dout_stride_h + col]) : 0.f;
+        for (int e = 0; e < 4; ++e) d[e] = *reinterpret_cast<const T *>(dc + ((uint32_t)(row + e < end ? row + e : end) * do_pitch + at_col));
+    };
+    auto ask_carry = [&](int c) { carry = *reinterpret_cast<const float4 *>(scalars_of(c) + kCarry * kChunk + row); };
+    auto ask_gates = [&](int c) {
+        seen = *reinterpret_cast<const float4 *>(scalars_of(c) + kSeenBeta * kChunk + row);
+        beta = *reinterpret_cast<const float4 *>(scalars_of(c) + kBeta * kChunk + row);
+    };
+    auto ask_last = [&](int c) { last = scalars_of(c)[kGate * kChunk + 63]; };
+    auto ask_kt = [&](int c, int i) {
+        const int64_t at = ((int64_t)(slot0 + c) * p.heads + hk) * kb + (int64_t)(wave * TW + i < 2 * KS ? wave * TW + i : 0) * 2 * NT * kFrag;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            load_frag<NT>(w.ktf + at + j * NT * kFrag, lane, ktf[i][j]);
+            load_frag<NT>(w.qtf + at + j * NT * kFrag, lane, qtf[i][j]);
         }
-    };
-    auto ask_t = [&](int c) {
-        const uint8_t *f = w.ttf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i >= from) load_frag<3>(f + upper_frag(wave, i) * 3 * kFrag, lane, tf[i]);
-    };
-    auto ask_kt = [&](int c) {
-        const int64_t at = ((int64_t)(slot0 + c) * p.heads + hk) * kb;
-#pragma unroll
-        for (int i = 0; i < TW; ++i)
-            if (wave * TW + i < 2 * KS)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    load_frag<NT>(w.ktf + at + ((wave * TW + i) * 2 + j) * NT * kFrag, lane, ktf[i][j]);
-                    load_frag<NT>(w.qtf + at + ((wave * TW + i) * 2 + j) * NT * kFrag, lane, qtf[i][j]);
-                }
     };
     auto put = [&](uint8_t *base, int terms, int tile, int n_, const u32x2 &x) {
         *reinterpret_cast<u32x2 *>(base + ((tile >> 1) * terms + n_) * kFrag + lane * 16 + (tile & 1) * 8) = x;
     };
-    if (chunks > 0) { ask_k(chunks - 1); ask_d(chunks - 1); ask_t(chunks - 1); ask_kt(chunks - 1); }
+    if (chunks > 0) {
+        const int c = chunks - 1;
+        ask_d(c);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) ask_k(c, i);
+        ask_carry(c);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ask_p(c, i);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ask_t(c, i);
+        ask_gates(c);
+        ask_last(c);
+#pragma unroll
+        for (int i = 0; i < TW; ++i) ask_kt(c, i);
+    }
 
     for (int c = chunks - 1; c >= 0; --c) {
+        const int next = c > 0 ? c - 1 : 0, left = total - c * kChunk;
         const int64_t sv = (int64_t)(slot0 + c) * p.v_heads + h;
 #pragma unroll
         for (int i = 0; i < TW; ++i) {
@@ -130,89 +136,118 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             split4<3>(x, f);
 #pragma unroll
             for (int j = 0; j < 3; ++j) put(lds.s, 3, t, j, f[j]);
-            if (has_col)
+            if (has_col) {
+                float *to = w.ds1 + sv * p.dim_k * p.dim_v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int k = row_of(t, 4 * g + e);
-                    if (k < p.dim_k) w.ds1[(sv * p.dim_k + k) * p.dim_v + col] = s[i][e];
+                    if (k < p.dim_k) to[(uint32_t)(k * p.dim_v + col)] = s[i][e];
                 }
+            }
         }
         {
-            const float y[4] = {d[0] * read.x, d[1] * read.y, d[2] * read.z, d[3] * read.w};
+            // Rows behind the last token have no dout.
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = left >= kChunk || row + e < left ? Elem<DT>::to_float(d[e]) : 0.f;
+            const float y[4] = {x[0] * read.x, x[1] * read.y, x[2] * read.z, x[3] * read.w};
             u32x2 fo[NT], f[3];
-            split4<NT>(d, fo);
+            split4<NT>(x, fo);
 #pragma unroll
             for (int j = 0; j < NT; ++j) put(lds.o, NT, wave, j, fo[j]);
             split4<3>(y, f);
 #pragma unroll
             for (int j = 0; j < 3; ++j) put(lds.q, 3, wave, j, f[j]);
         }
-        const float4 sb = seen, bt = beta;
         lds_barrier();
-        f32x4 u = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            bf16x8 b[3];
-            load_frag<3>(lds.s + i * 3 * kFrag, lane, b);
-            u = product<2>(kf[i], b, u);
-        }
-        u[0] *= carry.x; u[1] *= carry.y; u[2] *= carry.z; u[3] *= carry.w;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i >= from) {
-                bf16x8 b[NT];
-                load_frag<NT>(lds.o + i * NT * kFrag, lane, b);
-                u = product<2>(pf[i], b, u);
-            }
+        f32x4 u = {0.f, 0.f, 0.f, 0.f}, u2 = u, o = u, o2 = u;
         {
-            const float x[4] = {u[0], u[1], u[2], u[3]};
+            bf16x8 b[2][3], bo[2][NT];
+            load_frag<3>(lds.s, lane, b[0]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) load_frag<NT>(lds.o + i * NT * kFrag, lane, bo[i]);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                if (i + 1 < KS) load_frag<3>(lds.s + (i + 1) * 3 * kFrag, lane, b[(i + 1) & 1]);
+                stay();
+                product2<2>(kf[i], b[i & 1], u, u2);
+                if (i == 0) {
+                    if (from == 0) product2<2>(pf[0], bo[0], o, o2);
+                    product2<2>(pf[1], bo[1], o, o2);
+                }
+                stay();
+                ask_k(next, i);
+                if (i == 0) { ask_p(next, 0); ask_p(next, 1); }
+            }
+        }
+        ask_d(next);
+        {
+            u += u2;
+            o += o2;
+            const float x[4] = {u[0] * carry.x + o[0], u[1] * carry.y + o[1], u[2] * carry.z + o[2], u[3] * carry.w + o[3]};
             u32x2 f[3];
             split4<3>(x, f);
 #pragma unroll
             for (int j = 0; j < 3; ++j) put(lds.u, 3, wave, j, f[j]);
         }
-        const float gam = last;
-        if (c > 0) { ask_k(c - 1); ask_d(c - 1); }
         lds_barrier();
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i >= from) {
-                bf16x8 b[3];
-                load_frag<3>(lds.u + i * 3 * kFrag, lane, b);
-                x = product<2>(tf[i], b, x);
-            }
+        f32x4 x = {0.f, 0.f, 0.f, 0.f}, x2 = x;
         {
-            const float y[4] = {-sb.x * x[0], -sb.y * x[1], -sb.z * x[2], -sb.w * x[3]}, bx[4] = {bt.x * x[0], bt.y * x[1], bt.z * x[2], bt.w * x[3]};
+            bf16x8 b[2][3];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) load_frag<3>(lds.u + i * 3 * kFrag, lane, b[i]);
+            stay();
+            if (from == 0) product2<2>(tf[0], b[0], x, x2);
+            stay();
+            ask_carry(next);
+            product2<2>(tf[1], b[1], x, x2);
+            stay();
+            ask_t(next, 0);
+            ask_t(next, 1);
+            x += x2;
+        }
+        {
+            const float y[4] = {-seen.x * x[0], -seen.y * x[1], -seen.z * x[2], -seen.w * x[3]}, bx[4] = {beta.x * x[0], beta.y * x[1], beta.z * x[2], beta.w * x[3]};
             u32x2 f[3];
             split4<3>(y, f);
 #pragma unroll
             for (int j = 0; j < 3; ++j) put(lds.x, 3, wave, j, f[j]);
-            if (has_col)
+            if (has_col) {
+                float *to = w.dx + sv * kChunk * p.dim_v;
+                uint8_t *dc = reinterpret_cast<uint8_t *>(dv + (range.lo + (int64_t)c * kChunk) * bp.dv_stride_l);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int row = row_of(wave, 4 * g + e);
-                    const int64_t tok = range.lo + (int64_t)c * kChunk + row;
-                    w.dx[(sv * kChunk + row) * p.dim_v + col] = x[e];
-                    if (tok < range.hi) dv[tok * bp.dv_stride_l] = Elem<DT>::from_float(bx[e]);
+                    to[(uint32_t)((row + e) * p.dim_v + col)] = x[e];
+                    if (left >= kChunk || row + e < left) *reinterpret_cast<T *>(dc + ((uint32_t)(row + e) * dv_pitch + at_col)) = Elem<DT>::from_float(bx[e]);
                 }
+            }
+            ask_gates(next);
         }
-        if (c > 0) ask_t(c - 1);
         lds_barrier();
-#pragma unroll
-        for (int i = 0; i < TW; ++i) {
-            if (wave * TW + i >= 2 * KS) break;
-            s[i] *= gam;
+        {
+            bf16x8 bq[2][3], bx[2][3];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                bf16x8 b[3];
-                load_frag<3>(lds.q + j * 3 * kFrag, lane, b);
-                s[i] = product<2>(qtf[i][j], b, s[i]);
-                load_frag<3>(lds.x + j * 3 * kFrag, lane, b);
-                s[i] = product<2>(ktf[i][j], b, s[i]);
+                load_frag<3>(lds.q + j * 3 * kFrag, lane, bq[j]);
+                load_frag<3>(lds.x + j * 3 * kFrag, lane, bx[j]);
             }
+            stay();
+#pragma unroll
+            for (int i = 0; i < TW; ++i) {
+                if (wave * TW + i >= 2 * KS) break;
+                f32x4 small = {0.f, 0.f, 0.f, 0.f};
+                s[i] *= last;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    product2<2>(qtf[i][j], bq[j], s[i], small);
+                    product2<2>(ktf[i][j], bx[j], s[i], small);
+                }
+                s[i] += small;
+                stay();
+                ask_kt(next, i);
+            }
+            ask_last(next);
         }
-        if (c > 0) ask_kt(c - 1);
         lds_barrier();                                   // lds.q is written again before the next barrier
     }
     if (bp.dinitial_states == nullptr || !has_col) return;
@@ -227,57 +262,42 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
     }
 }
 
-// 8 elements of a row from column c on, zeros behind `cols`.
-template <int DT>
-__device__ __forceinline__ void row8(const typename Elem<DT>::type *row, int c, int cols, bool vec, float (&f)[8]) {
-    if (vec && c + 8 <= cols) {
-        if constexpr (DT == CC1D_F32) {
-            float lo[4], hi[4];
-            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c), lo);
-            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c + 4), hi);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[i + 4] = hi[i]; }
-        } else {
-            Elem<DT>::unpack(*reinterpret_cast<const u32x4 *>(row + c), f);
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? Elem<DT>::to_float(row[c + i]) : 0.f;
-}
+constexpr int kGradBlock = 512;
 
 template <int KS>
-struct GradStage { uint8_t u[4 * 3 * kFrag], s0[2 * KS * 3 * kFrag], ds1[2 * KS * 3 * kFrag]; };
-struct GradLower { float x1[kChunk][68], x2[kChunk][68]; };
+struct GradStage { uint8_t u[4 * 3 * kFrag], x[4 * 3 * kFrag], s0[2 * KS * 3 * kFrag], ds1[2 * KS * 3 * kFrag]; };
+// X1 and X2 as left operands: their rows (contraction over columns), scaled by rk of the column, in fp32; their columns
+// (contraction over rows), scaled by rq, and by beta rk, of the row, split as operands.
+struct GradLower { float rows[2][kChunk][68]; uint8_t columns[2][kTriFrags * 3 * kFrag]; };
 template <int KS>
 struct GradLds {
     union { GradStage<KS> stage; GradLower lower; };
     float gate[kScalars][kChunk];
-    float dg[kChunk], db[kChunk], end[4], inner[4];
+    float sums[2][3][kChunk];                            // q.dQ, k.Z, k.Y of each token, of either half of dim_k
+    float db[kChunk], end[8], inner[8];
 };
 
-__device__ __forceinline__ float over_columns(float v) {  // over the 16 lanes of a row of a result tile
-    v += __shfl_xor(v, 1); v += __shfl_xor(v, 2); v += __shfl_xor(v, 4); v += __shfl_xor(v, 8);
-    return v;
-}
-
-template <int DT, int KS>
-__global__ void __launch_bounds__(kBlock, 1)
-delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int vec_x, const int vec_s) {
+// Every chunk's gradients alone.  Eight wavefronts: 16 tokens' rows of dQ, Z and Y each, of one half of dim_k; of X1 the first
+// four, of X2 the others.  S0, dS1 and U pass through LDS once for all of them, 32 columns of dim_v at a time, split into their
+// terms.  VEC: rows of v and dout are whole 16-byte vectors, rows of the fp32 matrices in the workspace too.
+template <int DT, int KS, bool VEC>
+__global__ void __launch_bounds__(kGradBlock, 1)
+delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int vec_out) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n;
-    constexpr int TILES = 2 * KS;
+    constexpr int TILES = KS, OWN = (2 * KS + 7) / 8;    // 16-column tiles of a half; that a wavefront brings to LDS
     extern __shared__ uint4 raw[];
     GradLds<KS> &lds = *reinterpret_cast<GradLds<KS> *>(raw);
     const cc1d_delta_params &p = bp.fwd;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tile = wave & 3, side = wave >> 2;
     const int slot = (int)(blockIdx.x / (uint32_t)p.heads), hk = (int)(blockIdx.x % (uint32_t)p.heads);
     const int group = p.v_heads / p.heads;
     const ChunkAt at = chunk_at(p, w, slot);
     T *dq = static_cast<T *>(bp.dq) + hk * bp.dq_stride_h, *dk = static_cast<T *>(bp.dk) + hk * bp.dk_stride_h;
     if (p.cu_seqlens != nullptr && slot == 0) {          // tokens in front of the first sequence and behind the last
         auto clear = [&](int64_t lo, int64_t hi) {
-            for (int64_t t = lo + wave; t < hi; t += 4) {
+            for (int64_t t = lo + wave; t < hi; t += 8) {
                 for (int k = lane; k < p.dim_k; k += 64) {
                     dq[t * bp.dq_stride_l + k] = Elem<DT>::from_float(0.f);
                     dk[t * bp.dk_stride_l + k] = Elem<DT>::from_float(0.f);
@@ -293,56 +313,74 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
     }
     if (at.count <= 0) return;
     const int64_t sh = (int64_t)slot * p.heads + hk;
-    const int own = row_of(wave, m);                     // the token whose row this lane holds as a left operand
-    const int row = row_of(wave, 4 * g);                 // the first of the four whose results it holds
-    const bool there = own < at.count;
+    const int own = row_of(tile, m);                     // the token whose row this lane holds as a left operand
+    const int row = row_of(tile, 4 * g);                 // the first of the four whose results it holds
+    const int half = tile >> 1;                          // where those four stand in K^T, Q^T: step, and first or second four
+    const bool upper = tile & 1;
+    const int cols = own < at.count ? p.dim_v : 0;
+    const bool cut_k = p.dim_k < 32 * KS;
+    const uint8_t *kt = w.ktf + sh * w.kbytes() + side * TILES * 2 * NT * kFrag, *qt = w.qtf + sh * w.kbytes() + side * TILES * 2 * NT * kFrag;
 
     f32x4 tq[TILES], tk[TILES];                          // dQ, dK of all heads of the group
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) { tq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; tk[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
-    // An element of Q or K where the result tiles have it.
-    auto element = [&](const void *base, int64_t sb, int64_t sl, int64_t sh_, int t, int e) {
-        const int k = row_of(t, m);
-        return k < p.dim_k && row + e < at.count ? Elem<DT>::to_float(static_cast<const T *>(base)[at.b * sb + (at.lo + row + e) * sl + hk * sh_ + k]) : 0.f;
-    };
+    for (int t = 0; t < TILES; ++t) { tq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; tk[t] = tq[t]; }
 
     for (int j = 0; j < group; ++j) {
         const int h = hk * group + j;
         const int64_t sv = (int64_t)slot * p.v_heads + h;
-        for (int i = threadIdx.x; i < kScalars * kChunk; i += kBlock) (&lds.gate[0][0])[i] = w.scalars[sv * kScalars * kChunk + i];
-        f32x4 aq[TILES], az[TILES], ay[TILES], x1[4], x2[4];
+        for (int i = threadIdx.x; i < kScalars * kChunk; i += kGradBlock) (&lds.gate[0][0])[i] = w.scalars[sv * kScalars * kChunk + i];
+        f32x4 aq[TILES], az[TILES], ay[TILES], x[4];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) { aq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; az[t] = aq[t]; ay[t] = aq[t]; }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) { x1[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; x2[t] = x1[t]; }
+        for (int t = 0; t < 4; ++t) x[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
         float inner = 0.f, dxv = 0.f;
-        const T *dop = static_cast<const T *>(bp.dout) + at.b * bp.dout_stride_b + (at.lo + (there ? own : 0)) * bp.dout_stride_l + h * bp.dout_stride_h;
-        const T *vp = static_cast<const T *>(p.v) + at.b * p.v_stride_b + (at.lo + (there ? own : 0)) * p.v_stride_l + h * p.v_stride_h;
-        const float *up = w.u + (sv * kChunk + own) * p.dim_v, *xp = w.dx + (sv * kChunk + own) * p.dim_v;
+        const int64_t tok = at.lo + (cols ? own : 0);
+        const T *dop = static_cast<const T *>(bp.dout) + at.b * bp.dout_stride_b + tok * bp.dout_stride_l + h * bp.dout_stride_h;
+        const T *vp = static_cast<const T *>(p.v) + at.b * p.v_stride_b + tok * p.v_stride_l + h * p.v_stride_h;
+        // What 32 columns of v need, asked for a step ahead: this lane's row of dO, and of dX and V or of U; its share of S0 and dS1.
+        Row8<DT, VEC> ro, rv;
+        Row8<CC1D_F32, VEC> rx, rs[OWN], rd[OWN];
+        const float *s0 = w.s0 + sv * p.dim_k * p.dim_v, *ds1 = w.ds1 + sv * p.dim_k * p.dim_v;
+        const float *xp = (side == 0 ? w.dx : w.u) + sv * kChunk * p.dim_v;
+        auto ask = [&](int c) {
+            ro.ask(dop, c, cols);
+            if (side == 0) rv.ask(vp, c, p.dim_v);
+            rx.ask(xp + (uint32_t)(own * p.dim_v), c, p.dim_v);
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                const int t = wave + 8 * i < 2 * KS ? wave + 8 * i : 0, k = row_of(t, m);
+                const uint32_t to = (uint32_t)((k < p.dim_k ? k : 0) * p.dim_v);
+                rs[i].ask(s0 + to, c, p.dim_v);
+                rd[i].ask(ds1 + to, c, p.dim_v);
+            }
+        };
+        ask(8 * g);
         for (int v0 = 0; v0 < p.dim_v; v0 += 32) {
             const int c = v0 + 8 * g;
+            const bool cut = v0 + 32 > p.dim_v;
             float f[8], f2[8];
             bf16x8 fo[NT], fx[3], fu[3];
-            row8<DT>(dop, c, there ? p.dim_v : 0, vec_x, f);
-            split8<NT>(f, fo);
-            row8<CC1D_F32>(xp, c, p.dim_v, vec_s, f);
-            row8<DT>(vp, c, there ? p.dim_v : 0, vec_x, f2);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dxv += f[e] * f2[e];
+            ro.template operand<NT>(c, cols, true, fo);
+            rx.get(c, p.dim_v, cut, f);
             split8<3>(f, fx);
-            row8<CC1D_F32>(up, c, p.dim_v, vec_s, f);
-            split8<3>(f, fu);
-            __syncthreads();                             // the step before has been read
+            if (side == 0) {
+                rv.get(c, p.dim_v, cut, f2);
 #pragma unroll
-            for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4 *>(lds.stage.u + (wave * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(fu[n]);
+                for (int e = 0; e < 8; ++e) dxv += f[e] * f2[e];
+            }
+            lds_barrier();                             // the step before has been read
+            uint8_t *mine = (side == 0 ? lds.stage.x : lds.stage.u) + tile * 3 * kFrag + lane * 16;
 #pragma unroll
-            for (int i = 0; i < (TILES + 3) / 4; ++i) {
-                const int t = wave + 4 * i;
-                if (t >= TILES) break;
-                const int k = row_of(t, m);
+            for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4 *>(mine + n * kFrag) = bitcast<u32x4>(fx[n]);
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                const int t = wave + 8 * i;
+                if (t >= 2 * KS) break;
+                const int in = row_of(t, m) < p.dim_k ? p.dim_v : 0;
                 bf16x8 fs[3];
-                row8<CC1D_F32>(w.s0 + (sv * p.dim_k + (k < p.dim_k ? k : 0)) * p.dim_v, c, k < p.dim_k ? p.dim_v : 0, vec_s, f);
-                row8<CC1D_F32>(w.ds1 + (sv * p.dim_k + (k < p.dim_k ? k : 0)) * p.dim_v, c, k < p.dim_k ? p.dim_v : 0, vec_s, f2);
+                rs[i].get(c, in, cut || cut_k, f);
+                rd[i].get(c, in, cut || cut_k, f2);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) inner += f[e] * f2[e];
                 split8<3>(f, fs);
@@ -352,120 +390,153 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
 #pragma unroll
                 for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4 *>(lds.stage.ds1 + (t * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(fs[n]);
             }
-            __syncthreads();
+            if (v0 + 32 < p.dim_v) ask(c + 32);
+            lds_barrier();
+            load_frag<3>(lds.stage.x + tile * 3 * kFrag, lane, fx);
+            load_frag<3>(lds.stage.u + tile * 3 * kFrag, lane, fu);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                if ((t >> 1) <= (wave >> 1)) {
+                if ((t >> 1) <= half) {
                     bf16x8 b[3];
                     load_frag<3>(lds.stage.u + t * 3 * kFrag, lane, b);
-                    x1[t] = product<2>(fo, b, x1[t]);
-                    x2[t] = product<2>(fx, b, x2[t]);
+                    x[t] = side == 0 ? product<2>(fo, b, x[t]) : product<2>(fx, b, x[t]);
                 }
+            const uint8_t *sl = lds.stage.s0 + side * TILES * 3 * kFrag, *dl = lds.stage.ds1 + side * TILES * 3 * kFrag;
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
-                bf16x8 b[3];
-                load_frag<3>(lds.stage.s0 + t * 3 * kFrag, lane, b);
+                bf16x8 b[3], d[3];
+                load_frag<3>(sl + t * 3 * kFrag, lane, b);
+                load_frag<3>(dl + t * 3 * kFrag, lane, d);
                 aq[t] = product<2>(fo, b, aq[t]);
                 az[t] = product<2>(fx, b, az[t]);
-                load_frag<3>(lds.stage.ds1 + t * 3 * kFrag, lane, b);
-                ay[t] = product<2>(fu, b, ay[t]);
+                ay[t] = product<2>(fu, d, ay[t]);
             }
         }
-        __syncthreads();                                 // the stage becomes X1, X2
+        // K^T and Q^T of the half of the chunk that holds this wavefront's own tokens.
+        bf16x8 bk[TILES][NT], bq[TILES][NT];
+        auto ask_kq = [&](int s) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int jj = row_of(t, m);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = row + e;
-                float decay = 0.f;
-                if (i >= jj) decay = expf((lds.gate[kSumHi][i] - lds.gate[kSumHi][jj]) + (lds.gate[kSumLo][i] - lds.gate[kSumLo][jj]));
-                lds.lower.x1[i][jj] = i >= jj ? p.scale * x1[t][e] * decay : 0.f;
-                lds.lower.x2[i][jj] = i > jj ? -x2[t][e] * decay : 0.f;
+            for (int t = 0; t < TILES; ++t) {
+                load_frag<NT>(kt + (t * 2 + s) * NT * kFrag, lane, bk[t]);
+                load_frag<NT>(qt + (t * 2 + s) * NT * kFrag, lane, bq[t]);
             }
-        }
-        float to_last = 0.f;                             // sum over this lane's tokens of k.W
+        };
+        ask_kq(half);
+        lds_barrier();                                   // the stage becomes X1, X2
+        float rk[4], rq[4], beta[4], hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float gam = lds.gate[kGate][row + e], dec = lds.gate[kToEnd][row + e], rk = lds.gate[kKeyNorm][row + e];
+            rk[e] = lds.gate[kKeyNorm][row + e]; rq[e] = lds.gate[kQueryNorm][row + e]; beta[e] = lds.gate[kBeta][row + e];
+            hi[e] = lds.gate[kSumHi][row + e]; lo[e] = lds.gate[kSumLo][row + e];
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if ((t >> 1) > half) continue;
+            const int jj = row_of(t, m);
+            const float rj = lds.gate[kKeyNorm][jj], hj = lds.gate[kSumHi][jj], lj = lds.gate[kSumLo][jj];
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float d = x[t][e] * exp_of((hi[e] - hj) + (lo[e] - lj));
+                const float z = side == 0 ? (row + e >= jj ? p.scale * d : 0.f) : (row + e > jj ? -d : 0.f);
+                lds.lower.rows[side][row + e][jj] = z * rj;
+                y[e] = z * (side == 0 ? rq[e] : beta[e] * rk[e]);
+            }
+            // Column jj as a row of the transposed matrix: tile t, four of its elements from token `row` on.
+            u32x2 f[3];
+            split4<3>(y, f);
+            uint8_t *to = lds.lower.columns[side] + upper_frag(t, half) * 3 * kFrag + (g * 16 + m) * 16 + (tile & 1) * 8;
+#pragma unroll
+            for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2 *>(to + n * kFrag) = f[n];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float gam = lds.gate[kGate][row + e], dec = lds.gate[kToEnd][row + e];
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
                 aq[t][e] *= p.scale * gam;
                 az[t][e] *= -gam;
                 ay[t][e] *= dec;
-                to_last += ay[t][e] * rk * element(p.k, p.k_stride_b, p.k_stride_l, p.k_stride_h, t, e);
             }
         }
-        __syncthreads();
-        const uint8_t *kt = w.ktf + sh * w.kbytes(), *qt = w.qtf + sh * w.kbytes();
+        dxv = over_rows(dxv);
+        if (g == 0 && side == 0) lds.db[own] = dxv;
+        lds_barrier();
+        // Rows of X1 and X2 against K, their columns against Q and K.  The operand of the step that holds this lane's own four
+        // tokens also has their elements of K and Q, in the lane that has the results: what the gates' gradients multiply.
+        float to_last = 0.f;                             // this lane's share of sum k.W, while Y is W alone
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int c = 32 * s + 8 * g;
+        for (int t = 0; t < TILES; ++t) {
+            float ke[4];
+            four_of(bk[t], upper, ke);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to_last += ay[t][e] * (rk[e] * ke[e]);
+        }
+        auto row_products = [&](int s) {
             float f[8];
-            bf16x8 a[3], a2[3];
-            if (s <= (wave >> 1)) {                      // rows of X1, X2
+            bf16x8 a1[3], a2[3];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = lds.lower.x1[own][c + e] * lds.gate[kKeyNorm][c + e];
-                split8<3>(f, a);
+            for (int i = 0; i < 2; ++i) {
+                const float *from = &lds.lower.rows[i][own][32 * s + 8 * g];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = lds.lower.x2[own][c + e] * lds.gate[kKeyNorm][c + e];
-                split8<3>(f, a2);
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    bf16x8 b[NT];
-                    load_frag<NT>(kt + (t * 2 + s) * NT * kFrag, lane, b);
-                    aq[t] = product<2>(a, b, aq[t]);
-                    az[t] = product<2>(a2, b, az[t]);
-                }
+                for (int e = 0; e < 8; ++e) f[e] = from[e];
+                if (i == 0) split8<3>(f, a1); else split8<3>(f, a2);
             }
-            if (s >= (wave >> 1)) {                      // their columns
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = lds.lower.x1[c + e][own] * lds.gate[kQueryNorm][c + e];
-                split8<3>(f, a);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = lds.lower.x2[c + e][own] * (lds.gate[kBeta][c + e] * lds.gate[kKeyNorm][c + e]);
-                split8<3>(f, a2);
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    bf16x8 b[NT];
-                    load_frag<NT>(qt + (t * 2 + s) * NT * kFrag, lane, b);
-                    ay[t] = product<2>(a, b, ay[t]);
-                    load_frag<NT>(kt + (t * 2 + s) * NT * kFrag, lane, b);
-                    ay[t] = product<2>(a2, b, ay[t]);
-                }
-            }
-        }
-        dxv += __shfl_xor(dxv, 16); dxv += __shfl_xor(dxv, 32);
-        if (g == 0) lds.db[own] = dxv;
-        inner = wave_sum(inner);
-        to_last = wave_sum(to_last);
-        if (lane == 0) { lds.inner[wave] = inner; lds.end[wave] = to_last; }
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float rk = lds.gate[kKeyNorm][row + e], rq = lds.gate[kQueryNorm][row + e], beta = lds.gate[kBeta][row + e];
-            float qd = 0.f, kz = 0.f, ky = 0.f;
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
-                const float ke = rk * element(p.k, p.k_stride_b, p.k_stride_l, p.k_stride_h, t, e);
-                qd += aq[t][e] * rq * element(p.q, p.q_stride_b, p.q_stride_l, p.q_stride_h, t, e);
-                kz += az[t][e] * ke;
-                ky += ay[t][e] * ke;
-                tq[t][e] += aq[t][e];
-                tk[t][e] += beta * az[t][e] + ay[t][e];
+                aq[t] = product<2>(a1, bk[t], aq[t]);
+                az[t] = product<2>(a2, bk[t], az[t]);
             }
-            qd = over_columns(qd); kz = over_columns(kz); ky = over_columns(ky);
-            if (m == 0) {
-                lds.dg[row + e] = qd + beta * kz - ky;
-                lds.db[row + e] += kz;
+        };
+        auto column_products = [&](int s) {
+            bf16x8 a1[3], a2[3];
+            load_frag<3>(lds.lower.columns[0] + upper_frag(tile, s) * 3 * kFrag, lane, a1);
+            load_frag<3>(lds.lower.columns[1] + upper_frag(tile, s) * 3 * kFrag, lane, a2);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                ay[t] = product<2>(a1, bq[t], ay[t]);
+                ay[t] = product<2>(a2, bk[t], ay[t]);
+            }
+        };
+        row_products(half);
+        column_products(half);
+        ask_kq(1 - half);
+        if (half == 0) column_products(1); else row_products(0);
+        ask_kq(half);
+        float qd[4] = {0.f, 0.f, 0.f, 0.f}, kz[4] = {0.f, 0.f, 0.f, 0.f}, ky[4] = {0.f, 0.f, 0.f, 0.f};
+        {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                float ke[4], qe[4];
+                four_of(bk[t], upper, ke);
+                four_of(bq[t], upper, qe);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    qd[e] += aq[t][e] * qe[e];
+                    kz[e] += az[t][e] * ke[e];
+                    ky[e] += ay[t][e] * ke[e];
+                    tq[t][e] += aq[t][e];
+                    tk[t][e] += beta[e] * az[t][e] + ay[t][e];
+                }
             }
         }
-        __syncthreads();
+        inner = over_wave(inner);
+        to_last = over_wave(to_last);
+        if (lane == 0) { lds.inner[wave] = inner; lds.end[wave] = to_last; }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float d = rq[e] * over_columns(qd[e]), z = rk[e] * over_columns(kz[e]), y = rk[e] * over_columns(ky[e]);
+            if (m == 0) { lds.sums[side][0][row + e] = d; lds.sums[side][1][row + e] = z; lds.sums[side][2][row + e] = y; }
+        }
+        lds_barrier();
         if (wave == 0) {
-            float d = lds.dg[lane];
+            const float z = lds.sums[0][1][lane] + lds.sums[1][1][lane];
+            float d = (lds.sums[0][0][lane] + lds.sums[1][0][lane]) + lds.gate[kBeta][lane] * z - (lds.sums[0][2][lane] + lds.sums[1][2][lane]);
             if (lane == 63) {
-                const float both = (lds.inner[0] + lds.inner[1]) + (lds.inner[2] + lds.inner[3]);
-                d += ((lds.end[0] + lds.end[1]) + (lds.end[2] + lds.end[3])) + lds.gate[kGate][63] * both;
+                float both = 0.f, ends = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { both += lds.inner[i]; ends += lds.end[i]; }
+                d += ends + lds.gate[kGate][63] * both;
             }
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -477,41 +548,83 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
             if (lane < at.count) {
                 const int64_t to = ((int64_t)at.b * p.seqlen + at.lo + lane) * p.v_heads + h;
                 store_from_float(bp.dg, to, p.g_dtype, d);
-                store_from_float(bp.dbeta, to, p.beta_dtype, lds.db[lane]);
+                store_from_float(bp.dbeta, to, p.beta_dtype, lds.db[lane] + z);
             }
         }
-        __syncthreads();
+        lds_barrier();
     }
 
-    // The lengths' share, and out.
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float rk = lds.gate[kKeyNorm][row + e], rq = lds.gate[kQueryNorm][row + e];
-        float dotq = 0.f, dotk = 0.f;
-        if (p.qk_l2norm) {
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                dotq += tq[t][e] * element(p.q, p.q_stride_b, p.q_stride_l, p.q_stride_h, t, e);
-                dotk += tk[t][e] * element(p.k, p.k_stride_b, p.k_stride_l, p.k_stride_h, t, e);
-            }
-            dotq = over_columns(dotq) * rq * rq;
-            dotk = over_columns(dotk) * rk * rk;
-        }
-        if (row + e >= at.count) continue;
-        const int64_t tok = at.lo + row + e;
+    // The lengths' share.
+    if (p.qk_l2norm) {
+        float rk[4], rq[4], dotq[4] = {0.f, 0.f, 0.f, 0.f}, dotk[4] = {0.f, 0.f, 0.f, 0.f};
+        bf16x8 bk[TILES][NT], bq[TILES][NT];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const int k = row_of(t, m);
-            if (k >= p.dim_k) continue;
-            float a = tq[t][e], b = tk[t][e];
-            if (p.qk_l2norm) {
-                a = rq * (a - dotq * element(p.q, p.q_stride_b, p.q_stride_l, p.q_stride_h, t, e));
-                b = rk * (b - dotk * element(p.k, p.k_stride_b, p.k_stride_l, p.k_stride_h, t, e));
+            load_frag<NT>(kt + (t * 2 + half) * NT * kFrag, lane, bk[t]);
+            load_frag<NT>(qt + (t * 2 + half) * NT * kFrag, lane, bq[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            float ke[4], qe[4];
+            four_of(bk[t], upper, ke);
+            four_of(bq[t], upper, qe);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                dotq[e] += tq[t][e] * qe[e];
+                dotk[e] += tk[t][e] * ke[e];
             }
-            dq[at.b * bp.dq_stride_b + tok * bp.dq_stride_l + k] = Elem<DT>::from_float(a);
-            dk[at.b * bp.dk_stride_b + tok * bp.dk_stride_l + k] = Elem<DT>::from_float(b);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            dotq[e] = over_columns(dotq[e]);
+            dotk[e] = over_columns(dotk[e]);
+            if (m == 0) { lds.sums[side][0][row + e] = dotq[e]; lds.sums[side][1][row + e] = dotk[e]; }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            rk[e] = lds.gate[kKeyNorm][row + e]; rq[e] = lds.gate[kQueryNorm][row + e];
+            dotq[e] = (lds.sums[0][0][row + e] + lds.sums[1][0][row + e]) * rq[e] * rq[e];
+            dotk[e] = (lds.sums[0][1][row + e] + lds.sums[1][1][row + e]) * rk[e] * rk[e];
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            float ke[4], qe[4];
+            four_of(bk[t], upper, ke);
+            four_of(bq[t], upper, qe);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                tq[t][e] = rq[e] * (tq[t][e] - dotq[e] * qe[e]);
+                tk[t][e] = rk[e] * (tk[t][e] - dotk[e] * ke[e]);
+            }
         }
     }
+    // Out through LDS, so that whole rows leave.
+    constexpr int PITCH = 32 * KS + 8;
+    T *rows_out = reinterpret_cast<T *>(raw);            // the stage is free
+    auto leave = [&](const f32x4 (&v)[TILES], T *to, int64_t sb, int64_t sl) {
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rows_out[(row + e) * PITCH + row_of(side * TILES + t, m)] = Elem<DT>::from_float(v[t][e]);
+        lds_barrier();
+        T *base = to + at.b * sb + at.lo * sl;
+        for (int i = threadIdx.x; i < at.count * 4 * KS; i += kGradBlock) {    // 8 elements a lane
+            const int token = i / (4 * KS), c = i % (4 * KS) * 8;
+            if (c >= p.dim_k) continue;
+            const T *from = rows_out + token * PITCH + c;
+            T *d = base + token * sl + c;
+            if (vec_out && c + 8 <= p.dim_k) {
+#pragma unroll
+                for (int v4 = 0; v4 < (int)sizeof(T) / 2; ++v4) reinterpret_cast<u32x4 *>(d)[v4] = reinterpret_cast<const u32x4 *>(from)[v4];
+            } else {
+                for (int e = 0; e < 8 && c + e < p.dim_k; ++e) d[e] = from[e];
+            }
+        }
+    };
+    leave(tq, dq, bp.dq_stride_b, bp.dq_stride_l);
+    leave(tk, dk, bp.dk_stride_b, bp.dk_stride_l);
 }
 
 template <int DT, int KS>
@@ -521,12 +634,13 @@ int launch(const cc1d_delta_bwd_params &bp, const ChunkWork &w, hipStream_t stre
     CC1D_LAUNCH((delta_bwd_scan_kernel<DT, KS>), dim3((nh + 7) / 8 * 8 * tiles), dim3(kBlock), 0, stream, bp, w, nh, tiles);
     int st = launch_status();
     if (st != CC1D_OK || w.slots == 0) return st;
-    auto rows = [&](const void *x, int64_t b, int64_t l, int64_t h) {
-        const int v = vec_elems(p.x_dtype);
-        return aligned16(x) && b % v == 0 && l % v == 0 && h % v == 0;
-    };
-    const int vec_x = rows(bp.dout, bp.dout_stride_b, bp.dout_stride_l, bp.dout_stride_h) && rows(p.v, p.v_stride_b, p.v_stride_l, p.v_stride_h);
-    CC1D_LAUNCH((delta_grad_kernel<DT, KS>), dim3((uint32_t)((int64_t)w.slots * p.heads)), dim3(kBlock), sizeof(GradLds<KS>), stream, bp, w, vec_x, (int)(p.dim_v % 4 == 0));
+    const bool vec = p.dim_v % 8 == 0 && whole_rows(p.x_dtype, bp.dout, bp.dout_stride_b, bp.dout_stride_l, bp.dout_stride_h) &&
+                     whole_rows(p.x_dtype, p.v, p.v_stride_b, p.v_stride_l, p.v_stride_h);
+    const int vec_out = whole_rows(p.x_dtype, bp.dq, bp.dq_stride_b, bp.dq_stride_l, bp.dq_stride_h) &&
+                        whole_rows(p.x_dtype, bp.dk, bp.dk_stride_b, bp.dk_stride_l, bp.dk_stride_h);
+    const dim3 grid((uint32_t)((int64_t)w.slots * p.heads));
+    if (vec) CC1D_LAUNCH((delta_grad_kernel<DT, KS, true>), grid, dim3(kGradBlock), sizeof(GradLds<KS>), stream, bp, w, vec_out);
+    else CC1D_LAUNCH((delta_grad_kernel<DT, KS, false>), grid, dim3(kGradBlock), sizeof(GradLds<KS>), stream, bp, w, vec_out);
     return launch_status();
 }
 

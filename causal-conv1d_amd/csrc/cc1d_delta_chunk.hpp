@@ -84,7 +84,9 @@ __device__ __forceinline__ int first_slot(const cc1d_delta_params &p, const Chun
 }
 
 // N bfloat16 terms of 4 (8) numbers, term i in two (four) words, each the rest rounded to nearest: two leave 2^-18 of a
-// number, three nothing.
+// number, three nothing.  What a term leaves, x - hi, is one instruction, a dot product of the pair that hi stands in with
+// (-1, 0) or (0, -1) added to x; it is exact.  The pairs are kept in scalar registers: as immediates the compiler puts them into
+// the wrong half.
 __device__ __forceinline__ uint32_t rounded_pair(float lo, float hi) {
     bf16x2 h;
     h.x = (__bf16)lo;
@@ -93,14 +95,18 @@ __device__ __forceinline__ uint32_t rounded_pair(float lo, float hi) {
 }
 template <int N>
 __device__ __forceinline__ void split4(const float (&x)[4], u32x2 (&t)[N]) {
+    uint32_t low = 0x0000bf80u, high = 0xbf800000u;
+    asm("" : "+s"(low), "+s"(high));
     float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         t[n].x = rounded_pair(r[0], r[1]);
         t[n].y = rounded_pair(r[2], r[3]);
         if (n + 1 < N) {
-            r[0] -= bitcast<float>(t[n].x << 16); r[1] -= bitcast<float>(t[n].x & 0xffff0000u);
-            r[2] -= bitcast<float>(t[n].y << 16); r[3] -= bitcast<float>(t[n].y & 0xffff0000u);
+            r[0] = __builtin_amdgcn_fdot2_f32_bf16(bitcast<bf16x2>((uint32_t)t[n].x), bitcast<bf16x2>(low), r[0], false);
+            r[1] = __builtin_amdgcn_fdot2_f32_bf16(bitcast<bf16x2>((uint32_t)t[n].x), bitcast<bf16x2>(high), r[1], false);
+            r[2] = __builtin_amdgcn_fdot2_f32_bf16(bitcast<bf16x2>((uint32_t)t[n].y), bitcast<bf16x2>(low), r[2], false);
+            r[3] = __builtin_amdgcn_fdot2_f32_bf16(bitcast<bf16x2>((uint32_t)t[n].y), bitcast<bf16x2>(high), r[3], false);
         }
     }
 }
@@ -158,7 +164,8 @@ struct Row8 {
             }
         }
     }
-    __device__ __forceinline__ void get(int c, int cols, float (&f)[8]) const {
+    // `cut`: some lane's elements are not all inside.
+    __device__ __forceinline__ void get(int c, int cols, bool cut, float (&f)[8]) const {
         if constexpr (DT == CC1D_F32) {
             float lo[4], hi[4];
             Elem<DT>::unpack(r[0], lo);
@@ -168,8 +175,22 @@ struct Row8 {
         } else {
             Elem<DT>::unpack(r[0], f);
         }
+        if (cut)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = (VEC ? c : c + i) < cols ? f[i] : 0.f;
+            for (int i = 0; i < 8; ++i) f[i] = (VEC ? c : c + i) < cols ? f[i] : 0.f;
+    }
+    // As an operand of TERMS terms; bfloat16 is one as it stands.
+    template <int TERMS>
+    __device__ __forceinline__ void operand(int c, int cols, bool cut, bf16x8 (&t)[TERMS]) const {
+        if constexpr (DT == CC1D_BF16 && VEC) {
+            u32x4 w = r[0];
+            if (cut && c >= cols) { w.x = 0; w.y = 0; w.z = 0; w.w = 0; }
+            t[0] = bitcast<bf16x8>(w);
+        } else {
+            float f[8];
+            get(c, cols, cut, f);
+            split8<TERMS>(f, t);
+        }
     }
 };
 
@@ -213,14 +234,22 @@ __device__ __forceinline__ void product2(const bf16x8 (&a)[NA], const bf16x8 (&b
         }
 }
 
-// The number that element i of an operand's lane stands for.
+// The numbers that elements 0..3 (or, `upper`, 4..7) of an operand's lane stand for.
 template <int N>
-__device__ __forceinline__ float term_sum(const bf16x8 (&f)[N], int i) {
-    float v = (float)f[N - 1][i];
+__device__ __forceinline__ void four_of(const bf16x8 (&t)[N], bool upper, float (&f)[4]) {
 #pragma unroll
-    for (int n = N - 2; n >= 0; --n) v += (float)f[n][i];
-    return v;
+    for (int n = N - 1; n >= 0; --n) {
+        const u32x4 w = bitcast<u32x4>(t[n]);
+        const uint32_t a = upper ? w.z : w.x, b = upper ? w.w : w.y;
+        const float x[4] = {bitcast<float>(a << 16), bitcast<float>(a & 0xffff0000u), bitcast<float>(b << 16), bitcast<float>(b & 0xffff0000u)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = n == N - 1 ? x[i] : f[i] + x[i];
+    }
 }
+
+// Loads stay between the products where they are written: bunched, or moved, they hold the wavefront up while the
+// address unit works them off, 16 cycles each.
+__device__ __forceinline__ void stay() { __builtin_amdgcn_sched_barrier(0); }
 
 // A barrier that orders LDS alone: loads and stores of global memory stay in flight.
 __device__ __forceinline__ void lds_barrier() {

@@ -64,14 +64,14 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             float x[8];
-            kr[s].get(32 * s + 8 * g, cols, x);
+            kr[s].get(32 * s + 8 * g, cols, true, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) kk += x[i] * x[i];
-            split8<NT>(x, kf[s]);
-            qr[s].get(32 * s + 8 * g, cols, x);
+            kr[s].template operand<NT>(32 * s + 8 * g, cols, true, kf[s]);
+            qr[s].get(32 * s + 8 * g, cols, true, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) qq += x[i] * x[i];
-            split8<NT>(x, qf[s]);
+            qr[s].template operand<NT>(32 * s + 8 * g, cols, true, qf[s]);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
@@ -87,13 +87,13 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
                 if (!w.backward) *reinterpret_cast<u32x4 *>(qd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
             }
     }
-    kk += __shfl_xor(kk, 16); kk += __shfl_xor(kk, 32);
-    qq += __shfl_xor(qq, 16); qq += __shfl_xor(qq, 32);
+    kk = over_rows(kk);
+    qq = over_rows(qq);
     if (g == 0) {
         lds.norms[0][token] = p.qk_l2norm ? rsqrtf(kk + kNormEps) : 1.f;
         lds.norms[1][token] = p.qk_l2norm ? rsqrtf(qq + kNormEps) : 1.f;
     }
-    __syncthreads();
+    lds_barrier();
 
     // Gates.  Sums in 64 bits, kept as two floats: differences of large sums lose nothing.
     if (wave == 0) {
@@ -107,7 +107,7 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
             if (lane >= d) sum += o;
         }
         const double last = __shfl(sum, 63);
-        const float hi = (float)sum, gam = expf((float)sum), dec = expf((float)(last - sum));
+        const float hi = (float)sum, gam = exp_of((float)sum), dec = exp_of((float)(last - sum));
         const float rk = lds.norms[0][lane], rq = lds.norms[1][lane];
         lds.gate[kSeenBeta][lane] = beta * gam * rk;
         lds.gate[kBeta][lane] = beta;
@@ -120,7 +120,7 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
         lds.gate[kSumHi][lane] = hi;
         lds.gate[kSumLo][lane] = (float)(sum - (double)hi);
     }
-    __syncthreads();
+    lds_barrier();
     for (int i = threadIdx.x; i < kScalars * kChunk; i += kBlock) w.scalars[sv * kScalars * kChunk + i] = (&lds.gate[0][0])[i];
 
     // K K^T and Q K^T: this wavefront's 16 rows; columns behind the rows' last are nothing.
@@ -142,12 +142,12 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
         for (int e = 0; e < 4; ++e) {
             const int i = row_of(wave, 4 * g + e);
             float decay = 0.f;
-            if (i >= j) decay = expf((lds.gate[kSumHi][i] - lds.gate[kSumHi][j]) + (lds.gate[kSumLo][i] - lds.gate[kSumLo][j])) * lds.gate[kKeyNorm][j];
+            if (i >= j) decay = exp_of((lds.gate[kSumHi][i] - lds.gate[kSumHi][j]) + (lds.gate[kSumLo][i] - lds.gate[kSumLo][j])) * lds.gate[kKeyNorm][j];
             lds.a[i][j] = i > j ? a[e] * decay * (lds.gate[kBeta][i] * lds.gate[kKeyNorm][i]) : 0.f;
             read[ct][e] = i >= j ? r[e] * decay * (p.scale * lds.gate[kQueryNorm][i]) : 0.f;
         }
     }
-    __syncthreads();
+    lds_barrier();
 
     // T.  Diagonal blocks: lane = column.
     {
@@ -168,7 +168,7 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
             if ((c >> 4) > (r >> 4)) lds.t[r][c] = 0.f;
         }
     }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int d = 1; d < 4; ++d) {
         const int i = wave + d, j = wave;                // block (i, j)
@@ -183,7 +183,7 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) lds.t[16 * i + 4 * g + e][16 * j + m] = acc[e];
         }
-        __syncthreads();
+        lds_barrier();
     }
 
     // T and its transpose as left operands.
@@ -213,7 +213,7 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
         for (int e = 0; e < 4; ++e) lds.a[row_of(wave, 4 * g + e)][row_of(ct, m)] = read[ct][e];
-    __syncthreads();
+    lds_barrier();
     if (!w.backward)
         for (int s = 0; s <= (wave >> 1); ++s) {
         float x[8];
@@ -264,13 +264,13 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     };
     transposed(w.ktf + sh * w.kbytes());
     if (!w.backward) return;
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
             *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
-    __syncthreads();
+    lds_barrier();
     transposed(w.qtf + sh * w.kbytes());
 }
 

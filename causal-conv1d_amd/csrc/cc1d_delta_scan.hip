@@ -24,10 +24,6 @@ struct ScanLds {
     uint8_t d[CT][2 * 3 * kFrag];        // U to the chunk's end for S
 };
 
-// Loads stay between the products where they are written: bunched, or moved, they hold the wavefront up while the
-// address unit works them off, 16 cycles each.
-__device__ __forceinline__ void stay() { __builtin_amdgcn_sched_barrier(0); }
-
 // STATES: the state in front of every chunk, and U, go to memory too (for the backward), O does not.
 template <int DT, int KS, int CT, bool STATES>
 __global__ void __launch_bounds__(kBlock, CT == 1 ? 2 : 1)
