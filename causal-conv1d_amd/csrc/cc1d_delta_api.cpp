@@ -7,6 +7,7 @@ using namespace cc1d;
 
 namespace {
 
+bool aligned256(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
 bool dtype_ok(int d) { return d == CC1D_F32 || d == CC1D_F16 || d == CC1D_BF16; }
 bool on_elements(const void *p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & ((uintptr_t)elem_bytes(dtype) - 1)) == 0; }
 
@@ -31,51 +32,67 @@ int check_delta(const cc1d_delta_params &p) {
     if (p.sequences < 0 || (p.cu_seqlens == nullptr ? p.sequences != p.batch : p.batch != 1)) return CC1D_ERR_SHAPE;
     if (p.batch > 0 && p.seqlen > 0 && p.v_heads > 0) st = check_inputs(p);
     if (st != CC1D_OK) return st;
+    if (p.saved != nullptr && !aligned256(p.saved)) return CC1D_ERR_WORKSPACE;
     if (!on_elements(p.initial_states, CC1D_F32) || !on_elements(p.final_states, CC1D_F32) || !on_elements(p.out, p.x_dtype)) return CC1D_ERR_ROW_LAYOUT;
     return CC1D_OK;
 }
 
 // Sequences of this many tokens on average go by chunks.
 constexpr int kChunkedFrom = 24;
+// The scans reach the 64 rows of a chunk with 32 bits.
+bool near(int dtype, int64_t stride) { return stride >= 0 && stride * elem_bytes(dtype) < ((int64_t)1 << 31) / kChunk; }
+bool reachable(const cc1d_delta_params &p) {
+    return near(p.x_dtype, p.v_stride_l) && near(p.x_dtype, p.out_stride_l);
+}
 bool chunked(const cc1d_delta_params &p) {
-    return p.batch > 0 && p.v_heads > 0 && p.sequences > 0 && p.seqlen >= (int64_t)kChunkedFrom * (p.cu_seqlens == nullptr ? 1 : p.sequences);
+    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return false;
+    return p.saved != nullptr || (reachable(p) && p.seqlen >= (int64_t)kChunkedFrom * (p.cu_seqlens == nullptr ? 1 : p.sequences));
 }
 
-// Places in the workspace; returns its size.
-size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWork &w) {
+struct Places {
+    uint8_t *base;
+    size_t used = 0;
+    uint8_t *take(size_t bytes) {
+        uint8_t *at = base + used;
+        used += (bytes + 255) / 256 * 256;
+        return at;
+    }
+};
+// Places in the workspace and in `saved`; returns the workspace's size.
+size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWork &w, size_t *saved_bytes = nullptr) {
     w = ChunkWork();
-    w.chunks = (p.seqlen + kChunk - 1) / kChunk;
-    w.slots = p.cu_seqlens == nullptr ? p.batch * w.chunks : p.seqlen / kChunk + p.sequences + 1;
+    w.chunks = (int32_t)(((int64_t)p.seqlen + kChunk - 1) / kChunk);
+    const int64_t slots = p.cu_seqlens == nullptr ? (int64_t)p.batch * w.chunks : (int64_t)p.seqlen / kChunk + p.sequences + 1;
+    w.slots = (int32_t)(slots < INT32_MAX ? slots : INT32_MAX);
     w.ks = key_steps(p.dim_k);
     w.terms = p.x_dtype == CC1D_BF16 ? 1 : p.x_dtype == CC1D_F16 ? 2 : 3;
     w.pterms = p.x_dtype == CC1D_F32 ? 3 : 2;
     w.backward = backward;
     const size_t keys = (size_t)w.slots * p.heads, values = (size_t)w.slots * p.v_heads;
-    size_t used = 0;
-    auto take = [&](size_t bytes) {
-        uint8_t *at = base + used;
-        used += (bytes + 255) / 256 * 256;
-        return at;
-    };
-    w.kf = take(keys * w.kbytes()); w.ktf = take(keys * w.kbytes());
-    w.tf = take(values * w.tbytes());
-    w.scalars = reinterpret_cast<float *>(take(values * kScalars * kChunk * sizeof(float)));
+    const size_t state = values * p.dim_k * p.dim_v * sizeof(float), rows = values * kChunk * p.dim_v * sizeof(float);
+    Places saved{static_cast<uint8_t *>(p.saved)};
+    w.s0 = reinterpret_cast<float *>(saved.take(state));
+    w.u = reinterpret_cast<float *>(saved.take(rows));
+    if (saved_bytes != nullptr) *saved_bytes = saved.used;
+    Places work{base};
+    w.kf = work.take(keys * w.kbytes());
+    w.ktf = work.take(keys * w.kbytes());
+    w.scalars = reinterpret_cast<float *>(work.take(values * kScalars * kChunk * sizeof(float)));
     if (backward) {
-        const size_t state = values * p.dim_k * p.dim_v * sizeof(float), rows = values * kChunk * p.dim_v * sizeof(float);
-        w.qtf = take(keys * w.kbytes()); w.ttf = take(values * w.tbytes()); w.ptf = take(values * w.tbytes());
-        w.s0 = reinterpret_cast<float *>(take(state)); w.ds1 = reinterpret_cast<float *>(take(state));
-        w.u = reinterpret_cast<float *>(take(rows)); w.dx = reinterpret_cast<float *>(take(rows));
+        w.qtf = work.take(keys * w.kbytes()); w.ttf = work.take(values * w.tbytes()); w.ptf = work.take(values * w.tbytes());
+        w.ds1 = reinterpret_cast<float *>(work.take(state));
+        w.dx = reinterpret_cast<float *>(work.take(rows));
     } else {
-        w.qf = take(keys * w.kbytes()); w.pf = take(values * w.pbytes());
+        w.qf = work.take(keys * w.kbytes());
+        w.tf = work.take(values * w.tbytes()); w.pf = work.take(values * w.pbytes());
     }
-    return used;
+    return work.used;
 }
 // Grids of one workgroup a (slot, value head) and of one a (sequence, value head, 16 columns).
 bool fits(const cc1d_delta_params &p, const ChunkWork &w) {
-    const int64_t limit = thread_limit() / kBlock;
+    const int64_t limit = thread_limit() / 512;
     return (int64_t)w.slots * p.v_heads < limit && ((int64_t)p.sequences * p.v_heads + 8) * ((p.dim_v + 15) / 16) < limit;
 }
-
 }  // namespace
 
 extern "C" {
@@ -95,21 +112,32 @@ int cc1d_delta_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     if (st != CC1D_OK || !chunked(*p)) return st;
     ChunkWork w;
     *bytes = lay_out(*p, false, nullptr, w);
-    return fits(*p, w) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    return fits(*p, w) && reachable(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+}
+
+int cc1d_delta_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
+    if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
+    *bytes = 0;
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const int st = check_delta(*p);
+    if (st != CC1D_OK || p->batch == 0 || p->v_heads == 0 || p->sequences == 0 || p->seqlen == 0) return st;
+    ChunkWork w;
+    lay_out(*p, false, nullptr, w, bytes);
+    return CC1D_OK;
 }
 
 int cc1d_delta_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
     size_t need = 0;
     const int st = cc1d_delta_workspace_bytes(p, &need);
     if (st != CC1D_OK) return st;
-    if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
+    if (need > 0 && (workspace == nullptr || !aligned256(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
     if (p->batch == 0 || p->v_heads == 0 || p->sequences == 0) return CC1D_OK;
     const hipStream_t hs = static_cast<hipStream_t>(stream);
     if (!chunked(*p)) return launch_delta_tokens(*p, nullptr, p->sequences, hs);
     ChunkWork w;
     lay_out(*p, false, static_cast<uint8_t *>(workspace), w);
     const int done = launch_delta_prep(*p, w, hs);
-    return done != CC1D_OK ? done : launch_delta_scan(*p, w, false, hs);
+    return done != CC1D_OK ? done : launch_delta_scan(*p, w, p->saved != nullptr, hs);
 }
 
 int cc1d_validate_delta_bwd(const cc1d_delta_bwd_params *p) {
@@ -118,7 +146,7 @@ int cc1d_validate_delta_bwd(const cc1d_delta_bwd_params *p) {
     if (st != CC1D_OK) return st;
     const cc1d_delta_params &f = p->fwd;
     if (f.batch > 0 && f.seqlen > 0 && f.v_heads > 0 &&
-        (p->dout == nullptr || p->dq == nullptr || p->dk == nullptr || p->dv == nullptr || p->dg == nullptr || p->dbeta == nullptr)) return CC1D_ERR_NULL_POINTER;
+        (f.saved == nullptr || p->dout == nullptr || p->dq == nullptr || p->dk == nullptr || p->dv == nullptr || p->dg == nullptr || p->dbeta == nullptr)) return CC1D_ERR_NULL_POINTER;
     if (!on_elements(p->dout, f.x_dtype) || !on_elements(p->dq, f.x_dtype) || !on_elements(p->dk, f.x_dtype) || !on_elements(p->dv, f.x_dtype) ||
         !on_elements(p->dg, f.g_dtype) || !on_elements(p->dbeta, f.beta_dtype) || !on_elements(p->dfinal_states, CC1D_F32) ||
         !on_elements(p->dinitial_states, CC1D_F32)) return CC1D_ERR_ROW_LAYOUT;
@@ -132,23 +160,21 @@ int cc1d_delta_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *bytes
     if (st != CC1D_OK || p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return st;
     ChunkWork w;
     *bytes = lay_out(p->fwd, true, nullptr, w);
-    return fits(p->fwd, w) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    const bool far = !near(p->fwd.x_dtype, p->dout_stride_l) || !near(p->fwd.x_dtype, p->dv_stride_l);
+    return fits(p->fwd, w) && !far ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_delta_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
     size_t need = 0;
     int st = cc1d_delta_bwd_workspace_bytes(p, &need);
     if (st != CC1D_OK) return st;
-    if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
+    if (need > 0 && (workspace == nullptr || !aligned256(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
     if (p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return CC1D_OK;
     const hipStream_t hs = static_cast<hipStream_t>(stream);
     ChunkWork w;
     lay_out(p->fwd, true, static_cast<uint8_t *>(workspace), w);
-    if (w.slots > 0) {
-        st = launch_delta_prep(p->fwd, w, hs);
-        if (st == CC1D_OK) st = launch_delta_scan(p->fwd, w, true, hs);
-        if (st != CC1D_OK) return st;
-    }
+    if (w.slots > 0) st = launch_delta_prep(p->fwd, w, hs);
+    if (st != CC1D_OK) return st;
     return launch_delta_bwd(*p, w, hs);
 }
 

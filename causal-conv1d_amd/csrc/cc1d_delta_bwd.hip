@@ -1,5 +1,5 @@
-// The gated delta rule by chunks, backward (cc1d_delta_chunk.hpp).  The states in front of the chunks and U are computed
-// again (prep and scan kernels); then, with dS1 the gradient of the state behind a chunk:
+// The gated delta rule by chunks, backward (cc1d_delta_chunk.hpp).  The states in front of the chunks and U come from the forward,
+// T and P are made again (prep kernel); then, with dS1 the gradient of the state behind a chunk:
 //
 //   scan, last chunk first:   dU = P^T dO + diag(dec) K dS1,  dX = T^T dU,  dV = diag(beta) dX
 //                             dS0 = gam_last dS1 + (scale diag(gam) Q)^T dO - (diag(gam beta) K)^T dX

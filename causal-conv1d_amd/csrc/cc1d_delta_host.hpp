@@ -13,10 +13,10 @@ struct ChunkWork;
 // Token by token.  initial_states / final_states of `p` are the states read and written, `slots` of them, picked by
 // `indices` (NULL: sequence n has state n).
 int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, hipStream_t stream);
-// By chunks: what needs no state; then the states and outputs (`states`: only the states in front of the chunks and U).
+// By chunks: what needs no state; then the states and outputs (`save`: the states in front of the chunks and U are kept).
 int launch_delta_prep(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream);
-int launch_delta_scan(const cc1d_delta_params &p, const ChunkWork &w, bool states, hipStream_t stream);
-// Backward behind both (of a ChunkWork laid out for it): the gradients.
+int launch_delta_scan(const cc1d_delta_params &p, const ChunkWork &w, bool save, hipStream_t stream);
+// Backward, behind its own prep: the gradients.
 int launch_delta_bwd(const cc1d_delta_bwd_params &p, const ChunkWork &w, hipStream_t stream);
 
 // Every row of a (batch, seqlen, heads, dim) tensor starts on 16 bytes.
@@ -27,10 +27,6 @@ inline bool whole_rows(int dtype, const void *x, int64_t sb, int64_t sl, int64_t
 
 // 32-column steps of dim_k that have kernels.
 inline int key_steps(int dim_k) { return dim_k <= 32 ? 1 : dim_k <= 64 ? 2 : dim_k <= 128 ? 4 : 8; }
-
-// Workgroups of the scans take 32 columns of a state instead of 16 where that leaves one for every CU: the operands that a chunk's
-// columns share are then read half as often.
-inline bool wide_columns(const cc1d_delta_params &p) { return (int64_t)p.sequences * p.v_heads * ((p.dim_v + 31) / 32) >= 256; }
 
 template <typename F>
 int by_type_and_steps(int dtype, int steps, F &&f) {

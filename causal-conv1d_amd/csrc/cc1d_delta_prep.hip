@@ -15,11 +15,13 @@ constexpr int kPitch = 68;               // floats of a row of a 64 x 64 matrix 
 
 template <int DT, int KS>
 struct PrepLds {
-    uint8_t frags[4 * KS * Terms<DT>::n * kFrag];        // K, later Q
-    float a[kChunk][kPitch], t[kChunk][kPitch];
+    union {
+        uint8_t frags[4 * KS * Terms<DT>::n * kFrag];    // K, then Q; then T
+        float t[kChunk][kPitch];
+    };
+    float a[kChunk][kPitch];
     float scratch[4][16][17];
     float gate[kScalars][kChunk];
-    double sums[kChunk];
     float norms[2][kChunk];
 };
 
@@ -147,7 +149,45 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
             read[ct][e] = i >= j ? r[e] * decay * (p.scale * lds.gate[kQueryNorm][i]) : 0.f;
         }
     }
-    lds_barrier();
+    // K^T, then Q^T, gathered from the operands in LDS: token 32 s + 8 g + e is row m' of tile ct, dim_k index k is
+    // element k & 7 of lane group (k >> 3) & 3 of step k >> 5.
+    auto transposed = [&](uint8_t *dst) {
+#pragma unroll
+        for (int i = 0; i < (2 * KS + 3) / 4; ++i) {
+            const int t = wave + 4 * i;
+            if (t >= 2 * KS) break;
+            const int k = row_of(t, m);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint16_t x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int ct = 2 * s + (e >> 2), mm = 4 * g + (e & 3);
+                        x[e] = *reinterpret_cast<const uint16_t *>(lds.frags + ((ct * KS + (k >> 5)) * NT + n) * kFrag + (((k >> 3) & 3) * 16 + mm) * 16 + (k & 7) * 2);
+                    }
+                    u32x4 f;
+                    f.x = x[0] | (uint32_t)x[1] << 16; f.y = x[2] | (uint32_t)x[3] << 16;
+                    f.z = x[4] | (uint32_t)x[5] << 16; f.w = x[6] | (uint32_t)x[7] << 16;
+                    *reinterpret_cast<u32x4 *>(dst + ((t * 2 + s) * NT + n) * kFrag + lane * 16) = f;
+                }
+        }
+    };
+    if (first) {
+        transposed(w.ktf + sh * w.kbytes());
+        if (w.backward) {
+            lds_barrier();
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
+            lds_barrier();
+            transposed(w.qtf + sh * w.kbytes());
+        }
+    }
+    lds_barrier();                                       // T goes where the operands were
 
     // T.  Diagonal blocks: lane = column.
     {
@@ -186,8 +226,9 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
         lds_barrier();
     }
 
-    // T and its transpose as left operands.
-    for (int s = 0; s <= (wave >> 1); ++s) {
+    // T or, for the backward, its transpose as left operands.
+    if (!w.backward)
+        for (int s = 0; s <= (wave >> 1); ++s) {
         float x[8];
         bf16x8 f[3];
 #pragma unroll
@@ -236,42 +277,6 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
             for (int n = 0; n < 3; ++n)
                 *reinterpret_cast<u32x4 *>(w.ptf + sv * w.tbytes() + (upper_frag(wave, s) * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
         }
-    if (!first) return;
-    // K^T, then Q^T, gathered from the operands in LDS: token 32 s + 8 g + e is row m' of tile ct, dim_k index k is
-    // element k & 7 of lane group (k >> 3) & 3 of step k >> 5.
-    auto transposed = [&](uint8_t *dst) {
-#pragma unroll
-        for (int i = 0; i < (2 * KS + 3) / 4; ++i) {
-            const int t = wave + 4 * i;
-            if (t >= 2 * KS) break;
-            const int k = row_of(t, m);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint16_t x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int ct = 2 * s + (e >> 2), mm = 4 * g + (e & 3);
-                        x[e] = *reinterpret_cast<const uint16_t *>(lds.frags + ((ct * KS + (k >> 5)) * NT + n) * kFrag + (((k >> 3) & 3) * 16 + mm) * 16 + (k & 7) * 2);
-                    }
-                    u32x4 f;
-                    f.x = x[0] | (uint32_t)x[1] << 16; f.y = x[2] | (uint32_t)x[3] << 16;
-                    f.z = x[4] | (uint32_t)x[5] << 16; f.w = x[6] | (uint32_t)x[7] << 16;
-                    *reinterpret_cast<u32x4 *>(dst + ((t * 2 + s) * NT + n) * kFrag + lane * 16) = f;
-                }
-        }
-    };
-    transposed(w.ktf + sh * w.kbytes());
-    if (!w.backward) return;
-    lds_barrier();
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
-    lds_barrier();
-    transposed(w.qtf + sh * w.kbytes());
 }
 
 template <int DT, int KS, bool VEC>

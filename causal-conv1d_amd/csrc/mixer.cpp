@@ -101,8 +101,9 @@ cc1d_delta_params delta_params(const DeltaInputs &d, const OptTensor &init, cons
     return p;
 }
 
-at::Tensor delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
-                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm) {
+// (out, saved): saved is what the backward needs of the forward, empty if not wanted.
+std::tuple<at::Tensor, at::Tensor> delta_fwd_run(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm, bool save) {
     const DeltaInputs d = delta_inputs(q, k, v, g, beta);
     OptTensor init = initial_states;
     if (init.has_value()) init = rows_of(*init);
@@ -117,23 +118,42 @@ at::Tensor delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor 
         p.final_states = f.data_ptr<float>(); SET_STATE(p, final, f);
     }
     size_t bytes = 0;
+    at::Tensor saved;
+    if (save) {
+        check_status(cc1d_delta_saved_bytes(&p, &bytes), "gated_delta_rule");
+        saved = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+        p.saved = bytes ? saved.data_ptr() : nullptr;
+    }
     check_status(cc1d_delta_workspace_bytes(&p, &bytes), "gated_delta_rule");
     const at::Tensor ws = workspace_of(bytes, q);
     check_status(cc1d_delta_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "gated_delta_rule");
-    return out;
+    return {out, saved};
+}
+at::Tensor delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm) {
+    return std::get<0>(delta_fwd_run(q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, qk_l2norm, false));
+}
+std::tuple<at::Tensor, at::Tensor> delta_fwd_save(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm) {
+    return delta_fwd_run(q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, qk_l2norm, true);
 }
 
 // dq, dk, dv, dg, dbeta in their inputs' types, and dinitial_states (empty if not wanted).
 using Gradients6 = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 Gradients6 delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
-                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const at::Tensor &dout_, const OptTensor &dfinal_states,
-                     double scale, bool qk_l2norm, bool want_dinitial) {
+                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const at::Tensor &saved, const at::Tensor &dout_,
+                     const OptTensor &dfinal_states, double scale, bool qk_l2norm, bool want_dinitial) {
     const DeltaInputs d = delta_inputs(q, k, v, g, beta);
     OptTensor init = initial_states, dfinal = dfinal_states;
     if (init.has_value()) init = rows_of(*init);
     c10::DeviceGuard guard(q.device());
     cc1d_delta_bwd_params p = {};
     p.fwd = delta_params(d, init, cu_seqlens, scale, qk_l2norm);
+    size_t bytes = 0;
+    check_status(cc1d_delta_saved_bytes(&p.fwd, &bytes), "gated_delta_rule backward");
+    check_gpu(saved, q, "saved");
+    TORCH_CHECK(saved.is_contiguous() && saved.nbytes() >= bytes, "saved is not what the forward returned for these sizes");
+    p.fwd.saved = bytes ? saved.data_ptr() : nullptr;
     check_gpu(dout_, q, "dout");
     TORCH_CHECK(dout_.sizes() == v.sizes() && dout_.scalar_type() == v.scalar_type(), "dout must have the shape and dtype of v");
     const at::Tensor dout = rows_of(dout_);
@@ -151,7 +171,6 @@ Gradients6 delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor 
     p.dg = dg.data_ptr(); p.dbeta = dbeta.data_ptr();
     at::Tensor dinit = want_dinitial ? at::empty({p.fwd.sequences, d.v_heads, d.dim_k, d.dim_v}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
     if (want_dinitial) { p.dinitial_states = dinit.data_ptr<float>(); SET_STATE(p, dinit, dinit); }
-    size_t bytes = 0;
     check_status(cc1d_delta_bwd_workspace_bytes(&p, &bytes), "gated_delta_rule backward");
     const at::Tensor ws = workspace_of(bytes, q);
     check_status(cc1d_delta_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "gated_delta_rule backward");
@@ -189,8 +208,17 @@ at::Tensor delta_fwd_meta(const at::Tensor &, const at::Tensor &, const at::Tens
                           const OptTensor &, const OptTensor &, const OptTensor &, double, bool) {
     return at::empty_symint(v.sym_sizes(), v.options());
 }
+// How many bytes are saved shows only in the sizes that the kernel library lays out: the same sum.
+std::tuple<at::Tensor, at::Tensor> delta_fwd_save_meta(const at::Tensor &q, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const at::Tensor &,
+                          const OptTensor &, const OptTensor &cu, const OptTensor &, double, bool) {
+    const c10::SymInt chunks = (q.sym_size(1) + 63) / 64;
+    const c10::SymInt slots = cu.has_value() ? q.sym_size(1) / 64 + cu->sym_size(0) : q.sym_size(0) * chunks;
+    const c10::SymInt one = slots * v.sym_size(2) * v.sym_size(3) * 4, up = 255;
+    const c10::SymInt bytes = (one * q.sym_size(3) + up) / 256 * 256 + (one * 64 + up) / 256 * 256;
+    return {at::empty_symint(v.sym_sizes(), v.options()), at::empty_symint({bytes}, q.options().dtype(at::kByte))};
+}
 Gradients6 delta_bwd_meta(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
-                          const OptTensor &, const OptTensor &cu, const at::Tensor &, const OptTensor &, double, bool, bool want_dinitial) {
+                          const OptTensor &, const OptTensor &cu, const at::Tensor &, const at::Tensor &, const OptTensor &, double, bool, bool want_dinitial) {
     auto like = [](const at::Tensor &t) { return at::empty_symint(t.sym_sizes(), t.options()); };
     const c10::SymInt n = cu.has_value() ? cu->sym_size(0) - 1 : q.sym_size(0);
     const auto f32 = q.options().dtype(at::kFloat);
@@ -345,8 +373,10 @@ at::Tensor dequantize_meta(const at::Tensor &y8, const at::Tensor &, at::ScalarT
 TORCH_LIBRARY_FRAGMENT(DaoAILab, m) {
     m.def("_gated_delta_rule_fwd_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? initial_states, "
           "Tensor? cu_seqlens, Tensor(a!)? final_states_out, float scale, bool qk_l2norm) -> Tensor", {at::Tag::pt2_compliant_tag});
+    m.def("_gated_delta_rule_fwd_save_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? initial_states, "
+          "Tensor? cu_seqlens, Tensor(a!)? final_states_out, float scale, bool qk_l2norm) -> (Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
     m.def("_gated_delta_rule_bwd_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? initial_states, Tensor? cu_seqlens, "
-          "Tensor dout, Tensor? dfinal_states, float scale, bool qk_l2norm, bool want_dinitial) "
+          "Tensor saved, Tensor dout, Tensor? dfinal_states, float scale, bool qk_l2norm, bool want_dinitial) "
           "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
     m.def("_gated_delta_rule_update_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor(a!) state, "
           "Tensor? state_indices, float scale, bool qk_l2norm) -> Tensor", {at::Tag::pt2_compliant_tag});
@@ -358,6 +388,7 @@ TORCH_LIBRARY_FRAGMENT(DaoAILab, m) {
 
 TORCH_LIBRARY_IMPL(DaoAILab, CompositeExplicitAutograd, m) {
     m.impl("_gated_delta_rule_fwd_cpp", &delta_fwd);
+    m.impl("_gated_delta_rule_fwd_save_cpp", &delta_fwd_save);
     m.impl("_gated_delta_rule_bwd_cpp", &delta_bwd);
     m.impl("_gated_delta_rule_update_cpp", &delta_update);
     m.impl("_rms_norm_fwd_cpp", &norm_fwd);
@@ -368,6 +399,7 @@ TORCH_LIBRARY_IMPL(DaoAILab, CompositeExplicitAutograd, m) {
 
 TORCH_LIBRARY_IMPL(DaoAILab, Meta, m) {
     m.impl("_gated_delta_rule_fwd_cpp", &delta_fwd_meta);
+    m.impl("_gated_delta_rule_fwd_save_cpp", &delta_fwd_save_meta);
     m.impl("_gated_delta_rule_bwd_cpp", &delta_bwd_meta);
     m.impl("_gated_delta_rule_update_cpp", &delta_update_meta);
     m.impl("_rms_norm_fwd_cpp", &norm_fwd_meta);

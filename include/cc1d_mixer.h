@@ -61,14 +61,19 @@ typedef struct cc1d_delta_params {
     int64_t out_stride_b, out_stride_l, out_stride_h;
     float *final_states;             /* like initial_states (may be the same tensor), or NULL */
     int64_t final_stride_n, final_stride_h, final_stride_k;
+    void *saved;                     /* NULL, or cc1d_delta_saved_bytes() of device memory, 256-byte aligned: what the
+                                        backward needs of the forward (the state in front of every 64 tokens, and what
+                                        they added to it), written by cc1d_delta_fwd, read by cc1d_delta_bwd */
 } cc1d_delta_params;
 
 int cc1d_validate_delta(const cc1d_delta_params *p);
 /* Device memory the forward works in: 256-byte aligned, needs no initialisation, may be 0 bytes. */
 int cc1d_delta_workspace_bytes(const cc1d_delta_params *p, size_t *bytes);
+int cc1d_delta_saved_bytes(const cc1d_delta_params *p, size_t *bytes);
 int cc1d_delta_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream);
 
-/* Backward.  `fwd.out` and `fwd.final_states` are ignored: the states are computed again. */
+/* Backward.  `fwd` is the forward's block: `saved` is needed, `out` and `final_states` are ignored.  Tokens more than 2^25 bytes
+ * apart (in v, out, dout or dv) are refused with CC1D_ERR_TOO_LARGE here and where `saved` is given to the forward. */
 typedef struct cc1d_delta_bwd_params {
     cc1d_delta_params fwd;
     const void *dout;                /* (batch, seqlen, v_heads, dim_v) of x_dtype, unit stride along dim_v */
