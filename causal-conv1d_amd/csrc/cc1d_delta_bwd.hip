@@ -279,8 +279,9 @@ struct GradLds {
 
 // Every chunk's gradients alone.  Eight wavefronts: 16 tokens' rows of dQ, Z and Y each, of one half of dim_k; of X1 the first
 // four, of X2 the others.  S0, dS1 and U pass through LDS once for all of them, 32 columns of dim_v at a time, split into their
-// terms.  VEC: rows of v and dout are whole 16-byte vectors, rows of the fp32 matrices in the workspace too.
-template <int DT, int KS, bool VEC>
+// terms.  VEC: rows of v and dout are whole 16-byte vectors, rows of the fp32 matrices in the workspace too.  SHARED: several value
+// heads have these keys (one: their sums need no registers through the walk).
+template <int DT, int KS, bool VEC, bool SHARED>
 __global__ void __launch_bounds__(kGradBlock, 1)
 delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int vec_out) {
     using T = typename Elem<DT>::type;
@@ -292,7 +293,7 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tile = wave & 3, side = wave >> 2;
     const int slot = (int)(blockIdx.x / (uint32_t)p.heads), hk = (int)(blockIdx.x % (uint32_t)p.heads);
-    const int group = p.v_heads / p.heads;
+    const int group = SHARED ? p.v_heads / p.heads : 1;
     const ChunkAt at = chunk_at(p, w, slot);
     T *dq = static_cast<T *>(bp.dq) + hk * bp.dq_stride_h, *dk = static_cast<T *>(bp.dk) + hk * bp.dk_stride_h;
     if (p.cu_seqlens != nullptr && slot == 0) {          // tokens in front of the first sequence and behind the last
@@ -390,7 +391,9 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
 #pragma unroll
                 for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4 *>(lds.stage.ds1 + (t * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(fs[n]);
             }
+            stay();
             if (v0 + 32 < p.dim_v) ask(c + 32);
+            stay();
             lds_barrier();
             load_frag<3>(lds.stage.x + tile * 3 * kFrag, lane, fx);
             load_frag<3>(lds.stage.u + tile * 3 * kFrag, lane, fu);
@@ -400,6 +403,7 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
                     bf16x8 b[3];
                     load_frag<3>(lds.stage.u + t * 3 * kFrag, lane, b);
                     x[t] = side == 0 ? product<2>(fo, b, x[t]) : product<2>(fx, b, x[t]);
+                    stay();
                 }
             const uint8_t *sl = lds.stage.s0 + side * TILES * 3 * kFrag, *dl = lds.stage.ds1 + side * TILES * 3 * kFrag;
 #pragma unroll
@@ -410,6 +414,7 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
                 aq[t] = product<2>(fo, b, aq[t]);
                 az[t] = product<2>(fx, b, az[t]);
                 ay[t] = product<2>(fu, d, ay[t]);
+                stay();
             }
         }
         // K^T and Q^T of the half of the chunk that holds this wavefront's own tokens.
@@ -499,9 +504,12 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
             }
         };
         row_products(half);
+        stay();
         column_products(half);
+        stay();
         ask_kq(1 - half);
         if (half == 0) column_products(1); else row_products(0);
+        stay();
         ask_kq(half);
         float qd[4] = {0.f, 0.f, 0.f, 0.f}, kz[4] = {0.f, 0.f, 0.f, 0.f}, ky[4] = {0.f, 0.f, 0.f, 0.f};
         {
@@ -639,8 +647,11 @@ int launch(const cc1d_delta_bwd_params &bp, const ChunkWork &w, hipStream_t stre
     const int vec_out = whole_rows(p.x_dtype, bp.dq, bp.dq_stride_b, bp.dq_stride_l, bp.dq_stride_h) &&
                         whole_rows(p.x_dtype, bp.dk, bp.dk_stride_b, bp.dk_stride_l, bp.dk_stride_h);
     const dim3 grid((uint32_t)((int64_t)w.slots * p.heads));
-    if (vec) CC1D_LAUNCH((delta_grad_kernel<DT, KS, true>), grid, dim3(kGradBlock), sizeof(GradLds<KS>), stream, bp, w, vec_out);
-    else CC1D_LAUNCH((delta_grad_kernel<DT, KS, false>), grid, dim3(kGradBlock), sizeof(GradLds<KS>), stream, bp, w, vec_out);
+    auto go = [&](auto v, auto shared) {
+        CC1D_LAUNCH((delta_grad_kernel<DT, KS, decltype(v)::value, decltype(shared)::value>), grid, dim3(kGradBlock), sizeof(GradLds<KS>), stream, bp, w, vec_out);
+    };
+    auto either = [&](auto v) { p.v_heads > p.heads ? go(v, std::true_type()) : go(v, std::false_type()); };
+    vec ? either(std::true_type()) : either(std::false_type());
     return launch_status();
 }
 
