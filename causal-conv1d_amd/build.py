@@ -47,7 +47,7 @@ KERNEL_HEADERS = ["cc1d_device.hpp", "cc1d_internal.hpp", "cc1d_bwd_channellast_
 DELTA_HEADERS = ["cc1d_delta.hpp", "cc1d_delta_chunk.hpp", "cc1d_delta_host.hpp"]   # of the sources that begin with cc1d_delta
 PUBLIC_HEADERS = ["cc1d.h", "cc1d_mixer.h"]
 BINDING_SOURCES = ["causal_conv1d.cpp", "mixer.cpp"]
-BINDING_HEADERS = ["cc1d_torch.hpp"]
+BINDING_HEADERS = ["cc1d_torch.hpp", "cc1d_torch_calls.hpp"]
 
 LIB_NAME = "libcc1d.so"
 EXT_NAME = "causal_conv1d_cuda" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so")

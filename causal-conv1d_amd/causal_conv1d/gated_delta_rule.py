@@ -18,8 +18,9 @@ are, so q, k and v may be column slices of the channel-last convolution's output
 There is no host path.  `gated_delta_rule_ref` states the operator in plain PyTorch.
 """
 import torch
+from torch.compiler import is_compiling
 
-import causal_conv1d_cuda as _ext  # noqa: F401  (loading it registers the ops)
+import causal_conv1d_cuda as _ext              # loading it registers the ops
 
 _fwd = torch.ops.DaoAILab._gated_delta_rule_fwd_cpp
 _fwd_save = torch.ops.DaoAILab._gated_delta_rule_fwd_save_cpp
@@ -67,6 +68,11 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_states=None, retur
     final_states_out if given (which may be initial_states itself; without gradients only).
     cu_seqlens (sequences + 1,) int32 or int64, ascending from 0 to seqlen, with a batch of 1: sequence n is tokens
     cu_seqlens[n] .. cu_seqlens[n+1]-1; a sequence may be empty."""
+    if not is_compiling():
+        res = _ext._gated_delta_rule_call(q, k, v, g, beta, scale, initial_states, return_final_states, final_states_out,
+                                          cu_seqlens, qk_l2norm)
+        if res is not NotImplemented:
+            return res
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if cu_seqlens is not None:
@@ -90,6 +96,10 @@ def gated_delta_rule_update(q, k, v, g, beta, state, scale=None, state_indices=N
     behind the batch, for a few tokens at once.  state (slots, v_heads, dim_k, dim_v) float32.
     state_indices (batch,) int32: entry b uses state[state_indices[b]]; a negative index gives zeros and leaves
     every state alone.  No slot may be named twice."""
+    if not is_compiling():
+        res = _ext._gated_delta_rule_update_call(q, k, v, g, beta, state, state_indices, scale, qk_l2norm)
+        if res is not NotImplemented:
+            return res
     if scale is None:
         scale = q.shape[-1] ** -0.5
     return _update(q, k, v, g, beta, state, state_indices, float(scale), qk_l2norm)

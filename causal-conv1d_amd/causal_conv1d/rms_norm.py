@@ -9,8 +9,9 @@ computed.  x and residual are (..., dim); residual and weight are each of x's dt
 `rms_norm_ref` states the operator in plain PyTorch.
 """
 import torch
+from torch.compiler import is_compiling
 
-import causal_conv1d_cuda as _ext  # noqa: F401  (loading it registers the ops)
+import causal_conv1d_cuda as _ext              # loading it registers the ops
 
 _fwd = torch.ops.DaoAILab._rms_norm_fwd_cpp
 _bwd = torch.ops.DaoAILab._rms_norm_bwd_cpp
@@ -47,6 +48,10 @@ class RMSNormFn(torch.autograd.Function):
 
 def rms_norm_fn(x, weight, residual=None, eps=1e-5):
     """y, or (y, h) with a residual; y has x's dtype, h = x + residual has residual's."""
+    if not is_compiling():
+        res = _ext._rms_norm_call(x, weight, residual, eps)
+        if res is not NotImplemented:
+            return res
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         return RMSNormFn.apply(x, weight, residual, eps)
     y, h = _fwd(x, weight, residual, eps)
@@ -56,12 +61,20 @@ def rms_norm_fn(x, weight, residual=None, eps=1e-5):
 def rms_norm_quant_fn(x, weight, residual=None, eps=1e-5):
     """(y8, scales), or (y8, scales, h) with a residual: y8 (..., dim) float8_e4m3fn, scales (...) float32 with
     y = y8 * scales[..., None] and scales = max|y| / 448 of each row.  No backward."""
+    if not is_compiling():
+        res = _ext._rms_norm_quant_call(x, weight, residual, eps)
+        if res is not NotImplemented:
+            return res
     y8, scales, h = _quant(x.detach(), weight.detach(), None if residual is None else residual.detach(), eps)
     return (y8, scales) if residual is None else (y8, scales, h)
 
 
 def dequantize_rows(y8, scales, dtype=torch.bfloat16):
     """y8 (..., dim) float8_e4m3fn times scales (...), as `dtype`.  No backward."""
+    if not is_compiling():
+        res = _ext._dequantize_rows_call(y8, scales, dtype)
+        if res is not NotImplemented:
+            return res
     return _dequantize(y8, scales, dtype)
 
 

@@ -27,7 +27,7 @@
 #include <optional>
 
 #include "cc1d.h"
-#include "cc1d_torch.hpp"
+#include "cc1d_torch_calls.hpp"
 
 namespace {
 
@@ -463,14 +463,6 @@ void update_meta(const at::Tensor &, at::Tensor &, const at::Tensor &, const std
 // Each returns NotImplemented, having done nothing, for what the generic path in Python has to
 // handle: tensor subclasses, torch-function modes, tracing, arguments of other types or that still need a copy.
 
-bool plain(PyObject *o) { return THPVariable_CheckExact(o); }
-bool plain_or_none(PyObject *o) { return o == Py_None || plain(o); }
-std::optional<at::Tensor> optional_tensor(PyObject *o) {
-    return o == Py_None ? std::optional<at::Tensor>() : std::optional<at::Tensor>(THPVariable_Unpack(o));
-}
-bool generic_path_needed() {
-    return at::impl::torch_function_mode_enabled() || torch::jit::tracer::isTracing();
-}
 // Unit stride along seqlen or along dim.
 bool kernel_layout(const at::Tensor &t) { return t.dim() == 3 && (t.stride(1) == 1 || t.stride(2) == 1); }
 bool contiguous_or_none(const std::optional<at::Tensor> &t) { return !t.has_value() || t->is_contiguous(); }
@@ -479,13 +471,6 @@ bool contiguous_or_none(const std::optional<at::Tensor> &t) { return !t.has_valu
 at::Tensor states_like(const at::Tensor &x, int64_t width) {
     return at::empty({x.size(0), width - 1, x.size(1)}, x.options()).transpose(1, 2);
 }
-
-template <typename F>
-auto typed_op(const char *name) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
-}
-
-#define NOT_IMPLEMENTED() do { Py_INCREF(Py_NotImplemented); return Py_NotImplemented; } while (0)
 
 // (x, conv_state, weight, bias, silu, cache_seqlens, conv_state_indices) -> out
 PyObject *update_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -507,9 +492,6 @@ PyObject *update_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-bool functorch_active() {
-    return c10::impl::tls_local_dispatch_key_set().included_.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
-}
 // Real GPU memory that nobody watches being allocated: no fake tensor, dispatch mode or functorch transform.
 bool allocates_plainly(const at::Tensor &x) {
     return x.is_cuda() && !x.unsafeGetTensorImpl()->is_python_dispatch() && !c10::impl::TorchDispatchModeTLS::any_modes_set() && !functorch_active();
@@ -616,9 +598,6 @@ void register_node() {
 template <int... HOW>
 void register_nodes(std::integer_sequence<int, HOW...>) { (register_node<HOW>(), ...); }
 
-// What only the Python function answers for: functorch transforms and forward-mode gradients, which it refuses in its own words.
-bool python_graph_needed(const std::optional<at::Tensor> &t) { return t.has_value() && (t->has_names() || t->_fw_grad(0).defined()); }
-
 // (x, weight, bias, seq_idx, initial_states, return_final_states, final_states_out, silu)
 // -> out or (out, final_states), with their graph where gradients are wanted.  Tensors that still need a copy
 // into a layout of the kernels, and combinations that the Python layer refuses, are left to it.
@@ -711,7 +690,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("causal_conv1d_fwd_varlen_states", &causal_conv1d_fwd_varlen_states,
           "Causal conv1d forward and varlen final-state gather in one call");
     register_nodes(std::make_integer_sequence<int, (int)std::size(recorders)>{});
-    if (PyModule_AddFunctions(m.ptr(), direct_calls) != 0) throw pybind11::error_already_set();
+    if (PyModule_AddFunctions(m.ptr(), direct_calls) != 0 || PyModule_AddFunctions(m.ptr(), mixer_direct_calls()) != 0) throw pybind11::error_already_set();
 }
 
 TORCH_LIBRARY_FRAGMENT(DaoAILab, m) {
