@@ -39,6 +39,14 @@ __device__ __forceinline__ float load_as_float(const void *p, int64_t i, int dty
     if (dtype == CC1D_F16) return (float)static_cast<const _Float16 *>(p)[i];
     return (float)static_cast<const __bf16 *>(p)[i];
 }
+// The same in two halves, the load and what waits for it.
+__device__ __forceinline__ uint32_t load_bits(const void *p, int64_t i, int dtype) {
+    return dtype == CC1D_F32 ? static_cast<const uint32_t *>(p)[i] : (uint32_t)static_cast<const uint16_t *>(p)[i];
+}
+__device__ __forceinline__ float bits_as_float(uint32_t bits, int dtype) {
+    if (dtype == CC1D_F16) return (float)bitcast<_Float16>((uint16_t)bits);
+    return bitcast<float>(dtype == CC1D_F32 ? bits : bits << 16);
+}
 __device__ __forceinline__ void store_from_float(void *p, int64_t i, int dtype, float v) {
     if (dtype == CC1D_F32) static_cast<float *>(p)[i] = v;
     else if (dtype == CC1D_F16) static_cast<_Float16 *>(p)[i] = (_Float16)v;

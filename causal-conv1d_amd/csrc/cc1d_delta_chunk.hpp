@@ -200,26 +200,6 @@ __device__ __forceinline__ void load_frag(const uint8_t *base, int lane, bf16x8 
     for (int n = 0; n < N; ++n) f[n] = bitcast<bf16x8>(*reinterpret_cast<const u32x4 *>(base + n * kFrag + lane * 16));
 }
 
-// The same for R left operands against one right one; products of different rows follow each other, so none waits for its own sum.
-template <int MOST, int R, int NA, int NB>
-__device__ __forceinline__ void products(const bf16x8 (&a)[R][NA], const bf16x8 (&b)[NB], f32x4 *acc) {
-#pragma unroll
-    for (int sum = MOST; sum >= 0; --sum)
-#pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int j = sum - i;
-            if (j < 0 || j >= NB) continue;
-#pragma unroll
-            for (int r = 0; r < R; ++r) acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[r][i], b[j], acc[r], 0, 0, 0);
-        }
-}
-// The right operand that two result tiles are.
-template <int N>
-__device__ __forceinline__ void as_operand(const f32x4 &a, const f32x4 &b, bf16x8 (&t)[N]) {
-    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    split8<N>(x, t);
-}
-
 // Two accumulators, the largest products in one and the rest in the other: two chains of instructions that do not wait for each other.
 template <int MOST, int NA, int NB>
 __device__ __forceinline__ void product2(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 &large, f32x4 &rest) {
@@ -245,17 +225,6 @@ __device__ __forceinline__ void four_of(const bf16x8 (&t)[N], bool upper, float 
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = n == N - 1 ? x[i] : f[i] + x[i];
     }
-}
-
-// Loads stay between the products where they are written: bunched, or moved, they hold the wavefront up while the
-// address unit works them off, 16 cycles each.
-__device__ __forceinline__ void stay() { __builtin_amdgcn_sched_barrier(0); }
-
-// A barrier that orders LDS alone: loads and stores of global memory stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 }  // namespace cc1d

@@ -8,7 +8,9 @@
 // row of the state moves as whole 128-byte lines.  q and k go through LDS once, normalised, in fp32.  Both
 // products of a token are formed before its update, out = D^T q + (k.q) u, so that one reduction over the
 // lane groups serves both.  In a decode step nothing is computed worth mentioning: the state, read and written
-// once, is the floor.
+// once, is the floor.  It is read and written past the caches (nothing reads it before the next step): 96 states of
+// 32 heads of 128 x 128 take 73 us, 5.5 TB/s, and 100 through the caches; one request 7.5 us and 10, since no line is
+// left to be written back when the kernel ends.  Four wavefronts to a workgroup: 73 us, one 83.
 #include "cc1d_delta.hpp"
 #include "cc1d_delta_host.hpp"
 
@@ -26,37 +28,18 @@ struct StepArgs {
 };
 
 template <int DT>
-__device__ __forceinline__ void load4(const void *base, int64_t at, int n, bool vec, float (&f)[4]) {
+struct alignas(4 * sizeof(typename Elem<DT>::type)) Row4 { typename Elem<DT>::type x[4]; };
+
+// Four adjacent elements as they lie in memory; where rows are not whole vectors one by one, the first for those behind `cols`.
+template <int DT>
+__device__ __forceinline__ Row4<DT> load4(const void *base, int64_t at, int cols, bool vec) {
     using T = typename Elem<DT>::type;
     const T *x = static_cast<const T *>(base) + at;
-    if (vec) {
-        if (DT == CC1D_F32) {
-            const float4 r = *reinterpret_cast<const float4 *>(x);
-            f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
-        } else {
-            const u32x2 r = *reinterpret_cast<const u32x2 *>(x);
+    if (vec) return *reinterpret_cast<const Row4<DT> *>(x);
+    Row4<DT> r;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t w = i < 2 ? r.x : r.y;
-                const uint16_t h = (uint16_t)(i & 1 ? w >> 16 : w & 0xffffu);
-                f[i] = Elem<DT>::to_float(bitcast<T>(h));
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = i < n ? Elem<DT>::to_float(x[i]) : 0.f;
-}
-template <>
-__device__ __forceinline__ void load4<CC1D_F32>(const void *base, int64_t at, int n, bool vec, float (&f)[4]) {
-    const float *x = static_cast<const float *>(base) + at;
-    if (vec) {
-        const float4 r = *reinterpret_cast<const float4 *>(x);
-        f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = i < n ? x[i] : 0.f;
+    for (int i = 0; i < 4; ++i) r.x[i] = x[i < cols ? i : 0];
+    return r;
 }
 
 // KR: rows of the state a lane holds, dim_k <= 8 KR.
@@ -98,39 +81,74 @@ delta_step_kernel(const StepArgs a) {
         return;
     }
 
-    float s[KR][4];
-    const float *src = p.initial_states == nullptr ? nullptr : p.initial_states + slot * p.init_stride_n + h * p.init_stride_h;
-#pragma unroll
-    for (int i = 0; i < KR; ++i) {
-        const int row = rg * KR + i;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-        if (src != nullptr && row < p.dim_k && cols > 0) load4<CC1D_F32>(src, row * p.init_stride_k + c0, cols, a.vec_state, s[i]);
-    }
-
-    float *kq = &lds[wave][0][0], *qq = &lds[wave][1][0];
+    // Every load is made without a condition, of a place inside the tensor where the lane's own lies outside: a load behind
+    // a branch is waited for before the next.  The token's own loads go out in front of the state's, and are summed while
+    // those travel; the next token's in front of a token's products.
     constexpr int NE = (8 * KR + 63) / 64;               // elements of k and q a lane fetches
-    for (int64_t t = range.lo; t < range.hi; ++t) {
+    const int cc = cols > 0 ? c0 : 0;                    // lanes behind the last column repeat the first, and store nothing
+    struct Token { T k[NE], q[NE]; Row4<DT> v; uint32_t g, beta; };
+    auto ask = [&](int64_t t) {
+        Token x;
         const T *qp = static_cast<const T *>(p.q) + range.b * p.q_stride_b + t * p.q_stride_l + hk * p.q_stride_h;
         const T *kp = static_cast<const T *>(p.k) + range.b * p.k_stride_b + t * p.k_stride_l + hk * p.k_stride_h;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            const int i = lane + 64 * e < p.dim_k ? lane + 64 * e : 0;
+            x.k[e] = kp[i];
+            x.q[e] = qp[i];
+        }
+        x.g = load_bits(p.g, range.b * p.g_stride_b + t * p.g_stride_l + h * p.g_stride_h, p.g_dtype);
+        x.beta = load_bits(p.beta, range.b * p.beta_stride_b + t * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype);
+        x.v = load4<DT>(p.v, range.b * p.v_stride_b + t * p.v_stride_l + h * p.v_stride_h + cc, cols > 0 ? cols : 1, a.vec_x);
+        return x;
+    };
+    Token next = {};
+    if (range.lo < range.hi) next = ask(range.lo);
+    stay();
+
+    float s[KR][4];
+    const float *src = p.initial_states == nullptr ? nullptr : p.initial_states + slot * p.init_stride_n + h * p.init_stride_h;
+    if (src != nullptr) {
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            const int row = rg * KR + i;
+            const float *x = src + (row < p.dim_k ? row : 0) * p.init_stride_k + cc;
+            if (a.vec_state) {
+                const u32x4 r = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(x));
+                Elem<CC1D_F32>::unpack(r, s[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[i][j] = x[j < cols ? j : 0];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    }
+    stay();
+
+    float *kq = &lds[wave][0][0], *qq = &lds[wave][1][0];
+    for (int64_t t = range.lo; t < range.hi; ++t) {
         float ke[NE], qe[NE], kk = 0.f, qs = 0.f, dot = 0.f;
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
-            const int i = lane + 64 * e;
-            ke[e] = i < p.dim_k ? Elem<DT>::to_float(kp[i]) : 0.f;
-            qe[e] = i < p.dim_k ? Elem<DT>::to_float(qp[i]) : 0.f;
+            const bool there = lane + 64 * e < p.dim_k;
+            ke[e] = there ? Elem<DT>::to_float(next.k[e]) : 0.f;
+            qe[e] = there ? Elem<DT>::to_float(next.q[e]) : 0.f;
+            kk += ke[e] * ke[e]; qs += qe[e] * qe[e]; dot += ke[e] * qe[e];
         }
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (cols > 0) load4<DT>(p.v, range.b * p.v_stride_b + t * p.v_stride_l + h * p.v_stride_h + c0, cols, a.vec_x, v);
-        const float decay = expf(load_as_float(p.g, range.b * p.g_stride_b + t * p.g_stride_l + h * p.g_stride_h, p.g_dtype));
-        const float beta = load_as_float(p.beta, range.b * p.beta_stride_b + t * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype);
+        const float decay = exp_of(bits_as_float(next.g, p.g_dtype)), beta = bits_as_float(next.beta, p.beta_dtype);
+        float v[4];
 #pragma unroll
-        for (int e = 0; e < NE; ++e) { kk += ke[e] * ke[e]; qs += qe[e] * qe[e]; dot += ke[e] * qe[e]; }
-        dot = wave_sum(dot);
+        for (int j = 0; j < 4; ++j) v[j] = Elem<DT>::to_float(next.v.x[j]);
+        if (t + 1 < range.hi) next = ask(t + 1);
+        dot = over_wave(dot);
         float rk = 1.f, rq = p.scale;
         if (p.qk_l2norm) {
-            rk = rsqrtf(wave_sum(kk) + kNormEps);
-            rq = p.scale * rsqrtf(wave_sum(qs) + kNormEps);
+            rk = rsqrtf(over_wave(kk) + kNormEps);
+            rq = p.scale * rsqrtf(over_wave(qs) + kNormEps);
         }
         wave_lds_fence();                                // the token before has been read
 #pragma unroll
@@ -143,21 +161,19 @@ delta_step_kernel(const StepArgs a) {
 #pragma unroll
         for (int i = 0; i < KR; ++i) {
             const float ki = kq[rg * KR + i], qi = qq[rg * KR + i];
+            const bool there = rg * KR + i < p.dim_k;    // the rows behind the last hold what the first does
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[i][j] *= decay;
+                s[i][j] = there ? s[i][j] * decay : 0.f;
                 sk[j] += s[i][j] * ki;
                 sq[j] += s[i][j] * qi;
             }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int d = 8; d < 64; d <<= 1) { sk[j] += __shfl_xor(sk[j], d); sq[j] += __shfl_xor(sq[j], d); }
-        }
         float u[4], o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            sk[j] = over_rows(sk[j] + dpp_moved<0x128>(sk[j]));      // the lanes of a column are 8 apart
+            sq[j] = over_rows(sq[j] + dpp_moved<0x128>(sq[j]));
             u[j] = beta * (v[j] - sk[j]);
             o[j] = sq[j] + dot * rk * rq * u[j];
         }
@@ -183,8 +199,8 @@ delta_step_kernel(const StepArgs a) {
         if (row >= p.dim_k || cols <= 0) continue;
         float *d = dst + row * p.final_stride_k + c0;
         if (a.vec_state) {
-            float4 r; r.x = s[i][0]; r.y = s[i][1]; r.z = s[i][2]; r.w = s[i][3];
-            *reinterpret_cast<float4 *>(d) = r;
+            const u32x4 r = Elem<CC1D_F32>::pack(s[i]);
+            __builtin_nontemporal_store(r, reinterpret_cast<u32x4 *>(d));
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)

@@ -508,6 +508,16 @@ __device__ __forceinline__ void wait_for_loads() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+// Loads stay where they are written, in front of what follows.
+__device__ __forceinline__ void stay() { __builtin_amdgcn_sched_barrier(0); }
+
+// A barrier that orders LDS alone: loads and stores of global memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // Sum over the 64 lanes of a wave in a fixed butterfly order (deterministic).
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
