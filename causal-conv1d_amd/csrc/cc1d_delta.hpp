@@ -34,6 +34,29 @@ __device__ __forceinline__ float over_rows(float v) {    // over lanes m, m + 16
 }
 __device__ __forceinline__ float over_wave(float v) { return over_rows(over_columns(v)); }
 
+// A double moved by DPP, 0 where a lane has no source or its row of 16 is not in ROWS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved_or_zero(double v) {
+    const uint64_t x = bitcast<uint64_t>(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xf, true);
+    return bitcast<double>((uint64_t)hi << 32 | lo);
+}
+// Running sums over the 64 lanes.
+__device__ __forceinline__ double running_sum(double v) {
+    v += moved_or_zero<0x111, 0xf>(v);                   // row_shr: 1, 2, 4, 8
+    v += moved_or_zero<0x112, 0xf>(v);
+    v += moved_or_zero<0x114, 0xf>(v);
+    v += moved_or_zero<0x118, 0xf>(v);
+    v += moved_or_zero<0x142, 0xa>(v);                   // row_bcast:15: the last lane of rows 0 and 2 to rows 1 and 3
+    return v + moved_or_zero<0x143, 0xc>(v);             // row_bcast:31: the last lane of row 1 to rows 2 and 3
+}
+__device__ __forceinline__ double of_lane(double v, int lane) {
+    const uint64_t x = bitcast<uint64_t>(v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane);
+    return bitcast<double>((uint64_t)hi << 32 | lo);
+}
+
 __device__ __forceinline__ float load_as_float(const void *p, int64_t i, int dtype) {
     if (dtype == CC1D_F32) return static_cast<const float *>(p)[i];
     if (dtype == CC1D_F16) return (float)static_cast<const _Float16 *>(p)[i];

@@ -67,12 +67,15 @@ __device__ __forceinline__ ChunkAt chunk_at(const cc1d_delta_params &p, const Ch
         const int64_t lo = (int64_t)c * kChunk, left = p.seqlen - lo;
         return {lo, (int)(left < kChunk ? left : kChunk), n, n};
     }
-    // The last sequence whose first slot is not behind this one.
-    int a = 0, b = p.sequences;                          // a: first slot <= slot; sequence 0 begins at slot floor(cu[0] / 64)
+    // The last sequence whose first slot is not behind this one; sequence 0 begins at slot floor(cu[0] / 64).  64 candidates at
+    // once, one a lane (the whole wavefront is here): one load's wait up to 64 sequences, two up to 4096.
+    int a = 0, b = p.sequences;
     while (b - a > 1) {
-        const int mid = (a + b) >> 1;
-        const int64_t first = cu_entry(p.cu_seqlens, p.cu_seqlens_is_int64, mid, p.seqlen) / kChunk + mid;
-        if (first <= slot) a = mid; else b = mid;
+        const int step = (b - a + 63) >> 6, mine = a + (int)(threadIdx.x & 63) * step, i = mine < b ? mine : b - 1;
+        const int64_t first = cu_entry(p.cu_seqlens, p.cu_seqlens_is_int64, i, p.seqlen) / kChunk + i;
+        const int n = __popcll(__ballot(mine < b && (mine == a || first <= slot)));
+        a += (n - 1) * step;
+        b = a + step < b ? a + step : b;
     }
     const TokenRange r = sequence_tokens(p, a);
     const int64_t lo = r.lo + ((int64_t)slot - (r.lo / kChunk + a)) * kChunk, left = r.hi - lo;

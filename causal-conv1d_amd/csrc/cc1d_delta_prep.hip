@@ -2,8 +2,8 @@
 // One workgroup a chunk and value head: K K^T and Q K^T on the matrix cores, T = (I + A)^-1, and the operands of the
 // later kernels in the order in which these load them.
 //
-// T: the four 16 x 16 blocks on the diagonal by substitution, one wavefront each with a column a lane; the blocks below
-// from T_ij = -T_ii sum_{j <= k < i} A_ik T_kj by fp32 matrix instructions, the distance to the diagonal growing.
+// T: the four 16 x 16 blocks on the diagonal by substitution, one wavefront each with a column a lane; below it by fp32 matrix
+// instructions, first inside each half of 32, then between the halves: (I + A)^-1 of [[X, 0], [A, Y]] has -Y^-1 A X^-1 there.
 // Substitution and not the series of powers of A: those of keys that resemble each other grow to 1e8 before they vanish.
 #include "cc1d_delta_chunk.hpp"
 #include "cc1d_delta_host.hpp"
@@ -20,9 +20,7 @@ struct PrepLds {
         float t[kChunk][kPitch];
     };
     float a[kChunk][kPitch];
-    float scratch[4][16][17];
     float gate[kScalars][kChunk];
-    float norms[2][kChunk];
 };
 
 // The 16 x 16 product of two blocks in LDS, added to acc.
@@ -48,6 +46,15 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     if (at.count <= 0) return;
     const int64_t sh = (int64_t)slot * p.heads + hk, sv = (int64_t)slot * p.v_heads + h;
 
+    // Gates: asked for first, summed while K and Q travel.
+    uint32_t gate_bits = 0, beta_bits = 0;
+    {
+        const int64_t tok = at.lo + (lane < at.count ? lane : 0);
+        gate_bits = load_bits(p.g, at.b * p.g_stride_b + tok * p.g_stride_l + h * p.g_stride_h, p.g_dtype);
+        beta_bits = load_bits(p.beta, at.b * p.beta_stride_b + tok * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype);
+    }
+    stay();
+
     // Rows of K and Q as left operands; their lengths.
     const int token = row_of(wave, m);
     const bool there = token < at.count;
@@ -62,6 +69,18 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
         for (int s = 0; s < KS; ++s) {
             kr[s].ask(kp, 32 * s + 8 * g, cols);
             qr[s].ask(qp, 32 * s + 8 * g, cols);
+        }
+        stay();
+        // Sums of gates in 64 bits, kept as two floats: differences of large sums lose nothing.
+        if (wave == 0) {
+            const double sum = running_sum(lane < at.count ? (double)bounded_gate(bits_as_float(gate_bits, p.g_dtype)) : 0.0);
+            const double last = of_lane(sum, 63);
+            const float hi = (float)sum;
+            lds.gate[kBeta][lane] = lane < at.count ? bits_as_float(beta_bits, p.beta_dtype) : 0.f;
+            lds.gate[kGate][lane] = exp_of((float)sum);
+            lds.gate[kToEnd][lane] = exp_of((float)(last - sum));
+            lds.gate[kSumHi][lane] = hi;
+            lds.gate[kSumLo][lane] = (float)(sum - (double)hi);
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -92,38 +111,20 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     kk = over_rows(kk);
     qq = over_rows(qq);
     if (g == 0) {
-        lds.norms[0][token] = p.qk_l2norm ? rsqrtf(kk + kNormEps) : 1.f;
-        lds.norms[1][token] = p.qk_l2norm ? rsqrtf(qq + kNormEps) : 1.f;
+        lds.gate[kKeyNorm][token] = p.qk_l2norm ? rsqrtf(kk + kNormEps) : 1.f;
+        lds.gate[kQueryNorm][token] = p.qk_l2norm ? rsqrtf(qq + kNormEps) : 1.f;
     }
     lds_barrier();
 
-    // Gates.  Sums in 64 bits, kept as two floats: differences of large sums lose nothing.
-    if (wave == 0) {
-        const bool real = lane < at.count;
-        const int64_t tok = at.lo + (real ? lane : 0);
-        double sum = real ? (double)bounded_gate(load_as_float(p.g, at.b * p.g_stride_b + tok * p.g_stride_l + h * p.g_stride_h, p.g_dtype)) : 0.0;
-        const float beta = real ? load_as_float(p.beta, at.b * p.beta_stride_b + tok * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype) : 0.f;
+    if (wave == 0) {                                     // (the products below need none of these)
+        const float gam = lds.gate[kGate][lane], rk = lds.gate[kKeyNorm][lane];
+        lds.gate[kSeenBeta][lane] = lds.gate[kBeta][lane] * gam * rk;
+        lds.gate[kReadGate][lane] = p.scale * gam * lds.gate[kQueryNorm][lane];
+        lds.gate[kCarry][lane] = lds.gate[kToEnd][lane] * rk;
+        wave_lds_fence();
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double o = __shfl_up(sum, d);
-            if (lane >= d) sum += o;
-        }
-        const double last = __shfl(sum, 63);
-        const float hi = (float)sum, gam = exp_of((float)sum), dec = exp_of((float)(last - sum));
-        const float rk = lds.norms[0][lane], rq = lds.norms[1][lane];
-        lds.gate[kSeenBeta][lane] = beta * gam * rk;
-        lds.gate[kBeta][lane] = beta;
-        lds.gate[kReadGate][lane] = p.scale * gam * rq;
-        lds.gate[kCarry][lane] = dec * rk;
-        lds.gate[kKeyNorm][lane] = rk;
-        lds.gate[kQueryNorm][lane] = rq;
-        lds.gate[kGate][lane] = gam;
-        lds.gate[kToEnd][lane] = dec;
-        lds.gate[kSumHi][lane] = hi;
-        lds.gate[kSumLo][lane] = (float)(sum - (double)hi);
+        for (int i = 0; i < kScalars; ++i) w.scalars[(sv * kScalars + i) * kChunk + lane] = lds.gate[i][lane];
     }
-    lds_barrier();
-    for (int i = threadIdx.x; i < kScalars * kChunk; i += kBlock) w.scalars[sv * kScalars * kChunk + i] = (&lds.gate[0][0])[i];
 
     // K K^T and Q K^T: this wavefront's 16 rows; columns behind the rows' last are nothing.
     f32x4 read[4];                                       // P waits in registers until A is used up
@@ -209,22 +210,32 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
         }
     }
     lds_barrier();
+    auto put_block = [&](int i, int j, const f32x4 &acc, float sign) {
 #pragma unroll
-    for (int d = 1; d < 4; ++d) {
-        const int i = wave + d, j = wave;                // block (i, j)
-        if (i < 4) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            for (int k = j; k < i; ++k) acc = block_product(&lds.a[16 * i][16 * k], kPitch, &lds.t[16 * k][16 * j], kPitch, acc, m, g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) lds.scratch[wave][4 * g + e][m] = -acc[e];
-            wave_lds_fence();
-            acc = {0.f, 0.f, 0.f, 0.f};
-            acc = block_product(&lds.t[16 * i][16 * i], kPitch, &lds.scratch[wave][0][0], 17, acc, m, g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) lds.t[16 * i + 4 * g + e][16 * j + m] = acc[e];
-        }
-        lds_barrier();
+        for (int e = 0; e < 4; ++e) lds.t[16 * i + 4 * g + e][16 * j + m] = sign * acc[e];
+    };
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    if (wave < 2) {                                      // inside the halves
+        const int j = 2 * wave, i = j + 1;
+        put_block(i, j, block_product(&lds.a[16 * i][16 * j], kPitch, &lds.t[16 * j][16 * j], kPitch, zero, m, g), 1.f);
+        wave_lds_fence();
+        const f32x4 acc = block_product(&lds.t[16 * i][16 * i], kPitch, &lds.t[16 * i][16 * j], kPitch, zero, m, g);
+        wave_lds_fence();
+        put_block(i, j, acc, -1.f);
     }
+    lds_barrier();
+    {                                                    // between them, a block a wavefront
+        const int i = 2 + (wave >> 1), j = wave & 1;
+        f32x4 acc = zero;
+        for (int k = j; k < 2; ++k) acc = block_product(&lds.a[16 * i][16 * k], kPitch, &lds.t[16 * k][16 * j], kPitch, acc, m, g);
+        put_block(i, j, acc, 1.f);
+        lds_barrier();
+        acc = zero;
+        for (int k = 2; k <= i; ++k) acc = block_product(&lds.t[16 * i][16 * k], kPitch, &lds.t[16 * k][16 * j], kPitch, acc, m, g);
+        lds_barrier();
+        put_block(i, j, acc, -1.f);
+    }
+    lds_barrier();
 
     // T or, for the backward, its transpose as left operands.
     if (!w.backward)
