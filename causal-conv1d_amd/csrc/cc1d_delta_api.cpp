@@ -68,6 +68,10 @@ size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWo
     w.terms = p.x_dtype == CC1D_BF16 ? 1 : p.x_dtype == CC1D_F16 ? 2 : 3;
     w.pterms = p.x_dtype == CC1D_F32 ? 3 : 2;
     w.backward = backward;
+    w.by_heads = fast_div((uint32_t)p.heads);
+    w.by_v_heads = fast_div((uint32_t)p.v_heads);
+    w.by_group = fast_div((uint32_t)(p.heads > 0 ? p.v_heads / p.heads : 1));
+    w.by_chunks = fast_div((uint32_t)w.chunks);
     const size_t keys = (size_t)w.slots * p.heads, values = (size_t)w.slots * p.v_heads;
     const size_t state = values * p.dim_k * p.dim_v * sizeof(float), rows = values * kChunk * p.dim_v * sizeof(float);
     Places saved{static_cast<uint8_t *>(p.saved)};

@@ -41,8 +41,7 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
     const uint32_t xcd = blockIdx.x & 7u, idx = blockIdx.x >> 3;
     const uint32_t nh = idx / col_tiles * 8u + xcd;
     if (nh >= heads_total) return;
-    const int h = (int)(nh % (uint32_t)p.v_heads), n = (int)(nh / (uint32_t)p.v_heads);
-    const int hk = h / (p.v_heads / p.heads);
+    const int n = (int)divided(nh, w.by_v_heads), h = (int)nh - n * p.v_heads, hk = (int)divided((uint32_t)h, w.by_group);
     const TokenRange range = sequence_tokens(p, n);
     const int chunks = (int)((range.hi - range.lo + kChunk - 1) / kChunk);
     const int slot0 = first_slot(p, w, n, range), total = (int)(range.hi - range.lo);
@@ -292,7 +291,7 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
     const cc1d_delta_params &p = bp.fwd;
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tile = wave & 3, side = wave >> 2;
-    const int slot = (int)(blockIdx.x / (uint32_t)p.heads), hk = (int)(blockIdx.x % (uint32_t)p.heads);
+    const int slot = (int)divided(blockIdx.x, w.by_heads), hk = (int)blockIdx.x - slot * p.heads;
     const int group = SHARED ? p.v_heads / p.heads : 1;
     const ChunkAt at = chunk_at(p, w, slot);
     T *dq = static_cast<T *>(bp.dq) + hk * bp.dq_stride_h, *dk = static_cast<T *>(bp.dk) + hk * bp.dk_stride_h;

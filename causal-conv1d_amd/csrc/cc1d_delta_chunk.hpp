@@ -54,6 +54,7 @@ struct ChunkWork {
     int32_t slots, chunks;               // chunks: of one sequence without cu_seqlens
     int32_t ks, terms, pterms;           // 32-column steps of dim_k; terms of K and Q; of P
     int32_t backward;
+    FastDiv by_heads, by_v_heads, by_group, by_chunks;    // group: value heads of a key head
     __device__ __host__ int64_t kbytes() const { return (int64_t)4 * ks * terms * kFrag; }
     __device__ __host__ int64_t tbytes() const { return (int64_t)kTriFrags * 3 * kFrag; }
     __device__ __host__ int64_t pbytes() const { return (int64_t)kTriFrags * pterms * kFrag; }
@@ -63,7 +64,7 @@ struct ChunkWork {
 struct ChunkAt { int64_t lo; int count, b, n; };
 __device__ __forceinline__ ChunkAt chunk_at(const cc1d_delta_params &p, const ChunkWork &w, int slot) {
     if (p.cu_seqlens == nullptr) {
-        const int n = slot / w.chunks, c = slot - n * w.chunks;
+        const int n = (int)divided((uint32_t)slot, w.by_chunks), c = slot - n * w.chunks;
         const int64_t lo = (int64_t)c * kChunk, left = p.seqlen - lo;
         return {lo, (int)(left < kChunk ? left : kChunk), n, n};
     }

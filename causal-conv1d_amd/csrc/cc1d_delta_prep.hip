@@ -23,6 +23,12 @@ struct PrepLds {
     float gate[kScalars][kChunk];
 };
 
+// Wavefronts a SIMD: as many as the workgroups that LDS has room for.
+constexpr int prep_waves(int dt, int ks) {
+    const int terms = dt == CC1D_BF16 ? 1 : dt == CC1D_F16 ? 2 : 3;
+    return ks * terms <= 4 ? 4 : ks * terms <= 8 ? 3 : 1;
+}
+
 // The 16 x 16 product of two blocks in LDS, added to acc.
 __device__ __forceinline__ f32x4 block_product(const float *x, int px, const float *y, int py, f32x4 acc, int m, int g) {
 #pragma unroll
@@ -31,17 +37,25 @@ __device__ __forceinline__ f32x4 block_product(const float *x, int px, const flo
     return acc;
 }
 
+// x[i] -= a[i][k] x[k] for all i > k, k growing: a lane holds a column of both, a[i][k] is lane k's and the same for all.
+template <int K>
+__device__ __forceinline__ void below_diagonal(const float (&a)[16], float (&x)[16]) {
+#pragma unroll
+    for (int i = K + 1; i < 16; ++i) x[i] -= bitcast<float>(__builtin_amdgcn_readlane(bitcast<int>(a[i]), K)) * x[K];
+    if constexpr (K < 14) below_diagonal<K + 1>(a, x);
+}
+
 template <int DT, int KS, bool VEC>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, prep_waves(DT, KS))
 delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n, PT = Terms<DT>::p;
     extern __shared__ uint4 raw[];
     PrepLds<DT, KS> &lds = *reinterpret_cast<PrepLds<DT, KS> *>(raw);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-    const int slot = (int)(blockIdx.x / (uint32_t)p.v_heads), h = (int)(blockIdx.x % (uint32_t)p.v_heads);
-    const int group = p.v_heads / p.heads, hk = h / group;
-    const bool first = h % group == 0;                   // this workgroup writes what the heads of the group share
+    const int slot = (int)divided(blockIdx.x, w.by_v_heads), h = (int)blockIdx.x - slot * p.v_heads;
+    const int hk = (int)divided((uint32_t)h, w.by_group);
+    const bool first = h == 0 || (int)divided((uint32_t)h - 1u, w.by_group) != hk;                  // this workgroup writes what the heads of the group share
     const ChunkAt at = chunk_at(p, w, slot);
     if (at.count <= 0) return;
     const int64_t sh = (int64_t)slot * p.heads + hk, sv = (int64_t)slot * p.v_heads + h;
@@ -128,28 +142,47 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
 
     // K K^T and Q K^T: this wavefront's 16 rows; columns behind the rows' last are nothing.
     f32x4 read[4];                                       // P waits in registers until A is used up
+    float hi_i[4], lo_i[4], of_a[4], of_p[4];
 #pragma unroll
-    for (int ct = 0; ct < 4; ++ct) {
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, r = {0.f, 0.f, 0.f, 0.f};
-        if ((ct >> 1) <= (wave >> 1)) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                bf16x8 b[NT];
-                load_frag<NT>(lds.frags + (ct * KS + s) * NT * kFrag, lane, b);
-                a = product<2>(kf[s], b, a);
-                r = product<2>(qf[s], b, r);
-            }
-        }
-        const int j = row_of(ct, m);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = row_of(wave, 4 * g + e);
-            float decay = 0.f;
-            if (i >= j) decay = exp_of((lds.gate[kSumHi][i] - lds.gate[kSumHi][j]) + (lds.gate[kSumLo][i] - lds.gate[kSumLo][j])) * lds.gate[kKeyNorm][j];
-            lds.a[i][j] = i > j ? a[e] * decay * (lds.gate[kBeta][i] * lds.gate[kKeyNorm][i]) : 0.f;
-            read[ct][e] = i >= j ? r[e] * decay * (p.scale * lds.gate[kQueryNorm][i]) : 0.f;
-        }
+    for (int e = 0; e < 4; ++e) {
+        const int i = row_of(wave, 4 * g + e);
+        hi_i[e] = lds.gate[kSumHi][i];
+        lo_i[e] = lds.gate[kSumLo][i];
+        of_a[e] = lds.gate[kBeta][i] * lds.gate[kKeyNorm][i];
+        of_p[e] = p.scale * lds.gate[kQueryNorm][i];
     }
+    auto half = [&](int c2) {                            // columns 32 c2 on
+        f32x4 a[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, r[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        float hi_j[2], lo_j[2], norm_j[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int j = row_of(2 * c2 + c, m);
+            hi_j[c] = lds.gate[kSumHi][j];
+            lo_j[c] = lds.gate[kSumLo][j];
+            norm_j[c] = lds.gate[kKeyNorm][j];
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                bf16x8 b[NT];
+                load_frag<NT>(lds.frags + ((2 * c2 + c) * KS + s) * NT * kFrag, lane, b);
+                a[c] = product<2>(kf[s], b, a[c]);
+                r[c] = product<2>(qf[s], b, r[c]);
+            }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = row_of(wave, 4 * g + e), j = row_of(2 * c2 + c, m);
+                const float decay = exp_of((hi_i[e] - hi_j[c]) + (lo_i[e] - lo_j[c])) * norm_j[c];       // (above the diagonal whatever it is)
+                lds.a[i][j] = i > j ? a[c][e] * decay * of_a[e] : 0.f;
+                read[2 * c2 + c][e] = i >= j ? r[c][e] * decay * of_p[e] : 0.f;
+            }
+    };
+    half(0);
+    if (wave >= 2) half(1);
+    else read[2] = read[3] = f32x4{0.f, 0.f, 0.f, 0.f};
     // K^T, then Q^T, gathered from the operands in LDS: token 32 s + 8 g + e is row m' of tile ct, dim_k index k is
     // element k & 7 of lane group (k >> 3) & 3 of step k >> 5.
     auto transposed = [&](uint8_t *dst) {
@@ -190,24 +223,22 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     }
     lds_barrier();                                       // T goes where the operands were
 
-    // T.  Diagonal blocks: lane = column.
+    // T.  Diagonal blocks: a lane has a column of A and one of T, and reads the other columns of A from the lanes that have them.
     {
         const int o = 16 * wave;
-        float x[16];
+        float a[16], x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float v = i == m ? 1.f : 0.f;
-#pragma unroll
-            for (int k = 0; k < i; ++k) v -= lds.a[o + i][o + k] * x[k];
-            x[i] = v;
+            a[i] = lds.a[o + i][o + m];
+            x[i] = i == m ? 1.f : 0.f;
         }
+        below_diagonal<0>(a, x);
         if (g == 0)
 #pragma unroll
             for (int i = 0; i < 16; ++i) lds.t[o + i][o + m] = x[i];
-        for (int i = threadIdx.x; i < kChunk * kChunk; i += kBlock) {   // above the diagonal
-            const int r = i >> 6, c = i & 63;
-            if ((c >> 4) > (r >> 4)) lds.t[r][c] = 0.f;
-        }
+        if ((wave & 1) == 0)                             // above the diagonal, where a step of 32 columns reads it
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lds.t[o + 4 * g + e][o + 16 + m] = 0.f;
     }
     lds_barrier();
     auto put_block = [&](int i, int j, const f32x4 &acc, float sign) {

@@ -39,8 +39,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
     const uint32_t xcd = blockIdx.x & 7u, idx = blockIdx.x >> 3;
     const uint32_t nh = idx / col_tiles * 8u + xcd;
     if (nh >= heads_total) return;
-    const int h = (int)(nh % (uint32_t)p.v_heads), n = (int)(nh / (uint32_t)p.v_heads);
-    const int hk = h / (p.v_heads / p.heads);
+    const int n = (int)divided(nh, w.by_v_heads), h = (int)nh - n * p.v_heads, hk = (int)divided((uint32_t)h, w.by_group);
     const TokenRange range = sequence_tokens(p, n);
     const int chunks = (int)((range.hi - range.lo + kChunk - 1) / kChunk);
     const int slot0 = first_slot(p, w, n, range), total = (int)(range.hi - range.lo);
