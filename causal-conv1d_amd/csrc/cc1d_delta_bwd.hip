@@ -23,7 +23,7 @@ template <int DT, int KS>
 struct BwdScanLds {
     uint8_t s[KS * 3 * kFrag];                           // dS1
     uint8_t o[2 * Terms<DT>::n * kFrag];                 // dO
-    uint8_t q[2 * 3 * kFrag];                            // scale gam rq dO
+    uint8_t q[2][2 * 3 * kFrag];                         // scale gam rq dO, this chunk's and the last one's (no barrier between their use)
     uint8_t u[2 * 3 * kFrag];                            // dU
     uint8_t x[2 * 3 * kFrag];                            // -beta gam rk dX
 };
@@ -32,6 +32,7 @@ template <int DT, int KS>
 __global__ void __launch_bounds__(kBlock, 2)
 delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const uint32_t heads_total, const uint32_t col_tiles) {
     using T = typename Elem<DT>::type;
+    using Bits = typename BitsOf<DT>::type;
     constexpr int NT = Terms<DT>::n;
     constexpr int TW = (2 * KS + 3) / 4;                 // 16-row tiles of dS a wavefront owns
     __shared__ BwdScanLds<DT, KS> lds;
@@ -59,22 +60,11 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             for (int64_t t = range.hi + wave * 4 + g; t < p.seqlen; t += 16) dv[t * bp.dv_stride_l + col] = Elem<DT>::from_float(0.f);
     }
 
-    f32x4 s[TW];
-#pragma unroll
-    for (int i = 0; i < TW; ++i) {
-        const int t = wave * TW + i;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = row_of(t, 4 * g + e);
-            s[i][e] = bp.dfinal_states != nullptr && t < 2 * KS && k < p.dim_k && has_col ? bp.dfinal_states[n * bp.dfinal_stride_n + h * bp.dfinal_stride_h + k * bp.dfinal_stride_k + col] : 0.f;
-        }
-    }
-
     // As in the scan of the forward: operands asked for again between the products that have used them, without conditions.
     bf16x8 kf[KS][NT], tf[2][3], pf[2][3], ktf[TW][2][NT], qtf[TW][2][NT];
     float4 seen, beta, read, carry;
     float last;
-    T d[4];
+    Bits d[4];
     const int64_t kb = w.kbytes(), tb = w.tbytes();
     const int from = wave >> 1;                          // first step of a row of T^T and P^T
     const int row = row_of(wave, 4 * g);
@@ -88,7 +78,7 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
         const uint8_t *dc = reinterpret_cast<const uint8_t *>(dop + (int64_t)c * kChunk * bp.dout_stride_l);
         const int end = total - c * kChunk - 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = *reinterpret_cast<const T *>(dc + ((uint32_t)(row + e < end ? row + e : end) * do_pitch + at_col));
+        for (int e = 0; e < 4; ++e) d[e] = *reinterpret_cast<const Bits *>(dc + ((uint32_t)(row + e < end ? row + e : end) * do_pitch + at_col));
     };
     auto ask_carry = [&](int c) { carry = *reinterpret_cast<const float4 *>(scalars_of(c) + kCarry * kChunk + row); };
     auto ask_gates = [&](int c) {
@@ -123,6 +113,27 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
         for (int i = 0; i < TW; ++i) ask_kt(c, i);
     }
 
+    f32x4 s[TW];
+#pragma unroll
+    for (int i = 0; i < TW; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (bp.dfinal_states != nullptr) {
+        const float *from = bp.dfinal_states + n * bp.dfinal_stride_n + h * bp.dfinal_stride_h + col;
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = wave * TW + i, k = row_of(t, 4 * g + e);
+                s[i][e] = from[(t < 2 * KS && k < p.dim_k ? k : 0) * bp.dfinal_stride_k];
+            }
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = wave * TW + i, k = row_of(t, 4 * g + e);
+                if (t >= 2 * KS || k >= p.dim_k || !has_col) s[i][e] = 0.f;
+            }
+    }
+
     for (int c = chunks - 1; c >= 0; --c) {
         const int next = c > 0 ? c - 1 : 0, left = total - c * kChunk;
         const int64_t sv = (int64_t)(slot0 + c) * p.v_heads + h;
@@ -148,7 +159,7 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             // Rows behind the last token have no dout.
             float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = left >= kChunk || row + e < left ? Elem<DT>::to_float(d[e]) : 0.f;
+            for (int e = 0; e < 4; ++e) x[e] = left >= kChunk || row + e < left ? Elem<DT>::to_float(bitcast<T>(d[e])) : 0.f;
             const float y[4] = {x[0] * read.x, x[1] * read.y, x[2] * read.z, x[3] * read.w};
             u32x2 fo[NT], f[3];
             split4<NT>(x, fo);
@@ -156,7 +167,7 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             for (int j = 0; j < NT; ++j) put(lds.o, NT, wave, j, fo[j]);
             split4<3>(y, f);
 #pragma unroll
-            for (int j = 0; j < 3; ++j) put(lds.q, 3, wave, j, f[j]);
+            for (int j = 0; j < 3; ++j) put(lds.q[c & 1], 3, wave, j, f[j]);
         }
         lds_barrier();
         f32x4 u = {0.f, 0.f, 0.f, 0.f}, u2 = u, o = u, o2 = u;
@@ -227,7 +238,7 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             bf16x8 bq[2][3], bx[2][3];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                load_frag<3>(lds.q + j * 3 * kFrag, lane, bq[j]);
+                load_frag<3>(lds.q[c & 1] + j * 3 * kFrag, lane, bq[j]);
                 load_frag<3>(lds.x + j * 3 * kFrag, lane, bx[j]);
             }
             stay();
@@ -247,7 +258,6 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             }
             ask_last(next);
         }
-        lds_barrier();                                   // lds.q is written again before the next barrier
     }
     if (bp.dinitial_states == nullptr || !has_col) return;
 #pragma unroll

@@ -30,6 +30,7 @@ template <int DT, int KS, bool SAVE>
 __global__ void __launch_bounds__(kBlock, 2)
 delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t heads_total, const uint32_t col_tiles) {
     using T = typename Elem<DT>::type;
+    using Bits = typename BitsOf<DT>::type;
     constexpr int NT = Terms<DT>::n, NU = Terms<DT>::p, OUT = NU - 1;
     constexpr int TW = (2 * KS + 3) / 4;                 // 16-row tiles of S a wavefront owns
     __shared__ ScanLds<KS, NU> lds;
@@ -58,23 +59,12 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
             for (int64_t t = range.hi + wave * 4 + g; t < p.seqlen; t += 16) out[t * p.out_stride_l + col] = Elem<DT>::from_float(0.f);
     }
 
-    f32x4 s[TW];
-#pragma unroll
-    for (int i = 0; i < TW; ++i) {
-        const int t = wave * TW + i;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = row_of(t, 4 * g + e);
-            s[i][e] = p.initial_states != nullptr && t < 2 * KS && k < p.dim_k && has_col ? p.initial_states[n * p.init_stride_n + h * p.init_stride_h + k * p.init_stride_k + col] : 0.f;
-        }
-    }
-
     // Operands of the chunk at hand; each set is asked for again, for the next chunk, once it has been used.  No load stands behind a
     // condition (Row8): what a wavefront has no use for, and what lies behind the last token, is read from a place that exists.
     bf16x8 kf[KS][NT], qf[KS][NT], tf[2][3], pf[2][NU], ktf[TW][2][NT];
     float4 seen, beta, read, carry;
     float last;
-    T v[4];
+    Bits v[4];
     const int64_t kb = w.kbytes(), tb = w.tbytes(), pb = w.pbytes();
     const int steps = (wave >> 1) + 1;                   // of a row of T and P
     const int row = row_of(wave, 4 * g);
@@ -94,7 +84,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
         const uint8_t *vc = reinterpret_cast<const uint8_t *>(vp + (int64_t)c * kChunk * p.v_stride_l);
         const int end = total - c * kChunk - 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const T *>(vc + ((uint32_t)(row + e < end ? row + e : end) * v_pitch + at_col));
+        for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const Bits *>(vc + ((uint32_t)(row + e < end ? row + e : end) * v_pitch + at_col));
     };
     auto ask_t = [&](int c, int i) {
         load_frag<3>(w.tf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + lower_frag(wave, i < steps ? i : 0) * 3 * kFrag, lane, tf[i]);
@@ -125,6 +115,27 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
         for (int i = 0; i < TW; ++i) ask_kt(0, i);
 #pragma unroll
         for (int i = 0; i < 2; ++i) ask_p(0, i);
+    }
+
+    f32x4 s[TW];
+#pragma unroll
+    for (int i = 0; i < TW; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (p.initial_states != nullptr) {
+        const float *from = p.initial_states + n * p.init_stride_n + h * p.init_stride_h + col;
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = wave * TW + i, k = row_of(t, 4 * g + e);
+                s[i][e] = from[(t < 2 * KS && k < p.dim_k ? k : 0) * p.init_stride_k];
+            }
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = wave * TW + i, k = row_of(t, 4 * g + e);
+                if (t >= 2 * KS || k >= p.dim_k || !has_col) s[i][e] = 0.f;
+            }
     }
 
     for (int c = 0; c < chunks; ++c) {
@@ -171,7 +182,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                x[e] = bt[e] * Elem<DT>::to_float(v[e]) - sn[e] * ks[e];
+                x[e] = bt[e] * Elem<DT>::to_float(bitcast<T>(v[e])) - sn[e] * ks[e];
                 o[e] *= rd[e];
             }
             u32x2 f[3];

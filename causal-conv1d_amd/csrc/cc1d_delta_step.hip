@@ -27,26 +27,13 @@ struct StepArgs {
     uint32_t vec_state, vec_x;           // 16-byte rows of the state / 4 elements of v and out at once
 };
 
-template <int DT>
-struct alignas(4 * sizeof(typename Elem<DT>::type)) Row4 { typename Elem<DT>::type x[4]; };
-
-// Four adjacent elements as they lie in memory; where rows are not whole vectors one by one, the first for those behind `cols`.
-template <int DT>
-__device__ __forceinline__ Row4<DT> load4(const void *base, int64_t at, int cols, bool vec) {
-    using T = typename Elem<DT>::type;
-    const T *x = static_cast<const T *>(base) + at;
-    if (vec) return *reinterpret_cast<const Row4<DT> *>(x);
-    Row4<DT> r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.x[i] = x[i < cols ? i : 0];
-    return r;
-}
-
 // KR: rows of the state a lane holds, dim_k <= 8 KR.
 template <int DT, int KR>
 __global__ void __launch_bounds__(kBlock)
 delta_step_kernel(const StepArgs a) {
     using T = typename Elem<DT>::type;
+    using Bits = typename BitsOf<DT>::type;
+    struct alignas(4 * sizeof(Bits)) Four { Bits x[4]; };
     __shared__ float lds[4][2][8 * KR + 8];
     const cc1d_delta_params &p = a.p;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -86,11 +73,11 @@ delta_step_kernel(const StepArgs a) {
     // those travel; the next token's in front of a token's products.
     constexpr int NE = (8 * KR + 63) / 64;               // elements of k and q a lane fetches
     const int cc = cols > 0 ? c0 : 0;                    // lanes behind the last column repeat the first, and store nothing
-    struct Token { T k[NE], q[NE]; Row4<DT> v; uint32_t g, beta; };
+    struct Token { Bits k[NE], q[NE], v[4]; uint32_t g, beta; };
     auto ask = [&](int64_t t) {
         Token x;
-        const T *qp = static_cast<const T *>(p.q) + range.b * p.q_stride_b + t * p.q_stride_l + hk * p.q_stride_h;
-        const T *kp = static_cast<const T *>(p.k) + range.b * p.k_stride_b + t * p.k_stride_l + hk * p.k_stride_h;
+        const Bits *qp = static_cast<const Bits *>(p.q) + range.b * p.q_stride_b + t * p.q_stride_l + hk * p.q_stride_h;
+        const Bits *kp = static_cast<const Bits *>(p.k) + range.b * p.k_stride_b + t * p.k_stride_l + hk * p.k_stride_h;
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
             const int i = lane + 64 * e < p.dim_k ? lane + 64 * e : 0;
@@ -99,7 +86,13 @@ delta_step_kernel(const StepArgs a) {
         }
         x.g = load_bits(p.g, range.b * p.g_stride_b + t * p.g_stride_l + h * p.g_stride_h, p.g_dtype);
         x.beta = load_bits(p.beta, range.b * p.beta_stride_b + t * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype);
-        x.v = load4<DT>(p.v, range.b * p.v_stride_b + t * p.v_stride_l + h * p.v_stride_h + cc, cols > 0 ? cols : 1, a.vec_x);
+        const Bits *vp = static_cast<const Bits *>(p.v) + range.b * p.v_stride_b + t * p.v_stride_l + h * p.v_stride_h + cc;
+        if (a.vec_x) {
+            *reinterpret_cast<Four *>(x.v) = *reinterpret_cast<const Four *>(vp);
+        } else {                                         // (lanes behind the last column: the first)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.v[j] = vp[j < cols ? j : 0];
+        }
         return x;
     };
     Token next = {};
@@ -135,14 +128,14 @@ delta_step_kernel(const StepArgs a) {
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
             const bool there = lane + 64 * e < p.dim_k;
-            ke[e] = there ? Elem<DT>::to_float(next.k[e]) : 0.f;
-            qe[e] = there ? Elem<DT>::to_float(next.q[e]) : 0.f;
+            ke[e] = there ? Elem<DT>::to_float(bitcast<T>(next.k[e])) : 0.f;
+            qe[e] = there ? Elem<DT>::to_float(bitcast<T>(next.q[e])) : 0.f;
             kk += ke[e] * ke[e]; qs += qe[e] * qe[e]; dot += ke[e] * qe[e];
         }
         const float decay = exp_of(bits_as_float(next.g, p.g_dtype)), beta = bits_as_float(next.beta, p.beta_dtype);
         float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = Elem<DT>::to_float(next.v.x[j]);
+        for (int j = 0; j < 4; ++j) v[j] = Elem<DT>::to_float(bitcast<T>(next.v[j]));
         if (t + 1 < range.hi) next = ask(t + 1);
         dot = over_wave(dot);
         float rk = 1.f, rq = p.scale;
