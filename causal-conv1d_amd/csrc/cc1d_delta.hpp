@@ -51,6 +51,17 @@ __device__ __forceinline__ double running_sum(double v) {
     v += moved_or_zero<0x142, 0xa>(v);                   // row_bcast:15: the last lane of rows 0 and 2 to rows 1 and 3
     return v + moved_or_zero<0x143, 0xc>(v);             // row_bcast:31: the last lane of row 1 to rows 2 and 3
 }
+// What lane i and all behind it hold, summed.
+__device__ __forceinline__ float sum_from_here(float v) {
+    v += dpp_moved<0x101>(v);                            // row_shl: 1, 2, 4, 8
+    v += dpp_moved<0x102>(v);
+    v += dpp_moved<0x104>(v);
+    v += dpp_moved<0x108>(v);
+    const int bits = bitcast<int>(v), row = (threadIdx.x & 63) >> 4;
+    const float c = bitcast<float>(__builtin_amdgcn_readlane(bits, 48));                   // rows' totals
+    const float b = bitcast<float>(__builtin_amdgcn_readlane(bits, 32)) + c, a = bitcast<float>(__builtin_amdgcn_readlane(bits, 16)) + b;
+    return v + (row == 0 ? a : row == 1 ? b : row == 2 ? c : 0.f);
+}
 __device__ __forceinline__ double of_lane(double v, int lane) {
     const uint64_t x = bitcast<uint64_t>(v);
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane);

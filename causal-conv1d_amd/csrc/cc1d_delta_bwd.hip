@@ -273,29 +273,35 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
 
 constexpr int kGradBlock = 512;
 
+// 32 columns of U, dX, S0 and dS1 as operands.  A lane's 16 bytes lie turned by 2 g places among the 16 of its group: lanes that have
+// a row between them, 4 columns each, then write to different banks.
 template <int KS>
-struct GradStage { uint8_t u[4 * 3 * kFrag], x[4 * 3 * kFrag], s0[2 * KS * 3 * kFrag], ds1[2 * KS * 3 * kFrag]; };
+struct GradStage {
+    uint8_t u[4 * 3 * kFrag], x[4 * 3 * kFrag], s0[2 * KS * 3 * kFrag], ds1[2 * KS * 3 * kFrag];
+    static constexpr int kCopies = KS <= 4 ? 2 : 1;      // as many as there is room for
+};
 // X1 and X2 as left operands: their rows (contraction over columns), scaled by rk of the column, in fp32; their columns
 // (contraction over rows), scaled by rq, and by beta rk, of the row, split as operands.
 struct GradLower { float rows[2][kChunk][68]; uint8_t columns[2][kTriFrags * 3 * kFrag]; };
 template <int KS>
 struct GradLds {
-    union { GradStage<KS> stage; GradLower lower; };
+    union { GradStage<KS> stage[GradStage<KS>::kCopies]; GradLower lower; };
     float gate[kScalars][kChunk];
     float sums[2][3][kChunk];                            // q.dQ, k.Z, k.Y of each token, of either half of dim_k
     float db[kChunk], end[8], inner[8];
 };
 
 // Every chunk's gradients alone.  Eight wavefronts: 16 tokens' rows of dQ, Z and Y each, of one half of dim_k; of X1 the first
-// four, of X2 the others.  S0, dS1 and U pass through LDS once for all of them, 32 columns of dim_v at a time, split into their
-// terms.  VEC: rows of v and dout are whole 16-byte vectors, rows of the fp32 matrices in the workspace too.  SHARED: several value
+// four, of X2 the others.  S0, dS1, dX and U pass through LDS once for all of them, 32 columns of dim_v at a time, split into their
+// terms: eight lanes fetch a row's 128 bytes, and while the products of one step are under way other wavefronts split the
+// next step's numbers into the other copy.  VEC: rows of v and dout are whole 16-byte vectors, rows of the fp32 matrices in the workspace too.  SHARED: several value
 // heads have these keys (one: their sums need no registers through the walk).
 template <int DT, int KS, bool VEC, bool SHARED>
 __global__ void __launch_bounds__(kGradBlock, 1)
 delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int vec_out) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n;
-    constexpr int TILES = KS, OWN = (2 * KS + 7) / 8;    // 16-column tiles of a half; that a wavefront brings to LDS
+    constexpr int TILES = KS, OWN = (2 * KS + 3) / 4;    // 16-column tiles of a half; that two wavefronts bring to LDS
     extern __shared__ uint4 raw[];
     GradLds<KS> &lds = *reinterpret_cast<GradLds<KS> *>(raw);
     const cc1d_delta_params &p = bp.fwd;
@@ -335,99 +341,118 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
 #pragma unroll
     for (int t = 0; t < TILES; ++t) { tq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; tk[t] = tq[t]; }
 
+    // K^T and Q^T of the half of the chunk that holds this wavefront's own tokens; q.dQ and k.dK of those tokens.
+    bf16x8 bk[TILES][NT], bq[TILES][NT];
+    float rk[4], rq[4], dotq[4] = {0.f, 0.f, 0.f, 0.f}, dotk[4] = {0.f, 0.f, 0.f, 0.f};
+
     for (int j = 0; j < group; ++j) {
         const int h = hk * group + j;
         const int64_t sv = (int64_t)slot * p.v_heads + h;
-        for (int i = threadIdx.x; i < kScalars * kChunk; i += kGradBlock) (&lds.gate[0][0])[i] = w.scalars[sv * kScalars * kChunk + i];
         f32x4 aq[TILES], az[TILES], ay[TILES], x[4];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) { aq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; az[t] = aq[t]; ay[t] = aq[t]; }
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
         float inner = 0.f, dxv = 0.f;
-        const int64_t tok = at.lo + (cols ? own : 0);
-        const T *dop = static_cast<const T *>(bp.dout) + at.b * bp.dout_stride_b + tok * bp.dout_stride_l + h * bp.dout_stride_h;
-        const T *vp = static_cast<const T *>(p.v) + at.b * p.v_stride_b + tok * p.v_stride_l + h * p.v_stride_h;
-        // What 32 columns of v need, asked for a step ahead: this lane's row of dO, and of dX and V or of U; its share of S0 and dS1.
-        Row8<DT, VEC> ro, rv;
-        Row8<CC1D_F32, VEC> rx, rs[OWN], rd[OWN];
+        const T *dop = static_cast<const T *>(bp.dout) + at.b * bp.dout_stride_b + (at.lo + (cols ? own : 0)) * bp.dout_stride_l + h * bp.dout_stride_h;
+        // What 32 columns of v need, asked for a step ahead: this lane's row of dO as a left operand, and of everything else 4 columns
+        // of a row: eight rows of a tile are one wavefront's, the other eight its neighbour's.
+        const int in_tile = (wave & 1) * 8 + (lane >> 3), c4 = 4 * (lane & 7), brought = row_of(wave >> 1, in_tile);
+        const int place = (((lane & 7) >> 1) * 16 + ((in_tile + 2 * ((lane & 7) >> 1)) & 15)) * 16 + (lane & 1) * 8;
+        const int turned = g * 16 + ((m + 2 * g) & 15);  // the lane whose place in the stage is this one's operand
+        const T *vp = static_cast<const T *>(p.v) + at.b * p.v_stride_b + (at.lo + (brought < at.count ? brought : 0)) * p.v_stride_l + h * p.v_stride_h;
+        Row8<DT, VEC> ro;
+        Row4<DT, VEC> rv;
+        Row4<CC1D_F32, VEC> rx, ru, rs[OWN], rd[OWN];
         const float *s0 = w.s0 + sv * p.dim_k * p.dim_v, *ds1 = w.ds1 + sv * p.dim_k * p.dim_v;
-        const float *xp = (side == 0 ? w.dx : w.u) + sv * kChunk * p.dim_v;
-        auto ask = [&](int c) {
-            ro.ask(dop, c, cols);
-            if (side == 0) rv.ask(vp, c, p.dim_v);
-            rx.ask(xp + (uint32_t)(own * p.dim_v), c, p.dim_v);
+        const float *xp = w.dx + sv * kChunk * p.dim_v + (uint32_t)(brought * p.dim_v), *up = w.u + sv * kChunk * p.dim_v + (uint32_t)(brought * p.dim_v);
+        auto ask = [&](int v0) {
+            ro.ask(dop, v0 + 8 * g, cols);
+            const int c = v0 + c4;
+            rv.ask(vp, c, p.dim_v);
+            rx.ask(xp, c, p.dim_v);
+            ru.ask(up, c, p.dim_v);
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
-                const int t = wave + 8 * i < 2 * KS ? wave + 8 * i : 0, k = row_of(t, m);
-                const uint32_t to = (uint32_t)((k < p.dim_k ? k : 0) * p.dim_v);
+                const int t = (wave >> 1) + 4 * i, k = row_of(t, in_tile);
+                const uint32_t to = (uint32_t)((t < 2 * KS && k < p.dim_k ? k : 0) * p.dim_v);
                 rs[i].ask(s0 + to, c, p.dim_v);
                 rd[i].ask(ds1 + to, c, p.dim_v);
             }
         };
-        ask(8 * g);
-        for (int v0 = 0; v0 < p.dim_v; v0 += 32) {
-            const int c = v0 + 8 * g;
+        bf16x8 fo[NT];
+        auto bring = [&](int v0, GradStage<KS> &stage) {
+            const int c = v0 + c4;
             const bool cut = v0 + 32 > p.dim_v;
-            float f[8], f2[8];
-            bf16x8 fo[NT], fx[3], fu[3];
-            ro.template operand<NT>(c, cols, true, fo);
+            float f[4], f2[4];
+            u32x2 f3[3];
+            auto put = [&](uint8_t *base, int t) {
+#pragma unroll
+                for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2 *>(base + (t * 3 + n) * kFrag + place) = f3[n];
+            };
+            ro.template operand<NT>(v0 + 8 * g, cols, true, fo);
             rx.get(c, p.dim_v, cut, f);
-            split8<3>(f, fx);
-            if (side == 0) {
-                rv.get(c, p.dim_v, cut, f2);
+            rv.get(c, p.dim_v, cut, f2);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dxv += f[e] * f2[e];
-            }
-            lds_barrier();                             // the step before has been read
-            uint8_t *mine = (side == 0 ? lds.stage.x : lds.stage.u) + tile * 3 * kFrag + lane * 16;
-#pragma unroll
-            for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4 *>(mine + n * kFrag) = bitcast<u32x4>(fx[n]);
+            for (int e = 0; e < 4; ++e) dxv += f[e] * f2[e];
+            split4<3>(f, f3);
+            put(stage.x, wave >> 1);
+            ru.get(c, p.dim_v, cut, f);
+            split4<3>(f, f3);
+            put(stage.u, wave >> 1);
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
-                const int t = wave + 8 * i;
+                const int t = (wave >> 1) + 4 * i;
                 if (t >= 2 * KS) break;
-                const int in = row_of(t, m) < p.dim_k ? p.dim_v : 0;
-                bf16x8 fs[3];
+                const int in = row_of(t, in_tile) < p.dim_k ? p.dim_v : 0;
                 rs[i].get(c, in, cut || cut_k, f);
                 rd[i].get(c, in, cut || cut_k, f2);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) inner += f[e] * f2[e];
-                split8<3>(f, fs);
-#pragma unroll
-                for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4 *>(lds.stage.s0 + (t * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(fs[n]);
-                split8<3>(f2, fs);
-#pragma unroll
-                for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4 *>(lds.stage.ds1 + (t * 3 + n) * kFrag + lane * 16) = bitcast<u32x4>(fs[n]);
+                for (int e = 0; e < 4; ++e) inner += f[e] * f2[e];
+                split4<3>(f, f3);
+                put(stage.s0, t);
+                split4<3>(f2, f3);
+                put(stage.ds1, t);
             }
-            stay();
-            if (v0 + 32 < p.dim_v) ask(c + 32);
-            stay();
-            lds_barrier();
-            load_frag<3>(lds.stage.x + tile * 3 * kFrag, lane, fx);
-            load_frag<3>(lds.stage.u + tile * 3 * kFrag, lane, fu);
+        };
+        ask(0);
+        for (int i = threadIdx.x; i < kScalars * kChunk; i += kGradBlock) (&lds.gate[0][0])[i] = w.scalars[sv * kScalars * kChunk + i];
+        bring(0, lds.stage[0]);
+        if (32 < p.dim_v) ask(32);
+        lds_barrier();
+        constexpr int COPIES = GradStage<KS>::kCopies;
+        for (int v0 = 0; v0 < p.dim_v; v0 += 32) {
+            const GradStage<KS> &stage = lds.stage[COPIES == 2 ? (v0 >> 5) & 1 : 0];
+            bf16x8 fx[3], fu[3];
+            load_frag<3>(stage.x + tile * 3 * kFrag, turned, fx);
+            load_frag<3>(stage.u + tile * 3 * kFrag, turned, fu);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
                 if ((t >> 1) <= half) {
                     bf16x8 b[3];
-                    load_frag<3>(lds.stage.u + t * 3 * kFrag, lane, b);
+                    load_frag<3>(stage.u + t * 3 * kFrag, turned, b);
                     x[t] = side == 0 ? product<2>(fo, b, x[t]) : product<2>(fx, b, x[t]);
                     stay();
                 }
-            const uint8_t *sl = lds.stage.s0 + side * TILES * 3 * kFrag, *dl = lds.stage.ds1 + side * TILES * 3 * kFrag;
+            const uint8_t *sl = stage.s0 + side * TILES * 3 * kFrag, *dl = stage.ds1 + side * TILES * 3 * kFrag;
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
                 bf16x8 b[3], d[3];
-                load_frag<3>(sl + t * 3 * kFrag, lane, b);
-                load_frag<3>(dl + t * 3 * kFrag, lane, d);
+                load_frag<3>(sl + t * 3 * kFrag, turned, b);
+                load_frag<3>(dl + t * 3 * kFrag, turned, d);
                 aq[t] = product<2>(fo, b, aq[t]);
                 az[t] = product<2>(fx, b, az[t]);
                 ay[t] = product<2>(fu, d, ay[t]);
                 stay();
             }
+            if (v0 + 32 < p.dim_v) {
+                if (COPIES == 1) lds_barrier();          // the step has been read
+                bring(v0 + 32, lds.stage[COPIES == 2 ? ((v0 >> 5) + 1) & 1 : 0]);
+                stay();
+                if (v0 + 64 < p.dim_v) ask(v0 + 64);
+                lds_barrier();
+            }
         }
-        // K^T and Q^T of the half of the chunk that holds this wavefront's own tokens.
-        bf16x8 bk[TILES][NT], bq[TILES][NT];
         auto ask_kq = [&](int s) {
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
@@ -437,7 +462,7 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
         };
         ask_kq(half);
         lds_barrier();                                   // the stage becomes X1, X2
-        float rk[4], rq[4], beta[4], hi[4], lo[4];
+        float beta[4], hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             rk[e] = lds.gate[kKeyNorm][row + e]; rq[e] = lds.gate[kQueryNorm][row + e]; beta[e] = lds.gate[kBeta][row + e];
@@ -473,8 +498,10 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
                 ay[t][e] *= dec;
             }
         }
-        dxv = over_rows(dxv);
-        if (g == 0 && side == 0) lds.db[own] = dxv;
+        dxv += dpp_moved<0xB1>(dxv);                     // over the eight lanes of a row
+        dxv += dpp_moved<0x4E>(dxv);
+        dxv += dpp_moved<0x141>(dxv);                    // row_half_mirror
+        if ((lane & 7) == 0) lds.db[brought] = dxv;
         lds_barrier();
         // Rows of X1 and X2 against K, their columns against Q and K.  The operand of the step that holds this lane's own four
         // tokens also has their elements of K and Q, in the lane that has the results: what the gates' gradients multiply.
@@ -546,6 +573,11 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
             if (m == 0) { lds.sums[side][0][row + e] = d; lds.sums[side][1][row + e] = z; lds.sums[side][2][row + e] = y; }
         }
         lds_barrier();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            dotq[e] += lds.sums[0][0][row + e] + lds.sums[1][0][row + e];
+            dotk[e] += beta[e] * (lds.sums[0][1][row + e] + lds.sums[1][1][row + e]) + (lds.sums[0][2][row + e] + lds.sums[1][2][row + e]);
+        }
         if (wave == 0) {
             const float z = lds.sums[0][1][lane] + lds.sums[1][1][lane];
             float d = (lds.sums[0][0][lane] + lds.sums[1][0][lane]) + lds.gate[kBeta][lane] * z - (lds.sums[0][2][lane] + lds.sums[1][2][lane]);
@@ -555,11 +587,7 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
                 for (int i = 0; i < 8; ++i) { both += lds.inner[i]; ends += lds.end[i]; }
                 d += ends + lds.gate[kGate][63] * both;
             }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const float other = __shfl_down(d, o);
-                if (lane + o < 64) d += other;
-            }
+            d = sum_from_here(d);
             // Nothing stands in front of a sequence's first token for its gate to act on; the terms cancel up to rounding.
             if (lane == 0 && p.initial_states == nullptr && at.lo == sequence_tokens(p, at.n).lo) d = 0.f;
             if (lane < at.count) {
@@ -568,41 +596,16 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
                 store_from_float(bp.dbeta, to, p.beta_dtype, lds.db[lane] + z);
             }
         }
-        lds_barrier();
+        if (j + 1 < group) lds_barrier();
     }
 
-    // The lengths' share.
+    // The lengths' share: what lies along a key or query; the sums have one factor rk or rq already.
     if (p.qk_l2norm) {
-        float rk[4], rq[4], dotq[4] = {0.f, 0.f, 0.f, 0.f}, dotk[4] = {0.f, 0.f, 0.f, 0.f};
-        bf16x8 bk[TILES][NT], bq[TILES][NT];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            load_frag<NT>(kt + (t * 2 + half) * NT * kFrag, lane, bk[t]);
-            load_frag<NT>(qt + (t * 2 + half) * NT * kFrag, lane, bq[t]);
-        }
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            float ke[4], qe[4];
-            four_of(bk[t], upper, ke);
-            four_of(bq[t], upper, qe);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                dotq[e] += tq[t][e] * qe[e];
-                dotk[e] += tk[t][e] * ke[e];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            dotq[e] = over_columns(dotq[e]);
-            dotk[e] = over_columns(dotk[e]);
-            if (m == 0) { lds.sums[side][0][row + e] = dotq[e]; lds.sums[side][1][row + e] = dotk[e]; }
-        }
-        lds_barrier();
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             rk[e] = lds.gate[kKeyNorm][row + e]; rq[e] = lds.gate[kQueryNorm][row + e];
-            dotq[e] = (lds.sums[0][0][row + e] + lds.sums[1][0][row + e]) * rq[e] * rq[e];
-            dotk[e] = (lds.sums[0][1][row + e] + lds.sums[1][1][row + e]) * rk[e] * rk[e];
+            dotq[e] *= rq[e];
+            dotk[e] *= rk[e];
         }
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
@@ -619,18 +622,19 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
     // Out through LDS, so that whole rows leave.
     constexpr int PITCH = 32 * KS + 8;
     T *rows_out = reinterpret_cast<T *>(raw);            // the stage is free
-    auto leave = [&](const f32x4 (&v)[TILES], T *to, int64_t sb, int64_t sl) {
-        lds_barrier();
+    constexpr bool BOTH = 2 * kChunk * PITCH * sizeof(T) <= sizeof(GradStage<KS>) * GradStage<KS>::kCopies;   // at once
+    auto write = [&](const f32x4 (&v)[TILES], T *rows) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) rows_out[(row + e) * PITCH + row_of(side * TILES + t, m)] = Elem<DT>::from_float(v[t][e]);
-        lds_barrier();
+            for (int e = 0; e < 4; ++e) rows[(row + e) * PITCH + row_of(side * TILES + t, m)] = Elem<DT>::from_float(v[t][e]);
+    };
+    auto leave = [&](const T *rows, T *to, int64_t sb, int64_t sl) {
         T *base = to + at.b * sb + at.lo * sl;
         for (int i = threadIdx.x; i < at.count * 4 * KS; i += kGradBlock) {    // 8 elements a lane
             const int token = i / (4 * KS), c = i % (4 * KS) * 8;
             if (c >= p.dim_k) continue;
-            const T *from = rows_out + token * PITCH + c;
+            const T *from = rows + token * PITCH + c;
             T *d = base + token * sl + c;
             if (vec_out && c + 8 <= p.dim_k) {
 #pragma unroll
@@ -640,8 +644,17 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
             }
         }
     };
-    leave(tq, dq, bp.dq_stride_b, bp.dq_stride_l);
-    leave(tk, dk, bp.dk_stride_b, bp.dk_stride_l);
+    T *second = rows_out + (BOTH ? kChunk * PITCH : 0);
+    write(tq, rows_out);
+    if (BOTH) write(tk, second);
+    lds_barrier();
+    leave(rows_out, dq, bp.dq_stride_b, bp.dq_stride_l);
+    if (!BOTH) {
+        lds_barrier();
+        write(tk, second);
+        lds_barrier();
+    }
+    leave(second, dk, bp.dk_stride_b, bp.dk_stride_l);
 }
 
 template <int DT, int KS>

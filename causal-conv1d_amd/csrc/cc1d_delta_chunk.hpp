@@ -198,6 +198,30 @@ struct Row8 {
     }
 };
 
+// 4 elements of a row in the same manner.
+template <int DT, bool VEC>
+struct Row4 {
+    using T = typename Elem<DT>::type;
+    using Bits = typename BitsOf<DT>::type;
+    struct alignas(4 * sizeof(Bits)) Four { Bits x[4]; } r;
+    __device__ __forceinline__ void ask(const T *row, int c, int cols) {
+        const Bits *from = reinterpret_cast<const Bits *>(row);
+        if constexpr (VEC) {
+            r = *reinterpret_cast<const Four *>(from + (c < cols ? c : 0));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.x[i] = from[c + i < cols ? c + i : 0];
+        }
+    }
+    __device__ __forceinline__ void get(int c, int cols, bool cut, float (&f)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = Elem<DT>::to_float(bitcast<T>(r.x[i]));
+        if (cut)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = (VEC ? c : c + i) < cols ? f[i] : 0.f;
+    }
+};
+
 template <int N>
 __device__ __forceinline__ void load_frag(const uint8_t *base, int lane, bf16x8 (&f)[N]) {
 #pragma unroll
