@@ -29,7 +29,7 @@ struct BwdScanLds {
 };
 
 template <int DT, int KS>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(kBlock, scan_waves(DT, KS))
 delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const uint32_t heads_total, const uint32_t col_tiles) {
     using T = typename Elem<DT>::type;
     using Bits = typename BitsOf<DT>::type;

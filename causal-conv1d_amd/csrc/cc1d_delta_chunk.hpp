@@ -38,6 +38,9 @@ template <int DT> struct Terms { static constexpr int n = DT == CC1D_BF16 ? 1 : 
 enum { kSeenBeta, kBeta, kReadGate, kCarry, kKeyNorm, kQueryNorm, kGate, kToEnd, kSumHi, kSumLo, kScalars };
 //     beta gam rk   beta   scale gam rq  dec rk  rk        rq          gam    dec     G = hi + lo
 
+// Wavefronts a SIMD in the scans: two, or one with all registers where a chunk's operands do not fit in half of them.
+constexpr int scan_waves(int dt, int ks) { return ks * (dt == CC1D_BF16 ? 1 : dt == CC1D_F16 ? 2 : 3) <= 8 && ks <= 4 ? 2 : 1; }
+
 constexpr int kFrag = 1024;              // bytes of one operand of 16 x 32 bfloat16
 constexpr int kTriFrags = 6;             // of a triangular 64 x 64 matrix: 2 tiles x 1 step + 2 tiles x 2 steps
 __device__ __host__ __forceinline__ constexpr int lower_frag(int t, int s) { return t < 2 ? t : 2 + 2 * (t - 2) + s; }

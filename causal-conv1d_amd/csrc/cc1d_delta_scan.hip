@@ -27,7 +27,7 @@ struct ScanLds {
 // SAVE: the state in front of every chunk, and U, go to memory for the backward.  K and Q come from the prep kernel's copy:
 // read from their own rows, 64 bytes each, they made this kernel 10 to 20 % slower, as much as the copy costs.
 template <int DT, int KS, bool SAVE>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(kBlock, scan_waves(DT, KS))
 delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t heads_total, const uint32_t col_tiles) {
     using T = typename Elem<DT>::type;
     using Bits = typename BitsOf<DT>::type;
