@@ -147,12 +147,13 @@ norm_fwd_kernel(const cc1d_norm_params p, const int64_t first, const int64_t las
     const int64_t row = first + (T == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x);
     if (T == 64 && row >= last) return;
     const float over = 1.f / (float)p.dim;
+    float up = 1.f;
     auto put = [&](int c, const float (&y)[8], float inv) {
         const int n = p.dim - c;
         if constexpr (Q8) {
             float s[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = y[i] * inv;
+            for (int i = 0; i < 8; ++i) s[i] = y[i] * up * inv;
             const u32x2 r = pack_e4m3(s);
             uint8_t *d = static_cast<uint8_t *>(p.y8) + row * p.y8_stride + c;
             if (n >= 8) {
@@ -166,12 +167,12 @@ norm_fwd_kernel(const cc1d_norm_params p, const int64_t first, const int64_t las
             store8<XD>(p.y, row * p.y_stride + c, n, y);
         }
     };
-    // Writes the row's scale, returns what y is multiplied by: 0 for a row of zeros, NaN for a NaN, and for a row whose
-    // largest value is so small that the quotient would be infinite the largest number there is.
+    // Writes the row's scale, returns what y is multiplied by: 0 for a row of zeros, NaN for a NaN.  A row that is all so small that the
+    // quotient would be infinite is multiplied by 2^64 first.
     auto scale_of = [&](float most) {
         if (lane == 0) p.scales[row] = most * (1.f / 448.f);
-        const float inv = 448.f / most;
-        return most > 0.f ? (inv > 3.4028234664e38f ? 3.4028234664e38f : inv) : 0.f * most;
+        if (most < 0x1p-100f) up = 0x1p64f;
+        return most > 0.f ? 448.f / (most * up) : 0.f * most;
     };
 
     if constexpr (NV > 0) {
