@@ -68,17 +68,12 @@ __device__ __forceinline__ double of_lane(double v, int lane) {
     return bitcast<double>((uint64_t)hi << 32 | lo);
 }
 
-__device__ __forceinline__ float load_as_float(const void *p, int64_t i, int dtype) {
-    if (dtype == CC1D_F32) return static_cast<const float *>(p)[i];
-    if (dtype == CC1D_F16) return (float)static_cast<const _Float16 *>(p)[i];
-    return (float)static_cast<const __bf16 *>(p)[i];
-}
 // An element as bits.  Loaded elements that cross a loop's end are kept so: __bf16 would be turned into a float in front of it,
 // and waited for.
 template <int DT> struct BitsOf { typedef uint16_t type; };
 template <> struct BitsOf<CC1D_F32> { typedef uint32_t type; };
 
-// The same in two halves, the load and what waits for it.
+// A number of any of the three types, in two halves: the load, and what waits for it.
 __device__ __forceinline__ uint32_t load_bits(const void *p, int64_t i, int dtype) {
     return dtype == CC1D_F32 ? static_cast<const uint32_t *>(p)[i] : (uint32_t)static_cast<const uint16_t *>(p)[i];
 }

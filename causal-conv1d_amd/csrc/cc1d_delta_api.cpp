@@ -93,6 +93,7 @@ size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWo
         w.qtf = work.take(keys * w.kbytes()); w.ttf = work.take(values * w.tbytes()); w.ptf = work.take(values * w.tbytes());
         w.ds1 = reinterpret_cast<float *>(work.take(state));
         w.dx = reinterpret_cast<float *>(work.take(rows));
+        if (p.v_heads > p.heads) w.dqk = reinterpret_cast<float *>(work.take(values * 2 * kChunk * 32 * w.ks * sizeof(float)));
     } else {
         w.qf = work.take(keys * w.kbytes());
         w.tf = work.take(values * w.tbytes()); w.pf = work.take(values * w.pbytes());

@@ -291,12 +291,56 @@ struct GradLds {
     float db[kChunk], end[8], inner[8];
 };
 
+// dQ and dK leave through LDS, in whole rows; BOTH: at once.
+template <int KS> constexpr int kOutPitch = 32 * KS + 8;
+template <int DT, int KS> constexpr size_t kOutBytes = 2 * kChunk * kOutPitch<KS> * sizeof(typename Elem<DT>::type);
+template <int DT, int KS> constexpr bool kJoinBoth = kOutBytes<DT, KS> <= 64 * 1024;
+template <int DT, int KS, bool BOTH>
+__device__ __forceinline__ void rows_leave(const f32x4 (&tq)[KS], const f32x4 (&tk)[KS], void *lds, const cc1d_delta_bwd_params &bp, const ChunkAt &at, int hk, int vec_out) {
+    using T = typename Elem<DT>::type;
+    constexpr int PITCH = kOutPitch<KS>;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tile = wave & 3, side = wave >> 2, row = row_of(tile, 4 * g);
+    auto write = [&](const f32x4 (&v)[KS], T *rows) {
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rows[(row + e) * PITCH + row_of(side * KS + t, m)] = Elem<DT>::from_float(v[t][e]);
+    };
+    auto leave = [&](const T *rows, T *to, int64_t sb, int64_t sl) {
+        T *base = to + at.b * sb + at.lo * sl;
+        for (int i = threadIdx.x; i < at.count * 4 * KS; i += kGradBlock) {    // 8 elements a lane
+            const int token = i / (4 * KS), c = i % (4 * KS) * 8;
+            if (c >= bp.fwd.dim_k) continue;
+            const T *from = rows + token * PITCH + c;
+            T *d = base + token * sl + c;
+            if (vec_out && c + 8 <= bp.fwd.dim_k) {
+#pragma unroll
+                for (int v4 = 0; v4 < (int)sizeof(T) / 2; ++v4) reinterpret_cast<u32x4 *>(d)[v4] = reinterpret_cast<const u32x4 *>(from)[v4];
+            } else {
+                for (int e = 0; e < 8 && c + e < bp.fwd.dim_k; ++e) d[e] = from[e];
+            }
+        }
+    };
+    T *first = static_cast<T *>(lds), *second = first + (BOTH ? kChunk * PITCH : 0);
+    write(tq, first);
+    if (BOTH) write(tk, second);
+    lds_barrier();
+    leave(first, static_cast<T *>(bp.dq) + hk * bp.dq_stride_h, bp.dq_stride_b, bp.dq_stride_l);
+    if (!BOTH) {
+        lds_barrier();
+        write(tk, second);
+        lds_barrier();
+    }
+    leave(second, static_cast<T *>(bp.dk) + hk * bp.dk_stride_h, bp.dk_stride_b, bp.dk_stride_l);
+}
+
 // Every chunk's gradients alone.  Eight wavefronts: 16 tokens' rows of dQ, Z and Y each, of one half of dim_k; of X1 the first
 // four, of X2 the others.  S0, dS1, dX and U pass through LDS once for all of them, 32 columns of dim_v at a time, split into their
 // terms: eight lanes fetch a row's 128 bytes, and while the products of one step are under way other wavefronts split the
-// next step's numbers into the other copy.  VEC: rows of v and dout are whole 16-byte vectors, rows of the fp32 matrices in the workspace too.  SHARED: several value
-// heads have these keys (one: their sums need no registers through the walk).
-template <int DT, int KS, bool VEC, bool SHARED>
+// next step's numbers into the other copy.  VEC: rows of v and dout are whole 16-byte vectors, rows of the fp32 matrices in the workspace too.
+// A workgroup takes one value head; where several share a key head their shares of dq and dk go to the workspace in fp32.
+template <int DT, int KS, bool VEC>
 __global__ void __launch_bounds__(kGradBlock, 1)
 delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int vec_out) {
     using T = typename Elem<DT>::type;
@@ -307,20 +351,19 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
     const cc1d_delta_params &p = bp.fwd;
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tile = wave & 3, side = wave >> 2;
-    const int slot = (int)divided(blockIdx.x, w.by_heads), hk = (int)blockIdx.x - slot * p.heads;
-    const int group = SHARED ? p.v_heads / p.heads : 1;
+    const int slot = (int)divided(blockIdx.x, w.by_v_heads), h = (int)blockIdx.x - slot * p.v_heads, hk = (int)divided((uint32_t)h, w.by_group);
     const ChunkAt at = chunk_at(p, w, slot);
-    T *dq = static_cast<T *>(bp.dq) + hk * bp.dq_stride_h, *dk = static_cast<T *>(bp.dk) + hk * bp.dk_stride_h;
     if (p.cu_seqlens != nullptr && slot == 0) {          // tokens in front of the first sequence and behind the last
+        T *dq = static_cast<T *>(bp.dq) + hk * bp.dq_stride_h, *dk = static_cast<T *>(bp.dk) + hk * bp.dk_stride_h;     // (all heads of a group zeros)
         auto clear = [&](int64_t lo, int64_t hi) {
             for (int64_t t = lo + wave; t < hi; t += 8) {
                 for (int k = lane; k < p.dim_k; k += 64) {
                     dq[t * bp.dq_stride_l + k] = Elem<DT>::from_float(0.f);
                     dk[t * bp.dk_stride_l + k] = Elem<DT>::from_float(0.f);
                 }
-                for (int i = lane; i < group; i += 64) {
-                    store_from_float(bp.dg, t * p.v_heads + hk * group + i, p.g_dtype, 0.f);
-                    store_from_float(bp.dbeta, t * p.v_heads + hk * group + i, p.beta_dtype, 0.f);
+                if (lane == 0) {
+                    store_from_float(bp.dg, t * p.v_heads + h, p.g_dtype, 0.f);
+                    store_from_float(bp.dbeta, t * p.v_heads + h, p.beta_dtype, 0.f);
                 }
             }
         };
@@ -328,7 +371,7 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
         clear(sequence_tokens(p, p.sequences - 1).hi, p.seqlen);
     }
     if (at.count <= 0) return;
-    const int64_t sh = (int64_t)slot * p.heads + hk;
+    const int64_t sh = (int64_t)slot * p.heads + hk, sv = (int64_t)slot * p.v_heads + h;
     const int own = row_of(tile, m);                     // the token whose row this lane holds as a left operand
     const int row = row_of(tile, 4 * g);                 // the first of the four whose results it holds
     const int half = tile >> 1;                          // where those four stand in K^T, Q^T: step, and first or second four
@@ -337,17 +380,12 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
     const bool cut_k = p.dim_k < 32 * KS;
     const uint8_t *kt = w.ktf + sh * w.kbytes() + side * TILES * 2 * NT * kFrag, *qt = w.qtf + sh * w.kbytes() + side * TILES * 2 * NT * kFrag;
 
-    f32x4 tq[TILES], tk[TILES];                          // dQ, dK of all heads of the group
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) { tq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; tk[t] = tq[t]; }
-
     // K^T and Q^T of the half of the chunk that holds this wavefront's own tokens; q.dQ and k.dK of those tokens.
     bf16x8 bk[TILES][NT], bq[TILES][NT];
-    float rk[4], rq[4], dotq[4] = {0.f, 0.f, 0.f, 0.f}, dotk[4] = {0.f, 0.f, 0.f, 0.f};
+    f32x4 tq[TILES], tk[TILES];                          // dQ, dK
+    float rk[4], rq[4], dotq[4], dotk[4];
 
-    for (int j = 0; j < group; ++j) {
-        const int h = hk * group + j;
-        const int64_t sv = (int64_t)slot * p.v_heads + h;
+    {
         f32x4 aq[TILES], az[TILES], ay[TILES], x[4];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) { aq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; az[t] = aq[t]; ay[t] = aq[t]; }
@@ -559,8 +597,8 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
                     qd[e] += aq[t][e] * qe[e];
                     kz[e] += az[t][e] * ke[e];
                     ky[e] += ay[t][e] * ke[e];
-                    tq[t][e] += aq[t][e];
-                    tk[t][e] += beta[e] * az[t][e] + ay[t][e];
+                    tq[t][e] = aq[t][e];
+                    tk[t][e] = beta[e] * az[t][e] + ay[t][e];
                 }
             }
         }
@@ -575,8 +613,8 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
         lds_barrier();
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            dotq[e] += lds.sums[0][0][row + e] + lds.sums[1][0][row + e];
-            dotk[e] += beta[e] * (lds.sums[0][1][row + e] + lds.sums[1][1][row + e]) + (lds.sums[0][2][row + e] + lds.sums[1][2][row + e]);
+            dotq[e] = lds.sums[0][0][row + e] + lds.sums[1][0][row + e];
+            dotk[e] = beta[e] * (lds.sums[0][1][row + e] + lds.sums[1][1][row + e]) + (lds.sums[0][2][row + e] + lds.sums[1][2][row + e]);
         }
         if (wave == 0) {
             const float z = lds.sums[0][1][lane] + lds.sums[1][1][lane];
@@ -596,7 +634,6 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
                 store_from_float(bp.dbeta, to, p.beta_dtype, lds.db[lane] + z);
             }
         }
-        if (j + 1 < group) lds_barrier();
     }
 
     // The lengths' share: what lies along a key or query; the sums have one factor rk or rq already.
@@ -619,42 +656,45 @@ delta_grad_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
             }
         }
     }
-    // Out through LDS, so that whole rows leave.
-    constexpr int PITCH = 32 * KS + 8;
-    T *rows_out = reinterpret_cast<T *>(raw);            // the stage is free
-    constexpr bool BOTH = 2 * kChunk * PITCH * sizeof(T) <= sizeof(GradStage<KS>) * GradStage<KS>::kCopies;   // at once
-    auto write = [&](const f32x4 (&v)[TILES], T *rows) {
+    if (p.v_heads > p.heads) {
+        float *share = w.dqk + (sv * 2 * 8 + wave) * TILES * 256 + lane * 4;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) rows[(row + e) * PITCH + row_of(side * TILES + t, m)] = Elem<DT>::from_float(v[t][e]);
-    };
-    auto leave = [&](const T *rows, T *to, int64_t sb, int64_t sl) {
-        T *base = to + at.b * sb + at.lo * sl;
-        for (int i = threadIdx.x; i < at.count * 4 * KS; i += kGradBlock) {    // 8 elements a lane
-            const int token = i / (4 * KS), c = i % (4 * KS) * 8;
-            if (c >= p.dim_k) continue;
-            const T *from = rows + token * PITCH + c;
-            T *d = base + token * sl + c;
-            if (vec_out && c + 8 <= p.dim_k) {
-#pragma unroll
-                for (int v4 = 0; v4 < (int)sizeof(T) / 2; ++v4) reinterpret_cast<u32x4 *>(d)[v4] = reinterpret_cast<const u32x4 *>(from)[v4];
-            } else {
-                for (int e = 0; e < 8 && c + e < p.dim_k; ++e) d[e] = from[e];
-            }
+        for (int t = 0; t < TILES; ++t) {
+            *reinterpret_cast<f32x4 *>(share + t * 256) = tq[t];
+            *reinterpret_cast<f32x4 *>(share + (8 * TILES + t) * 256) = tk[t];
         }
-    };
-    T *second = rows_out + (BOTH ? kChunk * PITCH : 0);
-    write(tq, rows_out);
-    if (BOTH) write(tk, second);
-    lds_barrier();
-    leave(rows_out, dq, bp.dq_stride_b, bp.dq_stride_l);
-    if (!BOTH) {
-        lds_barrier();
-        write(tk, second);
-        lds_barrier();
+        return;
     }
-    leave(second, dk, bp.dk_stride_b, bp.dk_stride_l);
+    // The stage is free: all have read X1 and X2 in front of the last barrier.
+    constexpr bool BOTH = kOutBytes<DT, KS> <= sizeof(GradStage<KS>) * GradStage<KS>::kCopies;
+    rows_leave<DT, KS, BOTH>(tq, tk, raw, bp, at, hk, vec_out);
+}
+
+// dq and dk of a key head that several value heads share: their shares added up in the order of the heads.
+template <int DT, int KS>
+__global__ void __launch_bounds__(kGradBlock)
+delta_join_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int vec_out) {
+    extern __shared__ uint4 raw[];
+    const cc1d_delta_params &p = bp.fwd;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = p.v_heads / p.heads;
+    const int slot = (int)divided(blockIdx.x, w.by_heads), hk = (int)blockIdx.x - slot * p.heads;
+    const ChunkAt at = chunk_at(p, w, slot);
+    if (at.count <= 0) return;
+    const float *share = w.dqk + (((int64_t)slot * p.v_heads + hk * group) * 2 * 8 + wave) * KS * 256 + lane * 4;
+    f32x4 tq[KS], tk[KS];
+#pragma unroll
+    for (int t = 0; t < KS; ++t) { tq[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; tk[t] = tq[t]; }
+    for (int j = 0; j < group; ++j, share += 2 * 8 * KS * 256) {
+        f32x4 a[KS], b[KS];
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+            a[t] = *reinterpret_cast<const f32x4 *>(share + t * 256);
+            b[t] = *reinterpret_cast<const f32x4 *>(share + (8 * KS + t) * 256);
+        }
+#pragma unroll
+        for (int t = 0; t < KS; ++t) { tq[t] += a[t]; tk[t] += b[t]; }
+    }
+    rows_leave<DT, KS, kJoinBoth<DT, KS>>(tq, tk, raw, bp, at, hk, vec_out);
 }
 
 template <int DT, int KS>
@@ -668,12 +708,13 @@ int launch(const cc1d_delta_bwd_params &bp, const ChunkWork &w, hipStream_t stre
                      whole_rows(p.x_dtype, p.v, p.v_stride_b, p.v_stride_l, p.v_stride_h);
     const int vec_out = whole_rows(p.x_dtype, bp.dq, bp.dq_stride_b, bp.dq_stride_l, bp.dq_stride_h) &&
                         whole_rows(p.x_dtype, bp.dk, bp.dk_stride_b, bp.dk_stride_l, bp.dk_stride_h);
-    const dim3 grid((uint32_t)((int64_t)w.slots * p.heads));
-    auto go = [&](auto v, auto shared) {
-        CC1D_LAUNCH((delta_grad_kernel<DT, KS, decltype(v)::value, decltype(shared)::value>), grid, dim3(kGradBlock), sizeof(GradLds<KS>), stream, bp, w, vec_out);
+    auto go = [&](auto v) {
+        CC1D_LAUNCH((delta_grad_kernel<DT, KS, decltype(v)::value>), dim3((uint32_t)((int64_t)w.slots * p.v_heads)), dim3(kGradBlock), sizeof(GradLds<KS>), stream, bp, w, vec_out);
     };
-    auto either = [&](auto v) { p.v_heads > p.heads ? go(v, std::true_type()) : go(v, std::false_type()); };
-    vec ? either(std::true_type()) : either(std::false_type());
+    vec ? go(std::true_type()) : go(std::false_type());
+    st = launch_status();
+    if (st != CC1D_OK || p.v_heads == p.heads) return st;
+    CC1D_LAUNCH((delta_join_kernel<DT, KS>), dim3((uint32_t)((int64_t)w.slots * p.heads)), dim3(kGradBlock), kOutBytes<DT, KS> / (kJoinBoth<DT, KS> ? 1 : 2), stream, bp, w, vec_out);
     return launch_status();
 }
 

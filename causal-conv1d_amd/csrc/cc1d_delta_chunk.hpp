@@ -54,6 +54,7 @@ struct ChunkWork {
     float *scalars;                      // per (slot, value head): [kScalars][64]
     float *s0, *ds1;                     // per (slot, value head): (dim_k, dim_v)
     float *u, *dx;                       // per (slot, value head): (64, dim_v)
+    float *dqk;                          // per (slot, value head) of shared keys: its share of dq and dk, 64 x 32 ks each, in the lanes' order
     int32_t slots, chunks;               // chunks: of one sequence without cu_seqlens
     int32_t ks, terms, pterms;           // 32-column steps of dim_k; terms of K and Q; of P
     int32_t backward;
