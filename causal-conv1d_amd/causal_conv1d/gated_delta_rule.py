@@ -15,6 +15,9 @@ are, so q, k and v may be column slices of the channel-last convolution's output
     x = causal_conv1d_fn(x, weight, bias, activation="silu").transpose(1, 2)        # (batch, seqlen, channels)
     q, k, v = (t.unflatten(-1, (-1, d)) for t, d in zip(x.split(...), (dim_k, dim_k, dim_v)))
 
+Whole sequences are worked through in chunks of 64 tokens: a NaN or an infinity reaches its own head's outputs from the start of its chunk on,
+where the recurrence alone would give it to the tokens behind it only.  Other heads, sequences and earlier chunks do not see it.
+
 There is no host path.  `gated_delta_rule_ref` states the operator in plain PyTorch.
 """
 import torch
