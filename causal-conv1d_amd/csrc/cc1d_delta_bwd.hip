@@ -68,7 +68,7 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
 
     // As in the scan of the forward: operands asked for again between the products that have used them, without conditions.
     bf16x8 kf[KS][NT], tf[2][3], pf[2][3], ktf[TW][2][NT], qtf[TW][2][NT];
-    float4 seen, beta, read, carry;
+    float4 walk;                                         // of token row + (m & 3)
     float last;
     Bits d[4];
     const int64_t kb = w.kbytes(), tb = w.tbytes();
@@ -77,20 +77,15 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
     const T *dop = static_cast<const T *>(bp.dout) + range.b * bp.dout_stride_b + range.lo * bp.dout_stride_l + h * bp.dout_stride_h;
     auto scalars_of = [&](int c) { return w.scalars + ((int64_t)(slot0 + c) * p.v_heads + h) * kScalars * kChunk; };
     auto ask_k = [&](int c, int i) { load_frag<NT>(w.kf + ((int64_t)(slot0 + c) * p.heads + hk) * kb + (int64_t)(wave * KS + i) * NT * kFrag, lane, kf[i]); };
-    auto ask_p = [&](int c, int i) { load_frag<3>(w.ptf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + upper_frag(wave, i < from ? from : i) * 3 * kFrag, lane, pf[i]); };
-    auto ask_t = [&](int c, int i) { load_frag<3>(w.ttf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + upper_frag(wave, i < from ? from : i) * 3 * kFrag, lane, tf[i]); };
+    auto ask_p = [&](int c, int i) { load_frag<3>(w.ptf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + upper_frag(wave, i) * 3 * kFrag, lane, pf[i]); };
+    auto ask_t = [&](int c, int i) { load_frag<3>(w.ttf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + upper_frag(wave, i) * 3 * kFrag, lane, tf[i]); };
     auto ask_d = [&](int c) {
-        read = *reinterpret_cast<const float4 *>(scalars_of(c) + kReadGate * kChunk + row);
         const uint8_t *dc = reinterpret_cast<const uint8_t *>(dop + (int64_t)c * kChunk * bp.dout_stride_l);
         const int end = total - c * kChunk - 1;
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[e] = *reinterpret_cast<const Bits *>(dc + ((uint32_t)(row + e < end ? row + e : end) * do_pitch + at_col));
     };
-    auto ask_carry = [&](int c) { carry = *reinterpret_cast<const float4 *>(scalars_of(c) + kCarry * kChunk + row); };
-    auto ask_gates = [&](int c) {
-        seen = *reinterpret_cast<const float4 *>(scalars_of(c) + kSeenBeta * kChunk + row);
-        beta = *reinterpret_cast<const float4 *>(scalars_of(c) + kBeta * kChunk + row);
-    };
+    auto ask_walk = [&](int c) { walk = *reinterpret_cast<const float4 *>(scalars_of(c) + 4 * (row + (m & 3))); };
     auto ask_last = [&](int c) { last = scalars_of(c)[kGate * kChunk + 63]; };
     auto ask_kt = [&](int c, int i) {
         const int64_t at = ((int64_t)(slot0 + c) * p.heads + hk) * kb + (int64_t)(wave * TW + i < 2 * KS ? wave * TW + i : 0) * 2 * NT * kFrag;
@@ -108,12 +103,13 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
         ask_d(c);
 #pragma unroll
         for (int i = 0; i < KS; ++i) ask_k(c, i);
-        ask_carry(c);
+        ask_walk(c);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) ask_p(c, i);
+        for (int i = 0; i < 2; ++i)
+            if (i >= from) ask_p(c, i);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) ask_t(c, i);
-        ask_gates(c);
+        for (int i = 0; i < 2; ++i)
+            if (i >= from) ask_t(c, i);
         ask_last(c);
 #pragma unroll
         for (int i = 0; i < TW; ++i) ask_kt(c, i);
@@ -166,7 +162,9 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = left >= kChunk || row + e < left ? Elem<DT>::to_float(bitcast<T>(d[e])) : 0.f;
-            const float y[4] = {x[0] * read.x, x[1] * read.y, x[2] * read.z, x[3] * read.w};
+            float read[4];
+            of_quad(walk.z, read);
+            const float y[4] = {x[0] * read[0], x[1] * read[1], x[2] * read[2], x[3] * read[3]};
             u32x2 fo[NT], f[3];
             split4<NT>(x, fo);
 #pragma unroll
@@ -193,14 +191,21 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
                 }
                 stay();
                 ask_k(next, i);
-                if (i == 0) { ask_p(next, 0); ask_p(next, 1); }
+                if (i == 0) {
+                    if (from == 0) ask_p(next, 0);
+                    ask_p(next, 1);
+                }
             }
         }
+        const float4 now = walk;                             // the next chunk's are needed at its start
+        ask_walk(next);
         ask_d(next);
         {
             u += u2;
             o += o2;
-            const float x[4] = {u[0] * carry.x + o[0], u[1] * carry.y + o[1], u[2] * carry.z + o[2], u[3] * carry.w + o[3]};
+            float carry[4];
+            of_quad(now.w, carry);
+            const float x[4] = {u[0] * carry[0] + o[0], u[1] * carry[1] + o[1], u[2] * carry[2] + o[2], u[3] * carry[3] + o[3]};
             u32x2 f[3];
             split4<3>(x, f);
 #pragma unroll
@@ -215,15 +220,17 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
             stay();
             if (from == 0) product2<2>(tf[0], b[0], x, x2);
             stay();
-            ask_carry(next);
             product2<2>(tf[1], b[1], x, x2);
             stay();
-            ask_t(next, 0);
+            if (from == 0) ask_t(next, 0);
             ask_t(next, 1);
             x += x2;
         }
         {
-            const float y[4] = {-seen.x * x[0], -seen.y * x[1], -seen.z * x[2], -seen.w * x[3]}, bx[4] = {beta.x * x[0], beta.y * x[1], beta.z * x[2], beta.w * x[3]};
+            float seen[4], beta[4];
+            of_quad(now.x, seen);
+            of_quad(now.y, beta);
+            const float y[4] = {-seen[0] * x[0], -seen[1] * x[1], -seen[2] * x[2], -seen[3] * x[3]}, bx[4] = {beta[0] * x[0], beta[1] * x[1], beta[2] * x[2], beta[3] * x[3]};
             u32x2 f[3];
             split4<3>(y, f);
 #pragma unroll
@@ -237,7 +244,6 @@ delta_bwd_scan_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const u
                     if (left >= kChunk || row + e < left) *reinterpret_cast<T *>(dc + ((uint32_t)(row + e) * dv_pitch + at_col)) = Elem<DT>::from_float(bx[e]);
                 }
             }
-            ask_gates(next);
         }
         lds_barrier();
         {

@@ -34,9 +34,12 @@ __device__ __host__ __forceinline__ constexpr int row_of(int t, int m) { return 
 // Terms of q, k, v, dout; of P, U and S where they make outputs of 16 bits.
 template <int DT> struct Terms { static constexpr int n = DT == CC1D_BF16 ? 1 : DT == CC1D_F16 ? 2 : 3, p = DT == CC1D_F32 ? 3 : 2; };
 
-// Scalars of a chunk's tokens, one vector of 64 each, per (chunk, value head).
-enum { kSeenBeta, kBeta, kReadGate, kCarry, kKeyNorm, kQueryNorm, kGate, kToEnd, kSumHi, kSumLo, kScalars };
-//     beta gam rk   beta   scale gam rq  dec rk  rk        rq          gam    dec     G = hi + lo
+// Scalars of a chunk's tokens per (chunk, value head): what the walks need of a token, four numbers side by side, then one
+// vector of 64 each of what the gradients need.
+enum { kSeenBeta, kWalkBeta, kReadGate, kCarry };        // of token i at 4 i + these
+//     beta gam rk   beta       scale gam rq  dec rk
+enum { kBeta = 4, kKeyNorm, kQueryNorm, kGate, kToEnd, kSumHi, kSumLo, kScalars };
+//     beta       rk        rq          gam    dec     G = hi + lo
 
 // Wavefronts a SIMD in the scans: two, or one with all registers where a chunk's operands do not fit in half of them.
 constexpr int scan_waves(int dt, int ks) { return ks * (dt == CC1D_BF16 ? 1 : dt == CC1D_F16 ? 2 : 3) <= 8 && ks <= 4 ? 2 : 1; }
@@ -201,6 +204,14 @@ struct Row8 {
         }
     }
 };
+
+// One of a token's four numbers, for the four tokens of a lane group's rows: lane b of a quad has loaded token b's.
+__device__ __forceinline__ void of_quad(float x, float (&f)[4]) {
+    f[0] = dpp_moved<0x00>(x);
+    f[1] = dpp_moved<0x55>(x);
+    f[2] = dpp_moved<0xAA>(x);
+    f[3] = dpp_moved<0xFF>(x);
+}
 
 // 4 elements of a row in the same manner.
 template <int DT, bool VEC>

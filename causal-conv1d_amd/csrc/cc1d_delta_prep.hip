@@ -136,9 +136,13 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
 
     if (wave == 0) {                                     // (the products below need none of these)
         const float gam = lds.gate[kGate][lane], rk = lds.gate[kKeyNorm][lane];
-        lds.gate[kSeenBeta][lane] = lds.gate[kBeta][lane] * gam * rk;
-        lds.gate[kReadGate][lane] = p.scale * gam * lds.gate[kQueryNorm][lane];
-        lds.gate[kCarry][lane] = lds.gate[kToEnd][lane] * rk;
+        const float beta = lds.gate[kBeta][lane];
+        float4 walk;
+        walk.x = beta * gam * rk;                        // kSeenBeta, kWalkBeta, kReadGate, kCarry
+        walk.y = beta;
+        walk.z = p.scale * gam * lds.gate[kQueryNorm][lane];
+        walk.w = lds.gate[kToEnd][lane] * rk;
+        *reinterpret_cast<float4 *>(&lds.gate[0][0] + 4 * lane) = walk;
         wave_lds_fence();
 #pragma unroll
         for (int i = 0; i < kScalars; ++i) w.scalars[(sv * kScalars + i) * kChunk + lane] = lds.gate[i][lane];

@@ -69,7 +69,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
     // Operands of the chunk at hand; each set is asked for again, for the next chunk, once it has been used.  No load stands behind a
     // condition (Row8): what a wavefront has no use for, and what lies behind the last token, is read from a place that exists.
     bf16x8 kf[KS][NT], qf[KS][NT], tf[2][3], pf[2][NU], ktf[TW][2][NT];
-    float4 seen, beta, read, carry;
+    float4 walk;                                         // of token row + (m & 3)
     float last;
     Bits v[4];
     const int64_t kb = w.kbytes(), tb = w.tbytes(), pb = w.pbytes();
@@ -83,10 +83,6 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
         load_frag<NT>(w.qf + at, lane, qf[i]);
     };
     auto ask_v = [&](int c) {
-        const float *sc = scalars_of(c);
-        seen = *reinterpret_cast<const float4 *>(sc + kSeenBeta * kChunk + row);
-        beta = *reinterpret_cast<const float4 *>(sc + kBeta * kChunk + row);
-        read = *reinterpret_cast<const float4 *>(sc + kReadGate * kChunk + row);
         // Rows behind the last token take the last one's v: their beta is 0.
         const uint8_t *vc = reinterpret_cast<const uint8_t *>(vp + (int64_t)c * kChunk * p.v_stride_l);
         const int end = total - c * kChunk - 1;
@@ -94,11 +90,11 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
         for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const Bits *>(vc + ((uint32_t)(row + e < end ? row + e : end) * v_pitch + at_col));
     };
     auto ask_t = [&](int c, int i) {
-        load_frag<3>(w.tf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + lower_frag(wave, i < steps ? i : 0) * 3 * kFrag, lane, tf[i]);
+        load_frag<3>(w.tf + ((int64_t)(slot0 + c) * p.v_heads + h) * tb + lower_frag(wave, i) * 3 * kFrag, lane, tf[i]);
     };
-    auto ask_carry = [&](int c) { carry = *reinterpret_cast<const float4 *>(scalars_of(c) + kCarry * kChunk + row); };
+    auto ask_walk = [&](int c) { walk = *reinterpret_cast<const float4 *>(scalars_of(c) + 4 * (row + (m & 3))); };
     auto ask_p = [&](int c, int i) {
-        load_frag<NU>(w.pf + ((int64_t)(slot0 + c) * p.v_heads + h) * pb + lower_frag(wave, i < steps ? i : 0) * NU * kFrag, lane, pf[i]);
+        load_frag<NU>(w.pf + ((int64_t)(slot0 + c) * p.v_heads + h) * pb + lower_frag(wave, i) * NU * kFrag, lane, pf[i]);
     };
     auto ask_kt = [&](int c, int i) {                    // tile i of this wavefront's
         const int t = wave * TW + i < 2 * KS ? wave * TW + i : 0;
@@ -114,14 +110,16 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
 #pragma unroll
         for (int i = 0; i < KS; ++i) ask_kq(0, i);
         ask_v(0);
-        ask_carry(0);
+        ask_walk(0);
         ask_last(0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) ask_t(0, i);
+        for (int i = 0; i < 2; ++i)
+            if (i < steps) ask_t(0, i);
 #pragma unroll
         for (int i = 0; i < TW; ++i) ask_kt(0, i);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) ask_p(0, i);
+        for (int i = 0; i < 2; ++i)
+            if (i < steps) ask_p(0, i);
     }
 
     f32x4 s[TW];
@@ -185,8 +183,10 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
         {
             ks += ks2;
             o += o2;
-            const float bt[4] = {beta.x, beta.y, beta.z, beta.w}, sn[4] = {seen.x, seen.y, seen.z, seen.w}, rd[4] = {read.x, read.y, read.z, read.w};
-            float x[4];
+            float x[4], sn[4], bt[4], rd[4];
+            of_quad(walk.x, sn);
+            of_quad(walk.y, bt);
+            of_quad(walk.z, rd);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 x[e] = bt[e] * Elem<DT>::to_float(bitcast<T>(v[e])) - sn[e] * ks[e];
@@ -210,9 +210,11 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
             if (steps == 2) product2<2>(tf[1], b[1], u, u2);
             stay();
             ask_t(next, 0);
-            ask_t(next, 1);
+            if (steps == 2) ask_t(next, 1);
             u += u2;
-            const float x[4] = {u[0], u[1], u[2], u[3]}, y[4] = {x[0] * carry.x, x[1] * carry.y, x[2] * carry.z, x[3] * carry.w};
+            float carry[4];
+            of_quad(walk.w, carry);
+            const float x[4] = {u[0], u[1], u[2], u[3]}, y[4] = {x[0] * carry[0], x[1] * carry[1], x[2] * carry[2], x[3] * carry[3]};
             u32x2 f[3], fu[NU];
             split4<3>(y, f);
 #pragma unroll
@@ -235,7 +237,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
                 load_frag<NU>(lds.u + q * NU * kFrag, lane, bu[q]);
             }
             stay();
-            ask_carry(next);
+            ask_walk(next);
 #pragma unroll
             for (int i = 0; i < TW; ++i) {
                 if (wave * TW + i >= 2 * KS) break;
@@ -254,7 +256,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
             o += small;
             stay();
             ask_p(next, 0);
-            ask_p(next, 1);
+            if (steps == 2) ask_p(next, 1);
             ask_last(next);
         }
         if (has_col) {
