@@ -74,29 +74,32 @@ delta_step_kernel(const StepArgs a) {
     constexpr int NE = (8 * KR + 63) / 64;               // elements of k and q a lane fetches
     const int cc = cols > 0 ? c0 : 0;                    // lanes behind the last column repeat the first, and store nothing
     struct Token { Bits k[NE], q[NE], v[4]; uint32_t g, beta; };
-    auto ask = [&](int64_t t) {
+    const Bits *qp = static_cast<const Bits *>(p.q) + range.b * p.q_stride_b + range.lo * p.q_stride_l + hk * p.q_stride_h;
+    const Bits *kp = static_cast<const Bits *>(p.k) + range.b * p.k_stride_b + range.lo * p.k_stride_l + hk * p.k_stride_h;
+    const Bits *vp = static_cast<const Bits *>(p.v) + range.b * p.v_stride_b + range.lo * p.v_stride_l + h * p.v_stride_h + cc;
+    int64_t at_g = range.b * p.g_stride_b + range.lo * p.g_stride_l + h * p.g_stride_h;
+    int64_t at_beta = range.b * p.beta_stride_b + range.lo * p.beta_stride_l + h * p.beta_stride_h;
+    auto ask = [&]() {                                   // the token after the one asked for last
         Token x;
-        const Bits *qp = static_cast<const Bits *>(p.q) + range.b * p.q_stride_b + t * p.q_stride_l + hk * p.q_stride_h;
-        const Bits *kp = static_cast<const Bits *>(p.k) + range.b * p.k_stride_b + t * p.k_stride_l + hk * p.k_stride_h;
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
             const int i = lane + 64 * e < p.dim_k ? lane + 64 * e : 0;
             x.k[e] = kp[i];
             x.q[e] = qp[i];
         }
-        x.g = load_bits(p.g, range.b * p.g_stride_b + t * p.g_stride_l + h * p.g_stride_h, p.g_dtype);
-        x.beta = load_bits(p.beta, range.b * p.beta_stride_b + t * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype);
-        const Bits *vp = static_cast<const Bits *>(p.v) + range.b * p.v_stride_b + t * p.v_stride_l + h * p.v_stride_h + cc;
+        x.g = load_bits(p.g, at_g, p.g_dtype);
+        x.beta = load_bits(p.beta, at_beta, p.beta_dtype);
         if (a.vec_x) {
             *reinterpret_cast<Four *>(x.v) = *reinterpret_cast<const Four *>(vp);
         } else {                                         // (lanes behind the last column: the first)
 #pragma unroll
             for (int j = 0; j < 4; ++j) x.v[j] = vp[j < cols ? j : 0];
         }
+        qp += p.q_stride_l; kp += p.k_stride_l; vp += p.v_stride_l; at_g += p.g_stride_l; at_beta += p.beta_stride_l;
         return x;
     };
     Token next = {};
-    if (range.lo < range.hi) next = ask(range.lo);
+    if (range.lo < range.hi) next = ask();
     stay();
 
     float s[KR][4];
@@ -136,45 +139,48 @@ delta_step_kernel(const StepArgs a) {
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = Elem<DT>::to_float(bitcast<T>(next.v[j]));
-        if (t + 1 < range.hi) next = ask(t + 1);
-        dot = over_wave(dot);
+        if (t + 1 < range.hi) next = ask();
         float rk = 1.f, rq = p.scale;
-        if (p.qk_l2norm) {
+        auto lengths = [&]() {
+            dot = over_wave(dot);
+            if (!p.qk_l2norm) return;
             rk = rsqrtf(over_wave(kk) + kNormEps);
             rq = p.scale * rsqrtf(over_wave(qs) + kNormEps);
-        }
+        };
+        if (KR == 32) lengths();                         // (behind the sums below it would take a register too many for two wavefronts a SIMD)
         wave_lds_fence();                                // the token before has been read
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
             const int i = lane + 64 * e;
-            if (i < 8 * KR) { kq[i] = ke[e] * rk; qq[i] = qe[e] * rq; }
+            if (i < 8 * KR) { kq[i] = ke[e]; qq[i] = qe[e]; }
         }
         wave_lds_fence();
+        // Sums with the state as it is, the decay and the lengths' factors on the sums: nothing waits for those.  Rows behind the
+        // last, which hold what the first does, meet zeros.
         float sk[4] = {0.f, 0.f, 0.f, 0.f}, sq[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < KR; ++i) {
             const float ki = kq[rg * KR + i], qi = qq[rg * KR + i];
-            const bool there = rg * KR + i < p.dim_k;    // the rows behind the last hold what the first does
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[i][j] = there ? s[i][j] * decay : 0.f;
                 sk[j] += s[i][j] * ki;
                 sq[j] += s[i][j] * qi;
             }
         }
+        if (KR < 32) lengths();
         float u[4], o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             sk[j] = over_rows(sk[j] + dpp_moved<0x128>(sk[j]));      // the lanes of a column are 8 apart
             sq[j] = over_rows(sq[j] + dpp_moved<0x128>(sq[j]));
-            u[j] = beta * (v[j] - sk[j]);
-            o[j] = sq[j] + dot * rk * rq * u[j];
+            u[j] = beta * (v[j] - decay * rk * sk[j]) * rk;          // of k as it came
+            o[j] = rq * (decay * sq[j] + dot * u[j]);
         }
 #pragma unroll
         for (int i = 0; i < KR; ++i) {
             const float ki = kq[rg * KR + i];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] += ki * u[j];
+            for (int j = 0; j < 4; ++j) s[i][j] = s[i][j] * decay + ki * u[j];
         }
         if (rg == 0) {
             T *op = static_cast<T *>(p.out) + range.b * p.out_stride_b + t * p.out_stride_l + h * p.out_stride_h + c0;
