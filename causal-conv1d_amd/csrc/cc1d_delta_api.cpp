@@ -37,14 +37,15 @@ int check_delta(const cc1d_delta_params &p) {
     return CC1D_OK;
 }
 
-// Sequences of this many tokens on average go by chunks.  A token costs the token kernel 1.4 us as long as its states fill no more than
+// Sequences of this many tokens on average go by chunks.  A token costs the token kernel 1.3 us as long as its states fill no more than
 // the card, a chunk costs as much for one token as for 64.  Heads of 128 x 128, token by token / by chunks, us:
-//   bfloat16  32 heads:  8 tokens 16.8 / 14.7   256: 20 tokens 35.2 / 33.7   2048: 24 tokens 178 / 239, 40: 283 / 248
-//   float32   32 heads: 12 tokens 21.4 / 19.7   256: 40 tokens 60.3 / 62.3   2048: 64 tokens 408 / 553, 96: 611 / 823
+//   bfloat16  32 heads:  8 tokens 15.9 / 14.9   256: 20 tokens 33.7 / 32.3   2048: 32 tokens 203 / 235, 48: 293 / 251
+//   float32   32 heads: 12 tokens 20.5 / 19.4   256: 40 tokens 59.2 / 61.1   2048: 96 tokens 538 / 810, 128: 712 / 825
 int chunked_from(const cc1d_delta_params &p) {
     const int64_t heads = (int64_t)p.sequences * p.v_heads;
-    const int from = heads <= 128 ? 10 : heads <= 1024 ? 20 : 32;
-    return p.x_dtype == CC1D_F32 && heads > 128 ? 2 * from + (heads > 1024 ? 64 : 0) : from;
+    if (heads <= 128) return 10;
+    if (heads <= 1024) return p.x_dtype == CC1D_F32 ? 40 : 20;
+    return p.x_dtype == CC1D_F32 ? 160 : 40;
 }
 // The scans reach the 64 rows of a chunk with 32 bits.
 bool near(int dtype, int64_t stride) { return stride >= 0 && stride * elem_bytes(dtype) < ((int64_t)1 << 31) / kChunk; }

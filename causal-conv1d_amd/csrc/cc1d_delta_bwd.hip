@@ -15,7 +15,7 @@
 // every time (one workgroup for all heads of a key, adding in registers, was slower at every size: 4 x 2048 tokens of 8 and 16 heads
 // 656 us for forward and backward and 637 now, 512 tokens of 2 and 16 heads 224 and 106).
 //
-// 4 x 2048 tokens of 16 heads of 128 x 128 in bfloat16, 2048 chunks: prep 53 us, scan 195, gradients 214.  The scan's chain is
+// 4 x 2048 tokens of 16 heads of 128 x 128 in bfloat16, 2048 chunks: prep 54 us, scan 190, gradients 215.  The scan's chain is
 // the forward's with one product more, and it writes 200 MB for the gradients.  Those read 550 MB and write 67, 2.9 TB/s: a third of a
 // workgroup's time (24 us, one a CU) is the part behind the walk over dim_v, where nothing is on its way from memory.  Persistent workgroups that
 // ask for their next chunk in that part were no faster (224 us): 38 to 70 registers more.
