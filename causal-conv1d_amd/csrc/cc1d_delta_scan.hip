@@ -13,8 +13,8 @@
 //
 // What bounds it is the chain from chunk to chunk, 3800 cycles for 128 x 16 columns in bfloat16: S split and through LDS 550, K S and Q S
 // 680, R through LDS 400, T R 700, U through LDS 450, the last products 550, outputs 400.  512 tokens of 32 heads take 19 us.  A chunk's
-// operands are 92 KB in 16 bytes a lane, 1440 cycles of a CU's 64 bytes a cycle, and two workgroups on a CU share that: 4096 packed tokens of 32
-// heads take 114 us (121 with 104 KB; 156 with one workgroup a CU).  float16, two terms each of K and Q, has 143 KB and 7400 cycles: 16384 tokens of
+// operands are 82 KB in 16 bytes a lane, 1300 cycles of a CU's 64 bytes a cycle, and two workgroups on a CU share that: 4096 packed tokens of 32
+// heads take 114 us (121 with 104 KB; 156 with one workgroup a CU).  float16, two terms each of K and Q, has 130 KB and 7400 cycles: 16384 tokens of
 // 16 heads, 128 workgroups, take 651 us.  The states and U that a training forward writes are bandwidth: 4 x 2048 tokens
 // of 16 heads take 118 us without them and 167 with 200 MB of them.  Measured and not taken: 32 columns a workgroup, eight wavefronts
 // with O in four of them, a wavefront for all of dim_k without LDS, operands two chunks ahead, results stored four columns at a time.

@@ -89,3 +89,19 @@ def test_compiled_block(example, gpu_device):
         got = torch.compile(block, backend="aot_eager", fullgraph=True)(x, stream)
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_compiled_training(example, gpu_device):
+    """The same with gradients, which torch.compile takes through the Python functions' graph: the same kernels, the same bits (plain
+    operators around them may be traced into other ones, so float32's rounding of those is allowed: 2^-20 of the largest value)."""
+    block = block_of(example, 3)
+    x, stream = (torch.randn(1, 66, 96, device=gpu_device, requires_grad=True) for _ in range(2))
+    leaves = [x, stream] + list(block.parameters())
+    want = block(x, stream)
+    seeds = [torch.randn_like(t) for t in want]
+    want = list(want) + list(torch.autograd.grad(want, leaves, seeds))
+    got = torch.compile(block, backend="aot_eager", fullgraph=True)(x, stream)
+    got = list(got) + list(torch.autograd.grad(got, leaves, seeds))
+    for a, b in zip(got, want):
+        assert (a - b).abs().max() <= 2.0 ** -20 * b.abs().max()
