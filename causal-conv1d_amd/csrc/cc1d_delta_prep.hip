@@ -6,7 +6,7 @@
 // instructions, first inside each half of 32, then between the halves: (I + A)^-1 of [[X, 0], [A, Y]] has -Y^-1 A X^-1 there.
 // Substitution and not the series of powers of A: those of keys that resemble each other grow to 1e8 before they vanish.
 //
-// One workgroup a CU takes 12 us (256 chunks and heads of 128 in bfloat16), 16000 cycles of latency: 6500 until K and Q are in LDS and
+// One workgroup a CU takes 11.6 us (256 chunks and heads of 128 in bfloat16), 15500 cycles of latency: 6000 until K and Q are in LDS and
 // their lengths known, 2700 for the products, 2000 and 2400 for T's two parts, 2000 to write T and P.  Four to a CU share that: 2048 chunks 53 us, 160 MB
 // written.  K and Q are written out again in operand order: it costs a third of the writes, and saves the scan 10 to 20 %.
 #include "cc1d_delta_chunk.hpp"
@@ -116,16 +116,6 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
                 *reinterpret_cast<u32x4 *>(lds.frags + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
         }
     }
-    if (first) {
-        uint8_t *kd = w.kf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag, *qd = w.qf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag;
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                *reinterpret_cast<u32x4 *>(kd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
-                if (!w.backward) *reinterpret_cast<u32x4 *>(qd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
-            }
-    }
     kk = over_rows(kk);
     qq = over_rows(qq);
     if (g == 0) {
@@ -133,20 +123,6 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
         lds.gate[kQueryNorm][token] = p.qk_l2norm ? rsqrtf(qq + kNormEps) : 1.f;
     }
     lds_barrier();
-
-    if (wave == 0) {                                     // (the products below need none of these)
-        const float gam = lds.gate[kGate][lane], rk = lds.gate[kKeyNorm][lane];
-        const float beta = lds.gate[kBeta][lane];
-        float4 walk;
-        walk.x = beta * gam * rk;                        // kSeenBeta, kWalkBeta, kReadGate, kCarry
-        walk.y = beta;
-        walk.z = p.scale * gam * lds.gate[kQueryNorm][lane];
-        walk.w = lds.gate[kToEnd][lane] * rk;
-        *reinterpret_cast<float4 *>(&lds.gate[0][0] + 4 * lane) = walk;
-        wave_lds_fence();
-#pragma unroll
-        for (int i = 0; i < kScalars; ++i) w.scalars[(sv * kScalars + i) * kChunk + lane] = lds.gate[i][lane];
-    }
 
     // K K^T and Q K^T: this wavefront's 16 rows; columns behind the rows' last are nothing.
     f32x4 read[4];                                       // P waits in registers until A is used up
@@ -191,6 +167,30 @@ delta_prep_kernel(const cc1d_delta_params p, const ChunkWork w) {
     half(0);
     if (wave >= 2) half(1);
     else read[2] = read[3] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // What needs no more work leaves only here: stores in front of the products would hold those up.
+    if (wave == 0) {
+        const float gam = lds.gate[kGate][lane], rk = lds.gate[kKeyNorm][lane];
+        const float beta = lds.gate[kBeta][lane];
+        float4 walk;
+        walk.x = beta * gam * rk;                        // kSeenBeta, kWalkBeta, kReadGate, kCarry
+        walk.y = beta;
+        walk.z = p.scale * gam * lds.gate[kQueryNorm][lane];
+        walk.w = lds.gate[kToEnd][lane] * rk;
+        *reinterpret_cast<float4 *>(&lds.gate[0][0] + 4 * lane) = walk;
+        wave_lds_fence();
+#pragma unroll
+        for (int i = 0; i < kScalars; ++i) w.scalars[(sv * kScalars + i) * kChunk + lane] = lds.gate[i][lane];
+    }
+    if (first) {
+        uint8_t *kd = w.kf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag, *qd = w.qf + sh * w.kbytes() + (int64_t)wave * KS * NT * kFrag;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                *reinterpret_cast<u32x4 *>(kd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(kf[s][n]);
+                if (!w.backward) *reinterpret_cast<u32x4 *>(qd + (s * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(qf[s][n]);
+            }
+    }
     // K^T, then Q^T, gathered from the operands in LDS: token 32 s + 8 g + e is row m' of tile ct, dim_k index k is
     // element k & 7 of lane group (k >> 3) & 3 of step k >> 5.
     auto transposed = [&](uint8_t *dst) {
