@@ -30,6 +30,7 @@ int check_delta(const cc1d_delta_params &p) {
     int st = check_sizes(p);
     if (st != CC1D_OK) return st;
     if (p.sequences < 0 || (p.cu_seqlens == nullptr ? p.sequences != p.batch : p.batch != 1)) return CC1D_ERR_SHAPE;
+    if (p.sequences == 0 && p.batch > 0 && p.seqlen > 0) return CC1D_ERR_SHAPE;        // nobody would write their zeros
     if (p.batch > 0 && p.seqlen > 0 && p.v_heads > 0) st = check_inputs(p);
     if (st != CC1D_OK) return st;
     if (p.saved != nullptr && !aligned256(p.saved)) return CC1D_ERR_WORKSPACE;

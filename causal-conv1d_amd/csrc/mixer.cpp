@@ -86,6 +86,7 @@ int64_t sequences_of(const DeltaInputs &d, const OptTensor &cu) {
     check_gpu(*cu, d.q, "cu_seqlens");
     TORCH_CHECK(d.batch == 1, "cu_seqlens needs a batch of 1: sequences packed back to back");
     TORCH_CHECK(cu->dim() == 1 && cu->size(0) >= 1, "cu_seqlens must be (sequences + 1,)");
+    TORCH_CHECK(cu->size(0) > 1 || d.seqlen == 0, "cu_seqlens names no sequence, but there are tokens");
     TORCH_CHECK(cu->is_contiguous(), "cu_seqlens must be contiguous");
     TORCH_CHECK(cu->scalar_type() == at::kInt || cu->scalar_type() == at::kLong, "cu_seqlens must be int32 or int64");
     return cu->size(0) - 1;

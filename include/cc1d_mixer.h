@@ -31,8 +31,8 @@ extern "C" {
  * of q, k, v are rounded once as they are stored.
  *
  * Without cu_seqlens there are `batch` sequences of `seqlen` tokens.  With it (batch == 1) sequence n
- * is tokens cu_seqlens[n] .. cu_seqlens[n+1]-1, `sequences` of them, ascending; empty ones are
- * allowed, entries outside [0, seqlen] are clamped, and tokens of no sequence give zeros.
+ * is tokens cu_seqlens[n] .. cu_seqlens[n+1]-1, `sequences` of them (one at least where there are
+ * tokens), ascending; empty ones are allowed, entries outside [0, seqlen] are clamped, and tokens of no sequence give zeros.
  * Chunks of 64 tokens are worked out together: a NaN or infinity reaches its head's outputs from the
  * start of its chunk on.
  * ---------------------------------------------------------------------------------- */

@@ -111,6 +111,18 @@ def test_another_stream(pkg, gpu_device, seqlen):
 
 
 @pytest.mark.gpu
+def test_no_sequence(pkg, gpu_device):
+    """Tokens without a sequence are refused (nobody would write their zeros); without tokens there is nothing to do."""
+    q, k, v, g, beta, _ = make(1, 70, 1, 2, 32, 16, torch.bfloat16, gpu_device)
+    cu = torch.zeros(1, dtype=torch.int32, device=gpu_device)
+    for leaf in (v, v.detach().clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="names no sequence"):
+            pkg.gated_delta_rule_fn(q, k, leaf, g, beta, cu_seqlens=cu)
+    out, final = pkg.gated_delta_rule_fn(q[:, :0], k[:, :0], v[:, :0], g[:, :0], beta[:, :0], return_final_states=True, cu_seqlens=cu)
+    assert out.shape == (1, 0, 2, 16) and final.shape == (0, 2, 32, 16)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_values_that_are_not_finite_stay_where_they_belong(pkg, gpu_device, value):
     """In one sequence's token of one head: the chunks in front of it, the other heads and the other sequences do not notice, packed or

@@ -80,6 +80,11 @@ def test_validate_delta_paths(lib):
     p, keep = delta()                                    # packed sequences come in a batch of one
     p.cu_seqlens, p.sequences = cu.data_ptr(), 2
     assert v(p) == E_SHAPE
+    p, keep = delta(batch=1)                             # tokens that belong to no sequence need one that could clear them
+    p.cu_seqlens, p.sequences = cu.data_ptr(), 0
+    assert v(p) == E_SHAPE
+    p.seqlen = 0
+    assert v(p) == OK
     p, keep = delta(batch=0)
     p.q = p.k = p.v = p.g = p.beta = p.out = None
     assert v(p) == OK and lib.cc1d_delta_fwd(p, None, 0, None) == OK
