@@ -60,7 +60,7 @@ def rms_norm_fn(x, weight, residual=None, eps=1e-5):
 
 def rms_norm_quant_fn(x, weight, residual=None, eps=1e-5):
     """(y8, scales), or (y8, scales, h) with a residual: y8 (..., dim) float8_e4m3fn, scales (...) float32 with
-    y = y8 * scales[..., None] and scales = max|y| / 448 of each row.  No backward."""
+    y8 the code next to y / scales[..., None] and scales = max|y| / 448 of each row.  No backward."""
     if not is_compiling():
         res = _ext._rms_norm_quant_call(x, weight, residual, eps)
         if res is not NotImplemented:

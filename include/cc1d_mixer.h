@@ -134,8 +134,9 @@ int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
  *   h = x + residual      (summed in fp32, rounded once to r_dtype; without residual h = x)
  *   y = h rsqrt(mean(h^2) + eps) weight
  *
- * y8 / scales instead of y: scales[row] = max|y| / 448, y8 = y / scales[row] in e4m3 (to nearest, ties
- * to even).  A row of zeros has scale 0 and zeros.
+ * y8 / scales instead of y: scales[row] = max|y| / 448 (to a unit in fp32's last place), y8 = the fp32 quotient
+ * y / scales[row], to nearest, in e4m3, to nearest, ties to even both times; y is not rounded to x_dtype in between.  A
+ * row of zeros has scale 0 and zeros.  A scale below 2^-126 is rounded to what fp32 has there after the quotients are formed.
  * ---------------------------------------------------------------------------------- */
 typedef struct cc1d_norm_params {
     int64_t rows;
