@@ -160,7 +160,8 @@ int cc1d_validate_delta_bwd(const cc1d_delta_bwd_params *p) {
     if (st != CC1D_OK) return st;
     const cc1d_delta_params &f = p->fwd;
     if (f.batch > 0 && f.seqlen > 0 && f.v_heads > 0 &&
-        (f.saved == nullptr || p->dout == nullptr || p->dq == nullptr || p->dk == nullptr || p->dv == nullptr || p->dg == nullptr || p->dbeta == nullptr)) return CC1D_ERR_NULL_POINTER;
+        (f.saved == nullptr || p->dout == nullptr || p->dv == nullptr || p->dg == nullptr || p->dbeta == nullptr)) return CC1D_ERR_NULL_POINTER;
+    if (f.batch > 0 && f.seqlen > 0 && (p->dq == nullptr || p->dk == nullptr)) return CC1D_ERR_NULL_POINTER;           // (written without value heads too)
     if (!on_elements(p->dout, f.x_dtype) || !on_elements(p->dq, f.x_dtype) || !on_elements(p->dk, f.x_dtype) || !on_elements(p->dv, f.x_dtype) ||
         !on_elements(p->dg, f.g_dtype) || !on_elements(p->dbeta, f.beta_dtype) || !on_elements(p->dfinal_states, CC1D_F32) ||
         !on_elements(p->dinitial_states, CC1D_F32)) return CC1D_ERR_ROW_LAYOUT;
@@ -183,8 +184,9 @@ int cc1d_delta_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t works
     int st = cc1d_delta_bwd_workspace_bytes(p, &need);
     if (st != CC1D_OK) return st;
     if (need > 0 && (workspace == nullptr || !aligned256(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
-    if (p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return CC1D_OK;
     const hipStream_t hs = static_cast<hipStream_t>(stream);
+    if (p->fwd.v_heads == 0) return launch_delta_no_values(*p, hs);
+    if (p->fwd.batch == 0 || p->fwd.sequences == 0) return CC1D_OK;
     ChunkWork w;
     lay_out(p->fwd, true, static_cast<uint8_t *>(workspace), w);
     if (w.slots > 0) st = launch_delta_prep(p->fwd, w, hs);

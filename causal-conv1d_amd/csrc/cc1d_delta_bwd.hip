@@ -709,6 +709,20 @@ delta_join_kernel(const cc1d_delta_bwd_params bp, const ChunkWork w, const int v
     rows_leave<DT, KS, kJoinBoth<DT, KS>>(tq, tk, raw, bp, at, hk, vec_out);
 }
 
+// Without value heads nothing comes back to q and k: zeros, a wavefront a row of each.
+template <typename Bits>
+__global__ void __launch_bounds__(kBlock)
+delta_no_values_kernel(const cc1d_delta_bwd_params bp, const int64_t rows) {
+    const cc1d_delta_params &p = bp.fwd;
+    for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+        const int64_t h = r % p.heads, t = r / p.heads % p.seqlen, b = r / p.heads / p.seqlen;
+        for (int k = threadIdx.x & 63; k < p.dim_k; k += 64) {
+            static_cast<Bits *>(bp.dq)[b * bp.dq_stride_b + t * bp.dq_stride_l + h * bp.dq_stride_h + k] = 0;
+            static_cast<Bits *>(bp.dk)[b * bp.dk_stride_b + t * bp.dk_stride_l + h * bp.dk_stride_h + k] = 0;
+        }
+    }
+}
+
 template <int DT, int KS>
 int launch(const cc1d_delta_bwd_params &bp, const ChunkWork &w, hipStream_t stream) {
     const cc1d_delta_params &p = bp.fwd;
@@ -731,6 +745,15 @@ int launch(const cc1d_delta_bwd_params &bp, const ChunkWork &w, hipStream_t stre
 }
 
 }  // namespace
+
+int launch_delta_no_values(const cc1d_delta_bwd_params &bp, hipStream_t stream) {
+    const int64_t rows = (int64_t)bp.fwd.batch * bp.fwd.seqlen * bp.fwd.heads;
+    if (rows == 0) return CC1D_OK;
+    const dim3 grid((uint32_t)(rows < 4 * 8192 ? (rows + 3) / 4 : 8192));
+    if (bp.fwd.x_dtype == CC1D_F32) CC1D_LAUNCH(delta_no_values_kernel<uint32_t>, grid, dim3(kBlock), 0, stream, bp, rows);
+    else CC1D_LAUNCH(delta_no_values_kernel<uint16_t>, grid, dim3(kBlock), 0, stream, bp, rows);
+    return launch_status();
+}
 
 int launch_delta_bwd(const cc1d_delta_bwd_params &bp, const ChunkWork &w, hipStream_t stream) {
     return by_type_and_steps(bp.fwd.x_dtype, w.ks, [&](auto dt, auto ks) { return launch<decltype(dt)::value, decltype(ks)::value>(bp, w, stream); });

@@ -19,6 +19,9 @@ int launch_delta_scan(const cc1d_delta_params &p, const ChunkWork &w, bool save,
 // Backward, behind its own prep: the gradients.
 int launch_delta_bwd(const cc1d_delta_bwd_params &p, const ChunkWork &w, hipStream_t stream);
 
+// Its gradients of q and k where there are no value heads.
+int launch_delta_no_values(const cc1d_delta_bwd_params &bp, hipStream_t stream);
+
 // Every row of a (batch, seqlen, heads, dim) tensor starts on 16 bytes.
 inline bool whole_rows(int dtype, const void *x, int64_t sb, int64_t sl, int64_t sh) {
     const int v = vec_elems(dtype);

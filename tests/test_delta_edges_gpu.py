@@ -1,0 +1,21 @@
+"""The gated delta rule at the edges of what it takes.  Tolerances are those of test_gated_delta_rule_gpu.py and
+test_gated_delta_rule_bwd_gpu.py."""
+import pytest
+import torch
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim_k", [5, 64])
+def test_no_value_heads(pkg, gpu_device, dtype, dim_k):
+    """Nothing depends on q and k then: zeros, whatever the memory of the gradients held before."""
+    q, k = (torch.randn(2, 70, 3, dim_k, device=gpu_device, dtype=dtype).requires_grad_() for _ in range(2))
+    v = torch.randn(2, 70, 0, 16, device=gpu_device, dtype=dtype).requires_grad_()
+    g = torch.zeros(2, 70, 0, device=gpu_device)
+    out, final = pkg.gated_delta_rule_fn(q, k, v, g, g, return_final_states=True)
+    assert out.shape == v.shape and final.shape == (2, 0, dim_k, 16)
+    used = [torch.full_like(q, float("nan")) for _ in range(8)]              # what the allocator hands out next
+    torch.cuda.synchronize()
+    del used
+    dq, dk, dv = torch.autograd.grad([out, final], [q, k, v], [torch.ones_like(out), torch.ones_like(final)])
+    assert dv.shape == v.shape and torch.equal(dq, torch.zeros_like(q)) and torch.equal(dk, torch.zeros_like(k))
