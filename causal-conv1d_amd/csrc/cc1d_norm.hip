@@ -500,6 +500,9 @@ RowShape row_shape(int dim, int vectors) {
     const int lanes = (dim + 512 * vectors - 1) / (512 * vectors) * 64;
     return {lanes <= 512 ? 512 : 1024, vectors, lanes};
 }
+// Lanes step along such a row by 1024 vectors, and a step has to stay within 32 bits; norm_dweight_kernel takes 1024 threads for 32 columns, and a
+// launch has fewer than 2^32.
+constexpr int kLongestRow = INT32_MAX - 1024 * 8, kLongestRowBwd = (1 << 27) - 32;
 RowShape fwd_shape(int dim) { return row_shape(dim, 2); }
 RowShape bwd_shape(int dim) { return row_shape(dim, 1); }
 template <typename F>
@@ -536,6 +539,7 @@ int cc1d_validate_norm(const cc1d_norm_params *p) {
     if ((p->r_dtype != p->x_dtype && p->r_dtype != CC1D_F32) || (p->w_dtype != p->x_dtype && p->w_dtype != CC1D_F32)) return CC1D_ERR_DTYPE;
     if (p->rows < 0 || p->dim < 0) return CC1D_ERR_SHAPE;
     if (p->rows == 0 || p->dim == 0) return CC1D_OK;
+    if (p->dim > kLongestRow) return CC1D_ERR_TOO_LARGE;
     if (p->x == nullptr || p->weight == nullptr || (p->y == nullptr) == (p->y8 == nullptr)) return CC1D_ERR_NULL_POINTER;
     if ((p->residual == nullptr) != (p->h == nullptr)) return CC1D_ERR_NULL_POINTER;
     if (p->y8 != nullptr && p->scales == nullptr) return CC1D_ERR_NULL_POINTER;
@@ -574,6 +578,7 @@ int cc1d_validate_norm_bwd(const cc1d_norm_bwd_params *p) {
     if ((p->r_dtype != p->x_dtype && p->r_dtype != CC1D_F32) || (p->w_dtype != p->x_dtype && p->w_dtype != CC1D_F32)) return CC1D_ERR_DTYPE;
     if (p->rows < 0 || p->dim < 0) return CC1D_ERR_SHAPE;
     if (p->dim == 0) return CC1D_OK;
+    if (p->dim > kLongestRowBwd) return CC1D_ERR_TOO_LARGE;
     if (p->dweight == nullptr) return CC1D_ERR_NULL_POINTER;
     if (p->rows == 0) return CC1D_OK;
     if (p->h == nullptr || p->weight == nullptr || p->dy == nullptr) return CC1D_ERR_NULL_POINTER;
@@ -627,7 +632,7 @@ int cc1d_validate_dequantize(const cc1d_dequantize_params *p) {
 int cc1d_dequantize_rows(const cc1d_dequantize_params *p, cc1d_stream_t stream) {
     const int st = cc1d_validate_dequantize(p);
     if (st != CC1D_OK || p->rows == 0 || p->dim == 0) return st;
-    const uint32_t vecs = (uint32_t)(p->dim + 7) / 8;
+    const uint32_t vecs = ((uint32_t)p->dim + 7) / 8;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t slice = thread_limit() / vecs > 1 ? thread_limit() / vecs : 1;         // (a row has at most 2^28 vectors)
     for (int64_t first = 0; first < p->rows; first += slice) {

@@ -140,7 +140,7 @@ int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
  * ---------------------------------------------------------------------------------- */
 typedef struct cc1d_norm_params {
     int64_t rows;
-    int32_t dim;
+    int32_t dim;                     /* up to 2^31 - 8193; backward: 2^27 - 32 */
     int32_t x_dtype, r_dtype, w_dtype; /* of x and y; of residual and h; of weight */
     float eps;
     int32_t reserved0;
