@@ -5,6 +5,9 @@
 #include <torch/library.h>
 #include <torch/types.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
@@ -594,6 +597,47 @@ PyObject *delta_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- what autograd is told of an op ----------------------------------------------------
+// The graphs above (and those of the Python functions) are recorded around the ops, with gradients off inside.  An op that is called on
+// tensors that require a gradient all the same (the backward under create_graph, or the op itself) has no derivative: its results
+// say so when somebody asks for one, where the dispatcher's fallback would give zeros and a warning.
+
+template <typename T> void add_edge(torch::autograd::edge_list &, const T &) {}
+void add_edge(torch::autograd::edge_list &all, const at::Tensor &t) {
+    if (t.defined() && t.requires_grad()) all.push_back(torch::autograd::impl::gradient_edge(t));
+}
+void add_edge(torch::autograd::edge_list &all, const OptTensor &t) { if (t.has_value()) add_edge(all, *t); }
+
+void end_graph(const at::Tensor &t, const std::shared_ptr<torch::autograd::Node> &node) {
+    if (t.defined() && torch::autograd::isDifferentiableType(t.scalar_type())) torch::autograd::set_history(t, node);
+}
+template <typename... R>
+void end_graph(const std::tuple<R...> &all, const std::shared_ptr<torch::autograd::Node> &node) {
+    std::apply([&](const R &...t) { (end_graph(t, node), ...); }, all);
+}
+
+template <const char *NAME, typename F> struct Graphless;
+template <const char *NAME, typename R, typename... A>
+struct Graphless<NAME, R(A...)> {
+    static R call(A... args) {
+        static const auto op = typed_op<R(A...)>(NAME);
+        torch::autograd::edge_list edges;
+        if (at::GradMode::is_enabled()) (add_edge(edges, args), ...);
+        R r = [&] {
+            at::AutoDispatchBelowADInplaceOrView below;
+            return op.call(args...);
+        }();
+        if (!edges.empty()) end_graph(r, std::shared_ptr<torch::autograd::Node>(new torch::autograd::NotImplemented(NAME, std::move(edges)), torch::autograd::deleteNode));
+        return r;
+    }
+};
+#define OP_NAME(ID, OP) constexpr char ID[] = "DaoAILab::" OP
+OP_NAME(kDeltaFwd, "_gated_delta_rule_fwd_cpp");
+OP_NAME(kDeltaFwdSave, "_gated_delta_rule_fwd_save_cpp");
+OP_NAME(kDeltaBwd, "_gated_delta_rule_bwd_cpp");
+OP_NAME(kNormFwd, "_rms_norm_fwd_cpp");
+OP_NAME(kNormBwd, "_rms_norm_bwd_cpp");
+
 #define DIRECT_CALL(NAME, F) {NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&F)), METH_FASTCALL, nullptr}
 PyMethodDef calls[] = {DIRECT_CALL("_rms_norm_call", norm_call),
                        DIRECT_CALL("_rms_norm_quant_call", norm_quant_call),
@@ -642,4 +686,12 @@ TORCH_LIBRARY_IMPL(DaoAILab, Meta, m) {
     m.impl("_rms_norm_bwd_cpp", &norm_bwd_meta);
     m.impl("_rms_norm_quant_cpp", &norm_quant_meta);
     m.impl("_dequantize_rows_cpp", &dequantize_meta);
+}
+
+TORCH_LIBRARY_IMPL(DaoAILab, Autograd, m) {
+    m.impl("_gated_delta_rule_fwd_cpp", &Graphless<kDeltaFwd, decltype(delta_fwd)>::call);
+    m.impl("_gated_delta_rule_fwd_save_cpp", &Graphless<kDeltaFwdSave, decltype(delta_fwd_save)>::call);
+    m.impl("_gated_delta_rule_bwd_cpp", &Graphless<kDeltaBwd, decltype(delta_bwd)>::call);
+    m.impl("_rms_norm_fwd_cpp", &Graphless<kNormFwd, decltype(norm_fwd)>::call);
+    m.impl("_rms_norm_bwd_cpp", &Graphless<kNormBwd, decltype(norm_bwd)>::call);
 }

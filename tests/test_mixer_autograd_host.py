@@ -1,0 +1,62 @@
+"""What autograd is told by the mixer's operators, on meta tensors, without a GPU: nothing is cut off or left out without a word."""
+import pytest
+import torch
+
+
+def _meta(*shape, grad=False, dtype=torch.float32):
+    return torch.empty(*shape, device="meta", dtype=dtype, requires_grad=grad)
+
+
+def _delta(grad=False):
+    """q, k, v, g, beta, states"""
+    return [_meta(2, 9, 2, 16, grad=grad), _meta(2, 9, 2, 16, grad=grad), _meta(2, 9, 4, 24, grad=grad), _meta(2, 9, 4, grad=grad), _meta(2, 9, 4, grad=grad),
+            _meta(2, 4, 16, 24, grad=grad)]
+
+
+def _norm(grad=False):
+    """x, weight, residual"""
+    return [_meta(3, 40, grad=grad), _meta(40, grad=grad), _meta(3, 40, grad=grad)]
+
+
+def _delta_out(pkg, a):
+    return pkg.gated_delta_rule_fn(*a[:5], initial_states=a[5], return_final_states=True)
+
+
+def _norm_out(pkg, a):
+    return pkg.rms_norm_fn(a[0], a[1], residual=a[2])
+
+
+def _python_delta(pkg, a):
+    from causal_conv1d.gated_delta_rule import GatedDeltaRuleFn
+    return GatedDeltaRuleFn.apply(*a[:5], 0.25, a[5], True, None, False)
+
+
+def _python_norm(pkg, a):
+    from causal_conv1d.rms_norm import RMSNormFn
+    return RMSNormFn.apply(*a, 1e-5)
+
+
+@pytest.mark.parametrize("make,run", [(_delta, _delta_out), (_norm, _norm_out), (_delta, _python_delta), (_norm, _python_norm)])
+def test_second_derivatives_are_refused(pkg, make, run, recwarn):
+    """A first derivative may be asked for with its graph; differentiating that is an error, not a zero with a warning."""
+    leaves = make(grad=True)
+    outs = run(pkg, leaves)
+    grads = torch.autograd.grad(outs, leaves, [torch.empty_like(t) for t in outs], create_graph=True)
+    for g in grads:
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="derivative for .* is not implemented"):
+            torch.autograd.grad(g.sum(), leaves, allow_unused=True, retain_graph=True)
+    assert not [w for w in recwarn if "autograd kernel was not registered" in str(w.message)]
+    plain = torch.autograd.grad(run(pkg, leaves)[0].sum(), leaves[:2])
+    assert not any(g.requires_grad for g in plain)
+
+
+def test_ops_without_a_graph_say_so(pkg):
+    """The ops behind the functions, called as they are on tensors that require a gradient."""
+    ops = torch.ops.DaoAILab
+    q, k, v, g, beta, s = _delta(grad=True)
+    x, w, r = _norm(grad=True)
+    for outs in (ops._gated_delta_rule_fwd_cpp(q, k, v, g, beta, s, None, None, 0.25, False),
+                 ops._gated_delta_rule_fwd_save_cpp(q, k, v, g, beta, s, None, None, 0.25, False)[0], ops._rms_norm_fwd_cpp(x, w, r, 1e-5)[0]):
+        with pytest.raises(RuntimeError, match="derivative for .* is not implemented"):
+            outs.sum().backward()
