@@ -600,13 +600,20 @@ PyObject *delta_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
 // ---- what autograd is told of an op ----------------------------------------------------
 // The graphs above (and those of the Python functions) are recorded around the ops, with gradients off inside.  An op that is called on
 // tensors that require a gradient all the same (the backward under create_graph, or the op itself) has no derivative: its results
-// say so when somebody asks for one, where the dispatcher's fallback would give zeros and a warning.
+// say so when somebody asks for one, where the dispatcher's fallback would give zeros and a warning.  A tangent would be lost here
+// without a trace, so it is refused.
 
 template <typename T> void add_edge(torch::autograd::edge_list &, const T &) {}
 void add_edge(torch::autograd::edge_list &all, const at::Tensor &t) {
     if (t.defined() && t.requires_grad()) all.push_back(torch::autograd::impl::gradient_edge(t));
 }
 void add_edge(torch::autograd::edge_list &all, const OptTensor &t) { if (t.has_value()) add_edge(all, *t); }
+
+template <typename T> void refuse_tangent(const char *, const T &) {}
+void refuse_tangent(const char *name, const at::Tensor &t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name, ": forward-mode derivatives (jvp) are not implemented");
+}
+void refuse_tangent(const char *name, const OptTensor &t) { if (t.has_value()) refuse_tangent(name, *t); }
 
 void end_graph(const at::Tensor &t, const std::shared_ptr<torch::autograd::Node> &node) {
     if (t.defined() && torch::autograd::isDifferentiableType(t.scalar_type())) torch::autograd::set_history(t, node);
@@ -621,6 +628,7 @@ template <const char *NAME, typename R, typename... A>
 struct Graphless<NAME, R(A...)> {
     static R call(A... args) {
         static const auto op = typed_op<R(A...)>(NAME);
+        (refuse_tangent(NAME, args), ...);
         torch::autograd::edge_list edges;
         if (at::GradMode::is_enabled()) (add_edge(edges, args), ...);
         R r = [&] {

@@ -60,3 +60,19 @@ def test_ops_without_a_graph_say_so(pkg):
                  ops._gated_delta_rule_fwd_save_cpp(q, k, v, g, beta, s, None, None, 0.25, False)[0], ops._rms_norm_fwd_cpp(x, w, r, 1e-5)[0]):
         with pytest.raises(RuntimeError, match="derivative for .* is not implemented"):
             outs.sum().backward()
+
+
+@pytest.mark.parametrize("make,run", [(_delta, _delta_out), (_norm, _norm_out), (_delta, _python_delta), (_norm, _python_norm)])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(pkg, make, run, grad):
+    """Forward-mode differentiation: of any input, whether it requires a gradient or not, and with gradients off."""
+    args = make(grad=grad)
+    for i in range(len(args)):
+        with torch.autograd.forward_ad.dual_level():
+            dual = [torch.autograd.forward_ad.make_dual(t, torch.empty_like(t)) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(RuntimeError, match="jvp"):
+                run(pkg, dual)
+            if run in (_delta_out, _norm_out):
+                with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                    run(pkg, dual)
+    run(pkg, args)
