@@ -93,7 +93,8 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_states=None, retur
 
 
 def gated_delta_rule_update(q, k, v, g, beta, state, scale=None, state_indices=None, qk_l2norm=False):
-    """The step of a decode loop: out like v, and the states advanced in place.  No backward.
+    """The step of a decode loop: out like v, and the states advanced in place.  No backward: out
+    belongs to no graph, and a state that requires a gradient is refused where gradients are recorded.
 
     q, k (batch, heads, dim_k), v (batch, v_heads, dim_v), g, beta (batch, v_heads); or all of them with a seqlen axis
     behind the batch, for a few tokens at once.  state (slots, v_heads, dim_k, dim_v) float32.

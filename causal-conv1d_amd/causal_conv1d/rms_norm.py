@@ -65,7 +65,7 @@ def rms_norm_quant_fn(x, weight, residual=None, eps=1e-5):
         res = _ext._rms_norm_quant_call(x, weight, residual, eps)
         if res is not NotImplemented:
             return res
-    y8, scales, h = _quant(x.detach(), weight.detach(), None if residual is None else residual.detach(), eps)
+    y8, scales, h = _quant(x, weight, residual, eps)
     return (y8, scales) if residual is None else (y8, scales, h)
 
 

@@ -510,7 +510,6 @@ PyObject *norm_quant_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 4 || !plain_all(a, 2) || !plain_or_none(a[2]) || !PyFloat_Check(a[3]) || generic_path_needed()) NOT_IMPLEMENTED();
     static const auto op = typed_op<decltype(norm_quant)>("DaoAILab::_rms_norm_quant_cpp");
     const at::Tensor x = THPVariable_Unpack(a[0]), weight = THPVariable_Unpack(a[1]), r = or_undefined(optional_tensor(a[2]));
-    if (wants_grad({&x, &weight, &r})) NOT_IMPLEMENTED();
     std::tuple<at::Tensor, at::Tensor, at::Tensor> t;
     {
         pybind11::gil_scoped_release no_gil;
@@ -623,14 +622,25 @@ void end_graph(const std::tuple<R...> &all, const std::shared_ptr<torch::autogra
     std::apply([&](const R &...t) { (end_graph(t, node), ...); }, all);
 }
 
-template <const char *NAME, typename F> struct Graphless;
-template <const char *NAME, typename R, typename... A>
-struct Graphless<NAME, R(A...)> {
+// What an op writes in place: part of no graph that is being recorded, whose gradients it would make wrong.
+void check_written(const char *name, const at::Tensor &t) {
+    TORCH_CHECK(!t.defined() || !t.requires_grad() || !at::GradMode::is_enabled(), name, ": a tensor that is written in place requires a gradient");
+}
+void check_written(const char *name, const OptTensor &t) { if (t.has_value()) check_written(name, *t); }
+
+// ENDS: the op has a function that records a graph around it.  The others have no backward: their results belong to no graph.
+// WRITTEN: which argument is written in place, or -1.
+template <const char *NAME, bool ENDS, int WRITTEN, typename F> struct Graphless;
+template <const char *NAME, bool ENDS, int WRITTEN, typename R, typename... A>
+struct Graphless<NAME, ENDS, WRITTEN, R(A...)> {
     static R call(A... args) {
         static const auto op = typed_op<R(A...)>(NAME);
-        (refuse_tangent(NAME, args), ...);
+        if constexpr (WRITTEN >= 0) check_written(NAME, std::get<WRITTEN>(std::tie(args...)));
         torch::autograd::edge_list edges;
-        if (at::GradMode::is_enabled()) (add_edge(edges, args), ...);
+        if constexpr (ENDS) {
+            (refuse_tangent(NAME, args), ...);
+            if (at::GradMode::is_enabled()) (add_edge(edges, args), ...);
+        }
         R r = [&] {
             at::AutoDispatchBelowADInplaceOrView below;
             return op.call(args...);
@@ -643,8 +653,11 @@ struct Graphless<NAME, R(A...)> {
 OP_NAME(kDeltaFwd, "_gated_delta_rule_fwd_cpp");
 OP_NAME(kDeltaFwdSave, "_gated_delta_rule_fwd_save_cpp");
 OP_NAME(kDeltaBwd, "_gated_delta_rule_bwd_cpp");
+OP_NAME(kDeltaUpdate, "_gated_delta_rule_update_cpp");
 OP_NAME(kNormFwd, "_rms_norm_fwd_cpp");
 OP_NAME(kNormBwd, "_rms_norm_bwd_cpp");
+OP_NAME(kNormQuant, "_rms_norm_quant_cpp");
+OP_NAME(kDequantize, "_dequantize_rows_cpp");
 
 #define DIRECT_CALL(NAME, F) {NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&F)), METH_FASTCALL, nullptr}
 PyMethodDef calls[] = {DIRECT_CALL("_rms_norm_call", norm_call),
@@ -697,9 +710,12 @@ TORCH_LIBRARY_IMPL(DaoAILab, Meta, m) {
 }
 
 TORCH_LIBRARY_IMPL(DaoAILab, Autograd, m) {
-    m.impl("_gated_delta_rule_fwd_cpp", &Graphless<kDeltaFwd, decltype(delta_fwd)>::call);
-    m.impl("_gated_delta_rule_fwd_save_cpp", &Graphless<kDeltaFwdSave, decltype(delta_fwd_save)>::call);
-    m.impl("_gated_delta_rule_bwd_cpp", &Graphless<kDeltaBwd, decltype(delta_bwd)>::call);
-    m.impl("_rms_norm_fwd_cpp", &Graphless<kNormFwd, decltype(norm_fwd)>::call);
-    m.impl("_rms_norm_bwd_cpp", &Graphless<kNormBwd, decltype(norm_bwd)>::call);
+    m.impl("_gated_delta_rule_fwd_cpp", &Graphless<kDeltaFwd, true, 7, decltype(delta_fwd)>::call);
+    m.impl("_gated_delta_rule_fwd_save_cpp", &Graphless<kDeltaFwdSave, true, 7, decltype(delta_fwd_save)>::call);
+    m.impl("_gated_delta_rule_bwd_cpp", &Graphless<kDeltaBwd, true, -1, decltype(delta_bwd)>::call);
+    m.impl("_gated_delta_rule_update_cpp", &Graphless<kDeltaUpdate, false, 5, decltype(delta_update)>::call);
+    m.impl("_rms_norm_fwd_cpp", &Graphless<kNormFwd, true, -1, decltype(norm_fwd)>::call);
+    m.impl("_rms_norm_bwd_cpp", &Graphless<kNormBwd, true, -1, decltype(norm_bwd)>::call);
+    m.impl("_rms_norm_quant_cpp", &Graphless<kNormQuant, false, -1, decltype(norm_quant)>::call);
+    m.impl("_dequantize_rows_cpp", &Graphless<kDequantize, false, -1, decltype(dequantize)>::call);
 }

@@ -76,3 +76,32 @@ def test_tangents_are_refused(pkg, make, run, grad):
                 with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
                     run(pkg, dual)
     run(pkg, args)
+
+
+def test_what_has_no_backward_claims_none(pkg, recwarn):
+    """The decode step, the output in 8 bits and its reading back: results outside of any graph, through the functions and the ops."""
+    ops = torch.ops.DaoAILab
+    q, k, v, g, beta, _ = _delta(grad=True)
+    state = _meta(2, 4, 16, 24)
+    x, w, r = _norm(grad=True)
+    y8, scales = _meta(3, 40, dtype=torch.float8_e4m3fn), _meta(3, grad=True)
+    for outs in ([pkg.gated_delta_rule_update(q, k, v, g, beta, state)], [ops._gated_delta_rule_update_cpp(q, k, v, g, beta, state, None, 0.25, False)],
+                 pkg.rms_norm_quant_fn(x, w, residual=r), ops._rms_norm_quant_cpp(x, w, r, 1e-5), [pkg.dequantize_rows(y8, scales)],
+                 [ops._dequantize_rows_cpp(y8, scales, torch.bfloat16)]):
+        assert not any(t.requires_grad for t in outs)
+    assert not state.requires_grad
+    assert not [w for w in recwarn if "autograd kernel was not registered" in str(w.message)]
+
+
+def test_states_with_a_graph_are_not_written(pkg):
+    """What an operator writes in place may not be part of a graph that gradients are recorded for: its gradient would be wrong."""
+    q, k, v, g, beta, s = _delta()
+    leaf = _meta(2, 4, 16, 24, grad=True)
+    for state in (leaf, leaf * 2):
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            pkg.gated_delta_rule_update(q, k, v, g, beta, state)
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            pkg.gated_delta_rule_fn(q, k, v, g, beta, return_final_states=True, final_states_out=state)
+        with torch.no_grad():
+            pkg.gated_delta_rule_update(q, k, v, g, beta, state)
+            pkg.gated_delta_rule_fn(q, k, v, g, beta, return_final_states=True, final_states_out=state)
