@@ -628,6 +628,10 @@ void check_written(const char *name, const at::Tensor &t) {
 }
 void check_written(const char *name, const OptTensor &t) { if (t.has_value()) check_written(name, *t); }
 
+// As torch's own operators do, so that a graph which has saved the tensor notices.  Tensors made in inference mode count nothing.
+void count_write(const at::Tensor &t) { if (t.defined() && !t.is_inference()) torch::autograd::impl::bump_version(t); }
+void count_write(const OptTensor &t) { if (t.has_value()) count_write(*t); }
+
 // ENDS: the op has a function that records a graph around it.  The others have no backward: their results belong to no graph.
 // WRITTEN: which argument is written in place, or -1.
 template <const char *NAME, bool ENDS, int WRITTEN, typename F> struct Graphless;
@@ -645,6 +649,7 @@ struct Graphless<NAME, ENDS, WRITTEN, R(A...)> {
             at::AutoDispatchBelowADInplaceOrView below;
             return op.call(args...);
         }();
+        if constexpr (WRITTEN >= 0) count_write(std::get<WRITTEN>(std::tie(args...)));
         if (!edges.empty()) end_graph(r, std::shared_ptr<torch::autograd::Node>(new torch::autograd::NotImplemented(NAME, std::move(edges)), torch::autograd::deleteNode));
         return r;
     }

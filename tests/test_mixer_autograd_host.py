@@ -105,3 +105,25 @@ def test_states_with_a_graph_are_not_written(pkg):
         with torch.no_grad():
             pkg.gated_delta_rule_update(q, k, v, g, beta, state)
             pkg.gated_delta_rule_fn(q, k, v, g, beta, return_final_states=True, final_states_out=state)
+
+
+def test_writing_in_place_moves_the_version(pkg):
+    """As torch's own operators do: a graph that has saved a state notices that it has changed since."""
+    ops = torch.ops.DaoAILab
+    q, k, v, g, beta, _ = _delta()
+    for write in (lambda s: pkg.gated_delta_rule_update(q, k, v, g, beta, s), lambda s: ops._gated_delta_rule_update_cpp(q, k, v, g, beta, s, None, 0.25, False),
+                  lambda s: pkg.gated_delta_rule_fn(q, k, v, g, beta, initial_states=s, return_final_states=True, final_states_out=s),
+                  lambda s: ops._gated_delta_rule_fwd_save_cpp(q, k, v, g, beta, None, None, s, 0.25, False)):
+        state, w = _meta(2, 4, 16, 24), _meta(2, 4, 16, 24, grad=True)
+        out = (state * w).sum()
+        before = state._version
+        with torch.no_grad():
+            write(state)
+        assert state._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward()
+    with torch.inference_mode():
+        state = _meta(2, 4, 16, 24)
+        pkg.gated_delta_rule_update(q, k, v, g, beta, state)
+    with torch.no_grad():
+        pkg.gated_delta_rule_update(q, k, v, g, beta, state)                 # (a server's states, made in inference mode)
