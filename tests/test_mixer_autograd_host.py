@@ -1,6 +1,9 @@
 """What autograd is told by the mixer's operators, on meta tensors, without a GPU: nothing is cut off or left out without a word."""
+import contextlib
+
 import pytest
 import torch
+from torch._dynamo import compiled_autograd
 
 
 def _meta(*shape, grad=False, dtype=torch.float32):
@@ -127,3 +130,12 @@ def test_writing_in_place_moves_the_version(pkg):
         pkg.gated_delta_rule_update(q, k, v, g, beta, state)
     with torch.no_grad():
         pkg.gated_delta_rule_update(q, k, v, g, beta, state)                 # (a server's states, made in inference mode)
+
+
+@pytest.mark.parametrize("make,run", [(_delta, _delta_out), (_norm, _norm_out)])
+@pytest.mark.parametrize("compiled", [False, True], ids=["engine", "compiled_autograd"])
+def test_every_gradient_arrives(pkg, make, run, compiled):
+    leaves = make(grad=True)
+    with compiled_autograd._enable(torch.compile(backend="eager")) if compiled else contextlib.nullcontext():
+        sum(t.sum() for t in run(pkg, leaves)).backward()
+    assert [None if t.grad is None else t.grad.shape for t in leaves] == [t.shape for t in leaves]
