@@ -2,6 +2,7 @@
 import ctypes as C
 
 import pytest
+import torch
 
 import cabi
 import cabi_mixer as mixer
@@ -42,3 +43,22 @@ def test_rows_of_nearly_2_31_elements(lib):
         assert lib.cc1d_validate_norm_bwd(p) == want, dim
         if want != OK:
             assert lib.cc1d_norm_bwd_workspace_bytes(p, C.byref(n)) == want and lib.cc1d_norm_bwd(p, None, 0, None) == want
+
+
+@pytest.mark.parametrize("batch,seqlen,sequences", [(2, 100, None), (1, 64, None), (3, 0, None), (0, 70, None), (2, 1, None), (1, 100, 1), (1, 1000, 7), (1, 64, 3),
+                                                    (1, 5, 90), (1, 0, 1), (1, 0, 4), (1, 0, 0)])
+@pytest.mark.parametrize("v_heads,dim_k,dim_v", [(4, 16, 24), (2, 33, 7), (0, 16, 16)])
+def test_saved_bytes_of_a_traced_call(lib, pkg, batch, seqlen, sequences, v_heads, dim_k, dim_v):
+    """The shape that the op has on the meta device is what the library asks for."""
+    q = torch.empty(batch, seqlen, 2, dim_k)
+    v = torch.empty(batch, seqlen, v_heads, dim_v)
+    g = torch.empty(batch, seqlen, v_heads)
+    cu = None if sequences is None else torch.zeros(sequences + 1, dtype=torch.int32)
+    p = mixer.delta_params(q, q, v, g, g, v)
+    if cu is not None:
+        p.cu_seqlens, p.sequences = cu.data_ptr(), sequences
+    n = C.c_size_t()
+    assert lib.cc1d_delta_saved_bytes(p, C.byref(n)) == OK
+    meta = [None if t is None else t.to("meta") for t in (q, q, v, g, g, None, cu)]
+    out, saved = torch.ops.DaoAILab._gated_delta_rule_fwd_save_cpp(*meta, None, 1.0, False)
+    assert out.shape == v.shape and tuple(saved.shape) == (n.value,)
