@@ -3,6 +3,8 @@
 //   h = x + residual,  y = h r w,  r = rsqrt(mean(h^2) + eps)
 //   dx = dh + r (w dy) - h r^3 mean(h w dy),  dw = sum over rows of dy h r
 //
+// dx is formed as dh + r (w dy - (h r) (r mean(h w dy))), whose factors are of the size of w dy for rows of any size (r^3 is no normal
+// number of 32 bits for rows of 2^42 on, and infinite below 2^-42).
 // All of it is bound by memory: a few operations an element.  A row is held in registers between its one reading
 // and its one writing, NV vectors of 8 elements a lane: a wavefront a row (T = 64, no barrier), else a workgroup of
 // at most T lanes, as many wavefronts as the row fills.  Rows of any length and address take the same path, 16-byte
@@ -349,14 +351,15 @@ norm_bwd_kernel(const cc1d_norm_bwd_params p, float *planes, const int64_t rows_
 #pragma unroll
                 for (int i = 0; i < 8; ++i) { sq += h[v][i] * h[v][i]; hd += h[v][i] * (w[v][i] * dy[v][i]); }
             over_rows_waves(sq, hd);
-            const float r = rsqrtf(sq * over + p.eps), back = r * r * r * (hd * over);
+            const float r = rsqrtf(sq * over + p.eps), back = hd * over * r;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int c = (v * lanes + lane) * 8;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    dw[v][i] += dy[v][i] * (h[v][i] * r);
-                    d[v][i] += r * (w[v][i] * dy[v][i]) - h[v][i] * back;
+                    const float unit = h[v][i] * r;
+                    dw[v][i] += dy[v][i] * unit;
+                    d[v][i] += r * (w[v][i] * dy[v][i] - unit * back);
                 }
                 if (c < p.dim) put(row, c, d[v]);
             }
@@ -391,7 +394,7 @@ norm_bwd_kernel(const cc1d_norm_bwd_params p, float *planes, const int64_t rows_
                 for (int i = 0; i < 8; ++i) { sq += h[i] * h[i]; hd += h[i] * (wv[i] * dy[i]); }
             }
             over_rows_waves(sq, hd);
-            const float r = rsqrtf(sq * over + p.eps), back = r * r * r * (hd * over);
+            const float r = rsqrtf(sq * over + p.eps), back = hd * over * r;
             for (int c = lane * 8; c < p.dim; c += lanes * 8) {
                 float h[8], dy[8], wv[8], acc[8], d[8];
                 load8<RD>(p.h, row * p.h_stride, c, p.dim, h);
@@ -403,8 +406,9 @@ norm_bwd_kernel(const cc1d_norm_bwd_params p, float *planes, const int64_t rows_
                 if (p.dh != nullptr) load8<RD>(p.dh, row * p.dh_stride, c, p.dim, d);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    acc[i] += dy[i] * (h[i] * r);
-                    d[i] += r * (wv[i] * dy[i]) - h[i] * back;
+                    const float unit = h[i] * r;
+                    acc[i] += dy[i] * unit;
+                    d[i] += r * (wv[i] * dy[i] - unit * back);
                 }
                 store8<CC1D_F32>(plane, c, p.dim - c, acc);
                 put(row, c, d);
