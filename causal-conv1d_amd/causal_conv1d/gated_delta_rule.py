@@ -68,7 +68,7 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_states=None, retur
 
     scale: 1 / sqrt(dim_k) if None.  qk_l2norm: q and k are divided by their length, sqrt(sum of squares + 1e-6).
     initial_states (sequences, v_heads, dim_k, dim_v) float32, zeros if None; final_states like it, written to
-    final_states_out if given (which may be initial_states itself; without gradients only).
+    final_states_out if given (which may be initial_states itself; without gradients only, and with return_final_states only).
     cu_seqlens (sequences + 1,) int32 or int64, ascending from 0 to seqlen, with a batch of 1: sequence n is tokens
     cu_seqlens[n] .. cu_seqlens[n+1]-1; a sequence may be empty."""
     if not is_compiling():
@@ -81,7 +81,7 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_states=None, retur
     if cu_seqlens is not None:
         cu_seqlens = cu_seqlens.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states)):
-        if final_states_out is not None:
+        if return_final_states and final_states_out is not None:
             raise RuntimeError("final_states_out cannot be given where gradients are recorded")
         return GatedDeltaRuleFn.apply(q, k, v, g, beta, float(scale), initial_states, return_final_states, cu_seqlens, qk_l2norm)
     if not return_final_states:

@@ -139,3 +139,15 @@ def test_every_gradient_arrives(pkg, make, run, compiled):
     with compiled_autograd._enable(torch.compile(backend="eager")) if compiled else contextlib.nullcontext():
         sum(t.sum() for t in run(pkg, leaves)).backward()
     assert [None if t.grad is None else t.grad.shape for t in leaves] == [t.shape for t in leaves]
+
+
+def test_final_states_out_that_is_not_asked_for(pkg):
+    """Without return_final_states it is left alone, whichever of the two graphs records the call (a scale that is no float: the Python one)."""
+    a = _delta(grad=True)
+    for scale in (0.25, 1):
+        for args in (a, [t.detach() for t in a]):
+            s = _meta(2, 4, 16, 24)
+            out = pkg.gated_delta_rule_fn(*args[:5], scale=scale, initial_states=args[5], final_states_out=s)
+            assert out.shape == a[2].shape and s._version == 0
+        with pytest.raises(RuntimeError, match="where gradients are recorded"):
+            pkg.gated_delta_rule_fn(*a[:5], scale=scale, return_final_states=True, final_states_out=s)
