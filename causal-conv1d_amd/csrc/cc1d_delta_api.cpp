@@ -38,8 +38,8 @@ int check_delta(const cc1d_delta_params &p) {
     return CC1D_OK;
 }
 
-// Sequences of this many tokens on average go by chunks.  A token costs the token kernel 1.3 us as long as its states fill no more than
-// the card, a chunk costs as much for one token as for 64.  Heads of 128 x 128, token by token / by chunks, us:
+// Sequences of this many tokens on average go by chunks.  A token costs the token kernel 1.3 us as long as its states fill no more than the card,
+// a chunk costs as much for one token as for 64.  Measured with heads of 128 x 128 and applied to all, token by token / by chunks, us:
 //   bfloat16  32 heads:  8 tokens 15.9 / 14.9   256: 20 tokens 33.7 / 32.3   2048: 32 tokens 203 / 235, 48: 293 / 251
 //   float32   32 heads: 12 tokens 20.5 / 19.4   256: 40 tokens 59.2 / 61.1   2048: 96 tokens 538 / 810, 128: 712 / 825
 int chunked_from(const cc1d_delta_params &p) {
@@ -53,9 +53,29 @@ bool near(int dtype, int64_t stride) { return stride >= 0 && stride * elem_bytes
 bool reachable(const cc1d_delta_params &p) {
     return near(p.x_dtype, p.v_stride_l) && near(p.x_dtype, p.out_stride_l);
 }
-bool chunked(const cc1d_delta_params &p) {
-    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return false;
-    return p.saved != nullptr || (reachable(p) && p.seqlen >= (int64_t)chunked_from(p) * (p.cu_seqlens == nullptr ? 1 : p.sequences));
+// Grids of one workgroup a (slot, value head) and of one a (sequence or what names one, value head, 16 columns).
+bool grids_fit(const cc1d_delta_params &p, int64_t slots, int64_t walks) {
+    const int64_t limit = thread_limit() / 512;
+    return slots * p.v_heads < limit && (walks * p.v_heads + 8) * ((p.dim_v + 15) / 16) < limit;
+}
+// The average says nothing of the longest.  Packed sequences that go by tokens on average go by chunks one by one, from chunked_from() tokens
+// and from 64 on: the kernels see their lengths, the host does not.  One of 4096 tokens among 128 of one token, 32 heads: 6150 us by tokens
+// alone, 245 so; four of 1000 among 128 of eight: 1556 and 302.  Where all are short the chunks' workgroups find nothing to do: 128 of 16 tokens 226 us
+// and 247, 2048 of 4 tokens 1520 and 1611.  Not where the tokens are so few that one sequence of them all could not cost
+// much more than that (255: 330 us).
+int chunked_alone(const cc1d_delta_params &p) {
+    const int from = chunked_from(p);
+    return from > kChunk ? from : kChunk;
+}
+// How a call goes: by tokens, by chunks, or each packed sequence by its own length.
+enum class Way { tokens, chunks, both };
+Way way_of(const cc1d_delta_params &p) {
+    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return Way::tokens;
+    if (p.saved != nullptr) return Way::chunks;
+    if (!reachable(p)) return Way::tokens;
+    if (p.seqlen >= (int64_t)chunked_from(p) * (p.cu_seqlens == nullptr ? 1 : p.sequences)) return Way::chunks;
+    const int64_t chunks = ((int64_t)p.seqlen + kChunk - 1) / kChunk;
+    return p.cu_seqlens != nullptr && p.seqlen >= 4 * chunked_alone(p) && grids_fit(p, 2 * chunks, chunks) ? Way::both : Way::tokens;
 }
 
 struct Places {
@@ -68,10 +88,11 @@ struct Places {
     }
 };
 // Places in the workspace and in `saved`; returns the workspace's size.
-size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWork &w, size_t *saved_bytes = nullptr) {
+size_t lay_out(const cc1d_delta_params &p, bool backward, int shortest, uint8_t *base, ChunkWork &w, size_t *saved_bytes = nullptr) {
     w = ChunkWork();
     w.chunks = (int32_t)(((int64_t)p.seqlen + kChunk - 1) / kChunk);
-    const int64_t slots = p.cu_seqlens == nullptr ? (int64_t)p.batch * w.chunks : (int64_t)p.seqlen / kChunk + p.sequences + 1;
+    w.shortest = shortest;
+    const int64_t slots = p.cu_seqlens == nullptr ? (int64_t)p.batch * w.chunks : w.shortest > 0 ? 2 * (int64_t)w.chunks : (int64_t)p.seqlen / kChunk + p.sequences + 1;
     w.slots = (int32_t)(slots < INT32_MAX ? slots : INT32_MAX);
     w.ks = key_steps(p.dim_k);
     w.terms = p.x_dtype == CC1D_BF16 ? 1 : p.x_dtype == CC1D_F16 ? 2 : 3;
@@ -102,11 +123,6 @@ size_t lay_out(const cc1d_delta_params &p, bool backward, uint8_t *base, ChunkWo
     }
     return work.used;
 }
-// Grids of one workgroup a (slot, value head) and of one a (sequence, value head, 16 columns).
-bool fits(const cc1d_delta_params &p, const ChunkWork &w) {
-    const int64_t limit = thread_limit() / 512;
-    return (int64_t)w.slots * p.v_heads < limit && ((int64_t)p.sequences * p.v_heads + 8) * ((p.dim_v + 15) / 16) < limit;
-}
 }  // namespace
 
 extern "C" {
@@ -123,10 +139,11 @@ int cc1d_delta_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
     *bytes = 0;
     const int st = cc1d_validate_delta(p);
-    if (st != CC1D_OK || !chunked(*p)) return st;
+    const Way way = st == CC1D_OK ? way_of(*p) : Way::tokens;
+    if (way == Way::tokens) return st;
     ChunkWork w;
-    *bytes = lay_out(*p, false, nullptr, w);
-    return fits(*p, w) && reachable(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    *bytes = lay_out(*p, false, way == Way::both ? chunked_alone(*p) : 0, nullptr, w);
+    return grids_fit(*p, w.slots, w.walks(*p)) && reachable(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_delta_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
@@ -136,7 +153,7 @@ int cc1d_delta_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
     const int st = check_delta(*p);
     if (st != CC1D_OK) return st;
     ChunkWork w;
-    lay_out(*p, false, nullptr, w, bytes);               // (of packed sequences without tokens too: what a traced call reckons with)
+    lay_out(*p, false, 0, nullptr, w, bytes);               // (of packed sequences without tokens too: what a traced call reckons with)
     return CC1D_OK;
 }
 
@@ -147,11 +164,13 @@ int cc1d_delta_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace
     if (need > 0 && (workspace == nullptr || !aligned256(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
     if (p->batch == 0 || p->v_heads == 0 || p->sequences == 0) return CC1D_OK;
     const hipStream_t hs = static_cast<hipStream_t>(stream);
-    if (!chunked(*p)) return launch_delta_tokens(*p, nullptr, p->sequences, hs);
+    const Way way = way_of(*p);
+    if (way == Way::tokens) return launch_delta_tokens(*p, nullptr, p->sequences, 0, hs);
     ChunkWork w;
-    lay_out(*p, false, static_cast<uint8_t *>(workspace), w);
-    const int done = launch_delta_prep(*p, w, hs);
-    return done != CC1D_OK ? done : launch_delta_scan(*p, w, p->saved != nullptr, hs);
+    lay_out(*p, false, way == Way::both ? chunked_alone(*p) : 0, static_cast<uint8_t *>(workspace), w);
+    int done = launch_delta_prep(*p, w, hs);
+    if (done == CC1D_OK) done = launch_delta_scan(*p, w, p->saved != nullptr, hs);
+    return done != CC1D_OK || way == Way::chunks ? done : launch_delta_tokens(*p, nullptr, p->sequences, w.shortest, hs);
 }
 
 int cc1d_validate_delta_bwd(const cc1d_delta_bwd_params *p) {
@@ -174,9 +193,9 @@ int cc1d_delta_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *bytes
     const int st = cc1d_validate_delta_bwd(p);
     if (st != CC1D_OK || p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return st;
     ChunkWork w;
-    *bytes = lay_out(p->fwd, true, nullptr, w);
+    *bytes = lay_out(p->fwd, true, 0, nullptr, w);
     const bool far = !near(p->fwd.x_dtype, p->dout_stride_l) || !near(p->fwd.x_dtype, p->dv_stride_l);
-    return fits(p->fwd, w) && !far ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    return grids_fit(p->fwd, w.slots, w.walks(p->fwd)) && !far ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_delta_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
@@ -188,7 +207,7 @@ int cc1d_delta_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t works
     if (p->fwd.v_heads == 0) return launch_delta_no_values(*p, hs);
     if (p->fwd.batch == 0 || p->fwd.sequences == 0) return CC1D_OK;
     ChunkWork w;
-    lay_out(p->fwd, true, static_cast<uint8_t *>(workspace), w);
+    lay_out(p->fwd, true, 0, static_cast<uint8_t *>(workspace), w);
     if (w.slots > 0) st = launch_delta_prep(p->fwd, w, hs);
     if (st != CC1D_OK) return st;
     return launch_delta_bwd(*p, w, hs);
@@ -223,7 +242,7 @@ int cc1d_delta_step(const cc1d_delta_step_params *s, cc1d_stream_t stream) {
     p.initial_states = s->state; p.init_stride_n = s->state_stride_n; p.init_stride_h = s->state_stride_h; p.init_stride_k = s->state_stride_k;
     p.final_states = s->state; p.final_stride_n = s->state_stride_n; p.final_stride_h = s->state_stride_h; p.final_stride_k = s->state_stride_k;
     p.out = s->out; p.out_stride_b = s->out_stride_b; p.out_stride_l = s->out_stride_l; p.out_stride_h = s->out_stride_h;
-    return launch_delta_tokens(p, s->state_indices, s->state_slots, static_cast<hipStream_t>(stream));
+    return launch_delta_tokens(p, s->state_indices, s->state_slots, 0, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -50,7 +50,9 @@ __device__ __host__ __forceinline__ constexpr int lower_frag(int t, int s) { ret
 __device__ __host__ __forceinline__ constexpr int upper_frag(int t, int s) { return t < 2 ? 2 * t + s : 4 + (t - 2); }
 
 // Where everything lies in the workspace.  "slot": one chunk of one sequence; without cu_seqlens n ceil(seqlen / 64) + c, with
-// it floor(first token / 64) + n + c, which no two chunks share.
+// it floor(first token / 64) + n + c, which no two chunks share.  Where only sequences of `shortest` tokens go by chunks, 64 at least, each holds
+// a token whose number is a multiple of 64, and is named by the first of them, 64 f: slots 2 f + c, at most twice as many as it holds such
+// tokens; workgroups are counted by tokens then, however many sequences there are.
 struct ChunkWork {
     uint8_t *kf, *qf, *ktf, *qtf;        // per (slot, head): K, Q rows x dim_k; K^T, Q^T dim_k x rows
     uint8_t *tf, *pf, *ttf, *ptf;        // per (slot, value head): T, P lower; T^T, P^T upper
@@ -58,14 +60,40 @@ struct ChunkWork {
     float *s0, *ds1;                     // per (slot, value head): (dim_k, dim_v)
     float *u, *dx;                       // per (slot, value head): (64, dim_v)
     float *dqk;                          // per (slot, value head) of shared keys: its share of dq and dk, 64 x 32 ks each, in the lanes' order
-    int32_t slots, chunks;               // chunks: of one sequence without cu_seqlens
+    int32_t slots, chunks;               // chunks: of one sequence without cu_seqlens; of all tokens
     int32_t ks, terms, pterms;           // 32-column steps of dim_k; terms of K and Q; of P
     int32_t backward;
+    int32_t shortest;                    // packed sequences of fewer tokens are the token kernel's; 0: none
     FastDiv by_heads, by_v_heads, by_group, by_chunks;    // group: value heads of a key head
+    // What the scan has workgroups for: the sequences, or the tokens that may name one.
+    int64_t walks(const cc1d_delta_params &p) const { return shortest > 0 ? chunks : p.sequences; }
     __device__ __host__ int64_t kbytes() const { return (int64_t)4 * ks * terms * kFrag; }
     __device__ __host__ int64_t tbytes() const { return (int64_t)kTriFrags * 3 * kFrag; }
     __device__ __host__ int64_t pbytes() const { return (int64_t)kTriFrags * pterms * kFrag; }
 };
+
+// The last sequence whose place is not behind `target`; sequence 0's is not.  64 candidates at once, one a lane (the whole wavefront is here):
+// one load's wait up to 64 sequences, two up to 4096.
+template <typename F>
+__device__ __forceinline__ int last_sequence(const cc1d_delta_params &p, int64_t target, F &&place) {
+    int a = 0, b = p.sequences;
+    while (b - a > 1) {
+        const int step = (b - a + 63) >> 6, mine = a + (int)(threadIdx.x & 63) * step, i = mine < b ? mine : b - 1;
+        const int64_t at = place(cu_entry(p.cu_seqlens, p.cu_seqlens_is_int64, i, p.seqlen), i);
+        const int n = __popcll(__ballot(mine < b && (mine == a || at <= target)));
+        a += (n - 1) * step;
+        b = a + step < b ? a + step : b;
+    }
+    return a;
+}
+// The sequence that holds token `at`, if one does.
+__device__ __forceinline__ int sequence_of(const cc1d_delta_params &p, int64_t at) {
+    return last_sequence(p, at, [](int64_t first, int) { return first; });
+}
+// Whether a sequence goes by chunks and is named by token 64 f.
+__device__ __forceinline__ bool named(const TokenRange &r, const ChunkWork &w, int64_t f) {
+    return r.hi - r.lo >= w.shortest && (r.lo + kChunk - 1) / kChunk == f;
+}
 
 // Which chunk a slot is: tokens [lo, lo + count) of batch entry b, sequence n, or count = 0 if it is none.
 struct ChunkAt { int64_t lo; int count, b, n; };
@@ -75,23 +103,23 @@ __device__ __forceinline__ ChunkAt chunk_at(const cc1d_delta_params &p, const Ch
         const int64_t lo = (int64_t)c * kChunk, left = p.seqlen - lo;
         return {lo, (int)(left < kChunk ? left : kChunk), n, n};
     }
-    // The last sequence whose first slot is not behind this one; sequence 0 begins at slot floor(cu[0] / 64).  64 candidates at
-    // once, one a lane (the whole wavefront is here): one load's wait up to 64 sequences, two up to 4096.
-    int a = 0, b = p.sequences;
-    while (b - a > 1) {
-        const int step = (b - a + 63) >> 6, mine = a + (int)(threadIdx.x & 63) * step, i = mine < b ? mine : b - 1;
-        const int64_t first = cu_entry(p.cu_seqlens, p.cu_seqlens_is_int64, i, p.seqlen) / kChunk + i;
-        const int n = __popcll(__ballot(mine < b && (mine == a || first <= slot)));
-        a += (n - 1) * step;
-        b = a + step < b ? a + step : b;
+    if (w.shortest > 0) {
+        const int n = sequence_of(p, (int64_t)(slot >> 1) * kChunk);
+        const TokenRange r = sequence_tokens(p, n);
+        const int64_t f = (r.lo + kChunk - 1) / kChunk, lo = r.lo + (slot - 2 * f) * kChunk, left = r.hi - lo;
+        if (!named(r, w, f) || lo < r.lo || left <= 0) return {0, 0, 0, n};
+        return {lo, (int)(left < kChunk ? left : kChunk), 0, n};
     }
+    // The last sequence whose first slot is not behind this one; sequence 0 begins at slot floor(cu[0] / 64).
+    const int a = last_sequence(p, slot, [](int64_t first, int i) { return first / kChunk + i; });
     const TokenRange r = sequence_tokens(p, a);
     const int64_t lo = r.lo + ((int64_t)slot - (r.lo / kChunk + a)) * kChunk, left = r.hi - lo;
     if (lo < r.lo || left <= 0) return {0, 0, 0, a};
     return {lo, (int)(left < kChunk ? left : kChunk), 0, a};
 }
 __device__ __forceinline__ int first_slot(const cc1d_delta_params &p, const ChunkWork &w, int n, const TokenRange &r) {
-    return p.cu_seqlens == nullptr ? n * w.chunks : (int)(r.lo / kChunk) + n;
+    if (p.cu_seqlens == nullptr) return n * w.chunks;
+    return w.shortest > 0 ? 2 * (int)((r.lo + kChunk - 1) / kChunk) : (int)(r.lo / kChunk) + n;
 }
 
 // N bfloat16 terms of 4 (8) numbers, term i in two (four) words, each the rest rounded to nearest: two leave 2^-18 of a

@@ -48,8 +48,13 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
     const uint32_t xcd = blockIdx.x & 7u, idx = blockIdx.x >> 3;
     const uint32_t nh = idx / col_tiles * 8u + xcd;
     if (nh >= heads_total) return;
-    const int n = (int)divided(nh, w.by_v_heads), h = (int)nh - n * p.v_heads, hk = (int)divided((uint32_t)h, w.by_group);
+    int n = (int)divided(nh, w.by_v_heads);
+    const int h = (int)nh - n * p.v_heads, hk = (int)divided((uint32_t)h, w.by_group);
+    const bool mixed = w.shortest > 0;                   // n is f of a sequence, if there is one
+    const int f = n;
+    if (mixed) n = sequence_of(p, (int64_t)f * kChunk);
     const TokenRange range = sequence_tokens(p, n);
+    if (mixed && !named(range, w, f)) return;
     const int chunks = (int)((range.hi - range.lo + kChunk - 1) / kChunk);
     const int slot0 = first_slot(p, w, n, range), total = (int)(range.hi - range.lo);
     const int col0 = (int)(idx % col_tiles) * 16 + m;
@@ -60,7 +65,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
     const uint32_t at_col = (uint32_t)col * (uint32_t)sizeof(T);
 
     T *out = static_cast<T *>(p.out) + range.b * p.out_stride_b + h * p.out_stride_h;
-    if (p.cu_seqlens != nullptr && has_col) {            // tokens in front of the first sequence and behind the last
+    if (p.cu_seqlens != nullptr && !mixed && has_col) {  // tokens in front of the first sequence and behind the last
         if (n == 0)
             for (int64_t t = wave * 4 + g; t < range.lo; t += 16) out[t * p.out_stride_l + col] = Elem<DT>::from_float(0.f);
         if (n == p.sequences - 1)
@@ -288,7 +293,7 @@ delta_scan_kernel(const cc1d_delta_params p, const ChunkWork w, const uint32_t h
 
 template <int DT, int KS, bool SAVE>
 int launch(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream) {
-    const uint32_t tiles = (uint32_t)(p.dim_v + 15) / 16, nh = (uint32_t)((int64_t)p.sequences * p.v_heads);
+    const uint32_t tiles = (uint32_t)(p.dim_v + 15) / 16, nh = (uint32_t)(w.walks(p) * p.v_heads);
     CC1D_LAUNCH((delta_scan_kernel<DT, KS, SAVE>), dim3((nh + 7) / 8 * 8 * tiles), dim3(kBlock), 0, stream, p, w, nh, tiles);
     return launch_status();
 }

@@ -23,6 +23,7 @@ struct StepArgs {
     cc1d_delta_params p;                 // initial_states / final_states: the state, or the caller's two
     const int32_t *indices;
     int32_t slots;
+    int32_t longest;                     // sequences of this many tokens go by chunks; 0: none
     uint32_t items, col_tiles;
     uint32_t vec_state, vec_x;           // 16-byte rows of the state / 4 elements of v and out at once
 };
@@ -57,6 +58,8 @@ delta_step_kernel(const StepArgs a) {
         if (n == 0) clear(0, range.lo);
         if (n == p.sequences - 1) clear(range.hi, p.seqlen);
     }
+
+    if (a.longest > 0 && range.hi - range.lo >= a.longest) return;
 
     int64_t slot = n;
     if (a.indices != nullptr) slot = a.indices[n];
@@ -221,11 +224,12 @@ int launch_dtype(const StepArgs &a, hipStream_t stream) {
 }  // namespace
 
 
-int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, hipStream_t stream) {
+int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, int longest, hipStream_t stream) {
     StepArgs a = {};
     a.p = p;
     a.indices = indices;
     a.slots = slots;
+    a.longest = longest;
     a.col_tiles = (uint32_t)((p.dim_v + kStepCols - 1) / kStepCols);
     const int64_t items = (int64_t)p.sequences * p.v_heads * a.col_tiles;
     if (items == 0) return CC1D_OK;

@@ -33,8 +33,8 @@ extern "C" {
  * Without cu_seqlens there are `batch` sequences of `seqlen` tokens.  With it (batch == 1) sequence n
  * is tokens cu_seqlens[n] .. cu_seqlens[n+1]-1, `sequences` of them (one at least where there are
  * tokens), ascending; empty ones are allowed, entries outside [0, seqlen] are clamped, and tokens of no sequence give zeros.
- * Chunks of 64 tokens are worked out together: a NaN or infinity reaches its head's outputs from the
- * start of its chunk on.
+ * Short sequences go token by token, packed ones each by its own length; the others in chunks of 64 tokens, which are
+ * worked out together: a NaN or infinity reaches its head's outputs from the start of its chunk on.
  * ---------------------------------------------------------------------------------- */
 typedef struct cc1d_delta_params {
     int32_t batch, seqlen, heads, v_heads, dim_k, dim_v;

@@ -62,3 +62,18 @@ def test_saved_bytes_of_a_traced_call(lib, pkg, batch, seqlen, sequences, v_head
     meta = [None if t is None else t.to("meta") for t in (q, q, v, g, g, None, cu)]
     out, saved = torch.ops.DaoAILab._gated_delta_rule_fwd_save_cpp(*meta, None, 1.0, False)
     assert out.shape == v.shape and tuple(saved.shape) == (n.value,)
+
+
+def test_packed_sequences_are_not_all_judged_by_their_average(lib):
+    """One long sequence among many short ones goes by chunks, for which there has to be a workspace; the token kernel alone takes
+    none, and as long as the longest.  A few tokens, or a uniform batch of short sequences without a long one's worth of tokens, go by tokens."""
+    n = C.c_size_t()
+    for seqlen, sequences, v_heads, wanted in ((4224, 129, 32, True), (600, 300, 4, True), (255, 64, 32, False), (64, 16, 32, False)):
+        q, v, g = torch.empty(1, seqlen, 1, 16), torch.empty(1, seqlen, v_heads, 16), torch.empty(1, seqlen, v_heads)
+        p = mixer.delta_params(q.bfloat16(), q.bfloat16(), v.bfloat16(), g, g, v.bfloat16())
+        p.x_dtype = 2
+        cu = torch.zeros(sequences + 1, dtype=torch.int32)
+        p.cu_seqlens, p.sequences = cu.data_ptr(), sequences
+        p.heads = 1
+        assert lib.cc1d_delta_workspace_bytes(p, C.byref(n)) == OK
+        assert (n.value > 0) == wanted, (seqlen, sequences)
