@@ -48,11 +48,11 @@ int chunked_from(const cc1d_delta_params &p) {
     if (heads <= 1024) return p.x_dtype == CC1D_F32 ? 40 : 20;
     return p.x_dtype == CC1D_F32 ? 160 : 40;
 }
-// The scans reach the 64 rows of a chunk with 32 bits.
-bool near(int dtype, int64_t stride) { return stride >= 0 && stride * elem_bytes(dtype) < ((int64_t)1 << 31) / kChunk; }
-bool reachable(const cc1d_delta_params &p) {
-    return near(p.x_dtype, p.v_stride_l) && near(p.x_dtype, p.out_stride_l);
+// The scans reach the 64 rows of a chunk with 32 bits; a single token's stride is nowhere taken.
+bool near(const cc1d_delta_params &p, int64_t stride) {
+    return p.seqlen <= 1 || (stride >= 0 && stride * elem_bytes(p.x_dtype) < ((int64_t)1 << 31) / kChunk);
 }
+bool reachable(const cc1d_delta_params &p) { return near(p, p.v_stride_l) && near(p, p.out_stride_l); }
 // Grids of one workgroup a (slot, value head) and of one a (sequence or what names one, value head, 16 columns).
 bool grids_fit(const cc1d_delta_params &p, int64_t slots, int64_t walks) {
     const int64_t limit = thread_limit() / 512;
@@ -194,7 +194,7 @@ int cc1d_delta_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *bytes
     if (st != CC1D_OK || p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return st;
     ChunkWork w;
     *bytes = lay_out(p->fwd, true, 0, nullptr, w);
-    const bool far = !near(p->fwd.x_dtype, p->dout_stride_l) || !near(p->fwd.x_dtype, p->dv_stride_l);
+    const bool far = !near(p->fwd, p->dout_stride_l) || !near(p->fwd, p->dv_stride_l);
     return grids_fit(p->fwd, w.slots, w.walks(p->fwd)) && !far ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 

@@ -3,6 +3,8 @@ test_gated_delta_rule_bwd_gpu.py."""
 import pytest
 import torch
 
+from test_gated_delta_rule_gpu import make
+
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -19,3 +21,18 @@ def test_no_value_heads(pkg, gpu_device, dtype, dim_k):
     del used
     dq, dk, dv = torch.autograd.grad([out, final], [q, k, v], [torch.ones_like(out), torch.ones_like(final)])
     assert dv.shape == v.shape and torch.equal(dq, torch.zeros_like(q)) and torch.equal(dk, torch.zeros_like(k))
+
+
+@pytest.mark.gpu
+def test_one_token_of_any_stride(pkg, gpu_device):
+    """A training step over one token whose stride along the tokens is far beyond what a chunk's rows may have: the same bits."""
+    q, k, v, g, beta, _ = make(3, 1, 1, 2, 32, 16, torch.bfloat16, gpu_device, l2norm=True)
+    far = v.contiguous().as_strided(v.shape, (v[0].numel(), 1 << 30, 16, 1))
+    dout = torch.randn(v.shape, device=gpu_device).bfloat16()
+    results = []
+    for x, d in ((v.contiguous(), dout), (far, dout.as_strided(dout.shape, far.stride()))):
+        leaves = [t.detach().requires_grad_() for t in (q, k, x, g, beta)]
+        out = pkg.gated_delta_rule_fn(*leaves, qk_l2norm=True)
+        results.append([out, *torch.autograd.grad(out, leaves, d)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)

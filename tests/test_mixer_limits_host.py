@@ -77,3 +77,21 @@ def test_packed_sequences_are_not_all_judged_by_their_average(lib):
         p.heads = 1
         assert lib.cc1d_delta_workspace_bytes(p, C.byref(n)) == OK
         assert (n.value > 0) == wanted, (seqlen, sequences)
+
+
+def test_one_token_has_no_distance_to_the_next(lib):
+    """The stride between tokens is anything where there is one token a sequence: no reason to refuse a training call."""
+    n = C.c_size_t()
+    for seqlen, want in ((1, OK), (2, E_TOO_LARGE)):
+        q, v, g = torch.empty(2, seqlen, 1, 16), torch.empty(2, seqlen, 2, 16), torch.empty(2, seqlen, 2)
+        p = mixer.delta_params(q, q, v, g, g, v)
+        p.saved = 256
+        p.v_stride_l = p.out_stride_l = 1 << 23          # 2^25 bytes
+        assert lib.cc1d_delta_workspace_bytes(p, C.byref(n)) == want
+        b = mixer.DeltaBwdParams()
+        b.fwd = p
+        for name, t in (("dout", v), ("dq", q), ("dk", q), ("dv", v)):
+            mixer.put(b, name, t, "b", "l", "h")
+        b.dg = b.dbeta = g.data_ptr()
+        b.dout_stride_l = b.dv_stride_l = 1 << 23
+        assert lib.cc1d_delta_bwd_workspace_bytes(b, C.byref(n)) == want
