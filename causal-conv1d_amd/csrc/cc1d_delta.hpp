@@ -11,8 +11,9 @@ namespace cc1d {
 constexpr int kChunk = 64;               // tokens of a chunk
 constexpr float kNormEps = 1e-6f;        // under the root of qk_l2norm
 
-// exp(x) as 2^(x log2 e), the product in two floats: off by 2 units in the last place at most, 6 instructions where
-// expf takes 25.  -inf and everything below -104 give 0.
+// exp(x) as 2^(x log2 e), the product in two floats: 6 instructions where expf takes 25.  Off by 2 units in the last place at most where the
+// result is a normal number of 32 bits; 0 below that, from -87.4 on (the instruction gives no others), -inf included; an infinity or a NaN
+// where it is too large, from 88.8 on, after which the recurrence has no finite value either (D^T k meets an infinity in every column).
 __device__ __forceinline__ float exp_of(float x) {
     const float hi = x * 1.44269502f, lo = fmaf(x, 1.44269502f, -hi) + x * 1.92596299e-8f;
     const float e = __builtin_amdgcn_exp2f(hi);

@@ -36,3 +36,23 @@ def test_one_token_of_any_stride(pkg, gpu_device):
         results.append([out, *torch.autograd.grad(out, leaves, d)])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqlen", [1, 70])
+def test_gates_at_the_ends_of_the_exponential(pkg, gpu_device, seqlen):
+    """exp(g) by itself: a state of ones, read by a query of one row, nothing learned.  Two units in the last place where it is a normal number of 32
+    bits, 2^-126 at most below that; above the largest number nothing finite comes out."""
+    for g0 in (0.0, -1e-3, 3.7, -20.3, -87.0, 88.0, 88.7, -88.0, -95.0, -103.5, -104.5, -1e30, float("-inf")):
+        q, k = torch.zeros(1, seqlen, 1, 8, device=gpu_device), torch.zeros(1, seqlen, 1, 8, device=gpu_device)
+        q[..., 0] = 1
+        v, beta, g = torch.zeros(1, seqlen, 1, 8, device=gpu_device), torch.zeros(1, seqlen, 1, device=gpu_device), torch.zeros(1, seqlen, 1, device=gpu_device)
+        g[:, 0] = g0
+        out, final = pkg.gated_delta_rule_fn(q, k, v, g, beta, scale=1.0, initial_states=torch.ones(1, 1, 8, 8, device=gpu_device), return_final_states=True)
+        want = g[0, 0, 0].double().exp()
+        # (by chunks the state is read as the sum of three numbers of 16 bits, exact for a power of two)
+        assert ((out.double() - want).abs() <= 2 * 2.0 ** -23 * want + 2.0 ** -126).all() and ((final.double() - want).abs() <= 2 * 2.0 ** -23 * want + 2.0 ** -126).all(), g0
+    for g0 in (89.0, 100.0, float("inf"), float("nan")):
+        g[:, 0] = g0
+        out, final = pkg.gated_delta_rule_fn(q, k, v, g, beta, scale=1.0, initial_states=torch.ones(1, 1, 8, 8, device=gpu_device), return_final_states=True)
+        assert not torch.isfinite(out).any() and not torch.isfinite(final).any(), g0
