@@ -3,7 +3,8 @@ test_gated_delta_rule_bwd_gpu.py."""
 import pytest
 import torch
 
-from test_gated_delta_rule_gpu import make
+from test_gated_delta_rule_bwd_gpu import check as check_gradients
+from test_gated_delta_rule_gpu import close, make, recurrence
 
 
 @pytest.mark.gpu
@@ -56,3 +57,27 @@ def test_gates_at_the_ends_of_the_exponential(pkg, gpu_device, seqlen):
         g[:, 0] = g0
         out, final = pkg.gated_delta_rule_fn(q, k, v, g, beta, scale=1.0, initial_states=torch.ones(1, 1, 8, 8, device=gpu_device), return_final_states=True)
         assert not torch.isfinite(out).any() and not torch.isfinite(final).any(), g0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,group,dim_k,dim_v", [
+    (torch.float32, 2, 128, 32), (torch.float32, 2, 250, 24), (torch.bfloat16, 2, 256, 40), (torch.float16, 3, 224, 16),       # dq and dk leave one after the other
+    (torch.float32, 2, 96, 64), (torch.bfloat16, 2, 192, 64),                                                               # at once, their largest
+    (torch.bfloat16, 1, 192, 128), (torch.float16, 1, 160, 64), (torch.float32, 1, 176, 32), (torch.bfloat16, 2, 136, 72)])    # six steps of dim_k, whole vectors
+@pytest.mark.parametrize("l2norm", [False, True])
+def test_gradients_of_wide_heads(pkg, gpu_device, dtype, group, dim_k, dim_v, l2norm):
+    check_gradients(pkg, gpu_device, 1, 100, 2, group, dim_k, dim_v, dtype, l2norm, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sequences", [65, 130])
+def test_many_packed_sequences_by_chunks(pkg, gpu_device, sequences):
+    """More than 64: a chunk's sequence is found in two steps."""
+    lengths = [(37 * i) % 90 + 20 for i in range(sequences)]
+    q, k, v, g, beta, s0 = make(1, sum(lengths), 1, 1, 32, 16, torch.bfloat16, gpu_device, sequences=sequences, l2norm=True)
+    cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32).to(gpu_device)
+    out, final = pkg.gated_delta_rule_fn(q, k, v, g, beta, initial_states=s0, return_final_states=True, cu_seqlens=cu, qk_l2norm=True)
+    for i, (lo, hi) in enumerate(zip(cu.tolist()[:-1], cu.tolist()[1:])):
+        want, want_final = recurrence(*(t[:, lo:hi] for t in (q, k, v, g, beta)), s0[i:i + 1], True)
+        close(out[:, lo:hi], want, torch.bfloat16, 32, "out of sequence %d" % i)
+        close(final[i:i + 1], want_final, torch.float32, 32, "final of sequence %d" % i)
