@@ -12,7 +12,8 @@
 //
 // Products.  The matrix cores take 16-bit operands; a number x of 24 bits is the exact sum of three bfloat16
 // (each the rest, rounded), so a product of two such is nine exact products, of which the six largest carry it to
-// 2^-25.  bfloat16 q, k, v, dout are one term each and cost nothing, float16 is two.
+// 2^-25, for numbers from 2^-90 on (the terms of smaller ones fall below the normal numbers; 2^-100 is off by 1e-8 still).  bfloat16 q, k, v, dout are one
+// term each and cost nothing, float16 is two.
 // Six products on the 16-bit cores take 0.38 of the time of the fp32 ones; one and three together a third of that.
 //
 // Operand order.  An MFMA of 16 x 16 x 32 wants of its left operand 8 consecutive columns of one row a lane, of its right one 8

@@ -14,8 +14,8 @@
 // dw: a workgroup takes a run of rows, its lanes keep the sums of their columns in registers; one plane of partial sums a
 // workgroup, added up in the order of the planes by a second launch.  No atomics: the same bits every time.
 //
-// 16384 rows of 2560, residual in fp32: forward 93 to 99 us (5.1 to 5.4 TB/s), backward 122 (5.5) and 4.5 for dw's planes.  To 8 bits, 8192 rows of
-// 5120: 49 us (6.0 TB/s), and 20 back.  64 such rows: 4.7 us and 2.7, a launch, two reductions and a barrier each.
+// 16384 rows of 2560, residual in fp32: forward 99 to 106 us (4.7 to 5.1 TB/s), backward 122 (5.5) and 4.7 for dw's planes.  To 8 bits, 8192 rows of
+// 5120: 48 us (6.1 TB/s), and 20 back.  64 such rows: 4.7 us and 2.6, a launch, two reductions and a barrier each.
 #include "cc1d_device.hpp"
 #include "cc1d_internal.hpp"
 #include "cc1d_mixer.h"

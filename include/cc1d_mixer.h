@@ -27,8 +27,9 @@ extern "C" {
  *
  * Value head h reads q and k of head h / (v_heads / heads).  With qk_l2norm, q and k stand for
  * q rsqrt(sum q^2 + 1e-6) and k rsqrt(sum k^2 + 1e-6), each token and head for itself.
- * All products and sums are carried to fp32's precision whatever x_dtype is; out and the gradients
- * of q, k, v are rounded once as they are stored.
+ * States, gradients and fp32 outputs are carried to fp32's precision whatever x_dtype is (products to 2^-25 of their factors'
+ * values, sums in fp32; values below 2^-90 lose bits), and the gradients of q, k, v are rounded once as they are stored.  out of
+ * 16 bits is rounded once too, in chunks from products whose factors (the state, and what a chunk's tokens add to it) carry 2^-17.
  *
  * Without cu_seqlens there are `batch` sequences of `seqlen` tokens.  With it (batch == 1) sequence n
  * is tokens cu_seqlens[n] .. cu_seqlens[n+1]-1, `sequences` of them (one at least where there are

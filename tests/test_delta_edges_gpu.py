@@ -81,3 +81,24 @@ def test_many_packed_sequences_by_chunks(pkg, gpu_device, sequences):
         want, want_final = recurrence(*(t[:, lo:hi] for t in (q, k, v, g, beta)), s0[i:i + 1], True)
         close(out[:, lo:hi], want, torch.bfloat16, 32, "out of sequence %d" % i)
         close(final[i:i + 1], want_final, torch.float32, 32, "final of sequence %d" % i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("seqlen", [5, 130])
+def test_range_of_values(pkg, gpu_device, dtype, seqlen):
+    """v and the states times a power of two: outputs, states and the gradients of q exactly as many times as large, or, where the third terms
+    of numbers fall below the smallest normal one (2^-126 against 2^-100, at most half of it each), off by 2^-24 and a few sums of that."""
+    q, k, v, g, beta, s0 = make(1, seqlen, 2, 1, 64, 64, dtype, gpu_device, l2norm=True)
+
+    def run(power):
+        leaves = [q.detach().requires_grad_(), (v.float() * 2.0 ** power).to(dtype).requires_grad_()]
+        out, final = pkg.gated_delta_rule_fn(leaves[0], k, leaves[1], g, beta, initial_states=s0 * 2.0 ** power, return_final_states=True, qk_l2norm=True)
+        dq, _ = torch.autograd.grad([out, final], leaves, [torch.ones_like(out), torch.ones_like(final)])
+        return [t.detach().double() * 2.0 ** -power for t in (out, final, dq)]
+    base = run(0)
+    for power in (-80, 60, 110):
+        assert all(torch.equal(a, b) for a, b in zip(run(power), base)), power
+    # (a value of 16 bits may also come out one rounding beside the other)
+    for a, b, t in zip(run(-100), base, (dtype, torch.float32, dtype)):
+        assert (a - b).norm() <= (64 ** 0.5 * 2.0 ** -24 + (0 if t == torch.float32 else 2.0 ** -8)) * b.norm()
