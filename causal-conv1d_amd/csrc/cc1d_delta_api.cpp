@@ -75,7 +75,7 @@ Way way_of(const cc1d_delta_params &p) {
     if (!reachable(p)) return Way::tokens;
     if (p.seqlen >= (int64_t)chunked_from(p) * (p.cu_seqlens == nullptr ? 1 : p.sequences)) return Way::chunks;
     const int64_t chunks = ((int64_t)p.seqlen + kChunk - 1) / kChunk;
-    return p.cu_seqlens != nullptr && p.seqlen >= 4 * chunked_alone(p) && grids_fit(p, 2 * chunks, chunks) ? Way::both : Way::tokens;
+    return p.cu_seqlens != nullptr && p.seqlen >= 4 * kChunk && grids_fit(p, 2 * chunks, chunks) ? Way::both : Way::tokens;
 }
 
 struct Places {

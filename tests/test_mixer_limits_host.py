@@ -95,3 +95,14 @@ def test_one_token_has_no_distance_to_the_next(lib):
         b.dg = b.dbeta = g.data_ptr()
         b.dout_stride_l = b.dv_stride_l = 1 << 23
         assert lib.cc1d_delta_bwd_workspace_bytes(b, C.byref(n)) == want
+
+
+def test_long_sequences_of_float32_among_many_heads(lib):
+    """In float32 with many heads a sequence goes by chunks from 160 tokens on; a call that may hold one is looked at from 256 tokens on as well."""
+    n = C.c_size_t()
+    for seqlen, wanted in ((255, False), (256, True), (364, True)):
+        q, v, g = torch.empty(1, seqlen, 1, 16), torch.empty(1, seqlen, 32, 16), torch.empty(1, seqlen, 32)
+        p = mixer.delta_params(q, q, v, g, g, v)
+        cu = torch.zeros(66, dtype=torch.int32)
+        p.cu_seqlens, p.sequences = cu.data_ptr(), 65
+        assert lib.cc1d_delta_workspace_bytes(p, C.byref(n)) == OK and (n.value > 0) == wanted, seqlen
