@@ -41,10 +41,16 @@ KERNEL_SOURCES = [
     "cc1d_delta_prep.hip",
     "cc1d_delta_scan.hip",
     "cc1d_delta_bwd.hip",
+    "cc1d_linear_api.cpp",
+    "cc1d_linear_states.hip",
+] + ["cc1d_linear_%s_%s.hip" % (what, dtype) for what in ("out", "dq", "dk", "dv") for dtype in ("bf16", "f16", "f32")] + [
     "cc1d_norm.hip",
+    "cc1d_layer_norm.hip",
 ]
 KERNEL_HEADERS = ["cc1d_device.hpp", "cc1d_internal.hpp", "cc1d_bwd_channellast_kernel.hpp"]
-DELTA_HEADERS = ["cc1d_delta.hpp", "cc1d_delta_chunk.hpp", "cc1d_delta_host.hpp"]   # of the sources that begin with cc1d_delta
+DELTA_HEADERS = ["cc1d_delta.hpp", "cc1d_delta_chunk.hpp", "cc1d_delta_host.hpp"]   # of the sources that begin with cc1d_delta or cc1d_linear
+NORM_SOURCES, NORM_HEADERS = ("cc1d_norm.hip", "cc1d_layer_norm.hip"), ["cc1d_rows.hpp"]
+LINEAR_HEADERS = ["cc1d_linear.hpp", "cc1d_linear_device.hpp", "cc1d_linear_attend.hpp"]
 PUBLIC_HEADERS = ["cc1d.h", "cc1d_mixer.h"]
 BINDING_SOURCES = ["causal_conv1d.cpp", "mixer.cpp"]
 BINDING_HEADERS = ["cc1d_torch.hpp", "cc1d_torch_calls.hpp"]
@@ -103,6 +109,8 @@ def build_kernels(force=False, extra_flags=(), lib_path=None):
     lib_path = lib_path or os.path.join(HERE, LIB_NAME)
     headers = [os.path.join(CSRC, h) for h in KERNEL_HEADERS] + [os.path.join(INCLUDE, "cc1d.h")]
     delta = [os.path.join(CSRC, h) for h in DELTA_HEADERS]
+    norm = [os.path.join(CSRC, h) for h in NORM_HEADERS]
+    linear = [os.path.join(CSRC, h) for h in LINEAR_HEADERS]
     mixer = [os.path.join(INCLUDE, "cc1d_mixer.h")]
     tag = "" if not extra_flags else "_" + str(abs(hash(tuple(extra_flags))) % 10**8)
     jobs, objs = [], []
@@ -110,7 +118,7 @@ def build_kernels(force=False, extra_flags=(), lib_path=None):
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJDIR, os.path.splitext(src)[0] + tag + ".o")
         objs.append(o)
-        deps = [s] + headers + (delta + mixer if src.startswith("cc1d_delta") else mixer if src == "cc1d_norm.hip" else [])
+        deps = [s] + headers + (delta + mixer if src.startswith("cc1d_delta") else delta + linear + mixer if src.startswith("cc1d_linear") else norm + mixer if src in NORM_SOURCES else [])
         if force or not _newer(o, deps):
             jobs.append(compile_command(src, o, extra_flags))
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:

@@ -228,7 +228,14 @@ int cc1d_validate_delta_step(const cc1d_delta_step_params *p) {
 
 int cc1d_delta_step(const cc1d_delta_step_params *s, cc1d_stream_t stream) {
     const int st = cc1d_validate_delta_step(s);
-    if (st != CC1D_OK || s->batch == 0 || s->seqlen == 0 || s->v_heads == 0) return st;
+    return st != CC1D_OK ? st : launch_step_tokens(*s, static_cast<hipStream_t>(stream), true);
+}
+
+}  // extern "C"
+
+int cc1d::launch_step_tokens(const cc1d_delta_step_params &step, hipStream_t stream, bool rule) {
+    const cc1d_delta_step_params *s = &step;
+    if (s->batch == 0 || s->seqlen == 0 || s->v_heads == 0) return CC1D_OK;
     cc1d_delta_params p = {};
     p.batch = p.sequences = s->batch; p.seqlen = s->seqlen; p.heads = s->heads; p.v_heads = s->v_heads;
     p.dim_k = s->dim_k; p.dim_v = s->dim_v;
@@ -242,7 +249,5 @@ int cc1d_delta_step(const cc1d_delta_step_params *s, cc1d_stream_t stream) {
     p.initial_states = s->state; p.init_stride_n = s->state_stride_n; p.init_stride_h = s->state_stride_h; p.init_stride_k = s->state_stride_k;
     p.final_states = s->state; p.final_stride_n = s->state_stride_n; p.final_stride_h = s->state_stride_h; p.final_stride_k = s->state_stride_k;
     p.out = s->out; p.out_stride_b = s->out_stride_b; p.out_stride_l = s->out_stride_l; p.out_stride_h = s->out_stride_h;
-    return launch_delta_tokens(p, s->state_indices, s->state_slots, 0, static_cast<hipStream_t>(stream));
+    return launch_delta_tokens(p, s->state_indices, s->state_slots, 0, stream, rule);
 }
-
-}  // extern "C"

@@ -11,8 +11,11 @@ namespace cc1d {
 struct ChunkWork;
 
 // Token by token.  initial_states / final_states of `p` are the states read and written, `slots` of them, picked by
-// `indices` (NULL: sequence n has state n).  `longest`: sequences of that many tokens are left alone (0: none).
-int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, int longest, hipStream_t stream);
+// `indices` (NULL: sequence n has state n).  `longest`: sequences of that many tokens are left alone (0: none).  Without `rule`: linear
+// attention, whose beta may be NULL.
+int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, int longest, hipStream_t stream, bool rule = true);
+// A decode step of either, whose arguments have been checked.
+int launch_step_tokens(const cc1d_delta_step_params &step, hipStream_t stream, bool rule);
 // By chunks: what needs no state; then the states and outputs (`save`: the states in front of the chunks and U are kept).
 int launch_delta_prep(const cc1d_delta_params &p, const ChunkWork &w, hipStream_t stream);
 int launch_delta_scan(const cc1d_delta_params &p, const ChunkWork &w, bool save, hipStream_t stream);

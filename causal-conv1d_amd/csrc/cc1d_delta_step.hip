@@ -1,5 +1,5 @@
 // The gated delta rule token by token: the step of a decode loop, and whole sequences that are too short
-// to be worth cutting into chunks.
+// to be worth cutting into chunks.  And the same of linear attention, which has no D^T k.
 //
 //   D = exp(g) S,  u = beta (v - D^T k),  S = D + k u^T,  out = scale S^T q
 //
@@ -28,8 +28,8 @@ struct StepArgs {
     uint32_t vec_state, vec_x;           // 16-byte rows of the state / 4 elements of v and out at once
 };
 
-// KR: rows of the state a lane holds, dim_k <= 8 KR.
-template <int DT, int KR>
+// KR: rows of the state a lane holds, dim_k <= 8 KR.  RULE: the delta rule; else u = beta v, and beta may be missing.
+template <int DT, int KR, bool RULE>
 __global__ void __launch_bounds__(kBlock)
 delta_step_kernel(const StepArgs a) {
     using T = typename Elem<DT>::type;
@@ -91,7 +91,7 @@ delta_step_kernel(const StepArgs a) {
             x.q[e] = qp[i];
         }
         x.g = load_bits(p.g, at_g, p.g_dtype);
-        x.beta = load_bits(p.beta, at_beta, p.beta_dtype);
+        if (RULE || p.beta != nullptr) x.beta = load_bits(p.beta, at_beta, p.beta_dtype);
         if (a.vec_x) {
             *reinterpret_cast<Four *>(x.v) = *reinterpret_cast<const Four *>(vp);
         } else {                                         // (lanes behind the last column: the first)
@@ -138,7 +138,7 @@ delta_step_kernel(const StepArgs a) {
             qe[e] = there ? Elem<DT>::to_float(bitcast<T>(next.q[e])) : 0.f;
             kk += ke[e] * ke[e]; qs += qe[e] * qe[e]; dot += ke[e] * qe[e];
         }
-        const float decay = exp_of(bits_as_float(next.g, p.g_dtype)), beta = bits_as_float(next.beta, p.beta_dtype);
+        const float decay = exp_of(bits_as_float(next.g, p.g_dtype)), beta = RULE || p.beta != nullptr ? bits_as_float(next.beta, p.beta_dtype) : 1.f;
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = Elem<DT>::to_float(bitcast<T>(next.v[j]));
@@ -146,7 +146,7 @@ delta_step_kernel(const StepArgs a) {
         float rk = 1.f, rq = p.scale;
         auto lengths = [&]() {
             dot = over_wave(dot);
-            if (!p.qk_l2norm) return;
+            if (!RULE || !p.qk_l2norm) return;
             rk = rsqrtf(over_wave(kk) + kNormEps);
             rq = p.scale * rsqrtf(over_wave(qs) + kNormEps);
         };
@@ -166,7 +166,7 @@ delta_step_kernel(const StepArgs a) {
             const float ki = kq[rg * KR + i], qi = qq[rg * KR + i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                sk[j] += s[i][j] * ki;
+                if (RULE) sk[j] += s[i][j] * ki;
                 sq[j] += s[i][j] * qi;
             }
         }
@@ -174,9 +174,9 @@ delta_step_kernel(const StepArgs a) {
         float u[4], o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            sk[j] = over_rows(sk[j] + dpp_moved<0x128>(sk[j]));      // the lanes of a column are 8 apart
+            if (RULE) sk[j] = over_rows(sk[j] + dpp_moved<0x128>(sk[j]));        // the lanes of a column are 8 apart
             sq[j] = over_rows(sq[j] + dpp_moved<0x128>(sq[j]));
-            u[j] = beta * (v[j] - decay * rk * sk[j]) * rk;          // of k as it came
+            u[j] = RULE ? beta * (v[j] - decay * rk * sk[j]) * rk : beta * v[j]; // of k as it came
             o[j] = rq * (decay * sq[j] + dot * u[j]);
         }
 #pragma unroll
@@ -211,20 +211,28 @@ delta_step_kernel(const StepArgs a) {
     }
 }
 
-template <int DT, int KR>
+template <int DT, int KR, bool RULE>
 int launch_rows(const StepArgs &a, hipStream_t stream) {
-    CC1D_LAUNCH((delta_step_kernel<DT, KR>), dim3((a.items + 3) / 4), dim3(kBlock), 0, stream, a);
+    CC1D_LAUNCH((delta_step_kernel<DT, KR, RULE>), dim3((a.items + 3) / 4), dim3(kBlock), 0, stream, a);
     return launch_status();
 }
-template <int DT>
+template <int DT, bool RULE>
 int launch_dtype(const StepArgs &a, hipStream_t stream) {
-    return a.p.dim_k <= 64 ? launch_rows<DT, 8>(a, stream) : a.p.dim_k <= 128 ? launch_rows<DT, 16>(a, stream) : launch_rows<DT, 32>(a, stream);
+    return a.p.dim_k <= 64 ? launch_rows<DT, 8, RULE>(a, stream) : a.p.dim_k <= 128 ? launch_rows<DT, 16, RULE>(a, stream) : launch_rows<DT, 32, RULE>(a, stream);
+}
+template <bool RULE>
+int launch_rule(const StepArgs &a, hipStream_t stream) {
+    switch (a.p.x_dtype) {
+        case CC1D_F32: return launch_dtype<CC1D_F32, RULE>(a, stream);
+        case CC1D_F16: return launch_dtype<CC1D_F16, RULE>(a, stream);
+        default: return launch_dtype<CC1D_BF16, RULE>(a, stream);
+    }
 }
 
 }  // namespace
 
 
-int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, int longest, hipStream_t stream) {
+int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int slots, int longest, hipStream_t stream, bool rule) {
     StepArgs a = {};
     a.p = p;
     a.indices = indices;
@@ -242,11 +250,7 @@ int launch_delta_tokens(const cc1d_delta_params &p, const int32_t *indices, int 
                   whole(p.final_states, p.final_stride_n, p.final_stride_h, p.final_stride_k);
     a.vec_x = p.dim_v % 4 == 0 && p.v_stride_b % 4 == 0 && p.v_stride_l % 4 == 0 && p.v_stride_h % 4 == 0 &&
               (reinterpret_cast<uintptr_t>(p.v) & (4u * (uint32_t)elem_bytes(p.x_dtype) - 1u)) == 0;
-    switch (p.x_dtype) {
-        case CC1D_F32: return launch_dtype<CC1D_F32>(a, stream);
-        case CC1D_F16: return launch_dtype<CC1D_F16>(a, stream);
-        default: return launch_dtype<CC1D_BF16>(a, stream);
-    }
+    return rule ? launch_rule<true>(a, stream) : launch_rule<false>(a, stream);
 }
 
 }  // namespace cc1d

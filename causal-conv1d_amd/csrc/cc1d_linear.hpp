@@ -1,0 +1,102 @@
+// Linear attention with a decay for each head: what its kernels and its host side share.
+//
+//   S = exp(g[t]) S + beta[t] k[t] v[t]^T,   out[t] = scale S^T q[t]
+//
+// Sequences are cut into segments of kSegment tokens, segments into blocks of 64.  With G the running sum of g inside a segment,
+// E_ij = exp(G_i - G_j), S0 the state in front of a segment and dS1 the gradient of the one behind it:
+//
+//   out_i = scale (exp(G_i) q_i S0 + sum over j <= i of E_ij (q_i.k_j) beta_j v_j)
+//   dq_i  = scale (exp(G_i) dout_i S0^T + sum over j <= i of E_ij (dout_i.v_j) beta_j k_j)
+//   dk_j  = beta_j (exp(Gend - G_j) v_j dS1^T + sum over i >= j of E_ij (v_j.dout_i) scale q_i)
+//   dv_j  = beta_j (exp(Gend - G_j) k_j dS1 + sum over i >= j of E_ij (k_j.q_i) scale dout_i)
+//
+// These four are one kernel (linear_attend_kernel) on tensors x, y, z and a state: rows x_i of one block times the state, and products
+// x_i.y_j, weighted, times z_j over the blocks in front (REV: behind).  No state is carried inside a segment, so every block of every segment
+// is a workgroup of its own; what crosses segments is
+//
+//   S1 = exp(Gend) S0 + sum of exp(Gend - G_j) beta_j k_j v_j^T,   dS0 = exp(Gend) dS1 + sum of exp(G_i) scale q_i dout_i^T
+//
+// whose sums are one more kernel (linear_states_kernel), and whose recurrence over segments is elementwise (linear_scan_kernel).  The gates'
+// gradients come out of sums that are there: dg at a segment's first token is S0 . dS0 over all elements (nothing else reads that gate's product), and
+// dg[t + 1] = dg[t] - (q[t].dq[t] - k[t].dk[t]).
+//
+// Numbers of 24 bits on the 16-bit matrix cores: cc1d_delta_chunk.hpp.
+#pragma once
+
+#include "cc1d_delta_chunk.hpp"
+
+namespace cc1d {
+
+constexpr int kSegmentLog = 8, kSegment = 1 << kSegmentLog, kBlocks = kSegment / kChunk;
+
+// A (batch, seqlen, heads, dim) tensor; by_key: its heads are the key heads.
+struct LinearRows { const void *p; int64_t sb, sl, sh; int32_t by_key; };
+
+// Terms of the states and weighted products where they make outputs of x_dtype alone; where they make the gates' gradients too, which are fp32 and
+// small differences of large sums, three.
+constexpr int out_terms(int dt) { return dt == CC1D_F32 ? 3 : 2; }
+
+struct SegmentWork {
+    int32_t slots, chunks;               // segments of the call; of one sequence without cu_seqlens
+    int32_t kp, vp;                      // 32-column steps of dim_k, dim_v
+    FastDiv by_v_heads, by_chunks, by_group;
+    float *local;                        // per (slot, value head): a segment's own sum, [kp][vp] tiles of 32 x 32 in operand order
+    float *decay;                        // per (slot, value head): exp(Gend)
+    uint8_t *by_k, *by_v;                // per (slot, value head): states split into operands, contracted over dim_k and over dim_v
+    uint8_t *first;                      // S0 of the forward, contracted over dim_v: what a training forward saves
+    float *dot_q, *dot_k;                // per (slot, value head): q.dq and k.(dk / beta) of each token
+    float *inner;                        // per (slot, value head): S0 . dS0, a partial sum each tile
+    float *share_q, *share_k;            // shares of dq, dk of heads_each value heads: (shares, batch, seqlen, heads, dim_k)
+    int32_t heads_each, shares;          // value heads of a workgroup of the gradients of q and k; such workgroups a key head
+    __device__ __host__ int64_t tiles() const { return (int64_t)kp * vp; }
+};
+
+// Tokens [lo, lo + count) of batch entry b: segment c of sequence n, or count = 0 if a slot is none.
+struct SegmentAt { int64_t lo; int count, b, n, c; bool last; };
+__device__ __forceinline__ SegmentAt segment_at(const cc1d_delta_params &p, const SegmentWork &w, int slot) {
+    if (p.cu_seqlens == nullptr) {
+        const int n = (int)divided((uint32_t)slot, w.by_chunks), c = slot - n * w.chunks;
+        const int64_t lo = (int64_t)c << kSegmentLog, left = p.seqlen - lo;
+        return {lo, (int)(left < kSegment ? left : kSegment), n, n, c, left <= kSegment};
+    }
+    // As chunks of the gated delta rule: sequence n begins at slot floor(first token / kSegment) + n, and no two share one.
+    const int n = last_sequence(p, slot, [](int64_t first, int i) { return (first >> kSegmentLog) + i; });
+    const TokenRange r = sequence_tokens(p, n);
+    const int64_t c = slot - ((r.lo >> kSegmentLog) + n), lo = r.lo + (c << kSegmentLog), left = r.hi - lo;
+    if (c < 0 || left <= 0) return {0, 0, 0, n, 0, false};
+    return {lo, (int)(left < kSegment ? left : kSegment), 0, n, (int)c, left <= kSegment};
+}
+__device__ __forceinline__ int first_segment(const cc1d_delta_params &p, const SegmentWork &w, int n, const TokenRange &r) {
+    return p.cu_seqlens == nullptr ? n * w.chunks : (int)(r.lo >> kSegmentLog) + n;
+}
+
+// Which sums a segment's neighbours need: forward those in front of the last (and the last, if the states are asked for), backward those behind
+// the first.
+struct StatesArgs { LinearRows a, b; int32_t from_start, all; float factor; int32_t vec; };
+struct ScanArgs {
+    const float *first; int64_t first_n, first_h, first_k;     // the state it begins with, or NULL
+    float *last; int64_t last_n, last_h, last_k;               // where it ends, or NULL
+    int32_t to_end;                      // the last segment's own sum is there too: `last`, or S0 . dS0 of the first, need it
+    int32_t reverse, write_k, write_v, use_inner;
+};
+struct AttendArgs {
+    LinearRows x, y, z, u;               // u: what the rows of the result are multiplied with for the gates' gradients
+    const uint8_t *state;
+    int32_t d1, d2, steps, pairs;        // columns of x, y and of z; 32-column steps of them
+    int32_t first;                       // the first segment (REV: the last) has a state too
+    int32_t group, heads_each, shares;   // value heads of a key head, of a workgroup; workgroups of a key head
+    uint32_t items, col_tiles;           // (slot, key head, share); 128-column tiles of d2
+    FastDiv by_col_tiles, by_heads, by_shares;
+    void *out; int64_t out_b, out_l, out_h;   // of x_dtype, by value head or (DOTS) by key head; NULL: to `share`
+    float *share, *dots;
+};
+
+int launch_linear_states(const cc1d_delta_params &p, const SegmentWork &w, const StatesArgs &a, hipStream_t stream);
+int launch_linear_scan(const cc1d_delta_params &p, const SegmentWork &w, const ScanArgs &a, hipStream_t stream);
+// Instantiated one to a file.  DOTS: gradients of q and k.
+template <int DT, bool REV, bool DOTS>
+int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, bool vec, hipStream_t stream);
+int launch_linear_gates(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream);
+int launch_linear_join(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream);
+
+}  // namespace cc1d

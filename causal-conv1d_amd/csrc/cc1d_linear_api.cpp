@@ -1,0 +1,344 @@
+// C-ABI front of linear attention (cc1d_mixer.h): argument validation, layout of the workspace and the order of the launches.  Nothing
+// here allocates or synchronises; validation never touches the GPU.
+#include "cc1d_delta_host.hpp"
+#include "cc1d_linear.hpp"
+
+namespace cc1d {
+
+#define CC1D_ATTEND(DT)                                                                                                                          \
+    extern template int launch_attend<DT, false, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);   \
+    extern template int launch_attend<DT, true, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);    \
+    extern template int launch_attend<DT, false, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);    \
+    extern template int launch_attend<DT, true, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);
+CC1D_ATTEND(CC1D_F32)
+CC1D_ATTEND(CC1D_F16)
+CC1D_ATTEND(CC1D_BF16)
+#undef CC1D_ATTEND
+
+}  // namespace cc1d
+
+using namespace cc1d;
+
+namespace {
+
+bool aligned256(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
+
+// The blocks are the gated delta rule's, whose checks want a beta.
+template <typename P>
+P with_beta(const P &p) {
+    P q = p;
+    if (q.beta == nullptr) {
+        q.beta = q.g;
+        q.beta_dtype = q.g_dtype;
+    }
+    return q;
+}
+
+// Rows of a segment are reached with 32 bits.
+bool near(const cc1d_delta_params &p, int64_t stride) {
+    return p.seqlen <= 1 || (stride >= 0 && stride * elem_bytes(p.x_dtype) < ((int64_t)1 << 31) / kSegment);
+}
+bool reachable(const cc1d_delta_params &p) { return near(p, p.q_stride_l) && near(p, p.k_stride_l) && near(p, p.v_stride_l); }
+
+// Sequences of this many tokens on average go by segments; `saved`: all do.
+int segments_from(const cc1d_delta_params &p) { return 16; }
+bool by_segments(const cc1d_delta_params &p) {
+    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return false;
+    if (p.saved != nullptr) return true;
+    return reachable(p) && p.seqlen >= (int64_t)segments_from(p) * (p.cu_seqlens == nullptr ? 1 : p.sequences);
+}
+// Whether any segment has a state in front of it.
+bool has_states(const cc1d_delta_params &p, const SegmentWork &w) { return w.chunks > 1 || p.cu_seqlens != nullptr || p.initial_states != nullptr; }
+
+struct Places {
+    uint8_t *base;
+    size_t used = 0;
+    uint8_t *take(size_t bytes) {
+        uint8_t *at = base + used;
+        used += (bytes + 255) / 256 * 256;
+        return at;
+    }
+    float *floats(size_t n) { return reinterpret_cast<float *>(take(n * sizeof(float))); }
+};
+
+SegmentWork sizes_of(const cc1d_delta_params &p) {
+    SegmentWork w = {};
+    w.chunks = (int32_t)(((int64_t)p.seqlen + kSegment - 1) / kSegment);
+    const int64_t slots = p.cu_seqlens == nullptr ? (int64_t)p.batch * w.chunks : (int64_t)p.seqlen / kSegment + p.sequences + 1;
+    w.slots = (int32_t)(slots < INT32_MAX ? slots : INT32_MAX);
+    w.kp = (p.dim_k + 31) / 32;
+    w.vp = (p.dim_v + 31) / 32;
+    w.by_v_heads = fast_div((uint32_t)p.v_heads);
+    w.by_chunks = fast_div((uint32_t)w.chunks);
+    w.by_group = fast_div((uint32_t)(p.heads > 0 ? p.v_heads / p.heads : 1));
+    return w;
+}
+// Numbers of 32 x 32 tiles: of one state for every slot and value head.
+size_t state_tiles(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.tiles(); }
+
+// One workgroup a (slot, block, value head, 128 columns) and less; the scan's one wavefront a tile of each sequence's states.
+bool grids_fit(const cc1d_delta_params &p, const SegmentWork &w) {
+    return ((int64_t)w.slots * p.v_heads + 8) * kBlocks * ((w.vp + 3) / 4) < thread_limit() / kBlock &&
+           (int64_t)p.sequences * p.v_heads * w.tiles() < thread_limit() / kWave;
+}
+
+size_t lay_out_fwd(const cc1d_delta_params &p, uint8_t *base, SegmentWork &w) {
+    w = sizes_of(p);
+    Places work{base};
+    if (has_states(p, w) || p.final_states != nullptr) {
+        const size_t tiles = state_tiles(p, w);
+        w.local = work.floats(tiles * 1024);
+        w.decay = work.floats((size_t)w.slots * p.v_heads);
+        w.by_k = work.take(tiles * 2 * out_terms(p.x_dtype) * kFrag);
+    }
+    w.by_v = static_cast<uint8_t *>(p.saved);
+    return work.used;
+}
+
+// Value heads that a workgroup of the gradients of q and k takes one after the other: as many as leave four workgroups for every CU, since each
+// workgroup of a shared key head writes its share in fp32.
+void share_heads(const cc1d_delta_params &p, SegmentWork &w) {
+    const int group = p.v_heads / p.heads;
+    const int64_t each = (int64_t)w.slots * kBlocks * p.v_heads / 1024;
+    w.heads_each = each < 1 ? 1 : each > group ? group : (int32_t)each;
+    w.shares = (group + w.heads_each - 1) / w.heads_each;
+    w.heads_each = (group + w.shares - 1) / w.shares;
+    w.shares = (group + w.heads_each - 1) / w.heads_each;
+}
+bool gradient_of_states(const cc1d_delta_bwd_params &bp, const SegmentWork &w) {
+    return has_states(bp.fwd, w) || bp.dfinal_states != nullptr || bp.dinitial_states != nullptr;
+}
+size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &w) {
+    const cc1d_delta_params &p = bp.fwd;
+    w = sizes_of(p);
+    w.first = static_cast<uint8_t *>(p.saved);
+    Places work{base};
+    share_heads(p, w);
+    const size_t heads = (size_t)w.slots * p.v_heads;
+    if (gradient_of_states(bp, w)) {
+        const size_t tiles = state_tiles(p, w);
+        w.local = work.floats(tiles * 1024);
+        w.decay = work.floats(heads);
+        w.by_k = work.take(tiles * 2 * out_terms(p.x_dtype) * kFrag);
+        w.by_v = work.take(tiles * 2 * 3 * kFrag);
+        w.inner = work.floats(tiles);
+    }
+    w.dot_q = work.floats(heads * kSegment);
+    w.dot_k = work.floats(heads * kSegment);
+    if (w.shares > 1) {
+        const size_t plane = (size_t)p.batch * p.seqlen * p.heads * p.dim_k;
+        w.share_q = work.floats(w.shares * plane);
+        w.share_k = work.floats(w.shares * plane);
+    }
+    return work.used;
+}
+
+LinearRows rows(const void *x, int64_t sb, int64_t sl, int64_t sh, bool by_key) { return {x, sb, sl, sh, by_key}; }
+#define ROWS(P, NAME, KEY) rows(P.NAME, P.NAME##_stride_b, P.NAME##_stride_l, P.NAME##_stride_h, KEY)
+
+// Rows of whole 16-byte vectors, for x and y; of whole column pairs.
+bool whole(int dtype, const LinearRows &r, int dim) { return dim % 8 == 0 && whole_rows(dtype, r.p, r.sb, r.sl, r.sh); }
+bool paired(int dtype, const void *x, int64_t sb, int64_t sl, int64_t sh, int dim) {
+    return dim % 2 == 0 && (reinterpret_cast<uintptr_t>(x) & (2u * (uint32_t)elem_bytes(dtype) - 1u)) == 0 && sb % 2 == 0 && sl % 2 == 0 && sh % 2 == 0;
+}
+bool paired(int dtype, const LinearRows &r, int dim) { return paired(dtype, r.p, r.sb, r.sl, r.sh, dim); }
+
+int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool rev, bool dots, hipStream_t stream) {
+    if (w.slots == 0) return CC1D_OK;
+    a.group = p.v_heads / p.heads;
+    a.heads_each = dots ? w.heads_each : 1;
+    a.shares = dots ? w.shares : a.group;
+    a.steps = (a.d1 + 31) / 32;
+    a.pairs = (a.d2 + 31) / 32;
+    a.items = (uint32_t)w.slots * (uint32_t)p.heads * (uint32_t)a.shares;
+    a.col_tiles = dots ? 1u : (uint32_t)(a.d2 + 127) / 128;
+    a.by_col_tiles = fast_div(a.col_tiles);
+    a.by_heads = fast_div((uint32_t)p.heads);
+    a.by_shares = fast_div((uint32_t)a.shares);
+    const bool vec = whole(p.x_dtype, a.x, a.d1) && whole(p.x_dtype, a.y, a.d1) && paired(p.x_dtype, a.z, a.d2) &&
+                     (a.share != nullptr || paired(p.x_dtype, a.out, a.out_b, a.out_l, a.out_h, a.d2));
+    auto of_type = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (rev) return dots ? launch_attend<DT, true, true>(p, w, a, vec, stream) : launch_attend<DT, true, false>(p, w, a, vec, stream);
+        return dots ? launch_attend<DT, false, true>(p, w, a, vec, stream) : launch_attend<DT, false, false>(p, w, a, vec, stream);
+    };
+    switch (p.x_dtype) {
+        case CC1D_F32: return of_type(std::integral_constant<int, CC1D_F32>());
+        case CC1D_F16: return of_type(std::integral_constant<int, CC1D_F16>());
+        default: return of_type(std::integral_constant<int, CC1D_BF16>());
+    }
+}
+
+int forward(const cc1d_delta_params &p, const SegmentWork &w, hipStream_t stream) {
+    const LinearRows q = ROWS(p, q, true), k = ROWS(p, k, true), v = ROWS(p, v, false);
+    int st = CC1D_OK;
+    const bool states = has_states(p, w);
+    if (w.chunks > 1 || p.cu_seqlens != nullptr || p.final_states != nullptr) {
+        StatesArgs a = {};
+        a.a = k; a.b = v; a.all = p.final_states != nullptr;
+        a.vec = paired(p.x_dtype, k, p.dim_k) && paired(p.x_dtype, v, p.dim_v);
+        st = launch_linear_states(p, w, a, stream);
+        if (st != CC1D_OK) return st;
+    }
+    if (states || p.final_states != nullptr) {
+        ScanArgs a = {};
+        a.first = p.initial_states; a.first_n = p.init_stride_n; a.first_h = p.init_stride_h; a.first_k = p.init_stride_k;
+        a.last = p.final_states; a.last_n = p.final_stride_n; a.last_h = p.final_stride_h; a.last_k = p.final_stride_k;
+        a.to_end = p.final_states != nullptr;
+        a.write_k = states;
+        a.write_v = states && p.saved != nullptr;
+        st = launch_linear_scan(p, w, a, stream);
+        if (st != CC1D_OK) return st;
+    }
+    AttendArgs a = {};
+    a.x = q; a.y = k; a.z = v;
+    a.d1 = p.dim_k; a.d2 = p.dim_v;
+    a.state = w.by_k;
+    a.first = p.initial_states != nullptr;
+    a.out = p.out; a.out_b = p.out_stride_b; a.out_l = p.out_stride_l; a.out_h = p.out_stride_h;
+    return attend(p, w, a, false, false, stream);
+}
+
+int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream) {
+    const cc1d_delta_params &p = bp.fwd;
+    const LinearRows q = ROWS(p, q, true), k = ROWS(p, k, true), v = ROWS(p, v, false), dout = ROWS(bp, dout, false);
+    int st = CC1D_OK;
+    const bool initial = p.initial_states != nullptr, to_end = initial || bp.dinitial_states != nullptr;
+    if (w.slots > 0 && (w.chunks > 1 || p.cu_seqlens != nullptr || to_end)) {
+        StatesArgs a = {};
+        a.a = q; a.b = dout; a.from_start = 1; a.all = to_end; a.factor = p.scale;
+        a.vec = paired(p.x_dtype, q, p.dim_k) && paired(p.x_dtype, dout, p.dim_v);
+        st = launch_linear_states(p, w, a, stream);
+        if (st != CC1D_OK) return st;
+    }
+    if (gradient_of_states(bp, w)) {
+        ScanArgs a = {};
+        a.first = bp.dfinal_states; a.first_n = bp.dfinal_stride_n; a.first_h = bp.dfinal_stride_h; a.first_k = bp.dfinal_stride_k;
+        a.last = bp.dinitial_states; a.last_n = bp.dinit_stride_n; a.last_h = bp.dinit_stride_h; a.last_k = bp.dinit_stride_k;
+        a.to_end = to_end;
+        a.reverse = a.write_k = a.write_v = 1;
+        a.use_inner = 1 + initial;
+        st = launch_linear_scan(p, w, a, stream);
+        if (st != CC1D_OK) return st;
+    }
+    AttendArgs a = {};                                   // dq
+    a.x = dout; a.y = v; a.z = k; a.u = q;
+    a.d1 = p.dim_v; a.d2 = p.dim_k;
+    a.state = w.first;
+    a.first = initial;
+    a.out = bp.dq; a.out_b = bp.dq_stride_b; a.out_l = bp.dq_stride_l; a.out_h = bp.dq_stride_h;
+    a.share = w.share_q; a.dots = w.dot_q;
+    st = attend(p, w, a, false, true, stream);
+    if (st != CC1D_OK) return st;
+    a.x = v; a.y = dout; a.z = q; a.u = k;               // dk
+    a.state = w.by_v;
+    a.first = bp.dfinal_states != nullptr;
+    a.out = bp.dk; a.out_b = bp.dk_stride_b; a.out_l = bp.dk_stride_l; a.out_h = bp.dk_stride_h;
+    a.share = w.share_k; a.dots = w.dot_k;
+    st = attend(p, w, a, true, true, stream);
+    if (st != CC1D_OK) return st;
+    AttendArgs d = {};                                   // dv
+    d.x = k; d.y = q; d.z = dout;
+    d.d1 = p.dim_k; d.d2 = p.dim_v;
+    d.state = w.by_k;
+    d.first = bp.dfinal_states != nullptr;
+    d.out = bp.dv; d.out_b = bp.dv_stride_b; d.out_l = bp.dv_stride_l; d.out_h = bp.dv_stride_h;
+    st = attend(p, w, d, true, false, stream);
+    if (st == CC1D_OK) st = launch_linear_gates(bp, w, stream);
+    if (st == CC1D_OK && w.shares > 1 && w.slots > 0) st = launch_linear_join(bp, w, stream);
+    return st;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cc1d_validate_linear(const cc1d_delta_params *p) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const cc1d_delta_params q = with_beta(*p);
+    const int st = cc1d_validate_delta(&q);
+    return st == CC1D_OK && p->qk_l2norm != 0 ? CC1D_ERR_OPTION : st;
+}
+
+int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
+    if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
+    *bytes = 0;
+    const int st = cc1d_validate_linear(p);
+    if (st != CC1D_OK || !by_segments(*p)) return st;
+    SegmentWork w;
+    *bytes = lay_out_fwd(*p, nullptr, w);
+    return grids_fit(*p, w) && reachable(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+}
+
+int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
+    if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
+    *bytes = 0;
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    cc1d_delta_params q = with_beta(*p);
+    if (q.out == nullptr) q.out = const_cast<void *>(q.v);                 // (not needed for this)
+    const int st = cc1d_validate_delta(&q);
+    if (st != CC1D_OK) return st;
+    const SegmentWork w = sizes_of(*p);
+    *bytes = state_tiles(*p, w) * 2 * 3 * kFrag;
+    return CC1D_OK;
+}
+
+int cc1d_linear_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
+    size_t need = 0;
+    const int st = cc1d_linear_workspace_bytes(p, &need);
+    if (st != CC1D_OK) return st;
+    if (need > 0 && (workspace == nullptr || !aligned256(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
+    if (p->batch == 0 || p->v_heads == 0 || p->sequences == 0) return CC1D_OK;
+    const hipStream_t hs = static_cast<hipStream_t>(stream);
+    if (!by_segments(*p)) return launch_delta_tokens(*p, nullptr, p->sequences, 0, hs, false);
+    SegmentWork w;
+    lay_out_fwd(*p, static_cast<uint8_t *>(workspace), w);
+    return forward(*p, w, hs);
+}
+
+int cc1d_validate_linear_bwd(const cc1d_delta_bwd_params *p) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    cc1d_delta_bwd_params q = *p;
+    q.fwd = with_beta(q.fwd);
+    if (p->fwd.beta == nullptr) q.dbeta = q.dg;
+    const int st = cc1d_validate_delta_bwd(&q);
+    return st == CC1D_OK && p->fwd.qk_l2norm != 0 ? CC1D_ERR_OPTION : st;
+}
+
+int cc1d_linear_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *bytes) {
+    if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
+    *bytes = 0;
+    const int st = cc1d_validate_linear_bwd(p);
+    if (st != CC1D_OK || p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return st;
+    SegmentWork w;
+    *bytes = lay_out_bwd(*p, nullptr, w);
+    return grids_fit(p->fwd, w) && reachable(p->fwd) && near(p->fwd, p->dout_stride_l) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+}
+
+int cc1d_linear_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
+    size_t need = 0;
+    const int st = cc1d_linear_bwd_workspace_bytes(p, &need);
+    if (st != CC1D_OK) return st;
+    if (need > 0 && (workspace == nullptr || !aligned256(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
+    const hipStream_t hs = static_cast<hipStream_t>(stream);
+    if (p->fwd.v_heads == 0) return launch_delta_no_values(*p, hs);
+    if (p->fwd.batch == 0 || p->fwd.sequences == 0) return CC1D_OK;
+    SegmentWork w;
+    lay_out_bwd(*p, static_cast<uint8_t *>(workspace), w);
+    return backward(*p, w, hs);
+}
+
+int cc1d_validate_linear_step(const cc1d_delta_step_params *p) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const cc1d_delta_step_params q = with_beta(*p);
+    const int st = cc1d_validate_delta_step(&q);
+    return st == CC1D_OK && p->qk_l2norm != 0 ? CC1D_ERR_OPTION : st;
+}
+
+int cc1d_linear_step(const cc1d_delta_step_params *p, cc1d_stream_t stream) {
+    const int st = cc1d_validate_linear_step(p);
+    if (st != CC1D_OK) return st;
+    return launch_step_tokens(*p, static_cast<hipStream_t>(stream), false);
+}
+
+}  // extern "C"

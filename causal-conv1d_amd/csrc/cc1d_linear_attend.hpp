@@ -1,0 +1,397 @@
+// Linear attention, the kernel of out, dq, dk and dv (cc1d_linear.hpp):
+//
+//   r_i = f_i x_i.State + sum over j <= i (REV: j >= i) of E_ij c_j (x_i.y_j) z_j,   result row i = s_i r_i
+//
+//   out   x = q     y = k     z = v     State = S0     f = exp(G)         c = beta   s = scale
+//   dq    x = dout  y = v     z = k     State = S0^T   f = exp(G)         c = beta   s = scale      DOTS
+//   dk    x = v     y = dout  z = q     State = dS1^T  f = exp(Gend - G)  c = scale  s = beta  REV  DOTS
+//   dv    x = k     y = q     z = dout  State = dS1    f = exp(Gend - G)  c = scale  s = beta  REV
+//
+// A workgroup of four wavefronts makes 64 rows (one block of a segment) of up to 128 columns (CP = 2: 256).  A wavefront's result is 32 columns
+// of z, all rows (RT = 4), or half the rows where z has at most 64 columns (RT = 2): State and z are right operands that it reads for itself,
+// from memory in operand order and as column pairs (Pair8), so neither goes through LDS.  For the products x.y the wavefronts take 16 rows y_j each
+// against all 64 x_i, so that the result, transposed, is the left operand of the product with z in the lane that has it, four tokens at a time: weighted,
+// split into its terms and passed through LDS once, double-buffered, one barrier a block.
+//
+// E between two blocks is a product of two factors, exp(G_i - R) and exp(R - G_j), R between them, so that only a block with itself takes an exponential
+// an entry; there the tiles beyond the diagonal are left out.  Where gates grow (g > 0), each factor has to stay below 2^128.
+//
+// DOTS: several value heads of a key head one after the other, the sum of their rows kept in registers, and of each the rows' products with u
+// (q or k), which the gates' gradients are made of.  What several workgroups of a key head leave is joined by linear_join_kernel.
+#pragma once
+
+#include "cc1d_delta_host.hpp"
+#include "cc1d_linear_device.hpp"
+
+namespace cc1d {
+
+template <int DT, int KS, int PT>
+struct AttendLds {
+    uint8_t x[4 * KS * Terms<DT>::n * kFrag];
+    uint8_t p[2][8 * PT * kFrag];
+    GateLds gates;
+    float f[kChunk], s[kChunk];
+    float dots[4][kChunk];
+};
+
+constexpr int attend_waves(int dt, int cp) { return dt != CC1D_F32 && cp == 1 ? 2 : 1; }
+
+// KS: 32-column steps of x and y at once (their LDS); wider ones pass slab by slab.
+template <int DT, int KS, int RT, int CP, bool REV, bool DOTS, bool VEC>
+__global__ void __launch_bounds__(kBlock, attend_waves(DT, CP))
+linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
+    using T = typename Elem<DT>::type;
+    constexpr int NT = Terms<DT>::n, PT = DOTS ? 3 : out_terms(DT), MOST = PT - 1;
+    constexpr bool XREG = KS * NT <= 4;                  // x stays in registers
+    extern __shared__ uint4 raw[];
+    AttendLds<DT, KS, PT> &lds = *reinterpret_cast<AttendLds<DT, KS, PT> *>(raw);
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // The blocks of one segment and head, which read the same state and y and z, on one XCD; those with the most to do first.
+    const uint32_t idx = blockIdx.x >> 3, rest = idx / kBlocks, of_block = idx % kBlocks;
+    const uint32_t pos = divided(rest, a.by_col_tiles), ct = rest - pos * a.col_tiles, item = pos * 8u + (blockIdx.x & 7u);
+    if (item >= a.items) return;
+    const int r = REV ? (int)of_block : kBlocks - 1 - (int)of_block;
+    const uint32_t sh = divided(item, a.by_shares), share = item - sh * a.shares;
+    const int slot = (int)divided(sh, a.by_heads), hk = (int)sh - slot * p.heads;
+    const int h_first = hk * a.group + (int)share * a.heads_each, h_left = a.group - (int)share * a.heads_each;
+    const int h_count = !DOTS ? 1 : h_left < a.heads_each ? h_left : a.heads_each;
+
+    const int half = RT == 2 ? wave >> 1 : 0;            // which rows
+    const int pair0 = RT == 2 ? wave & 1 : (int)ct * 4 + wave;         // CP = 2: and pair0 + 4
+    const int i0 = 16 * RT * half;                       // first row of this wavefront's result
+    const int out_head = DOTS ? hk : h_first;
+    const SegmentAt at = segment_at(p, w, slot);
+
+    if (p.cu_seqlens != nullptr && (!DOTS || share == 0)) {            // tokens in front of the first sequence and behind the last
+        const int64_t front = sequence_tokens(p, 0).lo, back = sequence_tokens(p, p.sequences - 1).hi;
+        const int64_t from = ((int64_t)slot * kBlocks + r) * 4 + wave, step = (int64_t)w.slots * kBlocks * 4;
+        T *o = static_cast<T *>(a.out) + out_head * a.out_h;
+        auto clear = [&](int64_t t) {
+            if (a.share == nullptr) {
+                for (int c = (int)ct * 128 + lane; c < a.d2 && c < ((int)ct + CP) * 128; c += 64) o[t * a.out_l + c] = Elem<DT>::from_float(0.f);
+            } else {
+                for (int i = 0; i < a.shares; ++i)
+                    for (int c = lane; c < a.d2; c += 64) a.share[(((int64_t)i * p.seqlen + t) * p.heads + hk) * a.d2 + c] = 0.f;
+            }
+        };
+        for (int64_t t = from; t < front; t += step) clear(t);
+        for (int64_t t = back + from; t < p.seqlen; t += step) clear(t);
+    }
+    const int row0 = r * kChunk, own = at.count - row0;  // rows of this block, if any
+    if (own <= 0) return;
+    const int blocks = (at.count + kChunk - 1) / kChunk;
+    const int slabs = (a.steps + KS - 1) / KS;
+    const bool cut = a.d1 < 32 * KS * slabs;
+    const bool has_state = (REV ? !at.last : at.c > 0) || a.first;
+
+    f32x4 total[DOTS ? RT : 1][DOTS ? CP : 1][2];
+    if constexpr (DOTS)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int c = 0; c < CP; ++c) total[i][c][0] = total[i][c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[RT][CP][2];
+
+    for (int hi = 0; hi < h_count; ++hi) {
+        const int h = h_first + hi;
+        const int64_t sv = (int64_t)slot * p.v_heads + h;
+        auto rows_of = [&](const LinearRows &t) { return static_cast<const T *>(t.p) + at.b * t.sb + at.lo * t.sl + (t.by_key ? hk : h) * t.sh; };
+        const T *xb = rows_of(a.x), *yb = rows_of(a.y);
+        const uint8_t *zb = reinterpret_cast<const uint8_t *>(rows_of(a.z));
+        const uint32_t z_pitch = (uint32_t)(a.z.sl * (int64_t)sizeof(T));
+        auto token = [&](int t) { return t < at.count ? t : at.count - 1; };       // (rows behind the last weigh nothing, or are not stored)
+
+        Row8<DT, VEC> yr[KS];
+        auto ask_y = [&](int c, int slab) {
+            const T *row = yb + (int64_t)token(c * kChunk + row_of(wave, m)) * a.y.sl;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) yr[s].ask(row, 32 * (slab * KS + s) + 8 * g, a.d1);
+        };
+        auto stage_x = [&](int slab) {                   // 16 rows a wavefront
+            const T *row = xb + (int64_t)token(row0 + 16 * wave + m) * a.x.sl;
+            Row8<DT, VEC> xr[KS];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) xr[s].ask(row, 32 * (slab * KS + s) + 8 * g, a.d1);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                bf16x8 f[NT];
+                xr[s].template operand<NT>(32 * (slab * KS + s) + 8 * g, a.d1, cut, f);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) *reinterpret_cast<u32x4 *>(lds.x + ((wave * KS + s) * NT + n) * kFrag + lane * 16) = bitcast<u32x4>(f[n]);
+            }
+        };
+        const int turns = REV ? blocks - r : r + 1;
+        auto block_of = [&](int k) { return REV ? blocks - 1 - k : k; };           // the block itself comes last
+
+        if (hi > 0) lds_barrier();                       // the head before has read its gates and products
+        if (slabs == 1) ask_y(block_of(0), 0);
+        stage_x(0);
+        segment_gates(p, at, h, wave, lane, lds.gates);  // (its barriers are x's too)
+        if (wave == 0) {
+            const int t = row0 + lane;
+            lds.f[lane] = REV ? decay_between(lds.gates, t, kSegment - 1) : decay_since_start(lds.gates, t);
+            lds.s[lane] = REV ? lds.gates.beta[t] : p.scale;
+        }
+        // x as a left operand (its products with the state) and as a right one (y's with it): the same 8 columns of row 16 t + m.
+        bf16x8 xr[XREG ? 4 : 1][XREG ? KS : 1][NT];
+        auto load_x = [&]() {
+            if constexpr (XREG)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) load_frag<NT>(lds.x + (t * KS + s) * NT * kFrag, lane, xr[t][s]);
+        };
+        load_x();
+        auto x_of = [&](int t, int s, bf16x8 (&f)[NT]) {
+            if constexpr (XREG) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) f[n] = xr[t][s][n];
+            } else {
+                load_frag<NT>(lds.x + (t * KS + s) * NT * kFrag, lane, f);
+            }
+        };
+
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int c = 0; c < CP; ++c) acc[i][c][0] = acc[i][c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (has_state) {
+            const uint8_t *st = a.state + sv * (int64_t)a.steps * a.pairs * 2 * PT * kFrag + lane * 16;
+            for (int slab = 0; slab < slabs; ++slab) {
+                if (slab > 0) {
+                    lds_barrier();
+                    stage_x(slab);
+                    lds_barrier();
+                    load_x();
+                }
+#pragma unroll
+                for (int c = 0; c < CP; ++c) {
+                    const int pair = pair0 + 4 * c;
+                    if (pair >= a.pairs) continue;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const int step = slab * KS + s;
+                        if (step >= a.steps) break;
+                        bf16x8 b[2][PT];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) load_frag<PT>(st + (((int64_t)step * a.pairs + pair) * 2 + n) * PT * kFrag, 0, b[n]);
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            bf16x8 f[NT];
+                            if constexpr (RT == 4) x_of(i, s, f);
+                            else load_frag<NT>(lds.x + ((half * RT + i) * KS + s) * NT * kFrag, lane, f);
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) acc[i][c][n] = product<MOST>(f, b[n], acc[i][c][n]);
+                        }
+                    }
+                }
+            }
+        }
+        lds_barrier();                                   // f, s
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const float4 f = *reinterpret_cast<const float4 *>(&lds.f[i0 + 16 * i + 4 * g]);
+            const f32x4 by = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int c = 0; c < CP; ++c)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) acc[i][c][n] = has_state ? acc[i][c][n] * by : acc[i][c][n];
+        }
+        // Between blocks: R is G at the end of the block in front (REV: of this one).
+        const int border = REV ? row0 + kChunk - 1 : row0 > 0 ? row0 - 1 : 0;
+        float of_x[4];                                   // of row 16 t + m
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int i = row0 + 16 * t + m;
+            of_x[t] = turns > 1 ? (REV ? decay_between(lds.gates, i, border) : decay_between(lds.gates, border, i)) : 0.f;
+        }
+
+        for (int k = 0; k < turns; ++k) {
+            const int c0 = block_of(k);
+            const bool self = k == turns - 1;
+            Pair8<DT, VEC> zr[CP][2];
+            auto ask_z = [&]() {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    uint32_t off[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) off[e] = (uint32_t)token(c0 * kChunk + 32 * s + 8 * g + e) * z_pitch;
+#pragma unroll
+                    for (int c = 0; c < CP; ++c) zr[c][s].ask(zb, off, 32 * (pair0 + 4 * c) + 2 * m, a.d2);
+                }
+            };
+            ask_z();
+            f32x4 pt[4];                                 // rows: y's four tokens, columns: x's rows 16 t + m
+#pragma unroll
+            for (int t = 0; t < 4; ++t) pt[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const int y_half = wave >> 1;
+            auto meets = [&](int t, int s) { return !self || (REV ? t <= 2 * s + 1 : t >= 2 * s); };   // x's tile t, 32 of y's tokens
+            for (int slab = 0; slab < slabs; ++slab) {
+                if (slabs > 1) {
+                    lds_barrier();
+                    stage_x(slab);
+                    ask_y(c0, slab);
+                    lds_barrier();
+                    load_x();
+                }
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    bf16x8 f[NT];
+                    yr[s].template operand<NT>(32 * (slab * KS + s) + 8 * g, a.d1, cut, f);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        if (!meets(t, y_half)) continue;
+                        bf16x8 b[NT];
+                        x_of(t, s, b);
+                        pt[t] = product<2>(f, b, pt[t]);
+                    }
+                }
+            }
+            if (slabs == 1 && !self) ask_y(block_of(k + 1), 0);
+            // Weights, terms, and through LDS.
+            {
+                const int j0 = c0 * kChunk + row_of(wave, 4 * g);
+                float cj[4], hj[4], lj[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    cj[e] = REV ? (j0 + e < at.count ? p.scale : 0.f) : lds.gates.beta[j0 + e];
+                    hj[e] = lds.gates.hi[j0 + e];
+                    lj[e] = lds.gates.lo[j0 + e];
+                    if (!self) cj[e] *= REV ? decay_between(lds.gates, border, j0 + e) : decay_between(lds.gates, j0 + e, border);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    if (!meets(t, y_half)) continue;
+                    float x[4];
+                    if (self) {
+                        const int i = row0 + 16 * t + m;
+                        const float hx = lds.gates.hi[i], lx = lds.gates.lo[i];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float d = REV ? (hj[e] - hx) + (lj[e] - lx) : (hx - hj[e]) + (lx - lj[e]);
+                            x[e] = (REV ? j0 + e >= i : j0 + e <= i) ? pt[t][e] * (cj[e] * exp_of(d)) : 0.f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = pt[t][e] * (cj[e] * of_x[t]);
+                    }
+                    u32x2 f[PT];
+                    split4<PT>(x, f);
+#pragma unroll
+                    for (int n = 0; n < PT; ++n)
+                        *reinterpret_cast<u32x2 *>(lds.p[k & 1] + ((t * 2 + y_half) * PT + n) * kFrag + lane * 16 + (wave & 1) * 8) = f[n];
+                }
+            }
+            lds_barrier();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                bf16x8 fz[CP][2][NT];
+#pragma unroll
+                for (int c = 0; c < CP; ++c)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) zr[c][s].template operand<NT>(n, fz[c][n]);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    const int t = half * RT + i;
+                    if (!meets(t, s)) continue;
+                    bf16x8 f[PT];
+                    load_frag<PT>(lds.p[k & 1] + (t * 2 + s) * PT * kFrag, lane, f);
+#pragma unroll
+                    for (int c = 0; c < CP; ++c)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) acc[i][c][n] = product<MOST>(f, fz[c][n], acc[i][c][n]);
+                }
+            }
+        }
+
+        if constexpr (DOTS) {
+            const T *ub = rows_of(a.u);
+            float dot[RT][4];
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const T *row = ub + (int64_t)token(row0 + i0 + 16 * i + 4 * g + e) * a.u.sl;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int c = 0; c < CP; ++c) {
+                        const int col = 32 * (pair0 + 4 * c) + 2 * m;
+                        const float u0 = Elem<DT>::to_float(row[col < a.d2 ? col : 0]), u1 = Elem<DT>::to_float(row[col + 1 < a.d2 ? col + 1 : 0]);
+                        sum += col < a.d2 ? acc[i][c][0][e] * u0 : 0.f;
+                        sum += col + 1 < a.d2 ? acc[i][c][1][e] * u1 : 0.f;
+                    }
+                    dot[i][e] = over_columns(sum);
+                }
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const int row = i0 + 16 * i + 4 * g;
+                if (m == 0) *reinterpret_cast<float4 *>(&lds.dots[wave][row]) = make_float4(dot[i][0], dot[i][1], dot[i][2], dot[i][3]);
+                const float4 s = *reinterpret_cast<const float4 *>(&lds.s[row]);
+                const f32x4 by = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int c = 0; c < CP; ++c)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) total[i][c][n] += acc[i][c][n] * by;
+            }
+            lds_barrier();
+            if (wave == 0 && lane < own) {
+                float d = RT == 2 ? lds.dots[2 * (lane >> 5)][lane] + lds.dots[2 * (lane >> 5) + 1][lane]
+                                  : (lds.dots[0][lane] + lds.dots[1][lane]) + (lds.dots[2][lane] + lds.dots[3][lane]);
+                a.dots[sv * kSegment + row0 + lane] = REV ? d : p.scale * d;
+            }
+        }
+    }
+
+    // Rows leave as column pairs.
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int row = i0 + 16 * i + 4 * g;
+        float s[4] = {1.f, 1.f, 1.f, 1.f};
+        if constexpr (!DOTS) {
+            const float4 f = *reinterpret_cast<const float4 *>(&lds.s[row]);
+            s[0] = f.x; s[1] = f.y; s[2] = f.z; s[3] = f.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (row + e >= own) continue;
+            const int64_t tok = at.lo + row0 + row + e;
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+                const int col = 32 * (pair0 + 4 * c) + 2 * m;
+                float o0, o1;
+                if constexpr (DOTS) { o0 = total[i][c][0][e]; o1 = total[i][c][1][e]; }
+                else { o0 = s[e] * acc[i][c][0][e]; o1 = s[e] * acc[i][c][1][e]; }
+                if (a.share == nullptr) {
+                    store_pair<DT, VEC>(static_cast<T *>(a.out) + at.b * a.out_b + tok * a.out_l + out_head * a.out_h, col, a.d2, o0, o1);
+                } else {
+                    store_pair<CC1D_F32, false>(a.share + ((((int64_t)share * p.batch + at.b) * p.seqlen + tok) * p.heads + hk) * a.d2, col, a.d2, o0, o1);
+                }
+            }
+        }
+    }
+}
+
+// Of one type, direction and kind: each is a file of its own.
+template <int DT, bool REV, bool DOTS>
+int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, bool vec, hipStream_t stream) {
+    const dim3 grid((a.items + 7) / 8 * 8 * kBlocks * a.col_tiles);
+    auto go = [&](auto ks, auto rt, auto cp, auto v) {
+        constexpr int KS = decltype(ks)::value, RT = decltype(rt)::value, CP = decltype(cp)::value;
+        constexpr size_t lds = sizeof(AttendLds<DT, KS, DOTS ? 3 : out_terms(DT)>);
+        CC1D_LAUNCH((linear_attend_kernel<DT, KS, RT, CP, REV, DOTS, decltype(v)::value>), grid, dim3(kBlock), lds, stream, p, w, a);
+        return launch_status();
+    };
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
+    auto by_columns = [&](auto ks) {
+        if constexpr (DOTS)
+            if (a.d2 > 128) return vec ? go(ks, I4(), I2(), std::true_type()) : go(ks, I4(), I2(), std::false_type());
+        if (!vec) return go(ks, I4(), I1(), std::false_type());
+        return a.d2 <= 64 ? go(ks, I2(), I1(), std::true_type()) : go(ks, I4(), I1(), std::true_type());
+    };
+    return a.steps <= 2 ? by_columns(I2()) : by_columns(I4());
+}
+
+}  // namespace cc1d

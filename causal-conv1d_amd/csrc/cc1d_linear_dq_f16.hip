@@ -1,0 +1,6 @@
+// Linear attention, dq of f16 tensors (cc1d_linear_attend.hpp).
+#include "cc1d_linear_attend.hpp"
+
+namespace cc1d {
+template int launch_attend<CC1D_F16, false, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);
+}

@@ -1,4 +1,4 @@
-// PyTorch binding of cc1d_mixer.h: the gated delta rule and the root-mean-square norm as ops of the DaoAILab
+// PyTorch binding of cc1d_mixer.h: the gated delta rule, linear attention and the norms as ops of the DaoAILab
 // library, part of the extension module `causal_conv1d_cuda`.  Host-only C++: tensors are checked, results and
 // workspaces come from the caching allocator, launches go to the current stream of the tensors' device.
 #include <torch/extension.h>
@@ -41,15 +41,31 @@ at::Tensor workspace_of(size_t bytes, const at::Tensor &like) {
     return bytes ? empty_of({(int64_t)bytes}, at::kByte, like) : at::Tensor();
 }
 
-// ---- gated delta rule ----------------------------------------------------------------
+// ---- gated delta rule, linear attention ------------------------------------------------
+// One binding for both: the same parameter blocks, the second without lengths of q and k and with an optional beta.
+struct Recurrence {
+    int (*workspace_bytes)(const cc1d_delta_params *, size_t *);
+    int (*saved_bytes)(const cc1d_delta_params *, size_t *);
+    int (*fwd)(const cc1d_delta_params *, void *, size_t, cc1d_stream_t);
+    int (*bwd_workspace_bytes)(const cc1d_delta_bwd_params *, size_t *);
+    int (*bwd)(const cc1d_delta_bwd_params *, void *, size_t, cc1d_stream_t);
+    int (*step)(const cc1d_delta_step_params *, cc1d_stream_t);
+    const char *name, *name_bwd, *name_update;
+};
+constexpr Recurrence kDelta = {cc1d_delta_workspace_bytes, cc1d_delta_saved_bytes, cc1d_delta_fwd, cc1d_delta_bwd_workspace_bytes, cc1d_delta_bwd, cc1d_delta_step,
+                               "gated_delta_rule", "gated_delta_rule backward", "gated_delta_rule_update"};
+constexpr Recurrence kLinear = {cc1d_linear_workspace_bytes, cc1d_linear_saved_bytes, cc1d_linear_fwd, cc1d_linear_bwd_workspace_bytes, cc1d_linear_bwd, cc1d_linear_step,
+                                "linear_attention", "linear_attention backward", "linear_attention_update"};
 
 struct DeltaInputs {
-    at::Tensor q, k, v, g, beta;
+    at::Tensor q, k, v, g;
+    OptTensor beta;
     int64_t batch, seqlen, heads, v_heads, dim_k, dim_v;
 };
 
-DeltaInputs delta_inputs(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta) {
-    check_gpu(q, q, "q"); check_gpu(k, q, "k"); check_gpu(v, q, "v"); check_gpu(g, q, "g"); check_gpu(beta, q, "beta");
+DeltaInputs delta_inputs(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &opt_beta) {
+    check_gpu(q, q, "q"); check_gpu(k, q, "k"); check_gpu(v, q, "v"); check_gpu(g, q, "g");
+    if (opt_beta.has_value()) check_gpu(*opt_beta, q, "beta");
     TORCH_CHECK(q.dim() == 4, "q must be (batch, seqlen, heads, dim_k)");
     TORCH_CHECK(v.dim() == 4, "v must be (batch, seqlen, v_heads, dim_v)");
     DeltaInputs d;
@@ -59,9 +75,12 @@ DeltaInputs delta_inputs(const at::Tensor &q, const at::Tensor &k, const at::Ten
     CHECK_SHAPE(k, batch, seqlen, heads, dim_k);
     CHECK_SHAPE(v, batch, seqlen, v_heads, dim_v);
     CHECK_SHAPE(g, batch, seqlen, v_heads);
-    CHECK_SHAPE(beta, batch, seqlen, v_heads);
+    if (opt_beta.has_value()) {
+        const at::Tensor &beta = *opt_beta;
+        CHECK_SHAPE(beta, batch, seqlen, v_heads);
+    }
     TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have the same dtype");
-    d.q = rows_of(q); d.k = rows_of(k); d.v = rows_of(v); d.g = g; d.beta = beta;
+    d.q = rows_of(q); d.k = rows_of(k); d.v = rows_of(v); d.g = g; d.beta = opt_beta;
     return d;
 }
 
@@ -75,14 +94,14 @@ void set_inputs(P &p, const DeltaInputs &d, double scale, bool qk_l2norm) {
     p.dim_k = size32(d.dim_k, "dim_k"); p.dim_v = size32(d.dim_v, "dim_v");
     p.x_dtype = to_cc1d_dtype(d.q.scalar_type(), "q");
     p.g_dtype = to_cc1d_dtype(d.g.scalar_type(), "g");
-    p.beta_dtype = to_cc1d_dtype(d.beta.scalar_type(), "beta");
+    p.beta_dtype = d.beta.has_value() ? to_cc1d_dtype(d.beta->scalar_type(), "beta") : p.g_dtype;
     p.qk_l2norm = qk_l2norm ? 1 : 0;
     p.scale = (float)scale;
     p.q = d.q.data_ptr(); SET_STRIDES(p, q, d.q);
     p.k = d.k.data_ptr(); SET_STRIDES(p, k, d.k);
     p.v = d.v.data_ptr(); SET_STRIDES(p, v, d.v);
     p.g = d.g.data_ptr(); SET_STRIDES(p, g, d.g);
-    p.beta = d.beta.data_ptr(); SET_STRIDES(p, beta, d.beta);
+    if (d.beta.has_value()) { p.beta = d.beta->data_ptr(); SET_STRIDES(p, beta, (*d.beta)); }
 }
 
 void check_states(const at::Tensor &s, const DeltaInputs &d, int64_t n, const char *what) {
@@ -116,7 +135,7 @@ cc1d_delta_params delta_params(const DeltaInputs &d, const OptTensor &init, cons
 }
 
 // (out, saved): saved is what the backward needs of the forward, empty if not wanted.
-std::tuple<at::Tensor, at::Tensor> delta_fwd_run(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+std::tuple<at::Tensor, at::Tensor> delta_fwd_run(const Recurrence &of, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
                      const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm, bool save) {
     const DeltaInputs d = delta_inputs(q, k, v, g, beta);
     OptTensor init = initial_states;
@@ -134,27 +153,35 @@ std::tuple<at::Tensor, at::Tensor> delta_fwd_run(const at::Tensor &q, const at::
     size_t bytes = 0;
     at::Tensor saved;
     if (save) {
-        check_status(cc1d_delta_saved_bytes(&p, &bytes), "gated_delta_rule");
+        check_status(of.saved_bytes(&p, &bytes), of.name);
         saved = empty_of({(int64_t)bytes}, at::kByte, q);
         p.saved = bytes ? saved.data_ptr() : nullptr;
     }
-    check_status(cc1d_delta_workspace_bytes(&p, &bytes), "gated_delta_rule");
+    check_status(of.workspace_bytes(&p, &bytes), of.name);
     const at::Tensor ws = workspace_of(bytes, q);
-    check_status(cc1d_delta_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "gated_delta_rule");
+    check_status(of.fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), of.name);
     return {out, saved};
 }
 at::Tensor delta_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
                      const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm) {
-    return std::get<0>(delta_fwd_run(q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, qk_l2norm, false));
+    return std::get<0>(delta_fwd_run(kDelta, q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, qk_l2norm, false));
 }
 std::tuple<at::Tensor, at::Tensor> delta_fwd_save(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
                      const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale, bool qk_l2norm) {
-    return delta_fwd_run(q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, qk_l2norm, true);
+    return delta_fwd_run(kDelta, q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, qk_l2norm, true);
+}
+at::Tensor linear_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
+                      const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale) {
+    return std::get<0>(delta_fwd_run(kLinear, q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, false, false));
+}
+std::tuple<at::Tensor, at::Tensor> linear_fwd_save(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
+                      const OptTensor &initial_states, const OptTensor &cu_seqlens, const OptTensor &final_states_out, double scale) {
+    return delta_fwd_run(kLinear, q, k, v, g, beta, initial_states, cu_seqlens, final_states_out, scale, false, true);
 }
 
-// dq, dk, dv, dg, dbeta in their inputs' types, and dinitial_states (empty if not wanted).
+// dq, dk, dv, dg, dbeta in their inputs' types (dbeta empty without beta), and dinitial_states (empty if not wanted).
 using Gradients6 = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
-Gradients6 delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+Gradients6 delta_bwd_run(const Recurrence &of, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
                      const OptTensor &initial_states, const OptTensor &cu_seqlens, const at::Tensor &saved, const at::Tensor &dout_,
                      const OptTensor &dfinal_states, double scale, bool qk_l2norm, bool want_dinitial) {
     const DeltaInputs d = delta_inputs(q, k, v, g, beta);
@@ -164,7 +191,7 @@ Gradients6 delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor 
     cc1d_delta_bwd_params p = {};
     p.fwd = delta_params(d, init, cu_seqlens, scale, qk_l2norm);
     size_t bytes = 0;
-    check_status(cc1d_delta_saved_bytes(&p.fwd, &bytes), "gated_delta_rule backward");
+    check_status(of.saved_bytes(&p.fwd, &bytes), of.name_bwd);
     check_gpu(saved, q, "saved");
     TORCH_CHECK(saved.is_contiguous() && saved.nbytes() >= bytes, "saved is not what the forward returned for these sizes");
     p.fwd.saved = bytes ? saved.data_ptr() : nullptr;
@@ -178,24 +205,34 @@ Gradients6 delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor 
         p.dfinal_states = dfinal->data_ptr<float>(); SET_STATE(p, dfinal, (*dfinal));
     }
     at::Tensor dq = empty_of(q.sizes(), q.scalar_type(), q), dk = empty_of(k.sizes(), k.scalar_type(), k), dv = empty_of(v.sizes(), v.scalar_type(), v);
-    at::Tensor dg = empty_of(g.sizes(), g.scalar_type(), g), dbeta = empty_of(beta.sizes(), beta.scalar_type(), beta);
+    at::Tensor dg = empty_of(g.sizes(), g.scalar_type(), g), dbeta = beta.has_value() ? empty_of(beta->sizes(), beta->scalar_type(), q) : empty_of({0}, at::kFloat, q);
     p.dq = dq.data_ptr(); SET_STRIDES(p, dq, dq);
     p.dk = dk.data_ptr(); SET_STRIDES(p, dk, dk);
     p.dv = dv.data_ptr(); SET_STRIDES(p, dv, dv);
-    p.dg = dg.data_ptr(); p.dbeta = dbeta.data_ptr();
+    p.dg = dg.data_ptr(); p.dbeta = beta.has_value() ? dbeta.data_ptr() : nullptr;
     at::Tensor dinit = want_dinitial ? empty_of({p.fwd.sequences, d.v_heads, d.dim_k, d.dim_v}, at::kFloat, q) : empty_of({0}, at::kFloat, q);
     if (want_dinitial) { p.dinitial_states = dinit.data_ptr<float>(); SET_STATE(p, dinit, dinit); }
-    check_status(cc1d_delta_bwd_workspace_bytes(&p, &bytes), "gated_delta_rule backward");
+    check_status(of.bwd_workspace_bytes(&p, &bytes), of.name_bwd);
     const at::Tensor ws = workspace_of(bytes, q);
-    check_status(cc1d_delta_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "gated_delta_rule backward");
+    check_status(of.bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), of.name_bwd);
     return {dq, dk, dv, dg, dbeta, dinit};
 }
+Gradients6 delta_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                     const OptTensor &initial_states, const OptTensor &cu_seqlens, const at::Tensor &saved, const at::Tensor &dout,
+                     const OptTensor &dfinal_states, double scale, bool qk_l2norm, bool want_dinitial) {
+    return delta_bwd_run(kDelta, q, k, v, g, beta, initial_states, cu_seqlens, saved, dout, dfinal_states, scale, qk_l2norm, want_dinitial);
+}
+Gradients6 linear_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
+                      const OptTensor &initial_states, const OptTensor &cu_seqlens, const at::Tensor &saved, const at::Tensor &dout,
+                      const OptTensor &dfinal_states, double scale, bool want_dinitial) {
+    return delta_bwd_run(kLinear, q, k, v, g, beta, initial_states, cu_seqlens, saved, dout, dfinal_states, scale, false, want_dinitial);
+}
 
-at::Tensor delta_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+at::Tensor delta_update_run(const Recurrence &of, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
                         at::Tensor &state, const OptTensor &state_indices, double scale, bool qk_l2norm) {
     const bool flat = q.dim() == 3;                      // (batch, heads, dim): one token, no seqlen axis
     auto with_tokens = [&](const at::Tensor &t) { return flat ? t.unsqueeze(1) : t; };
-    const DeltaInputs d = delta_inputs(with_tokens(q), with_tokens(k), with_tokens(v), with_tokens(g), with_tokens(beta));
+    const DeltaInputs d = delta_inputs(with_tokens(q), with_tokens(k), with_tokens(v), with_tokens(g), beta.has_value() ? OptTensor(with_tokens(*beta)) : std::nullopt);
     cc1d_delta_step_params p = {};
     set_inputs(p, d, scale, qk_l2norm);
     check_gpu(state, q, "state");
@@ -214,8 +251,16 @@ at::Tensor delta_update(const at::Tensor &q, const at::Tensor &k, const at::Tens
     c10::DeviceGuard guard(q.device());
     at::Tensor out = empty_of({d.batch, d.seqlen, d.v_heads, d.dim_v}, d.v.scalar_type(), d.v);
     p.out = out.data_ptr(); SET_STRIDES(p, out, out);
-    check_status(cc1d_delta_step(&p, current_stream()), "gated_delta_rule_update");
+    check_status(of.step(&p, current_stream()), of.name_update);
     return flat ? out.squeeze(1) : out;
+}
+at::Tensor delta_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                        at::Tensor &state, const OptTensor &state_indices, double scale, bool qk_l2norm) {
+    return delta_update_run(kDelta, q, k, v, g, beta, state, state_indices, scale, qk_l2norm);
+}
+at::Tensor linear_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, at::Tensor &state,
+                         const OptTensor &beta, const OptTensor &state_indices, double scale) {
+    return delta_update_run(kLinear, q, k, v, g, beta, state, state_indices, scale, false);
 }
 
 at::Tensor delta_fwd_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const at::Tensor &,
@@ -241,6 +286,25 @@ Gradients6 delta_bwd_meta(const at::Tensor &q, const at::Tensor &k, const at::Te
 }
 at::Tensor delta_update_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const at::Tensor &,
                              at::Tensor &, const OptTensor &, double, bool) {
+    return at::empty_symint(v.sym_sizes(), v.options());
+}
+at::Tensor linear_fwd_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const OptTensor &,
+                           const OptTensor &, const OptTensor &, const OptTensor &, double) {
+    return at::empty_symint(v.sym_sizes(), v.options());
+}
+// Three terms of 16 bits of every state in front of a segment of 256 tokens, in tiles of 32 x 32: the library's sum.
+std::tuple<at::Tensor, at::Tensor> linear_fwd_save_meta(const at::Tensor &q, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const OptTensor &,
+                           const OptTensor &, const OptTensor &cu, const OptTensor &, double) {
+    const c10::SymInt slots = cu.has_value() ? q.sym_size(1) / 256 + cu->sym_size(0) : q.sym_size(0) * ((q.sym_size(1) + 255) / 256);
+    const c10::SymInt bytes = slots * v.sym_size(2) * ((q.sym_size(3) + 31) / 32) * ((v.sym_size(3) + 31) / 32) * 6144;
+    return {at::empty_symint(v.sym_sizes(), v.options()), at::empty_symint({bytes}, q.options().dtype(at::kByte))};
+}
+Gradients6 linear_bwd_meta(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
+                           const OptTensor &init, const OptTensor &cu, const at::Tensor &saved, const at::Tensor &dout, const OptTensor &dfinal, double scale, bool want_dinitial) {
+    return delta_bwd_meta(q, k, v, g, beta.has_value() ? *beta : at::empty({0}, q.options().dtype(at::kFloat)), init, cu, saved, dout, dfinal, scale, false, want_dinitial);
+}
+at::Tensor linear_update_meta(const at::Tensor &, const at::Tensor &, const at::Tensor &v, const at::Tensor &, at::Tensor &,
+                              const OptTensor &, const OptTensor &, double) {
     return at::empty_symint(v.sym_sizes(), v.options());
 }
 
@@ -350,6 +414,100 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &h, con
     return {dx, dres, dw};
 }
 
+// ---- layer norm ----------------------------------------------------------------------
+
+const OptTensor &checked_bias(const OptTensor &bias, const at::Tensor &weight, int64_t dim) {
+    if (bias.has_value()) {
+        check_gpu(*bias, weight, "bias");
+        TORCH_CHECK(bias->sizes() == at::IntArrayRef({dim}), "bias must have shape (dim)");
+        TORCH_CHECK(bias->scalar_type() == weight.scalar_type(), "bias must have the dtype of weight");
+    }
+    return bias;
+}
+
+// y, h where there is a residual (else empty), and with `save` each row's mean and 1 / standard deviation (else empty).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias_, const OptTensor &residual, double eps, bool save) {
+    const NormInputs n = norm_inputs(x, weight, residual);
+    c10::DeviceGuard guard(x.device());
+    const OptTensor bias = checked_bias(bias_, weight, n.x.size(1));
+    cc1d_layer_norm_params p = {};
+    p.rows = n.x.size(0); p.dim = size32(n.x.size(1), "dim"); p.eps = (float)eps;
+    p.x_dtype = p.r_dtype = to_cc1d_dtype(x.scalar_type(), "x");
+    p.w_dtype = to_cc1d_dtype(weight.scalar_type(), "weight");
+    p.x = n.x.data_ptr(); p.x_stride = n.x.stride(0);
+    p.weight = n.weight.data_ptr();
+    at::Tensor b, h, stats = empty_of({save ? p.rows : 0, 2}, at::kFloat, x);
+    if (bias.has_value()) { b = bias->contiguous(); p.bias = b.data_ptr(); }
+    if (residual.has_value()) {
+        p.r_dtype = to_cc1d_dtype(residual->scalar_type(), "residual");
+        p.residual = n.residual.data_ptr(); p.residual_stride = n.residual.stride(0);
+        h = empty_of(x.sizes(), residual->scalar_type(), x);
+        p.h = h.data_ptr(); p.h_stride = p.dim;
+    } else {
+        h = empty_of({0}, x.scalar_type(), x);
+    }
+    if (save && p.rows > 0) p.stats = stats.data_ptr<float>();
+    at::Tensor y = empty_of(x.sizes(), x.scalar_type(), x);
+    p.y = y.data_ptr(); p.y_stride = p.dim;
+    check_status(cc1d_layer_norm_fwd(&p, current_stream()), "layer_norm");
+    return {y, h, stats};
+}
+
+// h: what was normalised.  dx in the dtype of dy, dresidual in that of h; where the two are the same type they are one tensor, and
+// dresidual comes back empty.  dbias in the dtype of weight, empty if not wanted.
+using Gradients4 = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+Gradients4 layer_norm_bwd(const at::Tensor &h, const at::Tensor &stats, const at::Tensor &weight, const at::Tensor &dy, const OptTensor &dh, bool want_dbias) {
+    check_gpu(h, h, "h"); check_gpu(stats, h, "stats"); check_gpu(weight, h, "weight"); check_gpu(dy, h, "dy");
+    TORCH_CHECK(dy.sizes() == h.sizes(), "dy must have the shape of h");
+    const at::Tensor hr = as_rows(h), dyr = as_rows(dy), w = weight.contiguous();
+    const int64_t dim = hr.size(1);
+    CHECK_SHAPE(weight, dim);
+    TORCH_CHECK(stats.is_contiguous() && stats.scalar_type() == at::kFloat && stats.numel() == 2 * hr.size(0), "stats is not what the forward returned for these sizes");
+    c10::DeviceGuard guard(h.device());
+    cc1d_layer_norm_bwd_params p = {};
+    p.rows = hr.size(0); p.dim = size32(dim, "dim");
+    p.x_dtype = to_cc1d_dtype(dy.scalar_type(), "dy");
+    p.r_dtype = to_cc1d_dtype(h.scalar_type(), "h");
+    p.w_dtype = to_cc1d_dtype(weight.scalar_type(), "weight");
+    p.h = hr.data_ptr(); p.h_stride = hr.stride(0);
+    p.stats = stats.data_ptr<float>();
+    p.weight = w.data_ptr();
+    p.dy = dyr.data_ptr(); p.dy_stride = dyr.stride(0);
+    at::Tensor dhr;
+    if (dh.has_value()) {
+        check_gpu(*dh, h, "dh");
+        TORCH_CHECK(dh->sizes() == h.sizes() && dh->scalar_type() == h.scalar_type(), "dh must have the shape and dtype of h");
+        dhr = as_rows(*dh);
+        p.dh = dhr.data_ptr(); p.dh_stride = dhr.stride(0);
+    }
+    at::Tensor dx = empty_of(h.sizes(), dy.scalar_type(), h);
+    p.dx = dx.data_ptr(); p.dx_stride = dim;
+    const bool both = dy.scalar_type() != h.scalar_type();
+    at::Tensor dres = both ? empty_of(h.sizes(), h.scalar_type(), h) : empty_of({0}, h.scalar_type(), h);
+    if (both) { p.dresidual = dres.data_ptr(); p.dresidual_stride = dim; }
+    at::Tensor dw = empty_of({dim}, weight.scalar_type(), h), db = empty_of({want_dbias ? dim : 0}, weight.scalar_type(), h);
+    p.dweight = dw.data_ptr();
+    if (want_dbias) p.dbias = db.data_ptr();
+    size_t bytes = 0;
+    check_status(cc1d_layer_norm_bwd_workspace_bytes(&p, &bytes), "layer_norm backward");
+    const at::Tensor ws = workspace_of(bytes, h);
+    check_status(cc1d_layer_norm_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), "layer_norm backward");
+    return {dx, dres, dw, db};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd_meta(const at::Tensor &x, const at::Tensor &, const OptTensor &, const OptTensor &residual, double, bool save) {
+    c10::SymInt rows = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.sym_size(i);
+    return {at::empty_symint(x.sym_sizes(), x.options()), residual.has_value() ? at::empty_symint(x.sym_sizes(), residual->options()) : at::empty({0}, x.options()),
+            at::empty_symint({save ? rows : c10::SymInt(0), 2}, x.options().dtype(at::kFloat))};
+}
+Gradients4 layer_norm_bwd_meta(const at::Tensor &h, const at::Tensor &, const at::Tensor &weight, const at::Tensor &dy, const OptTensor &, bool want_dbias) {
+    return {at::empty_symint(h.sym_sizes(), dy.options()), dy.scalar_type() != h.scalar_type() ? at::empty_symint(h.sym_sizes(), h.options()) : at::empty({0}, h.options()),
+            at::empty_symint(weight.sym_sizes(), weight.options()), want_dbias ? at::empty_symint(weight.sym_sizes(), weight.options()) : at::empty({0}, weight.options())};
+}
+
+// ---- rows of 8 bits --------------------------------------------------------------------
+
 at::Tensor dequantize(const at::Tensor &y8, const at::Tensor &scales, at::ScalarType dtype) {
     check_gpu(y8, y8, "y8"); check_gpu(scales, y8, "scales");
     TORCH_CHECK(y8.scalar_type() == at::kFloat8_e4m3fn, "y8 must be float8_e4m3fn");
@@ -458,6 +616,74 @@ struct GatedDeltaRuleNode : public torch::autograd::Function<GatedDeltaRuleNode>
     }
 };
 
+// As GatedDeltaRuleNode; beta may be missing.
+struct LinearAttentionNode : public torch::autograd::Function<LinearAttentionNode> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,
+                                 const OptTensor &init, const OptTensor &cu, const OptTensor &final, double scale) {
+        static const auto op = typed_op<decltype(linear_fwd_save)>("DaoAILab::_linear_attention_fwd_save_cpp");
+        std::tuple<at::Tensor, at::Tensor> r;
+        {
+            pybind11::gil_scoped_release no_gil;
+            r = op.call(q, k, v, g, beta, init, cu, final, scale);
+        }
+        ctx->save_for_backward({q, k, v, g, or_undefined(beta), or_undefined(init), or_undefined(cu), std::get<1>(r)});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["dinit"] = init.has_value() && init->requires_grad();
+        ctx->set_materialize_grads(false);
+        return final.has_value() ? variable_list{std::get<0>(r), *final} : variable_list{std::get<0>(r)};
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        static const auto op = typed_op<decltype(linear_bwd)>("DaoAILab::_linear_attention_bwd_cpp");
+        const OptTensor dfinal = grads.size() > 1 ? if_defined(grads[1]) : std::nullopt;
+        at::Tensor dout = grads[0];
+        if (!dout.defined() && !dfinal.has_value()) return variable_list(9);
+        const variable_list s = ctx->get_saved_variables();
+        if (!dout.defined()) dout = at::zeros(s[2].sizes(), s[2].options());
+        const bool dinit = ctx->saved_data["dinit"].toBool();
+        auto r = op.call(s[0], s[1], s[2], s[3], if_defined(s[4]), if_defined(s[5]), if_defined(s[6]), s[7], dout, dfinal, ctx->saved_data["scale"].toDouble(), dinit);
+        variable_list all = {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r)};
+        all.resize(9);
+        if (s[4].defined()) all[4] = std::get<4>(r);
+        if (dinit) all[5] = std::get<5>(r);
+        return all;
+    }
+};
+
+// (y, h) or (y): saves what was normalised, its rows' statistics and the weight.
+struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias, const OptTensor &residual, double eps) {
+        static const auto op = typed_op<decltype(layer_norm_fwd)>("DaoAILab::_layer_norm_fwd_cpp");
+        std::tuple<at::Tensor, at::Tensor, at::Tensor> r;
+        {
+            pybind11::gil_scoped_release no_gil;
+            r = op.call(x, weight, bias, residual, eps, true);
+        }
+        ctx->save_for_backward({residual.has_value() ? std::get<1>(r) : x, std::get<2>(r), weight});
+        ctx->saved_data["dtype"] = x.scalar_type();
+        ctx->saved_data["residual"] = residual.has_value() && residual->requires_grad();
+        ctx->saved_data["bias"] = bias.has_value() && bias->requires_grad();
+        ctx->set_materialize_grads(false);
+        return residual.has_value() ? variable_list{std::get<0>(r), std::get<1>(r)} : variable_list{std::get<0>(r)};
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        static const auto op = typed_op<decltype(layer_norm_bwd)>("DaoAILab::_layer_norm_bwd_cpp");
+        const OptTensor dh = grads.size() > 1 ? if_defined(grads[1]) : std::nullopt;
+        at::Tensor dy = grads[0];
+        variable_list all(5);
+        if (!dy.defined() && !dh.has_value()) return all;
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &h = saved[0];
+        if (!dy.defined()) dy = at::zeros(h.sizes(), h.options().dtype(ctx->saved_data["dtype"].toScalarType()));
+        const bool bias = ctx->saved_data["bias"].toBool();
+        auto r = op.call(h, saved[1], saved[2], dy, dh, bias);
+        all[0] = std::get<0>(r);
+        all[1] = std::get<2>(r);
+        if (bias) all[2] = std::get<3>(r);
+        if (ctx->saved_data["residual"].toBool()) all[3] = all[0].scalar_type() == h.scalar_type() ? all[0] : std::get<1>(r);
+        return all;
+    }
+};
+
 bool wants_grad(std::initializer_list<const at::Tensor *> all) {
     if (!at::GradMode::is_enabled()) return false;
     for (const at::Tensor *t : all)
@@ -498,6 +724,28 @@ PyObject *norm_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
     } else {
         pybind11::gil_scoped_release no_gil;
         auto t = op.call(x, weight, residual, eps);
+        all = residual.has_value() ? variable_list{std::get<0>(t), std::get<1>(t)} : variable_list{std::get<0>(t)};
+    }
+    return residual.has_value() ? tuple_of(std::move(all)) : THPVariable_Wrap(std::move(all[0]));
+    END_HANDLE_TH_ERRORS
+}
+
+// (x, weight, bias, residual, eps) -> y or (y, h)
+PyObject *layer_norm_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5 || !plain_all(a, 2) || !plain_or_none(a[2]) || !plain_or_none(a[3]) || !PyFloat_Check(a[4]) || generic_path_needed()) NOT_IMPLEMENTED();
+    static const auto op = typed_op<decltype(layer_norm_fwd)>("DaoAILab::_layer_norm_fwd_cpp");
+    const at::Tensor x = THPVariable_Unpack(a[0]), weight = THPVariable_Unpack(a[1]);
+    const OptTensor bias = optional_tensor(a[2]), residual = optional_tensor(a[3]);
+    const double eps = PyFloat_AS_DOUBLE(a[4]);
+    const at::Tensor b = or_undefined(bias), r = or_undefined(residual);
+    variable_list all;
+    if (wants_grad({&x, &weight, &b, &r})) {
+        if (python_graph_needed({&x, &weight, &b, &r})) NOT_IMPLEMENTED();
+        all = LayerNormNode::apply(x, weight, bias, residual, eps);
+    } else {
+        pybind11::gil_scoped_release no_gil;
+        auto t = op.call(x, weight, bias, residual, eps, false);
         all = residual.has_value() ? variable_list{std::get<0>(t), std::get<1>(t)} : variable_list{std::get<0>(t)};
     }
     return residual.has_value() ? tuple_of(std::move(all)) : THPVariable_Wrap(std::move(all[0]));
@@ -596,6 +844,67 @@ PyObject *delta_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// (q, k, v, g, state, beta, state_indices, scale or None) -> out
+PyObject *linear_update_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 8 || !plain_all(a, 5) || !plain_or_none(a[5]) || !plain_or_none(a[6]) || !(a[7] == Py_None || PyFloat_Check(a[7])) || generic_path_needed()) NOT_IMPLEMENTED();
+    static const auto op = typed_op<decltype(linear_update)>("DaoAILab::_linear_attention_update_cpp");
+    const at::Tensor q = THPVariable_Unpack(a[0]), k = THPVariable_Unpack(a[1]), v = THPVariable_Unpack(a[2]);
+    at::Tensor g = THPVariable_Unpack(a[3]), state = THPVariable_Unpack(a[4]);
+    const OptTensor beta = optional_tensor(a[5]), indices = optional_tensor(a[6]);
+    if (q.dim() < 1 || (g.dim() == 1 && v.dim() < 3)) NOT_IMPLEMENTED();
+    const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)q.size(-1)) : PyFloat_AS_DOUBLE(a[7]);
+    at::Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (g.dim() == 1) g = g.expand(v.sizes().slice(0, v.dim() - 1));
+        out = op.call(q, k, v, g, state, beta, indices, scale);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, k, v, g, beta, scale or None, initial_states, return_final_states, final_states_out, cu_seqlens) -> out or (out, final_states)
+PyObject *linear_call(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10 || !plain_all(a, 4) || !plain_or_none(a[4]) || !(a[5] == Py_None || PyFloat_Check(a[5])) || !plain_or_none(a[6]) || !PyBool_Check(a[7]) ||
+        !plain_or_none(a[8]) || !plain_or_none(a[9]) || generic_path_needed())
+        NOT_IMPLEMENTED();
+    static const auto op = typed_op<decltype(linear_fwd)>("DaoAILab::_linear_attention_fwd_cpp");
+    const at::Tensor q = THPVariable_Unpack(a[0]), k = THPVariable_Unpack(a[1]), v = THPVariable_Unpack(a[2]);
+    at::Tensor g = THPVariable_Unpack(a[3]);
+    const OptTensor beta = optional_tensor(a[4]), init = optional_tensor(a[6]), cu = optional_tensor(a[9]);
+    const bool return_final = a[7] == Py_True;
+    OptTensor fin = return_final ? optional_tensor(a[8]) : std::nullopt;
+    if (q.dim() != 4 || v.dim() != 4 || (cu.has_value() && (cu->dim() != 1 || cu->size(0) < 1 || !cu->is_contiguous()))) NOT_IMPLEMENTED();
+    const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)q.size(-1)) : PyFloat_AS_DOUBLE(a[5]);
+    const at::Tensor b = or_undefined(beta), i = or_undefined(init);
+    const bool graph = wants_grad({&q, &k, &v, &g, &b, &i});
+    if (graph && (fin.has_value() || python_graph_needed({&q, &k, &v, &g, &b, &i}))) NOT_IMPLEMENTED();
+    if (g.dim() == 1) g = g.expand(v.sizes().slice(0, 3));
+    if (return_final && !fin.has_value())
+        fin = at::empty({cu.has_value() ? cu->size(0) - 1 : q.size(0), v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat));
+    variable_list all;
+    if (graph) {
+        all = LinearAttentionNode::apply(q, k, v, g, beta, init, cu, fin, scale);
+    } else {
+        pybind11::gil_scoped_release no_gil;
+        all.push_back(op.call(q, k, v, g, beta, init, cu, fin, scale));
+    }
+    if (!return_final) return THPVariable_Wrap(std::move(all[0]));
+    if (a[8] != Py_None) {                               // the caller's own object
+        PyObject *pair = PyTuple_New(2);
+        if (pair == nullptr) throw python_error();
+        PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(all[0])));
+        Py_INCREF(a[8]);
+        PyTuple_SET_ITEM(pair, 1, a[8]);
+        return pair;
+    }
+    if (!graph) all.push_back(*fin);
+    return tuple_of(std::move(all));
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- what autograd is told of an op ----------------------------------------------------
 // The graphs above (and those of the Python functions) are recorded around the ops, with gradients off inside.  An op that is called on
 // tensors that require a gradient all the same (the backward under create_graph, or the op itself) has no derivative: its results
@@ -663,6 +972,12 @@ OP_NAME(kNormFwd, "_rms_norm_fwd_cpp");
 OP_NAME(kNormBwd, "_rms_norm_bwd_cpp");
 OP_NAME(kNormQuant, "_rms_norm_quant_cpp");
 OP_NAME(kDequantize, "_dequantize_rows_cpp");
+OP_NAME(kLinearFwd, "_linear_attention_fwd_cpp");
+OP_NAME(kLinearFwdSave, "_linear_attention_fwd_save_cpp");
+OP_NAME(kLinearBwd, "_linear_attention_bwd_cpp");
+OP_NAME(kLinearUpdate, "_linear_attention_update_cpp");
+OP_NAME(kLayerNormFwd, "_layer_norm_fwd_cpp");
+OP_NAME(kLayerNormBwd, "_layer_norm_bwd_cpp");
 
 #define DIRECT_CALL(NAME, F) {NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&F)), METH_FASTCALL, nullptr}
 PyMethodDef calls[] = {DIRECT_CALL("_rms_norm_call", norm_call),
@@ -670,6 +985,9 @@ PyMethodDef calls[] = {DIRECT_CALL("_rms_norm_call", norm_call),
                        DIRECT_CALL("_dequantize_rows_call", dequantize_call),
                        DIRECT_CALL("_gated_delta_rule_call", delta_call),
                        DIRECT_CALL("_gated_delta_rule_update_call", delta_update_call),
+                       DIRECT_CALL("_linear_attention_call", linear_call),
+                       DIRECT_CALL("_linear_attention_update_call", linear_update_call),
+                       DIRECT_CALL("_layer_norm_call", layer_norm_call),
                        {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
@@ -690,6 +1008,17 @@ TORCH_LIBRARY_FRAGMENT(DaoAILab, m) {
     m.def("_rms_norm_bwd_cpp(Tensor h, Tensor weight, Tensor dy, Tensor? dh, float eps) -> (Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
     m.def("_rms_norm_quant_cpp(Tensor x, Tensor weight, Tensor? residual, float eps) -> (Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
     m.def("_dequantize_rows_cpp(Tensor y8, Tensor scales, ScalarType dtype) -> Tensor", {at::Tag::pt2_compliant_tag});
+    m.def("_linear_attention_fwd_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor? beta, Tensor? initial_states, "
+          "Tensor? cu_seqlens, Tensor(a!)? final_states_out, float scale) -> Tensor", {at::Tag::pt2_compliant_tag});
+    m.def("_linear_attention_fwd_save_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor? beta, Tensor? initial_states, "
+          "Tensor? cu_seqlens, Tensor(a!)? final_states_out, float scale) -> (Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+    m.def("_linear_attention_bwd_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor? beta, Tensor? initial_states, Tensor? cu_seqlens, "
+          "Tensor saved, Tensor dout, Tensor? dfinal_states, float scale, bool want_dinitial) "
+          "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+    m.def("_linear_attention_update_cpp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor(a!) state, Tensor? beta, "
+          "Tensor? state_indices, float scale) -> Tensor", {at::Tag::pt2_compliant_tag});
+    m.def("_layer_norm_fwd_cpp(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, float eps, bool save) -> (Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+    m.def("_layer_norm_bwd_cpp(Tensor h, Tensor stats, Tensor weight, Tensor dy, Tensor? dh, bool want_dbias) -> (Tensor, Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
 }
 
 TORCH_LIBRARY_IMPL(DaoAILab, CompositeExplicitAutograd, m) {
@@ -701,6 +1030,12 @@ TORCH_LIBRARY_IMPL(DaoAILab, CompositeExplicitAutograd, m) {
     m.impl("_rms_norm_bwd_cpp", &norm_bwd);
     m.impl("_rms_norm_quant_cpp", &norm_quant);
     m.impl("_dequantize_rows_cpp", &dequantize);
+    m.impl("_linear_attention_fwd_cpp", &linear_fwd);
+    m.impl("_linear_attention_fwd_save_cpp", &linear_fwd_save);
+    m.impl("_linear_attention_bwd_cpp", &linear_bwd);
+    m.impl("_linear_attention_update_cpp", &linear_update);
+    m.impl("_layer_norm_fwd_cpp", &layer_norm_fwd);
+    m.impl("_layer_norm_bwd_cpp", &layer_norm_bwd);
 }
 
 TORCH_LIBRARY_IMPL(DaoAILab, Meta, m) {
@@ -712,6 +1047,12 @@ TORCH_LIBRARY_IMPL(DaoAILab, Meta, m) {
     m.impl("_rms_norm_bwd_cpp", &norm_bwd_meta);
     m.impl("_rms_norm_quant_cpp", &norm_quant_meta);
     m.impl("_dequantize_rows_cpp", &dequantize_meta);
+    m.impl("_linear_attention_fwd_cpp", &linear_fwd_meta);
+    m.impl("_linear_attention_fwd_save_cpp", &linear_fwd_save_meta);
+    m.impl("_linear_attention_bwd_cpp", &linear_bwd_meta);
+    m.impl("_linear_attention_update_cpp", &linear_update_meta);
+    m.impl("_layer_norm_fwd_cpp", &layer_norm_fwd_meta);
+    m.impl("_layer_norm_bwd_cpp", &layer_norm_bwd_meta);
 }
 
 TORCH_LIBRARY_IMPL(DaoAILab, Autograd, m) {
@@ -723,4 +1064,10 @@ TORCH_LIBRARY_IMPL(DaoAILab, Autograd, m) {
     m.impl("_rms_norm_bwd_cpp", &Graphless<kNormBwd, true, -1, decltype(norm_bwd)>::call);
     m.impl("_rms_norm_quant_cpp", &Graphless<kNormQuant, false, -1, decltype(norm_quant)>::call);
     m.impl("_dequantize_rows_cpp", &Graphless<kDequantize, false, -1, decltype(dequantize)>::call);
+    m.impl("_linear_attention_fwd_cpp", &Graphless<kLinearFwd, true, 7, decltype(linear_fwd)>::call);
+    m.impl("_linear_attention_fwd_save_cpp", &Graphless<kLinearFwdSave, true, 7, decltype(linear_fwd_save)>::call);
+    m.impl("_linear_attention_bwd_cpp", &Graphless<kLinearBwd, true, -1, decltype(linear_bwd)>::call);
+    m.impl("_linear_attention_update_cpp", &Graphless<kLinearUpdate, false, 4, decltype(linear_update)>::call);
+    m.impl("_layer_norm_fwd_cpp", &Graphless<kLayerNormFwd, true, -1, decltype(layer_norm_fwd)>::call);
+    m.impl("_layer_norm_bwd_cpp", &Graphless<kLayerNormBwd, true, -1, decltype(layer_norm_bwd)>::call);
 }

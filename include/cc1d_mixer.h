@@ -130,6 +130,35 @@ int cc1d_validate_delta_step(const cc1d_delta_step_params *p);
 int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head, per sequence and value head, state S (dim_k, dim_v) in fp32:
+ *
+ *   S   = exp(g[t]) S + beta[t] k[t] v[t]^T
+ *   out[t] = scale S^T q[t]
+ *
+ * The blocks are the gated delta rule's, with what stands there about heads, strides, sequences and tokens of none.  beta may be NULL: 1
+ * (dbeta is then not written, beta_dtype not read).  Strides of 0 make a gate one number a head.  qk_l2norm has to be 0 (CC1D_ERR_OPTION).
+ * `saved` is of cc1d_linear_saved_bytes() here: the state in front of every 256 tokens.
+ *
+ * Short sequences go token by token, the others in segments of 256 tokens, each worked out in blocks of 64: a NaN or infinity reaches its
+ * head's outputs from the start of its 64 tokens on.  Gates are bounded from below by -200, which forgets everything.  Where they
+ * are positive, the states may grow by less than 2^128 over 256 tokens.
+ * Precision is the gated delta rule's; the factors that make out and dv of 16 bits carry 2^-17.
+ * Tokens 2^23 bytes apart or more (in q, k, v) go by tokens in the forward; there, with `saved`, and in the backward (dout too) they are refused
+ * with CC1D_ERR_TOO_LARGE.
+ * ---------------------------------------------------------------------------------- */
+int cc1d_validate_linear(const cc1d_delta_params *p);
+int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes);
+int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes);
+int cc1d_linear_fwd(const cc1d_delta_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream);
+
+int cc1d_validate_linear_bwd(const cc1d_delta_bwd_params *p);
+int cc1d_linear_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *bytes);
+int cc1d_linear_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream);
+
+int cc1d_validate_linear_step(const cc1d_delta_step_params *p);
+int cc1d_linear_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Root-mean-square norm over rows of `dim` elements, with the residual's addition:
  *
  *   h = x + residual      (summed in fp32, rounded once to r_dtype; without residual h = x)
@@ -188,6 +217,61 @@ typedef struct cc1d_norm_bwd_params {
 int cc1d_validate_norm_bwd(const cc1d_norm_bwd_params *p);
 int cc1d_norm_bwd_workspace_bytes(const cc1d_norm_bwd_params *p, size_t *bytes);
 int cc1d_norm_bwd(const cc1d_norm_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Layer norm over rows of `dim` elements, with the residual's addition:
+ *
+ *   h = x + residual      (summed in fp32, rounded once to r_dtype; without residual h = x)
+ *   n = (h - mean(h)) r,  r = rsqrt(mean((h - mean(h))^2) + eps),  y = n weight + bias
+ * ---------------------------------------------------------------------------------- */
+typedef struct cc1d_layer_norm_params {
+    int64_t rows;
+    int32_t dim;                     /* up to 2^31 - 8193; backward: 2^26 - 16 */
+    int32_t x_dtype, r_dtype, w_dtype; /* of x and y; of residual and h; of weight and bias */
+    float eps;
+    int32_t reserved0;
+    const void *x;                   /* (rows, dim), unit stride along dim */
+    int64_t x_stride;
+    const void *residual;            /* (rows, dim), or NULL */
+    int64_t residual_stride;
+    const void *weight;              /* (dim,) contiguous */
+    const void *bias;                /* (dim,) contiguous, or NULL */
+    void *h;                         /* (rows, dim); needed with residual, else NULL.  May be residual itself */
+    int64_t h_stride;
+    void *y;                         /* (rows, dim) of x_dtype */
+    int64_t y_stride;
+    float *stats;                    /* NULL, or (rows, 2), 8-byte aligned: each row's mean and r, for the backward */
+} cc1d_layer_norm_params;
+
+int cc1d_validate_layer_norm(const cc1d_layer_norm_params *p);
+int cc1d_layer_norm_fwd(const cc1d_layer_norm_params *p, cc1d_stream_t stream);
+
+/* Backward of y (and h): dx = dh + r (w dy - mean(w dy) - n mean(w dy n)), in x_dtype and / or r_dtype; dweight = sum over rows of
+ * dy n, dbias = sum over rows of dy, each rounded once to w_dtype.  Partial sums go to the workspace and are added in a fixed order. */
+typedef struct cc1d_layer_norm_bwd_params {
+    int64_t rows;
+    int32_t dim;
+    int32_t x_dtype, r_dtype, w_dtype;
+    int32_t reserved0, reserved1;
+    const void *h;                   /* (rows, dim) of r_dtype */
+    int64_t h_stride;
+    const float *stats;              /* (rows, 2), of the forward */
+    const void *weight;
+    const void *dy;                  /* (rows, dim) of x_dtype */
+    int64_t dy_stride;
+    const void *dh;                  /* (rows, dim) of r_dtype, or NULL */
+    int64_t dh_stride;
+    void *dx;                        /* (rows, dim) of x_dtype, or NULL */
+    int64_t dx_stride;
+    void *dresidual;                 /* (rows, dim) of r_dtype, or NULL */
+    int64_t dresidual_stride;
+    void *dweight;                   /* (dim,) of w_dtype */
+    void *dbias;                     /* (dim,) of w_dtype, or NULL */
+} cc1d_layer_norm_bwd_params;
+
+int cc1d_validate_layer_norm_bwd(const cc1d_layer_norm_bwd_params *p);
+int cc1d_layer_norm_bwd_workspace_bytes(const cc1d_layer_norm_bwd_params *p, size_t *bytes);
+int cc1d_layer_norm_bwd(const cc1d_layer_norm_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream);
 
 /* Rows of e4m3 values times their scales, as y_dtype. */
 typedef struct cc1d_dequantize_params {
