@@ -50,7 +50,7 @@ KERNEL_SOURCES = [
 KERNEL_HEADERS = ["cc1d_device.hpp", "cc1d_internal.hpp", "cc1d_bwd_channellast_kernel.hpp"]
 DELTA_HEADERS = ["cc1d_delta.hpp", "cc1d_delta_chunk.hpp", "cc1d_delta_host.hpp"]   # of the sources that begin with cc1d_delta or cc1d_linear
 NORM_SOURCES, NORM_HEADERS = ("cc1d_norm.hip", "cc1d_layer_norm.hip"), ["cc1d_rows.hpp"]
-LINEAR_HEADERS = ["cc1d_linear.hpp", "cc1d_linear_device.hpp", "cc1d_linear_attend.hpp"]
+LINEAR_HEADERS = ["cc1d_linear.hpp", "cc1d_linear_device.hpp", "cc1d_linear_attend.hpp", "cc1d_linear_tile.hpp"]
 PUBLIC_HEADERS = ["cc1d.h", "cc1d_mixer.h"]
 BINDING_SOURCES = ["causal_conv1d.cpp", "mixer.cpp"]
 BINDING_HEADERS = ["cc1d_torch.hpp", "cc1d_torch_calls.hpp"]

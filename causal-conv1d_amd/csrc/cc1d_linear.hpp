@@ -36,6 +36,14 @@ struct LinearRows { const void *p; int64_t sb, sl, sh; int32_t by_key; };
 // small differences of large sums, three.
 constexpr int out_terms(int dt) { return dt == CC1D_F32 ? 3 : 2; }
 
+// W of a state's operands, by sizes and type alone (what a forward saves has to be what its backward reads, whatever the layouts): those of
+// linear_tile_kernel where it may take the product of `d1` by `d2` columns.
+inline int operand_width(int dtype, int d1, int d2, bool gradient_of_keys) {
+    const bool tile = dtype != CC1D_F32 && d1 <= 128 && d1 % 8 == 0 && d2 % 8 == 0 && (!gradient_of_keys || d2 <= 128);
+    return !tile ? 2 : d2 <= 64 ? 4 : 8;
+}
+inline int operand_tiles(int width, int d2) { return (d2 + 16 * width - 1) / (16 * width) * width; }
+
 struct SegmentWork {
     int32_t slots, chunks;               // segments of the call; of one sequence without cu_seqlens
     int32_t kp, vp;                      // 32-column steps of dim_k, dim_v
@@ -47,6 +55,7 @@ struct SegmentWork {
     float *dot_q, *dot_k;                // per (slot, value head): q.dq and k.(dk / beta) of each token
     float *inner;                        // per (slot, value head): S0 . dS0, a partial sum each tile
     float *share_q, *share_k;            // shares of dq, dk of heads_each value heads: (shares, batch, seqlen, heads, dim_k)
+    int32_t k_width, v_width, k_tiles, v_tiles;                // of operands contracted over dim_k (out, dv), over dim_v (dq, dk)
     int32_t heads_each, shares;          // value heads of a workgroup of the gradients of q and k; such workgroups a key head
     __device__ __host__ int64_t tiles() const { return (int64_t)kp * vp; }
 };
@@ -79,10 +88,19 @@ struct ScanArgs {
     int32_t to_end;                      // the last segment's own sum is there too: `last`, or S0 . dS0 of the first, need it
     int32_t reverse, write_k, write_v, use_inner;
 };
+// A product with a state has a right operand of 16 columns a tile, PT terms of 1 KB each: [step of the contraction][tile][term].
+// Which columns of an operand of a state stand for which of the matrix: of every 16 W, tile t (0 .. W - 1) and lane m are column W m + t; W = 2 for the
+// general kernel, 4 or 8 for linear_tile_kernel.
+__device__ __forceinline__ int operand_place(int col, int width) {     // of 1 KB tiles of 16 columns: tile << 4 | m
+    const int in = col & (16 * width - 1);
+    return (col / (16 * width) * width + in % width) << 4 | in / width;
+}
 struct AttendArgs {
     LinearRows x, y, z, u;               // u: what the rows of the result are multiplied with for the gates' gradients
     const uint8_t *state;
-    int32_t d1, d2, steps, pairs;        // columns of x, y and of z; 32-column steps of them
+    int32_t d1, d2, steps;               // columns of x, y and of z; 32-column steps of x, y
+    int32_t width, tiles;                // W of the state's operands, and their number in a step
+    int32_t tile;                        // linear_tile_kernel takes it
     int32_t first;                       // the first segment (REV: the last) has a state too
     int32_t group, heads_each, shares;   // value heads of a key head, of a workgroup; workgroups of a key head
     uint32_t items, col_tiles;           // (slot, key head, share); 128-column tiles of d2

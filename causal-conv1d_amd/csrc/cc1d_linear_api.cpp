@@ -39,13 +39,17 @@ bool near(const cc1d_delta_params &p, int64_t stride) {
     return p.seqlen <= 1 || (stride >= 0 && stride * elem_bytes(p.x_dtype) < ((int64_t)1 << 31) / kSegment);
 }
 bool reachable(const cc1d_delta_params &p) { return near(p, p.q_stride_l) && near(p, p.k_stride_l) && near(p, p.v_stride_l); }
+bool reachable_out(const cc1d_delta_params &p) { return reachable(p) && near(p, p.out_stride_l); }
+bool reachable_gradients(const cc1d_delta_bwd_params &bp) {
+    return reachable(bp.fwd) && near(bp.fwd, bp.dout_stride_l) && near(bp.fwd, bp.dq_stride_l) && near(bp.fwd, bp.dk_stride_l) && near(bp.fwd, bp.dv_stride_l);
+}
 
 // Sequences of this many tokens on average go by segments; `saved`: all do.
 int segments_from(const cc1d_delta_params &p) { return 16; }
 bool by_segments(const cc1d_delta_params &p) {
     if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return false;
     if (p.saved != nullptr) return true;
-    return reachable(p) && p.seqlen >= (int64_t)segments_from(p) * (p.cu_seqlens == nullptr ? 1 : p.sequences);
+    return reachable_out(p) && p.seqlen >= (int64_t)segments_from(p) * (p.cu_seqlens == nullptr ? 1 : p.sequences);
 }
 // Whether any segment has a state in front of it.
 bool has_states(const cc1d_delta_params &p, const SegmentWork &w) { return w.chunks > 1 || p.cu_seqlens != nullptr || p.initial_states != nullptr; }
@@ -68,13 +72,19 @@ SegmentWork sizes_of(const cc1d_delta_params &p) {
     w.slots = (int32_t)(slots < INT32_MAX ? slots : INT32_MAX);
     w.kp = (p.dim_k + 31) / 32;
     w.vp = (p.dim_v + 31) / 32;
+    w.k_width = operand_width(p.x_dtype, p.dim_k, p.dim_v, false);
+    w.v_width = operand_width(p.x_dtype, p.dim_v, p.dim_k, true);
+    w.k_tiles = operand_tiles(w.k_width, p.dim_v);
+    w.v_tiles = operand_tiles(w.v_width, p.dim_k);
     w.by_v_heads = fast_div((uint32_t)p.v_heads);
     w.by_chunks = fast_div((uint32_t)w.chunks);
     w.by_group = fast_div((uint32_t)(p.heads > 0 ? p.v_heads / p.heads : 1));
     return w;
 }
-// Numbers of 32 x 32 tiles: of one state for every slot and value head.
+// Numbers of 32 x 32 tiles: of one state for every slot and value head; bytes of its operands.
 size_t state_tiles(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.tiles(); }
+size_t by_k_bytes(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.kp * w.k_tiles * out_terms(p.x_dtype) * kFrag; }
+size_t by_v_bytes(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.vp * w.v_tiles * 3 * kFrag; }
 
 // One workgroup a (slot, block, value head, 128 columns) and less; the scan's one wavefront a tile of each sequence's states.
 bool grids_fit(const cc1d_delta_params &p, const SegmentWork &w) {
@@ -89,20 +99,23 @@ size_t lay_out_fwd(const cc1d_delta_params &p, uint8_t *base, SegmentWork &w) {
         const size_t tiles = state_tiles(p, w);
         w.local = work.floats(tiles * 1024);
         w.decay = work.floats((size_t)w.slots * p.v_heads);
-        w.by_k = work.take(tiles * 2 * out_terms(p.x_dtype) * kFrag);
+        w.by_k = work.take(by_k_bytes(p, w));
     }
     w.by_v = static_cast<uint8_t *>(p.saved);
     return work.used;
 }
 
-// Value heads that a workgroup of the gradients of q and k takes one after the other: as many as leave four workgroups for every CU, since each
-// workgroup of a shared key head writes its share in fp32.
+// Value heads that a workgroup takes one after the other, of `items` (slots, value heads and column tiles): what belongs to their key head is read once for
+// all of them, and of the gradients of q and k, whose workgroups of a shared key head each write a share in fp32, that is less too; but
+// `workgroups` of them at least.
+int heads_of_workgroup(int group, int64_t items, int workgroups) {
+    const int64_t most = items / workgroups;
+    const int each = most < 1 ? 1 : most > group ? group : (int)most, shares = (group + each - 1) / each;
+    return (group + shares - 1) / shares;
+}
 void share_heads(const cc1d_delta_params &p, SegmentWork &w) {
     const int group = p.v_heads / p.heads;
-    const int64_t each = (int64_t)w.slots * kBlocks * p.v_heads / 1024;
-    w.heads_each = each < 1 ? 1 : each > group ? group : (int32_t)each;
-    w.shares = (group + w.heads_each - 1) / w.heads_each;
-    w.heads_each = (group + w.shares - 1) / w.shares;
+    w.heads_each = heads_of_workgroup(group, (int64_t)w.slots * p.v_heads * (w.v_width > 2 ? 1 : kBlocks), 256);
     w.shares = (group + w.heads_each - 1) / w.heads_each;
 }
 bool gradient_of_states(const cc1d_delta_bwd_params &bp, const SegmentWork &w) {
@@ -119,8 +132,8 @@ size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &
         const size_t tiles = state_tiles(p, w);
         w.local = work.floats(tiles * 1024);
         w.decay = work.floats(heads);
-        w.by_k = work.take(tiles * 2 * out_terms(p.x_dtype) * kFrag);
-        w.by_v = work.take(tiles * 2 * 3 * kFrag);
+        w.by_k = work.take(by_k_bytes(p, w));
+        w.by_v = work.take(by_v_bytes(p, w));
         w.inner = work.floats(tiles);
     }
     w.dot_q = work.floats(heads * kSegment);
@@ -136,7 +149,7 @@ size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &
 LinearRows rows(const void *x, int64_t sb, int64_t sl, int64_t sh, bool by_key) { return {x, sb, sl, sh, by_key}; }
 #define ROWS(P, NAME, KEY) rows(P.NAME, P.NAME##_stride_b, P.NAME##_stride_l, P.NAME##_stride_h, KEY)
 
-// Rows of whole 16-byte vectors, for x and y; of whole column pairs.
+// Rows of whole 16-byte vectors; of whole column pairs.
 bool whole(int dtype, const LinearRows &r, int dim) { return dim % 8 == 0 && whole_rows(dtype, r.p, r.sb, r.sl, r.sh); }
 bool paired(int dtype, const void *x, int64_t sb, int64_t sl, int64_t sh, int dim) {
     return dim % 2 == 0 && (reinterpret_cast<uintptr_t>(x) & (2u * (uint32_t)elem_bytes(dtype) - 1u)) == 0 && sb % 2 == 0 && sl % 2 == 0 && sh % 2 == 0;
@@ -146,17 +159,20 @@ bool paired(int dtype, const LinearRows &r, int dim) { return paired(dtype, r.p,
 int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool rev, bool dots, hipStream_t stream) {
     if (w.slots == 0) return CC1D_OK;
     a.group = p.v_heads / p.heads;
-    a.heads_each = dots ? w.heads_each : 1;
-    a.shares = dots ? w.shares : a.group;
     a.steps = (a.d1 + 31) / 32;
-    a.pairs = (a.d2 + 31) / 32;
+    a.width = dots ? w.v_width : w.k_width;
+    a.tiles = dots ? w.v_tiles : w.k_tiles;
+    const bool rows16 = whole(p.x_dtype, a.x, a.d1) && whole(p.x_dtype, a.y, a.d1);
+    a.tile = a.width > 2 && rows16 && whole(p.x_dtype, a.z, a.d2) && (!dots || whole(p.x_dtype, a.u, a.d2)) &&
+             (a.share != nullptr || whole(p.x_dtype, rows(a.out, a.out_b, a.out_l, a.out_h, false), a.d2));
+    a.heads_each = dots ? w.heads_each : a.tile ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads * ((a.d2 + 127) / 128), 512) : 1;
+    a.shares = (a.group + a.heads_each - 1) / a.heads_each;
     a.items = (uint32_t)w.slots * (uint32_t)p.heads * (uint32_t)a.shares;
     a.col_tiles = dots ? 1u : (uint32_t)(a.d2 + 127) / 128;
     a.by_col_tiles = fast_div(a.col_tiles);
     a.by_heads = fast_div((uint32_t)p.heads);
     a.by_shares = fast_div((uint32_t)a.shares);
-    const bool vec = whole(p.x_dtype, a.x, a.d1) && whole(p.x_dtype, a.y, a.d1) && paired(p.x_dtype, a.z, a.d2) &&
-                     (a.share != nullptr || paired(p.x_dtype, a.out, a.out_b, a.out_l, a.out_h, a.d2));
+    const bool vec = rows16 && paired(p.x_dtype, a.z, a.d2) && (a.share != nullptr || paired(p.x_dtype, a.out, a.out_b, a.out_l, a.out_h, a.d2));
     auto of_type = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         if (rev) return dots ? launch_attend<DT, true, true>(p, w, a, vec, stream) : launch_attend<DT, true, false>(p, w, a, vec, stream);
@@ -267,7 +283,7 @@ int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     if (st != CC1D_OK || !by_segments(*p)) return st;
     SegmentWork w;
     *bytes = lay_out_fwd(*p, nullptr, w);
-    return grids_fit(*p, w) && reachable(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    return grids_fit(*p, w) && reachable_out(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
@@ -279,7 +295,7 @@ int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
     const int st = cc1d_validate_delta(&q);
     if (st != CC1D_OK) return st;
     const SegmentWork w = sizes_of(*p);
-    *bytes = state_tiles(*p, w) * 2 * 3 * kFrag;
+    *bytes = by_v_bytes(*p, w);
     return CC1D_OK;
 }
 
@@ -312,7 +328,7 @@ int cc1d_linear_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *byte
     if (st != CC1D_OK || p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return st;
     SegmentWork w;
     *bytes = lay_out_bwd(*p, nullptr, w);
-    return grids_fit(p->fwd, w) && reachable(p->fwd) && near(p->fwd, p->dout_stride_l) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    return grids_fit(p->fwd, w) && reachable_gradients(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_linear_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {

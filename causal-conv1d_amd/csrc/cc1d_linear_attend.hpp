@@ -157,7 +157,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
 #pragma unroll
             for (int c = 0; c < CP; ++c) acc[i][c][0] = acc[i][c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (has_state) {
-            const uint8_t *st = a.state + sv * (int64_t)a.steps * a.pairs * 2 * PT * kFrag + lane * 16;
+            const uint8_t *st = a.state + sv * (int64_t)a.steps * a.tiles * PT * kFrag;
             for (int slab = 0; slab < slabs; ++slab) {
                 if (slab > 0) {
                     lds_barrier();
@@ -168,14 +168,20 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
 #pragma unroll
                 for (int c = 0; c < CP; ++c) {
                     const int pair = pair0 + 4 * c;
-                    if (pair >= a.pairs) continue;
+                    if (32 * pair >= a.d2) continue;
+                    int at_tile[2];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const int place = operand_place(32 * pair + 2 * m + n, a.width);
+                        at_tile[n] = (place >> 4) * PT * kFrag + (g * 16 + (place & 15)) * 16;
+                    }
 #pragma unroll
                     for (int s = 0; s < KS; ++s) {
                         const int step = slab * KS + s;
                         if (step >= a.steps) break;
                         bf16x8 b[2][PT];
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) load_frag<PT>(st + (((int64_t)step * a.pairs + pair) * 2 + n) * PT * kFrag, 0, b[n]);
+                        for (int n = 0; n < 2; ++n) load_frag<PT>(st + step * a.tiles * PT * kFrag + at_tile[n], 0, b[n]);
 #pragma unroll
                         for (int i = 0; i < RT; ++i) {
                             bf16x8 f[NT];
@@ -370,28 +376,6 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
             }
         }
     }
-}
-
-// Of one type, direction and kind: each is a file of its own.
-template <int DT, bool REV, bool DOTS>
-int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, bool vec, hipStream_t stream) {
-    const dim3 grid((a.items + 7) / 8 * 8 * kBlocks * a.col_tiles);
-    auto go = [&](auto ks, auto rt, auto cp, auto v) {
-        constexpr int KS = decltype(ks)::value, RT = decltype(rt)::value, CP = decltype(cp)::value;
-        constexpr size_t lds = sizeof(AttendLds<DT, KS, DOTS ? 3 : out_terms(DT)>);
-        CC1D_LAUNCH((linear_attend_kernel<DT, KS, RT, CP, REV, DOTS, decltype(v)::value>), grid, dim3(kBlock), lds, stream, p, w, a);
-        return launch_status();
-    };
-    using I1 = std::integral_constant<int, 1>;
-    using I2 = std::integral_constant<int, 2>;
-    using I4 = std::integral_constant<int, 4>;
-    auto by_columns = [&](auto ks) {
-        if constexpr (DOTS)
-            if (a.d2 > 128) return vec ? go(ks, I4(), I2(), std::true_type()) : go(ks, I4(), I2(), std::false_type());
-        if (!vec) return go(ks, I4(), I1(), std::false_type());
-        return a.d2 <= 64 ? go(ks, I2(), I1(), std::true_type()) : go(ks, I4(), I1(), std::true_type());
-    };
-    return a.steps <= 2 ? by_columns(I2()) : by_columns(I4());
 }
 
 }  // namespace cc1d

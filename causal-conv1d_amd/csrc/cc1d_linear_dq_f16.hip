@@ -1,5 +1,5 @@
-// Linear attention, dq of f16 tensors (cc1d_linear_attend.hpp).
-#include "cc1d_linear_attend.hpp"
+// Linear attention, dq of f16 tensors (cc1d_linear_attend.hpp, cc1d_linear_tile.hpp).
+#include "cc1d_linear_tile.hpp"
 
 namespace cc1d {
 template int launch_attend<CC1D_F16, false, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);

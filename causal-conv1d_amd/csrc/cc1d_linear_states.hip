@@ -158,15 +158,24 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
             t[c][4] = hi.x; t[c][5] = hi.y; t[c][6] = hi.z; t[c][7] = hi.w;
         }
     };
-    auto by_v_tile = [&](int slot) { return ((((int64_t)slot * p.v_heads + h) * w.vp + q) * w.kp + pi) * 2 * 3 * kFrag + lane * 16; };
+    // Where this lane's two columns lie among a step's operands (of one term).
+    int k_place[2], v_place[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int kc = operand_place(v0 + c, w.k_width), vc = operand_place(32 * pi + 2 * m + c, w.v_width);
+        k_place[c] = (kc >> 4) * KTERMS * kFrag + (g * 16 + (kc & 15)) * 16;
+        v_place[c] = (vc >> 4) * 3 * kFrag + (g * 16 + (vc & 15)) * 16;
+    }
+    auto by_k_step = [&](int slot) { return ((((int64_t)slot * p.v_heads + h) * w.kp + pi) * w.k_tiles) * KTERMS * kFrag; };
+    auto by_v_step = [&](int slot) { return ((((int64_t)slot * p.v_heads + h) * w.vp + q) * w.v_tiles) * 3 * kFrag; };
     // S0 . dS0 of a segment whose dS0 is at hand.
     auto inner = [&](int slot, const float (&t)[2][8]) {
-        const uint8_t *from = w.first + by_v_tile(slot);
+        const uint8_t *from = w.first + by_v_step(slot);
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             bf16x8 f[3];
-            load_frag<3>(from + c * 3 * kFrag, 0, f);
+            load_frag<3>(from + v_place[c], 0, f);
             float x[4];
             four_of(f, false, x);
 #pragma unroll
@@ -192,26 +201,26 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
             const int slot = chunk_of(i);
             if (i > 0 || a.first != nullptr) {
                 if (a.write_k) {
-                    uint8_t *to = w.by_k + place(slot) * 2 * KTERMS * kFrag + lane * 16;
+                    uint8_t *to = w.by_k + by_k_step(slot);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         bf16x8 f[KTERMS];
                         split8<KTERMS>(s[c], f);
 #pragma unroll
-                        for (int t = 0; t < KTERMS; ++t) *reinterpret_cast<u32x4 *>(to + (c * KTERMS + t) * kFrag) = bitcast<u32x4>(f[t]);
+                        for (int t = 0; t < KTERMS; ++t) *reinterpret_cast<u32x4 *>(to + k_place[c] + t * kFrag) = bitcast<u32x4>(f[t]);
                     }
                 }
                 if (a.write_v || a.use_inner) {
                     float t[2][8];
                     turned(t);
                     if (a.write_v) {
-                        uint8_t *to = w.by_v + by_v_tile(slot);
+                        uint8_t *to = w.by_v + by_v_step(slot);
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
                             bf16x8 f[3];
                             split8<3>(t[c], f);
 #pragma unroll
-                            for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4 *>(to + (c * 3 + k) * kFrag) = bitcast<u32x4>(f[k]);
+                            for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4 *>(to + v_place[c] + k * kFrag) = bitcast<u32x4>(f[k]);
                         }
                     }
                     if (a.use_inner && i > 0) inner(slot + 1, t);            // (reverse: what is behind this segment is in front of the one behind it)

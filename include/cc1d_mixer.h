@@ -143,8 +143,8 @@ int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
  * head's outputs from the start of its 64 tokens on.  Gates are bounded from below by -200, which forgets everything.  Where they
  * are positive, the states may grow by less than 2^128 over 256 tokens.
  * Precision is the gated delta rule's; the factors that make out and dv of 16 bits carry 2^-17.
- * Tokens 2^23 bytes apart or more (in q, k, v) go by tokens in the forward; there, with `saved`, and in the backward (dout too) they are refused
- * with CC1D_ERR_TOO_LARGE.
+ * Tokens 2^23 bytes apart or more (in q, k, v or out) go by tokens in the forward; there, with `saved`, and in the backward (in q, k, v, dout or their
+ * gradients) they are refused with CC1D_ERR_TOO_LARGE.
  * ---------------------------------------------------------------------------------- */
 int cc1d_validate_linear(const cc1d_delta_params *p);
 int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes);
