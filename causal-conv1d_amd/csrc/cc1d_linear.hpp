@@ -48,8 +48,7 @@ struct SegmentWork {
     int32_t slots, chunks;               // segments of the call; of one sequence without cu_seqlens
     int32_t kp, vp;                      // 32-column steps of dim_k, dim_v
     FastDiv by_v_heads, by_chunks, by_group;
-    float *gates;                        // per (slot, value head): G of 256 tokens as two floats, and their beta; NULL: not summed up
-    float *local;                        // per (slot, value head): a segment's own sum, [dim_k / 8][32 vp columns][8 of dim_k]
+    float *local;                        // per (slot, value head): a segment's own sum, [kp][vp] tiles of 32 x 32 in operand order
     float *decay;                        // per (slot, value head): exp(Gend)
     uint8_t *by_k, *by_v;                // per (slot, value head): states split into operands, contracted over dim_k and over dim_v
     uint8_t *first;                      // S0 of the forward, contracted over dim_v: what a training forward saves

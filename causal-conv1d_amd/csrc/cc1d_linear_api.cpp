@@ -54,12 +54,6 @@ bool by_segments(const cc1d_delta_params &p) {
 // Whether any segment has a state in front of it.
 bool has_states(const cc1d_delta_params &p, const SegmentWork &w) { return w.chunks > 1 || p.cu_seqlens != nullptr || p.initial_states != nullptr; }
 
-// Whether any segment's own sum is needed: the kernel that makes them leaves the gates summed up for the others.
-bool sums_wanted(const cc1d_delta_params &p, const SegmentWork &w) { return w.chunks > 1 || p.cu_seqlens != nullptr || p.final_states != nullptr; }
-bool gradient_sums_wanted(const cc1d_delta_bwd_params &bp, const SegmentWork &w) {
-    return w.slots > 0 && (w.chunks > 1 || bp.fwd.cu_seqlens != nullptr || bp.fwd.initial_states != nullptr || bp.dinitial_states != nullptr);
-}
-
 struct Places {
     uint8_t *base;
     size_t used = 0;
@@ -105,17 +99,15 @@ size_t lay_out_fwd(const cc1d_delta_params &p, uint8_t *base, SegmentWork &w) {
         const size_t tiles = state_tiles(p, w);
         w.local = work.floats(tiles * 1024);
         w.decay = work.floats((size_t)w.slots * p.v_heads);
-        if (sums_wanted(p, w)) w.gates = work.floats((size_t)w.slots * p.v_heads * 3 * kSegment);
         w.by_k = work.take(by_k_bytes(p, w));
     }
     w.by_v = static_cast<uint8_t *>(p.saved);
     return work.used;
 }
 
-// Value heads that a workgroup takes one after the other, of `items` (slots and value heads): what belongs to their key head is read once for
+// Value heads that a workgroup takes one after the other, of `items` (slots, value heads and column tiles): what belongs to their key head is read once for
 // all of them, and of the gradients of q and k, whose workgroups of a shared key head each write a share in fp32, that is less too; but
-// `workgroups` of them at least, one a CU (32 segments of 80 heads: out 112 us, with two 127; dq 192 and 207).  Not where z has more than 64 columns: out of 64
-// segments of 16 heads of 128 x 128, float16, 118 us each for itself and 138 in pairs, whose registers spill.
+// `workgroups` of them at least.
 int heads_of_workgroup(int group, int64_t items, int workgroups) {
     const int64_t most = items / workgroups;
     const int each = most < 1 ? 1 : most > group ? group : (int)most, shares = (group + each - 1) / each;
@@ -140,7 +132,6 @@ size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &
         const size_t tiles = state_tiles(p, w);
         w.local = work.floats(tiles * 1024);
         w.decay = work.floats(heads);
-        if (gradient_sums_wanted(bp, w)) w.gates = work.floats(heads * 3 * kSegment);
         w.by_k = work.take(by_k_bytes(p, w));
         w.by_v = work.take(by_v_bytes(p, w));
         w.inner = work.floats(tiles);
@@ -174,7 +165,7 @@ int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool 
     const bool rows16 = whole(p.x_dtype, a.x, a.d1) && whole(p.x_dtype, a.y, a.d1);
     a.tile = a.width > 2 && rows16 && whole(p.x_dtype, a.z, a.d2) && (!dots || whole(p.x_dtype, a.u, a.d2)) &&
              (a.share != nullptr || whole(p.x_dtype, rows(a.out, a.out_b, a.out_l, a.out_h, false), a.d2));
-    a.heads_each = dots ? w.heads_each : a.tile && a.width == 4 ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads, 256) : 1;
+    a.heads_each = dots ? w.heads_each : a.tile ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads * ((a.d2 + 127) / 128), 512) : 1;
     a.shares = (a.group + a.heads_each - 1) / a.heads_each;
     a.items = (uint32_t)w.slots * (uint32_t)p.heads * (uint32_t)a.shares;
     a.col_tiles = dots ? 1u : (uint32_t)(a.d2 + 127) / 128;
@@ -198,10 +189,10 @@ int forward(const cc1d_delta_params &p, const SegmentWork &w, hipStream_t stream
     const LinearRows q = ROWS(p, q, true), k = ROWS(p, k, true), v = ROWS(p, v, false);
     int st = CC1D_OK;
     const bool states = has_states(p, w);
-    if (sums_wanted(p, w)) {
+    if (w.chunks > 1 || p.cu_seqlens != nullptr || p.final_states != nullptr) {
         StatesArgs a = {};
         a.a = k; a.b = v; a.all = p.final_states != nullptr;
-        a.vec = whole(p.x_dtype, k, p.dim_k) && whole(p.x_dtype, v, p.dim_v);
+        a.vec = paired(p.x_dtype, k, p.dim_k) && paired(p.x_dtype, v, p.dim_v);
         st = launch_linear_states(p, w, a, stream);
         if (st != CC1D_OK) return st;
     }
@@ -229,10 +220,10 @@ int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t 
     const LinearRows q = ROWS(p, q, true), k = ROWS(p, k, true), v = ROWS(p, v, false), dout = ROWS(bp, dout, false);
     int st = CC1D_OK;
     const bool initial = p.initial_states != nullptr, to_end = initial || bp.dinitial_states != nullptr;
-    if (gradient_sums_wanted(bp, w)) {
+    if (w.slots > 0 && (w.chunks > 1 || p.cu_seqlens != nullptr || to_end)) {
         StatesArgs a = {};
         a.a = q; a.b = dout; a.from_start = 1; a.all = to_end; a.factor = p.scale;
-        a.vec = whole(p.x_dtype, q, p.dim_k) && whole(p.x_dtype, dout, p.dim_v);
+        a.vec = paired(p.x_dtype, q, p.dim_k) && paired(p.x_dtype, dout, p.dim_v);
         st = launch_linear_states(p, w, a, stream);
         if (st != CC1D_OK) return st;
     }

@@ -104,67 +104,6 @@ struct Pair8 {
     }
 };
 
-// N adjacent columns of eight rows, asked for at once (VEC: rows of whole 16-byte vectors, cols a multiple of N); a column of all eight rows is an
-// operand of a tile whose columns (or rows) are every N-th.
-template <int DT, int N, bool VEC>
-struct Columns8 {
-    static constexpr int WORDS = DT == CC1D_F32 ? N : N / 2;
-    uint32_t r[8][WORDS];
-    // Row i, columns from c on; those that are not there repeat the first.
-    __device__ __forceinline__ void ask(int i, const uint8_t *row, int c, int cols) {
-        if constexpr (VEC) {
-            const uint8_t *at = row + (uint32_t)(c < cols ? c : 0) * (DT == CC1D_F32 ? 4u : 2u);
-            if constexpr (WORDS == 1) {
-                r[i][0] = *reinterpret_cast<const uint32_t *>(at);
-            } else if constexpr (WORDS == 2) {
-                const u32x2 v = *reinterpret_cast<const u32x2 *>(at);
-                r[i][0] = v.x; r[i][1] = v.y;
-            } else {
-#pragma unroll
-                for (int q = 0; q < WORDS; q += 4) {
-                    const u32x4 v = *reinterpret_cast<const u32x4 *>(at + 4 * q);
-                    r[i][q] = v.x; r[i][q + 1] = v.y; r[i][q + 2] = v.z; r[i][q + 3] = v.w;
-                }
-            }
-        } else if constexpr (DT == CC1D_F32) {
-#pragma unroll
-            for (int q = 0; q < N; ++q) r[i][q] = reinterpret_cast<const uint32_t *>(row)[c + q < cols ? c + q : 0];
-        } else {
-            const uint16_t *x = reinterpret_cast<const uint16_t *>(row);
-#pragma unroll
-            for (int q = 0; q < N; q += 2) r[i][q / 2] = (uint32_t)x[c + q < cols ? c + q : 0] | (uint32_t)x[c + q + 1 < cols ? c + q + 1 : 0] << 16;
-        }
-    }
-    __device__ __forceinline__ u32x4 bits(int t) const { // of 16-bit types
-        const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;
-        const int q = t >> 1;
-        u32x4 w;
-        w.x = __builtin_amdgcn_perm(r[1][q], r[0][q], sel);
-        w.y = __builtin_amdgcn_perm(r[3][q], r[2][q], sel);
-        w.z = __builtin_amdgcn_perm(r[5][q], r[4][q], sel);
-        w.w = __builtin_amdgcn_perm(r[7][q], r[6][q], sel);
-        return w;
-    }
-    __device__ __forceinline__ void get(int t, float (&f)[8]) const {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (DT == CC1D_F32) f[i] = bitcast<float>(r[i][t]);
-            else if constexpr (DT == CC1D_F16) f[i] = (float)bitcast<_Float16>((uint16_t)((t & 1) ? r[i][t >> 1] >> 16 : r[i][t >> 1]));
-            else f[i] = bitcast<float>((t & 1) ? r[i][t >> 1] & 0xffff0000u : r[i][t >> 1] << 16);
-        }
-    }
-    template <int TERMS>
-    __device__ __forceinline__ void operand(int t, bf16x8 (&o)[TERMS]) const {
-        if constexpr (DT == CC1D_BF16 && TERMS == 1) {
-            o[0] = bitcast<bf16x8>(bits(t));
-        } else {
-            float f[8];
-            get(t, f);
-            split8<TERMS>(f, o);
-        }
-    }
-};
-
 // Two adjacent results to columns c, c + 1 of a row.
 template <int DT, bool VEC>
 __device__ __forceinline__ void store_pair(typename Elem<DT>::type *row, int c, int cols, float a, float b) {

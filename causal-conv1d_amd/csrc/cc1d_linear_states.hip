@@ -6,74 +6,67 @@
 namespace cc1d {
 namespace {
 
-// sum over a segment's tokens of weight_t a_t b_t^T, one workgroup a (slot, value head, 32 TB columns of b): a wavefront takes half of a's columns and half of
-// those of b.  The weight goes to b, which is split into three terms then; a stays as it is, one term in bfloat16.  No operand goes through
-// LDS: a lane reads TA (TB) adjacent columns of eight tokens (Columns8), 4 to 16 bytes a row, whose columns are the operands of as many tiles; its results are
-// then 4 TA adjacent rows, whole groups of eight as the state's operands want them, of TB adjacent columns.
-// It also leaves what the later kernels need of the gates: there a head's tokens lie v_heads apart, a cache line for each.
-template <int DT, int TA, int TB, bool VEC>
-__global__ void __launch_bounds__(kBlock, DT == CC1D_F32 || TA == 8 ? 1 : 2)
-linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const StatesArgs a, const FastDiv by_col_tiles, const uint32_t col_tiles) {
+// sum over a segment's tokens of weight_t a_t b_t^T, one workgroup a (slot, value head, 128 columns of b): a wavefront takes 32 columns of b, all
+// columns of a; where b has at most 64, two wavefronts share those and take half of a each.  The weight goes to b, which is split into three
+// terms then; a stays as it is, one term in bfloat16.  No operand goes through LDS: pairs of columns (Pair8) are loaded in the order
+// of the matrix instruction, and the result tiles of a pair of a's are eight consecutive rows of a lane, the operand order of the next product.
+// KT: 32-column steps of a that a wavefront takes.
+template <int DT, int KT, bool VEC>
+__global__ void __launch_bounds__(kBlock, KT <= 4 && DT != CC1D_F32 ? 2 : 1)
+linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const StatesArgs a, const int halves, const uint32_t col_tiles) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n;
     __shared__ GateLds gates;
     __shared__ float weight[kSegment];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t per = gridDim.x >> 3, item = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);       // heads of one segment, which may share a, on one XCD
-    const uint32_t sv = divided(item, by_col_tiles), ct = item - sv * col_tiles;
-    if (sv >= (uint32_t)w.slots * (uint32_t)p.v_heads) return;
+    const uint32_t sv = blockIdx.x / col_tiles, ct = blockIdx.x - sv * col_tiles;
     const int slot = (int)divided(sv, w.by_v_heads), h = (int)sv - slot * p.v_heads, hk = (int)divided((uint32_t)h, w.by_group);
     const SegmentAt at = segment_at(p, w, slot);
-    if (at.count <= 0) return;
-    const bool wanted = a.all || (a.from_start ? at.c > 0 : !at.last);
-    if (!wanted && ct != 0) return;
+    if (at.count <= 0 || !(a.all || (a.from_start ? at.c > 0 : !at.last))) return;
 
     segment_gates(p, at, h, wave, lane, gates);
     {
         const int i = threadIdx.x;
-        weight[i] = i >= at.count ? 0.f : a.from_start ? a.factor * decay_since_start(gates, i) : gates.beta[i] * decay_between(gates, i, kSegment - 1);
-        if (ct == 0) {
-            float *to = w.gates + (int64_t)sv * 3 * kSegment + i;
-            to[0] = gates.hi[i];
-            to[kSegment] = gates.lo[i];
-            to[2 * kSegment] = gates.beta[i];
-            if (i == 0) w.decay[sv] = decay_since_start(gates, kSegment - 1);
-        }
+        if (i < kSegment) weight[i] = i >= at.count ? 0.f : a.from_start ? a.factor * decay_since_start(gates, i) : gates.beta[i] * decay_between(gates, i, kSegment - 1);
+        if (i == 0 && ct == 0) w.decay[sv] = decay_since_start(gates, kSegment - 1);
     }
-    if (!wanted) return;
     lds_barrier();
 
-    const int a0 = 16 * TA * (wave >> 1), b0 = (int)ct * 32 * TB + 16 * TB * (wave & 1);           // first columns
-    if (a0 >= p.dim_k || b0 >= p.dim_v) return;
+    const int q = halves ? wave & 1 : (int)ct * 4 + wave, p0 = halves ? (wave >> 1) * KT : 0;
+    if (q >= w.vp || p0 >= w.kp) return;
+    const int cb = 32 * q + 2 * m;
     const uint8_t *ab = reinterpret_cast<const uint8_t *>(static_cast<const T *>(a.a.p) + at.b * a.a.sb + at.lo * a.a.sl + (a.a.by_key ? hk : h) * a.a.sh);
     const uint8_t *bb = reinterpret_cast<const uint8_t *>(static_cast<const T *>(a.b.p) + at.b * a.b.sb + at.lo * a.b.sl + (a.b.by_key ? hk : h) * a.b.sh);
     const uint32_t a_pitch = (uint32_t)(a.a.sl * (int64_t)sizeof(T)), b_pitch = (uint32_t)(a.b.sl * (int64_t)sizeof(T));
 
-    f32x4 acc[TA][TB];
+    f32x4 acc[KT][2][2];
 #pragma unroll
-    for (int i = 0; i < TA; ++i)
+    for (int i = 0; i < KT; ++i)
 #pragma unroll
-        for (int c = 0; c < TB; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Columns8<DT, TA, VEC> ra;
-    Columns8<DT, TB, VEC> rb;
+        for (int e = 0; e < 4; ++e) acc[i][e >> 1][e & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Pair8<DT, VEC> ra[KT], rb;
     auto ask = [&](int t0) {             // 32 tokens from t0 on; those behind the last take its rows, and their weight is 0
+        uint32_t at_a[8], at_b[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int t = t0 + 8 * g + e;
             const uint32_t tok = (uint32_t)(t < at.count ? t : at.count - 1);
-            rb.ask(e, bb + tok * b_pitch, b0 + TB * m, p.dim_v);
-            ra.ask(e, ab + tok * a_pitch, a0 + TA * m, p.dim_k);
+            at_a[e] = tok * a_pitch;
+            at_b[e] = tok * b_pitch;
         }
+        rb.ask(bb, at_b, cb, p.dim_v);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) ra[i].ask(ab, at_a, 32 * (p0 + i) + 2 * m, p.dim_k);
     };
     ask(0);
     for (int t0 = 0; t0 < at.count; t0 += 32) {
-        bf16x8 fb[TB][3], fa[TA][NT];
+        bf16x8 fb[2][3], fa[KT][2][NT];
         {
             const float4 w0 = *reinterpret_cast<const float4 *>(&weight[t0 + 8 * g]), w1 = *reinterpret_cast<const float4 *>(&weight[t0 + 8 * g + 4]);
             const float wt[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-            for (int n = 0; n < TB; ++n) {
+            for (int n = 0; n < 2; ++n) {
                 float f[8];
                 rb.get(n, f);
 #pragma unroll
@@ -82,30 +75,34 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
             }
         }
 #pragma unroll
-        for (int i = 0; i < TA; ++i) ra.template operand<NT>(i, fa[i]);
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) ra[i].template operand<NT>(n, fa[i][n]);
         if (t0 + 32 < at.count) ask(t0 + 32);
         stay();
 #pragma unroll
-        for (int c = 0; c < TB; ++c)
+        for (int i = 0; i < KT; ++i)
 #pragma unroll
-            for (int i = 0; i < TA; ++i) acc[i][c] = product<2>(fa[i], fb[c], acc[i][c]);
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) acc[i][n][c] = product<2>(fa[i][n], fb[c], acc[i][n][c]);
         stay();
     }
-    // This lane's results: rows a0 + 4 TA g + TA e + i, columns b0 + TB m + c.  Padding is 0: it meets other operands' padding.
-    const int k0 = a0 + 4 * TA * g, c0 = b0 + TB * m, columns = 32 * w.vp;
-    if (c0 >= columns) return;
+    // Rows of a's pair i: dim_k index 32 (p0 + i) + 8 g + 2 e + n.  Padding is 0: it meets other operands' padding.
 #pragma unroll
-    for (int u = 0; u < TA / 2; ++u) {
-        if (k0 + 8 * u >= 32 * w.kp) continue;
-        float *to = w.local + ((int64_t)sv * 4 * w.kp + k0 / 8 + u) * columns * 8 + c0 * 8;
+    for (int i = 0; i < KT; ++i) {
+        if (p0 + i >= w.kp) break;
+        float *to = w.local + (((int64_t)sv * w.kp + p0 + i) * w.vp + q) * 1024 + lane * 8;
 #pragma unroll
-        for (int c = 0; c < TB; ++c) {
-            if (c0 + c >= columns) continue;
+        for (int c = 0; c < 2; ++c) {
             float f[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = k0 + 8 * u + j < p.dim_k && c0 + c < p.dim_v ? acc[(8 * u + j) % TA][c][(8 * u + j) / TA] : 0.f;
-            *reinterpret_cast<float4 *>(to + c * 8) = make_float4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float4 *>(to + c * 8 + 4) = make_float4(f[4], f[5], f[6], f[7]);
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                    f[2 * e + n] = 32 * (p0 + i) + 8 * g + 2 * e + n < p.dim_k && cb + c < p.dim_v ? acc[i][n][c][e] : 0.f;
+            *reinterpret_cast<float4 *>(to + c * 512) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4 *>(to + c * 512 + 4) = make_float4(f[4], f[5], f[6], f[7]);
         }
     }
 }
@@ -117,10 +114,7 @@ __global__ void __launch_bounds__(64)
 linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArgs a, const FastDiv by_tiles, const FastDiv by_vp) {
     __shared__ float turn[32][36];
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
-    // The tiles of one state, which write into each other's lines, on one XCD.
-    const uint32_t per = gridDim.x >> 3, item = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
-    const uint32_t tiles = (uint32_t)w.tiles(), nh = divided(item, by_tiles), tile = item - nh * tiles;
-    if (nh >= (uint32_t)p.sequences * (uint32_t)p.v_heads) return;
+    const uint32_t tiles = (uint32_t)w.tiles(), nh = divided(blockIdx.x, by_tiles), tile = blockIdx.x - nh * tiles;
     const int n = (int)divided(nh, w.by_v_heads), h = (int)nh - n * p.v_heads;
     const int pi = (int)divided(tile, by_vp), q = (int)tile - pi * w.vp;
     const TokenRange range = sequence_tokens(p, n);
@@ -143,9 +137,12 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
     auto ask = [&](int i) {
         Step x;
         if (i >= summed) i = summed > 0 ? summed - 1 : 0;
-        const float4 *from = reinterpret_cast<const float4 *>(w.local + (((int64_t)chunk_of(i) * p.v_heads + h) * 4 * w.kp + 4 * pi + g) * 256 * w.vp + v0 * 8);
+        const float *from = w.local + place(chunk_of(i)) * 1024 + lane * 8;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x.x[c] = from[c];
+        for (int c = 0; c < 2; ++c) {
+            x.x[2 * c] = *reinterpret_cast<const float4 *>(from + c * 512);
+            x.x[2 * c + 1] = *reinterpret_cast<const float4 *>(from + c * 512 + 4);
+        }
         x.decay = w.decay[(int64_t)chunk_of(i) * p.v_heads + h];
         return x;
     };
@@ -256,59 +253,42 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
     }
 }
 
-// dg and dbeta of a segment, one workgroup a (slot, 16 value heads), a wavefront four of them: they leave through LDS, since a token's heads are neighbours in
-// memory and a head's tokens are not.
-constexpr int kGateHeads = 16;
+// dg and dbeta of a segment, one wavefront each (slot, value head).
 __global__ void __launch_bounds__(kBlock)
-linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const int first, const uint32_t head_tiles) {
-    __shared__ float dg_lds[kSegment][kGateHeads + 1], db_lds[kSegment][kGateHeads + 1];
+linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const uint32_t items, const int first) {
     const cc1d_delta_params &p = bp.fwd;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int slot = (int)(blockIdx.x / head_tiles), h0 = (int)(blockIdx.x % head_tiles) * kGateHeads;
-    const int heads = p.v_heads - h0 < kGateHeads ? p.v_heads - h0 : kGateHeads;
+    const int lane = threadIdx.x & 63;
+    const uint32_t sv = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (sv >= items) return;
+    const int slot = (int)divided(sv, w.by_v_heads), h = (int)sv - slot * p.v_heads;
     auto put = [&](int64_t at, float dg, float dbeta) {
         store_from_float(bp.dg, at, p.g_dtype, dg);
         if (p.beta != nullptr) store_from_float(bp.dbeta, at, p.beta_dtype, dbeta);
     };
-    const int own = (int)threadIdx.x % kGateHeads, token = (int)threadIdx.x / kGateHeads;
-    constexpr int kTokens = kBlock / kGateHeads;
-    if (p.cu_seqlens != nullptr && own < heads) {        // tokens in front of the first sequence and behind the last
-        const int64_t front = sequence_tokens(p, 0).lo, back = sequence_tokens(p, p.sequences - 1).hi, from = (int64_t)slot * kTokens + token, step = (int64_t)w.slots * kTokens;
-        for (int64_t t = from; t < front; t += step) put(t * p.v_heads + h0 + own, 0.f, 0.f);
-        for (int64_t t = back + from; t < p.seqlen; t += step) put(t * p.v_heads + h0 + own, 0.f, 0.f);
+    if (p.cu_seqlens != nullptr) {                       // tokens in front of the first sequence and behind the last
+        const int64_t front = sequence_tokens(p, 0).lo, back = sequence_tokens(p, p.sequences - 1).hi;
+        for (int64_t t = (int64_t)slot * 64 + lane; t < front; t += (int64_t)w.slots * 64) put(t * p.v_heads + h, 0.f, 0.f);
+        for (int64_t t = back + (int64_t)slot * 64 + lane; t < p.seqlen; t += (int64_t)w.slots * 64) put(t * p.v_heads + h, 0.f, 0.f);
     }
     const SegmentAt at = segment_at(p, w, slot);
     if (at.count <= 0) return;
-    for (int i = wave; i < heads; i += 4) {
-        const int h = h0 + i;
-        const int64_t sv = (int64_t)slot * p.v_heads + h;
-        float qd[kBlocks], kz[kBlocks], beta[kBlocks];
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {              // (behind the last token: of that one)
-            const int t = b * kChunk + lane < at.count ? b * kChunk + lane : at.count - 1;
-            qd[b] = w.dot_q[sv * kSegment + t];
-            kz[b] = w.dot_k[sv * kSegment + t];
-            beta[b] = 1.f;
-            if (p.beta != nullptr) beta[b] = bits_as_float(load_bits(p.beta, at.b * p.beta_stride_b + (at.lo + t) * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype), p.beta_dtype);
-        }
-        // The terms cancel up to rounding: their running sum is kept in 64 bits.
-        double dg = 0.0;
-        if (at.c > 0 || first) {
-            double sum = 0.0;
-            for (int64_t k = lane; k < w.tiles(); k += 64) sum += (double)w.inner[sv * w.tiles() + k];
-            dg = of_lane(running_sum(sum), 63);
-        }
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            const double change = b * kChunk + lane < at.count ? (double)qd[b] - (double)beta[b] * (double)kz[b] : 0.0, sum = running_sum(change);
-            dg_lds[b * kChunk + lane][i] = (float)(dg - (sum - change));
-            db_lds[b * kChunk + lane][i] = kz[b];
-            dg -= of_lane(sum, 63);
-        }
+    // The terms cancel up to rounding: their running sum is kept in 64 bits.
+    double dg = 0.0;
+    if (at.c > 0 || first) {
+        double sum = 0.0;
+        for (int64_t i = lane; i < w.tiles(); i += 64) sum += (double)w.inner[(int64_t)sv * w.tiles() + i];
+        dg = of_lane(running_sum(sum), 63);
     }
-    __syncthreads();
-    if (own < heads)
-        for (int t = token; t < at.count; t += kTokens) put(((int64_t)at.b * p.seqlen + at.lo + t) * p.v_heads + h0 + own, dg_lds[t][own], db_lds[t][own]);
+    for (int t0 = 0; t0 < at.count; t0 += 64) {
+        const int t = t0 + lane;
+        const bool there = t < at.count;
+        const int64_t tok = at.lo + (there ? t : 0);
+        const float beta = p.beta == nullptr ? 1.f : bits_as_float(load_bits(p.beta, at.b * p.beta_stride_b + tok * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype), p.beta_dtype);
+        const float qd = there ? w.dot_q[(int64_t)sv * kSegment + t] : 0.f, kz = there ? w.dot_k[(int64_t)sv * kSegment + t] : 0.f;
+        const double change = there ? (double)qd - (double)beta * (double)kz : 0.0, sum = running_sum(change);
+        if (there) put(((int64_t)at.b * p.seqlen + tok) * p.v_heads + h, (float)(dg - (sum - change)), kz);
+        dg -= of_lane(sum, 63);
+    }
 }
 
 // dq and dk of a key head whose value heads were several workgroups': their shares in a fixed order.
@@ -335,16 +315,17 @@ linear_join_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const in
 
 template <int DT>
 int launch_states(const cc1d_delta_params &p, const SegmentWork &w, const StatesArgs &a, hipStream_t stream) {
-    const uint32_t col_tiles = w.vp <= 2 ? 1 : (uint32_t)(w.vp + 3) / 4, items = (uint32_t)w.slots * (uint32_t)p.v_heads * col_tiles;
-    const FastDiv by_col_tiles = fast_div(col_tiles);
-    auto go = [&](auto ta, auto tb) {
-        constexpr int TA = decltype(ta)::value, TB = decltype(tb)::value;
-        if (a.vec) CC1D_LAUNCH((linear_states_kernel<DT, TA, TB, true>), dim3((items + 7) / 8 * 8), dim3(kBlock), 0, stream, p, w, a, by_col_tiles, col_tiles);
-        else CC1D_LAUNCH((linear_states_kernel<DT, TA, TB, false>), dim3((items + 7) / 8 * 8), dim3(kBlock), 0, stream, p, w, a, by_col_tiles, col_tiles);
+    const int halves = w.vp <= 2, each = halves ? (w.kp + 1) / 2 : w.kp;
+    const uint32_t col_tiles = halves ? 1 : (uint32_t)(w.vp + 3) / 4;
+    const dim3 grid((uint32_t)w.slots * (uint32_t)p.v_heads * col_tiles);
+    auto go = [&](auto kt) {
+        constexpr int KT = decltype(kt)::value;
+        if (a.vec) CC1D_LAUNCH((linear_states_kernel<DT, KT, true>), grid, dim3(kBlock), 0, stream, p, w, a, halves, col_tiles);
+        else CC1D_LAUNCH((linear_states_kernel<DT, KT, false>), grid, dim3(kBlock), 0, stream, p, w, a, halves, col_tiles);
         return launch_status();
     };
-    auto with = [&](auto ta) { return w.vp <= 2 ? go(ta, std::integral_constant<int, 2>()) : go(ta, std::integral_constant<int, 4>()); };
-    return w.kp <= 2 ? with(std::integral_constant<int, 2>()) : w.kp <= 4 ? with(std::integral_constant<int, 4>()) : with(std::integral_constant<int, 8>());
+    return each <= 1 ? go(std::integral_constant<int, 1>()) : each <= 2 ? go(std::integral_constant<int, 2>()) :
+           each <= 4 ? go(std::integral_constant<int, 4>()) : go(std::integral_constant<int, 8>());
 }
 
 }  // namespace
@@ -359,7 +340,7 @@ int launch_linear_states(const cc1d_delta_params &p, const SegmentWork &w, const
 }
 
 int launch_linear_scan(const cc1d_delta_params &p, const SegmentWork &w, const ScanArgs &a, hipStream_t stream) {
-    const dim3 grid((uint32_t)((int64_t)p.sequences * p.v_heads * w.tiles() + 7) / 8 * 8);
+    const dim3 grid((uint32_t)((int64_t)p.sequences * p.v_heads * w.tiles()));
     const FastDiv by_tiles = fast_div((uint32_t)w.tiles()), by_vp = fast_div((uint32_t)w.vp);
     if (out_terms(p.x_dtype) == 3) CC1D_LAUNCH(linear_scan_kernel<3>, grid, dim3(64), 0, stream, p, w, a, by_tiles, by_vp);
     else CC1D_LAUNCH(linear_scan_kernel<2>, grid, dim3(64), 0, stream, p, w, a, by_tiles, by_vp);
@@ -367,9 +348,9 @@ int launch_linear_scan(const cc1d_delta_params &p, const SegmentWork &w, const S
 }
 
 int launch_linear_gates(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream) {
-    if (w.slots == 0) return CC1D_OK;
-    const uint32_t head_tiles = (uint32_t)(bp.fwd.v_heads + kGateHeads - 1) / kGateHeads;
-    CC1D_LAUNCH(linear_gates_kernel, dim3((uint32_t)w.slots * head_tiles), dim3(kBlock), 0, stream, bp, w, (int)(bp.fwd.initial_states != nullptr), head_tiles);
+    const uint32_t items = (uint32_t)w.slots * (uint32_t)bp.fwd.v_heads;
+    if (items == 0) return CC1D_OK;
+    CC1D_LAUNCH(linear_gates_kernel, dim3((items + 3) / 4), dim3(kBlock), 0, stream, bp, w, items, (int)(bp.fwd.initial_states != nullptr));
     return launch_status();
 }
 

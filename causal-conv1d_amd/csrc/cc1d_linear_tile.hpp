@@ -66,6 +66,30 @@ __device__ __forceinline__ void product_rows(const bf16x8 (&a)[2][NA], const bf1
         }
 }
 
+// W adjacent 16-bit columns of eight rows; element t of all eight as an operand.
+template <int W>
+struct Wide8 {
+    uint32_t r[8][W / 2];
+    __device__ __forceinline__ void ask(int i, const uint8_t *at) {
+        if constexpr (W == 8) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(at);
+            r[i][0] = v.x; r[i][1] = v.y; r[i][W / 2 - 2] = v.z; r[i][W / 2 - 1] = v.w;
+        } else {
+            const u32x2 v = *reinterpret_cast<const u32x2 *>(at);
+            r[i][0] = v.x; r[i][1] = v.y;
+        }
+    }
+    __device__ __forceinline__ u32x4 column(int t) const {
+        const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;
+        const int q = t >> 1;
+        u32x4 w;
+        w.x = __builtin_amdgcn_perm(r[1][q], r[0][q], sel);
+        w.y = __builtin_amdgcn_perm(r[3][q], r[2][q], sel);
+        w.z = __builtin_amdgcn_perm(r[5][q], r[4][q], sel);
+        w.w = __builtin_amdgcn_perm(r[7][q], r[6][q], sel);
+        return w;
+    }
+};
 // W results to adjacent columns, all inside.
 template <int DT, int W>
 __device__ __forceinline__ void store_wide(typename Elem<DT>::type *to, const float (&o)[W]) {
@@ -147,17 +171,10 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
     const uint32_t x_pitch = (uint32_t)(a.x.sl * (int64_t)sizeof(T)), y_pitch = (uint32_t)(a.y.sl * (int64_t)sizeof(T)), z_pitch = (uint32_t)(a.z.sl * (int64_t)sizeof(T));
     auto head_of = [&](const LinearRows &t) { return static_cast<const uint8_t *>(t.p) + (at.b * t.sb + at.lo * t.sl + (t.by_key ? hk : h) * t.sh) * (int64_t)sizeof(T); };
     // What is on its way.
-    uint32_t gate_bits = 0, beta_bits = 0, low_bits = 0;
+    uint32_t gate_bits = 0, beta_bits = 0;
     u32x4 x[2][KS], yr[2][KS], in_state[IN_STATE];       // x, y: rows 16 i + m of 32, 8 columns: an operand either way
-    Columns8<DT, W, true> zr;
-    auto ask_gates = [&]() {                             // summed up already, or as they came
-        if (w.gates != nullptr) {
-            const uint32_t *from = reinterpret_cast<const uint32_t *>(w.gates) + ((int64_t)slot * p.v_heads + h) * 3 * kSegment + mine;
-            gate_bits = from[0];
-            low_bits = from[kSegment];
-            beta_bits = from[2 * kSegment];
-            return;
-        }
+    Wide8<W> zr;
+    auto ask_gates = [&]() {
         const int64_t tok = at.lo + token(mine);
         gate_bits = load_bits(p.g, at.b * p.g_stride_b + tok * p.g_stride_l + h * p.g_stride_h, p.g_dtype);
         if (p.beta != nullptr) beta_bits = load_bits(p.beta, at.b * p.beta_stride_b + tok * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype);
@@ -182,8 +199,9 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
     };
     auto ask_z = [&]() {                                 // columns that are not there: the first
         const uint8_t *zb = head_of(a.z);
+        const uint32_t col = (uint32_t)(col0 + W * m < a.d2 ? col0 + W * m : 0) * (uint32_t)sizeof(T);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) zr.ask(e, zb + (uint32_t)token(own * kStep + 8 * g + e) * z_pitch, col0 + W * m, a.d2);
+        for (int e = 0; e < 8; ++e) zr.ask(e, zb + ((uint32_t)token(own * kStep + 8 * g + e) * z_pitch + col));
     };
     auto ask_state = [&](int stage) {                    // steps that are not there: the last
         const uint8_t *st = a.state + ((int64_t)slot * p.v_heads + h) * a.steps * a.tiles * PT * kFrag + (int64_t)ct * STATE * kFrag + lane * 16;
@@ -209,16 +227,9 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
         if (hi > 0) lds_barrier();                       // the head before has been read
         // G, one token a lane.
         const bool first_half = threadIdx.x < kSegment;
-        float beta = 1.f;
-        double sum;
-        if (w.gates != nullptr) {
-            beta = bitcast<float>(beta_bits);
-            sum = (double)bitcast<float>(gate_bits) + (double)bitcast<float>(low_bits);
-        } else {
-            if (p.beta != nullptr) beta = bits_as_float(beta_bits, p.beta_dtype);
-            sum = running_sum(mine < at.count ? (double)bounded_gate(bits_as_float(gate_bits, p.g_dtype)) : 0.0);
-            if (first_half && lane == 63) lds.sums[wave] = sum;
-        }
+        const float beta = p.beta != nullptr ? bits_as_float(beta_bits, p.beta_dtype) : 1.f;
+        double sum = running_sum(mine < at.count ? (double)bounded_gate(bits_as_float(gate_bits, p.g_dtype)) : 0.0);
+        if (first_half && lane == 63) lds.sums[wave] = sum;
         if (has_state) {
 #pragma unroll
             for (int i = 0; i < IN_STATE; ++i)
@@ -226,9 +237,8 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
         }
         lds_barrier();
         if (has_state && STAGES > 1) ask_state(1);
-        if (w.gates == nullptr)
 #pragma unroll
-            for (int b = 0; b < kBlocks - 1; ++b) sum += b < (wave & 3) ? lds.sums[b] : 0.0;
+        for (int b = 0; b < kBlocks - 1; ++b) sum += b < (wave & 3) ? lds.sums[b] : 0.0;
         if (first_half) {
             const float h0 = (float)sum;
             lds.hi[mine] = h0;
@@ -296,15 +306,10 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
                     for (int s = 0; s < KS; ++s) *reinterpret_cast<u32x4 *>(lds.y + ((own * 2 + i) * KS + s) * kFrag + lane * 16) = yr[i][s];
             if (hi == 0 || !DOTS)
 #pragma unroll
-                for (int t = 0; t < W; ++t) *reinterpret_cast<u32x4 *>(lds.z + (own * W + t) * kFrag + lane * 16) = zr.bits(t);
+                for (int t = 0; t < W; ++t) *reinterpret_cast<u32x4 *>(lds.z + (own * W + t) * kFrag + lane * 16) = zr.column(t);
         }
         lds_barrier();                                   // y, z, factors
         const bool more = MANY && hi + 1 < h_count;
-        // x has arrived by now; without being told so the compiler waits for it in the loop below, and for all that is asked for here.
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(x[i][s]));
         if (more) {                                      // the next head's
             h += 1;
             ask_gates();
@@ -421,13 +426,13 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
             const uint8_t *ub = static_cast<const uint8_t *>(a.u.p) + (at.b * a.u.sb + at.lo * a.u.sl + hk * a.u.sh) * (int64_t)sizeof(T);      // (of the key head)
             if (more) ask_x();
             if (rows) {
-                const uint32_t u_pitch = (uint32_t)(a.u.sl * (int64_t)sizeof(T));
+                const uint32_t u_pitch = (uint32_t)(a.u.sl * (int64_t)sizeof(T)), col = (uint32_t)(W * m < a.d2 ? W * m : 0) * (uint32_t)sizeof(T);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int row = own * kStep + 16 * i + 4 * g;
-                    Columns8<DT, W, true> u;
+                    Wide8<W> u;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) u.ask(e, ub + (uint32_t)token(row + e) * u_pitch, W * m, a.d2);
+                    for (int e = 0; e < 4; ++e) u.ask(e, ub + ((uint32_t)token(row + e) * u_pitch + col));
                     stay();
                     float dot[4];
 #pragma unroll
@@ -498,9 +503,7 @@ int launch_tile(const cc1d_delta_params &p, const SegmentWork &w, const AttendAr
     };
     auto by_columns = [&](auto ks) {
         auto by_heads = [&](auto width) {
-            if constexpr (DOTS || decltype(width)::value == 4)
-                if (given.heads_each > 1 || given.share != nullptr) return go(ks, width, std::true_type());
-            return go(ks, width, std::false_type());
+            return given.heads_each > 1 || given.share != nullptr ? go(ks, width, std::true_type()) : go(ks, width, std::false_type());
         };
         return given.d2 <= 64 ? by_heads(std::integral_constant<int, 4>()) : by_heads(std::integral_constant<int, 8>());
     };
