@@ -284,6 +284,10 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
     }
 }
 
+// Workgroups of the backward on a CU, all of them at once: its registers leave four wavefronts a SIMD, and a workgroup may put its odd one on any
+// (16384 rows of 2560: two of five wavefronts 126 us, 5.3 TB/s, three 162, the last of them after the others; 8192 of 4096: two of eight 97, one 122).
+int bwd_a_cu(int dim) { return 4 / ((bwd_lanes(dim) + 255) / 256); }
+
 }  // namespace
 }  // namespace cc1d
 
@@ -346,7 +350,7 @@ int cc1d_layer_norm_bwd_workspace_bytes(const cc1d_layer_norm_bwd_params *p, siz
     *bytes = 0;
     const int st = cc1d_validate_layer_norm_bwd(p);
     if (st != CC1D_OK || p->dim == 0) return st;
-    *bytes = (size_t)bwd_parts(p->rows, p->dim) * (p->dbias != nullptr ? 2 : 1) * (size_t)p->dim * sizeof(float);
+    *bytes = (size_t)bwd_parts(p->rows, bwd_a_cu(p->dim)) * (p->dbias != nullptr ? 2 : 1) * (size_t)p->dim * sizeof(float);
     return CC1D_OK;
 }
 
@@ -355,7 +359,7 @@ int cc1d_layer_norm_bwd(const cc1d_layer_norm_bwd_params *p, void *workspace, si
     int st = cc1d_layer_norm_bwd_workspace_bytes(p, &need);
     if (st != CC1D_OK || p->dim == 0) return st;
     if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
-    const int64_t parts = bwd_parts(p->rows, p->dim);
+    const int64_t parts = bwd_parts(p->rows, bwd_a_cu(p->dim));
     const int width = p->dbias != nullptr ? 2 * p->dim : p->dim;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (p->rows > 0) {

@@ -105,9 +105,10 @@ size_t lay_out_fwd(const cc1d_delta_params &p, uint8_t *base, SegmentWork &w) {
     return work.used;
 }
 
-// Value heads that a workgroup takes one after the other, of `items` (slots, value heads and column tiles): what belongs to their key head is read once for
+// Value heads that a workgroup takes one after the other, of `items` (slots and value heads): what belongs to their key head is read once for
 // all of them, and of the gradients of q and k, whose workgroups of a shared key head each write a share in fp32, that is less too; but
-// `workgroups` of them at least.
+// `workgroups` of them at least, one a CU (32 segments of 80 heads: out 112 us, with two 127; dq 192 and 207).  Not where z has more than 64 columns: out of 64
+// segments of 16 heads of 128 x 128, float16, 118 us each for itself and 138 in pairs, whose registers spill.
 int heads_of_workgroup(int group, int64_t items, int workgroups) {
     const int64_t most = items / workgroups;
     const int each = most < 1 ? 1 : most > group ? group : (int)most, shares = (group + each - 1) / each;
@@ -165,7 +166,7 @@ int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool 
     const bool rows16 = whole(p.x_dtype, a.x, a.d1) && whole(p.x_dtype, a.y, a.d1);
     a.tile = a.width > 2 && rows16 && whole(p.x_dtype, a.z, a.d2) && (!dots || whole(p.x_dtype, a.u, a.d2)) &&
              (a.share != nullptr || whole(p.x_dtype, rows(a.out, a.out_b, a.out_l, a.out_h, false), a.d2));
-    a.heads_each = dots ? w.heads_each : a.tile ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads * ((a.d2 + 127) / 128), 512) : 1;
+    a.heads_each = dots ? w.heads_each : a.tile && a.width == 4 ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads, 256) : 1;
     a.shares = (a.group + a.heads_each - 1) / a.heads_each;
     a.items = (uint32_t)w.slots * (uint32_t)p.heads * (uint32_t)a.shares;
     a.col_tiles = dots ? 1u : (uint32_t)(a.d2 + 127) / 128;

@@ -310,6 +310,11 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
         }
         lds_barrier();                                   // y, z, factors
         const bool more = MANY && hi + 1 < h_count;
+        // x has arrived by now; without being told so the compiler waits for it in the loop below, and for all that is asked for here.
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(x[i][s]));
         if (more) {                                      // the next head's
             h += 1;
             ask_gates();
@@ -503,7 +508,9 @@ int launch_tile(const cc1d_delta_params &p, const SegmentWork &w, const AttendAr
     };
     auto by_columns = [&](auto ks) {
         auto by_heads = [&](auto width) {
-            return given.heads_each > 1 || given.share != nullptr ? go(ks, width, std::true_type()) : go(ks, width, std::false_type());
+            if constexpr (DOTS || decltype(width)::value == 4)
+                if (given.heads_each > 1 || given.share != nullptr) return go(ks, width, std::true_type());
+            return go(ks, width, std::false_type());
         };
         return given.d2 <= 64 ? by_heads(std::integral_constant<int, 4>()) : by_heads(std::integral_constant<int, 8>());
     };

@@ -336,6 +336,10 @@ dequantize_kernel(const cc1d_dequantize_params p, const uint32_t vecs, const int
     store8<YD>(p.y, row * p.y_stride + c, n, f);
 }
 
+// Workgroups of the backward on a CU: 1024 lanes (16384 rows of 2560: three
+// of 320 lanes 122 us, two 127, four 151: too many rows at once).
+int bwd_a_cu(int dim) { return 1024 / bwd_lanes(dim); }
+
 }  // namespace
 }  // namespace cc1d
 
@@ -402,7 +406,7 @@ int cc1d_norm_bwd_workspace_bytes(const cc1d_norm_bwd_params *p, size_t *bytes) 
     *bytes = 0;
     const int st = cc1d_validate_norm_bwd(p);
     if (st != CC1D_OK || p->dim == 0) return st;
-    *bytes = (size_t)bwd_parts(p->rows, p->dim) * (size_t)p->dim * sizeof(float);
+    *bytes = (size_t)bwd_parts(p->rows, bwd_a_cu(p->dim)) * (size_t)p->dim * sizeof(float);
     return CC1D_OK;
 }
 
@@ -411,7 +415,7 @@ int cc1d_norm_bwd(const cc1d_norm_bwd_params *p, void *workspace, size_t workspa
     int st = cc1d_norm_bwd_workspace_bytes(p, &need);
     if (st != CC1D_OK || p->dim == 0) return st;
     if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
-    const int64_t parts = bwd_parts(p->rows, p->dim);
+    const int64_t parts = bwd_parts(p->rows, bwd_a_cu(p->dim));
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (p->rows > 0) {
         const int64_t each = (p->rows + parts - 1) / parts;

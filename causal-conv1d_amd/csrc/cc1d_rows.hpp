@@ -196,11 +196,9 @@ int by_shape(const RowShape &s, F &&f) {
     return CC1D_ERR_SHAPE;
 }
 
-// Planes of partial sums, one a workgroup: as many workgroups as put at most 1024 lanes on a CU (16384 rows of 2560: three
-// of 320 lanes 122 us, two 127, four 151: too many rows at once), and no fewer than four rows to each.
-int64_t bwd_parts(int64_t rows, int dim) {
-    const RowShape s = bwd_shape(dim);
-    const int a_cu = 1024 / (s.lanes == 64 ? 256 : s.lanes);
+// Planes of partial sums, one a workgroup: `a_cu` workgroups a CU, and no fewer than four rows to each.
+int bwd_lanes(int dim) { const int lanes = bwd_shape(dim).lanes; return lanes == 64 ? 256 : lanes; }
+int64_t bwd_parts(int64_t rows, int a_cu) {
     const int64_t most = 256 * (a_cu > 1 ? a_cu : 1);
     int64_t each = (rows + most - 1) / most;
     if (each < 4) each = 4;
