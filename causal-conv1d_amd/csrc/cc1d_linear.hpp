@@ -57,9 +57,12 @@ struct SegmentWork {
     float *share_q, *share_k;            // shares of dq, dk of heads_each value heads: (shares, batch, seqlen, heads, dim_k)
     int32_t k_width, v_width, k_tiles, v_tiles;                // of operands contracted over dim_k (out, dv), over dim_v (dq, dk)
     int32_t heads_each, shares;          // value heads of a workgroup of the gradients of q and k; such workgroups a key head
+    int32_t shortest;                    // packed sequences of fewer tokens, kSegment at least, are the token kernel's; 0: none
+    __host__ int64_t walks(const cc1d_delta_params &p) const { return shortest > 0 ? chunks : p.sequences; }
     __device__ __host__ int64_t tiles() const { return (int64_t)kp * vp; }
 };
 
+__device__ __forceinline__ int64_t naming(const TokenRange &r) { return (r.lo + kSegment - 1) >> kSegmentLog; }
 // Tokens [lo, lo + count) of batch entry b: segment c of sequence n, or count = 0 if a slot is none.
 struct SegmentAt { int64_t lo; int count, b, n, c; bool last; };
 __device__ __forceinline__ SegmentAt segment_at(const cc1d_delta_params &p, const SegmentWork &w, int slot) {
@@ -68,7 +71,16 @@ __device__ __forceinline__ SegmentAt segment_at(const cc1d_delta_params &p, cons
         const int64_t lo = (int64_t)c << kSegmentLog, left = p.seqlen - lo;
         return {lo, (int)(left < kSegment ? left : kSegment), n, n, c, left <= kSegment};
     }
-    // As chunks of the gated delta rule: sequence n begins at slot floor(first token / kSegment) + n, and no two share one.
+    // As chunks of the gated delta rule.  Where only long sequences go by segments, each holds a token 256 f; with f of the first of these, its
+    // segment c is slot 2 f + c, which no two share.
+    if (w.shortest > 0) {
+        const int n = sequence_of(p, (int64_t)(slot >> 1) << kSegmentLog);
+        const TokenRange r = sequence_tokens(p, n);
+        const int64_t f = naming(r), c = slot - 2 * f, lo = r.lo + (c << kSegmentLog), left = r.hi - lo;
+        if (r.hi - r.lo < w.shortest || c < 0 || left <= 0) return {0, 0, 0, n, 0, false};
+        return {lo, (int)(left < kSegment ? left : kSegment), 0, n, (int)c, left <= kSegment};
+    }
+    // Else sequence n begins at slot floor(first token / kSegment) + n, and no two share one.
     const int n = last_sequence(p, slot, [](int64_t first, int i) { return (first >> kSegmentLog) + i; });
     const TokenRange r = sequence_tokens(p, n);
     const int64_t c = slot - ((r.lo >> kSegmentLog) + n), lo = r.lo + (c << kSegmentLog), left = r.hi - lo;
@@ -76,7 +88,7 @@ __device__ __forceinline__ SegmentAt segment_at(const cc1d_delta_params &p, cons
     return {lo, (int)(left < kSegment ? left : kSegment), 0, n, (int)c, left <= kSegment};
 }
 __device__ __forceinline__ int first_segment(const cc1d_delta_params &p, const SegmentWork &w, int n, const TokenRange &r) {
-    return p.cu_seqlens == nullptr ? n * w.chunks : (int)(r.lo >> kSegmentLog) + n;
+    return p.cu_seqlens == nullptr ? n * w.chunks : w.shortest > 0 ? 2 * (int)naming(r) : (int)(r.lo >> kSegmentLog) + n;
 }
 
 // Which sums a segment's neighbours need: forward those in front of the last (and the last, if the states are asked for), backward those behind

@@ -44,12 +44,27 @@ bool reachable_gradients(const cc1d_delta_bwd_params &bp) {
     return reachable(bp.fwd) && near(bp.fwd, bp.dout_stride_l) && near(bp.fwd, bp.dq_stride_l) && near(bp.fwd, bp.dk_stride_l) && near(bp.fwd, bp.dv_stride_l);
 }
 
-// Sequences of this many tokens on average go by segments; `saved`: all do.
-int segments_from(const cc1d_delta_params &p) { return 16; }
-bool by_segments(const cc1d_delta_params &p) {
-    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return false;
-    if (p.saved != nullptr) return true;
-    return reachable_out(p) && p.seqlen >= (int64_t)segments_from(p) * (p.cu_seqlens == nullptr ? 1 : p.sequences);
+// Sequences of this many tokens on average go by segments; `saved`: all do.  A token takes 1 us until the states of 512 heads of 128 x 128 (or as
+// many elements of other heads) fill the card, then time by their number, and segments cost by it from the start.  By tokens and by
+// segments: 16-bit types, 4 heads: 16 tokens 21 us and 20, 32 tokens 37 and 21; 256 heads: 32 tokens 40 and 36; 1024 heads: 64 tokens 162 and 136.
+// fp32, whose products take six matrix instructions for one to three: 4 heads: 24 tokens 27 and 27; 256 heads: 64 tokens 66 and 86, 128 tokens 123 and 109;
+// 512 heads: 512 tokens 582 and 632; 1024 heads: 1024 tokens 2126 and 2470.
+int64_t segments_from(const cc1d_delta_params &p, int64_t sequences) {
+    const double all = (double)sequences * p.v_heads * p.dim_k * p.dim_v / 16384.0;
+    const int64_t heads = all < 1024.0 ? (int64_t)all : 1024;
+    if (p.x_dtype == CC1D_F32) return heads >= 512 ? INT32_MAX : 22 + heads / 5;
+    return heads >= 960 ? 64 : 16 + heads / 20;
+}
+// The average says nothing of the longest.  Packed sequences that go by tokens on average go by segments one by one, from 256 tokens on: the
+// kernels see their lengths, the host does not.  Not where all their tokens together are few, nor where one sequence's heads fill
+// the card with tokens.
+enum class Way { tokens, segments, both };
+Way way_of(const cc1d_delta_params &p) {
+    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return Way::tokens;
+    if (p.saved != nullptr) return Way::segments;
+    if (!reachable_out(p)) return Way::tokens;
+    if (p.seqlen >= segments_from(p, p.sequences) * (p.cu_seqlens == nullptr ? 1 : p.sequences)) return Way::segments;
+    return p.cu_seqlens != nullptr && p.seqlen >= 2 * kSegment && segments_from(p, 1) <= kSegment ? Way::both : Way::tokens;
 }
 // Whether any segment has a state in front of it.
 bool has_states(const cc1d_delta_params &p, const SegmentWork &w) { return w.chunks > 1 || p.cu_seqlens != nullptr || p.initial_states != nullptr; }
@@ -65,10 +80,11 @@ struct Places {
     float *floats(size_t n) { return reinterpret_cast<float *>(take(n * sizeof(float))); }
 };
 
-SegmentWork sizes_of(const cc1d_delta_params &p) {
+SegmentWork sizes_of(const cc1d_delta_params &p, bool alone) {
     SegmentWork w = {};
+    w.shortest = alone ? kSegment : 0;
     w.chunks = (int32_t)(((int64_t)p.seqlen + kSegment - 1) / kSegment);
-    const int64_t slots = p.cu_seqlens == nullptr ? (int64_t)p.batch * w.chunks : (int64_t)p.seqlen / kSegment + p.sequences + 1;
+    const int64_t slots = p.cu_seqlens == nullptr ? (int64_t)p.batch * w.chunks : alone ? 2 * (int64_t)w.chunks : (int64_t)p.seqlen / kSegment + p.sequences + 1;
     w.slots = (int32_t)(slots < INT32_MAX ? slots : INT32_MAX);
     w.kp = (p.dim_k + 31) / 32;
     w.vp = (p.dim_v + 31) / 32;
@@ -89,11 +105,11 @@ size_t by_v_bytes(const cc1d_delta_params &p, const SegmentWork &w) { return (si
 // One workgroup a (slot, block, value head, 128 columns) and less; the scan's one wavefront a tile of each sequence's states.
 bool grids_fit(const cc1d_delta_params &p, const SegmentWork &w) {
     return ((int64_t)w.slots * p.v_heads + 8) * kBlocks * ((w.vp + 3) / 4) < thread_limit() / kBlock &&
-           (int64_t)p.sequences * p.v_heads * w.tiles() < thread_limit() / kWave;
+           w.walks(p) * p.v_heads * w.tiles() < thread_limit() / kWave;
 }
 
-size_t lay_out_fwd(const cc1d_delta_params &p, uint8_t *base, SegmentWork &w) {
-    w = sizes_of(p);
+size_t lay_out_fwd(const cc1d_delta_params &p, bool alone, uint8_t *base, SegmentWork &w) {
+    w = sizes_of(p, alone);
     Places work{base};
     if (has_states(p, w) || p.final_states != nullptr) {
         const size_t tiles = state_tiles(p, w);
@@ -124,7 +140,7 @@ bool gradient_of_states(const cc1d_delta_bwd_params &bp, const SegmentWork &w) {
 }
 size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &w) {
     const cc1d_delta_params &p = bp.fwd;
-    w = sizes_of(p);
+    w = sizes_of(p, false);
     w.first = static_cast<uint8_t *>(p.saved);
     Places work{base};
     share_heads(p, w);
@@ -281,9 +297,10 @@ int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     if (bytes == nullptr) return CC1D_ERR_NULL_POINTER;
     *bytes = 0;
     const int st = cc1d_validate_linear(p);
-    if (st != CC1D_OK || !by_segments(*p)) return st;
+    const Way way = st == CC1D_OK ? way_of(*p) : Way::tokens;
+    if (way == Way::tokens) return st;
     SegmentWork w;
-    *bytes = lay_out_fwd(*p, nullptr, w);
+    *bytes = lay_out_fwd(*p, way == Way::both, nullptr, w);
     return grids_fit(*p, w) && reachable_out(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
@@ -295,7 +312,7 @@ int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
     if (q.out == nullptr) q.out = const_cast<void *>(q.v);                 // (not needed for this)
     const int st = cc1d_validate_delta(&q);
     if (st != CC1D_OK) return st;
-    const SegmentWork w = sizes_of(*p);
+    const SegmentWork w = sizes_of(*p, false);
     *bytes = by_v_bytes(*p, w);
     return CC1D_OK;
 }
@@ -307,10 +324,12 @@ int cc1d_linear_fwd(const cc1d_delta_params *p, void *workspace, size_t workspac
     if (need > 0 && (workspace == nullptr || !aligned256(workspace) || workspace_bytes < need)) return CC1D_ERR_WORKSPACE;
     if (p->batch == 0 || p->v_heads == 0 || p->sequences == 0) return CC1D_OK;
     const hipStream_t hs = static_cast<hipStream_t>(stream);
-    if (!by_segments(*p)) return launch_delta_tokens(*p, nullptr, p->sequences, 0, hs, false);
+    const Way way = way_of(*p);
+    if (way == Way::tokens) return launch_delta_tokens(*p, nullptr, p->sequences, 0, hs, false);
     SegmentWork w;
-    lay_out_fwd(*p, static_cast<uint8_t *>(workspace), w);
-    return forward(*p, w, hs);
+    lay_out_fwd(*p, way == Way::both, static_cast<uint8_t *>(workspace), w);
+    const int done = forward(*p, w, hs);
+    return done != CC1D_OK || way == Way::segments ? done : launch_delta_tokens(*p, nullptr, p->sequences, w.shortest, hs, false);
 }
 
 int cc1d_validate_linear_bwd(const cc1d_delta_bwd_params *p) {

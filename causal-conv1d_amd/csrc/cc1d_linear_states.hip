@@ -115,9 +115,11 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
     __shared__ float turn[32][36];
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
     const uint32_t tiles = (uint32_t)w.tiles(), nh = divided(blockIdx.x, by_tiles), tile = blockIdx.x - nh * tiles;
-    const int n = (int)divided(nh, w.by_v_heads), h = (int)nh - n * p.v_heads;
+    const int walk = (int)divided(nh, w.by_v_heads), h = (int)nh - walk * p.v_heads;
+    const int n = w.shortest > 0 ? sequence_of(p, (int64_t)walk << kSegmentLog) : walk;             // (then of the sequence that holds that token, if it is the one that names it)
     const int pi = (int)divided(tile, by_vp), q = (int)tile - pi * w.vp;
     const TokenRange range = sequence_tokens(p, n);
+    if (w.shortest > 0 && (range.hi - range.lo < w.shortest || naming(range) != walk)) return;
     const int chunks = (int)((range.hi - range.lo + kSegment - 1) >> kSegmentLog), slot0 = first_segment(p, w, n, range);
     const int k0 = 32 * pi + 8 * g, v0 = 32 * q + 2 * m;
 
@@ -340,7 +342,7 @@ int launch_linear_states(const cc1d_delta_params &p, const SegmentWork &w, const
 }
 
 int launch_linear_scan(const cc1d_delta_params &p, const SegmentWork &w, const ScanArgs &a, hipStream_t stream) {
-    const dim3 grid((uint32_t)((int64_t)p.sequences * p.v_heads * w.tiles()));
+    const dim3 grid((uint32_t)(w.walks(p) * p.v_heads * w.tiles()));
     const FastDiv by_tiles = fast_div((uint32_t)w.tiles()), by_vp = fast_div((uint32_t)w.vp);
     if (out_terms(p.x_dtype) == 3) CC1D_LAUNCH(linear_scan_kernel<3>, grid, dim3(64), 0, stream, p, w, a, by_tiles, by_vp);
     else CC1D_LAUNCH(linear_scan_kernel<2>, grid, dim3(64), 0, stream, p, w, a, by_tiles, by_vp);
@@ -357,6 +359,7 @@ int launch_linear_gates(const cc1d_delta_bwd_params &bp, const SegmentWork &w, h
 int launch_linear_join(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream) {
     const cc1d_delta_params &p = bp.fwd;
     const int64_t rows = (int64_t)p.batch * p.seqlen * p.heads;
+    if (rows == 0) return CC1D_OK;
     const dim3 grid((uint32_t)(rows < 4 * 8192 ? (rows + 3) / 4 : 8192));
     switch (p.x_dtype) {
         case CC1D_F32: CC1D_LAUNCH(linear_join_kernel<CC1D_F32>, grid, dim3(kBlock), 0, stream, bp, w, rows); break;
