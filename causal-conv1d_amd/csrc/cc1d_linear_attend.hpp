@@ -25,27 +25,44 @@
 
 namespace cc1d {
 
+// Two places for the products, or one and a barrier more where two would leave a CU a single workgroup.
+constexpr int product_places(int dt, int ks) { return dt == CC1D_F32 && ks == 4 ? 1 : 2; }
 template <int DT, int KS, int PT>
 struct AttendLds {
     uint8_t x[4 * KS * Terms<DT>::n * kFrag];
-    uint8_t p[2][8 * PT * kFrag];
+    uint8_t p[product_places(DT, KS)][8 * PT * kFrag];
     GateLds gates;
     float f[kChunk], s[kChunk];
     float dots[4][kChunk];
 };
 
-constexpr int attend_waves(int dt, int cp) { return dt != CC1D_F32 && cp == 1 ? 2 : 1; }
+// Left operands of four tiles against one right one, their chains side by side.
+template <int MOST, int N, int NA, int NB>
+__device__ __forceinline__ void products_left(const bf16x8 (&a)[N][NA], const bf16x8 (&b)[NB], f32x4 *const (&acc)[N]) {
+#pragma unroll
+    for (int sum = MOST; sum >= 0; --sum)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = sum - i;
+            if (j < 0 || j >= NB) continue;
+#pragma unroll
+            for (int t = 0; t < N; ++t) *acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][i], b[j], *acc[t], 0, 0, 0);
+        }
+}
+
+// Wavefronts a SIMD that the registers leave: two where nothing has to be kept in memory for that.
+constexpr int attend_waves(int dt, bool dots, bool vec) { return !dots && (vec || dt != CC1D_F32) ? 2 : 1; }
 
 // KS: 32-column steps of x and y at once (their LDS); wider ones pass slab by slab.
 template <int DT, int KS, int RT, int CP, bool REV, bool DOTS, bool VEC>
-__global__ void __launch_bounds__(kBlock, attend_waves(DT, CP))
+__global__ void __launch_bounds__(kBlock, attend_waves(DT, DOTS, VEC))
 linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n, PT = DOTS ? 3 : out_terms(DT), MOST = PT - 1;
     constexpr bool XREG = KS * NT <= 4;                  // x stays in registers
     extern __shared__ uint4 raw[];
     AttendLds<DT, KS, PT> &lds = *reinterpret_cast<AttendLds<DT, KS, PT> *>(raw);
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // The blocks of one segment and head, which read the same state and y and z, on one XCD; those with the most to do first.
     const uint32_t idx = blockIdx.x >> 3, rest = idx / kBlocks, of_block = idx % kBlocks;
@@ -81,6 +98,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
     const int row0 = r * kChunk, own = at.count - row0;  // rows of this block, if any
     if (own <= 0) return;
     const int blocks = (at.count + kChunk - 1) / kChunk;
+    const bool rows = i0 < own;                          // of this wavefront's result
     const int slabs = (a.steps + KS - 1) / KS;
     const bool cut = a.d1 < 32 * KS * slabs;
     const bool has_state = (REV ? !at.last : at.c > 0) || a.first;
@@ -94,6 +112,11 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
     f32x4 acc[RT][CP][2];
 
     for (int hi = 0; hi < h_count; ++hi) {
+        if constexpr (DOTS) {                            // (addresses are made anew: kept over the loop they would take a hundred registers)
+            asm volatile("" : "+v"(lane));
+            m = lane & 15;
+            g = lane >> 4;
+        }
         const int h = h_first + hi;
         const int64_t sv = (int64_t)slot * p.v_heads + h;
         auto rows_of = [&](const LinearRows &t) { return static_cast<const T *>(t.p) + at.b * t.sb + at.lo * t.sl + (t.by_key ? hk : h) * t.sh; };
@@ -168,28 +191,35 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
 #pragma unroll
                 for (int c = 0; c < CP; ++c) {
                     const int pair = pair0 + 4 * c;
-                    if (32 * pair >= a.d2) continue;
+                    if (32 * pair >= a.d2 || !rows) continue;
                     int at_tile[2];
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         const int place = operand_place(32 * pair + 2 * m + n, a.width);
                         at_tile[n] = (place >> 4) * PT * kFrag + (g * 16 + (place & 15)) * 16;
                     }
+                    bf16x8 b[2][2][PT];
+                    auto ask_state = [&](int s) {        // (steps that are not there: the last, and x is 0)
+                        const int step = slab * KS + s < a.steps ? slab * KS + s : a.steps - 1;
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) load_frag<PT>(st + step * a.tiles * PT * kFrag + at_tile[n], 0, b[s & 1][n]);
+                    };
+                    ask_state(0);
 #pragma unroll
                     for (int s = 0; s < KS; ++s) {
-                        const int step = slab * KS + s;
-                        if (step >= a.steps) break;
-                        bf16x8 b[2][PT];
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) load_frag<PT>(st + step * a.tiles * PT * kFrag + at_tile[n], 0, b[n]);
+                        if (s + 1 < KS) ask_state(s + 1);
+                        bf16x8 f[RT][NT];
+                        f32x4 *to[2][RT];
 #pragma unroll
                         for (int i = 0; i < RT; ++i) {
-                            bf16x8 f[NT];
-                            if constexpr (RT == 4) x_of(i, s, f);
-                            else load_frag<NT>(lds.x + ((half * RT + i) * KS + s) * NT * kFrag, lane, f);
-#pragma unroll
-                            for (int n = 0; n < 2; ++n) acc[i][c][n] = product<MOST>(f, b[n], acc[i][c][n]);
+                            if constexpr (RT == 4) x_of(i, s, f[i]);
+                            else load_frag<NT>(lds.x + ((half * RT + i) * KS + s) * NT * kFrag, lane, f[i]);
+                            to[0][i] = &acc[i][c][0];
+                            to[1][i] = &acc[i][c][1];
                         }
+                        stay();
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) products_left<MOST>(f, b[s & 1][n], to[n]);
                     }
                 }
             }
@@ -213,26 +243,23 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
             of_x[t] = turns > 1 ? (REV ? decay_between(lds.gates, i, border) : decay_between(lds.gates, border, i)) : 0.f;
         }
 
+        Pair8<DT, VEC> zr[CP][2];
+        auto ask_z = [&](int block, int s) {
+            uint32_t off[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) off[e] = (uint32_t)token(block * kChunk + 32 * s + 8 * g + e) * z_pitch;
+#pragma unroll
+            for (int c = 0; c < CP; ++c) zr[c][s].ask(zb, off, 32 * (pair0 + 4 * c) + 2 * m, a.d2);
+        };
+        ask_z(block_of(0), 0);
+        ask_z(block_of(0), 1);
         for (int k = 0; k < turns; ++k) {
             const int c0 = block_of(k);
             const bool self = k == turns - 1;
-            Pair8<DT, VEC> zr[CP][2];
-            auto ask_z = [&]() {
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    uint32_t off[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) off[e] = (uint32_t)token(c0 * kChunk + 32 * s + 8 * g + e) * z_pitch;
-#pragma unroll
-                    for (int c = 0; c < CP; ++c) zr[c][s].ask(zb, off, 32 * (pair0 + 4 * c) + 2 * m, a.d2);
-                }
-            };
-            ask_z();
             f32x4 pt[4];                                 // rows: y's four tokens, columns: x's rows 16 t + m
 #pragma unroll
             for (int t = 0; t < 4; ++t) pt[t] = f32x4{0.f, 0.f, 0.f, 0.f};
             const int y_half = wave >> 1;
-            auto meets = [&](int t, int s) { return !self || (REV ? t <= 2 * s + 1 : t >= 2 * s); };   // x's tile t, 32 of y's tokens
             for (int slab = 0; slab < slabs; ++slab) {
                 if (slabs > 1) {
                     lds_barrier();
@@ -243,19 +270,26 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
                 }
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    bf16x8 f[NT];
-                    yr[s].template operand<NT>(32 * (slab * KS + s) + 8 * g, a.d1, cut, f);
+                    bf16x8 f[NT], b[4][NT];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        if (!meets(t, y_half)) continue;
-                        bf16x8 b[NT];
-                        x_of(t, s, b);
-                        pt[t] = product<2>(f, b, pt[t]);
-                    }
+                    for (int t = 0; t < 4; ++t) x_of(t, s, b[t]);
+                    yr[s].template operand<NT>(32 * (slab * KS + s) + 8 * g, a.d1, cut, f);
+                    stay();
+#pragma unroll
+                    for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) {
+                            const int j = sum - i;
+                            if (j < 0 || j >= NT) continue;
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) pt[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[i], b[t][j], pt[t], 0, 0, 0);
+                        }
                 }
             }
             if (slabs == 1 && !self) ask_y(block_of(k + 1), 0);
             // Weights, terms, and through LDS.
+            uint8_t *place = lds.p[product_places(DT, KS) == 1 ? 0 : k & 1];
+            if (product_places(DT, KS) == 1 && k > 0) lds_barrier();
             {
                 const int j0 = c0 * kChunk + row_of(wave, 4 * g);
                 float cj[4], hj[4], lj[4];
@@ -268,7 +302,6 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
                 }
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    if (!meets(t, y_half)) continue;
                     float x[4];
                     if (self) {
                         const int i = row0 + 16 * t + m;
@@ -286,49 +319,64 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
                     split4<PT>(x, f);
 #pragma unroll
                     for (int n = 0; n < PT; ++n)
-                        *reinterpret_cast<u32x2 *>(lds.p[k & 1] + ((t * 2 + y_half) * PT + n) * kFrag + lane * 16 + (wave & 1) * 8) = f[n];
+                        *reinterpret_cast<u32x2 *>(place + ((t * 2 + y_half) * PT + n) * kFrag + lane * 16 + (wave & 1) * 8) = f[n];
                 }
             }
             lds_barrier();
+            if (!self || rows)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                bf16x8 fz[CP][2][NT];
+                for (int s = 0; s < 2; ++s) {
+                    bf16x8 f[RT][PT];
 #pragma unroll
-                for (int c = 0; c < CP; ++c)
+                    for (int i = 0; i < RT; ++i) load_frag<PT>(place + ((half * RT + i) * 2 + s) * PT * kFrag, lane, f[i]);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) zr[c][s].template operand<NT>(n, fz[c][n]);
+                    for (int c = 0; c < CP; ++c) {
+                        bf16x8 fz[2][NT];
+                        f32x4 *to[2][RT];
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    const int t = half * RT + i;
-                    if (!meets(t, s)) continue;
-                    bf16x8 f[PT];
-                    load_frag<PT>(lds.p[k & 1] + (t * 2 + s) * PT * kFrag, lane, f);
+                        for (int n = 0; n < 2; ++n) {
+                            zr[c][s].template operand<NT>(n, fz[n]);
 #pragma unroll
-                    for (int c = 0; c < CP; ++c)
+                            for (int i = 0; i < RT; ++i) to[n][i] = &acc[i][c][n];
+                        }
+                        if (c == CP - 1 && !self) ask_z(block_of(k + 1), s);
+                        stay();
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) acc[i][c][n] = product<MOST>(f, fz[c][n], acc[i][c][n]);
+                        for (int n = 0; n < 2; ++n) products_left<MOST>(f, fz[n], to[n]);
+                    }
                 }
-            }
         }
 
         if constexpr (DOTS) {
             const T *ub = rows_of(a.u);
+            const uint32_t u_pitch = (uint32_t)(a.u.sl * (int64_t)sizeof(T));
             float dot[RT][4];
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
+            for (int i = 0; i < RT; ++i) {
+                T u[4][CP][2];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const T *row = ub + (int64_t)token(row0 + i0 + 16 * i + 4 * g + e) * a.u.sl;
+                    const T *row = reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(ub) + (uint32_t)token(row0 + i0 + 16 * i + 4 * g + e) * u_pitch);
+#pragma unroll
+                    for (int c = 0; c < CP; ++c) {
+                        const int col = 32 * (pair0 + 4 * c) + 2 * m;
+                        u[e][c][0] = row[col < a.d2 ? col : 0];
+                        u[e][c][1] = row[col + 1 < a.d2 ? col + 1 : 0];
+                    }
+                }
+                stay();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
                     float sum = 0.f;
 #pragma unroll
                     for (int c = 0; c < CP; ++c) {
                         const int col = 32 * (pair0 + 4 * c) + 2 * m;
-                        const float u0 = Elem<DT>::to_float(row[col < a.d2 ? col : 0]), u1 = Elem<DT>::to_float(row[col + 1 < a.d2 ? col + 1 : 0]);
-                        sum += col < a.d2 ? acc[i][c][0][e] * u0 : 0.f;
-                        sum += col + 1 < a.d2 ? acc[i][c][1][e] * u1 : 0.f;
+                        sum += col < a.d2 ? acc[i][c][0][e] * Elem<DT>::to_float(u[e][c][0]) : 0.f;
+                        sum += col + 1 < a.d2 ? acc[i][c][1][e] * Elem<DT>::to_float(u[e][c][1]) : 0.f;
                     }
                     dot[i][e] = over_columns(sum);
                 }
+            }
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 const int row = i0 + 16 * i + 4 * g;
@@ -350,32 +398,34 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
     }
 
     // Rows leave as column pairs.
+    auto leave = [&](auto *to, uint32_t pitch, auto type, auto vec) {  // the block's first row, bytes between rows
+        using E = std::remove_pointer_t<decltype(to)>;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int row = i0 + 16 * i + 4 * g;
-        float s[4] = {1.f, 1.f, 1.f, 1.f};
-        if constexpr (!DOTS) {
-            const float4 f = *reinterpret_cast<const float4 *>(&lds.s[row]);
-            s[0] = f.x; s[1] = f.y; s[2] = f.z; s[3] = f.w;
-        }
+        for (int i = 0; i < RT; ++i) {
+            const int row = i0 + 16 * i + 4 * g;
+            f32x4 s = {1.f, 1.f, 1.f, 1.f};
+            if constexpr (!DOTS) s = *reinterpret_cast<const f32x4 *>(&lds.s[row]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (row + e >= own) continue;
-            const int64_t tok = at.lo + row0 + row + e;
+            for (int e = 0; e < 4; ++e) {
+                if (row + e >= own) continue;
+                E *at_row = reinterpret_cast<E *>(reinterpret_cast<uint8_t *>(to) + (uint32_t)(row + e) * pitch);
 #pragma unroll
-            for (int c = 0; c < CP; ++c) {
-                const int col = 32 * (pair0 + 4 * c) + 2 * m;
-                float o0, o1;
-                if constexpr (DOTS) { o0 = total[i][c][0][e]; o1 = total[i][c][1][e]; }
-                else { o0 = s[e] * acc[i][c][0][e]; o1 = s[e] * acc[i][c][1][e]; }
-                if (a.share == nullptr) {
-                    store_pair<DT, VEC>(static_cast<T *>(a.out) + at.b * a.out_b + tok * a.out_l + out_head * a.out_h, col, a.d2, o0, o1);
-                } else {
-                    store_pair<CC1D_F32, false>(a.share + ((((int64_t)share * p.batch + at.b) * p.seqlen + tok) * p.heads + hk) * a.d2, col, a.d2, o0, o1);
+                for (int c = 0; c < CP; ++c) {
+                    float o0, o1;
+                    if constexpr (DOTS) { o0 = total[i][c][0][e]; o1 = total[i][c][1][e]; }
+                    else { o0 = s[e] * acc[i][c][0][e]; o1 = s[e] * acc[i][c][1][e]; }
+                    store_pair<decltype(type)::value, decltype(vec)::value>(at_row, 32 * (pair0 + 4 * c) + 2 * m, a.d2, o0, o1);
                 }
             }
         }
-    }
+    };
+    const int64_t tok = at.lo + row0;
+    if (!DOTS || a.share == nullptr)
+        leave(static_cast<T *>(a.out) + at.b * a.out_b + tok * a.out_l + out_head * a.out_h, (uint32_t)(a.out_l * (int64_t)sizeof(T)), std::integral_constant<int, DT>(),
+              std::bool_constant<VEC>());
+    else
+        leave(a.share + ((((int64_t)share * p.batch + at.b) * p.seqlen + tok) * p.heads + hk) * a.d2, (uint32_t)p.heads * (uint32_t)a.d2 * 4u, std::integral_constant<int, CC1D_F32>(),
+              std::false_type());
 }
 
 }  // namespace cc1d
