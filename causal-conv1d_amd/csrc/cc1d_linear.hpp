@@ -39,7 +39,7 @@ constexpr int out_terms(int dt) { return dt == CC1D_F32 ? 3 : 2; }
 // W of a state's operands, by sizes and type alone (what a forward saves has to be what its backward reads, whatever the layouts): those of
 // linear_tile_kernel where it may take the product of `d1` by `d2` columns.
 inline int operand_width(int dtype, int d1, int d2, bool gradient_of_keys) {
-    const bool tile = dtype != CC1D_F32 && d1 <= 128 && d1 % 8 == 0 && d2 % 8 == 0 && (!gradient_of_keys || d2 <= 128);
+    const bool tile = dtype != CC1D_F32 && d1 <= 128 && (!gradient_of_keys || d2 <= 128);
     return !tile ? 2 : d2 <= 64 ? 4 : 8;
 }
 inline int operand_tiles(int width, int d2) { return (d2 + 16 * width - 1) / (16 * width) * width; }
@@ -61,6 +61,20 @@ struct SegmentWork {
     __host__ int64_t walks(const cc1d_delta_params &p) const { return shortest > 0 ? chunks : p.sequences; }
     __device__ __host__ int64_t tiles() const { return (int64_t)kp * vp; }
 };
+
+// Rows that are not whole 16-byte vectors (odd sizes, odd strides or addresses) are copied to rows that are, zeros behind their columns, and results
+// from there: the kernels know no others.  16 heads of 100 x 100, 4 x 2048 tokens, bfloat16: 145 us forward and 358 backward, with kernels that read them element by
+// element 254 and 1034; 56 heads of 154 x 80, 7 x 239 tokens: 530 us for 1510.
+constexpr int kVector = 8;
+__host__ __device__ inline int padded(int dim) { return (dim + kVector - 1) / kVector * kVector; }
+struct CopyRows {
+    const uint8_t *from; uint8_t *to;
+    int64_t from_b, from_l, from_h, to_b, to_l, to_h;          // bytes
+    int32_t heads, dim;                  // columns that are there
+    FastDiv by_vectors;                  // vectors of a padded row
+};
+constexpr int kMostCopies = 4;
+struct CopyArgs { CopyRows of[kMostCopies]; int32_t elem, batch, seqlen; FastDiv by_seqlen; };
 
 __device__ __forceinline__ int64_t naming(const TokenRange &r) { return (r.lo + kSegment - 1) >> kSegmentLog; }
 // Tokens [lo, lo + count) of batch entry b: segment c of sequence n, or count = 0 if a slot is none.
@@ -93,7 +107,7 @@ __device__ __forceinline__ int first_segment(const cc1d_delta_params &p, const S
 
 // Which sums a segment's neighbours need: forward those in front of the last (and the last, if the states are asked for), backward those behind
 // the first.
-struct StatesArgs { LinearRows a, b; int32_t from_start, all; float factor; int32_t vec; };
+struct StatesArgs { LinearRows a, b; int32_t from_start, all; float factor; };
 struct ScanArgs {
     const float *first; int64_t first_n, first_h, first_k;     // the state it begins with, or NULL
     float *last; int64_t last_n, last_h, last_k;               // where it ends, or NULL
@@ -121,11 +135,13 @@ struct AttendArgs {
     float *share, *dots;
 };
 
+// `out`: from whole vectors to rows as they are, else the other way round.
+int launch_linear_copy(const CopyArgs &a, int copies, bool out, hipStream_t stream);
 int launch_linear_states(const cc1d_delta_params &p, const SegmentWork &w, const StatesArgs &a, hipStream_t stream);
 int launch_linear_scan(const cc1d_delta_params &p, const SegmentWork &w, const ScanArgs &a, hipStream_t stream);
 // Instantiated one to a file.  DOTS: gradients of q and k.
 template <int DT, bool REV, bool DOTS>
-int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, bool vec, hipStream_t stream);
+int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, hipStream_t stream);
 int launch_linear_gates(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream);
 int launch_linear_join(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream);
 

@@ -6,10 +6,10 @@
 namespace cc1d {
 
 #define CC1D_ATTEND(DT)                                                                                                                          \
-    extern template int launch_attend<DT, false, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);   \
-    extern template int launch_attend<DT, true, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);    \
-    extern template int launch_attend<DT, false, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);    \
-    extern template int launch_attend<DT, true, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, bool, hipStream_t);
+    extern template int launch_attend<DT, false, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);   \
+    extern template int launch_attend<DT, true, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);    \
+    extern template int launch_attend<DT, false, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);    \
+    extern template int launch_attend<DT, true, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);
 CC1D_ATTEND(CC1D_F32)
 CC1D_ATTEND(CC1D_F16)
 CC1D_ATTEND(CC1D_BF16)
@@ -108,7 +108,51 @@ bool grids_fit(const cc1d_delta_params &p, const SegmentWork &w) {
            w.walks(p) * p.v_heads * w.tiles() < thread_limit() / kWave;
 }
 
-size_t lay_out_fwd(const cc1d_delta_params &p, bool alone, uint8_t *base, SegmentWork &w) {
+LinearRows rows(const void *x, int64_t sb, int64_t sl, int64_t sh, bool by_key) { return {x, sb, sl, sh, by_key}; }
+#define ROWS(P, NAME, KEY) rows(P.NAME, P.NAME##_stride_b, P.NAME##_stride_l, P.NAME##_stride_h, KEY)
+bool whole(int dtype, const LinearRows &r, int dim) { return dim % kVector == 0 && whole_rows(dtype, r.p, r.sb, r.sl, r.sh); }
+
+// A call's tensors as the kernels read and write them; those whose rows are not whole vectors at their places in the workspace, and what it takes to bring them
+// there and back.
+struct Tensors {
+    const cc1d_delta_params &p;
+    Places &work;
+    CopyArgs in = {}, out = {};
+    int ins = 0, outs = 0;
+    Tensors(const cc1d_delta_params &params, Places &places) : p(params), work(places) {
+        in.elem = out.elem = elem_bytes(p.x_dtype);
+        in.batch = out.batch = p.batch;
+        in.seqlen = out.seqlen = p.seqlen;
+        in.by_seqlen = out.by_seqlen = fast_div((uint32_t)(p.seqlen > 0 ? p.seqlen : 1));
+    }
+    LinearRows place(const LinearRows &r, int dim, bool written) {
+        if (whole(p.x_dtype, r, dim)) return r;
+        const int heads = r.by_key ? p.heads : p.v_heads, pitch = padded(dim), e = elem_bytes(p.x_dtype);
+        LinearRows at = {nullptr, (int64_t)p.seqlen * heads * pitch, (int64_t)heads * pitch, pitch, r.by_key};
+        at.p = work.take((size_t)p.batch * at.sb * e);
+        const LinearRows &from = written ? at : r, &to = written ? r : at;
+        CopyRows &c = written ? out.of[outs++] : in.of[ins++];
+        c.from = static_cast<const uint8_t *>(from.p);
+        c.to = static_cast<uint8_t *>(const_cast<void *>(to.p));
+        c.from_b = from.sb * e; c.from_l = from.sl * e; c.from_h = from.sh * e;
+        c.to_b = to.sb * e; c.to_l = to.sl * e; c.to_h = to.sh * e;
+        c.heads = heads;
+        c.dim = dim;
+        c.by_vectors = fast_div((uint32_t)(pitch / kVector));
+        return at;
+    }
+    LinearRows read(const LinearRows &r, int dim) { return place(r, dim, false); }
+    LinearRows written(const LinearRows &r, int dim) { return place(r, dim, true); }
+};
+// The rows of a segment of a copy are reached with 32 bits as well.
+bool copies_reachable(const cc1d_delta_params &p) {
+    return (int64_t)p.v_heads * padded(p.dim_k > p.dim_v ? p.dim_k : p.dim_v) * elem_bytes(p.x_dtype) < ((int64_t)1 << 31) / kSegment;
+}
+
+struct Forward { LinearRows q, k, v, out; CopyArgs in, back; int ins, backs; };
+struct Backward { LinearRows q, k, v, dout, dq, dk, dv; CopyArgs in, back; int ins, backs; };
+
+size_t lay_out_fwd(const cc1d_delta_params &p, bool alone, uint8_t *base, SegmentWork &w, Forward &f) {
     w = sizes_of(p, alone);
     Places work{base};
     if (has_states(p, w) || p.final_states != nullptr) {
@@ -118,6 +162,12 @@ size_t lay_out_fwd(const cc1d_delta_params &p, bool alone, uint8_t *base, Segmen
         w.by_k = work.take(by_k_bytes(p, w));
     }
     w.by_v = static_cast<uint8_t *>(p.saved);
+    Tensors t(p, work);
+    f.q = t.read(ROWS(p, q, true), p.dim_k);
+    f.k = t.read(ROWS(p, k, true), p.dim_k);
+    f.v = t.read(ROWS(p, v, false), p.dim_v);
+    f.out = t.written(ROWS(p, out, false), p.dim_v);
+    f.in = t.in; f.ins = t.ins; f.back = t.out; f.backs = t.outs;
     return work.used;
 }
 
@@ -138,7 +188,7 @@ void share_heads(const cc1d_delta_params &p, SegmentWork &w) {
 bool gradient_of_states(const cc1d_delta_bwd_params &bp, const SegmentWork &w) {
     return has_states(bp.fwd, w) || bp.dfinal_states != nullptr || bp.dinitial_states != nullptr;
 }
-size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &w) {
+size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &w, Backward &f) {
     const cc1d_delta_params &p = bp.fwd;
     w = sizes_of(p, false);
     w.first = static_cast<uint8_t *>(p.saved);
@@ -156,32 +206,35 @@ size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &
     w.dot_q = work.floats(heads * kSegment);
     w.dot_k = work.floats(heads * kSegment);
     if (w.shares > 1) {
-        const size_t plane = (size_t)p.batch * p.seqlen * p.heads * p.dim_k;
+        const size_t plane = (size_t)p.batch * p.seqlen * p.heads * padded(p.dim_k);
         w.share_q = work.floats(w.shares * plane);
         w.share_k = work.floats(w.shares * plane);
     }
+    Tensors t(p, work);
+    f.q = t.read(ROWS(p, q, true), p.dim_k);
+    f.k = t.read(ROWS(p, k, true), p.dim_k);
+    f.v = t.read(ROWS(p, v, false), p.dim_v);
+    f.dout = t.read(ROWS(bp, dout, false), p.dim_v);
+    f.dq = ROWS(bp, dq, true);
+    f.dk = ROWS(bp, dk, true);
+    if (w.shares == 1) {                 // (linear_join_kernel writes rows of any kind)
+        f.dq = t.written(f.dq, p.dim_k);
+        f.dk = t.written(f.dk, p.dim_k);
+    }
+    f.dv = t.written(ROWS(bp, dv, false), p.dim_v);
+    f.in = t.in; f.ins = t.ins; f.back = t.out; f.backs = t.outs;
     return work.used;
 }
-
-LinearRows rows(const void *x, int64_t sb, int64_t sl, int64_t sh, bool by_key) { return {x, sb, sl, sh, by_key}; }
-#define ROWS(P, NAME, KEY) rows(P.NAME, P.NAME##_stride_b, P.NAME##_stride_l, P.NAME##_stride_h, KEY)
-
-// Rows of whole 16-byte vectors; of whole column pairs.
-bool whole(int dtype, const LinearRows &r, int dim) { return dim % 8 == 0 && whole_rows(dtype, r.p, r.sb, r.sl, r.sh); }
-bool paired(int dtype, const void *x, int64_t sb, int64_t sl, int64_t sh, int dim) {
-    return dim % 2 == 0 && (reinterpret_cast<uintptr_t>(x) & (2u * (uint32_t)elem_bytes(dtype) - 1u)) == 0 && sb % 2 == 0 && sl % 2 == 0 && sh % 2 == 0;
-}
-bool paired(int dtype, const LinearRows &r, int dim) { return paired(dtype, r.p, r.sb, r.sl, r.sh, dim); }
 
 int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool rev, bool dots, hipStream_t stream) {
     if (w.slots == 0) return CC1D_OK;
     a.group = p.v_heads / p.heads;
+    a.d1 = padded(a.d1);
+    a.d2 = padded(a.d2);
     a.steps = (a.d1 + 31) / 32;
     a.width = dots ? w.v_width : w.k_width;
     a.tiles = dots ? w.v_tiles : w.k_tiles;
-    const bool rows16 = whole(p.x_dtype, a.x, a.d1) && whole(p.x_dtype, a.y, a.d1);
-    a.tile = a.width > 2 && rows16 && whole(p.x_dtype, a.z, a.d2) && (!dots || whole(p.x_dtype, a.u, a.d2)) &&
-             (a.share != nullptr || whole(p.x_dtype, rows(a.out, a.out_b, a.out_l, a.out_h, false), a.d2));
+    a.tile = a.width > 2;
     a.heads_each = dots ? w.heads_each : a.tile && a.width == 4 ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads, 256) : 1;
     a.shares = (a.group + a.heads_each - 1) / a.heads_each;
     a.items = (uint32_t)w.slots * (uint32_t)p.heads * (uint32_t)a.shares;
@@ -189,11 +242,10 @@ int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool 
     a.by_col_tiles = fast_div(a.col_tiles);
     a.by_heads = fast_div((uint32_t)p.heads);
     a.by_shares = fast_div((uint32_t)a.shares);
-    const bool vec = rows16 && paired(p.x_dtype, a.z, a.d2) && (a.share != nullptr || paired(p.x_dtype, a.out, a.out_b, a.out_l, a.out_h, a.d2));
     auto of_type = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (rev) return dots ? launch_attend<DT, true, true>(p, w, a, vec, stream) : launch_attend<DT, true, false>(p, w, a, vec, stream);
-        return dots ? launch_attend<DT, false, true>(p, w, a, vec, stream) : launch_attend<DT, false, false>(p, w, a, vec, stream);
+        if (rev) return dots ? launch_attend<DT, true, true>(p, w, a, stream) : launch_attend<DT, true, false>(p, w, a, stream);
+        return dots ? launch_attend<DT, false, true>(p, w, a, stream) : launch_attend<DT, false, false>(p, w, a, stream);
     };
     switch (p.x_dtype) {
         case CC1D_F32: return of_type(std::integral_constant<int, CC1D_F32>());
@@ -202,14 +254,18 @@ int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool 
     }
 }
 
-int forward(const cc1d_delta_params &p, const SegmentWork &w, hipStream_t stream) {
-    const LinearRows q = ROWS(p, q, true), k = ROWS(p, k, true), v = ROWS(p, v, false);
-    int st = CC1D_OK;
+void set_out(AttendArgs &a, const LinearRows &r) {
+    a.out = const_cast<void *>(r.p);
+    a.out_b = r.sb; a.out_l = r.sl; a.out_h = r.sh;
+}
+
+int forward(const cc1d_delta_params &p, const SegmentWork &w, const Forward &f, hipStream_t stream) {
+    int st = launch_linear_copy(f.in, f.ins, false, stream);
+    if (st != CC1D_OK) return st;
     const bool states = has_states(p, w);
     if (w.chunks > 1 || p.cu_seqlens != nullptr || p.final_states != nullptr) {
         StatesArgs a = {};
-        a.a = k; a.b = v; a.all = p.final_states != nullptr;
-        a.vec = paired(p.x_dtype, k, p.dim_k) && paired(p.x_dtype, v, p.dim_v);
+        a.a = f.k; a.b = f.v; a.all = p.final_states != nullptr;
         st = launch_linear_states(p, w, a, stream);
         if (st != CC1D_OK) return st;
     }
@@ -224,23 +280,23 @@ int forward(const cc1d_delta_params &p, const SegmentWork &w, hipStream_t stream
         if (st != CC1D_OK) return st;
     }
     AttendArgs a = {};
-    a.x = q; a.y = k; a.z = v;
+    a.x = f.q; a.y = f.k; a.z = f.v;
     a.d1 = p.dim_k; a.d2 = p.dim_v;
     a.state = w.by_k;
     a.first = p.initial_states != nullptr;
-    a.out = p.out; a.out_b = p.out_stride_b; a.out_l = p.out_stride_l; a.out_h = p.out_stride_h;
-    return attend(p, w, a, false, false, stream);
+    set_out(a, f.out);
+    st = attend(p, w, a, false, false, stream);
+    return st != CC1D_OK ? st : launch_linear_copy(f.back, f.backs, true, stream);
 }
 
-int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream) {
+int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, const Backward &f, hipStream_t stream) {
     const cc1d_delta_params &p = bp.fwd;
-    const LinearRows q = ROWS(p, q, true), k = ROWS(p, k, true), v = ROWS(p, v, false), dout = ROWS(bp, dout, false);
-    int st = CC1D_OK;
+    int st = launch_linear_copy(f.in, f.ins, false, stream);
+    if (st != CC1D_OK) return st;
     const bool initial = p.initial_states != nullptr, to_end = initial || bp.dinitial_states != nullptr;
     if (w.slots > 0 && (w.chunks > 1 || p.cu_seqlens != nullptr || to_end)) {
         StatesArgs a = {};
-        a.a = q; a.b = dout; a.from_start = 1; a.all = to_end; a.factor = p.scale;
-        a.vec = paired(p.x_dtype, q, p.dim_k) && paired(p.x_dtype, dout, p.dim_v);
+        a.a = f.q; a.b = f.dout; a.from_start = 1; a.all = to_end; a.factor = p.scale;
         st = launch_linear_states(p, w, a, stream);
         if (st != CC1D_OK) return st;
     }
@@ -255,30 +311,31 @@ int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t 
         if (st != CC1D_OK) return st;
     }
     AttendArgs a = {};                                   // dq
-    a.x = dout; a.y = v; a.z = k; a.u = q;
+    a.x = f.dout; a.y = f.v; a.z = f.k; a.u = f.q;
     a.d1 = p.dim_v; a.d2 = p.dim_k;
     a.state = w.first;
     a.first = initial;
-    a.out = bp.dq; a.out_b = bp.dq_stride_b; a.out_l = bp.dq_stride_l; a.out_h = bp.dq_stride_h;
+    set_out(a, f.dq);
     a.share = w.share_q; a.dots = w.dot_q;
     st = attend(p, w, a, false, true, stream);
     if (st != CC1D_OK) return st;
-    a.x = v; a.y = dout; a.z = q; a.u = k;               // dk
+    a.x = f.v; a.y = f.dout; a.z = f.q; a.u = f.k;       // dk
     a.state = w.by_v;
     a.first = bp.dfinal_states != nullptr;
-    a.out = bp.dk; a.out_b = bp.dk_stride_b; a.out_l = bp.dk_stride_l; a.out_h = bp.dk_stride_h;
+    set_out(a, f.dk);
     a.share = w.share_k; a.dots = w.dot_k;
     st = attend(p, w, a, true, true, stream);
     if (st != CC1D_OK) return st;
     AttendArgs d = {};                                   // dv
-    d.x = k; d.y = q; d.z = dout;
+    d.x = f.k; d.y = f.q; d.z = f.dout;
     d.d1 = p.dim_k; d.d2 = p.dim_v;
     d.state = w.by_k;
     d.first = bp.dfinal_states != nullptr;
-    d.out = bp.dv; d.out_b = bp.dv_stride_b; d.out_l = bp.dv_stride_l; d.out_h = bp.dv_stride_h;
+    set_out(d, f.dv);
     st = attend(p, w, d, true, false, stream);
     if (st == CC1D_OK) st = launch_linear_gates(bp, w, stream);
     if (st == CC1D_OK && w.shares > 1 && w.slots > 0) st = launch_linear_join(bp, w, stream);
+    if (st == CC1D_OK) st = launch_linear_copy(f.back, f.backs, true, stream);
     return st;
 }
 
@@ -300,8 +357,9 @@ int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     const Way way = st == CC1D_OK ? way_of(*p) : Way::tokens;
     if (way == Way::tokens) return st;
     SegmentWork w;
-    *bytes = lay_out_fwd(*p, way == Way::both, nullptr, w);
-    return grids_fit(*p, w) && reachable_out(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    Forward f;
+    *bytes = lay_out_fwd(*p, way == Way::both, nullptr, w, f);
+    return grids_fit(*p, w) && reachable_out(*p) && (f.ins + f.backs == 0 || copies_reachable(*p)) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
@@ -327,8 +385,9 @@ int cc1d_linear_fwd(const cc1d_delta_params *p, void *workspace, size_t workspac
     const Way way = way_of(*p);
     if (way == Way::tokens) return launch_delta_tokens(*p, nullptr, p->sequences, 0, hs, false);
     SegmentWork w;
-    lay_out_fwd(*p, way == Way::both, static_cast<uint8_t *>(workspace), w);
-    const int done = forward(*p, w, hs);
+    Forward f;
+    lay_out_fwd(*p, way == Way::both, static_cast<uint8_t *>(workspace), w, f);
+    const int done = forward(*p, w, f, hs);
     return done != CC1D_OK || way == Way::segments ? done : launch_delta_tokens(*p, nullptr, p->sequences, w.shortest, hs, false);
 }
 
@@ -347,8 +406,9 @@ int cc1d_linear_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *byte
     const int st = cc1d_validate_linear_bwd(p);
     if (st != CC1D_OK || p->fwd.batch == 0 || p->fwd.v_heads == 0 || p->fwd.sequences == 0) return st;
     SegmentWork w;
-    *bytes = lay_out_bwd(*p, nullptr, w);
-    return grids_fit(p->fwd, w) && reachable_gradients(*p) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    Backward f;
+    *bytes = lay_out_bwd(*p, nullptr, w, f);
+    return grids_fit(p->fwd, w) && reachable_gradients(*p) && (f.ins + f.backs == 0 || copies_reachable(p->fwd)) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_linear_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {
@@ -360,8 +420,9 @@ int cc1d_linear_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t work
     if (p->fwd.v_heads == 0) return launch_delta_no_values(*p, hs);
     if (p->fwd.batch == 0 || p->fwd.sequences == 0) return CC1D_OK;
     SegmentWork w;
-    lay_out_bwd(*p, static_cast<uint8_t *>(workspace), w);
-    return backward(*p, w, hs);
+    Backward f;
+    lay_out_bwd(*p, static_cast<uint8_t *>(workspace), w, f);
+    return backward(*p, w, f, hs);
 }
 
 int cc1d_validate_linear_step(const cc1d_delta_step_params *p) {

@@ -51,11 +51,11 @@ __device__ __forceinline__ void products_left(const bf16x8 (&a)[N][NA], const bf
 }
 
 // Wavefronts a SIMD that the registers leave: two where nothing has to be kept in memory for that.
-constexpr int attend_waves(int dt, bool dots, bool vec) { return !dots && (vec || dt != CC1D_F32) ? 2 : 1; }
+constexpr int attend_waves(bool dots) { return dots ? 1 : 2; }
 
 // KS: 32-column steps of x and y at once (their LDS); wider ones pass slab by slab.
-template <int DT, int KS, int RT, int CP, bool REV, bool DOTS, bool VEC>
-__global__ void __launch_bounds__(kBlock, attend_waves(DT, DOTS, VEC))
+template <int DT, int KS, int RT, int CP, bool REV, bool DOTS>
+__global__ void __launch_bounds__(kBlock, attend_waves(DOTS))
 linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n, PT = DOTS ? 3 : out_terms(DT), MOST = PT - 1;
@@ -125,7 +125,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
         const uint32_t z_pitch = (uint32_t)(a.z.sl * (int64_t)sizeof(T));
         auto token = [&](int t) { return t < at.count ? t : at.count - 1; };       // (rows behind the last weigh nothing, or are not stored)
 
-        Row8<DT, VEC> yr[KS];
+        Row8<DT, true> yr[KS];
         auto ask_y = [&](int c, int slab) {
             const T *row = yb + (int64_t)token(c * kChunk + row_of(wave, m)) * a.y.sl;
 #pragma unroll
@@ -133,7 +133,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
         };
         auto stage_x = [&](int slab) {                   // 16 rows a wavefront
             const T *row = xb + (int64_t)token(row0 + 16 * wave + m) * a.x.sl;
-            Row8<DT, VEC> xr[KS];
+            Row8<DT, true> xr[KS];
 #pragma unroll
             for (int s = 0; s < KS; ++s) xr[s].ask(row, 32 * (slab * KS + s) + 8 * g, a.d1);
 #pragma unroll
@@ -243,7 +243,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
             of_x[t] = turns > 1 ? (REV ? decay_between(lds.gates, i, border) : decay_between(lds.gates, border, i)) : 0.f;
         }
 
-        Pair8<DT, VEC> zr[CP][2];
+        Pair8<DT> zr[CP][2];
         auto ask_z = [&](int block, int s) {
             uint32_t off[8];
 #pragma unroll
@@ -398,7 +398,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
     }
 
     // Rows leave as column pairs.
-    auto leave = [&](auto *to, uint32_t pitch, auto type, auto vec) {  // the block's first row, bytes between rows
+    auto leave = [&](auto *to, uint32_t pitch, auto type) {  // the block's first row, bytes between rows
         using E = std::remove_pointer_t<decltype(to)>;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -414,18 +414,16 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
                     float o0, o1;
                     if constexpr (DOTS) { o0 = total[i][c][0][e]; o1 = total[i][c][1][e]; }
                     else { o0 = s[e] * acc[i][c][0][e]; o1 = s[e] * acc[i][c][1][e]; }
-                    store_pair<decltype(type)::value, decltype(vec)::value>(at_row, 32 * (pair0 + 4 * c) + 2 * m, a.d2, o0, o1);
+                    store_pair<decltype(type)::value>(at_row, 32 * (pair0 + 4 * c) + 2 * m, a.d2, o0, o1);
                 }
             }
         }
     };
     const int64_t tok = at.lo + row0;
     if (!DOTS || a.share == nullptr)
-        leave(static_cast<T *>(a.out) + at.b * a.out_b + tok * a.out_l + out_head * a.out_h, (uint32_t)(a.out_l * (int64_t)sizeof(T)), std::integral_constant<int, DT>(),
-              std::bool_constant<VEC>());
+        leave(static_cast<T *>(a.out) + at.b * a.out_b + tok * a.out_l + out_head * a.out_h, (uint32_t)(a.out_l * (int64_t)sizeof(T)), std::integral_constant<int, DT>());
     else
-        leave(a.share + ((((int64_t)share * p.batch + at.b) * p.seqlen + tok) * p.heads + hk) * a.d2, (uint32_t)p.heads * (uint32_t)a.d2 * 4u, std::integral_constant<int, CC1D_F32>(),
-              std::false_type());
+        leave(a.share + ((((int64_t)share * p.batch + at.b) * p.seqlen + tok) * p.heads + hk) * a.d2, (uint32_t)p.heads * (uint32_t)a.d2 * 4u, std::integral_constant<int, CC1D_F32>());
 }
 
 }  // namespace cc1d

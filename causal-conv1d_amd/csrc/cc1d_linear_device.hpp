@@ -44,36 +44,22 @@ __device__ __forceinline__ float decay_since_start(const GateLds &lds, int to) {
 // Columns c, c + 1 (`c` even) of eight rows: the right operand of two result tiles, whose columns are the even and the odd ones of
 // 32, so that a lane loads both with one access and stores both of its results with one.  Eight consecutive rows of one column are what
 // the matrix instruction wants of a lane, and no 16-bit element has to cross lanes for it.
-template <int DT, bool VEC>
+template <int DT>
 struct Pair8 {
     static constexpr int W = DT == CC1D_F32 ? 2 : 1;
     uint32_t r[8][W];
     // at[i]: byte offset of row i from base; columns that are not there repeat the first.
     __device__ __forceinline__ void ask(const void *base, const uint32_t (&at)[8], int c, int cols) {
         const uint8_t *b = static_cast<const uint8_t *>(base);
-        if constexpr (VEC) {
-            const uint32_t o = (c < cols ? c : 0) * (uint32_t)(DT == CC1D_F32 ? 4 : 2);
+        const uint32_t o = (c < cols ? c : 0) * (uint32_t)(DT == CC1D_F32 ? 4 : 2);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (DT == CC1D_F32) {
-                    const u32x2 v = *reinterpret_cast<const u32x2 *>(b + (at[i] + o));
-                    r[i][0] = v.x;
-                    r[i][W - 1] = v.y;
-                } else {
-                    r[i][0] = *reinterpret_cast<const uint32_t *>(b + (at[i] + o));
-                }
-            }
-        } else {
-            const uint32_t o0 = c < cols ? c : 0, o1 = c + 1 < cols ? c + 1 : 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (DT == CC1D_F32) {
-                    r[i][0] = *reinterpret_cast<const uint32_t *>(b + (at[i] + o0 * 4));
-                    r[i][W - 1] = *reinterpret_cast<const uint32_t *>(b + (at[i] + o1 * 4));
-                } else {
-                    r[i][0] = (uint32_t)*reinterpret_cast<const uint16_t *>(b + (at[i] + o0 * 2)) |
-                              (uint32_t)*reinterpret_cast<const uint16_t *>(b + (at[i] + o1 * 2)) << 16;
-                }
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (DT == CC1D_F32) {
+                const u32x2 v = *reinterpret_cast<const u32x2 *>(b + (at[i] + o));
+                r[i][0] = v.x;
+                r[i][W - 1] = v.y;
+            } else {
+                r[i][0] = *reinterpret_cast<const uint32_t *>(b + (at[i] + o));
             }
         }
     }
@@ -105,24 +91,19 @@ struct Pair8 {
 };
 
 // Two adjacent results to columns c, c + 1 of a row.
-template <int DT, bool VEC>
+template <int DT>
 __device__ __forceinline__ void store_pair(typename Elem<DT>::type *row, int c, int cols, float a, float b) {
-    if constexpr (VEC) {
-        if (c >= cols) return;
-        if constexpr (DT == CC1D_F32) {
-            *reinterpret_cast<float2 *>(row + c) = make_float2(a, b);
-        } else if constexpr (DT == CC1D_F16) {
-            asm("" : "+v"(a), "+v"(b));  // (no fused multiply that rounds to fp16 in one step)
-            f16x2 h;
-            h.x = (_Float16)a;
-            h.y = (_Float16)b;
-            *reinterpret_cast<uint32_t *>(row + c) = bitcast<uint32_t>(h);
-        } else {
-            *reinterpret_cast<uint32_t *>(row + c) = rounded_pair(a, b);
-        }
+    if (c >= cols) return;
+    if constexpr (DT == CC1D_F32) {
+        *reinterpret_cast<float2 *>(row + c) = make_float2(a, b);
+    } else if constexpr (DT == CC1D_F16) {
+        asm("" : "+v"(a), "+v"(b));      // (no fused multiply that rounds to fp16 in one step)
+        f16x2 h;
+        h.x = (_Float16)a;
+        h.y = (_Float16)b;
+        *reinterpret_cast<uint32_t *>(row + c) = bitcast<uint32_t>(h);
     } else {
-        if (c < cols) row[c] = Elem<DT>::from_float(a);
-        if (c + 1 < cols) row[c + 1] = Elem<DT>::from_float(b);
+        *reinterpret_cast<uint32_t *>(row + c) = rounded_pair(a, b);
     }
 }
 

@@ -11,7 +11,7 @@ namespace {
 // terms then; a stays as it is, one term in bfloat16.  No operand goes through LDS: pairs of columns (Pair8) are loaded in the order
 // of the matrix instruction, and the result tiles of a pair of a's are eight consecutive rows of a lane, the operand order of the next product.
 // KT: 32-column steps of a that a wavefront takes.
-template <int DT, int KT, bool VEC>
+template <int DT, int KT>
 __global__ void __launch_bounds__(kBlock, KT <= 4 && DT != CC1D_F32 ? 2 : 1)
 linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const StatesArgs a, const int halves, const uint32_t col_tiles) {
     using T = typename Elem<DT>::type;
@@ -45,7 +45,7 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
     for (int i = 0; i < KT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][e >> 1][e & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Pair8<DT, VEC> ra[KT], rb;
+    Pair8<DT> ra[KT], rb;
     auto ask = [&](int t0) {             // 32 tokens from t0 on; those behind the last take its rows, and their weight is 0
         uint32_t at_a[8], at_b[8];
 #pragma unroll
@@ -103,6 +103,36 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
                     f[2 * e + n] = 32 * (p0 + i) + 8 * g + 2 * e + n < p.dim_k && cb + c < p.dim_v ? acc[i][n][c][e] : 0.f;
             *reinterpret_cast<float4 *>(to + c * 512) = make_float4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<float4 *>(to + c * 512 + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        }
+    }
+}
+
+// Rows to whole vectors and back, a wavefront a token of one tensor: bound by memory.
+template <typename E, bool OUT>
+__global__ void __launch_bounds__(kBlock)
+linear_copy_kernel(const CopyArgs a, const int64_t tokens) {
+    const CopyRows &c = a.of[blockIdx.y];
+    struct alignas(16) Vector { E e[kVector]; };
+    const int lane = threadIdx.x & 63, vectors = padded(c.dim) / kVector;
+    for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < tokens; t += (int64_t)gridDim.x * 4) {
+        const int64_t b = divided((uint32_t)t, a.by_seqlen), l = t - b * a.seqlen;
+        const uint8_t *from = c.from + b * c.from_b + l * c.from_l;
+        uint8_t *to = c.to + b * c.to_b + l * c.to_l;
+        for (int i = lane; i < c.heads * vectors; i += 64) {
+            const int h = (int)divided((uint32_t)i, c.by_vectors), col = (i - h * vectors) * kVector;
+            const E *x = reinterpret_cast<const E *>(from + h * c.from_h) + col;
+            E *y = reinterpret_cast<E *>(to + h * c.to_h) + col;
+            if constexpr (OUT) {
+                const Vector v = *reinterpret_cast<const Vector *>(x);
+#pragma unroll
+                for (int k = 0; k < kVector; ++k)
+                    if (col + k < c.dim) y[k] = v.e[k];
+            } else {
+                Vector v;
+#pragma unroll
+                for (int k = 0; k < kVector; ++k) v.e[k] = col + k < c.dim ? x[k] : (E)0;
+                *reinterpret_cast<Vector *>(y) = v;
+            }
         }
     }
 }
@@ -299,15 +329,16 @@ __global__ void __launch_bounds__(kBlock)
 linear_join_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const int64_t rows) {
     using T = typename Elem<DT>::type;
     const cc1d_delta_params &p = bp.fwd;
-    const int64_t plane = rows * p.dim_k;
+    const int pitch = padded(p.dim_k);
+    const int64_t plane = rows * pitch;
     for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
         const int64_t t = r / p.heads, b = t / p.seqlen;
         const int hk = (int)(r - t * p.heads);
         for (int k = threadIdx.x & 63; k < p.dim_k; k += 64) {
             float dq = 0.f, dk = 0.f;
             for (int i = 0; i < w.shares; ++i) {
-                dq += w.share_q[i * plane + r * p.dim_k + k];
-                dk += w.share_k[i * plane + r * p.dim_k + k];
+                dq += w.share_q[i * plane + r * pitch + k];
+                dk += w.share_k[i * plane + r * pitch + k];
             }
             static_cast<T *>(bp.dq)[b * bp.dq_stride_b + (t - b * p.seqlen) * bp.dq_stride_l + hk * bp.dq_stride_h + k] = Elem<DT>::from_float(dq);
             static_cast<T *>(bp.dk)[b * bp.dk_stride_b + (t - b * p.seqlen) * bp.dk_stride_l + hk * bp.dk_stride_h + k] = Elem<DT>::from_float(dk);
@@ -322,8 +353,7 @@ int launch_states(const cc1d_delta_params &p, const SegmentWork &w, const States
     const dim3 grid((uint32_t)w.slots * (uint32_t)p.v_heads * col_tiles);
     auto go = [&](auto kt) {
         constexpr int KT = decltype(kt)::value;
-        if (a.vec) CC1D_LAUNCH((linear_states_kernel<DT, KT, true>), grid, dim3(kBlock), 0, stream, p, w, a, halves, col_tiles);
-        else CC1D_LAUNCH((linear_states_kernel<DT, KT, false>), grid, dim3(kBlock), 0, stream, p, w, a, halves, col_tiles);
+        CC1D_LAUNCH((linear_states_kernel<DT, KT>), grid, dim3(kBlock), 0, stream, p, w, a, halves, col_tiles);
         return launch_status();
     };
     return each <= 1 ? go(std::integral_constant<int, 1>()) : each <= 2 ? go(std::integral_constant<int, 2>()) :
@@ -332,6 +362,18 @@ int launch_states(const cc1d_delta_params &p, const SegmentWork &w, const States
 
 }  // namespace
 
+int launch_linear_copy(const CopyArgs &a, int copies, bool out, hipStream_t stream) {
+    const int64_t tokens = (int64_t)a.batch * a.seqlen, blocks = (tokens + 3) / 4;
+    if (tokens == 0 || copies == 0) return CC1D_OK;
+    const dim3 grid((uint32_t)(blocks < 16384 ? blocks : 16384), (uint32_t)copies);
+    auto go = [&](auto e) {
+        using E = decltype(e);
+        if (out) CC1D_LAUNCH((linear_copy_kernel<E, true>), grid, dim3(kBlock), 0, stream, a, tokens);
+        else CC1D_LAUNCH((linear_copy_kernel<E, false>), grid, dim3(kBlock), 0, stream, a, tokens);
+        return launch_status();
+    };
+    return a.elem == 4 ? go(uint32_t()) : go(uint16_t());
+}
 int launch_linear_states(const cc1d_delta_params &p, const SegmentWork &w, const StatesArgs &a, hipStream_t stream) {
     if (w.slots == 0) return CC1D_OK;
     switch (p.x_dtype) {

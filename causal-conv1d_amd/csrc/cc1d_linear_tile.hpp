@@ -518,14 +518,14 @@ int launch_tile(const cc1d_delta_params &p, const SegmentWork &w, const AttendAr
 }
 
 template <int DT, bool REV, bool DOTS>
-int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, bool vec, hipStream_t stream) {
+int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, hipStream_t stream) {
     if constexpr (DT != CC1D_F32)
         if (a.tile != 0) return launch_tile<DT, REV, DOTS>(p, w, a, stream);
     const dim3 grid((a.items + 7) / 8 * 8 * kBlocks * a.col_tiles);
-    auto go = [&](auto ks, auto rt, auto cp, auto v) {
+    auto go = [&](auto ks, auto rt, auto cp) {
         constexpr int KS = decltype(ks)::value, RT = decltype(rt)::value, CP = decltype(cp)::value;
         constexpr size_t lds = sizeof(AttendLds<DT, KS, DOTS ? 3 : out_terms(DT)>);
-        CC1D_LAUNCH((linear_attend_kernel<DT, KS, RT, CP, REV, DOTS, decltype(v)::value>), grid, dim3(kBlock), lds, stream, p, w, a);
+        CC1D_LAUNCH((linear_attend_kernel<DT, KS, RT, CP, REV, DOTS>), grid, dim3(kBlock), lds, stream, p, w, a);
         return launch_status();
     };
     using I1 = std::integral_constant<int, 1>;
@@ -533,11 +533,16 @@ int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const Attend
     using I4 = std::integral_constant<int, 4>;
     auto by_columns = [&](auto ks) {
         if constexpr (DOTS)
-            if (a.d2 > 128) return vec ? go(ks, I4(), I2(), std::true_type()) : go(ks, I4(), I2(), std::false_type());
-        if (!vec) return go(ks, I4(), I1(), std::false_type());
-        return a.d2 <= 64 ? go(ks, I2(), I1(), std::true_type()) : go(ks, I4(), I1(), std::true_type());
+            if (a.d2 > 128) return go(ks, I4(), I2());
+        return a.d2 <= 64 ? go(ks, I2(), I1()) : go(ks, I4(), I1());
     };
-    return a.steps <= 2 ? by_columns(I2()) : by_columns(I4());
+    if constexpr (DT == CC1D_F32) {
+        return a.steps <= 2 ? by_columns(I2()) : by_columns(I4());
+    } else {                             // (more than 128 columns of x, or, of the gradients of q and k, of z)
+        if constexpr (DOTS)
+            if (a.steps <= 2) return go(I2(), I4(), I2());
+        return by_columns(I4());
+    }
 }
 
 }  // namespace cc1d
