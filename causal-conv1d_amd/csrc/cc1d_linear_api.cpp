@@ -44,16 +44,21 @@ bool reachable_gradients(const cc1d_delta_bwd_params &bp) {
     return reachable(bp.fwd) && near(bp.fwd, bp.dout_stride_l) && near(bp.fwd, bp.dq_stride_l) && near(bp.fwd, bp.dk_stride_l) && near(bp.fwd, bp.dv_stride_l);
 }
 
-// Sequences of this many tokens on average go by segments; `saved`: all do.  A token takes 1 us until the states of 512 heads of 128 x 128 (or as
-// many elements of other heads) fill the card, then time by their number, and segments cost by it from the start.  By tokens and by
-// segments: 16-bit types, 4 heads: 16 tokens 21 us and 20, 32 tokens 37 and 21; 256 heads: 32 tokens 40 and 36; 1024 heads: 64 tokens 162 and 136.
-// fp32, whose products take six matrix instructions for one to three: 4 heads: 24 tokens 27 and 27; 256 heads: 64 tokens 66 and 86, 128 tokens 123 and 109;
-// 512 heads: 512 tokens 582 and 632; 1024 heads: 1024 tokens 2126 and 2470.
+// Sequences of this many tokens on average go by segments; `saved`: all do.  A token takes 0.7 to 1 us until the states of 512 heads of 128 x 128 (or as
+// many elements of other heads) fill the card, then time by their number; a segment costs by heads and by their elements.  By tokens and
+// by segments, us: 16-bit types, 128 x 128, 4 heads: 16 tokens 21 and 20; 256: 24 tokens 31 and 36, 32 tokens 39 and 36; 1024: 48 tokens 127 and 135,
+// 64 tokens 162 and 138; 32 x 32, 1024 heads: 32 tokens 28 and 29; 2880: 64 tokens 80 and 82.  float32, whose products take six matrix instructions for
+// one to three, 128 x 128, 4 heads: 24 tokens 27 and 24; 256: 48 tokens 51 and 60, 64 tokens 66 and 61; 512: 96 tokens 116 and 132, 128 tokens 150 and 140;
+// 1024: 128 tokens 267 and 298, 256 tokens 540 and 420; 32 x 32, 2880 heads: 512 tokens 569 and 968.
 int64_t segments_from(const cc1d_delta_params &p, int64_t sequences) {
-    const double all = (double)sequences * p.v_heads * p.dim_k * p.dim_v / 16384.0;
-    const int64_t heads = all < 1024.0 ? (int64_t)all : 1024;
-    if (p.x_dtype == CC1D_F32) return heads >= 512 ? INT32_MAX : 22 + heads / 5;
-    return heads >= 960 ? 64 : 16 + heads / 20;
+    const double heads = (double)sequences * p.v_heads, size = (double)p.dim_k * p.dim_v / 16384.0, most = heads < 1e6 ? heads : 1e6;
+    if (p.x_dtype == CC1D_F32) {
+        if (heads >= 2048.0 && size <= 0.25) return INT32_MAX;
+        const int64_t from = 22 + (int64_t)(most * (0.05 + 0.14 * size));
+        return from < 170 ? from : 170;
+    }
+    const int64_t from = 16 + (int64_t)(most * (0.016 + 0.03 * size)), cap = heads * size >= 512.0 ? 50 : 96;
+    return from < cap ? from : cap;
 }
 // The average says nothing of the longest.  Packed sequences that go by tokens on average go by segments one by one, from 256 tokens on: the
 // kernels see their lengths, the host does not.  Not where all their tokens together are few, nor where one sequence's heads fill

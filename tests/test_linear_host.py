@@ -153,9 +153,9 @@ def test_ways_of_a_call(lib):
         return n.value > 0
     b16, f32 = torch.bfloat16, torch.float32
     for args, want in (((1, 15, 4, 64, b16), False), ((1, 16, 4, 64, b16), True), ((1, 21, 4, 64, f32), False), ((1, 22, 4, 64, f32), True),
-                       ((16, 63, 64, 128, b16), False), ((16, 64, 64, 128, b16), True), ((16, 5000, 64, 128, f32), False), ((1, 160, 4, 64, b16, 10), True),
-                       ((1, 159, 4, 64, b16, 10), False), ((1, 511, 4, 64, b16, 40), False), ((1, 512, 4, 64, b16, 40), True), ((1, 512, 4, 64, f32, 40), True),
-                       ((1, 2000, 512, 128, f32, 40), False)):
+                       ((16, 49, 64, 128, b16), False), ((16, 50, 64, 128, b16), True), ((16, 169, 64, 128, f32), False), ((16, 170, 64, 128, f32), True),
+                       ((32, 5000, 64, 32, f32), False), ((1, 160, 4, 64, b16, 10), True), ((1, 159, 4, 64, b16, 10), False), ((1, 511, 4, 64, b16, 40), False),
+                       ((1, 512, 4, 64, b16, 40), True), ((1, 512, 4, 64, f32, 40), True), ((1, 2000, 2048, 32, f32, 40), False)):
         assert wants(*args) == want, args
 
 

@@ -44,9 +44,9 @@ def test_each_by_its_own_length(pkg, gpu_device, name, dtype, front, behind):
         cases.check({"out": torch.cat([out[:, edges[i]:edges[i] + n] for i in which]), "final": final[which]}, part, grads=False)
 
 
-@pytest.mark.parametrize("dtype,batch,v_heads,seqlen", [(FP32, 4, 128, 40), (BF16, 8, 128, 63), (BF16, 8, 128, 64)])
+@pytest.mark.parametrize("dtype,batch,v_heads,seqlen", [(FP32, 4, 128, 40), (FP32, 2, 256, 120), (BF16, 8, 128, 49), (BF16, 8, 128, 50)])
 def test_many_heads(pkg, gpu_device, dtype, batch, v_heads, seqlen):
-    """States that fill the card: in float32 by tokens whatever the length, in 16 bits from 64 tokens on by segments."""
+    """States that fill the card, by tokens and by segments."""
     s = cases.inputs(gpu_device, batch, seqlen, 2, v_heads, 128, 128, dtype)
     cases.check(cases.run(pkg, s, grads=False), s, grads=False)
 
@@ -321,3 +321,43 @@ def test_together_in_training_and_in_a_decode_loop(pkg, gpu_device):
         both = torch.cat([head, torch.stack(tails, 1)], 1)
     assert (both - out).abs().max() <= 1000 * 2.0 ** -24 * 4 * out.abs().max()
     assert (state - final).abs().max() <= 1000 * 2.0 ** -24 * 4 * final.abs().max()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("cu", [None, [3, 200, 200, 280, 340]])
+def test_rows_that_are_no_whole_vectors(pkg, gpu_device, dtype, cu):
+    """Each tensor on its own at an odd address, with an odd stride or with a column more, in both directions: the bits of aligned copies; and what
+    surrounds them is left alone."""
+    s = cases.inputs(gpu_device, 1 if cu else 2, 340, 1, 2, 32, 64, dtype, sequences=len(cu) - 1 if cu else 0, slices=False)
+    want = cases.run(pkg, s, cu)
+
+    def moved(t, how):
+        shape = list(t.shape)
+        if how == "address":
+            room = torch.full((t.numel() + 1,), 7.0, device=gpu_device, dtype=t.dtype)
+            view = room[1:].view(shape)
+        elif how == "stride":
+            room = torch.full((shape[0], shape[1], shape[2] * shape[3] + 3), 7.0, device=gpu_device, dtype=t.dtype)
+            view = room[..., :-3].unflatten(-1, shape[2:])
+        else:
+            room = torch.full(shape[:3] + [shape[3] + 1], 7.0, device=gpu_device, dtype=t.dtype)
+            view = room[..., :-1]
+        view.copy_(t)
+        return room, view
+    for how in ("address", "stride", "column"):
+        for names in (["q"], ["k"], ["v"], ["dout"], ["q", "k", "v", "dout"]):
+            rooms = {n: moved(s[n], how) for n in names}
+            before = {n: r[0].clone() for n, r in rooms.items()}
+            got = cases.run(pkg, dict(s, **{n: r[1] for n, r in rooms.items()}), cu)
+            for n in want:
+                assert torch.equal(got[n], want[n]), (how, names, n)
+            for n in names:
+                assert torch.equal(rooms[n][0], before[n])
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("dims", [(100, 100), (41, 32), (154, 80), (128, 63), (130, 260), (7, 250)])
+def test_odd_sizes_of_many_segments(pkg, gpu_device, dtype, dims):
+    """More than one segment, shared key heads, states: each size's rows end inside a vector."""
+    s = cases.inputs(gpu_device, 2, 530, 1, 3, *dims, dtype, slices=False)
+    cases.check(cases.run(pkg, s), s)
