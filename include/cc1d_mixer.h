@@ -1,7 +1,8 @@
 /*
  * cc1d_mixer.h — C ABI of the operators that stand next to the causal convolution in a
- * linear-attention mixer: the gated delta rule (chunked forward and backward, recurrent step) and the
- * root-mean-square norm with the residual's addition (forward, backward, output in 8 bits).
+ * linear-attention mixer: the gated delta rule and linear attention with a decay for each head (each forward and backward
+ * over sequences, recurrent step), the root-mean-square norm (forward, backward, output in 8 bits) and the layer norm (forward, backward),
+ * both with the residual's addition.
  * No counterpart in Dao-AILab/causal-conv1d.
  *
  * Conventions are those of cc1d.h: raw device pointers, element strides as int64_t, sizes as int32_t,
@@ -139,12 +140,13 @@ int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
  * (dbeta is then not written, beta_dtype not read).  Strides of 0 make a gate one number a head.  qk_l2norm has to be 0 (CC1D_ERR_OPTION).
  * `saved` is of cc1d_linear_saved_bytes() here: the state in front of every 256 tokens.
  *
- * Short sequences go token by token, the others in segments of 256 tokens, each worked out in blocks of 64: a NaN or infinity reaches its
+ * Short sequences go token by token, packed ones each by its own length; the others in segments of 256 tokens, worked out in blocks of 64: a NaN or infinity reaches its
  * head's outputs from the start of its 64 tokens on.  Gates are bounded from below by -200, which forgets everything.  Where they
  * are positive, the states may grow by less than 2^128 over 256 tokens.
  * Precision is the gated delta rule's; the factors that make out and dv of 16 bits carry 2^-17.
  * Tokens 2^23 bytes apart or more (in q, k, v or out) go by tokens in the forward; there, with `saved`, and in the backward (in q, k, v, dout or their
- * gradients) they are refused with CC1D_ERR_TOO_LARGE.
+ * gradients) they are refused with CC1D_ERR_TOO_LARGE.  Tensors whose rows are not whole 16-byte vectors of 8 columns are copied to the
+ * workspace, whose size is therefore of these pointers and strides; it is refused where v_heads such rows take 2^23 bytes.
  * ---------------------------------------------------------------------------------- */
 int cc1d_validate_linear(const cc1d_delta_params *p);
 int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes);
