@@ -43,7 +43,7 @@ KERNEL_SOURCES = [
     "cc1d_delta_bwd.hip",
     "cc1d_linear_api.cpp",
     "cc1d_linear_states.hip",
-] + ["cc1d_linear_%s_%s.hip" % (what, dtype) for what in ("out", "dq", "dk", "dv") for dtype in ("bf16", "f16", "f32")] + [
+] + ["cc1d_linear_%s_%s.hip" % (what, dtype) for what in ("out", "dqk", "dv") for dtype in ("bf16", "f16", "f32")] + [
     "cc1d_norm.hip",
     "cc1d_layer_norm.hip",
 ]

@@ -5,11 +5,10 @@
 
 namespace cc1d {
 
-#define CC1D_ATTEND(DT)                                                                                                                          \
-    extern template int launch_attend<DT, false, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);   \
-    extern template int launch_attend<DT, true, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);    \
-    extern template int launch_attend<DT, false, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);    \
-    extern template int launch_attend<DT, true, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);
+#define CC1D_ATTEND(DT)                                                                                                                   \
+    extern template int launch_attend<DT, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);     \
+    extern template int launch_attend<DT, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);      \
+    extern template int launch_attend_pair<DT>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, const AttendArgs &, hipStream_t);
 CC1D_ATTEND(CC1D_F32)
 CC1D_ATTEND(CC1D_F16)
 CC1D_ATTEND(CC1D_BF16)
@@ -107,9 +106,10 @@ size_t state_tiles(const cc1d_delta_params &p, const SegmentWork &w) { return (s
 size_t by_k_bytes(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.kp * w.k_tiles * out_terms(p.x_dtype) * kFrag; }
 size_t by_v_bytes(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.vp * w.v_tiles * 3 * kFrag; }
 
-// One workgroup a (slot, block, value head, 128 columns) and less; the scan's one wavefront a tile of each sequence's states.
-bool grids_fit(const cc1d_delta_params &p, const SegmentWork &w) {
-    return ((int64_t)w.slots * p.v_heads + 8) * kBlocks * ((w.vp + 3) / 4) < thread_limit() / kBlock &&
+// One workgroup a (slot, block, value head, 128 columns) and less, of two such products at once in the backward; the scan's one wavefront a tile of each
+// sequence's states.
+bool grids_fit(const cc1d_delta_params &p, const SegmentWork &w, int products) {
+    return ((int64_t)w.slots * p.v_heads + 8) * kBlocks * (products > (w.vp + 3) / 4 ? products : (w.vp + 3) / 4) < thread_limit() / kBlock &&
            w.walks(p) * p.v_heads * w.tiles() < thread_limit() / kWave;
 }
 
@@ -178,7 +178,7 @@ size_t lay_out_fwd(const cc1d_delta_params &p, bool alone, uint8_t *base, Segmen
 
 // Value heads that a workgroup takes one after the other, of `items` (slots and value heads): what belongs to their key head is read once for
 // all of them, and of the gradients of q and k, whose workgroups of a shared key head each write a share in fp32, that is less too; but
-// `workgroups` of them at least, one a CU (32 segments of 80 heads: out 112 us, with two 127; dq 192 and 207).  Not where z has more than 64 columns: out of 64
+// `workgroups` of them at least, one a CU (32 segments of 80 heads: out 112 us, with two 127).  Not where z has more than 64 columns: out of 64
 // segments of 16 heads of 128 x 128, float16, 118 us each for itself and 138 in pairs, whose registers spill.
 int heads_of_workgroup(int group, int64_t items, int workgroups) {
     const int64_t most = items / workgroups;
@@ -187,7 +187,7 @@ int heads_of_workgroup(int group, int64_t items, int workgroups) {
 }
 void share_heads(const cc1d_delta_params &p, SegmentWork &w) {
     const int group = p.v_heads / p.heads;
-    w.heads_each = heads_of_workgroup(group, (int64_t)w.slots * p.v_heads * (w.v_width > 2 ? 1 : kBlocks), 256);
+    w.heads_each = heads_of_workgroup(group, (int64_t)w.slots * p.v_heads * (w.v_width > 2 ? 1 : kBlocks), 128);
     w.shares = (group + w.heads_each - 1) / w.heads_each;
 }
 bool gradient_of_states(const cc1d_delta_bwd_params &bp, const SegmentWork &w) {
@@ -231,8 +231,7 @@ size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &
     return work.used;
 }
 
-int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool rev, bool dots, hipStream_t stream) {
-    if (w.slots == 0) return CC1D_OK;
+AttendArgs prepared(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool dots) {
     a.group = p.v_heads / p.heads;
     a.d1 = padded(a.d1);
     a.d2 = padded(a.d2);
@@ -240,23 +239,34 @@ int attend(const cc1d_delta_params &p, const SegmentWork &w, AttendArgs a, bool 
     a.width = dots ? w.v_width : w.k_width;
     a.tiles = dots ? w.v_tiles : w.k_tiles;
     a.tile = a.width > 2;
-    a.heads_each = dots ? w.heads_each : a.tile && a.width == 4 ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads, 256) : 1;
+    a.heads_each = dots ? w.heads_each : a.width == 4 ? heads_of_workgroup(a.group, (int64_t)w.slots * p.v_heads, 256) : 1;
     a.shares = (a.group + a.heads_each - 1) / a.heads_each;
     a.items = (uint32_t)w.slots * (uint32_t)p.heads * (uint32_t)a.shares;
-    a.col_tiles = dots ? 1u : (uint32_t)(a.d2 + 127) / 128;
+    a.col_tiles = dots ? 1u : (uint32_t)(a.d2 + (a.width == 4 ? 63 : 127)) / (a.width == 4 ? 64 : 128);
     a.by_col_tiles = fast_div(a.col_tiles);
     a.by_heads = fast_div((uint32_t)p.heads);
     a.by_shares = fast_div((uint32_t)a.shares);
-    auto of_type = [&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-        if (rev) return dots ? launch_attend<DT, true, true>(p, w, a, stream) : launch_attend<DT, true, false>(p, w, a, stream);
-        return dots ? launch_attend<DT, false, true>(p, w, a, stream) : launch_attend<DT, false, false>(p, w, a, stream);
-    };
+    return a;
+}
+template <typename F>
+int by_type(const cc1d_delta_params &p, F &&f) {
     switch (p.x_dtype) {
-        case CC1D_F32: return of_type(std::integral_constant<int, CC1D_F32>());
-        case CC1D_F16: return of_type(std::integral_constant<int, CC1D_F16>());
-        default: return of_type(std::integral_constant<int, CC1D_BF16>());
+        case CC1D_F32: return f(std::integral_constant<int, CC1D_F32>());
+        case CC1D_F16: return f(std::integral_constant<int, CC1D_F16>());
+        default: return f(std::integral_constant<int, CC1D_BF16>());
     }
+}
+int attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &given, bool rev, hipStream_t stream) {
+    if (w.slots == 0) return CC1D_OK;
+    const AttendArgs a = prepared(p, w, given, false);
+    return by_type(p, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return rev ? launch_attend<DT, true>(p, w, a, stream) : launch_attend<DT, false>(p, w, a, stream);
+    });
+}
+int attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &q, const AttendArgs &k, hipStream_t stream) {
+    if (w.slots == 0) return CC1D_OK;
+    return by_type(p, [&](auto dt) { return launch_attend_pair<decltype(dt)::value>(p, w, prepared(p, w, q, true), prepared(p, w, k, true), stream); });
 }
 
 void set_out(AttendArgs &a, const LinearRows &r) {
@@ -290,7 +300,7 @@ int forward(const cc1d_delta_params &p, const SegmentWork &w, const Forward &f, 
     a.state = w.by_k;
     a.first = p.initial_states != nullptr;
     set_out(a, f.out);
-    st = attend(p, w, a, false, false, stream);
+    st = attend(p, w, a, false, stream);
     return st != CC1D_OK ? st : launch_linear_copy(f.back, f.backs, true, stream);
 }
 
@@ -315,21 +325,20 @@ int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, const Backwa
         st = launch_linear_scan(p, w, a, stream);
         if (st != CC1D_OK) return st;
     }
-    AttendArgs a = {};                                   // dq
-    a.x = f.dout; a.y = f.v; a.z = f.k; a.u = f.q;
-    a.d1 = p.dim_v; a.d2 = p.dim_k;
-    a.state = w.first;
-    a.first = initial;
-    set_out(a, f.dq);
-    a.share = w.share_q; a.dots = w.dot_q;
-    st = attend(p, w, a, false, true, stream);
-    if (st != CC1D_OK) return st;
-    a.x = f.v; a.y = f.dout; a.z = f.q; a.u = f.k;       // dk
-    a.state = w.by_v;
-    a.first = bp.dfinal_states != nullptr;
-    set_out(a, f.dk);
-    a.share = w.share_k; a.dots = w.dot_k;
-    st = attend(p, w, a, true, true, stream);
+    AttendArgs dq = {}, dk = {};
+    dq.x = f.dout; dq.y = f.v; dq.z = f.k; dq.u = f.q;
+    dq.d1 = p.dim_v; dq.d2 = p.dim_k;
+    dq.state = w.first;
+    dq.first = initial;
+    set_out(dq, f.dq);
+    dq.share = w.share_q; dq.dots = w.dot_q;
+    dk.x = f.v; dk.y = f.dout; dk.z = f.q; dk.u = f.k;
+    dk.d1 = p.dim_v; dk.d2 = p.dim_k;
+    dk.state = w.by_v;
+    dk.first = bp.dfinal_states != nullptr;
+    set_out(dk, f.dk);
+    dk.share = w.share_k; dk.dots = w.dot_k;
+    st = attend_pair(p, w, dq, dk, stream);
     if (st != CC1D_OK) return st;
     AttendArgs d = {};                                   // dv
     d.x = f.k; d.y = f.q; d.z = f.dout;
@@ -337,7 +346,7 @@ int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, const Backwa
     d.state = w.by_k;
     d.first = bp.dfinal_states != nullptr;
     set_out(d, f.dv);
-    st = attend(p, w, d, true, false, stream);
+    st = attend(p, w, d, true, stream);
     if (st == CC1D_OK) st = launch_linear_gates(bp, w, stream);
     if (st == CC1D_OK && w.shares > 1 && w.slots > 0) st = launch_linear_join(bp, w, stream);
     if (st == CC1D_OK) st = launch_linear_copy(f.back, f.backs, true, stream);
@@ -364,7 +373,7 @@ int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     SegmentWork w;
     Forward f;
     *bytes = lay_out_fwd(*p, way == Way::both, nullptr, w, f);
-    return grids_fit(*p, w) && reachable_out(*p) && (f.ins + f.backs == 0 || copies_reachable(*p)) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    return grids_fit(*p, w, 1) && reachable_out(*p) && (f.ins + f.backs == 0 || copies_reachable(*p)) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
@@ -413,7 +422,7 @@ int cc1d_linear_bwd_workspace_bytes(const cc1d_delta_bwd_params *p, size_t *byte
     SegmentWork w;
     Backward f;
     *bytes = lay_out_bwd(*p, nullptr, w, f);
-    return grids_fit(p->fwd, w) && reachable_gradients(*p) && (f.ins + f.backs == 0 || copies_reachable(p->fwd)) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    return grids_fit(p->fwd, w, 2) && reachable_gradients(*p) && (f.ins + f.backs == 0 || copies_reachable(p->fwd)) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_linear_bwd(const cc1d_delta_bwd_params *p, void *workspace, size_t workspace_bytes, cc1d_stream_t stream) {

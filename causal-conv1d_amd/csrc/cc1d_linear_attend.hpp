@@ -59,8 +59,7 @@ constexpr int attend_waves(bool dots) { return dots ? 1 : 2; }
 
 // KS: 32-column steps of x and y at once (their LDS); wider ones pass slab by slab.
 template <int DT, int KS, int RT, int CP, bool REV, bool DOTS>
-__global__ void __launch_bounds__(kBlock, attend_waves(DOTS))
-linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
+__device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, const uint32_t workgroup) {
     using T = typename Elem<DT>::type;
     constexpr int NT = Terms<DT>::n, PT = DOTS ? 3 : out_terms(DT), MOST = PT - 1;
     constexpr bool XREG = KS * NT <= 4;                  // x stays in registers
@@ -69,8 +68,8 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
     int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // The blocks of one segment and head, which read the same state and y and z, on one XCD; those with the most to do first.
-    const uint32_t idx = blockIdx.x >> 3, rest = idx / kBlocks, of_block = idx % kBlocks;
-    const uint32_t pos = divided(rest, a.by_col_tiles), ct = rest - pos * a.col_tiles, item = pos * 8u + (blockIdx.x & 7u);
+    const uint32_t idx = workgroup >> 3, rest = idx / kBlocks, of_block = idx % kBlocks;
+    const uint32_t pos = divided(rest, a.by_col_tiles), ct = rest - pos * a.col_tiles, item = pos * 8u + (workgroup & 7u);
     if (item >= a.items) return;
     const int r = REV ? (int)of_block : kBlocks - 1 - (int)of_block;
     const uint32_t sh = divided(item, a.by_shares), share = item - sh * a.shares;
@@ -428,6 +427,20 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
         leave(static_cast<T *>(a.out) + at.b * a.out_b + tok * a.out_l + out_head * a.out_h, (uint32_t)(a.out_l * (int64_t)sizeof(T)), std::integral_constant<int, DT>());
     else
         leave(a.share + ((((int64_t)share * p.batch + at.b) * p.seqlen + tok) * p.heads + hk) * a.d2, (uint32_t)p.heads * (uint32_t)a.d2 * 4u, std::integral_constant<int, CC1D_F32>());
+}
+
+template <int DT, int KS, int RT, bool REV>
+__global__ void __launch_bounds__(kBlock, attend_waves(false))
+linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
+    attend_rows<DT, KS, RT, 1, REV, false>(p, w, a, blockIdx.x);
+}
+// dq and dk in one launch, half its workgroups each: neither waits for the other, and one alone may leave CUs idle (24 workgroups each: 25 us, one
+// after the other 47; 128 each of linear_tile_pair_kernel: 32 and 49; 256 each, which fill the card: 380 and 385).
+template <int DT, int KS, int RT, int CP>
+__global__ void __launch_bounds__(kBlock, attend_waves(true))
+linear_attend_pair_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs q, const AttendArgs k, const uint32_t half) {
+    if (blockIdx.x < half) attend_rows<DT, KS, RT, CP, false, true>(p, w, q, blockIdx.x);
+    else attend_rows<DT, KS, RT, CP, true, true>(p, w, k, blockIdx.x - half);
 }
 
 }  // namespace cc1d

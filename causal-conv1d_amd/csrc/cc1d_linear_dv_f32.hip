@@ -2,5 +2,5 @@
 #include "cc1d_linear_tile.hpp"
 
 namespace cc1d {
-template int launch_attend<CC1D_F32, true, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);
+template int launch_attend<CC1D_F32, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);
 }

@@ -329,7 +329,7 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
     }
 }
 
-// dq and dk of a key head whose value heads were several workgroups': their shares in a fixed order.  Bound by memory: eight shares of 8192 rows of 128, 67 MB, 19 us.
+// dq and dk of a key head whose value heads were several workgroups': their shares in a fixed order.  Bound by memory: four shares of 8192 rows of 128 each, 34 MB, 12 us.
 template <int DT>
 __global__ void __launch_bounds__(kBlock)
 linear_join_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const int64_t rows) {

@@ -15,7 +15,7 @@
 // there to y; each token's two are made once, by one lane.  Among the same 32 tokens it is exp(G_i - B) exp(B - G_j), B in front of them all, unless
 // the gates reach e^60 there: then an exponential an entry.
 //
-// 32 segments of 80 heads of 128 x 64 (a training step of 4 x 2048 tokens, one key head), bfloat16: out 114 us, dv 108, dq 195, dk 190; out's
+// 32 segments of 80 heads of 128 x 64 (a training step of 4 x 2048 tokens, one key head), bfloat16: out 114 us, dv 108, dq and dk 380; out's
 // matrix instructions come to 0.6 PFLOP/s.  A workgroup fills a CU's LDS, so that nobody hides what it waits for: of out's 114 the products take 40 (the
 // matrix cores' own time 19), the product with the state 24 (32 KB of operands a head, 9 of matrix cores), the gates, barriers and start
 // 37, z's way to LDS 11, stores 10.  Tried: half the rows a workgroup and two of them a CU (out 127: state and y are read twice); 16 rows a wavefront, balanced
@@ -120,8 +120,7 @@ __device__ __forceinline__ void store_wide(typename Elem<DT>::type *to, const fl
 
 // MANY: several value heads to a workgroup (DOTS: whose rows are added up, or leave as a share).
 template <int DT, int KS, int W, bool REV, bool DOTS, bool MANY>
-__global__ void __launch_bounds__(kTileBlock, 2)
-linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
+__device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, const uint32_t workgroup, const uint32_t workgroups) {
     using T = typename Elem<DT>::type;
     constexpr bool JOIN = DOTS && MANY;
     constexpr int NT = Terms<DT>::n, PT = DOTS ? 3 : 2, MOST = PT - 1;
@@ -133,7 +132,7 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Heads of one segment, which may share y and z, on one XCD.
-    const uint32_t per = gridDim.x >> 3, at_item = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+    const uint32_t per = workgroups >> 3, at_item = (workgroup & 7u) * per + (workgroup >> 3);
     const uint32_t item = divided(at_item, a.by_col_tiles), ct = at_item - item * a.col_tiles;
     if (item >= a.items) return;
     const uint32_t sh = divided(item, a.by_shares), share = item - sh * a.shares;
@@ -502,54 +501,92 @@ linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendA
     }
 }
 
-template <int DT, bool REV, bool DOTS>
-int launch_tile(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &given, hipStream_t stream) {
-    auto go = [&](auto ks, auto width, auto many) {
-        constexpr int KS = decltype(ks)::value, W = decltype(width)::value;
-        AttendArgs a = given;
-        a.col_tiles = (uint32_t)((a.d2 + 16 * W - 1) / (16 * W));
-        a.by_col_tiles = fast_div(a.col_tiles);
-        const dim3 grid((a.items * a.col_tiles + 7) / 8 * 8);
-        CC1D_LAUNCH((linear_tile_kernel<DT, KS, W, REV, DOTS, decltype(many)::value>), grid, dim3(kTileBlock), sizeof(TileLds<KS, W>), stream, p, w, a);
-        return launch_status();
-    };
-    auto by_columns = [&](auto ks) {
-        auto by_heads = [&](auto width) {
-            if constexpr (DOTS || decltype(width)::value == 4)
-                if (given.heads_each > 1 || given.share != nullptr) return go(ks, width, std::true_type());
-            return go(ks, width, std::false_type());
-        };
-        return given.d2 <= 64 ? by_heads(std::integral_constant<int, 4>()) : by_heads(std::integral_constant<int, 8>());
-    };
-    return given.d1 <= 64 ? by_columns(std::integral_constant<int, 2>()) : by_columns(std::integral_constant<int, 4>());
+template <int DT, int KS, int W, bool REV, bool MANY>
+__global__ void __launch_bounds__(kTileBlock, 2)
+linear_tile_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
+    tile_rows<DT, KS, W, REV, false, MANY>(p, w, a, blockIdx.x, gridDim.x);
+}
+// dq and dk in one launch (linear_attend_pair_kernel).
+template <int DT, int KS, int W, bool MANY>
+__global__ void __launch_bounds__(kTileBlock, 2)
+linear_tile_pair_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs q, const AttendArgs k, const uint32_t half) {
+    if (blockIdx.x < half) tile_rows<DT, KS, W, false, true, MANY>(p, w, q, blockIdx.x, half);
+    else tile_rows<DT, KS, W, true, true, MANY>(p, w, k, blockIdx.x - half, half);
 }
 
-template <int DT, bool REV, bool DOTS>
+// f(KS, W) for these columns of x and z.
+template <typename F>
+int by_tiles(const AttendArgs &a, F &&f) {
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    if (a.d2 <= 64) return a.d1 <= 64 ? f(I2(), I4()) : f(I4(), I4());
+    return a.d1 <= 64 ? f(I2(), I8()) : f(I4(), I8());
+}
+
+template <int DT, bool REV>
 int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, hipStream_t stream) {
-    if constexpr (DT != CC1D_F32)
-        if (a.tile != 0) return launch_tile<DT, REV, DOTS>(p, w, a, stream);
+    if constexpr (DT != CC1D_F32) {
+        if (a.tile != 0)
+            return by_tiles(a, [&](auto ks, auto width) {
+                constexpr int KS = decltype(ks)::value, W = decltype(width)::value;
+                const dim3 grid((a.items * a.col_tiles + 7) / 8 * 8);
+                if constexpr (W == 4) {
+                    if (a.heads_each > 1) {
+                        CC1D_LAUNCH((linear_tile_kernel<DT, KS, W, REV, true>), grid, dim3(kTileBlock), sizeof(TileLds<KS, W>), stream, p, w, a);
+                        return launch_status();
+                    }
+                }
+                CC1D_LAUNCH((linear_tile_kernel<DT, KS, W, REV, false>), grid, dim3(kTileBlock), sizeof(TileLds<KS, W>), stream, p, w, a);
+                return launch_status();
+            });
+    }
     const dim3 grid((a.items + 7) / 8 * 8 * kBlocks * a.col_tiles);
+    auto go = [&](auto ks, auto rt) {
+        constexpr int KS = decltype(ks)::value, RT = decltype(rt)::value;
+        CC1D_LAUNCH((linear_attend_kernel<DT, KS, RT, REV>), grid, dim3(kBlock), sizeof(AttendLds<DT, KS, out_terms(DT)>), stream, p, w, a);
+        return launch_status();
+    };
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
+    if constexpr (DT == CC1D_F32)        // (16-bit types: more than 128 columns of x)
+        if (a.steps <= 2) return a.d2 <= 64 ? go(I2(), I2()) : go(I2(), I4());
+    return a.d2 <= 64 ? go(I4(), I2()) : go(I4(), I4());
+}
+
+template <int DT>
+int launch_attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &q, const AttendArgs &k, hipStream_t stream) {
+    if constexpr (DT != CC1D_F32) {
+        if (q.tile != 0)
+            return by_tiles(q, [&](auto ks, auto width) {
+                constexpr int KS = decltype(ks)::value, W = decltype(width)::value;
+                const uint32_t half = (q.items + 7) / 8 * 8;
+                if (q.share != nullptr || q.heads_each > 1)
+                    CC1D_LAUNCH((linear_tile_pair_kernel<DT, KS, W, true>), dim3(2 * half), dim3(kTileBlock), sizeof(TileLds<KS, W>), stream, p, w, q, k, half);
+                else
+                    CC1D_LAUNCH((linear_tile_pair_kernel<DT, KS, W, false>), dim3(2 * half), dim3(kTileBlock), sizeof(TileLds<KS, W>), stream, p, w, q, k, half);
+                return launch_status();
+            });
+    }
+    const uint32_t half = (q.items + 7) / 8 * 8 * kBlocks;
     auto go = [&](auto ks, auto rt, auto cp) {
         constexpr int KS = decltype(ks)::value, RT = decltype(rt)::value, CP = decltype(cp)::value;
-        constexpr size_t lds = sizeof(AttendLds<DT, KS, DOTS ? 3 : out_terms(DT)>);
-        CC1D_LAUNCH((linear_attend_kernel<DT, KS, RT, CP, REV, DOTS>), grid, dim3(kBlock), lds, stream, p, w, a);
+        CC1D_LAUNCH((linear_attend_pair_kernel<DT, KS, RT, CP>), dim3(2 * half), dim3(kBlock), sizeof(AttendLds<DT, KS, 3>), stream, p, w, q, k, half);
         return launch_status();
     };
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I4 = std::integral_constant<int, 4>;
     auto by_columns = [&](auto ks) {
-        if constexpr (DOTS)
-            if (a.d2 > 128) return go(ks, I4(), I2());
-        return a.d2 <= 64 ? go(ks, I2(), I1()) : go(ks, I4(), I1());
+        if (q.d2 > 128) return go(ks, I4(), I2());
+        return q.d2 <= 64 ? go(ks, I2(), I1()) : go(ks, I4(), I1());
     };
     if constexpr (DT == CC1D_F32) {
-        return a.steps <= 2 ? by_columns(I2()) : by_columns(I4());
-    } else {                             // (more than 128 columns of x, or, of the gradients of q and k, of z)
-        if constexpr (DOTS)
-            if (a.steps <= 2) return go(I2(), I4(), I2());
-        return by_columns(I4());
+        if (q.steps <= 2) return by_columns(I2());
+    } else {                             // (more than 128 columns of x or z)
+        if (q.steps <= 2) return go(I2(), I4(), I2());
     }
+    return by_columns(I4());
 }
 
 }  // namespace cc1d
