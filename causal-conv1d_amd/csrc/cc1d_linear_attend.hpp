@@ -19,8 +19,8 @@
 // DOTS: several value heads of a key head one after the other, the sum of their rows kept in registers, and of each the rows' products with u
 // (q or k), which the gates' gradients are made of.  What several workgroups of a key head leave is joined by linear_join_kernel.
 //
-// float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 194 us (with sums and scan), backward 709; bfloat16 of 256 x 256:
-// 380 and 1157.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
+// float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 196 us (with sums and scan), backward 705; bfloat16 of 256 x 256:
+// 330 and 957.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
 // and LDS: 24 workgroups of a small call take 19 us, the matrix cores' part of which is 5.
 #pragma once
 
@@ -30,7 +30,7 @@
 namespace cc1d {
 
 // Two places for the products, or one and a barrier more where two would leave a CU a single workgroup.
-constexpr int product_places(int dt, int ks) { return dt == CC1D_F32 && ks == 4 ? 1 : 2; }
+constexpr int product_places(int dt, int ks) { return dt == CC1D_F32 && ks >= 4 ? 1 : 2; }
 template <int DT, int KS, int PT>
 struct AttendLds {
     uint8_t x[4 * KS * Terms<DT>::n * kFrag];
@@ -57,7 +57,7 @@ __device__ __forceinline__ void products_left(const bf16x8 (&a)[N][NA], const bf
 // Wavefronts a SIMD that the registers leave: two where nothing has to be kept in memory for that.
 constexpr int attend_waves(bool dots) { return dots ? 1 : 2; }
 
-// KS: 32-column steps of x and y at once (their LDS); wider ones pass slab by slab.
+// KS: 32-column steps of x and y at once (their LDS); wider ones, more than 256 columns, pass slab by slab.
 template <int DT, int KS, int RT, int CP, bool REV, bool DOTS>
 __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, const uint32_t workgroup) {
     using T = typename Elem<DT>::type;
@@ -210,6 +210,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
                     ask_state(0);
 #pragma unroll
                     for (int s = 0; s < KS; ++s) {
+                        if (KS == 8 && slab * KS + s >= a.steps) break;
                         if (s + 1 < KS) ask_state(s + 1);
                         bf16x8 f[RT][NT];
                         f32x4 *to[2][RT];
@@ -273,6 +274,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
                 }
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
+                    if (KS == 8 && slab * KS + s >= a.steps) break;
                     bf16x8 f[NT], b[4][NT];
 #pragma unroll
                     for (int t = 0; t < 4; ++t) x_of(t, s, b[t]);

@@ -524,6 +524,9 @@ int by_tiles(const AttendArgs &a, F &&f) {
     return a.d1 <= 64 ? f(I2(), I8()) : f(I4(), I8());
 }
 
+// Steps of x and y at once, beyond 128 columns: eight, or four slab by slab where eight steps' LDS leaves fewer workgroups a CU and the barriers weigh less: float32's
+// out and dv, and dq and dk of at most 64 columns of z.  16 heads, 4 x 2048 tokens, eight and four: bfloat16, 256 x 256 forward 329 us and 383, backward 953 and
+// 1152, 256 x 64 forward 119 and 147, 64 x 256 backward 479 and 399; float32, 256 x 256 forward 971 and 802, 192 x 192 backward (dq and dk by eight) 1570 and 1821.
 template <int DT, bool REV>
 int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, hipStream_t stream) {
     if constexpr (DT != CC1D_F32) {
@@ -549,9 +552,13 @@ int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const Attend
     };
     using I2 = std::integral_constant<int, 2>;
     using I4 = std::integral_constant<int, 4>;
-    if constexpr (DT == CC1D_F32)        // (16-bit types: more than 128 columns of x)
+    using I8 = std::integral_constant<int, 8>;
+    if constexpr (DT == CC1D_F32) {
         if (a.steps <= 2) return a.d2 <= 64 ? go(I2(), I2()) : go(I2(), I4());
-    return a.d2 <= 64 ? go(I4(), I2()) : go(I4(), I4());
+        return a.d2 <= 64 ? go(I4(), I2()) : go(I4(), I4());
+    } else {                             // (more than 128 columns of x)
+        return a.d2 <= 64 ? go(I8(), I2()) : go(I8(), I4());
+    }
 }
 
 template <int DT>
@@ -577,16 +584,20 @@ int launch_attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const A
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
     auto by_columns = [&](auto ks) {
         if (q.d2 > 128) return go(ks, I4(), I2());
         return q.d2 <= 64 ? go(ks, I2(), I1()) : go(ks, I4(), I1());
     };
     if constexpr (DT == CC1D_F32) {
         if (q.steps <= 2) return by_columns(I2());
+        if (q.steps <= 4 || q.d2 <= 64) return by_columns(I4());
     } else {                             // (more than 128 columns of x or z)
         if (q.steps <= 2) return go(I2(), I4(), I2());
+        if (q.steps <= 4) return go(I4(), I4(), I2());
+        if (q.d2 <= 64) return go(I4(), I2(), I1());
     }
-    return by_columns(I4());
+    return q.d2 > 128 ? go(I8(), I4(), I2()) : go(I8(), I4(), I1());
 }
 
 }  // namespace cc1d
