@@ -18,7 +18,10 @@
 //
 // whose sums are one more kernel (linear_states_kernel), and whose recurrence over segments is elementwise (linear_scan_kernel).  The gates'
 // gradients come out of sums that are there: dg at a segment's first token is S0 . dS0 over all elements (nothing else reads that gate's product), and
-// dg[t + 1] = dg[t] - (q[t].dq[t] - k[t].dk[t]).
+// dg[t + 1] = dg[t] - (q[t].dq[t] - k[t].dk[t]).  These cancel: S0 . dS0 is some 2^-11 of the norms' product, and what a segment's differences are off by adds
+// up over its tokens.  So the sums are made in 64 bits, of dq and dk before they are rounded, and what the last token leaves over against the next segment's
+// S0 . dS0 (or 0, behind the last one) is taken back evenly (16 heads with a constant decay each, 2 x 1000 tokens, the sum of dg over the tokens: off by FIGURES
+// of itself, with sums of 32 bits and without that 2e-6).
 //
 // Numbers of 24 bits on the 16-bit matrix cores: cc1d_delta_chunk.hpp.
 #pragma once
@@ -52,8 +55,8 @@ struct SegmentWork {
     float *decay;                        // per (slot, value head): exp(Gend)
     uint8_t *by_k, *by_v;                // per (slot, value head): states split into operands, contracted over dim_k and over dim_v
     uint8_t *first;                      // S0 of the forward, contracted over dim_v: what a training forward saves
-    float *dot_q, *dot_k;                // per (slot, value head): q.dq and k.(dk / beta) of each token
-    float *inner;                        // per (slot, value head): S0 . dS0, a partial sum each tile
+    double *dot_q, *dot_k;               // per (slot, value head): q.dq and k.(dk / beta) of each token
+    double *inner;                       // per (slot, value head): S0 . dS0, a partial sum each tile
     float *share_q, *share_k;            // shares of dq, dk of heads_each value heads: (shares, batch, seqlen, heads, dim_k)
     int32_t k_width, v_width, k_tiles, v_tiles;                // of operands contracted over dim_k (out, dv), over dim_v (dq, dk)
     int32_t heads_each, shares;          // value heads of a workgroup of the gradients of q and k; such workgroups a key head
@@ -132,7 +135,8 @@ struct AttendArgs {
     uint32_t items, col_tiles;           // (slot, key head, share); 128-column tiles of d2
     FastDiv by_col_tiles, by_heads, by_shares;
     void *out; int64_t out_b, out_l, out_h;   // of x_dtype, by value head or (DOTS) by key head; NULL: to `share`
-    float *share, *dots;
+    float *share;
+    double *dots;
 };
 
 // `out`: from whole vectors to rows as they are, else the other way round.

@@ -82,6 +82,7 @@ struct Places {
         return at;
     }
     float *floats(size_t n) { return reinterpret_cast<float *>(take(n * sizeof(float))); }
+    double *doubles(size_t n) { return reinterpret_cast<double *>(take(n * sizeof(double))); }
 };
 
 SegmentWork sizes_of(const cc1d_delta_params &p, bool alone) {
@@ -206,10 +207,10 @@ size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &
         w.decay = work.floats(heads);
         w.by_k = work.take(by_k_bytes(p, w));
         w.by_v = work.take(by_v_bytes(p, w));
-        w.inner = work.floats(tiles);
+        w.inner = work.doubles(tiles);
     }
-    w.dot_q = work.floats(heads * kSegment);
-    w.dot_k = work.floats(heads * kSegment);
+    w.dot_q = work.doubles(heads * kSegment);
+    w.dot_k = work.doubles(heads * kSegment);
     if (w.shares > 1) {
         const size_t plane = (size_t)p.batch * p.seqlen * p.heads * padded(p.dim_k);
         w.share_q = work.floats(w.shares * plane);

@@ -37,7 +37,7 @@ struct AttendLds {
     uint8_t p[product_places(DT, KS)][8 * PT * kFrag];
     GateLds gates;
     float f[kChunk], s[kChunk];
-    float dots[4][kChunk];
+    double dots[4][kChunk];
 };
 
 // Left operands of four tiles against one right one, their chains side by side.
@@ -355,7 +355,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
         if constexpr (DOTS) {
             const T *ub = rows_of(a.u);
             const uint32_t u_pitch = (uint32_t)(a.u.sl * (int64_t)sizeof(T));
-            float dot[RT][4];
+            double dot[RT][4];
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 T u[4][CP][2];
@@ -372,12 +372,12 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
                 stay();
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float sum = 0.f;
+                    double sum = 0.0;
 #pragma unroll
                     for (int c = 0; c < CP; ++c) {
                         const int col = 32 * (pair0 + 4 * c) + 2 * m;
-                        sum += col < a.d2 ? acc[i][c][0][e] * Elem<DT>::to_float(u[e][c][0]) : 0.f;
-                        sum += col + 1 < a.d2 ? acc[i][c][1][e] * Elem<DT>::to_float(u[e][c][1]) : 0.f;
+                        sum += col < a.d2 ? (double)acc[i][c][0][e] * (double)Elem<DT>::to_float(u[e][c][0]) : 0.0;
+                        sum += col + 1 < a.d2 ? (double)acc[i][c][1][e] * (double)Elem<DT>::to_float(u[e][c][1]) : 0.0;
                     }
                     dot[i][e] = over_columns(sum);
                 }
@@ -385,7 +385,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 const int row = i0 + 16 * i + 4 * g;
-                if (m == 0) *reinterpret_cast<float4 *>(&lds.dots[wave][row]) = make_float4(dot[i][0], dot[i][1], dot[i][2], dot[i][3]);
+                if (m < 4) lds.dots[wave][row + m] = m == 1 ? dot[i][1] : m == 2 ? dot[i][2] : m == 3 ? dot[i][3] : dot[i][0];
                 const float4 s = *reinterpret_cast<const float4 *>(&lds.s[row]);
                 const f32x4 by = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -395,9 +395,9 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
             }
             lds_barrier();
             if (wave == 0 && lane < own) {
-                float d = RT == 2 ? lds.dots[2 * (lane >> 5)][lane] + lds.dots[2 * (lane >> 5) + 1][lane]
+                const double d = RT == 2 ? lds.dots[2 * (lane >> 5)][lane] + lds.dots[2 * (lane >> 5) + 1][lane]
                                   : (lds.dots[0][lane] + lds.dots[1][lane]) + (lds.dots[2][lane] + lds.dots[3][lane]);
-                a.dots[sv * kSegment + row0 + lane] = REV ? d : p.scale * d;
+                a.dots[sv * kSegment + row0 + lane] = REV ? d : (double)p.scale * d;
             }
         }
     }

@@ -41,6 +41,18 @@ __device__ __forceinline__ float decay_since_start(const GateLds &lds, int to) {
     return fmaf(e, lds.lo[to], e);       // |lo| < 2^-8 |hi| 2^-16: the next term is nothing
 }
 
+// Sums over the 16 lanes of a row of a result tile, and over all 64.
+__device__ __forceinline__ double over_columns(double v) {
+    v += moved_or_zero<0xB1, 0xf>(v);    // (quad_perm, row_ror: every lane has a source)
+    v += moved_or_zero<0x4E, 0xf>(v);
+    v += moved_or_zero<0x124, 0xf>(v);
+    return v + moved_or_zero<0x128, 0xf>(v);
+}
+__device__ __forceinline__ double over_wave(double v) {
+    v = over_columns(v);
+    return (of_lane(v, 0) + of_lane(v, 16)) + (of_lane(v, 32) + of_lane(v, 48));
+}
+
 // Columns c, c + 1 (`c` even) of eight rows: the right operand of two result tiles, whose columns are the even and the odd ones of
 // 32, so that a lane loads both with one access and stores both of its results with one.  Eight consecutive rows of one column are what
 // the matrix instruction wants of a lane, and no 16-bit element has to cross lanes for it.

@@ -61,8 +61,19 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
 #pragma unroll
         for (int i = 0; i < KT; ++i) ra[i].ask(ab, at_a, 32 * (p0 + i) + 2 * m, p.dim_k);
     };
+    // The matrix cores round their sums downwards by a little, 1e-8 of them over a segment, and S0 . dS0 does not average away what all elements are off by:
+    // odd columns are summed up with the other sign, and so are tokens 64 to 191.
+    float sign = 1.f;
+    auto turn = [&]() {
+        sign = -sign;
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][e >> 1][e & 1] = -acc[i][e >> 1][e & 1];
+    };
     ask(0);
     for (int t0 = 0; t0 < at.count; t0 += 32) {
+        if (t0 == 64 || t0 == 192) turn();
         bf16x8 fb[2][3], fa[KT][2][NT];
         {
             const float4 w0 = *reinterpret_cast<const float4 *>(&weight[t0 + 8 * g]), w1 = *reinterpret_cast<const float4 *>(&weight[t0 + 8 * g + 4]);
@@ -72,7 +83,7 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
                 float f[8];
                 rb.get(n, f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] *= wt[e];
+                for (int e = 0; e < 8; ++e) f[e] *= (n == 0 ? sign : -sign) * wt[e];
                 split8<3>(f, fb[n]);
             }
         }
@@ -102,7 +113,7 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
-                    f[2 * e + n] = 32 * (p0 + i) + 8 * g + 2 * e + n < p.dim_k && cb + c < p.dim_v ? acc[i][n][c][e] : 0.f;
+                    f[2 * e + n] = 32 * (p0 + i) + 8 * g + 2 * e + n < p.dim_k && cb + c < p.dim_v ? (c == 0 ? sign : -sign) * acc[i][n][c][e] : 0.f;
             *reinterpret_cast<float4 *>(to + c * 512) = make_float4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<float4 *>(to + c * 512 + 4) = make_float4(f[4], f[5], f[6], f[7]);
         }
@@ -208,7 +219,7 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
     // S0 . dS0 of a segment whose dS0 is at hand.
     auto inner = [&](int slot, const float (&t)[2][8]) {
         const uint8_t *from = w.first + by_v_step(slot);
-        float sum = 0.f;
+        double sum = 0.0;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             bf16x8 f[3];
@@ -216,10 +227,10 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
             float x[4];
             four_of(f, false, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += x[e] * t[c][e];
+            for (int e = 0; e < 4; ++e) sum = fma((double)x[e], (double)t[c][e], sum);
             four_of(f, true, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += x[e] * t[c][4 + e];
+            for (int e = 0; e < 4; ++e) sum = fma((double)x[e], (double)t[c][4 + e], sum);
         }
         sum = over_wave(sum);
         if (lane == 0) w.inner[place(slot)] = sum;
@@ -310,22 +321,38 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
     }
     const SegmentAt at = segment_at(p, w, slot);
     if (at.count <= 0) return;
-    // The terms cancel up to rounding: their running sum is kept in 64 bits.
-    double dg = 0.0;
-    if (at.c > 0 || first) {
+    auto inner = [&](int64_t of) {                       // S0 . dS0
         double sum = 0.0;
-        for (int64_t i = lane; i < w.tiles(); i += 64) sum += (double)w.inner[(int64_t)sv * w.tiles() + i];
-        dg = of_lane(running_sum(sum), 63);
+        for (int64_t i = lane; i < w.tiles(); i += 64) sum += w.inner[of * w.tiles() + i];
+        return over_wave(sum);
+    };
+    double change[kBlocks], total = 0.0;
+    float kz[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const int t = b * kChunk + lane, there = t < at.count ? t : at.count - 1;
+        float beta = 1.f;
+        if (p.beta != nullptr) beta = bits_as_float(load_bits(p.beta, at.b * p.beta_stride_b + (at.lo + there) * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype), p.beta_dtype);
+        const double qd = w.dot_q[(int64_t)sv * kSegment + there], z = w.dot_k[(int64_t)sv * kSegment + there];
+        kz[b] = (float)z;
+        change[b] = t < at.count ? qd - (double)beta * z : 0.0;
     }
-    for (int t0 = 0; t0 < at.count; t0 += 64) {
-        const int t = t0 + lane;
-        const bool there = t < at.count;
-        const int64_t tok = at.lo + (there ? t : 0);
-        const float beta = p.beta == nullptr ? 1.f : bits_as_float(load_bits(p.beta, at.b * p.beta_stride_b + tok * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype), p.beta_dtype);
-        const float qd = there ? w.dot_q[(int64_t)sv * kSegment + t] : 0.f, kz = there ? w.dot_k[(int64_t)sv * kSegment + t] : 0.f;
-        const double change = there ? (double)qd - (double)beta * (double)kz : 0.0, sum = running_sum(change);
-        if (there) put(((int64_t)at.b * p.seqlen + tok) * p.v_heads + h, (float)(dg - (sum - change)), kz);
-        dg -= of_lane(sum, 63);
+    double dg = at.c > 0 || first ? inner(sv) : 0.0, rest = 0.0;
+    const bool known = !at.last || !bp.dfinal_states;    // what comes behind the last token
+    const double end = at.last || !known ? 0.0 : inner((int64_t)sv + p.v_heads);
+    double before[kBlocks];                              // changes in front of each token
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const double sum = running_sum(change[b]);
+        before[b] = total + (sum - change[b]);
+        total += of_lane(sum, 63);
+    }
+    if (known) rest = end - (dg - total);
+    rest = fabs(rest) < 1e300 ? rest / at.count : 0.0;   // (of numbers)
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const int t = b * kChunk + lane;
+        if (t < at.count) put(((int64_t)at.b * p.seqlen + at.lo + t) * p.v_heads + h, (float)((dg - before[b]) + rest * t), kz[b]);
     }
 }
 
