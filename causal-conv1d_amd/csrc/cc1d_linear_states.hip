@@ -62,18 +62,9 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
         for (int i = 0; i < KT; ++i) ra[i].ask(ab, at_a, 32 * (p0 + i) + 2 * m, p.dim_k);
     };
     // The matrix cores round their sums downwards by a little, 1e-8 of them over a segment, and S0 . dS0 does not average away what all elements are off by:
-    // odd columns are summed up with the other sign, and so are tokens 64 to 191.
-    float sign = 1.f;
-    auto turn = [&]() {
-        sign = -sign;
-#pragma unroll
-        for (int i = 0; i < KT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][e >> 1][e & 1] = -acc[i][e >> 1][e & 1];
-    };
+    // odd columns are summed up with the other sign.
     ask(0);
     for (int t0 = 0; t0 < at.count; t0 += 32) {
-        if (t0 == 64 || t0 == 192) turn();
         bf16x8 fb[2][3], fa[KT][2][NT];
         {
             const float4 w0 = *reinterpret_cast<const float4 *>(&weight[t0 + 8 * g]), w1 = *reinterpret_cast<const float4 *>(&weight[t0 + 8 * g + 4]);
@@ -83,7 +74,7 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
                 float f[8];
                 rb.get(n, f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] *= (n == 0 ? sign : -sign) * wt[e];
+                for (int e = 0; e < 8; ++e) f[e] *= n == 0 ? wt[e] : -wt[e];
                 split8<3>(f, fb[n]);
             }
         }
@@ -113,7 +104,7 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
-                    f[2 * e + n] = 32 * (p0 + i) + 8 * g + 2 * e + n < p.dim_k && cb + c < p.dim_v ? (c == 0 ? sign : -sign) * acc[i][n][c][e] : 0.f;
+                    f[2 * e + n] = 32 * (p0 + i) + 8 * g + 2 * e + n < p.dim_k && cb + c < p.dim_v ? (c == 0 ? acc[i][n][c][e] : -acc[i][n][c][e]) : 0.f;
             *reinterpret_cast<float4 *>(to + c * 512) = make_float4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<float4 *>(to + c * 512 + 4) = make_float4(f[4], f[5], f[6], f[7]);
         }

@@ -448,16 +448,16 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                     double dot[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        double sum_u = 0.0;
+                        float sum_u = 0.f;
 #pragma unroll
                         for (int t = 0; t < W / 2; ++t) {
                             const uint32_t two = u.r[e][t];
                             float u0, u1;
                             if constexpr (DT == CC1D_F16) { u0 = (float)bitcast<f16x2>(two).x; u1 = (float)bitcast<f16x2>(two).y; }
                             else { u0 = bitcast<float>(two << 16); u1 = bitcast<float>(two & 0xffff0000u); }
-                            sum_u = fma((double)acc[i][2 * t][e], (double)u0, fma((double)acc[i][2 * t + 1][e], (double)u1, sum_u));
+                            sum_u = fmaf(acc[i][2 * t][e], u0, fmaf(acc[i][2 * t + 1][e], u1, sum_u));
                         }
-                        dot[e] = over_columns(W * m < a.d2 ? sum_u : 0.0);
+                        dot[e] = over_columns(W * m < a.d2 ? (double)sum_u : 0.0);
                     }
                     const double mine_dot = m == 1 ? dot[1] : m == 2 ? dot[2] : m == 3 ? dot[3] : dot[0];
                     if (m < 4 && row + m < at.count) a.dots[sv * kSegment + row + m] = REV ? mine_dot : (double)p.scale * mine_dot;

@@ -361,3 +361,29 @@ def test_odd_sizes_of_many_segments(pkg, gpu_device, dtype, dims):
     """More than one segment, shared key heads, states: each size's rows end inside a vector."""
     s = cases.inputs(gpu_device, 2, 530, 1, 3, *dims, dtype, slices=False)
     cases.check(cases.run(pkg, s), s)
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_gradient_of_a_constant_decay(pkg, gpu_device, seed):
+    """Its sum over many tokens, where the error of a segment's S0.dS0 stands in every one of its tokens.  Elements of S0 and dS0 are off by some 2^-23 of
+    their size each, independently: S0.dS0 by 2^-23 |S0| |dS0| / sqrt(elements), here four times that, for 256 tokens, and over the segments as they come.
+    An offset that all elements share, of 2^-24 as much, would be past it where states have a mean."""
+    from causal_conv1d.linear_attention import linear_attention_ref
+    b, l, h, d = 2, 1000, 8, 128
+    s = cases.inputs(gpu_device, b, l, h, h, d, d, BF16, decay="head", beta=False, seed=seed, slices=False)
+    s["g"] = -0.7 * 0.45 ** torch.arange(h, device=gpu_device, dtype=torch.float32)
+    got = cases.run(pkg, s)["dg"].double()
+    w = {n: s[n].detach().double().requires_grad_() for n in ("q", "k", "v", "g", "states")}
+    state, outs, states = w["states"], [], []
+    for t in range(0, l, 256):
+        state.retain_grad()
+        states.append(state)
+        e = min(l, t + 256)
+        out, state = linear_attention_ref(w["q"][:, t:e], w["k"][:, t:e], w["v"][:, t:e], w["g"].expand(b, e - t, h), initial_states=state, return_final_states=True)
+        outs.append(out)
+    ((torch.cat(outs, 1) * s["dout"].double()).sum() + (state * s["dfinal"].double()).sum()).backward()
+    bound = sum((x.norm(dim=(2, 3)) * x.grad.norm(dim=(2, 3))).sum(0) for x in states) * 256 * 4 * 2.0 ** -23 / d
+    off = (got - w["g"].grad).abs()
+    # and what the tokens between add: q.dq and k.dk off by 2^-24 |q| |dq| / sqrt(d) each, twice that, added up over up to 256 tokens and summed over these
+    between = 4 * 2.0 ** -24 / d ** 0.5 * 256 / 3 ** 0.5 * (w["q"].grad.norm(dim=-1) * w["q"].norm(dim=-1)).square().sum((0, 1)).sqrt()
+    assert (off <= bound + between + 2.0 ** -23 * w["g"].grad.abs()).all(), (off / (bound + between)).tolist()
