@@ -143,11 +143,11 @@ struct AttendArgs {
 int launch_linear_copy(const CopyArgs &a, int copies, bool out, hipStream_t stream);
 int launch_linear_states(const cc1d_delta_params &p, const SegmentWork &w, const StatesArgs &a, hipStream_t stream);
 int launch_linear_scan(const cc1d_delta_params &p, const SegmentWork &w, const ScanArgs &a, hipStream_t stream);
-// Instantiated one to a file: out (REV: dv), and dq and dk together.
+// Instantiated one to a file: out (REV: dv), and dq and dk together, in float32 with dv if given.
 template <int DT, bool REV>
 int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, hipStream_t stream);
 template <int DT>
-int launch_attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &q, const AttendArgs &k, hipStream_t stream);
+int launch_attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &q, const AttendArgs &k, const AttendArgs *v, hipStream_t stream);
 int launch_linear_gates(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream);
 int launch_linear_join(const cc1d_delta_bwd_params &bp, const SegmentWork &w, hipStream_t stream);
 

@@ -8,7 +8,7 @@ namespace cc1d {
 #define CC1D_ATTEND(DT)                                                                                                                   \
     extern template int launch_attend<DT, false>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);     \
     extern template int launch_attend<DT, true>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, hipStream_t);      \
-    extern template int launch_attend_pair<DT>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, const AttendArgs &, hipStream_t);
+    extern template int launch_attend_pair<DT>(const cc1d_delta_params &, const SegmentWork &, const AttendArgs &, const AttendArgs &, const AttendArgs *, hipStream_t);
 CC1D_ATTEND(CC1D_F32)
 CC1D_ATTEND(CC1D_F16)
 CC1D_ATTEND(CC1D_BF16)
@@ -257,17 +257,20 @@ int by_type(const cc1d_delta_params &p, F &&f) {
         default: return f(std::integral_constant<int, CC1D_BF16>());
     }
 }
-int attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &given, bool rev, hipStream_t stream) {
+int attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &given, hipStream_t stream) {
     if (w.slots == 0) return CC1D_OK;
     const AttendArgs a = prepared(p, w, given, false);
+    return by_type(p, [&](auto dt) { return launch_attend<decltype(dt)::value, false>(p, w, a, stream); });
+}
+int attend_gradients(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &dq, const AttendArgs &dk, const AttendArgs &dv, hipStream_t stream) {
+    if (w.slots == 0) return CC1D_OK;
+    const AttendArgs q = prepared(p, w, dq, true), k = prepared(p, w, dk, true), v = prepared(p, w, dv, false);
+    const bool together = p.x_dtype == CC1D_F32 && (2 * (uint64_t)q.items + (uint64_t)v.items * v.col_tiles) * kBlocks <= 256;
     return by_type(p, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        return rev ? launch_attend<DT, true>(p, w, a, stream) : launch_attend<DT, false>(p, w, a, stream);
+        const int st = launch_attend_pair<DT>(p, w, q, k, together ? &v : nullptr, stream);
+        return st != CC1D_OK || together ? st : launch_attend<DT, true>(p, w, v, stream);
     });
-}
-int attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &q, const AttendArgs &k, hipStream_t stream) {
-    if (w.slots == 0) return CC1D_OK;
-    return by_type(p, [&](auto dt) { return launch_attend_pair<decltype(dt)::value>(p, w, prepared(p, w, q, true), prepared(p, w, k, true), stream); });
 }
 
 void set_out(AttendArgs &a, const LinearRows &r) {
@@ -301,7 +304,7 @@ int forward(const cc1d_delta_params &p, const SegmentWork &w, const Forward &f, 
     a.state = w.by_k;
     a.first = p.initial_states != nullptr;
     set_out(a, f.out);
-    st = attend(p, w, a, false, stream);
+    st = attend(p, w, a, stream);
     return st != CC1D_OK ? st : launch_linear_copy(f.back, f.backs, true, stream);
 }
 
@@ -339,15 +342,13 @@ int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, const Backwa
     dk.first = bp.dfinal_states != nullptr;
     set_out(dk, f.dk);
     dk.share = w.share_k; dk.dots = w.dot_k;
-    st = attend_pair(p, w, dq, dk, stream);
-    if (st != CC1D_OK) return st;
-    AttendArgs d = {};                                   // dv
+    AttendArgs d = {};                   // dv
     d.x = f.k; d.y = f.q; d.z = f.dout;
     d.d1 = p.dim_k; d.d2 = p.dim_v;
     d.state = w.by_k;
     d.first = bp.dfinal_states != nullptr;
     set_out(d, f.dv);
-    st = attend(p, w, d, true, stream);
+    st = attend_gradients(p, w, dq, dk, d, stream);
     if (st == CC1D_OK) st = launch_linear_gates(bp, w, stream);
     if (st == CC1D_OK && w.shares > 1 && w.slots > 0) st = launch_linear_join(bp, w, stream);
     if (st == CC1D_OK) st = launch_linear_copy(f.back, f.backs, true, stream);

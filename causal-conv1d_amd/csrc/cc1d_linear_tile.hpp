@@ -562,7 +562,7 @@ int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const Attend
 }
 
 template <int DT>
-int launch_attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &q, const AttendArgs &k, hipStream_t stream) {
+int launch_attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &q, const AttendArgs &k, const AttendArgs *v, hipStream_t stream) {
     if constexpr (DT != CC1D_F32) {
         if (q.tile != 0)
             return by_tiles(q, [&](auto ks, auto width) {
@@ -578,7 +578,10 @@ int launch_attend_pair(const cc1d_delta_params &p, const SegmentWork &w, const A
     const uint32_t half = (q.items + 7) / 8 * 8 * kBlocks;
     auto go = [&](auto ks, auto rt, auto cp) {
         constexpr int KS = decltype(ks)::value, RT = decltype(rt)::value, CP = decltype(cp)::value;
-        CC1D_LAUNCH((linear_attend_pair_kernel<DT, KS, RT, CP>), dim3(2 * half), dim3(kBlock), sizeof(AttendLds<DT, KS, 3>), stream, p, w, q, k, half);
+        constexpr size_t lds = sizeof(AttendLds<DT, KS, 3>), lds_v = DT == CC1D_F32 ? sizeof(AttendLds<DT, RT == 2 ? 2 : 4, 3>) : 0;
+        const uint32_t more = v != nullptr ? (v->items + 7) / 8 * 8 * kBlocks * v->col_tiles : 0;
+        CC1D_LAUNCH((linear_attend_pair_kernel<DT, KS, RT, CP>), dim3(2 * half + more), dim3(kBlock), lds > lds_v || v == nullptr ? lds : lds_v, stream, p, w, q, k, v != nullptr ? *v : q,
+                    half);
         return launch_status();
     };
     using I1 = std::integral_constant<int, 1>;
