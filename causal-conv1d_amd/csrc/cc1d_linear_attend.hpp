@@ -56,7 +56,7 @@ __device__ __forceinline__ void products_left(const bf16x8 (&a)[N][NA], const bf
 
 // Wavefronts a SIMD that the registers leave: two where nothing, or next to nothing, has to be kept in memory for that (dq and dk of 64 columns, float32, dim_v 256:
 // backward 741 us, with one 1012).
-constexpr int attend_waves(bool dots, int rt) { return dots && rt == 4 ? 1 : 2; }
+constexpr int attend_waves(bool dots, int ks, int rt, int cp) { return dots && rt == 4 && (ks > 2 || cp > 1) ? 1 : 2; }
 
 // KS: 32-column steps of x and y at once (their LDS); wider ones, more than 256 columns, pass slab by slab.
 template <int DT, int KS, int RT, int CP, bool REV, bool DOTS>
@@ -433,7 +433,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
 }
 
 template <int DT, int KS, int RT, bool REV>
-__global__ void __launch_bounds__(kBlock, attend_waves(false, RT))
+__global__ void __launch_bounds__(kBlock, attend_waves(false, KS, RT, 1))
 linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
     attend_rows<DT, KS, RT, 1, REV, false>(p, w, a, blockIdx.x);
 }
@@ -441,7 +441,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
 // after the other 47; 128 each of linear_tile_pair_kernel: 32 and 49; 256 each, which fill the card: 380 and 385).  float32: dv's workgroups behind them, if all together
 // are no more than CUs (24 each: 26 us, for 25 and 20); more of them would run one wavefront a SIMD here and two by themselves.
 template <int DT, int KS, int RT, int CP>
-__global__ void __launch_bounds__(kBlock, attend_waves(true, RT))
+__global__ void __launch_bounds__(kBlock, attend_waves(true, KS, RT, CP))
 linear_attend_pair_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs q, const AttendArgs k, const AttendArgs v, const uint32_t half) {
     if (blockIdx.x < half) attend_rows<DT, KS, RT, CP, false, true>(p, w, q, blockIdx.x);
     else if (DT != CC1D_F32 || blockIdx.x < 2 * half) attend_rows<DT, KS, RT, CP, true, true>(p, w, k, blockIdx.x - half);
