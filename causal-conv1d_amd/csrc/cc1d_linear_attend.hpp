@@ -19,8 +19,8 @@
 // DOTS: several value heads of a key head one after the other, the sum of their rows kept in registers, and of each the rows' products with u
 // (q or k), which the gates' gradients are made of.  What several workgroups of a key head leave is joined by linear_join_kernel.
 //
-// float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 196 us (with sums and scan), backward 705; bfloat16 of 256 x 256:
-// 330 and 957.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
+// float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 196 us (with sums and scan), backward 552; bfloat16 of 256 x 256:
+// 330 and 952.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
 // and LDS: 24 workgroups of a small call take 19 us, the matrix cores' part of which is 5.
 #pragma once
 
@@ -30,7 +30,7 @@
 namespace cc1d {
 
 // Two places for the products, or one and a barrier more where two would leave a CU a single workgroup.
-constexpr int product_places(int dt, int ks) { return dt == CC1D_F32 && ks >= 4 ? 1 : 2; }
+constexpr int product_places(int dt, int ks) { return ks >= (dt == CC1D_F32 ? 4 : 8) ? 1 : 2; }
 template <int DT, int KS, int PT>
 struct AttendLds {
     uint8_t x[4 * KS * Terms<DT>::n * kFrag];
@@ -54,9 +54,10 @@ __device__ __forceinline__ void products_left(const bf16x8 (&a)[N][NA], const bf
         }
 }
 
-// Wavefronts a SIMD that the registers leave: two where nothing, or next to nothing, has to be kept in memory for that (dq and dk of 64 columns, float32, dim_v 256:
-// backward 741 us, with one 1012).
-constexpr int attend_waves(bool dots, int ks, int rt, int cp) { return dots && rt == 4 && (ks > 2 || cp > 1) ? 1 : 2; }
+// Wavefronts a SIMD that the registers leave: two where nothing, or next to nothing, has to be kept in memory for that and LDS leaves two workgroups (dq and dk,
+// 16 heads, 4 x 2048 tokens, backward with two and with one: float32, 128 x 128 603 us and 746, 64 x 256 741 and 1012; bfloat16, 128 x 256 447 and 605; float32,
+// 128 x 256, whose LDS leaves one, 1262 and 1150).
+constexpr int attend_waves(bool dots, int dt, int ks, int cp) { return dots && (cp > 1 || (dt == CC1D_F32 && ks == 8)) ? 1 : 2; }
 
 // KS: 32-column steps of x and y at once (their LDS); wider ones, more than 256 columns, pass slab by slab.
 template <int DT, int KS, int RT, int CP, bool REV, bool DOTS>
@@ -433,7 +434,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
 }
 
 template <int DT, int KS, int RT, bool REV>
-__global__ void __launch_bounds__(kBlock, attend_waves(false, KS, RT, 1))
+__global__ void __launch_bounds__(kBlock, attend_waves(false, DT, KS, 1))
 linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
     attend_rows<DT, KS, RT, 1, REV, false>(p, w, a, blockIdx.x);
 }
@@ -441,7 +442,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
 // after the other 47; 128 each of linear_tile_pair_kernel: 32 and 49; 256 each, which fill the card: 380 and 385).  float32: dv's workgroups behind them, if all together
 // are no more than CUs (24 each: 26 us, for 25 and 20); more of them would run one wavefront a SIMD here and two by themselves.
 template <int DT, int KS, int RT, int CP>
-__global__ void __launch_bounds__(kBlock, attend_waves(true, KS, RT, CP))
+__global__ void __launch_bounds__(kBlock, attend_waves(true, DT, KS, CP))
 linear_attend_pair_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs q, const AttendArgs k, const AttendArgs v, const uint32_t half) {
     if (blockIdx.x < half) attend_rows<DT, KS, RT, CP, false, true>(p, w, q, blockIdx.x);
     else if (DT != CC1D_F32 || blockIdx.x < 2 * half) attend_rows<DT, KS, RT, CP, true, true>(p, w, k, blockIdx.x - half);
