@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kBlock, attend_waves(false, DT, KS, 1))
 linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs a) {
     attend_rows<DT, KS, RT, 1, REV, false>(p, w, a, blockIdx.x);
 }
-// dq and dk in one launch, half of 2 half workgroups each: neither waits for the other, and one alone may leave CUs idle (24 workgroups each: 25 us, one
+// dq and dk in one launch, `half` workgroups each: neither waits for the other, and one alone may leave CUs idle (24 workgroups each: 25 us, one
 // after the other 47; 128 each of linear_tile_pair_kernel: 32 and 49; 256 each, which fill the card: 380 and 385).  float32: dv's workgroups behind them, if all together
 // are no more than CUs (24 each: 26 us, for 25 and 20); more of them would run one wavefront a SIMD here and two by themselves.
 template <int DT, int KS, int RT, int CP>
