@@ -440,7 +440,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
 }
 // dq and dk in one launch, `half` workgroups each: neither waits for the other, and one alone may leave CUs idle (24 workgroups each: 25 us, one
 // after the other 47; 128 each of linear_tile_pair_kernel: 32 and 49; 256 each, which fill the card: 380 and 385).  float32: dv's workgroups behind them, if all together
-// are no more than CUs (24 each: 26 us, for 25 and 20); more of them would run one wavefront a SIMD here and two by themselves.
+// are no more than CUs (24 each: 26 us, for 25 and 20); more of them leave no CU idle by themselves.
 template <int DT, int KS, int RT, int CP>
 __global__ void __launch_bounds__(kBlock, attend_waves(true, DT, KS, CP))
 linear_attend_pair_kernel(const cc1d_delta_params p, const SegmentWork w, const AttendArgs q, const AttendArgs k, const AttendArgs v, const uint32_t half) {
