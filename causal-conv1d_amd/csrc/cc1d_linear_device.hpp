@@ -36,6 +36,11 @@ __device__ __forceinline__ void segment_gates(const cc1d_delta_params &p, const 
 __device__ __forceinline__ float decay_between(const GateLds &lds, int from, int to) {        // exp(G_to - G_from)
     return exp_of((lds.hi[to] - lds.hi[from]) + (lds.lo[to] - lds.lo[from]));
 }
+// exp of a sum of gates: what 32 bits leave of it (2^-19 of a sum of 32 to 64, and of its exponential) counts as well.
+__device__ __forceinline__ float exp_of_sum(double x) {
+    const float hi = (float)x, e = exp_of(hi);
+    return fmaf(e, (float)(x - (double)hi), e);
+}
 __device__ __forceinline__ float decay_since_start(const GateLds &lds, int to) {
     const float e = exp_of(lds.hi[to]);
     return fmaf(e, lds.lo[to], e);       // |lo| < 2^-8 |hi| 2^-16: the next term is nothing

@@ -293,7 +293,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
         lds_barrier();                                   // G; the state has been read
         if (first_half) {
             const double start = lds.ends[mine >> 5], end = lds.ends[(mine >> 5) + 1], last = lds.ends[kSteps];
-            const float up = exp_of((float)(sum - start)), down = exp_of((float)(end - sum)), back = exp_of((float)(start - sum));
+            const float up = exp_of_sum(sum - start), down = exp_of_sum(end - sum), back = exp_of_sum(start - sum);
             const float weigh = mine >= at.count ? 0.f : REV ? p.scale : beta;
             lds.of_x[mine] = REV ? down : up;
             lds.of_y[mine] = weigh * (REV ? up : down);
@@ -301,7 +301,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
             lds.back[mine] = REV ? back : weigh * back;
             const uint64_t steep = __ballot(fabs(sum - start) > 60.0);
             if ((lane & 31) == 0) lds.steep[mine >> 5] = (uint32_t)(steep >> (lane & 32)) != 0u;
-            lds.f[mine] = exp_of((float)(REV ? last - sum : sum));
+            lds.f[mine] = exp_of_sum(REV ? last - sum : sum);
             lds.s[mine] = REV ? beta : p.scale;
         }
         if (rows) {
@@ -403,7 +403,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                         split8<PT>(v, f[i]);
                     }
                 } else {
-                    const float between = exp_of((float)(REV ? lds.ends[j] - border : border - lds.ends[j + 1]));
+                    const float between = exp_of_sum(REV ? lds.ends[j] - border : border - lds.ends[j + 1]);
                     const f32x4 y0 = *reinterpret_cast<const f32x4 *>(&lds.of_y[j * kStep + 8 * g]), y1 = *reinterpret_cast<const f32x4 *>(&lds.of_y[j * kStep + 8 * g + 4]);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
