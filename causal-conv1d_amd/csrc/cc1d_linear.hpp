@@ -18,8 +18,10 @@
 //
 // whose sums are one more kernel (linear_states_kernel), and whose recurrence over segments is elementwise (linear_scan_kernel).  The gates'
 // gradients come out of sums that are there: dg at a segment's first token is S0 . dS0 over all elements (nothing else reads that gate's product), and
-// dg[t + 1] = dg[t] - (q[t].dq[t] - k[t].dk[t]).  These cancel: S0 . dS0 is some 2^-11 of the norms' product, and what a segment's differences are off by adds
-// up over its tokens.  So the sums are made in 64 bits, of dq and dk before they are rounded, and what the last token leaves over against the next segment's
+// dg[t + 1] = dg[t] - (q[t].dq[t] - k[t].dk[t]).  What a token reads of itself, scale beta_t (dout_t.v_t) (q_t.k_t), is in both products and is left out of both:
+// where gates are strong it is nearly all of them, and nothing of dg (gates of -5, 320 tokens, heads of 128 x 64, bfloat16: dg off by 1.2e-6 of itself, with it 1.7e-4).
+// What remains still cancels: S0 . dS0 is some 2^-11 of the norms' product, and what a segment's differences are off by adds
+// up over its tokens.  So the sums are made in 64 bits (linear_tile_kernel: 32 for the four or eight products inside a lane), of dq and dk before they are rounded, and what the last token leaves over against the next segment's
 // S0 . dS0 (or 0, behind the last one) is taken back evenly (16 heads with a constant decay each, 2 x 1000 tokens, the sum of dg over the tokens, six seeds: off by
 // 1e-8 to 5e-7 of itself; with sums of 32 bits, without that and without linear_states_kernel's alternating signs 7e-7 to 3e-6).
 //
@@ -55,7 +57,8 @@ struct SegmentWork {
     float *decay;                        // per (slot, value head): exp(Gend)
     uint8_t *by_k, *by_v;                // per (slot, value head): states split into operands, contracted over dim_k and over dim_v
     uint8_t *first;                      // S0 of the forward, contracted over dim_v: what a training forward saves
-    double *dot_q, *dot_k;               // per (slot, value head): q.dq and k.(dk / beta) of each token
+    double *dot_q, *dot_k;               // per (slot, value head): q.dq and k.(dk / beta) of each token, without its own share
+    float *self_k, *qk;                  // that share of k.(dk / beta) is self_k qk: scale dout.v; per (slot, key head): q.k
     double *inner;                       // per (slot, value head): S0 . dS0, a partial sum each tile
     float *share_q, *share_k;            // shares of dq, dk of heads_each value heads: (shares, batch, seqlen, heads, dim_k)
     int32_t k_width, v_width, k_tiles, v_tiles;                // of operands contracted over dim_k (out, dv), over dim_v (dq, dk)
@@ -137,6 +140,7 @@ struct AttendArgs {
     void *out; int64_t out_b, out_l, out_h;   // of x_dtype, by value head or (DOTS) by key head; NULL: to `share`
     float *share;
     double *dots;
+    float *selves, *uz;                  // dk, with beta
 };
 
 // `out`: from whole vectors to rows as they are, else the other way round.

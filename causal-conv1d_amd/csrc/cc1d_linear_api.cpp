@@ -211,6 +211,10 @@ size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &
     }
     w.dot_q = work.doubles(heads * kSegment);
     w.dot_k = work.doubles(heads * kSegment);
+    if (p.beta != nullptr) {
+        w.self_k = work.floats(heads * kSegment);
+        w.qk = work.floats((size_t)w.slots * p.heads * kSegment);
+    }
     if (w.shares > 1) {
         const size_t plane = (size_t)p.batch * p.seqlen * p.heads * padded(p.dim_k);
         w.share_q = work.floats(w.shares * plane);
@@ -341,7 +345,7 @@ int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, const Backwa
     dk.state = w.by_v;
     dk.first = bp.dfinal_states != nullptr;
     set_out(dk, f.dk);
-    dk.share = w.share_k; dk.dots = w.dot_k;
+    dk.share = w.share_k; dk.dots = w.dot_k; dk.selves = w.self_k; dk.uz = w.qk;
     AttendArgs d = {};                   // dv
     d.x = f.k; d.y = f.q; d.z = f.dout;
     d.d1 = p.dim_k; d.d2 = p.dim_v;

@@ -17,7 +17,7 @@
 // an entry; there the tiles beyond the diagonal are left out.  Where gates grow (g > 0), each factor has to stay below 2^128.
 //
 // DOTS: several value heads of a key head one after the other, the sum of their rows kept in registers, and of each the rows' products with u
-// (q or k), which the gates' gradients are made of.  What several workgroups of a key head leave is joined by linear_join_kernel.
+// (q or k), which the gates' gradients are made of.  There a row's own z stays out of the products; it joins the sum of the heads at the end, with a weight in fp32.  What several workgroups of a key head leave is joined by linear_join_kernel.
 //
 // float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 196 us (with sums and scan), backward 552; bfloat16 of 256 x 256:
 // 330 and 952.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
@@ -38,6 +38,7 @@ struct AttendLds {
     GateLds gates;
     float f[kChunk], s[kChunk];
     double dots[4][kChunk];
+    float of_self[kChunk];               // the weighted product of a token with itself
 };
 
 // Left operands of four tiles against one right one, their chains side by side.
@@ -108,6 +109,19 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
     const bool cut = a.d1 < 32 * KS * slabs;
     const bool has_state = (REV ? !at.last : at.c > 0) || a.first;
 
+    auto token = [&](int t) { return t < at.count ? t : at.count - 1; };           // (rows behind the last weigh nothing, or are not stored)
+    auto ask_rows = [&](const uint8_t *base, uint32_t pitch, int i, T (&r)[4][CP][2]) {          // rows as a result has them; columns that are not there: the first
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const T *row = reinterpret_cast<const T *>(base + (uint32_t)token(row0 + i0 + 16 * i + 4 * g + e) * pitch);
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+                const int col = 32 * (pair0 + 4 * c) + 2 * m;
+                r[e][c][0] = row[col < a.d2 ? col : 0];
+                r[e][c][1] = row[col + 1 < a.d2 ? col + 1 : 0];
+            }
+        }
+    };
     f32x4 total[DOTS ? RT : 1][DOTS ? CP : 1][2];
     if constexpr (DOTS)
 #pragma unroll
@@ -116,6 +130,10 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
             for (int c = 0; c < CP; ++c) total[i][c][0] = total[i][c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     f32x4 acc[RT][CP][2];
 
+    float self_sum = 0.f;                                // wavefront 0: of row `lane`, over the heads
+    auto all_columns = [&]() {                           // of row `lane`, from the wavefronts that have it
+        return RT == 2 ? lds.dots[2 * (lane >> 5)][lane] + lds.dots[2 * (lane >> 5) + 1][lane] : (lds.dots[0][lane] + lds.dots[1][lane]) + (lds.dots[2][lane] + lds.dots[3][lane]);
+    };
     for (int hi = 0; hi < h_count; ++hi) {
         if constexpr (DOTS) {                            // (addresses are made anew: kept over the loop they would take a hundred registers)
             asm volatile("" : "+v"(lane));
@@ -128,7 +146,6 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
         const T *xb = rows_of(a.x), *yb = rows_of(a.y);
         const uint8_t *zb = reinterpret_cast<const uint8_t *>(rows_of(a.z));
         const uint32_t z_pitch = (uint32_t)(a.z.sl * (int64_t)sizeof(T));
-        auto token = [&](int t) { return t < at.count ? t : at.count - 1; };       // (rows behind the last weigh nothing, or are not stored)
 
         Row8<DT, true> yr[KS];
         auto ask_y = [&](int c, int slab) {
@@ -316,7 +333,9 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float d = REV ? (hj[e] - hx) + (lj[e] - lx) : (hx - hj[e]) + (lx - lj[e]);
-                            x[e] = (REV ? j0 + e >= i : j0 + e <= i) ? pt[t][e] * (cj[e] * exp_of(d)) : 0.f;
+                            // DOTS: without the token itself
+                            x[e] = (DOTS ? (REV ? j0 + e > i : j0 + e < i) : REV ? j0 + e >= i : j0 + e <= i) ? pt[t][e] * (cj[e] * exp_of(d)) : 0.f;
+                            if (DOTS && j0 + e == i) lds.of_self[16 * t + m] = pt[t][e] * cj[e];
                         }
                     } else {
 #pragma unroll
@@ -355,22 +374,13 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
         }
 
         if constexpr (DOTS) {
-            const T *ub = rows_of(a.u);
+            const uint8_t *ub = reinterpret_cast<const uint8_t *>(rows_of(a.u));
             const uint32_t u_pitch = (uint32_t)(a.u.sl * (int64_t)sizeof(T));
             double dot[RT][4];
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 T u[4][CP][2];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const T *row = reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(ub) + (uint32_t)token(row0 + i0 + 16 * i + 4 * g + e) * u_pitch);
-#pragma unroll
-                    for (int c = 0; c < CP; ++c) {
-                        const int col = 32 * (pair0 + 4 * c) + 2 * m;
-                        u[e][c][0] = row[col < a.d2 ? col : 0];
-                        u[e][c][1] = row[col + 1 < a.d2 ? col + 1 : 0];
-                    }
-                }
+                ask_rows(ub, u_pitch, i, u);
                 stay();
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -397,10 +407,55 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
             }
             lds_barrier();
             if (wave == 0 && lane < own) {
-                const double d = RT == 2 ? lds.dots[2 * (lane >> 5)][lane] + lds.dots[2 * (lane >> 5) + 1][lane]
-                                  : (lds.dots[0][lane] + lds.dots[1][lane]) + (lds.dots[2][lane] + lds.dots[3][lane]);
+                const float of_self = lds.of_self[lane];
+                self_sum = fmaf(of_self, lds.s[lane], self_sum);
+                if (a.selves != nullptr) a.selves[sv * kSegment + row0 + lane] = of_self;
+                const double d = all_columns();
                 a.dots[sv * kSegment + row0 + lane] = REV ? d : (double)p.scale * d;
             }
+        }
+    }
+
+    if constexpr (DOTS) {                                // the tokens themselves
+        if (wave == 0) lds.of_self[lane] = self_sum;     // (read by that lane alone so far)
+        lds_barrier();
+        auto of_key = [&](const LinearRows &t, int i, T (&r)[4][CP][2]) {
+            ask_rows(reinterpret_cast<const uint8_t *>(static_cast<const T *>(t.p) + at.b * t.sb + at.lo * t.sl + hk * t.sh), (uint32_t)(t.sl * (int64_t)sizeof(T)), i, r);
+        };
+        const bool uz = a.uz != nullptr && share == 0;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            T z[4][CP][2];
+            of_key(a.z, i, z);
+            const f32x4 by = *reinterpret_cast<const f32x4 *>(&lds.of_self[i0 + 16 * i + 4 * g]);
+            stay();
+            if (uz) {
+                T u[4][CP][2];
+                of_key(a.u, i, u);
+                stay();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    double sum = 0.0;
+#pragma unroll
+                    for (int c = 0; c < CP; ++c) {
+                        const int col = 32 * (pair0 + 4 * c) + 2 * m;
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) sum += col + n < a.d2 ? (double)Elem<DT>::to_float(z[e][c][n]) * (double)Elem<DT>::to_float(u[e][c][n]) : 0.0;
+                    }
+                    sum = over_columns(sum);
+                    if (m == 0) lds.dots[wave][i0 + 16 * i + 4 * g + e] = sum;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < CP; ++c)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) total[i][c][n][e] = fmaf(by[e], Elem<DT>::to_float(z[e][c][n]), total[i][c][n][e]);
+        }
+        if (uz) {
+            lds_barrier();
+            if (wave == 0 && lane < own) a.uz[((int64_t)slot * p.heads + hk) * kSegment + row0 + lane] = (float)all_columns();
         }
     }
 

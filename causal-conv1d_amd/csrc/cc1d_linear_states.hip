@@ -325,7 +325,9 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
         float beta = 1.f;
         if (p.beta != nullptr) beta = bits_as_float(load_bits(p.beta, at.b * p.beta_stride_b + (at.lo + there) * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype), p.beta_dtype);
         const double qd = w.dot_q[(int64_t)sv * kSegment + there], z = w.dot_k[(int64_t)sv * kSegment + there];
-        kz[b] = (float)z;
+        kz[b] = 0.f;
+        if (p.beta != nullptr)
+            kz[b] = (float)(z + (double)w.self_k[(int64_t)sv * kSegment + there] * (double)w.qk[((int64_t)slot * p.heads + divided((uint32_t)h, w.by_group)) * kSegment + there]);
         change[b] = t < at.count ? qd - (double)beta * z : 0.0;
     }
     double dg = at.c > 0 || first ? inner(sv) : 0.0, rest = 0.0;

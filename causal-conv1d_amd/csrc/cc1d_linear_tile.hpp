@@ -38,6 +38,7 @@ struct TileLds {
     float of_x[kSegment], of_y[kSegment];                              // factors of E
     float weigh[kSegment], back[kSegment];                             // y's weight; where x and y share 32 tokens: exp(G at their start - G)
     float f[kSegment], s[kSegment];
+    float of_self[kSegment];             // the weighted product of a token with itself
     double ends[kSteps + 1];             // G at the borders of 32 tokens
     double sums[kBlocks];
     int32_t steep[kSteps];               // whether `back` is too large to be used
@@ -165,6 +166,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
     const bool rows = own < steps, whole = (own + 1) * kStep <= at.count;
     auto token = [&](int t) { return t < at.count ? t : at.count - 1; };           // (rows behind the last weigh nothing, or are not stored)
 
+    float self_sum[2] = {0.f, 0.f};      // of row 16 i + 4 g + m, m < 4, over the heads
     f32x4 total[JOIN ? 2 : 1][JOIN ? W : 1], acc[2][W];
     if constexpr (JOIN)
 #pragma unroll
@@ -216,6 +218,22 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
             const int f = wave + 8 * i < SB * STATE ? wave + 8 * i : SB * STATE - 1, s = stage * SB + f / STATE, step = s < a.steps ? s : a.steps - 1;
             in_state[i] = *reinterpret_cast<const u32x4 *>(st + (step * a.tiles * PT + f % STATE) * kFrag);
         }
+    };
+    // DOTS, rows 16 i + 4 g + (0 .. 3) of this wavefront's 32: of u columns W m .. W m + W - 1, of z column W m + t.
+    auto both_of = [](uint32_t two, float &first, float &second) {
+        if constexpr (DT == CC1D_F16) { first = (float)bitcast<f16x2>(two).x; second = (float)bitcast<f16x2>(two).y; }
+        else { first = bitcast<float>(two << 16); second = bitcast<float>(two & 0xffff0000u); }
+    };
+    auto ask_u = [&](int i, Wide8<W> &u) {
+        const uint8_t *ub = static_cast<const uint8_t *>(a.u.p) + (at.b * a.u.sb + at.lo * a.u.sl + hk * a.u.sh) * (int64_t)sizeof(T);      // (of the key head)
+        const uint32_t u_pitch = (uint32_t)(a.u.sl * (int64_t)sizeof(T)), col = (uint32_t)(W * m < a.d2 ? W * m : 0) * (uint32_t)sizeof(T);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u.ask(e, ub + ((uint32_t)token(own * kStep + 16 * i + 4 * g + e) * u_pitch + col));
+    };
+    auto z_rows = [&](int i, int t, float (&f)[4]) {
+        const u32x2 r = *reinterpret_cast<const u32x2 *>(lds.z + (own * W + t) * kFrag + ((2 * i + (g >> 1)) * 16 + m) * 16 + (g & 1) * 8);
+        both_of(r.x, f[0], f[1]);
+        both_of(r.y, f[2], f[3]);
     };
     // In the order in which it is needed.  DOTS: y is the value head's, x too; else z is.
     ask_gates();
@@ -369,6 +387,15 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                 bf16x8 f[2][PT];
                 if (self) {
                     const int yj = own * kStep + 8 * g;
+                    if constexpr (DOTS) {                // of x's row m: lane (m, 2 i + m / 8) has it
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float both = 0.f;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) both = (m & 7) == e ? pt[i][e >> 2][e & 3] : both;
+                            if (g == 2 * i + (m >> 3)) lds.of_self[own * kStep + 16 * i + m] = both * lds.weigh[own * kStep + 16 * i + m];
+                        }
+                    }
                     if (lds.steep[own] != 0) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
@@ -399,7 +426,10 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                     for (int i = 0; i < 2; ++i) {
                         float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = (REV ? 8 * g + e >= 16 * i + m : 8 * g + e <= 16 * i + m) ? pt[i][e >> 2][e & 3] : 0.f;
+                        for (int e = 0; e < 8; ++e) {    // (DOTS: without the token itself)
+                            const int y_row = 8 * g + e, x_row = 16 * i + m;
+                            v[e] = (DOTS ? (REV ? y_row > x_row : y_row < x_row) : REV ? y_row >= x_row : y_row <= x_row) ? pt[i][e >> 2][e & 3] : 0.f;
+                        }
                         split8<PT>(v, f[i]);
                     }
                 } else {
@@ -434,16 +464,14 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
         }
         stay();
         if constexpr (DOTS) {
-            const uint8_t *ub = static_cast<const uint8_t *>(a.u.p) + (at.b * a.u.sb + at.lo * a.u.sl + hk * a.u.sh) * (int64_t)sizeof(T);      // (of the key head)
             if (more) ask_x();
             if (rows) {
-                const uint32_t u_pitch = (uint32_t)(a.u.sl * (int64_t)sizeof(T)), col = (uint32_t)(W * m < a.d2 ? W * m : 0) * (uint32_t)sizeof(T);
+                wave_lds_fence();                        // of_self
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int row = own * kStep + 16 * i + 4 * g;
                     Wide8<W> u;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) u.ask(e, ub + ((uint32_t)token(row + e) * u_pitch + col));
+                    ask_u(i, u);
                     stay();
                     double dot[4];
 #pragma unroll
@@ -451,16 +479,19 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                         float sum_u = 0.f;
 #pragma unroll
                         for (int t = 0; t < W / 2; ++t) {
-                            const uint32_t two = u.r[e][t];
                             float u0, u1;
-                            if constexpr (DT == CC1D_F16) { u0 = (float)bitcast<f16x2>(two).x; u1 = (float)bitcast<f16x2>(two).y; }
-                            else { u0 = bitcast<float>(two << 16); u1 = bitcast<float>(two & 0xffff0000u); }
+                            both_of(u.r[e][t], u0, u1);
                             sum_u = fmaf(acc[i][2 * t][e], u0, fmaf(acc[i][2 * t + 1][e], u1, sum_u));
                         }
                         dot[e] = over_columns(W * m < a.d2 ? (double)sum_u : 0.0);
                     }
                     const double mine_dot = m == 1 ? dot[1] : m == 2 ? dot[2] : m == 3 ? dot[3] : dot[0];
-                    if (m < 4 && row + m < at.count) a.dots[sv * kSegment + row + m] = REV ? mine_dot : (double)p.scale * mine_dot;
+                    const float of_self = lds.of_self[row + (m & 3)];
+                    self_sum[i] = fmaf(of_self, lds.s[row + (m & 3)], JOIN ? self_sum[i] : 0.f);
+                    if (m < 4 && row + m < at.count) {
+                        a.dots[sv * kSegment + row + m] = REV ? mine_dot : (double)p.scale * mine_dot;
+                        if (a.selves != nullptr) a.selves[sv * kSegment + row + m] = of_self;
+                    }
                     const f32x4 by = *reinterpret_cast<const f32x4 *>(&lds.s[row]);
 #pragma unroll
                     for (int t = 0; t < W; ++t) {
@@ -476,6 +507,43 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                 const int first = 16 * i + 4 * g;
                 f32x4 s = {1.f, 1.f, 1.f, 1.f};
                 if constexpr (!DOTS) s = *reinterpret_cast<const f32x4 *>(&lds.s[own * kStep + first]);
+                if constexpr (DOTS) {                    // the tokens themselves
+                    if (m < 4) lds.of_self[own * kStep + first + m] = self_sum[i];
+                    wave_lds_fence();
+                    const f32x4 by = *reinterpret_cast<const f32x4 *>(&lds.of_self[own * kStep + first]);
+                    if (a.uz != nullptr && share == 0) {
+                        Wide8<W> u;
+                        ask_u(i, u);
+                        float sum_uz[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int t = 0; t < W; t += 2) {
+                            float z0[4], z1[4];
+                            z_rows(i, t, z0);
+                            z_rows(i, t + 1, z1);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float u0, u1;
+                                both_of(u.r[e][t / 2], u0, u1);
+                                sum_uz[e] = fmaf(u0, z0[e], fmaf(u1, z1[e], sum_uz[e]));
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float all = over_columns(W * m < a.d2 ? sum_uz[e] : 0.f);
+                            if (m == e && own * kStep + first + e < at.count) a.uz[((int64_t)slot * p.heads + hk) * kSegment + own * kStep + first + e] = all;
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < W; ++t) {
+                        float zt[4];
+                        z_rows(i, t, zt);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (JOIN) total[i][t][e] = fmaf(by[e], zt[e], total[i][t][e]);
+                            else acc[i][t][e] = fmaf(by[e], zt[e], acc[i][t][e]);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float o[W];

@@ -3,7 +3,11 @@
 dbeta[j] is the sum over i of E_ij (dout_i.v_j) (q_i.k_j), E_ij = exp(G_i - G_j).  With 2^-25.3 for the mean square of a rounding to 24 bits, E is a product of
 two or three exponentials (2^-23.9 each with the last rounding of its own, 2^-23 at worst) and meets three more products: 2^-23.1.  Sums: 2^-24.3 for
 dout.v, four steps of 32 columns; 2^-23.8 for the rows times z, eight steps of 32 tokens; 2^-24.3 for the products inside a lane.  Together 2^-22.7; twice
-that is the bound."""
+that is the bound.
+
+dg is a running sum, over 256 tokens at most, of what token t reads less what it wrote, without its own share in either: dg[t] - dg[t+1], each side
+with the error above.  Closed at both ends of a segment, the running sum of n independent errors is off by sqrt(n / 6) of one.  Where gates are strong
+a token's own share is nearly all of q.dq and of k.dk, and nothing of dg."""
 import pytest
 import torch
 
@@ -11,6 +15,10 @@ import linear_cases as cases
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 DBETA = 2.0 ** -21.7
+
+
+def bound_of_dg(want):
+    return DBETA * (256 / 6) ** 0.5 * (torch.diff(want, dim=1).norm() / want.norm()).item()
 
 
 def off(got, want):
@@ -60,3 +68,28 @@ def test_weights_gradient_behind_strong_gates(pkg, gpu_device, dtype, dims, head
     s["beta"] = s["beta"].float()
     got, want = cases.run(pkg, s, dfinal=False), cases.reference(s, dfinal=False)
     assert off(got["dbeta"], want["dbeta"]) <= DBETA, off(got["dbeta"], want["dbeta"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dims", [(64, 64), (128, 64), (64, 128), (128, 128), (160, 96), (96, 192)])
+@pytest.mark.parametrize("rate", [0.02, 0.3, 1.6, 5.0])
+def test_gates_gradient(pkg, gpu_device, dtype, dims, rate):
+    s = cases.inputs(gpu_device, 1, 320, 1, 2, *dims, dtype, seed=dims[0])
+    s["g"] = -rate * (0.9 + 0.2 * torch.rand(1, 320, 2, generator=torch.Generator(device=gpu_device).manual_seed(3), device=gpu_device))
+    s["beta"] = s["beta"].float()
+    got, want = cases.run(pkg, s), cases.reference(s)
+    assert off(got["dg"], want["dg"]) <= bound_of_dg(want["dg"]), (off(got["dg"], want["dg"]), bound_of_dg(want["dg"]))
+    assert off(got["dbeta"], want["dbeta"]) <= DBETA, off(got["dbeta"], want["dbeta"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dims", [(32, 32), (72, 72)])
+def test_gates_gradient_of_many_heads(pkg, gpu_device, dims):
+    """Several value heads a workgroup, several workgroups a key head."""
+    s = cases.inputs(gpu_device, 4, 200, 1, 80, *dims, BF16, states=False)
+    s["g"], s["beta"] = s["g"] * 40, s["beta"].float()
+    got, want = cases.run(pkg, s, dfinal=False), cases.reference(s, dfinal=False)
+    assert off(got["dg"], want["dg"]) <= bound_of_dg(want["dg"])
+    assert off(got["dbeta"], want["dbeta"]) <= DBETA
+    cases.check(got, s, dfinal=False)
