@@ -317,7 +317,7 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
         for (int64_t i = lane; i < w.tiles(); i += 64) sum += w.inner[of * w.tiles() + i];
         return over_wave(sum);
     };
-    double change[kBlocks], total = 0.0;
+    double change[kBlocks], size[kBlocks], total = 0.0, sizes = 0.0;
     float kz[kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
@@ -329,23 +329,26 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
         if (p.beta != nullptr)
             kz[b] = (float)(z + (double)w.self_k[(int64_t)sv * kSegment + there] * (double)w.qk[((int64_t)slot * p.heads + divided((uint32_t)h, w.by_group)) * kSegment + there]);
         change[b] = t < at.count ? qd - (double)beta * z : 0.0;
+        size[b] = t < at.count ? fabs(qd) + fabs((double)beta * z) : 0.0;
     }
     double dg = at.c > 0 || first ? inner(sv) : 0.0, rest = 0.0;
     const bool known = !at.last || !bp.dfinal_states;    // what comes behind the last token
     const double end = at.last || !known ? 0.0 : inner((int64_t)sv + p.v_heads);
-    double before[kBlocks];                              // changes in front of each token
+    double before[kBlocks], share[kBlocks];              // changes in front of each token, and the sizes of what they are differences of
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
-        const double sum = running_sum(change[b]);
+        const double sum = running_sum(change[b]), all = running_sum(size[b]);
         before[b] = total + (sum - change[b]);
+        share[b] = sizes + (all - size[b]);
         total += of_lane(sum, 63);
+        sizes += of_lane(all, 63);
     }
     if (known) rest = end - (dg - total);
-    rest = fabs(rest) < 1e300 ? rest / at.count : 0.0;   // (of numbers)
+    rest = fabs(rest) < 1e300 && sizes > 0.0 ? rest / sizes : 0.0;       // (of numbers)
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
         const int t = b * kChunk + lane;
-        if (t < at.count) put(((int64_t)at.b * p.seqlen + at.lo + t) * p.v_heads + h, (float)((dg - before[b]) + rest * t), kz[b]);
+        if (t < at.count) put(((int64_t)at.b * p.seqlen + at.lo + t) * p.v_heads + h, (float)((dg - before[b]) + rest * share[b]), kz[b]);
     }
 }
 

@@ -6,7 +6,8 @@ dout.v, four steps of 32 columns; 2^-23.8 for the rows times z, eight steps of 3
 that is the bound.
 
 dg is a running sum, over 256 tokens at most, of what token t reads less what it wrote, without its own share in either: dg[t] - dg[t+1], each side
-with the error above.  Closed at both ends of a segment, the running sum of n independent errors is off by sqrt(n / 6) of one.  Where gates are strong
+with the error above.  Closed at both ends of a segment, the running sum of n independent errors is off by sqrt(n / 6) of one, and no token's by more than
+those in front of it make.  Where gates are strong
 a token's own share is nearly all of q.dq and of k.dk, and nothing of dg."""
 import pytest
 import torch
@@ -93,3 +94,16 @@ def test_gates_gradient_of_many_heads(pkg, gpu_device, dims):
     assert off(got["dg"], want["dg"]) <= bound_of_dg(want["dg"])
     assert off(got["dbeta"], want["dbeta"]) <= DBETA
     cases.check(got, s, dfinal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128), (160, 96)])
+def test_gates_gradient_in_front_of_larger_ones(pkg, gpu_device, dtype, dims):
+    """Strong gates with small gradients, and behind them, in the same segment, weak ones with gradients some thousand times as large.  (Behind larger ones
+    the running sum keeps their error.)"""
+    s = cases.inputs(gpu_device, 1, 320, 1, 2, *dims, dtype, states=False, seed=dims[0])
+    s["g"][:, :128] = s["g"][:, :128] - 6.0
+    s["beta"] = s["beta"].float()
+    got, want = cases.run(pkg, s, dfinal=False)["dg"][:, :128], cases.reference(s, dfinal=False)["dg"][:, :128]
+    assert off(got, want) <= bound_of_dg(want), (off(got, want), bound_of_dg(want))
