@@ -10,8 +10,8 @@ weight, or None for 1.  g and beta are of any of the three dtypes.  v_heads is a
 h // (v_heads // heads).  Any strides with the last dimension contiguous are taken as they are, so q, k and v may be column slices
 of the channel-last convolution's output.  A state-space block with a step size dt and rates A is v = x, k = B, q = C, g = dt A, beta = dt, scale = 1.
 
-Gates below -200 count as -200, which leaves nothing of a float32 state.  They may be positive, as long as a state grows by less than 2^128 over
-256 tokens.  Whole sequences are worked through in blocks of 64 tokens: a NaN or an infinity reaches its own head's outputs from the start of
+Gates below -200 count as -200, which leaves nothing of a float32 state.  They may be positive, as long as they add up to less than 32 (a state grows by
+less than 2^46) over any run of at most 256 tokens: beyond that, what falls far and is brought back may be lost.  Whole sequences are worked through in blocks of 64 tokens: a NaN or an infinity reaches its own head's outputs from the start of
 its block on.  Other heads, sequences and earlier blocks do not see it.
 
 There is no host path.  `linear_attention_ref` states the operator in plain PyTorch.

@@ -14,7 +14,9 @@
 // split into its terms and passed through LDS once, double-buffered, one barrier a block.
 //
 // E between two blocks is a product of two factors, exp(G_i - R) and exp(R - G_j), R between them, so that only a block with itself takes an exponential
-// an entry; there the tiles beyond the diagonal are left out.  Where gates grow (g > 0), each factor has to stay below 2^128.
+// an entry; there the tiles beyond the diagonal are left out.  A factor below e^-87 is nothing, whatever
+// the others are: with gates that add up to no more than 32 over any run of tokens, two of those lift it by e^64 at most, and what is lost weighs less than e^-23.
+// (An exponential an entry wherever a gate is positive: linear_tile_pair_kernel<bfloat16, 2, 8, several heads> 4 % slower for all gates.)
 //
 // DOTS: several value heads of a key head one after the other, the sum of their rows kept in registers, and of each the rows' products with u
 // (q or k), which the gates' gradients are made of.  There a row's own z stays out of the products; it joins the sum of the heads at the end, with a weight in fp32.  What several workgroups of a key head leave is joined by linear_join_kernel.

@@ -142,7 +142,7 @@ int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
  *
  * Short sequences go token by token, packed ones each by its own length; the others in segments of 256 tokens, worked out in blocks of 64: a NaN or infinity reaches its
  * head's outputs from the start of its 64 tokens on.  Gates are bounded from below by -200, which forgets everything.  Where they
- * are positive, the states may grow by less than 2^128 over 256 tokens.
+ * are positive, they may add up to less than 32 over any run of at most 256 tokens (a state may grow by less than 2^46).
  * Precision is the gated delta rule's; the factors that make out and dv of 16 bits carry 2^-17.
  * Tokens 2^23 bytes apart or more (in q, k, v or out) go by tokens in the forward; there, with `saved`, and in the backward (in q, k, v, dout or their
  * gradients) they are refused with CC1D_ERR_TOO_LARGE.  Tensors whose rows are not whole 16-byte vectors of 8 columns are copied to the
