@@ -59,17 +59,6 @@ int64_t segments_from(const cc1d_delta_params &p, int64_t sequences) {
     const int64_t from = 16 + (int64_t)(most * (0.016 + 0.03 * size)), cap = heads * size >= 512.0 ? 50 : 96;
     return from < cap ? from : cap;
 }
-// The average says nothing of the longest.  Packed sequences that go by tokens on average go by segments one by one, from 256 tokens on: the
-// kernels see their lengths, the host does not.  Not where all their tokens together are few, nor where one sequence's heads fill
-// the card with tokens.
-enum class Way { tokens, segments, both };
-Way way_of(const cc1d_delta_params &p) {
-    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return Way::tokens;
-    if (p.saved != nullptr) return Way::segments;
-    if (!reachable_out(p)) return Way::tokens;
-    if (p.seqlen >= segments_from(p, p.sequences) * (p.cu_seqlens == nullptr ? 1 : p.sequences)) return Way::segments;
-    return p.cu_seqlens != nullptr && p.seqlen >= 2 * kSegment && segments_from(p, 1) <= kSegment ? Way::both : Way::tokens;
-}
 // Whether any segment has a state in front of it.
 bool has_states(const cc1d_delta_params &p, const SegmentWork &w) { return w.chunks > 1 || p.cu_seqlens != nullptr || p.initial_states != nullptr; }
 
@@ -175,6 +164,26 @@ size_t lay_out_fwd(const cc1d_delta_params &p, bool alone, uint8_t *base, Segmen
     f.out = t.written(ROWS(p, out, false), p.dim_v);
     f.in = t.in; f.ins = t.ins; f.back = t.out; f.backs = t.outs;
     return work.used;
+}
+
+// Without `saved` the token kernel takes what the segments' do not.
+bool segments_fit(const cc1d_delta_params &p, bool alone) {
+    SegmentWork w;
+    Forward f;
+    lay_out_fwd(p, alone, nullptr, w, f);
+    return grids_fit(p, w, 1) && reachable_out(p) && (f.ins + f.backs == 0 || copies_reachable(p));
+}
+// The average says nothing of the longest.  Packed sequences that go by tokens on average go by segments one by one, from 256 tokens on: the
+// kernels see their lengths, the host does not.  Not where all their tokens together are few, nor where one sequence's heads fill
+// the card with tokens.
+enum class Way { tokens, segments, both };
+Way way_of(const cc1d_delta_params &p) {
+    if (p.batch == 0 || p.v_heads == 0 || p.sequences == 0 || p.seqlen == 0) return Way::tokens;
+    if (p.saved != nullptr) return Way::segments;
+    if (!reachable_out(p)) return Way::tokens;
+    const Way way = p.seqlen >= segments_from(p, p.sequences) * (p.cu_seqlens == nullptr ? 1 : p.sequences) ? Way::segments :
+                    p.cu_seqlens != nullptr && p.seqlen >= 2 * kSegment && segments_from(p, 1) <= kSegment ? Way::both : Way::tokens;
+    return way == Way::tokens || segments_fit(p, way == Way::both) ? way : Way::tokens;
 }
 
 // Value heads that a workgroup takes one after the other, of `items` (slots and value heads): what belongs to their key head is read once for
@@ -379,7 +388,7 @@ int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes) {
     SegmentWork w;
     Forward f;
     *bytes = lay_out_fwd(*p, way == Way::both, nullptr, w, f);
-    return grids_fit(*p, w, 1) && reachable_out(*p) && (f.ins + f.backs == 0 || copies_reachable(*p)) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
+    return p->saved == nullptr || segments_fit(*p, false) ? CC1D_OK : CC1D_ERR_TOO_LARGE;
 }
 
 int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {

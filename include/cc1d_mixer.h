@@ -144,9 +144,10 @@ int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
  * head's outputs from the start of its 64 tokens on.  Gates are bounded from below by -200, which forgets everything.  Where they
  * are positive, they may add up to less than 32 over any run of at most 256 tokens (a state may grow by less than 2^46).
  * Precision is the gated delta rule's; the factors that make out and dv of 16 bits carry 2^-17.
- * Tokens 2^23 bytes apart or more (in q, k, v or out) go by tokens in the forward; there, with `saved`, and in the backward (in q, k, v, dout or their
- * gradients) they are refused with CC1D_ERR_TOO_LARGE.  Tensors whose rows are not whole 16-byte vectors of 8 columns are copied to the
- * workspace, whose size is therefore of these pointers and strides; it is refused where v_heads such rows take 2^23 bytes.
+ * Tensors whose rows are not whole 16-byte vectors of 8 columns are copied to the workspace, whose size is therefore of these pointers and strides.
+ * Tokens 2^23 bytes apart or more (in q, k, v or out), v_heads rows to be copied of 2^23 bytes together, and more than 2^21 segments times value heads go by tokens in
+ * the forward; there, with `saved`, and in the backward (tokens of dout and the gradients too, and half as many segments) they are refused with
+ * CC1D_ERR_TOO_LARGE.
  * ---------------------------------------------------------------------------------- */
 int cc1d_validate_linear(const cc1d_delta_params *p);
 int cc1d_linear_workspace_bytes(const cc1d_delta_params *p, size_t *bytes);
