@@ -33,7 +33,7 @@ def _new_states(q, v, cu_seqlens):
 
 
 class LinearAttentionFn(torch.autograd.Function):
-    """Saves the inputs and the state in front of every 256 tokens, 6 bytes an element."""
+    """Saves the inputs and the states between segments of 256 tokens (with initial states that in front of the first too), 6 bytes an element."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, scale, initial_states, return_final_states, cu_seqlens):

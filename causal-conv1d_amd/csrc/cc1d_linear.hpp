@@ -50,17 +50,20 @@ inline int operand_width(int dtype, int d1, int d2, bool gradient_of_keys) {
 }
 inline int operand_tiles(int width, int d2) { return (d2 + 16 * width - 1) / (16 * width) * width; }
 
+// States lie by borders between a sequence's segments (border_behind), of which packed sequences of a few tokens have none; where a state in front of the
+// first segment or behind the last is there too, by slots.
 struct SegmentWork {
     int32_t slots, chunks;               // segments of the call; of one sequence without cu_seqlens
+    int64_t borders;
     int32_t kp, vp;                      // 32-column steps of dim_k, dim_v
     FastDiv by_v_heads, by_chunks, by_group;
-    float *local;                        // per (slot, value head): a segment's own sum, [kp][vp] tiles of 32 x 32 in operand order
+    float *local;                        // per (state, value head): a segment's own sum, [kp][vp] tiles of 32 x 32 in operand order
     float *decay;                        // per (slot, value head): exp(Gend)
-    uint8_t *by_k, *by_v;                // per (slot, value head): states split into operands, contracted over dim_k and over dim_v
+    uint8_t *by_k, *by_v;                // per (state, value head): states split into operands, contracted over dim_k and over dim_v
     uint8_t *first;                      // S0 of the forward, contracted over dim_v: what a training forward saves
-    double *dot_q, *dot_k;               // per (slot, value head): q.dq and k.(dk / beta) of each token, without its own share
-    float *self_k, *qk;                  // that share of k.(dk / beta) is self_k qk: scale dout.v; per (slot, key head): q.k
-    double *inner;                       // per (slot, value head): S0 . dS0, a partial sum each tile
+    double *dot_q, *dot_k;               // (batch, v_heads, seqlen): q.dq and k.(dk / beta) of each token, without its own share
+    float *self_k, *qk;                  // that share of k.(dk / beta) is self_k qk: scale dout.v; (batch, heads, seqlen): q.k
+    double *inner;                       // per (state, value head): S0 . dS0, a partial sum each tile
     float *share_q, *share_k;            // shares of dq, dk of heads_each value heads: (shares, batch, seqlen, heads, dim_k)
     int32_t k_width, v_width, k_tiles, v_tiles;                // of operands contracted over dim_k (out, dv), over dim_v (dq, dk)
     int32_t heads_each, shares;          // value heads of a workgroup of the gradients of q and k; such workgroups a key head
@@ -108,6 +111,12 @@ __device__ __forceinline__ SegmentAt segment_at(const cc1d_delta_params &p, cons
     if (c < 0 || left <= 0) return {0, 0, 0, n, 0, false};
     return {lo, (int)(left < kSegment ? left : kSegment), 0, n, (int)c, left <= kSegment};
 }
+// The border behind a segment, which the one in front of it is 1 less than: borders between 256 tokens of a packed sequence and the next lie behind different
+// tokens 256 f, as many segments as they are apart.
+__device__ __forceinline__ int64_t border_behind(const cc1d_delta_params &p, const SegmentWork &w, int n, int64_t lo, int c) {
+    return p.cu_seqlens == nullptr ? (int64_t)n * (w.chunks - 1) + c : lo >> kSegmentLog;
+}
+__device__ __forceinline__ int64_t border_behind(const cc1d_delta_params &p, const SegmentWork &w, const SegmentAt &at) { return border_behind(p, w, at.n, at.lo, at.c); }
 __device__ __forceinline__ int first_segment(const cc1d_delta_params &p, const SegmentWork &w, int n, const TokenRange &r) {
     return p.cu_seqlens == nullptr ? n * w.chunks : w.shortest > 0 ? 2 * (int)naming(r) : (int)(r.lo >> kSegmentLog) + n;
 }

@@ -80,6 +80,7 @@ SegmentWork sizes_of(const cc1d_delta_params &p, bool alone) {
     w.chunks = (int32_t)(((int64_t)p.seqlen + kSegment - 1) / kSegment);
     const int64_t slots = p.cu_seqlens == nullptr ? (int64_t)p.batch * w.chunks : alone ? 2 * (int64_t)w.chunks : (int64_t)p.seqlen / kSegment + p.sequences + 1;
     w.slots = (int32_t)(slots < INT32_MAX ? slots : INT32_MAX);
+    w.borders = (int64_t)p.batch * (w.chunks > 0 ? w.chunks - 1 : 0);      // (packed: one behind every token 256 f but the last)
     w.kp = (p.dim_k + 31) / 32;
     w.vp = (p.dim_v + 31) / 32;
     w.k_width = operand_width(p.x_dtype, p.dim_k, p.dim_v, false);
@@ -91,10 +92,13 @@ SegmentWork sizes_of(const cc1d_delta_params &p, bool alone) {
     w.by_group = fast_div((uint32_t)(p.heads > 0 ? p.v_heads / p.heads : 1));
     return w;
 }
-// Numbers of 32 x 32 tiles: of one state for every slot and value head; bytes of its operands.
-size_t state_tiles(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.tiles(); }
-size_t by_k_bytes(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.kp * w.k_tiles * out_terms(p.x_dtype) * kFrag; }
-size_t by_v_bytes(const cc1d_delta_params &p, const SegmentWork &w) { return (size_t)w.slots * p.v_heads * w.vp * w.v_tiles * 3 * kFrag; }
+// Numbers of 32 x 32 tiles of states, at every border or at every segment, for every value head; bytes of their operands.
+size_t states_of(const cc1d_delta_params &p, const SegmentWork &w, bool all) { return (size_t)(all ? (int64_t)w.slots : w.borders) * p.v_heads; }
+size_t state_tiles(const cc1d_delta_params &p, const SegmentWork &w, bool all) { return states_of(p, w, all) * w.tiles(); }
+size_t by_k_bytes(const cc1d_delta_params &p, const SegmentWork &w, bool all) { return states_of(p, w, all) * w.kp * w.k_tiles * out_terms(p.x_dtype) * kFrag; }
+size_t by_v_bytes(const cc1d_delta_params &p, const SegmentWork &w, bool all) { return states_of(p, w, all) * w.vp * w.v_tiles * 3 * kFrag; }
+// `saved` is never nothing: it says that a backward follows.
+constexpr size_t kLeastSaved = 256;
 
 // One workgroup a (slot, block, value head, 128 columns) and less, of two such products at once in the backward; the scan's one wavefront a tile of each
 // sequence's states.
@@ -151,10 +155,9 @@ size_t lay_out_fwd(const cc1d_delta_params &p, bool alone, uint8_t *base, Segmen
     w = sizes_of(p, alone);
     Places work{base};
     if (has_states(p, w) || p.final_states != nullptr) {
-        const size_t tiles = state_tiles(p, w);
-        w.local = work.floats(tiles * 1024);
+        w.local = work.floats(state_tiles(p, w, p.final_states != nullptr) * 1024);
         w.decay = work.floats((size_t)w.slots * p.v_heads);
-        w.by_k = work.take(by_k_bytes(p, w));
+        w.by_k = work.take(by_k_bytes(p, w, p.initial_states != nullptr));
     }
     w.by_v = static_cast<uint8_t *>(p.saved);
     Tensors t(p, work);
@@ -203,26 +206,28 @@ void share_heads(const cc1d_delta_params &p, SegmentWork &w) {
 bool gradient_of_states(const cc1d_delta_bwd_params &bp, const SegmentWork &w) {
     return has_states(bp.fwd, w) || bp.dfinal_states != nullptr || bp.dinitial_states != nullptr;
 }
+// Sums of all segments, the first's too: its S0 . dS0 or the gradient of the initial states.
+bool needs_all_sums(const cc1d_delta_bwd_params &bp) { return bp.fwd.initial_states != nullptr || bp.dinitial_states != nullptr; }
 size_t lay_out_bwd(const cc1d_delta_bwd_params &bp, uint8_t *base, SegmentWork &w, Backward &f) {
     const cc1d_delta_params &p = bp.fwd;
     w = sizes_of(p, false);
     w.first = static_cast<uint8_t *>(p.saved);
     Places work{base};
     share_heads(p, w);
-    const size_t heads = (size_t)w.slots * p.v_heads;
+    const size_t tokens = (size_t)p.batch * p.seqlen;
     if (gradient_of_states(bp, w)) {
-        const size_t tiles = state_tiles(p, w);
-        w.local = work.floats(tiles * 1024);
-        w.decay = work.floats(heads);
-        w.by_k = work.take(by_k_bytes(p, w));
-        w.by_v = work.take(by_v_bytes(p, w));
-        w.inner = work.doubles(tiles);
+        const bool initial = p.initial_states != nullptr, final = bp.dfinal_states != nullptr;
+        w.local = work.floats(state_tiles(p, w, needs_all_sums(bp)) * 1024);
+        w.decay = work.floats((size_t)w.slots * p.v_heads);
+        w.by_k = work.take(by_k_bytes(p, w, final));
+        w.by_v = work.take(by_v_bytes(p, w, final));
+        w.inner = work.doubles(state_tiles(p, w, initial));
     }
-    w.dot_q = work.doubles(heads * kSegment);
-    w.dot_k = work.doubles(heads * kSegment);
+    w.dot_q = work.doubles(tokens * p.v_heads);
+    w.dot_k = work.doubles(tokens * p.v_heads);
     if (p.beta != nullptr) {
-        w.self_k = work.floats(heads * kSegment);
-        w.qk = work.floats((size_t)w.slots * p.heads * kSegment);
+        w.self_k = work.floats(tokens * p.v_heads);
+        w.qk = work.floats(tokens * p.heads);
     }
     if (w.shares > 1) {
         const size_t plane = (size_t)p.batch * p.seqlen * p.heads * padded(p.dim_k);
@@ -325,7 +330,7 @@ int backward(const cc1d_delta_bwd_params &bp, const SegmentWork &w, const Backwa
     const cc1d_delta_params &p = bp.fwd;
     int st = launch_linear_copy(f.in, f.ins, false, stream);
     if (st != CC1D_OK) return st;
-    const bool initial = p.initial_states != nullptr, to_end = initial || bp.dinitial_states != nullptr;
+    const bool initial = p.initial_states != nullptr, to_end = needs_all_sums(bp);
     if (w.slots > 0 && (w.chunks > 1 || p.cu_seqlens != nullptr || to_end)) {
         StatesArgs a = {};
         a.a = f.q; a.b = f.dout; a.from_start = 1; a.all = to_end; a.factor = p.scale;
@@ -400,7 +405,7 @@ int cc1d_linear_saved_bytes(const cc1d_delta_params *p, size_t *bytes) {
     const int st = cc1d_validate_delta(&q);
     if (st != CC1D_OK) return st;
     const SegmentWork w = sizes_of(*p, false);
-    *bytes = by_v_bytes(*p, w);
+    *bytes = kLeastSaved + by_v_bytes(*p, w, p->initial_states != nullptr);
     return CC1D_OK;
 }
 

@@ -110,6 +110,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
     const int slabs = (a.steps + KS - 1) / KS;
     const bool cut = a.d1 < 32 * KS * slabs;
     const bool has_state = (REV ? !at.last : at.c > 0) || a.first;
+    const int64_t state = a.first ? (int64_t)slot : border_behind(p, w, at) - !REV;
 
     auto token = [&](int t) { return t < at.count ? t : at.count - 1; };           // (rows behind the last weigh nothing, or are not stored)
     auto ask_rows = [&](const uint8_t *base, uint32_t pitch, int i, T (&r)[4][CP][2]) {          // rows as a result has them; columns that are not there: the first
@@ -143,7 +144,6 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
             g = lane >> 4;
         }
         const int h = h_first + hi;
-        const int64_t sv = (int64_t)slot * p.v_heads + h;
         auto rows_of = [&](const LinearRows &t) { return static_cast<const T *>(t.p) + at.b * t.sb + at.lo * t.sl + (t.by_key ? hk : h) * t.sh; };
         const T *xb = rows_of(a.x), *yb = rows_of(a.y);
         const uint8_t *zb = reinterpret_cast<const uint8_t *>(rows_of(a.z));
@@ -204,7 +204,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
 #pragma unroll
             for (int c = 0; c < CP; ++c) acc[i][c][0] = acc[i][c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (has_state) {
-            const uint8_t *st = a.state + sv * (int64_t)a.steps * a.tiles * PT * kFrag;
+            const uint8_t *st = a.state + (state * p.v_heads + h) * a.steps * a.tiles * PT * kFrag;
             for (int slab = 0; slab < slabs; ++slab) {
                 if (slab > 0) {
                     lds_barrier();
@@ -411,9 +411,10 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
             if (wave == 0 && lane < own) {
                 const float of_self = lds.of_self[lane];
                 self_sum = fmaf(of_self, lds.s[lane], self_sum);
-                if (a.selves != nullptr) a.selves[sv * kSegment + row0 + lane] = of_self;
+                const int64_t to = ((int64_t)at.b * p.v_heads + h) * p.seqlen + at.lo + row0 + lane;
+                if (a.selves != nullptr) a.selves[to] = of_self;
                 const double d = all_columns();
-                a.dots[sv * kSegment + row0 + lane] = REV ? d : (double)p.scale * d;
+                a.dots[to] = REV ? d : (double)p.scale * d;
             }
         }
     }
@@ -457,7 +458,7 @@ __device__ __forceinline__ void attend_rows(const cc1d_delta_params &p, const Se
         }
         if (uz) {
             lds_barrier();
-            if (wave == 0 && lane < own) a.uz[((int64_t)slot * p.heads + hk) * kSegment + row0 + lane] = (float)all_columns();
+            if (wave == 0 && lane < own) a.uz[((int64_t)at.b * p.heads + hk) * p.seqlen + at.lo + row0 + lane] = (float)all_columns();
         }
     }
 

@@ -92,11 +92,12 @@ linear_states_kernel(const cc1d_delta_params p, const SegmentWork w, const State
                 for (int c = 0; c < 2; ++c) acc[i][n][c] = product<2>(fa[i][n], fb[c], acc[i][n][c]);
         stay();
     }
+    const int64_t state = a.all ? (int64_t)slot : border_behind(p, w, at) - a.from_start;         // (of whom it meets)
     // Rows of a's pair i: dim_k index 32 (p0 + i) + 8 g + 2 e + n.  Padding is 0: it meets other operands' padding.
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
         if (p0 + i >= w.kp) break;
-        float *to = w.local + (((int64_t)sv * w.kp + p0 + i) * w.vp + q) * 1024 + lane * 8;
+        float *to = w.local + (((state * p.v_heads + h) * w.kp + p0 + i) * w.vp + q) * 1024 + lane * 8;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             float f[8];
@@ -168,21 +169,25 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
             s[c][e] = 0.f;
             if (a.first != nullptr && k0 + e < p.dim_k && v0 + c < p.dim_v) s[c][e] = a.first[n * a.first_n + h * a.first_h + (k0 + e) * a.first_k + v0 + c];
         }
-    auto place = [&](int slot) { return ((int64_t)slot * p.v_heads + h) * tiles + tile; };
+    // Segment c's own sum lies where the state does that it makes: behind it (REVERSE: in front), and states where the segment is that reads them.
+    const int64_t border0 = border_behind(p, w, n, range.lo, 0);
+    auto sum_of = [&](int c) { return a.to_end ? (int64_t)slot0 + c : border0 + c - a.reverse; };
+    auto state_of = [&](int c) { return a.first != nullptr ? (int64_t)slot0 + c : border0 + c - 1 + a.reverse; };
+    auto place = [&](int64_t state) { return (state * p.v_heads + h) * tiles + tile; };
     struct Step { float4 x[4]; float decay; };
     // Segment i of the walk; its sum is there only if somebody behind it in the walk needs it.
-    auto chunk_of = [&](int i) { return slot0 + (a.reverse ? chunks - 1 - i : i); };
+    auto chunk_of = [&](int i) { return a.reverse ? chunks - 1 - i : i; };
     const int summed = a.to_end ? chunks : chunks - 1;
     auto ask = [&](int i) {
         Step x;
         if (i >= summed) i = summed > 0 ? summed - 1 : 0;
-        const float *from = w.local + place(chunk_of(i)) * 1024 + lane * 8;
+        const float *from = w.local + place(sum_of(chunk_of(i))) * 1024 + lane * 8;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             x.x[2 * c] = *reinterpret_cast<const float4 *>(from + c * 512);
             x.x[2 * c + 1] = *reinterpret_cast<const float4 *>(from + c * 512 + 4);
         }
-        x.decay = w.decay[(int64_t)chunk_of(i) * p.v_heads + h];
+        x.decay = w.decay[(int64_t)(slot0 + chunk_of(i)) * p.v_heads + h];
         return x;
     };
     auto turned = [&](float (&t)[2][8]) {                // lane (m, g): rows 2 m + c of dim_k, columns 8 g + e of dim_v
@@ -205,11 +210,12 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
         k_place[c] = (kc >> 4) * KTERMS * kFrag + (g * 16 + (kc & 15)) * 16;
         v_place[c] = (vc >> 4) * 3 * kFrag + (g * 16 + (vc & 15)) * 16;
     }
-    auto by_k_step = [&](int slot) { return ((((int64_t)slot * p.v_heads + h) * w.kp + pi) * w.k_tiles) * KTERMS * kFrag; };
-    auto by_v_step = [&](int slot) { return ((((int64_t)slot * p.v_heads + h) * w.vp + q) * w.v_tiles) * 3 * kFrag; };
-    // S0 . dS0 of a segment whose dS0 is at hand.
-    auto inner = [&](int slot, const float (&t)[2][8]) {
-        const uint8_t *from = w.first + by_v_step(slot);
+    auto by_k_step = [&](int64_t state) { return (((state * p.v_heads + h) * w.kp + pi) * w.k_tiles) * KTERMS * kFrag; };
+    auto by_v_step = [&](int64_t state) { return (((state * p.v_heads + h) * w.vp + q) * w.v_tiles) * 3 * kFrag; };
+    // S0 . dS0 of a segment whose dS0 is at hand: S0 as the forward left it.
+    auto inner = [&](int c, const float (&t)[2][8]) {
+        const int64_t state = a.use_inner == 2 ? (int64_t)slot0 + c : border0 + c - 1;
+        const uint8_t *from = w.first + by_v_step(state);
         double sum = 0.0;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -224,7 +230,7 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
             for (int e = 0; e < 4; ++e) sum = fma((double)x[e], (double)t[c][4 + e], sum);
         }
         sum = over_wave(sum);
-        if (lane == 0) w.inner[place(slot)] = sum;
+        if (lane == 0) w.inner[place(state)] = sum;
     };
 
     constexpr int AHEAD = 4;             // segments asked for ahead: the loop waits for memory alone
@@ -237,32 +243,32 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
         for (int j = 0; j < AHEAD; ++j) {
             const int i = i0 + j;
             if (i >= chunks) break;
-            const int slot = chunk_of(i);
+            const int c = chunk_of(i);
             if (i > 0 || a.first != nullptr) {
                 if (a.write_k) {
-                    uint8_t *to = w.by_k + by_k_step(slot);
+                    uint8_t *to = w.by_k + by_k_step(state_of(c));
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
+                    for (int o = 0; o < 2; ++o) {
                         bf16x8 f[KTERMS];
-                        split8<KTERMS>(s[c], f);
+                        split8<KTERMS>(s[o], f);
 #pragma unroll
-                        for (int t = 0; t < KTERMS; ++t) *reinterpret_cast<u32x4 *>(to + k_place[c] + t * kFrag) = bitcast<u32x4>(f[t]);
+                        for (int t = 0; t < KTERMS; ++t) *reinterpret_cast<u32x4 *>(to + k_place[o] + t * kFrag) = bitcast<u32x4>(f[t]);
                     }
                 }
                 if (a.write_v || a.use_inner) {
                     float t[2][8];
                     turned(t);
                     if (a.write_v) {
-                        uint8_t *to = w.by_v + by_v_step(slot);
+                        uint8_t *to = w.by_v + by_v_step(state_of(c));
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
+                        for (int o = 0; o < 2; ++o) {
                             bf16x8 f[3];
-                            split8<3>(t[c], f);
+                            split8<3>(t[o], f);
 #pragma unroll
-                            for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4 *>(to + v_place[c] + k * kFrag) = bitcast<u32x4>(f[k]);
+                            for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4 *>(to + v_place[o] + k * kFrag) = bitcast<u32x4>(f[k]);
                         }
                     }
-                    if (a.use_inner && i > 0) inner(slot + 1, t);            // (reverse: what is behind this segment is in front of the one behind it)
+                    if (a.use_inner && i > 0) inner(c + 1, t);               // (reverse: what is behind this segment is in front of the one behind it)
                 }
             }
             if (i < summed) {
@@ -270,9 +276,9 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
                 const float add[2][8] = {{x.x[0].x, x.x[0].y, x.x[0].z, x.x[0].w, x.x[1].x, x.x[1].y, x.x[1].z, x.x[1].w},
                                          {x.x[2].x, x.x[2].y, x.x[2].z, x.x[2].w, x.x[3].x, x.x[3].y, x.x[3].z, x.x[3].w}};
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+                for (int o = 0; o < 2; ++o)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) s[c][e] = fmaf(x.decay, s[c][e], add[c][e]);
+                    for (int e = 0; e < 8; ++e) s[o][e] = fmaf(x.decay, s[o][e], add[o][e]);
             }
             if (summed > 0) next[j] = ask(i + AHEAD);
         }
@@ -280,7 +286,7 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
     if (a.use_inner == 2 && chunks > 0) {                // there is an initial state, and its gradient is at hand
         float t[2][8];
         turned(t);
-        inner(slot0, t);
+        inner(0, t);
     }
     if (a.last == nullptr) return;
 #pragma unroll
@@ -312,11 +318,13 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
     }
     const SegmentAt at = segment_at(p, w, slot);
     if (at.count <= 0) return;
+    const int64_t state = first ? (int64_t)slot : border_behind(p, w, at) - 1;
     auto inner = [&](int64_t of) {                       // S0 . dS0
         double sum = 0.0;
-        for (int64_t i = lane; i < w.tiles(); i += 64) sum += w.inner[of * w.tiles() + i];
+        for (int64_t i = lane; i < w.tiles(); i += 64) sum += w.inner[(of * p.v_heads + h) * w.tiles() + i];
         return over_wave(sum);
     };
+    const int64_t token0 = ((int64_t)at.b * p.v_heads + h) * p.seqlen + at.lo;
     double change[kBlocks], size[kBlocks], total = 0.0, sizes = 0.0;
     float kz[kBlocks];
 #pragma unroll
@@ -324,16 +332,16 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
         const int t = b * kChunk + lane, there = t < at.count ? t : at.count - 1;
         float beta = 1.f;
         if (p.beta != nullptr) beta = bits_as_float(load_bits(p.beta, at.b * p.beta_stride_b + (at.lo + there) * p.beta_stride_l + h * p.beta_stride_h, p.beta_dtype), p.beta_dtype);
-        const double qd = w.dot_q[(int64_t)sv * kSegment + there], z = w.dot_k[(int64_t)sv * kSegment + there];
+        const double qd = w.dot_q[token0 + there], z = w.dot_k[token0 + there];
         kz[b] = 0.f;
         if (p.beta != nullptr)
-            kz[b] = (float)(z + (double)w.self_k[(int64_t)sv * kSegment + there] * (double)w.qk[((int64_t)slot * p.heads + divided((uint32_t)h, w.by_group)) * kSegment + there]);
+            kz[b] = (float)(z + (double)w.self_k[token0 + there] * (double)w.qk[((int64_t)at.b * p.heads + divided((uint32_t)h, w.by_group)) * p.seqlen + at.lo + there]);
         change[b] = t < at.count ? qd - (double)beta * z : 0.0;
         size[b] = t < at.count ? fabs(qd) + fabs((double)beta * z) : 0.0;
     }
-    double dg = at.c > 0 || first ? inner(sv) : 0.0, rest = 0.0;
+    double dg = at.c > 0 || first ? inner(state) : 0.0, rest = 0.0;
     const bool known = !at.last || !bp.dfinal_states;    // what comes behind the last token
-    const double end = at.last || !known ? 0.0 : inner((int64_t)sv + p.v_heads);
+    const double end = at.last || !known ? 0.0 : inner(state + 1);
     double before[kBlocks], share[kBlocks];              // changes in front of each token, and the sizes of what they are differences of
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {

@@ -162,6 +162,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
     if (at.count <= 0) return;
     const int steps = (at.count + kStep - 1) / kStep;
     const bool has_state = (REV ? !at.last : at.c > 0) || a.first;
+    const int64_t state = a.first ? (int64_t)slot : border_behind(p, w, at) - !REV;
     const int own = wave < 4 ? wave : 11 - wave;         // which 32 rows
     const bool rows = own < steps, whole = (own + 1) * kStep <= at.count;
     auto token = [&](int t) { return t < at.count ? t : at.count - 1; };           // (rows behind the last weigh nothing, or are not stored)
@@ -212,7 +213,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
         for (int e = 0; e < 8; ++e) zr.ask(e, zb + ((uint32_t)token(own * kStep + 8 * g + e) * z_pitch + col));
     };
     auto ask_state = [&](int stage) {                    // steps that are not there: the last
-        const uint8_t *st = a.state + ((int64_t)slot * p.v_heads + h) * a.steps * a.tiles * PT * kFrag + (int64_t)ct * STATE * kFrag + lane * 16;
+        const uint8_t *st = a.state + (state * p.v_heads + h) * a.steps * a.tiles * PT * kFrag + (int64_t)ct * STATE * kFrag + lane * 16;
 #pragma unroll
         for (int i = 0; i < IN_STATE; ++i) {
             const int f = wave + 8 * i < SB * STATE ? wave + 8 * i : SB * STATE - 1, s = stage * SB + f / STATE, step = s < a.steps ? s : a.steps - 1;
@@ -246,7 +247,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
         asm volatile("" : "+v"(lane));                   // (addresses are made anew: kept over the loop they would take a hundred registers)
         m = lane & 15;
         g = lane >> 4;
-        const int64_t sv = (int64_t)slot * p.v_heads + h;
+        const int h_now = h;
         stay();
         if (hi > 0) lds_barrier();                       // the head before has been read
         // G, one token a lane.
@@ -489,8 +490,9 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                     const float of_self = lds.of_self[row + (m & 3)];
                     self_sum[i] = fmaf(of_self, lds.s[row + (m & 3)], JOIN ? self_sum[i] : 0.f);
                     if (m < 4 && row + m < at.count) {
-                        a.dots[sv * kSegment + row + m] = REV ? mine_dot : (double)p.scale * mine_dot;
-                        if (a.selves != nullptr) a.selves[sv * kSegment + row + m] = of_self;
+                        const int64_t to = ((int64_t)at.b * p.v_heads + h_now) * p.seqlen + at.lo + row + m;
+                        a.dots[to] = REV ? mine_dot : (double)p.scale * mine_dot;
+                        if (a.selves != nullptr) a.selves[to] = of_self;
                     }
                     const f32x4 by = *reinterpret_cast<const f32x4 *>(&lds.s[row]);
 #pragma unroll
@@ -530,7 +532,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float all = over_columns(W * m < a.d2 ? sum_uz[e] : 0.f);
-                            if (m == e && own * kStep + first + e < at.count) a.uz[((int64_t)slot * p.heads + hk) * kSegment + own * kStep + first + e] = all;
+                            if (m == e && own * kStep + first + e < at.count) a.uz[((int64_t)at.b * p.heads + hk) * p.seqlen + at.lo + own * kStep + first + e] = all;
                         }
                     }
 #pragma unroll
@@ -555,7 +557,7 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                     const int row = own * kStep + first + e;
                     if ((!whole && row >= at.count) || col0 + W * m >= a.d2) continue;
                     if (!JOIN || a.share == nullptr) {
-                        const int64_t head = DOTS ? hk : (int)(sv - (int64_t)slot * p.v_heads);
+                        const int64_t head = DOTS ? hk : h_now;
                         T *base = static_cast<T *>(a.out) + at.b * a.out_b + at.lo * a.out_l + head * a.out_h + col0;
                         store_wide<DT, W>(base + ((uint32_t)row * (uint32_t)a.out_l + W * m), o);
                     } else {

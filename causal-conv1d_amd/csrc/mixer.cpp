@@ -292,14 +292,15 @@ at::Tensor linear_fwd_meta(const at::Tensor &, const at::Tensor &, const at::Ten
                            const OptTensor &, const OptTensor &, const OptTensor &, double) {
     return at::empty_symint(v.sym_sizes(), v.options());
 }
-// Three terms of 16 bits of every state in front of a segment of 256 tokens, in operands of 32 rows of dim_v and 16 columns of dim_k, whose number is
+// Three terms of 16 bits of every state between two segments of 256 tokens (with initial states: in front of every segment), in operands of 32 rows of dim_v and 16 columns of dim_k, whose number is
 // whole to 2, 4 or 8 of them: the library's sum.
 std::tuple<at::Tensor, at::Tensor> linear_fwd_save_meta(const at::Tensor &q, const at::Tensor &, const at::Tensor &v, const at::Tensor &, const OptTensor &,
-                           const OptTensor &, const OptTensor &cu, const OptTensor &, double) {
-    const c10::SymInt slots = cu.has_value() ? q.sym_size(1) / 256 + cu->sym_size(0) : q.sym_size(0) * ((q.sym_size(1) + 255) / 256);
+                           const OptTensor &init, const OptTensor &cu, const OptTensor &, double) {
+    const c10::SymInt chunks = (q.sym_size(1) + 255) / 256;
+    const c10::SymInt states = !init.has_value() ? q.sym_size(0) * (chunks.max(1) - 1) : cu.has_value() ? q.sym_size(1) / 256 + cu->sym_size(0) : q.sym_size(0) * chunks;
     const int64_t dk = q.sym_size(3).guard_int(__FILE__, __LINE__), dv = v.sym_size(3).guard_int(__FILE__, __LINE__);
     const int64_t width = q.scalar_type() == at::kFloat || dk > 128 || dv > 128 ? 2 : dk <= 64 ? 4 : 8;
-    const c10::SymInt bytes = slots * v.sym_size(2) * ((dv + 31) / 32) * ((dk + 16 * width - 1) / (16 * width) * width) * 3 * 1024;
+    const c10::SymInt bytes = 256 + states * v.sym_size(2) * ((dv + 31) / 32) * ((dk + 16 * width - 1) / (16 * width) * width) * 3 * 1024;
     return {at::empty_symint(v.sym_sizes(), v.options()), at::empty_symint({bytes}, q.options().dtype(at::kByte))};
 }
 Gradients6 linear_bwd_meta(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const OptTensor &beta,

@@ -138,7 +138,8 @@ int cc1d_delta_step(const cc1d_delta_step_params *p, cc1d_stream_t stream);
  *
  * The blocks are the gated delta rule's, with what stands there about heads, strides, sequences and tokens of none.  beta may be NULL: 1
  * (dbeta is then not written, beta_dtype not read).  Strides of 0 make a gate one number a head.  qk_l2norm has to be 0 (CC1D_ERR_OPTION).
- * `saved` is of cc1d_linear_saved_bytes() here: the state in front of every 256 tokens.
+ * `saved` is of cc1d_linear_saved_bytes() here: the state between every two segments of 256 tokens, and with initial_states that in front of the first too (a
+ * backward's block gives them, or NULL, as its forward's did).
  *
  * Short sequences go token by token, packed ones each by its own length; the others in segments of 256 tokens, worked out in blocks of 64: a NaN or infinity reaches its
  * head's outputs from the start of its 64 tokens on.  Gates are bounded from below by -200, which forgets everything.  Where they
