@@ -4,8 +4,10 @@
 //   dx = dh + r (w dy - mean(w dy) - n mean(w dy n)),  dw = sum over rows of dy n,  db = sum over rows of dy
 //
 // Rows lie in registers as the root-mean-square norm's do (cc1d_norm.hip), and memory bounds it as well.  The mean goes first and the squares are those of
-// differences, two sums one behind the other: of a row whose mean is large beside its spread, mean(h^2) - mean(h)^2 would leave nothing.  A
-// training forward leaves each row's mean and r for the backward, 8 bytes a row, which saves that one its first pair of sums.
+// differences, two sums one behind the other: of a row whose mean is large beside its spread, mean(h^2) - mean(h)^2 would leave nothing.  The mean itself is
+// rounded, by up to some 2^-22 of it, which may be more than the spread: the differences' own mean, one more sum beside that of their squares, is taken off
+// them (2560 numbers of 100003, whose y is the bias: off by 0.43 without).  A training forward leaves each row's mean and r for the backward, 8 bytes a row, which saves that one its first pair of
+// sums; the differences' mean it makes anew beside its own two.
 // db's partial sums lie behind dw's in the same planes.
 //
 // 16384 rows of 2560, residual in fp32: forward 110 us (4.6 TB/s), backward 127 (5.3) and 4.5 for the planes; 8192 of 5120, bfloat16: 60 (5.6); 64 such rows: 4.7 us, a
@@ -19,7 +21,7 @@ namespace {
 template <int XD, int RD, int WD, int T, int NV>
 __global__ void __launch_bounds__(threads_of(T))
 layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const int64_t last) {
-    __shared__ float lds[2][16];
+    __shared__ float lds[3][16];
     const int lane = T == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x, lanes = T == 64 ? 64 : (int)blockDim.x;
     const int64_t row = first + (T == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x);
     if (T == 64 && row >= last) return;
@@ -32,7 +34,7 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
         Raw8<XD> x[NV];
         Raw8<RD> res[NV];
         Raw8<WD> w[NV], b[NV];
-        float h[NV][8], sum = 0.f, sq = 0.f;
+        float h[NV][8], sum[1] = {0.f}, of_differences[2] = {0.f, 0.f};  // their sum, and of their squares
 #pragma unroll
         for (int v = 0; v < NV; ++v) x[v].load(p.x, row * p.x_stride, (v * lanes + lane) * 8, p.dim);
         if (p.residual != nullptr) {
@@ -58,19 +60,22 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
                 if (c < p.dim) store8<RD>(p.h, row * p.h_stride + c, p.dim - c, h[v]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += h[v][i];
+            for (int i = 0; i < 8; ++i) sum[0] += h[v][i];
         }
-        const float mean = over_row<T, false>(sum, lds[0]) * over;
+        over_row<T>(sum, lds);
+        const float mean = sum[0] * over;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int n = p.dim - (v * lanes + lane) * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 h[v][i] = i < n ? h[v][i] - mean : 0.f;
-                sq += h[v][i] * h[v][i];
+                of_differences[0] += h[v][i];
+                of_differences[1] += h[v][i] * h[v][i];
             }
         }
-        const float r = rsqrtf(over_row<T, false>(sq, lds[1]) * over + p.eps);
+        over_row<T>(of_differences, lds + 1);
+        const float off = of_differences[0] * over, r = rsqrtf(fmaxf(of_differences[1] * over - off * off, 0.f) + p.eps);
         keep(mean, r);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -81,11 +86,11 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
             for (int i = 0; i < 8; ++i) bf[i] = 0.f;
             if (p.bias != nullptr) b[v].to(bf);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[v][i] = fmaf(h[v][i] * r, wf[i], bf[i]);
+            for (int i = 0; i < 8; ++i) h[v][i] = fmaf((h[v][i] - off) * r, wf[i], bf[i]);
             if (c < p.dim) store8<XD>(p.y, row * p.y_stride + c, p.dim - c, h[v]);
         }
     } else {
-        float sum = 0.f, sq = 0.f;
+        float sum[1] = {0.f}, of_differences[2] = {0.f, 0.f};
         for (int c = lane * 8; c < p.dim; c += lanes * 8) {
             float h[8];
             load8<XD>(p.x, row * p.x_stride, c, p.dim, h);
@@ -98,9 +103,10 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
                 store8<RD>(p.h, row * p.h_stride + c, p.dim - c, h);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += h[i];
+            for (int i = 0; i < 8; ++i) sum[0] += h[i];
         }
-        const float mean = over_row<T, false>(sum, lds[0]) * over;
+        over_row<T>(sum, lds);
+        const float mean = sum[0] * over;
         auto centred = [&](int c, float (&h)[8]) {       // each lane reads the h that it wrote
             if (p.h != nullptr) load8<RD>(p.h, row * p.h_stride, c, p.dim, h);
             else load8<XD>(p.x, row * p.x_stride, c, p.dim, h);
@@ -111,9 +117,10 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
             float h[8];
             centred(c, h);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sq += h[i] * h[i];
+            for (int i = 0; i < 8; ++i) { of_differences[0] += h[i]; of_differences[1] += h[i] * h[i]; }
         }
-        const float r = rsqrtf(over_row<T, false>(sq, lds[1]) * over + p.eps);
+        over_row<T>(of_differences, lds + 1);
+        const float off = of_differences[0] * over, r = rsqrtf(fmaxf(of_differences[1] * over - off * off, 0.f) + p.eps);
         keep(mean, r);
         for (int c = lane * 8; c < p.dim; c += lanes * 8) {
             float h[8], w[8], b[8];
@@ -123,7 +130,7 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
             for (int i = 0; i < 8; ++i) b[i] = 0.f;
             if (p.bias != nullptr) load8<WD>(p.bias, 0, c, p.dim, b);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = fmaf(h[i] * r, w[i], b[i]);
+            for (int i = 0; i < 8; ++i) h[i] = fmaf((h[i] - off) * r, w[i], b[i]);
             store8<XD>(p.y, row * p.y_stride + c, p.dim - c, h);
         }
     }
@@ -134,7 +141,7 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
 template <int XD, int RD, int WD, int T, int NV>
 __global__ void __launch_bounds__(threads_of(T))
 layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const int64_t rows_each) {
-    __shared__ float lds[2][2][16];
+    __shared__ float lds[2][3][16];
     const int lane = T == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x, lanes = T == 64 ? 64 : (int)blockDim.x;
     const int wave = threadIdx.x >> 6;
     const int64_t begin = blockIdx.x * rows_each, last = begin + rows_each < p.rows ? begin + rows_each : p.rows;
@@ -149,18 +156,14 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
         if (p.dresidual != nullptr) store8<RD>(p.dresidual, row * p.dresidual_stride + c, n, d);
     };
     int turn = 0;                                        // which half of `lds`: a row's sums may still be read when the next one's are written
-    auto over_rows_waves = [&](float &a, float &b) {
-        a = over_lanes<false>(a);
-        b = over_lanes<false>(b);
-        if constexpr (T > 64) {
-            const int waves = blockDim.x >> 6;
-            if ((threadIdx.x & 63) == 0) { lds[turn][0][wave] = a; lds[turn][1][wave] = b; }
-            lds_barrier();
-            a = lds[turn][0][0];
-            b = lds[turn][1][0];
-            for (int i = 1; i < waves; ++i) { a += lds[turn][0][i]; b += lds[turn][1][i]; }
-            turn ^= 1;
-        }
+    // Of a row's differences times r: their own mean `off`, and with n what is left of them the means of w dy and of w dy n.  `sums`: of these differences, of
+    // w dy, of the products.
+    struct Means { float off, m1, m2; };
+    auto means_of = [&](float (&sums)[3]) {
+        over_row<T>(sums, lds[turn]);
+        turn ^= 1;
+        const float off = sums[0] * over;
+        return Means{off, sums[1] * over, (sums[2] - off * sums[1]) * over};
     };
     if constexpr (NV > 0) {
         Raw8<WD> wr[NV];
@@ -176,7 +179,7 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
         for (int64_t row = first; row < last; row += step) {
             Raw8<RD, true> hr[NV], dhr[NV];
             Raw8<XD, true> dyr[NV];
-            float h[NV][8], dy[NV][8], d[NV][8], m1 = 0.f, m2 = 0.f;
+            float h[NV][8], dy[NV][8], d[NV][8], sums[3] = {0.f, 0.f, 0.f};
             const float2 st = *reinterpret_cast<const float2 *>(p.stats + 2 * row);
 #pragma unroll
             for (int v = 0; v < NV; ++v) hr[v].load(p.h, row * p.h_stride, (v * lanes + lane) * 8, p.dim);
@@ -199,21 +202,21 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
             for (int v = 0; v < NV; ++v)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    h[v][i] = (h[v][i] - st.x) * st.y;
-                    m1 += w[v][i] * dy[v][i];
-                    m2 += (w[v][i] * dy[v][i]) * h[v][i];
+                    h[v][i] = i < p.dim - (v * lanes + lane) * 8 ? (h[v][i] - st.x) * st.y : 0.f;
+                    sums[0] += h[v][i];
+                    sums[1] += w[v][i] * dy[v][i];
+                    sums[2] += (w[v][i] * dy[v][i]) * h[v][i];
                 }
-            over_rows_waves(m1, m2);
-            m1 *= over;
-            m2 *= over;
+            const Means m = means_of(sums);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int c = (v * lanes + lane) * 8;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    dw[v][i] += dy[v][i] * h[v][i];
+                    const float n = h[v][i] - m.off;
+                    dw[v][i] += dy[v][i] * n;
                     db[v][i] += dy[v][i];
-                    d[v][i] += st.y * ((w[v][i] * dy[v][i] - m1) - h[v][i] * m2);
+                    d[v][i] += st.y * ((w[v][i] * dy[v][i] - m.m1) - n * m.m2);
                 }
                 if (c < p.dim) put(row, c, d[v]);
             }
@@ -247,7 +250,7 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
         }
     } else {
         for (int64_t row = first; row < last; row += step) {
-            float m1 = 0.f, m2 = 0.f;
+            float sums[3] = {0.f, 0.f, 0.f};
             const float2 st = *reinterpret_cast<const float2 *>(p.stats + 2 * row);
             for (int c = lane * 8; c < p.dim; c += lanes * 8) {
                 float h[8], dy[8], wv[8];
@@ -255,11 +258,14 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
                 load8<XD>(p.dy, row * p.dy_stride, c, p.dim, dy);
                 load8<WD>(p.weight, 0, c, p.dim, wv);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { m1 += wv[i] * dy[i]; m2 += (wv[i] * dy[i]) * ((h[i] - st.x) * st.y); }
+                for (int i = 0; i < 8; ++i) {
+                    const float difference = i < p.dim - c ? (h[i] - st.x) * st.y : 0.f;
+                    sums[0] += difference;
+                    sums[1] += wv[i] * dy[i];
+                    sums[2] += (wv[i] * dy[i]) * difference;
+                }
             }
-            over_rows_waves(m1, m2);
-            m1 *= over;
-            m2 *= over;
+            const Means m = means_of(sums);
             for (int c = lane * 8; c < p.dim; c += lanes * 8) {
                 float h[8], dy[8], wv[8], dw[8], db[8], d[8];
                 load8<RD>(p.h, row * p.h_stride, c, p.dim, h);
@@ -274,10 +280,10 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
                 if (p.dh != nullptr) load8<RD>(p.dh, row * p.dh_stride, c, p.dim, d);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float n = (h[i] - st.x) * st.y;
+                    const float n = (h[i] - st.x) * st.y - m.off;
                     dw[i] += dy[i] * n;
                     db[i] += dy[i];
-                    d[i] += st.y * ((wv[i] * dy[i] - m1) - n * m2);
+                    d[i] += st.y * ((wv[i] * dy[i] - m.m1) - n * m.m2);
                 }
                 store8<CC1D_F32>(plane, c, p.dim - c, dw);
                 if (bias) store8<CC1D_F32>(plane_b, c, p.dim - c, db);

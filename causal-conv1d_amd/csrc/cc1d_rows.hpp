@@ -117,6 +117,28 @@ __device__ __forceinline__ float over_row(float v, float *lds) {
     return v;
 }
 
+// Sums of several numbers at once, one barrier, the same bits in every lane (the lanes' own orders of over_lanes may part them by a rounding); `lds` is for
+// these alone.
+template <int T, int N>
+__device__ __forceinline__ void over_row(float (&v)[N], float (*lds)[16]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = bitcast<float>(__builtin_amdgcn_readfirstlane(bitcast<int>(over_lanes<false>(v[k]))));
+    if constexpr (T > 64) {
+        const int waves = blockDim.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) lds[k][threadIdx.x >> 6] = v[k];
+        }
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = lds[k][0];
+        for (int i = 1; i < waves; ++i) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] += lds[k][i];
+        }
+    }
+}
+
 constexpr int threads_of(int T) { return T == 64 ? 256 : T; }
 
 // The sum of the planes of `width` columns, in a fixed order: 32 columns a workgroup, 32 groups of lanes take every 32nd plane, 8 at a time.  The
