@@ -38,7 +38,7 @@ struct TileLds {
     float of_x[kSegment], of_y[kSegment];                              // factors of E
     float weigh[kSegment], back[kSegment];                             // y's weight; where x and y share 32 tokens: exp(G at their start - G)
     float f[kSegment], s[kSegment];
-    float of_self[kSegment];             // the weighted product of a token with itself
+    float of_self[kSegment], self_sum[kSegment];         // the weighted product of a token with itself, and over the heads
     double ends[kSteps + 1];             // G at the borders of 32 tokens
     double sums[kBlocks];
     int32_t steep[kSteps];               // whether `back` is too large to be used
@@ -167,7 +167,6 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
     const bool rows = own < steps, whole = (own + 1) * kStep <= at.count;
     auto token = [&](int t) { return t < at.count ? t : at.count - 1; };           // (rows behind the last weigh nothing, or are not stored)
 
-    float self_sum[2] = {0.f, 0.f};      // of row 16 i + 4 g + m, m < 4, over the heads
     f32x4 total[JOIN ? 2 : 1][JOIN ? W : 1], acc[2][W];
     if constexpr (JOIN)
 #pragma unroll
@@ -391,9 +390,9 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                     if constexpr (DOTS) {                // of x's row m: lane (m, 2 i + m / 8) has it
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float both = 0.f;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) both = (m & 7) == e ? pt[i][e >> 2][e & 3] : both;
+                            const f32x4 lo = pt[i][0], up = pt[i][1];
+                            const float b0 = m & 1 ? lo[1] : lo[0], b1 = m & 1 ? lo[3] : lo[2], b2 = m & 1 ? up[1] : up[0], b3 = m & 1 ? up[3] : up[2];
+                            const float c0 = m & 2 ? b1 : b0, c1 = m & 2 ? b3 : b2, both = m & 4 ? c1 : c0;
                             if (g == 2 * i + (m >> 3)) lds.of_self[own * kStep + 16 * i + m] = both * lds.weigh[own * kStep + 16 * i + m];
                         }
                     }
@@ -487,12 +486,14 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                         dot[e] = over_columns(W * m < a.d2 ? (double)sum_u : 0.0);
                     }
                     const double mine_dot = m == 1 ? dot[1] : m == 2 ? dot[2] : m == 3 ? dot[3] : dot[0];
-                    const float of_self = lds.of_self[row + (m & 3)];
-                    self_sum[i] = fmaf(of_self, lds.s[row + (m & 3)], JOIN ? self_sum[i] : 0.f);
-                    if (m < 4 && row + m < at.count) {
-                        const int64_t to = ((int64_t)at.b * p.v_heads + h_now) * p.seqlen + at.lo + row + m;
-                        a.dots[to] = REV ? mine_dot : (double)p.scale * mine_dot;
-                        if (a.selves != nullptr) a.selves[to] = of_self;
+                    if (m < 4) {
+                        const float of_self = lds.of_self[row + m], weighed = of_self * lds.s[row + m];
+                        lds.self_sum[row + m] = JOIN && hi > 0 ? lds.self_sum[row + m] + weighed : weighed;
+                        if (row + m < at.count) {
+                            const int64_t to = ((int64_t)at.b * p.v_heads + h_now) * p.seqlen + at.lo + row + m;
+                            a.dots[to] = REV ? mine_dot : (double)p.scale * mine_dot;
+                            if (a.selves != nullptr) a.selves[to] = of_self;
+                        }
                     }
                     const f32x4 by = *reinterpret_cast<const f32x4 *>(&lds.s[row]);
 #pragma unroll
@@ -510,9 +511,8 @@ __device__ __forceinline__ void tile_rows(const cc1d_delta_params &p, const Segm
                 f32x4 s = {1.f, 1.f, 1.f, 1.f};
                 if constexpr (!DOTS) s = *reinterpret_cast<const f32x4 *>(&lds.s[own * kStep + first]);
                 if constexpr (DOTS) {                    // the tokens themselves
-                    if (m < 4) lds.of_self[own * kStep + first + m] = self_sum[i];
                     wave_lds_fence();
-                    const f32x4 by = *reinterpret_cast<const f32x4 *>(&lds.of_self[own * kStep + first]);
+                    const f32x4 by = *reinterpret_cast<const f32x4 *>(&lds.self_sum[own * kStep + first]);
                     if (a.uz != nullptr && share == 0) {
                         Wide8<W> u;
                         ask_u(i, u);
