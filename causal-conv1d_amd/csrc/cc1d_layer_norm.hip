@@ -10,7 +10,7 @@
 // sums; the differences' mean it makes anew beside its own two.
 // db's partial sums lie behind dw's in the same planes.
 //
-// 16384 rows of 2560, residual in fp32: forward 110 us (4.6 TB/s), backward 127 (5.3) and 4.5 for the planes; 8192 of 5120, bfloat16: 60 (5.6); 64 such rows: 4.7 us, a
+// 16384 rows of 2560, residual in fp32: forward 118 us (4.3 TB/s; 107 at best), backward 134 (5.0; 128) and 5 for the planes; 8192 of 5120, bfloat16: 62 (5.4); 64 such rows: 4.6 us, a
 // launch and two reductions one behind the other.
 #include "cc1d_rows.hpp"
 
@@ -294,7 +294,7 @@ layer_norm_bwd_kernel(const cc1d_layer_norm_bwd_params p, float *planes, const i
 }
 
 // Workgroups of the backward on a CU, all of them at once: its registers leave four wavefronts a SIMD, and a workgroup may put its odd one on any
-// (16384 rows of 2560: two of five wavefronts 126 us, 5.3 TB/s, three 162, the last of them after the others; 8192 of 4096: two of eight 97, one 122).
+// (16384 rows of 2560: two of five wavefronts 126 us, three 162, the last of them after the others; 8192 of 4096: two of eight 97, one 122).
 int bwd_a_cu(int dim) { return 4 / ((bwd_lanes(dim) + 255) / 256); }
 
 }  // namespace

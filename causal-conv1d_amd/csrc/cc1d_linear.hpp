@@ -24,7 +24,7 @@
 // up over its tokens.  So the sums are made in 64 bits (linear_tile_kernel: 32 for the four or eight products inside a lane), of dq and dk before they are rounded, and what the last token leaves over against the next segment's
 // S0 . dS0 (or 0, behind the last one) is taken back in proportion to the sizes of the products in front: where the errors arise, and not among
 // the small gradients in front of large ones (16 heads with a constant decay each, 2 x 1000 tokens, the sum of dg over the tokens, six seeds: off by
-// 1e-8 to 5e-7 of itself; with sums of 32 bits, without that and without linear_states_kernel's alternating signs 7e-7 to 3e-6).
+// 3e-8 to 5e-7 of itself, the plain form by 1e-7 to 6e-7; with sums of 32 bits, without that and without linear_states_kernel's alternating signs 7e-7 to 3e-6).
 //
 // Numbers of 24 bits on the 16-bit matrix cores: cc1d_delta_chunk.hpp.
 #pragma once

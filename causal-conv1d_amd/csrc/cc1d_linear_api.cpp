@@ -48,7 +48,8 @@ bool reachable_gradients(const cc1d_delta_bwd_params &bp) {
 // by segments, us: 16-bit types, 128 x 128, 4 heads: 16 tokens 21 and 20; 256: 24 tokens 31 and 36, 32 tokens 39 and 36; 1024: 48 tokens 127 and 135,
 // 64 tokens 162 and 138; 32 x 32, 1024 heads: 32 tokens 28 and 29; 2880: 64 tokens 80 and 82.  float32, whose products take six matrix instructions for
 // one to three, 128 x 128, 4 heads: 24 tokens 27 and 24; 256: 48 tokens 51 and 60, 64 tokens 66 and 61; 512: 96 tokens 116 and 132, 128 tokens 150 and 140;
-// 1024: 128 tokens 267 and 298, 256 tokens 540 and 420; 32 x 32, 2880 heads: 512 tokens 569 and 968.
+// 1024: 128 tokens 267 and 298, 256 tokens 540 and 420.  Many small ones go by tokens at any length: 2880 of 32 x 32: 256 tokens 286 and 447, 4096 tokens 4480
+// and 7560; 2048 of 64 x 64: 256 tokens 395 and 379, 1024 tokens 1380 and 1580, 4096 tokens 6030 and 6410; 8192 of 64 x 64: 4096 tokens 21400 and 25600.
 int64_t segments_from(const cc1d_delta_params &p, int64_t sequences) {
     const double heads = (double)sequences * p.v_heads, size = (double)p.dim_k * p.dim_v / 16384.0, most = heads < 1e6 ? heads : 1e6;
     if (p.x_dtype == CC1D_F32) {

@@ -21,8 +21,8 @@
 // DOTS: several value heads of a key head one after the other, the sum of their rows kept in registers, and of each the rows' products with u
 // (q or k), which the gates' gradients are made of.  There a row's own z stays out of the products; it joins the sum of the heads at the end, with a weight in fp32.  What several workgroups of a key head leave is joined by linear_join_kernel.
 //
-// float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 196 us (with sums and scan), backward 552; bfloat16 of 256 x 256:
-// 330 and 952.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
+// float32 takes six matrix instructions a product, 16 heads of 128 x 128, 4 x 2048 tokens: forward 219 us (with sums, scan and the last states), backward 588; bfloat16 of 256 x 256:
+// 352 and 994.  A block's chain of loads, splits, LDS and products is what it takes time for, with one or two workgroups a CU by registers
 // and LDS: 24 workgroups of a small call take 19 us, the matrix cores' part of which is 5.
 #pragma once
 
@@ -59,7 +59,7 @@ __device__ __forceinline__ void products_left(const bf16x8 (&a)[N][NA], const bf
 
 // Wavefronts a SIMD that the registers leave: two where nothing, or next to nothing, has to be kept in memory for that and LDS leaves two workgroups (dq and dk,
 // 16 heads, 4 x 2048 tokens, backward with two and with one: float32, 128 x 128 603 us and 746, 64 x 256 741 and 1012; bfloat16, 128 x 256 447 and 605; float32,
-// 128 x 256, whose LDS leaves one, 1262 and 1150).
+// 128 x 256, whose LDS leaves one, 1262 and 1150; since then, with own shares out of the products, 3 % more).
 constexpr int attend_waves(bool dots, int dt, int ks, int cp) { return dots && (cp > 1 || (dt == CC1D_F32 && ks == 8)) ? 1 : 2; }
 
 // KS: 32-column steps of x and y at once (their LDS); wider ones, more than 256 columns, pass slab by slab.
@@ -497,7 +497,7 @@ linear_attend_kernel(const cc1d_delta_params p, const SegmentWork w, const Atten
     attend_rows<DT, KS, RT, 1, REV, false>(p, w, a, blockIdx.x);
 }
 // dq and dk in one launch, `half` workgroups each: neither waits for the other, and one alone may leave CUs idle (24 workgroups each: 25 us, one
-// after the other 47; 128 each of linear_tile_pair_kernel: 32 and 49; 256 each, which fill the card: 380 and 385).  float32: dv's workgroups behind them, if all together
+// after the other 47; 128 each of linear_tile_pair_kernel: 32 and 49; 256 each, which fill the card: 380 and 385 at best).  float32: dv's workgroups behind them, if all together
 // are no more than CUs (24 each: 26 us, for 25 and 20); more of them leave no CU idle by themselves.
 template <int DT, int KS, int RT, int CP>
 __global__ void __launch_bounds__(kBlock, attend_waves(true, DT, KS, CP))

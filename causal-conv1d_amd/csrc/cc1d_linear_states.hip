@@ -11,7 +11,7 @@ namespace {
 // terms then; a stays as it is, one term in bfloat16.  No operand goes through LDS: pairs of columns (Pair8) are loaded in the order
 // of the matrix instruction, and the result tiles of a pair of a's are eight consecutive rows of a lane, the operand order of the next product.
 // KT: 32-column steps of a that a wavefront takes.
-// 32 segments of 80 heads of 128 x 64, bfloat16: 72 us, 84 MB read and 84 written, 2.3 TB/s; 64 segments of 16 heads of 128 x 128, float16: 62.  Splits, addresses
+// 32 segments of 80 heads of 128 x 64, bfloat16: 71 us, 86 MB read and 73 written, 2.2 TB/s; 64 segments of 16 heads of 128 x 128, float16: 63.  Splits, addresses
 // and loads of 4 bytes share the time; two steps asked for ahead: 74 and 65; loads of 8 bytes with 4 x 4 tiles a wavefront: 89 and 71.
 template <int DT, int KT>
 __global__ void __launch_bounds__(kBlock, KT <= 4 && DT != CC1D_F32 ? 2 : 1)
@@ -145,7 +145,7 @@ linear_copy_kernel(const CopyArgs a, const int64_t tokens) {
 
 // The recurrence over a sequence's segments, one wavefront a tile of 32 x 32 of one (sequence, value head): elementwise, bound by memory.  In front
 // of every segment (REVERSE: behind it) the state leaves as operands: contracted over dim_k as it lies, contracted over dim_v turned around through LDS.
-// 4 sequences of 8 segments, 80 heads of 128 x 64: 57 us forward (84 MB of sums read, 105 of operands of both kinds written, 3.3 TB/s), 87 backward (63 MB of the
+// 4 sequences of 8 segments, 80 heads of 128 x 64: 57 us forward (73 MB of sums read, 183 of operands of both kinds written, 4.5 TB/s), 88 backward (110 MB of the
 // forward's operands more).  Those asked for ahead too: 92, their registers leave fewer wavefronts.
 template <int KTERMS>
 __global__ void __launch_bounds__(64)
@@ -298,7 +298,7 @@ linear_scan_kernel(const cc1d_delta_params p, const SegmentWork w, const ScanArg
     }
 }
 
-// dg and dbeta of a segment, one wavefront each (slot, value head): bound by latency and by stores v_heads apart, 20 us for 2560 of them; sixteen heads a workgroup
+// dg and dbeta of a segment, one wavefront each (slot, value head): bound by latency and by stores v_heads apart, 19 us for 2560 of them; sixteen heads a workgroup
 // whose results pass through LDS 20 as well, and of 8 heads 8.5 for 6.
 __global__ void __launch_bounds__(kBlock)
 linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const uint32_t items, const int first) {
@@ -360,7 +360,7 @@ linear_gates_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const u
     }
 }
 
-// dq and dk of a key head whose value heads were several workgroups': their shares in a fixed order.  Bound by memory: four shares of 8192 rows of 128 each, 34 MB, 12 us.
+// dq and dk of a key head whose value heads were several workgroups': their shares in a fixed order.  Bound by memory: four shares of 8192 rows of 128 each, 34 MB, 13 us.
 template <int DT>
 __global__ void __launch_bounds__(kBlock)
 linear_join_kernel(const cc1d_delta_bwd_params bp, const SegmentWork w, const int64_t rows) {

@@ -12,11 +12,11 @@
 // and stores as many of a result's.  Its 8 rows of one column are an operand.
 //
 // E between different 32 tokens is a product of three factors: from x to the border of its 32 tokens, from border to border, and from
-// there to y; each token's two are made once, by one lane.  Among the same 32 tokens it is exp(G_i - B) exp(B - G_j), B in front of them all, unless
+// there to y; each token's two are made once, by one lane, of sums of 64 bits (exp_of_sum).  Among the same 32 tokens it is exp(G_i - B) exp(B - G_j), B in front of them all, unless
 // the gates reach e^60 there: then an exponential an entry.
 //
-// 32 segments of 80 heads of 128 x 64 (a training step of 4 x 2048 tokens, one key head), bfloat16: out 114 us, dv 108, dq and dk 380; out's
-// matrix instructions come to 0.6 PFLOP/s.  A workgroup fills a CU's LDS, so that nobody hides what it waits for: of out's 114 the products take 40 (the
+// 32 segments of 80 heads of 128 x 64 (a training step of 4 x 2048 tokens, one key head), bfloat16: out 119 us, dv 108, dq and dk 398 (traced means; the
+// best 116, 105 and 383); out's matrix instructions come to 0.6 PFLOP/s.  A workgroup fills a CU's LDS, so that nobody hides what it waits for: of out's time the products take 40 (the
 // matrix cores' own time 19), the product with the state 24 (32 KB of operands a head, 9 of matrix cores), the gates, barriers and start
 // 37, z's way to LDS 11, stores 10.  Tried: half the rows a workgroup and two of them a CU (out 127: state and y are read twice); 16 rows a wavefront, balanced
 // (equal, with spills in dq); dq and dk with two terms of state and products (22 us less each; the gates' gradients, small differences of their dots, would
@@ -597,6 +597,7 @@ int by_tiles(const AttendArgs &a, F &&f) {
 // Steps of x and y at once, beyond 128 columns: eight, or four slab by slab where eight steps' LDS leaves fewer workgroups a CU and the barriers weigh less: float32's
 // out and dv, and dq and dk of at most 64 columns of z.  16 heads, 4 x 2048 tokens, eight and four: bfloat16, 256 x 256 forward 329 us and 383, backward 953 and
 // 1152, 256 x 64 forward 119 and 147, 64 x 256 backward 479 and 399; float32, 256 x 256 forward 971 and 802, 192 x 192 backward (dq and dk by eight) 1570 and 1821.
+// (Backward since then, own shares out of the products: 3 to 5 % more.)
 template <int DT, bool REV>
 int launch_attend(const cc1d_delta_params &p, const SegmentWork &w, const AttendArgs &a, hipStream_t stream) {
     if constexpr (DT != CC1D_F32) {

@@ -8,14 +8,16 @@ that is the bound.
 dg is a running sum, over 256 tokens at most, of what token t reads less what it wrote, without its own share in either: dg[t] - dg[t+1], each side
 with the error above.  Closed at both ends of a segment, the running sum of n independent errors is off by sqrt(n / 6) of one, and no token's by more than
 those in front of it make.  Where gates are strong
-a token's own share is nearly all of q.dq and of k.dk, and nothing of dg."""
+a token's own share is nearly all of q.dq and of k.dk, and nothing of dg.
+
+States and their gradients: a segment's decay is one exponential for all elements, 2^-22.4 off at worst.  With two segments' and the sums above 2^-21.1."""
 import pytest
 import torch
 
 import linear_cases as cases
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
-DBETA = 2.0 ** -21.7
+DBETA, STATES = 2.0 ** -21.7, 2.0 ** -21.1
 
 
 def bound_of_dg(want):
@@ -82,6 +84,7 @@ def test_gates_gradient(pkg, gpu_device, dtype, dims, rate):
     got, want = cases.run(pkg, s), cases.reference(s)
     assert off(got["dg"], want["dg"]) <= bound_of_dg(want["dg"]), (off(got["dg"], want["dg"]), bound_of_dg(want["dg"]))
     assert off(got["dbeta"], want["dbeta"]) <= DBETA, off(got["dbeta"], want["dbeta"])
+    assert off(got["final"], want["final"]) <= STATES and off(got["dstates"], want["dstates"]) <= STATES, (off(got["final"], want["final"]), off(got["dstates"], want["dstates"]))
 
 
 @pytest.mark.gpu
