@@ -17,6 +17,9 @@
 namespace cc1d {
 namespace {
 
+// The difference of two sums may come out below 0; a NaN stays.
+__device__ __forceinline__ float reciprocal_spread(float variance, float eps) { return rsqrtf((variance < 0.f ? 0.f : variance) + eps); }
+
 // XD: x and y; RD: residual and h; WD: weight and bias.  NV = 0: a row is read three times.
 template <int XD, int RD, int WD, int T, int NV>
 __global__ void __launch_bounds__(threads_of(T))
@@ -75,7 +78,7 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
             }
         }
         over_row<T>(of_differences, lds + 1);
-        const float off = of_differences[0] * over, r = rsqrtf(fmaxf(of_differences[1] * over - off * off, 0.f) + p.eps);
+        const float off = of_differences[0] * over, r = reciprocal_spread(of_differences[1] * over - off * off, p.eps);
         keep(mean, r);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -120,7 +123,7 @@ layer_norm_fwd_kernel(const cc1d_layer_norm_params p, const int64_t first, const
             for (int i = 0; i < 8; ++i) { of_differences[0] += h[i]; of_differences[1] += h[i] * h[i]; }
         }
         over_row<T>(of_differences, lds + 1);
-        const float off = of_differences[0] * over, r = rsqrtf(fmaxf(of_differences[1] * over - off * off, 0.f) + p.eps);
+        const float off = of_differences[0] * over, r = reciprocal_spread(of_differences[1] * over - off * off, p.eps);
         keep(mean, r);
         for (int c = lane * 8; c < p.dim; c += lanes * 8) {
             float h[8], w[8], b[8];

@@ -48,3 +48,26 @@ def test_spread_far_below_the_mean(pkg, gpu_device, dim, offset, residual):
         want, bound = dh + s["dh"].double(), bound + N_EFF * s["dh"].double().abs()
     assert ((got["dx"] - want).abs() <= bound + 2.0 ** -24 * want.abs()).all()
     assert ((got["dweight"] - dw).abs() <= (s["dy"].double().abs() * (1 + unit) * (rel + 80 * 2.0 ** -24)).sum(0)).all()
+
+
+@pytest.mark.parametrize("dim", [64, 700, 2560, 17000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_no_number_stays_none(pkg, gpu_device, dim, bad):
+    """A row with a NaN or an infinity has no mean: all of it is NaN, forward and backward, and no other row is."""
+    s = make(gpu_device, 5, dim, FP32, None, FP32)
+    clean = run(pkg, s)
+    s["x"][2, dim // 2] = bad
+    got = run(pkg, s)
+    for n in ("y", "dx"):
+        assert got[n][2].isnan().all(), n
+        assert torch.equal(got[n][[0, 1, 3, 4]], clean[n][[0, 1, 3, 4]]), n
+
+
+@pytest.mark.parametrize("dim", [700, 17000])
+def test_numbers_whose_sums_overflow(pkg, gpu_device, dim):
+    """Rows past float32's range have no spread in float32 either: no finite wrong ones come out of it but zeros (and the bias)."""
+    s = make(gpu_device, 3, dim, FP32, None, FP32, bias=False)
+    for size in (1e25, 3e38):
+        s["x"] = torch.where(torch.arange(dim, device=gpu_device) % 2 == 0, size, 0.5 * size).expand(3, -1).contiguous()
+        y = pkg.layer_norm_fn(s["x"], s["weight"])
+        assert ((y == 0) | y.isnan()).all()
