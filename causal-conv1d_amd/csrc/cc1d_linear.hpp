@@ -39,7 +39,9 @@ constexpr int kSegmentLog = 8, kSegment = 1 << kSegmentLog, kBlocks = kSegment /
 struct LinearRows { const void *p; int64_t sb, sl, sh; int32_t by_key; };
 
 // Terms of the states and weighted products where they make outputs of x_dtype alone; where they make the gates' gradients too, which are fp32 and
-// small differences of large sums, three.
+// small differences of large sums, three.  Two carry 2^-17 beside the 2^-8 or 2^-11 that out and dv are rounded to: against 64 bits both are off by 1.7e-3 (bfloat16) or
+// 2.1e-4 (float16) of themselves with two as with three, and by 2e-5 to 1e-4 from what 32 bits all the way would have rounded to, with three by 1e-5 to 3.5e-5.  Three
+// cost a prompt of 4 x 2048 tokens, 80 heads of 128 x 64, 224 us for 184, its training step 929 for 873.
 constexpr int out_terms(int dt) { return dt == CC1D_F32 ? 3 : 2; }
 
 // W of a state's operands, by sizes and type alone (what a forward saves has to be what its backward reads, whatever the layouts): those of
